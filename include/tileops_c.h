@@ -56,7 +56,7 @@ const char* tileops_status_string(int status);
 /* Device-side error word, read back by the host after the stream is
  * synchronised: 0 = none; 1 = a bounded mbarrier wait timed out (attention,
  * gated delta net); 2 = a malformed cu_seqlens was passed to
- * tileops_gdn_prefill_varlen_fwd.  The first code set is kept until cleared. */
+ * tileops_gdn_prefill_varlen_fwd, tileops_glr_fwd or tileops_glr_bwd.  The first code set is kept until cleared. */
 int tileops_device_error_flag(void* stream, int clear);
 
 /* Self-test of the give-up path the tensor-core kernels take when a wait
@@ -134,6 +134,46 @@ int tileops_fused_add_layer_norm_fwd(const void* x, const void* residual, const 
                                      int64_t N, double eps, int dtype, int affine_dtype,
                                      void* stream);
 
+/* ---- sandwich norm: between two blocks ---------------------------------- */
+
+#define TILEOPS_NORM_RMS 0   /* v / sqrt(mean v^2 + eps) */
+#define TILEOPS_NORM_LAYER 1 /* (v - mean) / sqrt(var + eps), biased variance */
+
+/* Per row of N:  p = norm(x) * post_weight + post_bias;
+ * s = round_dtype(residual_scale * residual + gate * p)  -> residual_out;
+ * y = round_dtype(norm(s) * pre_weight + pre_bias), statistics in fp32, those
+ * of the second norm over the rounded s.  x, residual, y, residual_out (M, N)
+ * of `dtype` (f32/f16/bf16), none of the outputs an input; post_weight,
+ * pre_weight, post_bias, pre_bias (N,) and gate (gate_rows, N) of
+ * `affine_dtype` (`dtype` or f32).  Row m takes gate row m / (M / gate_rows);
+ * gate_rows divides M.  gate NULL means 1 (gate_rows then 1), a bias NULL
+ * means 0.  No counterpart in the reference. */
+int tileops_sandwich_norm_fwd(const void* x, const void* residual, const void* post_weight,
+                              const void* pre_weight, const void* gate, const void* post_bias,
+                              const void* pre_bias, void* y, void* residual_out, int64_t M,
+                              int64_t N, int64_t gate_rows, int norm, double eps,
+                              double residual_scale, int dtype, int affine_dtype, void* stream);
+
+/* Bytes of scratch tileops_sandwich_norm_bwd needs, or -1 for an unsupported
+ * shape.  has_bias: post_bias or pre_bias has a gradient. */
+int64_t tileops_sandwich_norm_bwd_workspace_bytes(int64_t M, int64_t N, int64_t gate_rows,
+                                                  int has_bias);
+
+/* Gradients of tileops_sandwich_norm_fwd from dy and d_residual_out (NULL =
+ * zeros), its x and its residual_out: dx, d_residual (M, N) of `dtype`;
+ * d_post_weight, d_pre_weight, d_post_bias, d_pre_bias (N,) and d_gate
+ * (gate_rows, N) of `affine_dtype`, summed in fp32 in a fixed order.  d_gate
+ * needs gate and d_post_bias needs post_bias; those two and d_pre_bias may be
+ * NULL (not written).  `workspace` holds
+ * tileops_sandwich_norm_bwd_workspace_bytes() bytes, 16-byte aligned.  M >= 1. */
+int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_out, const void* x,
+                              const void* residual_out, const void* post_weight,
+                              const void* pre_weight, const void* gate, const void* post_bias,
+                              void* dx, void* d_residual, void* d_post_weight, void* d_pre_weight,
+                              void* d_gate, void* d_post_bias, void* d_pre_bias, void* workspace,
+                              int64_t M, int64_t N, int64_t gate_rows, int norm, double eps,
+                              double residual_scale, int dtype, int affine_dtype, void* stream);
+
 /* ---- 1-D convolution (NCL) ---------------------------------------------- */
 
 #define TILEOPS_ACT_NONE 0
@@ -195,6 +235,63 @@ int tileops_mha_fwd(const void* q, const void* k, const void* v, void* o, float*
 int tileops_gla_decode_fwd(const void* q, const void* k, const void* v, const void* gk,
                            const void* state, void* o, void* new_state, int64_t batch,
                            int64_t heads, int64_t dim_k, int64_t dim_v, double scale, int dtype,
+                           void* stream);
+
+/* ---- gated linear recurrence --------------------------------------------- */
+
+#define TILEOPS_GLR_SEGMENT 64 /* tokens between two saved states */
+
+/* Per channel, with k = decay_scale * softplus(decay_param):
+ *   a_t = exp(-k sigmoid(decay_gate_t));
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t;  y_t = h_t,
+ * h in fp32.  x, input_gate, decay_gate (batch, seq_len, dim) of `dtype`
+ * (f32/f16/bf16), channels contiguous, with their own batch and token strides
+ * in elements (>= 0); y (batch, seq_len, dim) dense; decay_param (dim,),
+ * initial_state (NULL = zeros) and final_state (sequences, dim) fp32.
+ * states (NULL = not written): (batch, ceil(seq_len / TILEOPS_GLR_SEGMENT), dim)
+ * fp32, the state before each segment, which tileops_glr_bwd takes.
+ * cu_seqlens (NULL = one sequence per batch row): an int32 DEVICE array of
+ * num_seqs + 1 offsets, batch 1, the rules of tileops_gdn_prefill_varlen_fwd
+ * (0 = cu[0] <= ... <= cu[num_seqs] = seq_len; device error 2 and meaningless
+ * results otherwise, never an access out of range).  batch up to 65535,
+ * seq_len >= 1.  No output may alias an input.  No counterpart in the
+ * reference. */
+int tileops_glr_fwd(const void* x, const void* input_gate, const void* decay_gate,
+                    const float* decay_param, const float* initial_state,
+                    const int32_t* cu_seqlens, int64_t num_seqs, void* y, float* final_state,
+                    float* states, int64_t batch, int64_t seq_len, int64_t dim,
+                    int64_t x_stride_b, int64_t x_stride_t, int64_t i_stride_b,
+                    int64_t i_stride_t, int64_t r_stride_b, int64_t r_stride_t,
+                    double decay_scale, int dtype, void* stream);
+
+/* Bytes of scratch tileops_glr_bwd needs, or -1 for an unsupported shape. */
+int64_t tileops_glr_bwd_workspace_bytes(int64_t batch, int64_t seq_len, int64_t dim);
+
+/* Gradients of tileops_glr_fwd from dy (batch, seq_len, dim) of `dtype` and
+ * d_final_state (sequences, dim) fp32 (NULL = zeros), with the forward's
+ * inputs, its states and its initial_state: dx, d_input_gate, d_decay_gate
+ * dense, of `dtype`; d_decay_param (dim,) and d_initial_state (sequences, dim)
+ * fp32, summed in a fixed order.  `workspace` holds
+ * tileops_glr_bwd_workspace_bytes() bytes, 16-byte aligned. */
+int tileops_glr_bwd(const void* dy, const void* x, const void* input_gate,
+                    const void* decay_gate, const float* decay_param, const float* states,
+                    const float* initial_state, const float* d_final_state,
+                    const int32_t* cu_seqlens, int64_t num_seqs, void* dx, void* d_input_gate,
+                    void* d_decay_gate, float* d_decay_param, float* d_initial_state,
+                    void* workspace, int64_t batch, int64_t seq_len, int64_t dim,
+                    int64_t g_stride_b, int64_t g_stride_t, int64_t x_stride_b,
+                    int64_t x_stride_t, int64_t i_stride_b, int64_t i_stride_t,
+                    int64_t r_stride_b, int64_t r_stride_t, double decay_scale, int dtype,
+                    void* stream);
+
+/* One token of every sequence: x, input_gate, decay_gate (batch, dim) of
+ * `dtype` with their own row strides, state (batch, dim) fp32 -> y (batch, dim)
+ * of `dtype` and new_state (batch, dim) fp32.  new_state may be state itself
+ * (updated in place) and may not overlap it otherwise. */
+int tileops_glr_decode_fwd(const void* x, const void* input_gate, const void* decay_gate,
+                           const float* decay_param, const float* state, void* y,
+                           float* new_state, int64_t batch, int64_t dim, int64_t x_stride,
+                           int64_t i_stride, int64_t r_stride, double decay_scale, int dtype,
                            void* stream);
 
 /* ---- Mamba-2 SSD chunk scan --------------------------------------------- */

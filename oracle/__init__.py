@@ -21,6 +21,6 @@ against flash-linear-attention's CPU reference recurrence (the probe's
 ref_api library).
 """
 
-from oracle import reference
+from oracle import recurrent, reference
 
-__all__ = ["reference"]
+__all__ = ["recurrent", "reference"]

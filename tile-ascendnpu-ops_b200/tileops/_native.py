@@ -73,6 +73,9 @@ _SIGNATURES: dict[str, list] = {
     "tileops_gelu_and_mul_fwd": [_p, _p, _i64, _i64, _i, _p],
     "tileops_gelu_tanh_and_mul_fwd": [_p, _p, _i64, _i64, _i, _p],
     "tileops_fused_add_layer_norm_fwd": [_p, _p, _p, _p, _p, _p, _i64, _i64, _d, _i, _i, _p],
+    "tileops_sandwich_norm_fwd": [_p] * 9 + [_i64] * 3 + [_i, _d, _d, _i, _i, _p],
+    "tileops_sandwich_norm_bwd_workspace_bytes": [_i64] * 3 + [_i],
+    "tileops_sandwich_norm_bwd": [_p] * 16 + [_i64] * 3 + [_i, _d, _d, _i, _i, _p],
     "tileops_conv1d_depthwise_fwd": [_p, _p, _p, _p] + [_i64] * 8 + [_i, _i, _i, _p],
     "tileops_conv1d_direct_fwd": [_p, _p, _p, _p] + [_i64] * 10 + [_i, _p],
     "tileops_mha_fwd": [_p, _p, _p, _p, _p] + [_i64] * 6 + [_i, _d, _i, _p],
@@ -82,6 +85,10 @@ _SIGNATURES: dict[str, list] = {
     "tileops_gdn_varlen_workspace_bytes": [_i64] * 5,
     "tileops_gdn_prefill_varlen_fwd": [_p] * 6 + [_i64] + [_p] * 4 + [_i64] * 5 + [_d, _i, _i, _p],
     "tileops_gla_decode_fwd": [_p] * 7 + [_i64] * 4 + [_d, _i, _p],
+    "tileops_glr_fwd": [_p] * 6 + [_i64] + [_p] * 3 + [_i64] * 9 + [_d, _i, _p],
+    "tileops_glr_bwd_workspace_bytes": [_i64] * 3,
+    "tileops_glr_bwd": [_p] * 9 + [_i64] + [_p] * 6 + [_i64] * 11 + [_d, _i, _p],
+    "tileops_glr_decode_fwd": [_p] * 7 + [_i64] * 5 + [_d, _i, _p],
     "tileops_ssd_chunk_scan_fwd": [_p] * 7 + [_i64] * 7 + [_i, _p],
     "tileops_device_error_flag": [_p, _i],
     "tileops_selftest_wait_timeout": [_p, _i64, _i64, _p, _p],
@@ -123,6 +130,8 @@ def lib() -> ctypes.CDLL:
                     "tileops_status_string": ctypes.c_char_p,
                     "tileops_gdn_workspace_bytes": ctypes.c_int64,
                     "tileops_gdn_varlen_workspace_bytes": ctypes.c_int64,
+                    "tileops_glr_bwd_workspace_bytes": ctypes.c_int64,
+                    "tileops_sandwich_norm_bwd_workspace_bytes": ctypes.c_int64,
                 }.get(name, ctypes.c_int)
             _lib = handle
     return _lib

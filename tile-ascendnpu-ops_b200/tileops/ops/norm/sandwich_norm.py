@@ -1,0 +1,216 @@
+"""Sandwich norm ops: from the end of one block to the start of the next.
+
+FusedAddLayerNormFwdOp adds a block's output to the residual stream and
+normalises the sum for the next block; these ops also normalise the block's
+output first, scale it by the block's gate and scale the stream::
+
+    p = norm(x) * post_weight + post_bias         x: the block's output
+    s = residual_scale * residual + gate * p      residual_out, rounded
+    y = norm(s) * pre_weight + pre_bias           the next block's input
+
+norm is RMS (``v / sqrt(mean(v^2) + eps)``) or LayerNorm, statistics in fp32;
+the second one's are over the rounded s, as in FusedAddLayerNormFwdOp.
+
+    FusedSandwichNormFwdOp(M=None, N=None, dtype=None, norm="rms", eps=1e-6,
+                           residual_scale=1.0, kernel_map=None)
+    forward(x, residual, post_weight, pre_weight, gate=None, post_bias=None, pre_bias=None)
+        -> (y, residual_out)
+
+    FusedSandwichNormBwdOp(the same)
+    forward(dy, d_residual_out, x, residual_out, post_weight, pre_weight, gate=None,
+            post_bias=None, pre_bias=None)
+        -> (dx, d_residual, d_post_weight, d_pre_weight, d_gate, d_post_bias, d_pre_bias)
+
+x, residual and the gradients of rows are (..., N) of ``dtype``.  Parameters
+are (N,), all of ``dtype`` or all float32.  gate is (N,) or (G, N): the rows
+are G equal consecutive groups (a batch of G samples) with a gate each; None
+means 1.  A bias of None means 0.  The backward op takes the forward's x and
+residual_out and the same parameters; ``d_residual_out`` may be None, and
+gradients of what was None are None.  Gradients have their tensors' types,
+summed in fp32 in a fixed order.
+"""
+
+from __future__ import annotations
+
+from typing import Dict, Optional
+
+import torch
+
+from tileops.device import get_device_backend
+from tileops.kernels.kernel_base import Kernel
+from tileops.kernels.norm import FusedSandwichNormBwdKernel, FusedSandwichNormFwdKernel
+
+from ..op_base import Op
+
+__all__ = ["FusedSandwichNormBwdOp", "FusedSandwichNormFwdOp"]
+
+
+class _SandwichNormOp(Op):
+    _op_name = ""
+
+    def __init__(
+        self,
+        M: Optional[int] = None,
+        N: Optional[int] = None,
+        dtype: Optional[torch.dtype] = None,
+        norm: str = "rms",
+        eps: float = 1e-6,
+        residual_scale: float = 1.0,
+        kernel_map: Optional[Dict[str, Kernel]] = None,
+    ):
+        if norm not in ("rms", "layer"):
+            raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
+        self.M = M
+        self.N = N
+        self.dtype = dtype
+        self._committed = (M, N, dtype)
+        self.norm = norm
+        self.eps = eps
+        self.residual_scale = residual_scale
+        self.dispatch_kernel(kernel_map)
+        self._kernel_cache: Dict[tuple, Kernel] = {}
+        self._last: Optional[tuple[int, int, int, int]] = None
+
+    def _check(self, rows: tuple, params: tuple, gate: Optional[torch.Tensor]) -> int:
+        """Validate ((name, tensor), ...) rows and parameters; returns M."""
+        is_device_tensor = get_device_backend().is_device_tensor
+        for name, t in rows + params + (("gate", gate),):
+            if t is not None and not is_device_tensor(t):
+                raise ValueError(f"{name} must be a {get_device_backend().name} tensor")
+        x = dict(rows)["x"]
+        committed_m, committed_n, committed_dtype = self._committed
+        dtype = committed_dtype or x.dtype
+        if x.dim() < 1 or x.shape[-1] < 1:
+            raise ValueError(f"Expected x of shape (..., N) with N >= 1, got {tuple(x.shape)}")
+        N = x.shape[-1]
+        M = x.numel() // N
+        affine = params[0][1].dtype
+        if affine not in (dtype, torch.float32):
+            raise ValueError(f"Expected {params[0][0]}.dtype {dtype} or {torch.float32}, "
+                             f"got {affine}")
+        for name, t in rows:
+            if t is None:
+                continue
+            if t.dtype != dtype:
+                raise ValueError(f"Expected {name}.dtype {dtype}, got {t.dtype}")
+            if t.shape != x.shape:
+                raise ValueError(f"Expected {name} shape {tuple(x.shape)}, got {tuple(t.shape)}")
+            if t.device != x.device:
+                raise ValueError(f"Expected {name} on {x.device}, got {t.device}")
+        for name, t in params + (("gate", gate),):
+            if t is None:
+                continue
+            if t.dtype != affine:
+                raise ValueError(f"Expected {name}.dtype {affine}, got {t.dtype}")
+            if t.device != x.device:
+                raise ValueError(f"Expected {name} on {x.device}, got {t.device}")
+            if name != "gate" and t.shape != (N,):
+                raise ValueError(f"Expected {name} shape {(N,)}, got {tuple(t.shape)}")
+        if gate is not None and (gate.dim() not in (1, 2) or gate.shape[-1] != N
+                                 or gate.dim() == 2 and (gate.shape[0] < 1 or M % gate.shape[0])):
+            raise ValueError(f"Expected gate shape {(N,)} or (G, {N}) with G dividing the {M} "
+                             f"rows, got {tuple(gate.shape)}")
+        if committed_n is not None and committed_n != N:
+            raise ValueError(f"Expected hidden dim {committed_n}, got {N}")
+        if committed_m is not None and committed_m != M:
+            raise ValueError(f"Expected M={committed_m} (product of leading dims), got {M}")
+        self.M, self.N, self.dtype = M, N, dtype
+        vectors = sum(t is not None for _, t in params)
+        self._last = (M, N, dtype.itemsize,
+                      (vectors + (0 if gate is None else gate.numel() // N)) * affine.itemsize)
+        return M
+
+    def _get_kernel(self, device_index) -> Kernel:
+        key = (self.M, self.N, self.dtype, device_index)
+        if key not in self._kernel_cache:
+            self._kernel_cache[key] = self.kernel_map[self._op_name](
+                self.M, self.N, self.norm, self.eps, self.residual_scale, self.dtype)
+        return self._kernel_cache[key]
+
+    def _work(self, flops: int, rows: int, passes: int) -> tuple[int, int]:
+        if self._last is None:
+            raise RuntimeError(f"{type(self).__name__}.eval_roofline() requires a prior "
+                               "forward() call to bind input shape and dtype")
+        M, N, eb, vectors = self._last
+        return flops * M * N, rows * M * N * eb + passes * vectors * N
+
+
+def _flat(t: Optional[torch.Tensor], M: int, N: int) -> Optional[torch.Tensor]:
+    return None if t is None else t.contiguous().view(M, N)
+
+
+def _param(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.contiguous()
+
+
+class FusedSandwichNormFwdOp(_SandwichNormOp):
+    """Norm of a block's output, gate, scaled residual and the next block's norm.
+
+    Args:
+        M: Optional committed row count (product of the leading dims).
+        N: Optional committed hidden dimension.
+        dtype: float32, float16 or bfloat16 (inferred from ``x`` when None).
+        norm: ``"rms"`` or ``"layer"``, for both norms.
+        eps: Epsilon of both norms.
+        residual_scale: Constant factor of the residual stream.
+        kernel_map: Optional kernel override dictionary.
+    """
+
+    _op_name = "sandwich_norm_fwd"
+
+    @property
+    def default_kernel_map(self) -> Dict[str, Kernel]:
+        return {self._op_name: FusedSandwichNormFwdKernel}
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor,
+                pre_weight: torch.Tensor, gate: Optional[torch.Tensor] = None,
+                post_bias: Optional[torch.Tensor] = None,
+                pre_bias: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Return ``(y, residual_out)``, both shaped like ``x``."""
+        M = self._check((("x", x), ("residual", residual)),
+                        (("post_weight", post_weight), ("pre_weight", pre_weight),
+                         ("post_bias", post_bias), ("pre_bias", pre_bias)), gate)
+        N = self.N
+        y, residual_out = self._get_kernel(x.device.index)(
+            _flat(x, M, N), _flat(residual, M, N), _param(post_weight), _param(pre_weight),
+            None if gate is None else gate.contiguous().view(-1, N), _param(post_bias),
+            _param(pre_bias))
+        return y.view(x.shape), residual_out.view(x.shape)
+
+    def eval_roofline(self) -> tuple[int, int]:
+        """``(14 * M * N, 4 * M * N * elem_bytes + the parameters once)`` of the last forward."""
+        return self._work(14, 4, 1)
+
+
+class FusedSandwichNormBwdOp(_SandwichNormOp):
+    """Gradients of FusedSandwichNormFwdOp; the same constructor arguments."""
+
+    _op_name = "sandwich_norm_bwd"
+
+    @property
+    def default_kernel_map(self) -> Dict[str, Kernel]:
+        return {self._op_name: FusedSandwichNormBwdKernel}
+
+    def forward(self, dy: torch.Tensor, d_residual_out: Optional[torch.Tensor], x: torch.Tensor,
+                residual_out: torch.Tensor, post_weight: torch.Tensor, pre_weight: torch.Tensor,
+                gate: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                pre_bias: Optional[torch.Tensor] = None):
+        """Return ``(dx, d_residual, d_post_weight, d_pre_weight, d_gate, d_post_bias,
+        d_pre_bias)``, None in the place of a gradient of what was None."""
+        M = self._check((("x", x), ("dy", dy), ("d_residual_out", d_residual_out),
+                         ("residual_out", residual_out)),
+                        (("post_weight", post_weight), ("pre_weight", pre_weight),
+                         ("post_bias", post_bias), ("pre_bias", pre_bias)), gate)
+        N = self.N
+        dx, d_residual, *grads = self._get_kernel(x.device.index)(
+            _flat(dy, M, N), _flat(d_residual_out, M, N), _flat(x, M, N),
+            _flat(residual_out, M, N), _param(post_weight), _param(pre_weight),
+            None if gate is None else gate.contiguous().view(-1, N), _param(post_bias),
+            _param(pre_bias))
+        if gate is not None:
+            grads[2] = grads[2].view(gate.shape)
+        return dx.view(x.shape), d_residual.view(x.shape), *grads
+
+    def eval_roofline(self) -> tuple[int, int]:
+        """``(30 * M * N, 6 * M * N * elem_bytes + the parameters and their gradients)``."""
+        return self._work(30, 6, 2)
