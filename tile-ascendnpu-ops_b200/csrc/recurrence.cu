@@ -25,6 +25,7 @@ namespace tileops {
 namespace {
 
 constexpr int kSegment = TILEOPS_GLR_SEGMENT;  // tokens between saved states
+constexpr float kNearLog = -0.25f;  // log a above it: by series
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- the gates of one element ----
@@ -54,7 +55,7 @@ __device__ __forceinline__ void decay_from_log(float la, float& a, float& m2) {
   p = fmaf(la, p, 1.0f);
   const float q = la * p;
   const float e = ex2_approx_f(kLog2e * la);
-  const bool near = la > -0.25f;
+  const bool near = la > kNearLog;
   a = near ? 1.0f + q : e;
   m2 = near ? -q * (2.0f + q) : fmaf(-e, e, 1.0f);
 }
@@ -90,32 +91,77 @@ struct Strides {
   int64_t xb, xt, ib, it, rb, rt, gb, gt;  // x, input gate, decay gate, dy: batch and token
 };
 
-// ---- vectors of channels ----
-template <int Bytes> struct Word;
-template <> struct Word<2> { using type = uint16_t; };
-template <> struct Word<4> { using type = uint32_t; };
-template <> struct Word<8> { using type = uint2; };
-template <> struct Word<16> { using type = uint4; };
+// ---- two channels at a time ----
+// The kernels below give a lane two neighbouring channels: their arithmetic is
+// packed (fma.rn.f32x2 and its kin, one issue slot for both).
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// V channels of one token, read or written by one access.
-template <typename T, int V>
-struct Chans {
-  using W = typename Word<V * sizeof(T)>::type;
-  W w;
-  __device__ __forceinline__ void load(const T* p) { w = __ldcs(reinterpret_cast<const W*>(p)); }
-  __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<W*>(p), w); }
-  __device__ __forceinline__ float get(int v) const {
-    T e[V];
-    memcpy(e, &w, sizeof(w));
-    return Cvt<T>::to_f(e[v]);
+template <typename T>
+struct Pair;  // two values of T as they lie in memory
+template <>
+struct Pair<float> {
+  using Word = uint2;
+  static __device__ __forceinline__ float2 get(Word w) {
+    return make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
   }
-  __device__ __forceinline__ void set(const float* f) {
-    T e[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) e[v] = Cvt<T>::from_f(f[v]);
-    memcpy(&w, e, sizeof(w));
+  static __device__ __forceinline__ Word set(float2 v) {
+    return make_uint2(__float_as_uint(v.x), __float_as_uint(v.y));
   }
 };
+template <>
+struct Pair<__nv_bfloat16> {
+  using Word = uint32_t;
+  static __device__ __forceinline__ float2 get(Word w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ Word set(float2 v) {
+    const __nv_bfloat162 r = __float22bfloat162_rn(v);
+    Word w;
+    memcpy(&w, &r, 4);
+    return w;
+  }
+};
+template <>
+struct Pair<__half> {
+  using Word = uint32_t;
+  static __device__ __forceinline__ float2 get(Word w) {
+    __half2 h;
+    memcpy(&h, &w, 4);
+    return __half22float2(h);
+  }
+  static __device__ __forceinline__ Word set(float2 v) {
+    const __half2 r = __float22half2_rn(v);
+    Word w;
+    memcpy(&w, &r, 4);
+    return w;
+  }
+};
+
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+  const float2 t = fmul2(z, both(-kLog2e));
+  const float2 d = fadd2(make_float2(ex2_approx_f(t.x), ex2_approx_f(t.y)), both(1.0f));
+  return make_float2(rcp_approx_f(d.x), rcp_approx_f(d.y));
+}
+
+// decay_from_log of two channels; kNear: both are known to be near zero.
+template <bool kNear>
+__device__ __forceinline__ void decay2(float2 la, float2& a, float2& m2) {
+  float2 p = ffma2(la, both(1.0f / 720.0f), both(1.0f / 120.0f));
+  p = ffma2(la, p, both(1.0f / 24.0f));
+  p = ffma2(la, p, both(1.0f / 6.0f));
+  p = ffma2(la, p, both(0.5f));
+  p = ffma2(la, p, both(1.0f));
+  const float2 q = fmul2(la, p);
+  a = fadd2(q, both(1.0f));
+  m2 = fmul2(q, ffma2(q, both(-1.0f), both(-2.0f)));
+  if (!kNear) {
+    const float2 t = fmul2(la, both(kLog2e));
+    const float2 e = make_float2(ex2_approx_f(t.x), ex2_approx_f(t.y));
+    const float2 f = ffma2(e, fmul2(e, both(-1.0f)), both(1.0f));
+    if (!(la.x > kNearLog)) a.x = e.x, m2.x = f.x;
+    if (!(la.y > kNearLog)) a.y = e.y, m2.y = f.y;
+  }
+}
 
 // ---- clusters: CTAs that share one channel block and split its tokens ----
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -133,10 +179,11 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Writes v to the place p has in the shared memory of CTA `rank` of the cluster.
-__device__ __forceinline__ void st_cluster(float2* p, uint32_t rank, float2 v) {
+__device__ __forceinline__ void st_cluster(float4* p, uint32_t rank, float4 v) {
   uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(p)), there;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(v.x), "f"(v.y)
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(v.x),
+               "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
 }
 
@@ -147,23 +194,105 @@ __device__ __forceinline__ void st_cluster(float2* p, uint32_t rank, float2 v) {
 // H alone is taken, whatever the forgotten state was.
 constexpr float kForget = -1.0f;
 
+struct Run {
+  float2 A, H;  // of two channels
+  __device__ __forceinline__ Run(float2 a, float2 h) : A(a), H(h) {}
+  __device__ __forceinline__ explicit Run(float4 w)
+      : A(make_float2(w.x, w.y)), H(make_float2(w.z, w.w)) {}
+  __device__ __forceinline__ float4 word() const { return make_float4(A.x, A.y, H.x, H.y); }
+};
+
 template <bool kPacked>
-__device__ __forceinline__ float apply(float2 run, float h) {
-  const float next = fmaf(run.x, h, run.y);
-  return kPacked && run.x < 0.0f ? run.y : next;
+__device__ __forceinline__ float2 apply(const Run& run, float2 h) {
+  float2 next = ffma2(run.A, h, run.H);
+  if (kPacked) {
+    if (run.A.x < 0.0f) next.x = run.H.x;
+    if (run.A.y < 0.0f) next.y = run.H.y;
+  }
+  return next;
 }
 template <bool kPacked>
-__device__ __forceinline__ float2 join(float2 first, float2 then) {
-  float2 r = make_float2(first.x * then.x, fmaf(then.x, first.y, then.y));
+__device__ __forceinline__ Run join(const Run& first, const Run& then) {
+  Run r(fmul2(first.A, then.A), apply<kPacked>(then, first.H));
   if (kPacked) {
-    if (first.x < 0.0f) r.x = kForget;
-    if (then.x < 0.0f) r = then;
+    if (first.A.x < 0.0f || then.A.x < 0.0f) r.A.x = kForget;
+    if (first.A.y < 0.0f || then.A.y < 0.0f) r.A.y = kForget;
   }
   return r;
 }
 
-constexpr int kMaxWarps = 8;     // warps of a CTA
-constexpr int kMaxCluster = 8;   // CTAs of a cluster
+constexpr int kMaxWarps = 8;    // warps of a CTA
+constexpr int kMaxCluster = 8;  // CTAs of a cluster
+constexpr int kChans = 64;      // channels of a CTA: two a lane
+
+// ---- a warp's rows in shared memory ----
+// A tile is kRows tokens of the 64 channels of the warp, rows of one tensor one
+// below another.  The warp copies its own tiles and only it reads them, so no
+// barrier but its own is needed.  kBytes: what one copy moves, the widest that
+// the tensors' addresses and strides allow (16; 4; 2 by plain loads, as
+// cp.async has no such size).
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src), "r"(in ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Copies `len` rows (0 <= len <= kRows) starting at `row0`, which points at the first of
+// the CTA's channels; `left` of them exist (0 < left).  What does not exist is
+// filled with zeros and not read: its source is `row0` itself.
+template <typename T, int kRows, int kBytes>
+__device__ __forceinline__ void copy_tile(T* tile, const T* row0, int64_t stride, int len,
+                                          int64_t left, int lane) {
+  constexpr int kEach = kBytes / sizeof(T);   // elements of one copy
+  constexpr int kPerRow = kChans / kEach;     // copies of a row
+  static_assert(kPerRow >= 8 && (kPerRow % 32 == 0 || 32 % kPerRow == 0), "copies of a row");
+#pragma unroll
+  for (int i = 0; i < kRows * kPerRow / 32; ++i) {
+    const int at = i * 32 + lane, row = at / kPerRow, col = at % kPerRow * kEach;
+    const bool in = row < len && col < left;
+    const T* src = in ? row0 + row * stride + col : row0;
+    T* dst = tile + row * kChans + col;
+    if constexpr (kBytes == 16)
+      copy16(dst, src, in);
+    else if constexpr (kBytes == 4)
+      copy4(dst, src, in);
+    else
+      *dst = in ? *src : Cvt<T>::from_f(0.0f);
+  }
+}
+
+// Stores two neighbouring channels; kBytes < the pair's size: one by one.
+template <typename T, int kBytes>
+__device__ __forceinline__ void store_pair(T* p, float2 v, int have) {
+  if constexpr (kBytes >= 2 * sizeof(T)) {
+    if (have > 0)
+      __stcs(reinterpret_cast<typename Pair<T>::Word*>(p), Pair<T>::set(v));
+  } else {
+    if (have > 0) p[0] = Cvt<T>::from_f(v.x);
+    if (have > 1) p[1] = Cvt<T>::from_f(v.y);
+  }
+}
+__device__ __forceinline__ float2 load_state(const float* p, int have) {
+  return make_float2(p && have > 0 ? p[0] : 0.0f, p && have > 1 ? p[1] : 0.0f);
+}
+__device__ __forceinline__ void store_state(float* p, float2 v, int have) {
+  if (have > 0) p[0] = v.x;
+  if (have > 1) p[1] = v.y;
+}
 
 // Which of `count` tokens from t0 on start a sequence, as bits; the sequence of t0 in n0.
 // Empty sequences start no token.  Every lane returns the same.
@@ -192,41 +321,80 @@ struct FwdArgs {
   int* err;
 };
 
-// One CTA (or cluster of CTAs) owns 32 V channels of one batch row and walks
-// along its tokens; a lane owns V channels and a warp kRun tokens at a time:
-//   1. load x and the gates of the run, all loads before the first use;
+// One CTA (or cluster of CTAs) owns 64 channels of one batch row and walks along
+// its tokens; a lane owns two channels and a warp kRun tokens at a time:
+//   1. x and the gates of the run, copied to the warp's tiles a step or two ahead;
 //   2. a_t, u_t into registers, and the run's map (A, H);
-//   3. exchange the maps: between warps through shared memory, between the
+//   3. the maps are exchanged: between warps through shared memory, between the
 //      CTAs of a cluster through distributed shared memory;
 //   4. the state before the run, from the maps before it and the carried state;
 //   5. the run again, token by token from that state, and the stores.
 // Step 5 repeats the sequential recurrence itself, so y differs from it by the
 // rounding of the state a run starts with only.  x and the gates are read once
 // and y is written once.
-template <typename T, int V, int kRun, bool kPacked>
-__global__ void __launch_bounds__(kMaxWarps * 32) glr_fwd_scan(const FwdArgs p) {
-  __shared__ float2 warp_run[2][kMaxWarps][32 * V];
-  __shared__ float2 cta_run[2][kMaxCluster][32 * V];
+constexpr int kRun = 16;
+
+template <bool kNear, typename T>
+__device__ __forceinline__ void fwd_run(const T* tiles, int lane, float2 k, float2* a, float2* u) {
+  using P = Pair<T>;
+  using Word = typename P::Word;
+  constexpr int kTile = kRun * kChans;
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) {
+    const Word* w = reinterpret_cast<const Word*>(tiles + j * kChans) + lane;
+    const float2 xv = P::get(w[0]);
+    const float2 si = sigmoid2(P::get(w[kTile / 2]));
+    const float2 sr = sigmoid2(P::get(w[kTile]));
+    float2 m2;
+    decay2<kNear>(fmul2(sr, fmul2(k, both(-1.0f))), a[j], m2);
+    const float2 m = make_float2(sqrt_approx_f(m2.x), sqrt_approx_f(m2.y));
+    u[j] = fmul2(fmul2(m, si), xv);
+  }
+}
+
+template <typename T, int kBytes, bool kPacked, int kStages>
+__global__ void __launch_bounds__(kMaxWarps * 32, 2) glr_fwd_scan(const FwdArgs p) {
+  constexpr int kTile = kRun * kChans;  // elements
+  extern __shared__ __align__(16) char dynamic_smem[];
+  __shared__ float4 warp_run[2][kMaxWarps][32];   // (A, H) of two channels
+  __shared__ float4 cta_run[2][kMaxCluster][32];
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
   const int warps = blockDim.x >> 5;
   const uint32_t size = cluster_size(), rank = cluster_rank();
-  const int64_t b = blockIdx.y;
-  const int64_t ch = static_cast<int64_t>(blockIdx.x / size) * (32 * V) + lane * V;
-  const bool active = ch < p.D;
-  const int64_t T_ = p.T, D = p.D;
-  const T* xp = static_cast<const T*>(p.x) + b * p.st.xb + ch;
-  const T* ip = static_cast<const T*>(p.ig) + b * p.st.ib + ch;
-  const T* rp = static_cast<const T*>(p.rg) + b * p.st.rb + ch;
-  T* yp = static_cast<T*>(p.y) + b * T_ * D + ch;
+  const int64_t b = blockIdx.y, T_ = p.T, D = p.D;
+  const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * kChans, ch = ch0 + 2 * lane;
+  const int have = ch + 1 < D ? 2 : (ch < D ? 1 : 0);  // channels of this lane
+  T* ring = reinterpret_cast<T*>(dynamic_smem) + warp * (kStages * 3 * kTile);
   const int64_t nseg = (T_ + kSegment - 1) / kSegment;
+  const int64_t stride = static_cast<int64_t>(kRun) * warps * size;  // tokens of a step
+
+  int64_t next = static_cast<int64_t>(rank * warps + warp) * kRun;  // run to be copied next
+  const T* xn = static_cast<const T*>(p.x) + b * p.st.xb + ch0 + next * p.st.xt;
+  const T* in = static_cast<const T*>(p.ig) + b * p.st.ib + ch0 + next * p.st.it;
+  const T* rn = static_cast<const T*>(p.rg) + b * p.st.rb + ch0 + next * p.st.rt;
+  auto fetch = [&](int stage) {
+    if (next < T_) {
+      const int len = T_ - next < kRun ? static_cast<int>(T_ - next) : kRun;
+      T* t = ring + stage * (3 * kTile);
+      copy_tile<T, kRun, kBytes>(t, xn, p.st.xt, len, D - ch0, lane);
+      copy_tile<T, kRun, kBytes>(t + kTile, in, p.st.it, len, D - ch0, lane);
+      copy_tile<T, kRun, kBytes>(t + 2 * kTile, rn, p.st.rt, len, D - ch0, lane);
+      xn += stride * p.st.xt;
+      in += stride * p.st.it;
+      rn += stride * p.st.rt;
+      next += stride;
+    }
+    copies_commit();  // a group a step, empty past the end
+  };
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) fetch(s);
 
   if (kPacked) {
     // Sequences without a token end where they began; the offsets are checked once.
     for (int n = rank * warps + warp; n < p.N; n += size * warps)
-      if (p.cu[n + 1] <= p.cu[n] && active)
-        for (int v = 0; v < V; ++v)
-          p.hT[n * D + ch + v] = p.h0 ? p.h0[n * D + ch + v] : 0.0f;
+      if (p.cu[n + 1] <= p.cu[n])
+        store_state(p.hT + n * D + ch, load_state(p.h0 ? p.h0 + n * D + ch : nullptr, have), have);
     if (blockIdx.x == 0 && warp == 0) {
       bool bad = false;
       for (int n = lane; n < p.N; n += 32) bad |= p.cu[n + 1] < p.cu[n];
@@ -235,129 +403,104 @@ __global__ void __launch_bounds__(kMaxWarps * 32) glr_fwd_scan(const FwdArgs p) 
     }
   }
 
-  float k[V], carry[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    k[v] = active ? decay_rate(p.lam[ch + v], p.c) : 0.0f;
-    carry[v] = !kPacked && active && p.h0 ? p.h0[b * D + ch + v] : 0.0f;
-  }
-
+  const float2 lam = load_state(p.lam + ch, have);
+  const float2 k = make_float2(have > 0 ? decay_rate(lam.x, p.c) : 0.0f,
+                               have > 1 ? decay_rate(lam.y, p.c) : 0.0f);
+  // sigmoid <= 1: no log a of this warp is below -max k.
+  const bool near = __all_sync(~0u, k.x < -kNearLog && k.y < -kNearLog);
+  float2 carry = both(0.0f);
+  if (!kPacked) carry = load_state(p.h0 ? p.h0 + b * D + ch : nullptr, have);
   if (size > 1) cluster_sync();  // every CTA runs before its shared memory is written
-  const int64_t stride = static_cast<int64_t>(kRun) * warps * size;
-  int par = 0;
+
+  int par = 0, stage = 0;
   for (int64_t base = 0; base < T_; base += stride, par ^= 1) {
     const int64_t t0 = base + static_cast<int64_t>(rank * warps + warp) * kRun;
-    const int64_t left64 = T_ - t0;
-    const int len = left64 >= kRun ? kRun : (left64 > 0 ? static_cast<int>(left64) : 0);
-    Chans<T, V> xr[kRun], ir[kRun], rr[kRun];
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if (active && j < len) {
-        xr[j].load(xp + (t0 + j) * p.st.xt);
-        ir[j].load(ip + (t0 + j) * p.st.it);
-        rr[j].load(rp + (t0 + j) * p.st.rt);
-      } else {
-        memset(&xr[j], 0, sizeof(xr[j]));
-        memset(&ir[j], 0, sizeof(ir[j]));
-        memset(&rr[j], 0, sizeof(rr[j]));
-      }
-    }
+    const int64_t left = T_ - t0;
+    const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
     // Bit j: token t0 + j starts a sequence (one bit more than the run has
     // tokens, for the end of its last one).
     uint32_t starts = 0;
     if (kPacked && len > 0) starts = start_bits(p.cu, p.N, t0, kRun + 1, lane);
 
-    float a[kRun][V], u[kRun][V];
-    float2 run[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) run[v] = make_float2(1.0f, 0.0f);
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const Gates g = gates_of(ir[j].get(v), rr[j].get(v), k[v]);
-        a[j][v] = j < len ? g.a : 1.0f;  // past the end: the identity
-        u[j][v] = j < len ? sqrt_approx_f(g.m2) * g.si * xr[j].get(v) : 0.0f;
-      }
-      if (kPacked && (starts >> j & 1) && j < len) {
-        const int64_t n = seq_of(p.cu, p.N, t0 + j);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          u[j][v] = fmaf(a[j][v], active && p.h0 ? p.h0[n * D + ch + v] : 0.0f, u[j][v]);
-          a[j][v] = kForget;
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) run[v] = join<kPacked>(run[v], make_float2(a[j][v], u[j][v]));
+    float2 a[kRun], u[kRun];
+    copies_wait<kStages - 1>();
+    __syncwarp();  // the tiles of this step have landed, whichever lane copied them
+    const T* tiles = ring + stage * (3 * kTile);
+    if (len > 0) {
+      if (near)
+        fwd_run<true>(tiles, lane, k, a, u);
+      else
+        fwd_run<false>(tiles, lane, k, a, u);
     }
-
+    __syncwarp();  // read by every lane before they are overwritten
+    fetch(stage);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    if (len < kRun)
 #pragma unroll
-    for (int v = 0; v < V; ++v) warp_run[par][warp][lane * V + v] = run[v];
+      for (int j = 0; j < kRun; ++j)
+        if (j >= len) a[j] = both(1.0f), u[j] = both(0.0f);  // past the end: the identity
+    if (kPacked && (starts & ((1u << kRun) - 1)))
+#pragma unroll
+      for (int j = 0; j < kRun; ++j)
+        if ((starts >> j & 1) && j < len) {
+          const int64_t n = seq_of(p.cu, p.N, t0 + j);
+          u[j] = ffma2(a[j], load_state(p.h0 ? p.h0 + n * D + ch : nullptr, have), u[j]);
+          a[j] = both(kForget);
+        }
+    Run run = {a[0], u[0]};
+#pragma unroll
+    for (int j = 1; j < kRun; ++j) run = join<kPacked>(run, Run{a[j], u[j]});
+
+    warp_run[par][warp][lane] = run.word();
     __syncthreads();
-    float h[V];
+    float2 h;
     if (size > 1) {
       // The CTA's map, to every CTA of the cluster (warp w writes to CTA w, w + warps, ...).
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float2 all = warp_run[par][0][lane * V + v];
-        for (int w = 1; w < warps; ++w) all = join<kPacked>(all, warp_run[par][w][lane * V + v]);
-        for (uint32_t r = warp; r < size; r += warps)
-          st_cluster(&cta_run[par][rank][lane * V + v], r, all);
-      }
+      Run all(warp_run[par][0][lane]);
+      for (int w = 1; w < warps; ++w) all = join<kPacked>(all, Run(warp_run[par][w][lane]));
+      for (uint32_t r = warp; r < size; r += warps)
+        st_cluster(&cta_run[par][rank][lane], r, all.word());
       cluster_sync();
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        for (uint32_t r = 0; r < size; ++r) {
-          if (r == rank) h[v] = carry[v];
-          carry[v] = apply<kPacked>(cta_run[par][r][lane * V + v], carry[v]);
-        }
+      for (uint32_t r = 0; r < size; ++r) {
+        if (r == rank) h = carry;
+        carry = apply<kPacked>(Run(cta_run[par][r][lane]), carry);
+      }
+      for (int w = 0; w < warp; ++w) h = apply<kPacked>(Run(warp_run[par][w][lane]), h);
     } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = carry[v];
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        for (int w = 0; w < warps; ++w)
-          carry[v] = apply<kPacked>(warp_run[par][w][lane * V + v], carry[v]);
+      for (int w = 0; w < warps; ++w) {
+        if (w == warp) h = carry;
+        carry = apply<kPacked>(Run(warp_run[par][w][lane]), carry);
+      }
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      for (int w = 0; w < warp; ++w)
-        h[v] = apply<kPacked>(warp_run[par][w][lane * V + v], h[v]);
 
-    if (p.states && len > 0 && t0 % kSegment == 0 && active)
-#pragma unroll
-      for (int v = 0; v < V; ++v) p.states[(b * nseg + t0 / kSegment) * D + ch + v] = h[v];
+    if (p.states && len > 0 && t0 % kSegment == 0)
+      store_state(p.states + (b * nseg + t0 / kSegment) * D + ch, h, have);
+    T* yp = static_cast<T*>(p.y) + (b * T_ + t0) * D + ch;
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = apply<kPacked>(make_float2(a[j][v], u[j][v]), h[v]);
-      if (active && j < len) {
-        Chans<T, V> o;
-        o.set(h);
-        o.store(yp + (t0 + j) * D);
-        if (kPacked && ((starts >> (j + 1) & 1) || t0 + j + 1 == T_)) {
-          const int64_t n = seq_of(p.cu, p.N, t0 + j);
-#pragma unroll
-          for (int v = 0; v < V; ++v) p.hT[n * D + ch + v] = h[v];
-        }
+      h = apply<kPacked>(Run{a[j], u[j]}, h);
+      if (j < len) {
+        store_pair<T, kBytes>(yp + j * D, h, have);
+        if (kPacked && ((starts >> (j + 1) & 1) || t0 + j + 1 == T_))
+          store_state(p.hT + seq_of(p.cu, p.N, t0 + j) * D + ch, h, have);
       }
     }
-    if (!kPacked && len > 0 && t0 + len == T_ && active)
-#pragma unroll
-      for (int v = 0; v < V; ++v) p.hT[b * D + ch + v] = h[v];
+    if (!kPacked && len > 0 && t0 + len == T_) store_state(p.hT + b * D + ch, h, have);
   }
+  copies_wait<0>();
 }
 
-// Channels per lane and the tokens' split over warps and CTAs.  V is the widest of
-// one 4-byte access that every row pointer and stride allows.
+// The tokens' split over warps and CTAs: a run a warp, up to kMaxWarps; then
+// clusters of 2, 4 or 8 CTAs along the tokens while the channels and batch rows
+// alone give fewer than three CTAs an SM.
 struct ScanGrid {
   int warps, cluster;
   int64_t blocks;
 };
 
-inline ScanGrid scan_grid(int64_t batch, int64_t seq_len, int64_t dim, int chans, int run) {
+inline ScanGrid scan_grid(int64_t batch, int64_t seq_len, int64_t dim, int run) {
   ScanGrid g;
-  g.blocks = (dim + chans - 1) / chans;
+  g.blocks = (dim + kChans - 1) / kChans;
   const int64_t runs = (seq_len + run - 1) / run;
   g.warps = static_cast<int>(std::min<int64_t>(runs, kMaxWarps));
   g.cluster = 1;
@@ -367,11 +510,16 @@ inline ScanGrid scan_grid(int64_t batch, int64_t seq_len, int64_t dim, int chans
   return g;
 }
 
-template <typename K, typename A>
-int launch_scan(K kernel, const ScanGrid& g, int64_t batch, const A& args, cudaStream_t s) {
+template <typename A>
+int launch_scan(void (*kernel)(A), const ScanGrid& g, int64_t batch, size_t smem, const A& args,
+                cudaStream_t s) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem)) != cudaSuccess)
+    return TILEOPS_ELAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(g.blocks * g.cluster), static_cast<unsigned>(batch));
   cfg.blockDim = dim3(static_cast<unsigned>(g.warps * 32));
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -387,24 +535,35 @@ int launch_scan(K kernel, const ScanGrid& g, int64_t batch, const A& args, cudaS
   return TILEOPS_OK;
 }
 
-// Whether rows of V elements can be read as one word: base and strides of each tensor.
-inline bool rows_fit(const void* p, int64_t sb, int64_t st, int itemsize, int V) {
-  return reinterpret_cast<uintptr_t>(p) % (V * itemsize) == 0 && sb % V == 0 && st % V == 0;
+// The widest copy (16, 4 or 2 bytes) that a tensor's base and strides allow.
+inline int copy_bytes(const void* p, int64_t sb, int64_t st, int64_t itemsize) {
+  for (int bytes : {16, 4})
+    if (reinterpret_cast<uintptr_t>(p) % bytes == 0 && sb * itemsize % bytes == 0 &&
+        st * itemsize % bytes == 0)
+      return bytes;
+  return 2;
 }
 
 template <typename T>
 int launch_fwd(const FwdArgs& a, int64_t batch, cudaStream_t s) {
-  constexpr int kRun = 16, kWide = 4 / sizeof(T);
-  const int eb = sizeof(T);
-  const bool wide = kWide > 1 && a.D % kWide == 0 && rows_fit(a.x, a.st.xb, a.st.xt, eb, kWide) &&
-                    rows_fit(a.ig, a.st.ib, a.st.it, eb, kWide) &&
-                    rows_fit(a.rg, a.st.rb, a.st.rt, eb, kWide) && rows_fit(a.y, 0, 0, eb, kWide);
-  const ScanGrid g = scan_grid(batch, a.T, a.D, wide ? 32 * kWide : 32, kRun);
-  if (wide)
-    return a.cu ? launch_scan(glr_fwd_scan<T, kWide, kRun, true>, g, batch, a, s)
-                : launch_scan(glr_fwd_scan<T, kWide, kRun, false>, g, batch, a, s);
-  return a.cu ? launch_scan(glr_fwd_scan<T, 1, kRun, true>, g, batch, a, s)
-              : launch_scan(glr_fwd_scan<T, 1, kRun, false>, g, batch, a, s);
+  constexpr int kStages = sizeof(T) == 2 ? 2 : 1;  // about 100 KB of tiles: two CTAs an SM
+  constexpr int64_t eb = sizeof(T);
+  const int bytes = std::min({copy_bytes(a.x, a.st.xb, a.st.xt, eb),
+                              copy_bytes(a.ig, a.st.ib, a.st.it, eb),
+                              copy_bytes(a.rg, a.st.rb, a.st.rt, eb),
+                              copy_bytes(a.y, a.D, a.D, eb)});
+  const ScanGrid g = scan_grid(batch, a.T, a.D, kRun);
+  const size_t smem = static_cast<size_t>(g.warps) * kStages * 3 * kRun * kChans * sizeof(T);
+  auto go = [&](auto packed, auto plain) {
+    return launch_scan(a.cu ? packed : plain, g, batch, smem, a, s);
+  };
+  if (bytes == 16)
+    return go(glr_fwd_scan<T, 16, true, kStages>, glr_fwd_scan<T, 16, false, kStages>);
+  if constexpr (sizeof(T) == 2) {
+    if (bytes == 2)
+      return go(glr_fwd_scan<T, 2, true, kStages>, glr_fwd_scan<T, 2, false, kStages>);
+  }
+  return go(glr_fwd_scan<T, 4, true, kStages>, glr_fwd_scan<T, 4, false, kStages>);
 }
 
 template <typename T>
