@@ -25,7 +25,6 @@ namespace tileops {
 namespace {
 
 constexpr int kSegment = TILEOPS_GLR_SEGMENT;  // tokens between saved states
-constexpr float kNearLog = -0.25f;  // log a above it: by series
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- the gates of one element ----
@@ -43,28 +42,32 @@ __device__ __forceinline__ float sigmoid_f(float z) {
   return rcp_approx_f(1.0f + ex2_approx_f(-kLog2e * z));
 }
 
-// a and 1 - a^2 from log a <= 0.  Near zero both come from q = a - 1 = expm1(log a)
-// (Taylor series to the sixth power: off by less than log_a^6 / 5040 = 5e-8 of q at
-// -1/4): 1 - a^2 = -q (2 + q) has no cancellation, and 1 + q rounds once, where an
-// approximate exponential's error would be carried along the whole sequence.
-__device__ __forceinline__ void decay_from_log(float la, float& a, float& m2) {
-  float p = fmaf(la, 1.0f / 720.0f, 1.0f / 120.0f);
-  p = fmaf(la, p, 1.0f / 24.0f);
-  p = fmaf(la, p, 1.0f / 6.0f);
-  p = fmaf(la, p, 0.5f);
-  p = fmaf(la, p, 1.0f);
-  const float q = la * p;
-  const float e = ex2_approx_f(kLog2e * la);
-  const bool near = la > kNearLog;
-  a = near ? 1.0f + q : e;
-  m2 = near ? -q * (2.0f + q) : fmaf(-e, e, 1.0f);
+// a and 1 - a^2 from f = -log a >= 0.  Near zero both come from g = 1 - a = 1 - exp(-f):
+// 1 - a^2 = g (1 + a) has no cancellation, and a = 1 - g rounds once, where an approximate
+// exponential's error would be carried along the whole sequence.  g / f on [0, 1/4] is a
+// polynomial of degree 4 fitted here by Remez exchange on the relative error: 8e-9 with
+// its coefficients in fp32, a seventh of half a step.
+constexpr float kNear = 0.25f;
+constexpr float kG0 = 1.0f, kG1 = -0.4999994933605194f, kG2 = 0.16665081679821014f,
+                kG3 = -0.041488952934741974f, kG4 = 0.007510221563279629f;
+
+__device__ __forceinline__ void decay_of(float f, float& a, float& m2) {
+  float p = fmaf(f, kG4, kG3);
+  p = fmaf(f, p, kG2);
+  p = fmaf(f, p, kG1);
+  p = fmaf(f, p, kG0);
+  const float g = f * p;
+  const float e = ex2_approx_f(-kLog2e * f);
+  const bool near = f < kNear;
+  a = near ? 1.0f - g : e;
+  m2 = near ? g * (1.0f + a) : fmaf(-e, e, 1.0f);
 }
 
 __device__ __forceinline__ Gates gates_of(float i, float r, float k) {
   Gates g;
   g.si = sigmoid_f(i);
   g.sr = sigmoid_f(r);
-  decay_from_log(-k * g.sr, g.a, g.m2);
+  decay_of(k * g.sr, g.a, g.m2);
   return g;
 }
 
@@ -94,6 +97,15 @@ struct Strides {
 // ---- two channels at a time ----
 // The kernels below give a lane two neighbouring channels: their arithmetic is
 // packed (fma.rn.f32x2 and its kin, one issue slot for both).
+__device__ __forceinline__ float2 fsub2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "sub.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 template <typename T>
@@ -137,29 +149,35 @@ struct Pair<__half> {
   }
 };
 
-__device__ __forceinline__ float2 sigmoid2(float2 z) {
-  const float2 t = fmul2(z, both(-kLog2e));
-  const float2 d = fadd2(make_float2(ex2_approx_f(t.x), ex2_approx_f(t.y)), both(1.0f));
+// Constants of the packed arithmetic, handed over as kernel arguments: from there
+// they go to uniform registers, where literals would take a register pair each.
+struct Consts {
+  float2 nlog2e = {-kLog2e, -kLog2e}, one = {1.0f, 1.0f}, g1 = {kG1, kG1}, g2 = {kG2, kG2},
+         g3 = {kG3, kG3}, g4 = {kG4, kG4};
+};
+
+__device__ __forceinline__ float2 sigmoid2(float2 z, const Consts& c) {
+  const float2 t = fmul2(z, c.nlog2e);
+  const float2 d = fadd2(make_float2(ex2_approx_f(t.x), ex2_approx_f(t.y)), c.one);
   return make_float2(rcp_approx_f(d.x), rcp_approx_f(d.y));
 }
 
-// decay_from_log of two channels; kNear: both are known to be near zero.
-template <bool kNear>
-__device__ __forceinline__ void decay2(float2 la, float2& a, float2& m2) {
-  float2 p = ffma2(la, both(1.0f / 720.0f), both(1.0f / 120.0f));
-  p = ffma2(la, p, both(1.0f / 24.0f));
-  p = ffma2(la, p, both(1.0f / 6.0f));
-  p = ffma2(la, p, both(0.5f));
-  p = ffma2(la, p, both(1.0f));
-  const float2 q = fmul2(la, p);
-  a = fadd2(q, both(1.0f));
-  m2 = fmul2(q, ffma2(q, both(-1.0f), both(-2.0f)));
-  if (!kNear) {
-    const float2 t = fmul2(la, both(kLog2e));
+// decay_of of two channels; kAllNear: both are known to be near zero.
+template <bool kAllNear>
+__device__ __forceinline__ void decay2(float2 f, float2& a, float2& m2, const Consts& c) {
+  float2 p = ffma2(f, c.g4, c.g3);
+  p = ffma2(f, p, c.g2);
+  p = ffma2(f, p, c.g1);
+  p = ffma2(f, p, c.one);
+  const float2 g = fmul2(f, p);
+  a = fsub2(c.one, g);
+  m2 = fmul2(g, fadd2(a, c.one));
+  if (!kAllNear) {
+    const float2 t = fmul2(f, c.nlog2e);
     const float2 e = make_float2(ex2_approx_f(t.x), ex2_approx_f(t.y));
-    const float2 f = ffma2(e, fmul2(e, both(-1.0f)), both(1.0f));
-    if (!(la.x > kNearLog)) a.x = e.x, m2.x = f.x;
-    if (!(la.y > kNearLog)) a.y = e.y, m2.y = f.y;
+    const float2 o = fsub2(c.one, fmul2(e, e));
+    if (!(f.x < kNear)) a.x = e.x, m2.x = o.x;
+    if (!(f.y < kNear)) a.y = e.y, m2.y = o.y;
   }
 }
 
@@ -221,7 +239,10 @@ __device__ __forceinline__ Run join(const Run& first, const Run& then) {
   return r;
 }
 
-constexpr int kMaxWarps = 8;    // warps of a CTA
+#ifndef GLR_WARPS
+#define GLR_WARPS 8
+#endif
+constexpr int kMaxWarps = GLR_WARPS;    // warps of a CTA
 constexpr int kMaxCluster = 8;  // CTAs of a cluster
 constexpr int kChans = 64;      // channels of a CTA: two a lane
 
@@ -260,6 +281,14 @@ __device__ __forceinline__ void copy_tile(T* tile, const T* row0, int64_t stride
   constexpr int kEach = kBytes / sizeof(T);   // elements of one copy
   constexpr int kPerRow = kChans / kEach;     // copies of a row
   static_assert(kPerRow >= 8 && (kPerRow % 32 == 0 || 32 % kPerRow == 0), "copies of a row");
+  if (kBytes == 16 && len == kRows && left >= kChans) {
+    const T* src = row0 + lane / kPerRow * stride + lane % kPerRow * kEach;
+    T* dst = tile + lane * kEach;
+#pragma unroll
+    for (int i = 0; i < kRows * kPerRow / 32; ++i, src += (32 / kPerRow) * stride)
+      copy16(dst + i * 32 * kEach, src, true);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kRows * kPerRow / 32; ++i) {
     const int at = i * 32 + lane, row = at / kPerRow, col = at % kPerRow * kEach;
@@ -319,6 +348,7 @@ struct FwdArgs {
   int N;
   float c;
   int* err;
+  Consts consts;
 };
 
 // One CTA (or cluster of CTAs) owns 64 channels of one batch row and walks along
@@ -332,10 +362,26 @@ struct FwdArgs {
 // Step 5 repeats the sequential recurrence itself, so y differs from it by the
 // rounding of the state a run starts with only.  x and the gates are read once
 // and y is written once.
-constexpr int kRun = 16;
+#ifndef GLR_FILL
+#define GLR_FILL 3
+#endif
+#ifndef GLR_RUN
+#define GLR_RUN 16
+#endif
+#ifndef GLR_WARPS
+#define GLR_WARPS 8
+#endif
+#ifndef GLR_MINB
+#define GLR_MINB 2
+#endif
+#ifndef GLR_STAGES
+#define GLR_STAGES 2
+#endif
+constexpr int kRun = GLR_RUN;
 
-template <bool kNear, typename T>
-__device__ __forceinline__ void fwd_run(const T* tiles, int lane, float2 k, float2* a, float2* u) {
+template <bool kAllNear, typename T>
+__device__ __forceinline__ void fwd_run(const T* tiles, int lane, float2 k, const Consts& c, float2* a,
+                                        float2* u) {
   using P = Pair<T>;
   using Word = typename P::Word;
   constexpr int kTile = kRun * kChans;
@@ -343,17 +389,18 @@ __device__ __forceinline__ void fwd_run(const T* tiles, int lane, float2 k, floa
   for (int j = 0; j < kRun; ++j) {
     const Word* w = reinterpret_cast<const Word*>(tiles + j * kChans) + lane;
     const float2 xv = P::get(w[0]);
-    const float2 si = sigmoid2(P::get(w[kTile / 2]));
-    const float2 sr = sigmoid2(P::get(w[kTile]));
+    const float2 si = sigmoid2(P::get(w[kTile / 2]), c);
+    const float2 sr = sigmoid2(P::get(w[kTile]), c);
     float2 m2;
-    decay2<kNear>(fmul2(sr, fmul2(k, both(-1.0f))), a[j], m2);
+    decay2<kAllNear>(fmul2(sr, k), a[j], m2, c);
     const float2 m = make_float2(sqrt_approx_f(m2.x), sqrt_approx_f(m2.y));
     u[j] = fmul2(fmul2(m, si), xv);
   }
 }
 
 template <typename T, int kBytes, bool kPacked, int kStages>
-__global__ void __launch_bounds__(kMaxWarps * 32, 2) glr_fwd_scan(const FwdArgs p) {
+__global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
+    glr_fwd_scan(const __grid_constant__ FwdArgs p) {
   constexpr int kTile = kRun * kChans;  // elements
   extern __shared__ __align__(16) char dynamic_smem[];
   __shared__ float4 warp_run[2][kMaxWarps][32];   // (A, H) of two channels
@@ -406,11 +453,18 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) glr_fwd_scan(const FwdArgs 
   const float2 lam = load_state(p.lam + ch, have);
   const float2 k = make_float2(have > 0 ? decay_rate(lam.x, p.c) : 0.0f,
                                have > 1 ? decay_rate(lam.y, p.c) : 0.0f);
-  // sigmoid <= 1: no log a of this warp is below -max k.
-  const bool near = __all_sync(~0u, k.x < -kNearLog && k.y < -kNearLog);
+  // -log a = k sigmoid(r) <= k.
+  const bool near = __all_sync(~0u, k.x < kNear && k.y < kNear);
   float2 carry = both(0.0f);
   if (!kPacked) carry = load_state(p.h0 ? p.h0 + b * D + ch : nullptr, have);
-  if (size > 1) cluster_sync();  // every CTA runs before its shared memory is written
+  // Maps of warps and CTAs that do not exist stay the identity.
+  const float4 identity = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
+  for (int w = warp; w < kMaxWarps; w += warps)
+    warp_run[0][w][lane] = warp_run[1][w][lane] = identity;
+  for (int r = warp; r < kMaxCluster; r += warps)
+    cta_run[0][r][lane] = cta_run[1][r][lane] = identity;
+  __syncthreads();
+  if (size > 1) cluster_sync();  // every CTA got here before another writes its maps
 
   int par = 0, stage = 0;
   for (int64_t base = 0; base < T_; base += stride, par ^= 1) {
@@ -428,9 +482,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) glr_fwd_scan(const FwdArgs 
     const T* tiles = ring + stage * (3 * kTile);
     if (len > 0) {
       if (near)
-        fwd_run<true>(tiles, lane, k, a, u);
+        fwd_run<true>(tiles, lane, k, p.consts, a, u);
       else
-        fwd_run<false>(tiles, lane, k, a, u);
+        fwd_run<false>(tiles, lane, k, p.consts, a, u);
     }
     __syncwarp();  // read by every lane before they are overwritten
     fetch(stage);
@@ -453,21 +507,27 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) glr_fwd_scan(const FwdArgs 
 
     warp_run[par][warp][lane] = run.word();
     __syncthreads();
-    float2 h;
+    float2 h = carry;
     if (size > 1) {
       // The CTA's map, to every CTA of the cluster (warp w writes to CTA w, w + warps, ...).
       Run all(warp_run[par][0][lane]);
-      for (int w = 1; w < warps; ++w) all = join<kPacked>(all, Run(warp_run[par][w][lane]));
+#pragma unroll
+      for (int w = 1; w < kMaxWarps; ++w)
+        all = join<kPacked>(all, Run(warp_run[par][w][lane]));
       for (uint32_t r = warp; r < size; r += warps)
         st_cluster(&cta_run[par][rank][lane], r, all.word());
       cluster_sync();
-      for (uint32_t r = 0; r < size; ++r) {
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxCluster; ++r) {
         if (r == rank) h = carry;
         carry = apply<kPacked>(Run(cta_run[par][r][lane]), carry);
       }
-      for (int w = 0; w < warp; ++w) h = apply<kPacked>(Run(warp_run[par][w][lane]), h);
+#pragma unroll
+      for (int w = 0; w < kMaxWarps - 1; ++w)
+        if (w < warp) h = apply<kPacked>(Run(warp_run[par][w][lane]), h);
     } else {
-      for (int w = 0; w < warps; ++w) {
+#pragma unroll
+      for (int w = 0; w < kMaxWarps; ++w) {
         if (w == warp) h = carry;
         carry = apply<kPacked>(Run(warp_run[par][w][lane]), carry);
       }
@@ -476,13 +536,21 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) glr_fwd_scan(const FwdArgs 
     if (p.states && len > 0 && t0 % kSegment == 0)
       store_state(p.states + (b * nseg + t0 / kSegment) * D + ch, h, have);
     T* yp = static_cast<T*>(p.y) + (b * T_ + t0) * D + ch;
+    if (!kPacked && kBytes == 16 && len == kRun && ch0 + kChans <= D) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      h = apply<kPacked>(Run{a[j], u[j]}, h);
-      if (j < len) {
-        store_pair<T, kBytes>(yp + j * D, h, have);
-        if (kPacked && ((starts >> (j + 1) & 1) || t0 + j + 1 == T_))
-          store_state(p.hT + seq_of(p.cu, p.N, t0 + j) * D + ch, h, have);
+      for (int j = 0; j < kRun; ++j, yp += D) {
+        h = apply<kPacked>(Run{a[j], u[j]}, h);
+        store_pair<T, kBytes>(yp, h, 2);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        h = apply<kPacked>(Run{a[j], u[j]}, h);
+        if (j < len) {
+          store_pair<T, kBytes>(yp + j * D, h, have);
+          if (kPacked && ((starts >> (j + 1) & 1) || t0 + j + 1 == T_))
+            store_state(p.hT + seq_of(p.cu, p.N, t0 + j) * D + ch, h, have);
+        }
       }
     }
     if (!kPacked && len > 0 && t0 + len == T_) store_state(p.hT + b * D + ch, h, have);
@@ -504,14 +572,14 @@ inline ScanGrid scan_grid(int64_t batch, int64_t seq_len, int64_t dim, int run) 
   const int64_t runs = (seq_len + run - 1) / run;
   g.warps = static_cast<int>(std::min<int64_t>(runs, kMaxWarps));
   g.cluster = 1;
-  while (g.cluster < kMaxCluster && g.blocks * batch * g.cluster < 3 * sm_count() &&
+  while (g.cluster < kMaxCluster && g.blocks * batch * g.cluster < GLR_FILL * sm_count() &&
          g.cluster * g.warps < runs)
     g.cluster *= 2;
   return g;
 }
 
 template <typename A>
-int launch_scan(void (*kernel)(A), const ScanGrid& g, int64_t batch, size_t smem, const A& args,
+int launch_scan(void (*kernel)(const A), const ScanGrid& g, int64_t batch, size_t smem, const A& args,
                 cudaStream_t s) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
@@ -546,7 +614,7 @@ inline int copy_bytes(const void* p, int64_t sb, int64_t st, int64_t itemsize) {
 
 template <typename T>
 int launch_fwd(const FwdArgs& a, int64_t batch, cudaStream_t s) {
-  constexpr int kStages = sizeof(T) == 2 ? 2 : 1;  // about 100 KB of tiles: two CTAs an SM
+  constexpr int kStages = sizeof(T) == 2 ? GLR_STAGES : GLR_STAGES / 2;  // about 100 KB of tiles: two CTAs an SM
   constexpr int64_t eb = sizeof(T);
   const int bytes = std::min({copy_bytes(a.x, a.st.xb, a.st.xt, eb),
                               copy_bytes(a.ig, a.st.ib, a.st.it, eb),
@@ -686,7 +754,7 @@ extern "C" int tileops_glr_fwd(const void* x, const void* input_gate, const void
   const Strides st{x_stride_b, x_stride_t, i_stride_b, i_stride_t, r_stride_b, r_stride_t, 0, 0};
   const FwdArgs args{x, input_gate, decay_gate, decay_param, initial_state, cu_seqlens, y,
                      final_state, states, seq_len, dim, st, static_cast<int>(num_seqs),
-                     static_cast<float>(decay_scale), cu_seqlens ? device_error_ptr() : nullptr};
+                     static_cast<float>(decay_scale), cu_seqlens ? device_error_ptr() : nullptr, Consts()};
   switch (dtype) {
     case TILEOPS_DT_F32: return launch_fwd<float>(args, batch, s);
     case TILEOPS_DT_F16: return launch_fwd<__half>(args, batch, s);
