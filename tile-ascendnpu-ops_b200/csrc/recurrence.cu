@@ -337,6 +337,16 @@ __device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t
   return bits;
 }
 
+// Warp w passes on to the next one, which waits: hardware barrier 1 + w counts
+// the 32 threads of each.  A warp passes a second time only after the state has
+// gone all the way round, so its successor has long waited for the first.
+__device__ __forceinline__ void link_pass(int w) {
+  asm volatile("bar.arrive %0, 64;" ::"r"(1 + w) : "memory");
+}
+__device__ __forceinline__ void link_wait(int w) {
+  asm volatile("bar.sync %0, 64;" ::"r"(1 + w) : "memory");
+}
+
 struct FwdArgs {
   const void *x, *ig, *rg;
   const float *lam, *h0;
@@ -505,10 +515,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
 #pragma unroll
     for (int j = 1; j < kRun; ++j) run = join<kPacked>(run, Run{a[j], u[j]});
 
-    warp_run[par][warp][lane] = run.word();
-    __syncthreads();
     float2 h = carry;
     if (size > 1) {
+      warp_run[par][warp][lane] = run.word();
+      __syncthreads();
       // The CTA's map, to every CTA of the cluster (warp w writes to CTA w, w + warps, ...).
       Run all(warp_run[par][0][lane]);
 #pragma unroll
@@ -526,10 +536,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
       for (int w = 0; w < kMaxWarps - 1; ++w)
         if (w < warp) h = apply<kPacked>(Run(warp_run[par][w][lane]), h);
     } else {
-#pragma unroll
-      for (int w = 0; w < kMaxWarps; ++w) {
-        if (w == warp) h = carry;
-        carry = apply<kPacked>(Run(warp_run[par][w][lane]), carry);
+      // A chain from warp to warp: the state goes on as soon as it is known, and
+      // each warp waits for its predecessor alone.
+      if (base > 0 || warp > 0) {
+        if (warps > 1) link_wait(warp == 0 ? warps - 1 : warp - 1);
+        h = make_float2(warp_run[0][warp][lane].x, warp_run[0][warp][lane].y);
+      }
+      if (warp + 1 < warps || base + stride < T_) {
+        const int to = warp + 1 == warps ? 0 : warp + 1;
+        const float2 out = apply<kPacked>(run, h);
+        *reinterpret_cast<float2*>(&warp_run[0][to][lane]) = out;
+        if (warps > 1) link_pass(warp);
       }
     }
 
