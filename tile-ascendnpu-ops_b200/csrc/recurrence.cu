@@ -220,6 +220,11 @@ struct Run {
   __device__ __forceinline__ float4 word() const { return make_float4(A.x, A.y, H.x, H.y); }
 };
 
+__device__ __forceinline__ Run shuffle_up(const Run& r, int by) {
+  return Run(make_float2(__shfl_up_sync(~0u, r.A.x, by), __shfl_up_sync(~0u, r.A.y, by)),
+             make_float2(__shfl_up_sync(~0u, r.H.x, by), __shfl_up_sync(~0u, r.H.y, by)));
+}
+
 template <bool kPacked>
 __device__ __forceinline__ float2 apply(const Run& run, float2 h) {
   float2 next = ffma2(run.A, h, run.H);
@@ -244,11 +249,17 @@ __device__ __forceinline__ Run join(const Run& first, const Run& then) {
 #endif
 constexpr int kMaxWarps = GLR_WARPS;    // warps of a CTA
 constexpr int kMaxCluster = 8;  // CTAs of a cluster
-constexpr int kChans = 64;      // channels of a CTA: two a lane
+#ifndef GLR_CHANS
+#define GLR_CHANS 32
+#endif
+constexpr int kChans = GLR_CHANS;         // channels of a CTA: two a lane
+constexpr int kPairs = kChans / 2;        // lanes side by side
+constexpr int kGroups = 32 / kPairs;      // groups of lanes, one after another in time
 
 // ---- a warp's rows in shared memory ----
-// A tile is kRows tokens of the 64 channels of the warp, rows of one tensor one
-// below another.  The warp copies its own tiles and only it reads them, so no
+// A tile is kWarpRun tokens of the channels of the warp, rows of one tensor one
+// below another, a row left out after each group's so that the groups read
+// different banks.  The warp copies its own tiles and only it reads them, so no
 // barrier but its own is needed.  kBytes: what one copy moves, the widest that
 // the tensors' addresses and strides allow (16; 4; 2 by plain loads, as
 // cp.async has no such size).
@@ -272,33 +283,39 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Copies `len` rows (0 <= len <= kRows) starting at `row0`, which points at the first of
-// the CTA's channels; `left` of them exist (0 < left).  What does not exist is
-// filled with zeros and not read: its source is `row0` itself.
-template <typename T, int kRows, int kBytes>
+constexpr int kRun = 16;                      // tokens of a lane
+constexpr int kWarpRun = kRun * kGroups;      // tokens of a warp
+constexpr int kTile = (kWarpRun + kGroups) * kChans;  // elements
+__device__ __forceinline__ constexpr int tile_row(int row) {
+  return (row + row / kRun) * kChans;
+}
+
+// Copies `len` rows (0 < len <= kWarpRun) starting at `row0`, which points at the first
+// of the CTA's channels; `left` of them exist (0 < left).  What does not exist
+// is filled with zeros and not read: its source is `row0` itself.
+template <typename T, int kBytes>
 __device__ __forceinline__ void copy_tile(T* tile, const T* row0, int64_t stride, int len,
                                           int64_t left, int lane) {
   constexpr int kEach = kBytes / sizeof(T);   // elements of one copy
   constexpr int kPerRow = kChans / kEach;     // copies of a row
-  static_assert(kPerRow >= 8 && (kPerRow % 32 == 0 || 32 % kPerRow == 0), "copies of a row");
-  if (kBytes == 16 && len == kRows && left >= kChans) {
-    const T* src = row0 + lane / kPerRow * stride + lane % kPerRow * kEach;
-    T* dst = tile + lane * kEach;
+  constexpr int kRows = 32 / kPerRow;         // rows of one instruction
+  static_assert(32 % kPerRow == 0 && (kRows % kRun == 0 || kRun % kRows == 0), "copies of a row");
+  const int r0 = lane / kPerRow, col = lane % kPerRow * kEach;
+  const T* src = row0 + r0 * stride + col;
+  if (kBytes == 16 && len == kWarpRun && left >= kChans) {
 #pragma unroll
-    for (int i = 0; i < kRows * kPerRow / 32; ++i, src += (32 / kPerRow) * stride)
-      copy16(dst + i * 32 * kEach, src, true);
+    for (int i = 0; i < kWarpRun / kRows; ++i, src += kRows * stride)
+      copy16(tile + tile_row(i * kRows + r0) + col, src, true);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < kRows * kPerRow / 32; ++i) {
-    const int at = i * 32 + lane, row = at / kPerRow, col = at % kPerRow * kEach;
-    const bool in = row < len && col < left;
-    const T* src = in ? row0 + row * stride + col : row0;
-    T* dst = tile + row * kChans + col;
+  for (int i = 0; i < kWarpRun / kRows; ++i, src += kRows * stride) {
+    const bool in = i * kRows + r0 < len && col < left;
+    T* dst = tile + tile_row(i * kRows + r0) + col;
     if constexpr (kBytes == 16)
-      copy16(dst, src, in);
+      copy16(dst, in ? src : row0, in);
     else if constexpr (kBytes == 4)
-      copy4(dst, src, in);
+      copy4(dst, in ? src : row0, in);
     else
       *dst = in ? *src : Cvt<T>::from_f(0.0f);
   }
@@ -323,18 +340,26 @@ __device__ __forceinline__ void store_state(float* p, float2 v, int have) {
   if (have > 1) p[1] = v.y;
 }
 
-// Which of `count` tokens from t0 on start a sequence, as bits; the sequence of t0 in n0.
-// Empty sequences start no token.  Every lane returns the same.
-__device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t t0, int count,
+// Which tokens of a lane's run start a sequence: bit j for token t0 + j, j = 0 .. kRun (one
+// more than the run has, for the end of its last token).  Empty sequences start
+// no token.  w0: the first token of the warp's run, the same in every lane.
+__device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t w0, int group,
                                                int lane) {
-  const int n0 = seq_of(cu, N, t0);
-  uint32_t bits = cu[n0] == t0 ? 1u : 0u;
+  const int n0 = seq_of(cu, N, w0);
+  uint64_t bits = cu[n0] == w0 ? 1 : 0;
+  uint32_t beyond = 0;  // token w0 + 64
+  static_assert(kWarpRun <= 64, "bits of a warp's run");
   for (int n = n0 + 1; n < N; n += 32) {
-    const int64_t at = n + lane < N ? cu[n + lane] - t0 : count;
-    bits |= __reduce_or_sync(~0u, at > 0 && at < count ? 1u << at : 0u);
-    if (__shfl_sync(~0u, static_cast<int>(at < count), 31) == 0) break;
+    const int64_t at = n + lane < N ? cu[n + lane] - w0 : kWarpRun + 1;
+    const uint64_t mine = at > 0 && at < 64 ? 1ull << at : 0ull;
+    bits |= static_cast<uint64_t>(__reduce_or_sync(~0u, static_cast<uint32_t>(mine >> 32))) << 32 |
+            __reduce_or_sync(~0u, static_cast<uint32_t>(mine));
+    beyond |= __any_sync(~0u, at == 64);
+    if (__shfl_sync(~0u, static_cast<int>(at <= kWarpRun), 31) == 0) break;
   }
-  return bits;
+  uint32_t run = static_cast<uint32_t>(bits >> (group * kRun)) & ((1u << (kRun + 1)) - 1);
+  if (group * kRun + kRun == 64) run |= beyond << kRun;
+  return run;
 }
 
 // Warp w passes on to the next one, which waits: hardware barrier 1 + w counts
@@ -361,8 +386,8 @@ struct FwdArgs {
   Consts consts;
 };
 
-// One CTA (or cluster of CTAs) owns 64 channels of one batch row and walks along
-// its tokens; a lane owns two channels and a warp kRun tokens at a time:
+// One CTA (or cluster of CTAs) owns 16 channels of one batch row and walks along
+// its tokens; a lane owns two channels and 16 tokens of its warp's 64 at a time:
 //   1. x and the gates of the run, copied to the warp's tiles a step or two ahead;
 //   2. a_t, u_t into registers, and the run's map (A, H);
 //   3. the maps are exchanged: between warps through shared memory, between the
@@ -373,13 +398,7 @@ struct FwdArgs {
 // rounding of the state a run starts with only.  x and the gates are read once
 // and y is written once.
 #ifndef GLR_FILL
-#define GLR_FILL 3
-#endif
-#ifndef GLR_RUN
-#define GLR_RUN 16
-#endif
-#ifndef GLR_WARPS
-#define GLR_WARPS 8
+#define GLR_FILL 2
 #endif
 #ifndef GLR_MINB
 #define GLR_MINB 2
@@ -387,56 +406,53 @@ struct FwdArgs {
 #ifndef GLR_STAGES
 #define GLR_STAGES 2
 #endif
-constexpr int kRun = GLR_RUN;
 
+// Decays and inputs of a lane's run.
 template <bool kAllNear, typename T>
-__device__ __forceinline__ void fwd_run(const T* tiles, int lane, float2 k, const Consts& c, float2* a,
+__device__ __forceinline__ void fwd_run(const T* mine, float2 k, const Consts& c, float2* a,
                                         float2* u) {
   using P = Pair<T>;
   using Word = typename P::Word;
-  constexpr int kTile = kRun * kChans;
 #pragma unroll
   for (int j = 0; j < kRun; ++j) {
-    const Word* w = reinterpret_cast<const Word*>(tiles + j * kChans) + lane;
-    const float2 xv = P::get(w[0]);
-    const float2 si = sigmoid2(P::get(w[kTile / 2]), c);
-    const float2 sr = sigmoid2(P::get(w[kTile]), c);
+    const Word* w = reinterpret_cast<const Word*>(mine + j * kChans);
+    const float2 si = sigmoid2(P::get(w[kTile / 2]), c), sr = sigmoid2(P::get(w[kTile]), c);
     float2 m2;
     decay2<kAllNear>(fmul2(sr, k), a[j], m2, c);
     const float2 m = make_float2(sqrt_approx_f(m2.x), sqrt_approx_f(m2.y));
-    u[j] = fmul2(fmul2(m, si), xv);
+    u[j] = fmul2(fmul2(m, si), P::get(w[0]));
   }
 }
 
 template <typename T, int kBytes, bool kPacked, int kStages>
 __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
     glr_fwd_scan(const __grid_constant__ FwdArgs p) {
-  constexpr int kTile = kRun * kChans;  // elements
   extern __shared__ __align__(16) char dynamic_smem[];
-  __shared__ float4 warp_run[2][kMaxWarps][32];   // (A, H) of two channels
-  __shared__ float4 cta_run[2][kMaxCluster][32];
+  __shared__ float4 warp_run[2][kMaxWarps][kPairs];  // (A, H) of two channels
+  __shared__ float4 cta_run[2][kMaxCluster][kPairs];
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
   const int warps = blockDim.x >> 5;
   const uint32_t size = cluster_size(), rank = cluster_rank();
   const int64_t b = blockIdx.y, T_ = p.T, D = p.D;
-  const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * kChans, ch = ch0 + 2 * lane;
+  const int group = lane / kPairs, pair = lane % kPairs;
+  const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * kChans, ch = ch0 + 2 * pair;
   const int have = ch + 1 < D ? 2 : (ch < D ? 1 : 0);  // channels of this lane
   T* ring = reinterpret_cast<T*>(dynamic_smem) + warp * (kStages * 3 * kTile);
   const int64_t nseg = (T_ + kSegment - 1) / kSegment;
-  const int64_t stride = static_cast<int64_t>(kRun) * warps * size;  // tokens of a step
+  const int64_t stride = static_cast<int64_t>(kWarpRun) * warps * size;  // tokens of a step
 
-  int64_t next = static_cast<int64_t>(rank * warps + warp) * kRun;  // run to be copied next
+  int64_t next = static_cast<int64_t>(rank * warps + warp) * kWarpRun;  // to be copied next
   const T* xn = static_cast<const T*>(p.x) + b * p.st.xb + ch0 + next * p.st.xt;
   const T* in = static_cast<const T*>(p.ig) + b * p.st.ib + ch0 + next * p.st.it;
   const T* rn = static_cast<const T*>(p.rg) + b * p.st.rb + ch0 + next * p.st.rt;
   auto fetch = [&](int stage) {
     if (next < T_) {
-      const int len = T_ - next < kRun ? static_cast<int>(T_ - next) : kRun;
+      const int len = T_ - next < kWarpRun ? static_cast<int>(T_ - next) : kWarpRun;
       T* t = ring + stage * (3 * kTile);
-      copy_tile<T, kRun, kBytes>(t, xn, p.st.xt, len, D - ch0, lane);
-      copy_tile<T, kRun, kBytes>(t + kTile, in, p.st.it, len, D - ch0, lane);
-      copy_tile<T, kRun, kBytes>(t + 2 * kTile, rn, p.st.rt, len, D - ch0, lane);
+      copy_tile<T, kBytes>(t, xn, p.st.xt, len, D - ch0, lane);
+      copy_tile<T, kBytes>(t + kTile, in, p.st.it, len, D - ch0, lane);
+      copy_tile<T, kBytes>(t + 2 * kTile, rn, p.st.rt, len, D - ch0, lane);
       xn += stride * p.st.xt;
       in += stride * p.st.it;
       rn += stride * p.st.rt;
@@ -449,7 +465,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
 
   if (kPacked) {
     // Sequences without a token end where they began; the offsets are checked once.
-    for (int n = rank * warps + warp; n < p.N; n += size * warps)
+    for (int64_t n = (rank * warps + warp) * kGroups + group; n < p.N;
+         n += size * warps * kGroups)
       if (p.cu[n + 1] <= p.cu[n])
         store_state(p.hT + n * D + ch, load_state(p.h0 ? p.h0 + n * D + ch : nullptr, have), have);
     if (blockIdx.x == 0 && warp == 0) {
@@ -470,31 +487,32 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
   // Maps of warps and CTAs that do not exist stay the identity.
   const float4 identity = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
   for (int w = warp; w < kMaxWarps; w += warps)
-    warp_run[0][w][lane] = warp_run[1][w][lane] = identity;
+    warp_run[0][w][pair] = warp_run[1][w][pair] = identity;
   for (int r = warp; r < kMaxCluster; r += warps)
-    cta_run[0][r][lane] = cta_run[1][r][lane] = identity;
+    cta_run[0][r][pair] = cta_run[1][r][pair] = identity;
   __syncthreads();
   if (size > 1) cluster_sync();  // every CTA got here before another writes its maps
 
   int par = 0, stage = 0;
   for (int64_t base = 0; base < T_; base += stride, par ^= 1) {
-    const int64_t t0 = base + static_cast<int64_t>(rank * warps + warp) * kRun;
+    const int64_t w0 = base + static_cast<int64_t>(rank * warps + warp) * kWarpRun;
+    const int64_t t0 = w0 + group * kRun;
     const int64_t left = T_ - t0;
     const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
     // Bit j: token t0 + j starts a sequence (one bit more than the run has
     // tokens, for the end of its last one).
     uint32_t starts = 0;
-    if (kPacked && len > 0) starts = start_bits(p.cu, p.N, t0, kRun + 1, lane);
+    if (kPacked && w0 < T_) starts = start_bits(p.cu, p.N, w0, group, lane);
 
     float2 a[kRun], u[kRun];
     copies_wait<kStages - 1>();
     __syncwarp();  // the tiles of this step have landed, whichever lane copied them
-    const T* tiles = ring + stage * (3 * kTile);
-    if (len > 0) {
+    const T* mine = ring + stage * (3 * kTile) + tile_row(group * kRun) + 2 * pair;
+    if (w0 < T_) {
       if (near)
-        fwd_run<true>(tiles, lane, k, p.consts, a, u);
+        fwd_run<true>(mine, k, p.consts, a, u);
       else
-        fwd_run<false>(tiles, lane, k, p.consts, a, u);
+        fwd_run<false>(mine, k, p.consts, a, u);
     }
     __syncwarp();  // read by every lane before they are overwritten
     fetch(stage);
@@ -514,41 +532,57 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
     Run run = {a[0], u[0]};
 #pragma unroll
     for (int j = 1; j < kRun; ++j) run = join<kPacked>(run, Run{a[j], u[j]});
+    // Joined along the lane groups: `run` ends with this group's, `before` with the last one's.
+#pragma unroll
+    for (int off = kPairs; off < 32; off *= 2) {
+      const Run earlier = shuffle_up(run, off);
+      if (lane >= off) run = join<kPacked>(earlier, run);
+    }
+    const Run before = shuffle_up(run, kPairs);
+    const bool last = group == kGroups - 1;  // its `run` is the whole warp's
 
     float2 h = carry;
     if (size > 1) {
-      warp_run[par][warp][lane] = run.word();
+      if (last) warp_run[par][warp][pair] = run.word();
       __syncthreads();
       // The CTA's map, to every CTA of the cluster (warp w writes to CTA w, w + warps, ...).
-      Run all(warp_run[par][0][lane]);
+      Run all(warp_run[par][0][pair]);
 #pragma unroll
       for (int w = 1; w < kMaxWarps; ++w)
-        all = join<kPacked>(all, Run(warp_run[par][w][lane]));
-      for (uint32_t r = warp; r < size; r += warps)
-        st_cluster(&cta_run[par][rank][lane], r, all.word());
+        all = join<kPacked>(all, Run(warp_run[par][w][pair]));
+      if (last)
+        for (uint32_t r = warp; r < size; r += warps)
+          st_cluster(&cta_run[par][rank][pair], r, all.word());
+      __syncwarp();
       cluster_sync();
 #pragma unroll
       for (uint32_t r = 0; r < kMaxCluster; ++r) {
         if (r == rank) h = carry;
-        carry = apply<kPacked>(Run(cta_run[par][r][lane]), carry);
+        carry = apply<kPacked>(Run(cta_run[par][r][pair]), carry);
       }
 #pragma unroll
       for (int w = 0; w < kMaxWarps - 1; ++w)
-        if (w < warp) h = apply<kPacked>(Run(warp_run[par][w][lane]), h);
+        if (w < warp) h = apply<kPacked>(Run(warp_run[par][w][pair]), h);
     } else {
       // A chain from warp to warp: the state goes on as soon as it is known, and
       // each warp waits for its predecessor alone.
+      float4* link = warp_run[0][0];  // [warp][pair]: the state before a warp's run
       if (base > 0 || warp > 0) {
         if (warps > 1) link_wait(warp == 0 ? warps - 1 : warp - 1);
-        h = make_float2(warp_run[0][warp][lane].x, warp_run[0][warp][lane].y);
+        else __syncwarp();
+        const float4 v = link[warp * kPairs + pair];
+        h = make_float2(v.x, v.y);
       }
       if (warp + 1 < warps || base + stride < T_) {
         const int to = warp + 1 == warps ? 0 : warp + 1;
         const float2 out = apply<kPacked>(run, h);
-        *reinterpret_cast<float2*>(&warp_run[0][to][lane]) = out;
+        if (warps == 1) __syncwarp();  // read above before it is overwritten
+        if (last) link[to * kPairs + pair] = make_float4(out.x, out.y, 0.0f, 0.0f);
+        __syncwarp();
         if (warps > 1) link_pass(warp);
       }
     }
+    if (group > 0) h = apply<kPacked>(before, h);
 
     if (p.states && len > 0 && t0 % kSegment == 0)
       store_state(p.states + (b * nseg + t0 / kSegment) * D + ch, h, have);
@@ -637,8 +671,8 @@ int launch_fwd(const FwdArgs& a, int64_t batch, cudaStream_t s) {
                               copy_bytes(a.ig, a.st.ib, a.st.it, eb),
                               copy_bytes(a.rg, a.st.rb, a.st.rt, eb),
                               copy_bytes(a.y, a.D, a.D, eb)});
-  const ScanGrid g = scan_grid(batch, a.T, a.D, kRun);
-  const size_t smem = static_cast<size_t>(g.warps) * kStages * 3 * kRun * kChans * sizeof(T);
+  const ScanGrid g = scan_grid(batch, a.T, a.D, kWarpRun);
+  const size_t smem = static_cast<size_t>(g.warps) * kStages * 3 * kTile * sizeof(T);
   auto go = [&](auto packed, auto plain) {
     return launch_scan(a.cu ? packed : plain, g, batch, smem, a, s);
   };
