@@ -239,7 +239,7 @@ int tileops_gla_decode_fwd(const void* q, const void* k, const void* v, const vo
 
 /* ---- gated linear recurrence --------------------------------------------- */
 
-#define TILEOPS_GLR_SEGMENT 64 /* tokens between two saved states */
+#define TILEOPS_GLR_SEGMENT 32 /* tokens between two saved states */
 
 /* Per channel, with k = decay_scale * softplus(decay_param):
  *   a_t = exp(-k sigmoid(decay_gate_t));

@@ -148,7 +148,7 @@ def glr_bwd(dy, x, input_gate, decay_gate, decay_param, initial_state=None, d_fi
 
 
 def glr_states(x, input_gate, decay_gate, decay_param, initial_state=None, decay_scale=8.0,
-               segment: int = 64):
+               segment: int = 32):
     """The state before every ``segment`` tokens, and its bound (no packed sequences)."""
     h0 = _wide(initial_state)
     y, _, ey, _ = glr_fwd(x, input_gate, decay_gate, decay_param, initial_state,

@@ -82,8 +82,8 @@ def test_oracle_states_and_identity_gates():
     lam, h0 = torch.zeros(2), torch.randn(1, 2)
     states, bound = ref.glr_states(x, i, r, lam, h0)
     y, final, _, _ = ref.glr_fwd(x, i, r, lam, h0)
-    assert states.shape == (1, 3, 2) and torch.equal(states[0, 0], h0[0].double())
-    assert torch.equal(states[0, 2], y[0, 127]) and torch.equal(final[0], y[0, -1])
+    assert states.shape == (1, 5, 2) and torch.equal(states[0, 0], h0[0].double())
+    assert torch.equal(states[0, 4], y[0, 127]) and torch.equal(final[0], y[0, -1])
     assert (bound[:, 1:] > 0).all()
     shut = torch.full_like(r, -float("inf"))
     y, final, _, _ = ref.glr_fwd(x, i, shut, lam, h0)
@@ -182,9 +182,9 @@ def test_recurrence_rejects_wrong_states_and_offsets(accept_cpu):
     with pytest.raises(ValueError, match="states.shape"):
         bwd(dy, *args, torch.randn(1, 1, 8))
     with pytest.raises(ValueError, match="d_final_state.shape"):
-        bwd(dy, *args, torch.randn(1, 2, 8), None, torch.randn(2, 8))
+        bwd(dy, *args, torch.randn(1, 3, 8), None, torch.randn(2, 8))
     with pytest.raises(ValueError, match="dy.shape"):
-        bwd(dy[:, :64], *args, torch.randn(1, 2, 8))
+        bwd(dy[:, :64], *args, torch.randn(1, 3, 8))
 
 
 def test_decode_rejects_wrong_inputs(accept_cpu):
@@ -251,7 +251,7 @@ def test_rooflines_and_init_args():
                                              dtype=torch.float16, save_states=True)
     op = GatedLinearRecurrenceBwdOp(2, 100, 64, dtype=torch.float32)
     assert op.eval_roofline() == (40 * 12800,
-                                  7 * 12800 * 4 + 4 * 2 * 2 * 64 + 8 * 128 + 8 * 64)
+                                  7 * 12800 * 4 + 4 * 2 * 4 * 64 + 8 * 128 + 8 * 64)
     op = GatedLinearRecurrenceDecodeOp(3, 64, dtype=torch.float32)
     assert op.eval_roofline() == (20 * 192, 4 * 192 * 4 + 8 * 192 + 4 * 64)
     with pytest.raises(RuntimeError, match="requires a prior"):

@@ -220,9 +220,13 @@ struct Run {
   __device__ __forceinline__ float4 word() const { return make_float4(A.x, A.y, H.x, H.y); }
 };
 
-__device__ __forceinline__ Run shuffle_up(const Run& r, int by) {
-  return Run(make_float2(__shfl_up_sync(~0u, r.A.x, by), __shfl_up_sync(~0u, r.A.y, by)),
-             make_float2(__shfl_up_sync(~0u, r.H.x, by), __shfl_up_sync(~0u, r.H.y, by)));
+// The map of the lane `by` below (backwards: above).
+template <bool kBackwards>
+__device__ __forceinline__ Run shuffle_by(const Run& r, int by) {
+  auto f = [&](float v) {
+    return kBackwards ? __shfl_down_sync(~0u, v, by) : __shfl_up_sync(~0u, v, by);
+  };
+  return Run(make_float2(f(r.A.x), f(r.A.y)), make_float2(f(r.H.x), f(r.H.y)));
 }
 
 template <bool kPacked>
@@ -244,17 +248,27 @@ __device__ __forceinline__ Run join(const Run& first, const Run& then) {
   return r;
 }
 
-#ifndef GLR_WARPS
-#define GLR_WARPS 8
+#ifndef GLR_FILL
+#define GLR_FILL 2
 #endif
-constexpr int kMaxWarps = GLR_WARPS;    // warps of a CTA
+#ifndef GLR_BSTAGES
+#define GLR_BSTAGES 2
+#endif
+constexpr int kMaxWarps = 8;    // warps of a CTA
 constexpr int kMaxCluster = 8;  // CTAs of a cluster
-#ifndef GLR_CHANS
-#define GLR_CHANS 32
-#endif
-constexpr int kChans = GLR_CHANS;         // channels of a CTA: two a lane
-constexpr int kPairs = kChans / 2;        // lanes side by side
-constexpr int kGroups = 32 / kPairs;      // groups of lanes, one after another in time
+
+// How a warp lies over channels and tokens: `Chans` channels side by side, two a lane,
+// and groups of lanes one after another in time, `Run` tokens a lane.
+template <int Chans, int Run>
+struct Geo {
+  static constexpr int kChans = Chans, kRun = Run;
+  static constexpr int kPairs = Chans / 2, kGroups = 32 / kPairs;
+  static constexpr int kWarpRun = Run * kGroups;                // tokens of a warp
+  static constexpr int kTile = (kWarpRun + kGroups) * Chans;    // elements of its tile
+  static __device__ __forceinline__ constexpr int tile_row(int row) {
+    return (row + row / Run) * Chans;
+  }
+};
 
 // ---- a warp's rows in shared memory ----
 // A tile is kWarpRun tokens of the channels of the warp, rows of one tensor one
@@ -283,35 +297,28 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-constexpr int kRun = 16;                      // tokens of a lane
-constexpr int kWarpRun = kRun * kGroups;      // tokens of a warp
-constexpr int kTile = (kWarpRun + kGroups) * kChans;  // elements
-__device__ __forceinline__ constexpr int tile_row(int row) {
-  return (row + row / kRun) * kChans;
-}
-
 // Copies `len` rows (0 < len <= kWarpRun) starting at `row0`, which points at the first
 // of the CTA's channels; `left` of them exist (0 < left).  What does not exist
 // is filled with zeros and not read: its source is `row0` itself.
-template <typename T, int kBytes>
+template <typename G, int kBytes, typename T>
 __device__ __forceinline__ void copy_tile(T* tile, const T* row0, int64_t stride, int len,
                                           int64_t left, int lane) {
   constexpr int kEach = kBytes / sizeof(T);   // elements of one copy
-  constexpr int kPerRow = kChans / kEach;     // copies of a row
+  constexpr int kPerRow = G::kChans / kEach;     // copies of a row
   constexpr int kRows = 32 / kPerRow;         // rows of one instruction
-  static_assert(32 % kPerRow == 0 && (kRows % kRun == 0 || kRun % kRows == 0), "copies of a row");
+  static_assert(32 % kPerRow == 0 && (kRows % G::kRun == 0 || G::kRun % kRows == 0), "copies of a row");
   const int r0 = lane / kPerRow, col = lane % kPerRow * kEach;
   const T* src = row0 + r0 * stride + col;
-  if (kBytes == 16 && len == kWarpRun && left >= kChans) {
+  if (kBytes == 16 && len == G::kWarpRun && left >= G::kChans) {
 #pragma unroll
-    for (int i = 0; i < kWarpRun / kRows; ++i, src += kRows * stride)
-      copy16(tile + tile_row(i * kRows + r0) + col, src, true);
+    for (int i = 0; i < G::kWarpRun / kRows; ++i, src += kRows * stride)
+      copy16(tile + G::tile_row(i * kRows + r0) + col, src, true);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < kWarpRun / kRows; ++i, src += kRows * stride) {
+  for (int i = 0; i < G::kWarpRun / kRows; ++i, src += kRows * stride) {
     const bool in = i * kRows + r0 < len && col < left;
-    T* dst = tile + tile_row(i * kRows + r0) + col;
+    T* dst = tile + G::tile_row(i * kRows + r0) + col;
     if constexpr (kBytes == 16)
       copy16(dst, in ? src : row0, in);
     else if constexpr (kBytes == 4)
@@ -343,22 +350,23 @@ __device__ __forceinline__ void store_state(float* p, float2 v, int have) {
 // Which tokens of a lane's run start a sequence: bit j for token t0 + j, j = 0 .. kRun (one
 // more than the run has, for the end of its last token).  Empty sequences start
 // no token.  w0: the first token of the warp's run, the same in every lane.
+template <typename G>
 __device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t w0, int group,
                                                int lane) {
   const int n0 = seq_of(cu, N, w0);
   uint64_t bits = cu[n0] == w0 ? 1 : 0;
   uint32_t beyond = 0;  // token w0 + 64
-  static_assert(kWarpRun <= 64, "bits of a warp's run");
+  static_assert(G::kWarpRun <= 64, "bits of a warp's run");
   for (int n = n0 + 1; n < N; n += 32) {
-    const int64_t at = n + lane < N ? cu[n + lane] - w0 : kWarpRun + 1;
+    const int64_t at = n + lane < N ? cu[n + lane] - w0 : G::kWarpRun + 1;
     const uint64_t mine = at > 0 && at < 64 ? 1ull << at : 0ull;
     bits |= static_cast<uint64_t>(__reduce_or_sync(~0u, static_cast<uint32_t>(mine >> 32))) << 32 |
             __reduce_or_sync(~0u, static_cast<uint32_t>(mine));
     beyond |= __any_sync(~0u, at == 64);
-    if (__shfl_sync(~0u, static_cast<int>(at <= kWarpRun), 31) == 0) break;
+    if (__shfl_sync(~0u, static_cast<int>(at <= G::kWarpRun), 31) == 0) break;
   }
-  uint32_t run = static_cast<uint32_t>(bits >> (group * kRun)) & ((1u << (kRun + 1)) - 1);
-  if (group * kRun + kRun == 64) run |= beyond << kRun;
+  uint32_t run = static_cast<uint32_t>(bits >> (group * G::kRun)) & ((1u << (G::kRun + 1)) - 1);
+  if (group * G::kRun + G::kRun == 64) run |= beyond << G::kRun;
   return run;
 }
 
@@ -372,6 +380,102 @@ __device__ __forceinline__ void link_wait(int w) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + w) : "memory");
 }
 
+// Joins the maps of a warp's lane groups in their order (backwards: from the last): `run`
+// comes back as the map up to and with the lane's own, and the result is the
+// one up to its predecessor (of no meaning in the first group).
+template <typename G, bool kPacked, bool kBackwards>
+__device__ __forceinline__ Run scan_groups(Run& run, int lane) {
+#pragma unroll
+  for (int off = G::kPairs; off < 32; off *= 2) {
+    const Run other = shuffle_by<kBackwards>(run, off);
+    if (kBackwards ? lane + off < 32 : lane >= off) run = join<kPacked>(other, run);
+  }
+  return shuffle_by<kBackwards>(run, G::kPairs);
+}
+
+// ---- the state before a warp's run ----
+// Warps take their runs in the order of the scan: q = step * warps * size + rank * warps
+// + warp (size CTAs of a cluster, this one `rank`).
+template <typename G>
+struct Exchange {
+  float4 warp_run[2][kMaxWarps][G::kPairs];  // (A, H) of two channels
+  float4 cta_run[2][kMaxCluster][G::kPairs];
+
+  // Maps of warps and CTAs that do not exist stay the identity.
+  __device__ __forceinline__ void init(int warp, int warps, uint32_t size, int pair) {
+    const float4 identity = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
+    for (int w = warp; w < kMaxWarps; w += warps)
+      warp_run[0][w][pair] = warp_run[1][w][pair] = identity;
+    for (int r = warp; r < kMaxCluster; r += warps)
+      cta_run[0][r][pair] = cta_run[1][r][pair] = identity;
+    __syncthreads();
+    if (size > 1) cluster_sync();  // every CTA got here before another writes its maps
+  }
+
+  // `run`: the map of the whole warp's run, in the lanes of `holder`.  carry: the state
+  // before the step (a cluster) or before everything (one CTA).  Two buffers in turn:
+  // one is written again only after a barrier that every reader has passed.
+  template <bool kPacked>
+  __device__ __forceinline__ float2 before(const Run& run, bool holder, float2& carry, int par,
+                                           bool first, bool more, int warp, int warps,
+                                           uint32_t size, uint32_t rank, int pair) {
+    float2 h = carry;
+    if (size > 1) {
+      if (holder) warp_run[par][warp][pair] = run.word();
+      __syncthreads();
+      // The CTA's map, to every CTA of the cluster (warp w writes to CTA w, w + warps, ...).
+      Run all(warp_run[par][0][pair]);
+#pragma unroll
+      for (int w = 1; w < kMaxWarps; ++w)
+        all = join<kPacked>(all, Run(warp_run[par][w][pair]));
+      if (holder)
+        for (uint32_t r = warp; r < size; r += warps)
+          st_cluster(&cta_run[par][rank][pair], r, all.word());
+      __syncwarp();
+      cluster_sync();
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxCluster; ++r) {
+        if (r == rank) h = carry;
+        carry = apply<kPacked>(Run(cta_run[par][r][pair]), carry);
+      }
+#pragma unroll
+      for (int w = 0; w < kMaxWarps - 1; ++w)
+        if (w < warp) h = apply<kPacked>(Run(warp_run[par][w][pair]), h);
+    } else {
+      // A chain from warp to warp: the state goes on as soon as it is known, and
+      // each warp waits for its predecessor alone.
+      float4* link = warp_run[0][0];  // [warp][pair]: the state before a warp's run
+      if (!first || warp > 0) {
+        if (warps > 1)
+          link_wait(warp == 0 ? warps - 1 : warp - 1);
+        else
+          __syncwarp();
+        const float4 v = link[warp * G::kPairs + pair];
+        h = make_float2(v.x, v.y);
+      }
+      if (more || warp + 1 < warps) {
+        const int to = warp + 1 == warps ? 0 : warp + 1;
+        const float2 out = apply<kPacked>(run, h);
+        if (warps == 1) __syncwarp();  // read above before it is overwritten
+        if (holder) link[to * G::kPairs + pair] = make_float4(out.x, out.y, 0.0f, 0.0f);
+        __syncwarp();
+        if (warps > 1) link_pass(warp);
+      }
+    }
+    return h;
+  }
+};
+
+// cu_seqlens must be 0 = cu[0] <= ... <= cu[N] = total; reported otherwise.
+__device__ __forceinline__ void check_seqlens(const int32_t* cu, int N, int64_t total, int lane,
+                                              int* err) {
+  bool bad = false;
+  for (int n = lane; n < N; n += 32) bad |= cu[n + 1] < cu[n];
+  bad |= cu[0] != 0 || cu[N] != total;
+  if (bad) report_device_error(err, kErrBadSeqlens);
+}
+
+// ---- forward ----
 struct FwdArgs {
   const void *x, *ig, *rg;
   const float *lam, *h0;
@@ -386,37 +490,16 @@ struct FwdArgs {
   Consts consts;
 };
 
-// One CTA (or cluster of CTAs) owns 16 channels of one batch row and walks along
-// its tokens; a lane owns two channels and 16 tokens of its warp's 64 at a time:
-//   1. x and the gates of the run, copied to the warp's tiles a step or two ahead;
-//   2. a_t, u_t into registers, and the run's map (A, H);
-//   3. the maps are exchanged: between warps through shared memory, between the
-//      CTAs of a cluster through distributed shared memory;
-//   4. the state before the run, from the maps before it and the carried state;
-//   5. the run again, token by token from that state, and the stores.
-// Step 5 repeats the sequential recurrence itself, so y differs from it by the
-// rounding of the state a run starts with only.  x and the gates are read once
-// and y is written once.
-#ifndef GLR_FILL
-#define GLR_FILL 2
-#endif
-#ifndef GLR_MINB
-#define GLR_MINB 2
-#endif
-#ifndef GLR_STAGES
-#define GLR_STAGES 2
-#endif
-
 // Decays and inputs of a lane's run.
-template <bool kAllNear, typename T>
+template <typename G, bool kAllNear, typename T>
 __device__ __forceinline__ void fwd_run(const T* mine, float2 k, const Consts& c, float2* a,
                                         float2* u) {
   using P = Pair<T>;
   using Word = typename P::Word;
 #pragma unroll
-  for (int j = 0; j < kRun; ++j) {
-    const Word* w = reinterpret_cast<const Word*>(mine + j * kChans);
-    const float2 si = sigmoid2(P::get(w[kTile / 2]), c), sr = sigmoid2(P::get(w[kTile]), c);
+  for (int j = 0; j < G::kRun; ++j) {
+    const Word* w = reinterpret_cast<const Word*>(mine + j * G::kChans);
+    const float2 si = sigmoid2(P::get(w[G::kTile / 2]), c), sr = sigmoid2(P::get(w[G::kTile]), c);
     float2 m2;
     decay2<kAllNear>(fmul2(sr, k), a[j], m2, c);
     const float2 m = make_float2(sqrt_approx_f(m2.x), sqrt_approx_f(m2.y));
@@ -424,35 +507,46 @@ __device__ __forceinline__ void fwd_run(const T* mine, float2 k, const Consts& c
   }
 }
 
-template <typename T, int kBytes, bool kPacked, int kStages>
-__global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
+// One CTA (or cluster of CTAs) owns 32 or 16 channels of one batch row and walks along
+// its tokens; a lane owns two channels and 16 tokens of its warp's 32 or 64 at a time:
+//   1. x and the gates of the run, copied to the warp's tiles a step or two ahead;
+//   2. a_t, u_t into registers, and the run's map (A, H);
+//   3. the maps are joined: between groups of lanes by shuffles, between warps through
+//      shared memory, between the CTAs of a cluster through distributed shared memory;
+//   4. so each lane has the state before its run;
+//   5. the run again, token by token from that state, and the stores.
+// Step 5 repeats the sequential recurrence itself, so y differs from it by the
+// rounding of the state a run starts with only.  x and the gates are read once
+// and y is written once.
+template <typename T, typename G, int kBytes, bool kPacked, int kStages>
+__global__ void __launch_bounds__(kMaxWarps * 32, 2)
     glr_fwd_scan(const __grid_constant__ FwdArgs p) {
+  constexpr int kRun = G::kRun, kTile = G::kTile;
   extern __shared__ __align__(16) char dynamic_smem[];
-  __shared__ float4 warp_run[2][kMaxWarps][kPairs];  // (A, H) of two channels
-  __shared__ float4 cta_run[2][kMaxCluster][kPairs];
+  __shared__ Exchange<G> ex;
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
   const int warps = blockDim.x >> 5;
   const uint32_t size = cluster_size(), rank = cluster_rank();
   const int64_t b = blockIdx.y, T_ = p.T, D = p.D;
-  const int group = lane / kPairs, pair = lane % kPairs;
-  const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * kChans, ch = ch0 + 2 * pair;
+  const int group = lane / G::kPairs, pair = lane % G::kPairs;
+  const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * G::kChans, ch = ch0 + 2 * pair;
   const int have = ch + 1 < D ? 2 : (ch < D ? 1 : 0);  // channels of this lane
   T* ring = reinterpret_cast<T*>(dynamic_smem) + warp * (kStages * 3 * kTile);
   const int64_t nseg = (T_ + kSegment - 1) / kSegment;
-  const int64_t stride = static_cast<int64_t>(kWarpRun) * warps * size;  // tokens of a step
+  const int64_t stride = static_cast<int64_t>(G::kWarpRun) * warps * size;  // tokens of a step
 
-  int64_t next = static_cast<int64_t>(rank * warps + warp) * kWarpRun;  // to be copied next
+  int64_t next = static_cast<int64_t>(rank * warps + warp) * G::kWarpRun;  // to be copied next
   const T* xn = static_cast<const T*>(p.x) + b * p.st.xb + ch0 + next * p.st.xt;
   const T* in = static_cast<const T*>(p.ig) + b * p.st.ib + ch0 + next * p.st.it;
   const T* rn = static_cast<const T*>(p.rg) + b * p.st.rb + ch0 + next * p.st.rt;
   auto fetch = [&](int stage) {
     if (next < T_) {
-      const int len = T_ - next < kWarpRun ? static_cast<int>(T_ - next) : kWarpRun;
+      const int len = T_ - next < G::kWarpRun ? static_cast<int>(T_ - next) : G::kWarpRun;
       T* t = ring + stage * (3 * kTile);
-      copy_tile<T, kBytes>(t, xn, p.st.xt, len, D - ch0, lane);
-      copy_tile<T, kBytes>(t + kTile, in, p.st.it, len, D - ch0, lane);
-      copy_tile<T, kBytes>(t + 2 * kTile, rn, p.st.rt, len, D - ch0, lane);
+      copy_tile<G, kBytes>(t, xn, p.st.xt, len, D - ch0, lane);
+      copy_tile<G, kBytes>(t + kTile, in, p.st.it, len, D - ch0, lane);
+      copy_tile<G, kBytes>(t + 2 * kTile, rn, p.st.rt, len, D - ch0, lane);
       xn += stride * p.st.xt;
       in += stride * p.st.it;
       rn += stride * p.st.rt;
@@ -464,17 +558,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
   for (int s = 0; s < kStages; ++s) fetch(s);
 
   if (kPacked) {
-    // Sequences without a token end where they began; the offsets are checked once.
-    for (int64_t n = (rank * warps + warp) * kGroups + group; n < p.N;
-         n += size * warps * kGroups)
+    // Sequences without a token end where they began.
+    for (int64_t n = (rank * warps + warp) * G::kGroups + group; n < p.N;
+         n += size * warps * G::kGroups)
       if (p.cu[n + 1] <= p.cu[n])
         store_state(p.hT + n * D + ch, load_state(p.h0 ? p.h0 + n * D + ch : nullptr, have), have);
-    if (blockIdx.x == 0 && warp == 0) {
-      bool bad = false;
-      for (int n = lane; n < p.N; n += 32) bad |= p.cu[n + 1] < p.cu[n];
-      bad |= p.cu[0] != 0 || p.cu[p.N] != T_;
-      if (bad) report_device_error(p.err, kErrBadSeqlens);
-    }
+    if (blockIdx.x == 0 && warp == 0) check_seqlens(p.cu, p.N, T_, lane, p.err);
   }
 
   const float2 lam = load_state(p.lam + ch, have);
@@ -484,35 +573,26 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
   const bool near = __all_sync(~0u, k.x < kNear && k.y < kNear);
   float2 carry = both(0.0f);
   if (!kPacked) carry = load_state(p.h0 ? p.h0 + b * D + ch : nullptr, have);
-  // Maps of warps and CTAs that do not exist stay the identity.
-  const float4 identity = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
-  for (int w = warp; w < kMaxWarps; w += warps)
-    warp_run[0][w][pair] = warp_run[1][w][pair] = identity;
-  for (int r = warp; r < kMaxCluster; r += warps)
-    cta_run[0][r][pair] = cta_run[1][r][pair] = identity;
-  __syncthreads();
-  if (size > 1) cluster_sync();  // every CTA got here before another writes its maps
+  ex.init(warp, warps, size, pair);
 
   int par = 0, stage = 0;
   for (int64_t base = 0; base < T_; base += stride, par ^= 1) {
-    const int64_t w0 = base + static_cast<int64_t>(rank * warps + warp) * kWarpRun;
+    const int64_t w0 = base + static_cast<int64_t>(rank * warps + warp) * G::kWarpRun;
     const int64_t t0 = w0 + group * kRun;
     const int64_t left = T_ - t0;
     const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
-    // Bit j: token t0 + j starts a sequence (one bit more than the run has
-    // tokens, for the end of its last one).
     uint32_t starts = 0;
-    if (kPacked && w0 < T_) starts = start_bits(p.cu, p.N, w0, group, lane);
+    if (kPacked && w0 < T_) starts = start_bits<G>(p.cu, p.N, w0, group, lane);
 
     float2 a[kRun], u[kRun];
     copies_wait<kStages - 1>();
     __syncwarp();  // the tiles of this step have landed, whichever lane copied them
-    const T* mine = ring + stage * (3 * kTile) + tile_row(group * kRun) + 2 * pair;
+    const T* mine = ring + stage * (3 * kTile) + G::tile_row(group * kRun) + 2 * pair;
     if (w0 < T_) {
       if (near)
-        fwd_run<true>(mine, k, p.consts, a, u);
+        fwd_run<G, true>(mine, k, p.consts, a, u);
       else
-        fwd_run<false>(mine, k, p.consts, a, u);
+        fwd_run<G, false>(mine, k, p.consts, a, u);
     }
     __syncwarp();  // read by every lane before they are overwritten
     fetch(stage);
@@ -532,62 +612,15 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
     Run run = {a[0], u[0]};
 #pragma unroll
     for (int j = 1; j < kRun; ++j) run = join<kPacked>(run, Run{a[j], u[j]});
-    // Joined along the lane groups: `run` ends with this group's, `before` with the last one's.
-#pragma unroll
-    for (int off = kPairs; off < 32; off *= 2) {
-      const Run earlier = shuffle_up(run, off);
-      if (lane >= off) run = join<kPacked>(earlier, run);
-    }
-    const Run before = shuffle_up(run, kPairs);
-    const bool last = group == kGroups - 1;  // its `run` is the whole warp's
-
-    float2 h = carry;
-    if (size > 1) {
-      if (last) warp_run[par][warp][pair] = run.word();
-      __syncthreads();
-      // The CTA's map, to every CTA of the cluster (warp w writes to CTA w, w + warps, ...).
-      Run all(warp_run[par][0][pair]);
-#pragma unroll
-      for (int w = 1; w < kMaxWarps; ++w)
-        all = join<kPacked>(all, Run(warp_run[par][w][pair]));
-      if (last)
-        for (uint32_t r = warp; r < size; r += warps)
-          st_cluster(&cta_run[par][rank][pair], r, all.word());
-      __syncwarp();
-      cluster_sync();
-#pragma unroll
-      for (uint32_t r = 0; r < kMaxCluster; ++r) {
-        if (r == rank) h = carry;
-        carry = apply<kPacked>(Run(cta_run[par][r][pair]), carry);
-      }
-#pragma unroll
-      for (int w = 0; w < kMaxWarps - 1; ++w)
-        if (w < warp) h = apply<kPacked>(Run(warp_run[par][w][pair]), h);
-    } else {
-      // A chain from warp to warp: the state goes on as soon as it is known, and
-      // each warp waits for its predecessor alone.
-      float4* link = warp_run[0][0];  // [warp][pair]: the state before a warp's run
-      if (base > 0 || warp > 0) {
-        if (warps > 1) link_wait(warp == 0 ? warps - 1 : warp - 1);
-        else __syncwarp();
-        const float4 v = link[warp * kPairs + pair];
-        h = make_float2(v.x, v.y);
-      }
-      if (warp + 1 < warps || base + stride < T_) {
-        const int to = warp + 1 == warps ? 0 : warp + 1;
-        const float2 out = apply<kPacked>(run, h);
-        if (warps == 1) __syncwarp();  // read above before it is overwritten
-        if (last) link[to * kPairs + pair] = make_float4(out.x, out.y, 0.0f, 0.0f);
-        __syncwarp();
-        if (warps > 1) link_pass(warp);
-      }
-    }
-    if (group > 0) h = apply<kPacked>(before, h);
+    const Run earlier = scan_groups<G, kPacked, false>(run, lane);
+    float2 h = ex.template before<kPacked>(run, group == G::kGroups - 1, carry, par, base == 0,
+                                           base + stride < T_, warp, warps, size, rank, pair);
+    if (group > 0) h = apply<kPacked>(earlier, h);
 
     if (p.states && len > 0 && t0 % kSegment == 0)
       store_state(p.states + (b * nseg + t0 / kSegment) * D + ch, h, have);
     T* yp = static_cast<T*>(p.y) + (b * T_ + t0) * D + ch;
-    if (!kPacked && kBytes == 16 && len == kRun && ch0 + kChans <= D) {
+    if (!kPacked && kBytes == 16 && len == kRun && ch0 + G::kChans <= D) {
 #pragma unroll
       for (int j = 0; j < kRun; ++j, yp += D) {
         h = apply<kPacked>(Run{a[j], u[j]}, h);
@@ -609,29 +642,277 @@ __global__ void __launch_bounds__(kMaxWarps * 32, GLR_MINB)
   copies_wait<0>();
 }
 
-// The tokens' split over warps and CTAs: a run a warp, up to kMaxWarps; then
-// clusters of 2, 4 or 8 CTAs along the tokens while the channels and batch rows
-// alone give fewer than three CTAs an SM.
+// ---- backward ----
+struct BwdArgs {
+  const void *dy, *x, *ig, *rg;
+  const float *lam, *states, *h0, *dhT;
+  const int32_t* cu;
+  void *dx, *di, *dr;
+  float *part, *dh0;
+  int64_t T, D;
+  Strides st;
+  int N;
+  float c;
+  int* err;
+  Consts consts;
+};
+
+__device__ __forceinline__ float2 rsqrt2_or_0(float2 v) {
+  float2 r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+  // 1 / m enters with factors that go to zero faster than m does.
+  return make_float2(v.x > 0.0f ? r.x : 0.0f, v.y > 0.0f ? r.y : 0.0f);
+}
+
+// Gates of a lane's run and u_t = m sigma_i x.
+template <typename G, bool kAllNear, typename T>
+__device__ __forceinline__ void bwd_gates(const T* mine, float2 k, const Consts& c, float2* a,
+                                          float2* u, float2* si, float2* sr) {
+  using P = Pair<T>;
+  using Word = typename P::Word;
+#pragma unroll
+  for (int j = 0; j < G::kRun; ++j) {
+    const Word* w = reinterpret_cast<const Word*>(mine + j * G::kChans);
+    si[j] = sigmoid2(P::get(w[G::kTile / 2]), c);
+    sr[j] = sigmoid2(P::get(w[G::kTile]), c);
+    float2 m2;
+    decay2<kAllNear>(fmul2(sr[j], k), a[j], m2, c);
+    u[j] = fmul2(fmul2(fmul2(m2, rsqrt2_or_0(m2)), si[j]), P::get(w[0]));
+  }
+}
+
+// The gradients of one token, from G = dL/dh_t; hp is the state before it.
+struct TokenGrads {
+  float2 dx, di, dr, dk, back;  // dk = -d log a / d k's factor; back = a G
+};
+template <bool kAllNear>
+__device__ __forceinline__ TokenGrads token_grads(float2 g, float2 hp, float2 x, float2 a,
+                                                  float2 si, float2 sr, float2 k,
+                                                  const Consts& c) {
+  float2 a2, m2;
+  decay2<kAllNear>(fmul2(sr, k), a2, m2, c);
+  const float2 rm = rsqrt2_or_0(m2);
+  TokenGrads o;
+  const float2 sx = fmul2(si, x);                       // sigma_i x
+  o.dx = fmul2(g, fmul2(fmul2(m2, rm), si));
+  o.di = fmul2(fmul2(o.dx, x), fsub2(c.one, si));
+  o.back = fmul2(a, g);
+  const float2 dla = fmul2(o.back, fsub2(hp, fmul2(fmul2(a, sx), rm)));
+  o.dk = fmul2(sr, dla);
+  o.dr = fmul2(fmul2(o.dk, k), fsub2(sr, c.one));
+  return o;
+}
+
+// The forward kernel's walk from the last token to the first.  What is carried is
+// c_t = a_t G_t, the gradient of the state before token t: G_t = dy_t + c_{t+1}, so a run
+// of tokens is again a map c -> A c + H, with the decays' product and
+// H = a_t (dy_t + H).  The states h are walked anew from the forward's saved ones, one a
+// warp's run.  A lane takes 8 tokens: decay, state and both sigmoids of each stay in
+// registers, so no element's gates are computed twice but for m.
+template <typename T, typename G, int kBytes, bool kPacked, int kStages>
+__global__ void __launch_bounds__(kMaxWarps * 32, 2)
+    glr_bwd_scan(const __grid_constant__ BwdArgs p) {
+  constexpr int kRun = G::kRun, kTile = G::kTile;
+  static_assert(G::kWarpRun == kSegment, "a saved state for every run of a warp");
+  using P = Pair<T>;
+  using Word = typename P::Word;
+  extern __shared__ __align__(16) char dynamic_smem[];
+  __shared__ Exchange<G> ex;
+  const int lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
+  const int warps = blockDim.x >> 5;
+  const uint32_t size = cluster_size(), rank = cluster_rank();
+  const int64_t b = blockIdx.y, T_ = p.T, D = p.D;
+  const int group = lane / G::kPairs, pair = lane % G::kPairs;
+  const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * G::kChans, ch = ch0 + 2 * pair;
+  const int have = ch + 1 < D ? 2 : (ch < D ? 1 : 0);  // channels of this lane
+  T* ring = reinterpret_cast<T*>(dynamic_smem) + warp * (kStages * 4 * kTile);
+  const int64_t runs = (T_ + G::kWarpRun - 1) / G::kWarpRun;
+  const int64_t stride = static_cast<int64_t>(warps) * size;  // runs of a step
+
+  // Runs are counted from the last one, q = 0; run q begins at token (runs - 1 - q) kWarpRun.
+  int64_t next = rank * warps + warp;  // to be copied next
+  auto fetch = [&](int stage) {
+    if (next < runs) {
+      const int64_t t = (runs - 1 - next) * G::kWarpRun;
+      const int len = T_ - t < G::kWarpRun ? static_cast<int>(T_ - t) : G::kWarpRun;
+      T* to = ring + stage * (4 * kTile);
+      copy_tile<G, kBytes>(to, static_cast<const T*>(p.x) + b * p.st.xb + t * p.st.xt + ch0,
+                           p.st.xt, len, D - ch0, lane);
+      copy_tile<G, kBytes>(to + kTile, static_cast<const T*>(p.ig) + b * p.st.ib + t * p.st.it + ch0,
+                           p.st.it, len, D - ch0, lane);
+      copy_tile<G, kBytes>(to + 2 * kTile,
+                           static_cast<const T*>(p.rg) + b * p.st.rb + t * p.st.rt + ch0, p.st.rt,
+                           len, D - ch0, lane);
+      copy_tile<G, kBytes>(to + 3 * kTile,
+                           static_cast<const T*>(p.dy) + b * p.st.gb + t * p.st.gt + ch0, p.st.gt,
+                           len, D - ch0, lane);
+      next += stride;
+    }
+    copies_commit();  // a group a step, empty past the end
+  };
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) fetch(s);
+
+  if (kPacked) {
+    // The gradient of an empty sequence's state passes through.
+    for (int64_t n = (rank * warps + warp) * G::kGroups + group; n < p.N;
+         n += size * warps * G::kGroups)
+      if (p.cu[n + 1] <= p.cu[n])
+        store_state(p.dh0 + n * D + ch, load_state(p.dhT ? p.dhT + n * D + ch : nullptr, have),
+                    have);
+    if (blockIdx.x == 0 && warp == 0) check_seqlens(p.cu, p.N, T_, lane, p.err);
+  }
+
+  const float2 lam = load_state(p.lam + ch, have);
+  const float2 k = make_float2(have > 0 ? decay_rate(lam.x, p.c) : 0.0f,
+                               have > 1 ? decay_rate(lam.y, p.c) : 0.0f);
+  const bool near = __all_sync(~0u, k.x < kNear && k.y < kNear);
+  float2 carry = both(0.0f), dk = both(0.0f);
+  if (!kPacked) carry = load_state(p.dhT ? p.dhT + b * D + ch : nullptr, have);
+  ex.init(warp, warps, size, pair);
+
+  int par = 0, stage = 0;
+  for (int64_t base = 0; base < runs; base += stride, par ^= 1) {
+    const int64_t q = base + rank * warps + warp;
+    const bool mine_exists = q < runs;
+    const int64_t w0 = mine_exists ? (runs - 1 - q) * G::kWarpRun : 0;
+    const int64_t t0 = w0 + group * kRun;
+    const int64_t left = mine_exists ? T_ - t0 : 0;
+    const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
+    float2 state = both(0.0f);
+    uint32_t starts = 0;
+    if (mine_exists) {
+      state = load_state(p.states + (b * runs + w0 / kSegment) * D + ch, have);
+      if (kPacked) starts = start_bits<G>(p.cu, p.N, w0, group, lane);
+    }
+    // Token j ends its sequence / begins it.
+    auto ends = [&](int j) {
+      return kPacked && j < len && ((starts >> (j + 1) & 1) || t0 + j + 1 == T_);
+    };
+    auto begins = [&](int j) { return kPacked && j < len && (starts >> j & 1); };
+    auto of_seq = [&](const float* v, int j) {  // v of token j's sequence
+      return load_state(v ? v + seq_of(p.cu, p.N, t0 + j) * D + ch : nullptr, have);
+    };
+
+    float2 a[kRun], hp[kRun], si[kRun], sr[kRun];
+    copies_wait<kStages - 1>();
+    __syncwarp();  // the tiles of this step have landed, whichever lane copied them
+    const T* mine = ring + stage * (4 * kTile) + G::tile_row(group * kRun) + 2 * pair;
+    if (mine_exists) {
+      if (near)
+        bwd_gates<G, true>(mine, k, p.consts, a, hp, si, sr);
+      else
+        bwd_gates<G, false>(mine, k, p.consts, a, hp, si, sr);
+    }
+    if (len < kRun)
+#pragma unroll
+      for (int j = 0; j < kRun; ++j)
+        if (j >= len) a[j] = both(1.0f), hp[j] = si[j] = sr[j] = both(0.0f);  // the identity
+    auto word = [&](int tensor, int j) {
+      return P::get(*reinterpret_cast<const Word*>(mine + tensor * kTile + j * G::kChans));
+    };
+    auto dy_at = [&](int j) { return j < len ? word(3, j) : both(0.0f); };
+
+    // Maps of the run: of the states (forwards) and of what is carried (backwards).
+    Run fwd(both(1.0f), both(0.0f)), bwd(both(1.0f), both(0.0f));
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      if (begins(j)) fwd = Run(both(kForget), of_seq(p.h0, j));
+      fwd = join<kPacked>(fwd, Run(a[j], hp[j]));
+    }
+#pragma unroll
+    for (int j = kRun - 1; j >= 0; --j) {
+      if (ends(j)) bwd = Run(both(kForget), of_seq(p.dhT, j));
+      bwd = join<kPacked>(bwd, Run(a[j], fmul2(a[j], dy_at(j))));
+    }
+    const Run earlier = scan_groups<G, kPacked, false>(fwd, lane);
+    const Run later = scan_groups<G, kPacked, true>(bwd, lane);
+    float2 cr = ex.template before<kPacked>(bwd, group == 0, carry, par, base == 0,
+                                            base + stride < runs, warp, warps, size, rank, pair);
+    if (group < G::kGroups - 1) cr = apply<kPacked>(later, cr);
+    float2 h = group > 0 ? apply<kPacked>(earlier, state) : state;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      if (begins(j)) h = of_seq(p.h0, j);
+      const float2 u = hp[j];
+      hp[j] = h;
+      h = ffma2(a[j], h, u);
+    }
+
+    const int64_t row0 = (b * T_ + t0) * D + ch;
+    T *dxp = static_cast<T*>(p.dx) + row0, *dip = static_cast<T*>(p.di) + row0,
+      *drp = static_cast<T*>(p.dr) + row0;
+#pragma unroll
+    for (int j = kRun - 1; j >= 0; --j) {
+      if (ends(j)) cr = of_seq(p.dhT, j);
+      if (j < len) {
+        const float2 x = word(0, j), g = fadd2(word(3, j), cr);
+        const TokenGrads o = near ? token_grads<true>(g, hp[j], x, a[j], si[j], sr[j], k, p.consts)
+                                  : token_grads<false>(g, hp[j], x, a[j], si[j], sr[j], k, p.consts);
+        store_pair<T, kBytes>(dxp + j * D, o.dx, have);
+        store_pair<T, kBytes>(dip + j * D, o.di, have);
+        store_pair<T, kBytes>(drp + j * D, o.dr, have);
+        dk = fadd2(dk, o.dk);
+        cr = o.back;
+        if (begins(j)) {
+          const int64_t n = seq_of(p.cu, p.N, t0 + j);
+          store_state(p.dh0 + n * D + ch, cr, have);
+        }
+      }
+    }
+    if (!kPacked && mine_exists && t0 == 0) store_state(p.dh0 + b * D + ch, cr, have);
+    __syncwarp();  // read by every lane before they are overwritten
+    fetch(stage);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  copies_wait<0>();
+
+  // d k of the CTA's tokens: lane groups, then warps, in a fixed order.
+#pragma unroll
+  for (int off = G::kPairs; off < 32; off *= 2) {
+    dk.x += __shfl_xor_sync(~0u, dk.x, off);
+    dk.y += __shfl_xor_sync(~0u, dk.y, off);
+  }
+  __syncthreads();  // the maps have been read
+  if (group == 0) ex.warp_run[0][warp][pair] = make_float4(dk.x, dk.y, 0.0f, 0.0f);
+  __syncthreads();
+  if (warp == 0 && group == 0) {
+    float2 sum = both(0.0f);
+    for (int w = 0; w < warps; ++w) {
+      sum.x += ex.warp_run[0][w][pair].x;
+      sum.y += ex.warp_run[0][w][pair].y;
+    }
+    store_state(p.part + (b * size + rank) * D + ch, sum, have);
+  }
+}
+
+// ---- launches ----
+// The tokens' split over warps and CTAs: a run a warp, up to kMaxWarps; then clusters of
+// 2, 4 or 8 CTAs along the tokens while the channels and batch rows alone give fewer
+// CTAs than there are SMs.
 struct ScanGrid {
   int warps, cluster;
   int64_t blocks;
 };
 
-inline ScanGrid scan_grid(int64_t batch, int64_t seq_len, int64_t dim, int run) {
+template <typename G>
+ScanGrid scan_grid(int64_t batch, int64_t seq_len, int64_t dim) {
   ScanGrid g;
-  g.blocks = (dim + kChans - 1) / kChans;
-  const int64_t runs = (seq_len + run - 1) / run;
+  g.blocks = (dim + G::kChans - 1) / G::kChans;
+  const int64_t runs = (seq_len + G::kWarpRun - 1) / G::kWarpRun;
   g.warps = static_cast<int>(std::min<int64_t>(runs, kMaxWarps));
   g.cluster = 1;
-  while (g.cluster < kMaxCluster && g.blocks * batch * g.cluster < GLR_FILL * sm_count() &&
+  while (g.cluster < kMaxCluster && g.blocks * batch * g.cluster < GLR_FILL * sm_count() / 2 &&
          g.cluster * g.warps < runs)
     g.cluster *= 2;
   return g;
 }
 
 template <typename A>
-int launch_scan(void (*kernel)(const A), const ScanGrid& g, int64_t batch, size_t smem, const A& args,
-                cudaStream_t s) {
+int launch_scan(void (*kernel)(const A), const ScanGrid& g, int64_t batch, size_t smem,
+                const A& args, cudaStream_t s) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return TILEOPS_ELAUNCH;
@@ -663,83 +944,63 @@ inline int copy_bytes(const void* p, int64_t sb, int64_t st, int64_t itemsize) {
   return 2;
 }
 
+template <typename T, typename G, int kBytes, int kStages>
+int launch_fwd_geo(const FwdArgs& a, int64_t batch, cudaStream_t s) {
+  const ScanGrid g = scan_grid<G>(batch, a.T, a.D);
+  const size_t smem = static_cast<size_t>(g.warps) * kStages * 3 * G::kTile * sizeof(T);
+  return launch_scan(a.cu ? glr_fwd_scan<T, G, kBytes, true, kStages>
+                          : glr_fwd_scan<T, G, kBytes, false, kStages>,
+                     g, batch, smem, a, s);
+}
+
 template <typename T>
 int launch_fwd(const FwdArgs& a, int64_t batch, cudaStream_t s) {
-  constexpr int kStages = sizeof(T) == 2 ? GLR_STAGES : GLR_STAGES / 2;  // about 100 KB of tiles: two CTAs an SM
+  constexpr int kStages = sizeof(T) == 2 ? 2 : 1;  // about 100 KB of tiles: two CTAs an SM
   constexpr int64_t eb = sizeof(T);
+  using Wide = Geo<32, 16>;
+  using Narrow = Geo<16, 16>;
   const int bytes = std::min({copy_bytes(a.x, a.st.xb, a.st.xt, eb),
                               copy_bytes(a.ig, a.st.ib, a.st.it, eb),
                               copy_bytes(a.rg, a.st.rb, a.st.rt, eb),
                               copy_bytes(a.y, a.D, a.D, eb)});
-  const ScanGrid g = scan_grid(batch, a.T, a.D, kWarpRun);
-  const size_t smem = static_cast<size_t>(g.warps) * kStages * 3 * kTile * sizeof(T);
-  auto go = [&](auto packed, auto plain) {
-    return launch_scan(a.cu ? packed : plain, g, batch, smem, a, s);
-  };
+  // Sixteen channels a CTA cost more copies and shuffles an element (8 x 4096 x 4096 bf16:
+  // 266 us against 233 us), but make twice the CTAs: 1 x 16384 x 4096 149 us against 159 us.
+  const bool few = (a.D + 31) / 32 * batch < 2 * sm_count();
   if (bytes == 16)
-    return go(glr_fwd_scan<T, 16, true, kStages>, glr_fwd_scan<T, 16, false, kStages>);
+    return few ? launch_fwd_geo<T, Narrow, 16, kStages>(a, batch, s)
+               : launch_fwd_geo<T, Wide, 16, kStages>(a, batch, s);
   if constexpr (sizeof(T) == 2) {
-    if (bytes == 2)
-      return go(glr_fwd_scan<T, 2, true, kStages>, glr_fwd_scan<T, 2, false, kStages>);
+    if (bytes == 2) return launch_fwd_geo<T, Wide, 2, kStages>(a, batch, s);
   }
-  return go(glr_fwd_scan<T, 4, true, kStages>, glr_fwd_scan<T, 4, false, kStages>);
+  return launch_fwd_geo<T, Narrow, 4, kStages>(a, batch, s);
+}
+
+using BwdGeo = Geo<16, 8>;
+
+template <typename T, int kBytes>
+int launch_bwd_bytes(const BwdArgs& a, int64_t batch, cudaStream_t s) {
+  constexpr int kStages = sizeof(T) == 2 ? GLR_BSTAGES : GLR_BSTAGES / 2;
+  const ScanGrid g = scan_grid<BwdGeo>(batch, a.T, a.D);
+  const size_t smem = static_cast<size_t>(g.warps) * kStages * 4 * BwdGeo::kTile * sizeof(T);
+  return launch_scan(a.cu ? glr_bwd_scan<T, BwdGeo, kBytes, true, kStages>
+                          : glr_bwd_scan<T, BwdGeo, kBytes, false, kStages>,
+                     g, batch, smem, a, s);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(128)
-    glr_bwd_simple(const T* dy, const T* x, const T* ig, const T* rg, const float* lam,
-                   const float* states, const float* h0, const float* dhT, const int32_t* cu, int N,
-                   T* dx, T* di, T* dr, float* part, float* dh0, int64_t T_, int64_t D, Strides st,
-                   float c) {
-  const int64_t d = blockIdx.x * 128ll + threadIdx.x, b = blockIdx.y;
-  if (d >= D) return;
-  const float k = decay_rate(lam[d], c);
-  const int64_t nseg = (T_ + kSegment - 1) / kSegment;
-  if (cu)
-    for (int n = 0; n < N; ++n)
-      if (cu[n + 1] <= cu[n]) dh0[n * D + d] = dhT ? dhT[n * D + d] : 0.0f;
-  float back = cu ? 0.0f : (dhT ? dhT[b * D + d] : 0.0f), dk = 0.0f;
-  for (int64_t seg = nseg - 1; seg >= 0; --seg) {
-    float hp[kSegment];
-    float h = states[(b * nseg + seg) * D + d];
-    const int64_t t0 = seg * kSegment;
-    const int len = static_cast<int>(T_ - t0 < kSegment ? T_ - t0 : kSegment);
-    for (int j = 0; j < len; ++j) {
-      const int64_t t = t0 + j;
-      if (cu) {
-        const int n = seq_of(cu, N, t);
-        if (cu[n] == t) h = h0 ? h0[n * D + d] : 0.0f;
-      }
-      hp[j] = h;
-      const Gates g = gates_of(Cvt<T>::to_f(ig[b * st.ib + t * st.it + d]),
-                               Cvt<T>::to_f(rg[b * st.rb + t * st.rt + d]), k);
-      h = fmaf(g.a, h, sqrtf(g.m2) * g.si * Cvt<T>::to_f(x[b * st.xb + t * st.xt + d]));
-    }
-    for (int j = len - 1; j >= 0; --j) {
-      const int64_t t = t0 + j;
-      int n = 0;
-      if (cu) {
-        n = seq_of(cu, N, t);
-        if (cu[n + 1] == t + 1) back = dhT ? dhT[n * D + d] : 0.0f;
-      }
-      const Gates g = gates_of(Cvt<T>::to_f(ig[b * st.ib + t * st.it + d]),
-                               Cvt<T>::to_f(rg[b * st.rb + t * st.rt + d]), k);
-      const float xv = Cvt<T>::to_f(x[b * st.xb + t * st.xt + d]);
-      const float G = Cvt<T>::to_f(dy[b * st.gb + t * st.gt + d]) + back;
-      const float m = sqrtf(g.m2), over_m = g.m2 > 0.0f ? 1.0f / m : 0.0f * g.m2;
-      const float gx = G * m * g.si;
-      const float dla = g.a * G * (hp[j] - g.a * g.si * xv * over_m);
-      const int64_t o = (b * T_ + t) * D + d;
-      dx[o] = Cvt<T>::from_f(gx);
-      di[o] = Cvt<T>::from_f(gx * xv * (1.0f - g.si));
-      dr[o] = Cvt<T>::from_f(-k * g.sr * (1.0f - g.sr) * dla);
-      dk = fmaf(-g.sr, dla, dk);
-      back = g.a * G;
-      if (cu && cu[n] == t) dh0[n * D + d] = back;
-    }
+int launch_bwd(const BwdArgs& a, int64_t batch, cudaStream_t s) {
+  constexpr int64_t eb = sizeof(T);
+  const int bytes = std::min({copy_bytes(a.dy, a.st.gb, a.st.gt, eb),
+                              copy_bytes(a.x, a.st.xb, a.st.xt, eb),
+                              copy_bytes(a.ig, a.st.ib, a.st.it, eb),
+                              copy_bytes(a.rg, a.st.rb, a.st.rt, eb),
+                              copy_bytes(a.dx, a.D, a.D, eb), copy_bytes(a.di, a.D, a.D, eb),
+                              copy_bytes(a.dr, a.D, a.D, eb)});
+  if (bytes == 16) return launch_bwd_bytes<T, 16>(a, batch, s);
+  if constexpr (sizeof(T) == 2) {
+    if (bytes == 2) return launch_bwd_bytes<T, 2>(a, batch, s);
   }
-  if (!cu) dh0[b * D + d] = back;
-  part[b * D + d] = dk;
+  return launch_bwd_bytes<T, 4>(a, batch, s);
 }
 
 // dlambda = c sigmoid(lambda) sum of the partial sums, added in a fixed order.
@@ -749,15 +1010,7 @@ __global__ void __launch_bounds__(128)
   if (d >= D) return;
   float s = 0.0f;
   for (int64_t p = 0; p < parts; ++p) s += part[p * D + d];
-  dlam[d] = s * c / (1.0f + expf(-lam[d]));
-}
-
-// cu_seqlens must be 0 = cu[0] <= ... <= cu[N] = total; reported otherwise.
-__global__ void glr_check_seqlens(const int32_t* cu, int N, int64_t total, int* err) {
-  bool bad = false;
-  for (int n = threadIdx.x; n < N; n += blockDim.x) bad |= cu[n + 1] < cu[n];
-  if (threadIdx.x == 0) bad |= cu[0] != 0 || cu[N] != total;
-  if (bad) report_device_error(err, kErrBadSeqlens);
+  dlam[d] = -s * c / (1.0f + expf(-lam[d]));
 }
 
 template <typename T>
@@ -772,8 +1025,6 @@ __global__ void __launch_bounds__(128)
   y[b * D + d] = Cvt<T>::from_f(h);
   hn[b * D + d] = h;
 }
-
-int64_t bwd_parts(int64_t batch, int64_t, int64_t) { return batch; }
 
 // Sizes every kernel here indexes with: batch in a grid's y, 64-bit element offsets.
 bool bad_shape(int64_t batch, int64_t seq_len, int64_t dim) {
@@ -815,7 +1066,7 @@ extern "C" int tileops_glr_fwd(const void* x, const void* input_gate, const void
 
 extern "C" int64_t tileops_glr_bwd_workspace_bytes(int64_t batch, int64_t seq_len, int64_t dim) {
   if (bad_shape(batch, seq_len, dim)) return -1;
-  return bwd_parts(batch, seq_len, dim) * dim * 4;
+  return batch * kMaxCluster * dim * 4;  // a partial sum a CTA along the tokens
 }
 
 extern "C" int tileops_glr_bwd(const void* dy, const void* x, const void* input_gate,
@@ -840,28 +1091,23 @@ extern "C" int tileops_glr_bwd(const void* dy, const void* x, const void* input_
   cudaStream_t s = as_stream(stream);
   const Strides st{x_stride_b, x_stride_t, i_stride_b, i_stride_t,
                    r_stride_b, r_stride_t, g_stride_b, g_stride_t};
-  const unsigned gx = static_cast<unsigned>((dim + 127) / 128);
-  const dim3 grid(gx, static_cast<unsigned>(batch));
-  const int N = static_cast<int>(num_seqs);
   const float c = static_cast<float>(decay_scale);
   float* part = static_cast<float*>(workspace);
-  if (cu_seqlens) glr_check_seqlens<<<1, 128, 0, s>>>(cu_seqlens, N, seq_len, device_error_ptr());
-  auto go = [&](auto zero) {
-    using T = decltype(zero);
-    glr_bwd_simple<T><<<grid, 128, 0, s>>>(
-        static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const T*>(input_gate),
-        static_cast<const T*>(decay_gate), decay_param, states, initial_state, d_final_state,
-        cu_seqlens, N, static_cast<T*>(dx), static_cast<T*>(d_input_gate),
-        static_cast<T*>(d_decay_gate), part, d_initial_state, seq_len, dim, st, c);
-    glr_dparam<<<gx, 128, 0, s>>>(part, decay_param, d_decay_param,
-                                  bwd_parts(batch, seq_len, dim), dim, c);
-    return launch_status();
-  };
+  const BwdArgs args{dy, x, input_gate, decay_gate, decay_param, states, initial_state,
+                     d_final_state, cu_seqlens, dx, d_input_gate, d_decay_gate, part,
+                     d_initial_state, seq_len, dim, st, static_cast<int>(num_seqs), c,
+                     cu_seqlens ? device_error_ptr() : nullptr, Consts()};
+  int status;
   switch (dtype) {
-    case TILEOPS_DT_F32: return go(float());
-    case TILEOPS_DT_F16: return go(__half());
-    default: return go(__nv_bfloat16());
+    case TILEOPS_DT_F32: status = launch_bwd<float>(args, batch, s); break;
+    case TILEOPS_DT_F16: status = launch_bwd<__half>(args, batch, s); break;
+    default: status = launch_bwd<__nv_bfloat16>(args, batch, s);
   }
+  if (status != TILEOPS_OK) return status;
+  const int64_t parts = batch * scan_grid<BwdGeo>(batch, seq_len, dim).cluster;
+  glr_dparam<<<static_cast<unsigned>((dim + 127) / 128), 128, 0, s>>>(part, decay_param,
+                                                                      d_decay_param, parts, dim, c);
+  return launch_status();
 }
 
 extern "C" int tileops_glr_decode_fwd(const void* x, const void* input_gate,

@@ -18,7 +18,7 @@ from tileops.kernels.kernel_base import Kernel, check_dtype
 __all__ = ["GatedLinearRecurrenceBwdKernel", "GatedLinearRecurrenceDecodeKernel",
            "GatedLinearRecurrenceFwdKernel"]
 
-SEGMENT = 64  # tokens between two saved states (TILEOPS_GLR_SEGMENT)
+SEGMENT = 32  # tokens between two saved states (TILEOPS_GLR_SEGMENT)
 
 
 def _channels_last(t: torch.Tensor) -> torch.Tensor:

@@ -28,7 +28,7 @@ A decay gate of -inf has a = 1 exactly and takes no input: a padded token.
 x, input_gate, decay_gate, dy are (batch, seq_len, dim) -- (batch, dim) for
 decode -- of ``dtype``; column slices of a wider tensor are read in place.
 decay_param (dim,), the states (batch, dim) and ``states`` (batch,
-ceil(seq_len / 64), dim) are float32.  Packed sequences follow the GDN op:
+ceil(seq_len / 32), dim) are float32.  Packed sequences follow the GDN op:
 batch 1, ``cu_seqlens`` an integer device tensor of N + 1 offsets 0, ...,
 seq_len, one initial and final state per sequence; offsets that break this
 rule set the device error flag to 2.  Like every op here, these build no
@@ -53,7 +53,7 @@ from tileops.ops.op_base import Op
 __all__ = ["GatedLinearRecurrenceBwdOp", "GatedLinearRecurrenceDecodeOp",
            "GatedLinearRecurrenceFwdOp"]
 
-_SEGMENT = 64
+_SEGMENT = 32
 
 
 def _check(device: torch.device, name: str, t: torch.Tensor, shape: tuple,
