@@ -17,6 +17,7 @@
 // predecessor from initial_state by selection, not by a zero factor, so
 // infinities and NaN of one sequence never reach another.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "device_error.cuh"
@@ -350,13 +351,18 @@ __device__ __forceinline__ void store_state(float* p, float2 v, int have) {
 // Which tokens of a lane's run start a sequence: bit j for token t0 + j, j = 0 .. kRun (one
 // more than the run has, for the end of its last token).  Empty sequences start
 // no token.  w0: the first token of the warp's run, the same in every lane.
+// lo, hi: the bounds of the sequence that the last search found; a run strictly
+// inside them needs no search.
 template <typename G>
 __device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t w0, int group,
-                                               int lane) {
-  const int n0 = seq_of(cu, N, w0);
-  uint64_t bits = cu[n0] == w0 ? 1 : 0;
-  uint32_t beyond = 0;  // token w0 + 64
+                                               int lane, int64_t& lo, int64_t& hi) {
   static_assert(G::kWarpRun <= 64, "bits of a warp's run");
+  if (lo < w0 && w0 + G::kWarpRun < hi) return 0;
+  const int n0 = seq_of(cu, N, w0);
+  lo = cu[n0];
+  hi = cu[n0 + 1];
+  uint64_t bits = lo == w0 ? 1 : 0;
+  uint32_t beyond = 0;  // token w0 + 64
   for (int n = n0 + 1; n < N; n += 32) {
     const int64_t at = n + lane < N ? cu[n + lane] - w0 : G::kWarpRun + 1;
     const uint64_t mine = at > 0 && at < 64 ? 1ull << at : 0ull;
@@ -575,6 +581,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
   if (!kPacked) carry = load_state(p.h0 ? p.h0 + b * D + ch : nullptr, have);
   ex.init(warp, warps, size, pair);
 
+  int64_t seq_lo = 0, seq_hi = 0;
   int par = 0, stage = 0;
   for (int64_t base = 0; base < T_; base += stride, par ^= 1) {
     const int64_t w0 = base + static_cast<int64_t>(rank * warps + warp) * G::kWarpRun;
@@ -582,7 +589,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     const int64_t left = T_ - t0;
     const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
     uint32_t starts = 0;
-    if (kPacked && w0 < T_) starts = start_bits<G>(p.cu, p.N, w0, group, lane);
+    bool bounds = false;  // a sequence starts or ends in the warp's run
+    if (kPacked && w0 < T_) {
+      starts = start_bits<G>(p.cu, p.N, w0, group, lane, seq_lo, seq_hi);
+      bounds = __any_sync(~0u, starts != 0) || w0 + G::kWarpRun >= T_;
+    }
 
     float2 a[kRun], u[kRun];
     copies_wait<kStages - 1>();
@@ -601,7 +612,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
 #pragma unroll
       for (int j = 0; j < kRun; ++j)
         if (j >= len) a[j] = both(1.0f), u[j] = both(0.0f);  // past the end: the identity
-    if (kPacked && (starts & ((1u << kRun) - 1)))
+    if (kPacked && bounds)
 #pragma unroll
       for (int j = 0; j < kRun; ++j)
         if ((starts >> j & 1) && j < len) {
@@ -610,8 +621,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
           a[j] = both(kForget);
         }
     Run run = {a[0], u[0]};
+    if (kPacked && bounds)
 #pragma unroll
-    for (int j = 1; j < kRun; ++j) run = join<kPacked>(run, Run{a[j], u[j]});
+      for (int j = 1; j < kRun; ++j) run = join<true>(run, Run{a[j], u[j]});
+    else
+#pragma unroll
+      for (int j = 1; j < kRun; ++j) run = join<false>(run, Run{a[j], u[j]});
     const Run earlier = scan_groups<G, kPacked, false>(run, lane);
     float2 h = ex.template before<kPacked>(run, group == G::kGroups - 1, carry, par, base == 0,
                                            base + stride < T_, warp, warps, size, rank, pair);
@@ -620,10 +635,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     if (p.states && len > 0 && t0 % kSegment == 0)
       store_state(p.states + (b * nseg + t0 / kSegment) * D + ch, h, have);
     T* yp = static_cast<T*>(p.y) + (b * T_ + t0) * D + ch;
-    if (!kPacked && kBytes == 16 && len == kRun && ch0 + G::kChans <= D) {
+    if (!bounds && kBytes == 16 && len == kRun && ch0 + G::kChans <= D) {
 #pragma unroll
       for (int j = 0; j < kRun; ++j, yp += D) {
-        h = apply<kPacked>(Run{a[j], u[j]}, h);
+        h = apply<false>(Run{a[j], u[j]}, h);
         store_pair<T, kBytes>(yp, h, 2);
       }
     } else {
@@ -657,12 +672,14 @@ struct BwdArgs {
   Consts consts;
 };
 
-__device__ __forceinline__ float2 rsqrt2_or_0(float2 v) {
+// 1 / sqrt(v), of the least normal number where v is less: finite where m = 0, and it
+// enters with factors (sigma_r and k, or sigmoid(lambda)) that are 0 there.
+__device__ __forceinline__ float2 rsqrt2(float2 v) {
+  constexpr float kLeast = 1.17549435e-38f;
   float2 r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
-  // 1 / m enters with factors that go to zero faster than m does.
-  return make_float2(v.x > 0.0f ? r.x : 0.0f, v.y > 0.0f ? r.y : 0.0f);
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(fmaxf(v.x, kLeast)));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(fmaxf(v.y, kLeast)));
+  return r;
 }
 
 // Gates of a lane's run and u_t = m sigma_i x.
@@ -678,7 +695,7 @@ __device__ __forceinline__ void bwd_gates(const T* mine, float2 k, const Consts&
     sr[j] = sigmoid2(P::get(w[G::kTile]), c);
     float2 m2;
     decay2<kAllNear>(fmul2(sr[j], k), a[j], m2, c);
-    u[j] = fmul2(fmul2(fmul2(m2, rsqrt2_or_0(m2)), si[j]), P::get(w[0]));
+    u[j] = fmul2(fmul2(fmul2(m2, rsqrt2(m2)), si[j]), P::get(w[0]));
   }
 }
 
@@ -692,7 +709,7 @@ __device__ __forceinline__ TokenGrads token_grads(float2 g, float2 hp, float2 x,
                                                   const Consts& c) {
   float2 a2, m2;
   decay2<kAllNear>(fmul2(sr, k), a2, m2, c);
-  const float2 rm = rsqrt2_or_0(m2);
+  const float2 rm = rsqrt2(m2);
   TokenGrads o;
   const float2 sx = fmul2(si, x);                       // sigma_i x
   o.dx = fmul2(g, fmul2(fmul2(m2, rm), si));
@@ -773,6 +790,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
   if (!kPacked) carry = load_state(p.dhT ? p.dhT + b * D + ch : nullptr, have);
   ex.init(warp, warps, size, pair);
 
+  int64_t seq_lo = 0, seq_hi = 0;
   int par = 0, stage = 0;
   for (int64_t base = 0; base < runs; base += stride, par ^= 1) {
     const int64_t q = base + rank * warps + warp;
@@ -782,16 +800,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     const int64_t left = mine_exists ? T_ - t0 : 0;
     const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
     float2 state = both(0.0f);
-    uint32_t starts = 0;
+    uint32_t starts = 0, stops = 0;  // bit j: token j begins its sequence / ends it
+    bool bounds = false;             // one of the warp's tokens does
     if (mine_exists) {
       state = load_state(p.states + (b * runs + w0 / kSegment) * D + ch, have);
-      if (kPacked) starts = start_bits<G>(p.cu, p.N, w0, group, lane);
+      if (kPacked) {
+        starts = start_bits<G>(p.cu, p.N, w0, group, lane, seq_lo, seq_hi);
+        bounds = __any_sync(~0u, starts != 0) || w0 + G::kWarpRun >= T_;
+        if (bounds && len > 0) {
+          stops = starts >> 1 | (t0 + len == T_ ? 1u << (len - 1) : 0u);
+          stops &= (1u << len) - 1;
+          starts &= (1u << len) - 1;
+        }
+      }
     }
-    // Token j ends its sequence / begins it.
-    auto ends = [&](int j) {
-      return kPacked && j < len && ((starts >> (j + 1) & 1) || t0 + j + 1 == T_);
-    };
-    auto begins = [&](int j) { return kPacked && j < len && (starts >> j & 1); };
+    auto begins = [&](int j) { return kPacked && bounds && (starts >> j & 1); };
+    auto ends = [&](int j) { return kPacked && bounds && (stops >> j & 1); };
     auto of_seq = [&](const float* v, int j) {  // v of token j's sequence
       return load_state(v ? v + seq_of(p.cu, p.N, t0 + j) * D + ch : nullptr, have);
     };
@@ -816,16 +840,27 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     auto dy_at = [&](int j) { return j < len ? word(3, j) : both(0.0f); };
 
     // Maps of the run: of the states (forwards) and of what is carried (backwards).
+    // `plain`: nothing begins, ends or is missing in the warp's run, so nothing is asked.
+    const bool plain = mine_exists && !bounds && kBytes == 16 && ch0 + G::kChans <= D &&
+                       w0 + G::kWarpRun <= T_;
     Run fwd(both(1.0f), both(0.0f)), bwd(both(1.0f), both(0.0f));
+    if (plain) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if (begins(j)) fwd = Run(both(kForget), of_seq(p.h0, j));
-      fwd = join<kPacked>(fwd, Run(a[j], hp[j]));
-    }
+      for (int j = 0; j < kRun; ++j) fwd = join<false>(fwd, Run(a[j], hp[j]));
+      bwd.A = fwd.A;
 #pragma unroll
-    for (int j = kRun - 1; j >= 0; --j) {
-      if (ends(j)) bwd = Run(both(kForget), of_seq(p.dhT, j));
-      bwd = join<kPacked>(bwd, Run(a[j], fmul2(a[j], dy_at(j))));
+      for (int j = kRun - 1; j >= 0; --j) bwd.H = fmul2(a[j], fadd2(word(3, j), bwd.H));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (begins(j)) fwd = Run(both(kForget), of_seq(p.h0, j));
+        fwd = join<kPacked>(fwd, Run(a[j], hp[j]));
+      }
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) {
+        if (ends(j)) bwd = Run(both(kForget), of_seq(p.dhT, j));
+        bwd = join<kPacked>(bwd, Run(a[j], fmul2(a[j], dy_at(j))));
+      }
     }
     const Run earlier = scan_groups<G, kPacked, false>(fwd, lane);
     const Run later = scan_groups<G, kPacked, true>(bwd, lane);
@@ -833,35 +868,52 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
                                             base + stride < runs, warp, warps, size, rank, pair);
     if (group < G::kGroups - 1) cr = apply<kPacked>(later, cr);
     float2 h = group > 0 ? apply<kPacked>(earlier, state) : state;
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if (begins(j)) h = of_seq(p.h0, j);
-      const float2 u = hp[j];
-      hp[j] = h;
-      h = ffma2(a[j], h, u);
-    }
-
     const int64_t row0 = (b * T_ + t0) * D + ch;
     T *dxp = static_cast<T*>(p.dx) + row0, *dip = static_cast<T*>(p.di) + row0,
       *drp = static_cast<T*>(p.dr) + row0;
+    // The states before each token, then the tokens' gradients from the last on.
+    auto finish = [&](auto all_near, auto asks) {
 #pragma unroll
-    for (int j = kRun - 1; j >= 0; --j) {
-      if (ends(j)) cr = of_seq(p.dhT, j);
-      if (j < len) {
-        const float2 x = word(0, j), g = fadd2(word(3, j), cr);
-        const TokenGrads o = near ? token_grads<true>(g, hp[j], x, a[j], si[j], sr[j], k, p.consts)
-                                  : token_grads<false>(g, hp[j], x, a[j], si[j], sr[j], k, p.consts);
-        store_pair<T, kBytes>(dxp + j * D, o.dx, have);
-        store_pair<T, kBytes>(dip + j * D, o.di, have);
-        store_pair<T, kBytes>(drp + j * D, o.dr, have);
+      for (int j = 0; j < kRun; ++j) {
+        if (asks.value && begins(j)) h = of_seq(p.h0, j);
+        const float2 u = hp[j];
+        hp[j] = h;
+        h = ffma2(a[j], h, u);
+      }
+      if (!asks.value) {
+        dxp += (kRun - 1) * D;
+        dip += (kRun - 1) * D;
+        drp += (kRun - 1) * D;
+      }
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) {
+        if (asks.value && ends(j)) cr = of_seq(p.dhT, j);
+        if (asks.value && j >= len) continue;
+        const TokenGrads o = token_grads<all_near.value>(
+            fadd2(word(3, j), cr), hp[j], word(0, j), a[j], si[j], sr[j], k, p.consts);
         dk = fadd2(dk, o.dk);
         cr = o.back;
-        if (begins(j)) {
-          const int64_t n = seq_of(p.cu, p.N, t0 + j);
-          store_state(p.dh0 + n * D + ch, cr, have);
+        if (asks.value) {
+          store_pair<T, kBytes>(dxp + j * D, o.dx, have);
+          store_pair<T, kBytes>(dip + j * D, o.di, have);
+          store_pair<T, kBytes>(drp + j * D, o.dr, have);
+          if (begins(j)) store_state(p.dh0 + seq_of(p.cu, p.N, t0 + j) * D + ch, cr, have);
+        } else {
+          store_pair<T, kBytes>(dxp, o.dx, 2);
+          store_pair<T, kBytes>(dip, o.di, 2);
+          store_pair<T, kBytes>(drp, o.dr, 2);
+          dxp -= D;
+          dip -= D;
+          drp -= D;
         }
       }
-    }
+    };
+    if (plain && near)
+      finish(std::true_type(), std::false_type());
+    else if (plain)
+      finish(std::false_type(), std::false_type());
+    else
+      finish(std::false_type(), std::true_type());
     if (!kPacked && mine_exists && t0 == 0) store_state(p.dh0 + b * D + ch, cr, have);
     __syncwarp();  // read by every lane before they are overwritten
     fetch(stage);
