@@ -81,9 +81,22 @@ __device__ __forceinline__ float decay_rate(float lambda, float c) {
 }
 
 // ---- packed sequences ----
-// The sequence token t belongs to: the last n with cu[n] <= t, in [0, N).
-__device__ __forceinline__ int seq_of(const int32_t* cu, int N, int64_t t) {
-  int lo = 0, hi = N;  // cu[lo] <= t (or lo = 0), cu[hi] > t (or hi = N)
+// The sequence token t belongs to, the last n with cu[n] <= t, in [0, N); from a guess
+// nearby: doubling steps away from it, then halves.
+__device__ __forceinline__ int seq_near(const int32_t* cu, int N, int64_t t, int guess) {
+  int lo = guess, hi = guess + 1;
+  if (cu[guess] <= t) {
+    for (int by = 1; hi < N && cu[hi] <= t; by *= 2) {
+      lo = hi;
+      hi = N - hi < by ? N : hi + by;
+    }
+  } else {
+    hi = guess;
+    for (int by = 1; lo > 0 && cu[lo] > t; by *= 2) {
+      hi = lo;
+      lo = lo < by ? 0 : lo - by;
+    }
+  }
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (cu[mid] <= t) lo = mid; else hi = mid;
@@ -348,32 +361,78 @@ __device__ __forceinline__ void store_state(float* p, float2 v, int have) {
   if (have > 1) p[1] = v.y;
 }
 
+// Where a warp is among the packed sequences, the same in all lanes.
+struct Seqs {
+  int n0;          // the sequence of the run's first token w0
+  int64_t lo, hi;  // its bounds
+};
+
 // Which tokens of a lane's run start a sequence: bit j for token t0 + j, j = 0 .. kRun (one
 // more than the run has, for the end of its last token).  Empty sequences start
-// no token.  w0: the first token of the warp's run, the same in every lane.
-// lo, hi: the bounds of the sequence that the last search found; a run strictly
-// inside them needs no search.
+// no token.  w0: the first token of the warp's run, the same in every lane.  A
+// run strictly inside the sequence found last needs no search; one that is not
+// costs two loads by the whole warp where the next sequence is near.
 template <typename G>
 __device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t w0, int group,
-                                               int lane, int64_t& lo, int64_t& hi) {
+                                               int lane, Seqs& s) {
   static_assert(G::kWarpRun <= 64, "bits of a warp's run");
-  if (lo < w0 && w0 + G::kWarpRun < hi) return 0;
-  const int n0 = seq_of(cu, N, w0);
-  lo = cu[n0];
-  hi = cu[n0 + 1];
-  uint64_t bits = lo == w0 ? 1 : 0;
+  if (s.lo < w0 && w0 + G::kWarpRun < s.hi) return 0;
+  if (cu[s.n0] <= w0) {
+    for (;;) {  // forwards: entries after n0 that are <= w0
+      const int n = s.n0 + 1 + lane;
+      const uint32_t past = __ballot_sync(~0u, n < N && cu[n] <= w0);
+      s.n0 += __popc(past);
+      if (past != ~0u) break;
+    }
+  } else {
+    for (;;) {  // backwards: the nearest entry <= w0 (the first one if there is none)
+      const int n = s.n0 - lane;
+      const uint32_t found = __ballot_sync(~0u, n <= 0 || cu[n] <= w0);
+      s.n0 = max(0, s.n0 - (found ? __ffs(found) - 1 : 32));
+      if (found) break;
+    }
+  }
+  s.lo = cu[s.n0];
+  s.hi = cu[s.n0 + 1];
+  uint64_t bits = s.lo == w0 ? 1 : 0;
   uint32_t beyond = 0;  // token w0 + 64
-  for (int n = n0 + 1; n < N; n += 32) {
-    const int64_t at = n + lane < N ? cu[n + lane] - w0 : G::kWarpRun + 1;
+  for (int n = s.n0 + 1;; n += 32) {
+    const int64_t far = n + lane < N ? cu[n + lane] - w0 : G::kWarpRun + 1;
+    const int at = static_cast<int>(min(max(far, int64_t{-1}), int64_t{G::kWarpRun + 1}));
     const uint64_t mine = at > 0 && at < 64 ? 1ull << at : 0ull;
     bits |= static_cast<uint64_t>(__reduce_or_sync(~0u, static_cast<uint32_t>(mine >> 32))) << 32 |
             __reduce_or_sync(~0u, static_cast<uint32_t>(mine));
     beyond |= __any_sync(~0u, at == 64);
-    if (__shfl_sync(~0u, static_cast<int>(at <= G::kWarpRun), 31) == 0) break;
+    if (n + 32 >= N || __shfl_sync(~0u, static_cast<int>(at <= G::kWarpRun), 31) == 0) break;
   }
   uint32_t run = static_cast<uint32_t>(bits >> (group * G::kRun)) & ((1u << (G::kRun + 1)) - 1);
   if (group * G::kRun + G::kRun == 64) run |= beyond << G::kRun;
   return run;
+}
+
+// For each token of `bits` (of the lane's run), v of its sequence into slot[token][lane].
+// Rolled on purpose, like put_bounds: unrolled over the tokens the searches made the kernels
+// miss the instruction cache (5 us a bound).
+__device__ __forceinline__ void get_bounds(uint32_t bits, const float* v, float2* slot,
+                                           const int32_t* cu, int N, int64_t t0, int64_t D,
+                                           int64_t ch, int have, int lane, int n0) {
+#pragma unroll 1
+  for (; bits; bits &= bits - 1) {
+    const int j = __ffs(bits) - 1;
+    const int64_t n = seq_near(cu, N, t0 + j, n0);
+    slot[j * 32 + lane] = load_state(v ? v + n * D + ch : nullptr, have);
+  }
+}
+// The reverse: slot[token][lane] to v of the token's sequence.
+__device__ __forceinline__ void put_bounds(uint32_t bits, float* v, const float2* slot,
+                                           const int32_t* cu, int N, int64_t t0, int64_t D,
+                                           int64_t ch, int have, int lane, int n0) {
+#pragma unroll 1
+  for (; bits; bits &= bits - 1) {
+    const int j = __ffs(bits) - 1;
+    const int64_t n = seq_near(cu, N, t0 + j, n0);
+    store_state(v + n * D + ch, slot[j * 32 + lane], have);
+  }
 }
 
 // Warp w passes on to the next one, which waits: hardware barrier 1 + w counts
@@ -388,13 +447,15 @@ __device__ __forceinline__ void link_wait(int w) {
 
 // Joins the maps of a warp's lane groups in their order (backwards: from the last): `run`
 // comes back as the map up to and with the lane's own, and the result is the
-// one up to its predecessor (of no meaning in the first group).
+// one up to its predecessor (of no meaning in the first group).  bounds: the
+// warp's run has tokens that forget.
 template <typename G, bool kPacked, bool kBackwards>
-__device__ __forceinline__ Run scan_groups(Run& run, int lane) {
+__device__ __forceinline__ Run scan_groups(Run& run, int lane, bool bounds) {
 #pragma unroll
   for (int off = G::kPairs; off < 32; off *= 2) {
     const Run other = shuffle_by<kBackwards>(run, off);
-    if (kBackwards ? lane + off < 32 : lane >= off) run = join<kPacked>(other, run);
+    const Run longer = kPacked && bounds ? join<true>(other, run) : join<false>(other, run);
+    if (kBackwards ? lane + off < 32 : lane >= off) run = longer;
   }
   return shuffle_by<kBackwards>(run, G::kPairs);
 }
@@ -422,7 +483,7 @@ struct Exchange {
   // before the step (a cluster) or before everything (one CTA).  Two buffers in turn:
   // one is written again only after a barrier that every reader has passed.
   template <bool kPacked>
-  __device__ __forceinline__ float2 before(const Run& run, bool holder, float2& carry, int par,
+  __device__ __forceinline__ float2 before(const Run& run, bool bounds, bool holder, float2& carry, int par,
                                            bool first, bool more, int warp, int warps,
                                            uint32_t size, uint32_t rank, int pair) {
     float2 h = carry;
@@ -461,7 +522,7 @@ struct Exchange {
       }
       if (more || warp + 1 < warps) {
         const int to = warp + 1 == warps ? 0 : warp + 1;
-        const float2 out = apply<kPacked>(run, h);
+        const float2 out = kPacked && bounds ? apply<true>(run, h) : apply<false>(run, h);
         if (warps == 1) __syncwarp();  // read above before it is overwritten
         if (holder) link[to * G::kPairs + pair] = make_float4(out.x, out.y, 0.0f, 0.0f);
         __syncwarp();
@@ -581,18 +642,23 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
   if (!kPacked) carry = load_state(p.h0 ? p.h0 + b * D + ch : nullptr, have);
   ex.init(warp, warps, size, pair);
 
-  int64_t seq_lo = 0, seq_hi = 0;
+  Seqs seqs{0, 0, 0};
   int par = 0, stage = 0;
   for (int64_t base = 0; base < T_; base += stride, par ^= 1) {
     const int64_t w0 = base + static_cast<int64_t>(rank * warps + warp) * G::kWarpRun;
     const int64_t t0 = w0 + group * kRun;
     const int64_t left = T_ - t0;
     const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
-    uint32_t starts = 0;
-    bool bounds = false;  // a sequence starts or ends in the warp's run
+    uint32_t starts = 0, stops = 0;  // bit j: token j begins its sequence / ends it
+    bool bounds = false;             // one of the warp's tokens does
     if (kPacked && w0 < T_) {
-      starts = start_bits<G>(p.cu, p.N, w0, group, lane, seq_lo, seq_hi);
+      starts = start_bits<G>(p.cu, p.N, w0, group, lane, seqs);
       bounds = __any_sync(~0u, starts != 0) || w0 + G::kWarpRun >= T_;
+      if (bounds) {
+        if (len > 0)
+          stops = (starts >> 1 | (t0 + len == T_ ? 1u << (len - 1) : 0u)) & ((1u << len) - 1);
+        starts &= (1u << len) - 1;
+      }
     }
 
     float2 a[kRun], u[kRun];
@@ -606,20 +672,23 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
         fwd_run<G, false>(mine, k, p.consts, a, u);
     }
     __syncwarp();  // read by every lane before they are overwritten
-    fetch(stage);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+    // A run with bounds keeps its tile a while longer, for their states.
+    float2* slot = reinterpret_cast<float2*>(ring + stage * (3 * kTile));
+    static_assert(3 * kTile * sizeof(T) >= kRun * 32 * sizeof(float2), "a state for every token");
+    if (!bounds) fetch(stage);
     if (len < kRun)
 #pragma unroll
       for (int j = 0; j < kRun; ++j)
         if (j >= len) a[j] = both(1.0f), u[j] = both(0.0f);  // past the end: the identity
-    if (kPacked && bounds)
+    if (kPacked && bounds) {
+      get_bounds(starts, p.h0, slot, p.cu, p.N, t0, D, ch, have, lane, seqs.n0);
 #pragma unroll
       for (int j = 0; j < kRun; ++j)
-        if ((starts >> j & 1) && j < len) {
-          const int64_t n = seq_of(p.cu, p.N, t0 + j);
-          u[j] = ffma2(a[j], load_state(p.h0 ? p.h0 + n * D + ch : nullptr, have), u[j]);
+        if (starts >> j & 1) {
+          u[j] = ffma2(a[j], slot[j * 32 + lane], u[j]);
           a[j] = both(kForget);
         }
+    }
     Run run = {a[0], u[0]};
     if (kPacked && bounds)
 #pragma unroll
@@ -627,10 +696,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     else
 #pragma unroll
       for (int j = 1; j < kRun; ++j) run = join<false>(run, Run{a[j], u[j]});
-    const Run earlier = scan_groups<G, kPacked, false>(run, lane);
-    float2 h = ex.template before<kPacked>(run, group == G::kGroups - 1, carry, par, base == 0,
+    const Run earlier = scan_groups<G, kPacked, false>(run, lane, bounds);
+    float2 h = ex.template before<kPacked>(run, bounds, group == G::kGroups - 1, carry, par, base == 0,
                                            base + stride < T_, warp, warps, size, rank, pair);
-    if (group > 0) h = apply<kPacked>(earlier, h);
+    if (group > 0) h = kPacked && bounds ? apply<true>(earlier, h) : apply<false>(earlier, h);
 
     if (p.states && len > 0 && t0 % kSegment == 0)
       store_state(p.states + (b * nseg + t0 / kSegment) * D + ch, h, have);
@@ -647,11 +716,16 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
         h = apply<kPacked>(Run{a[j], u[j]}, h);
         if (j < len) {
           store_pair<T, kBytes>(yp + j * D, h, have);
-          if (kPacked && ((starts >> (j + 1) & 1) || t0 + j + 1 == T_))
-            store_state(p.hT + seq_of(p.cu, p.N, t0 + j) * D + ch, h, have);
+          if (kPacked && (stops >> j & 1)) slot[j * 32 + lane] = h;
         }
       }
     }
+    if (kPacked && bounds) {
+      put_bounds(stops, p.hT, slot, p.cu, p.N, t0, D, ch, have, lane, seqs.n0);
+      __syncwarp();
+      fetch(stage);
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
     if (!kPacked && len > 0 && t0 + len == T_) store_state(p.hT + b * D + ch, h, have);
   }
   copies_wait<0>();
@@ -745,27 +819,33 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
   const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * G::kChans, ch = ch0 + 2 * pair;
   const int have = ch + 1 < D ? 2 : (ch < D ? 1 : 0);  // channels of this lane
   T* ring = reinterpret_cast<T*>(dynamic_smem) + warp * (kStages * 4 * kTile);
+  // Packed sequences: the state before a token that begins one, what is handed to one that ends one.
+  float2* first_slot = reinterpret_cast<float2*>(dynamic_smem + warps * (kStages * 4 * kTile) * sizeof(T)) +
+                       warp * (2 * kRun * 32);
+  float2* last_slot = first_slot + kRun * 32;
   const int64_t runs = (T_ + G::kWarpRun - 1) / G::kWarpRun;
   const int64_t stride = static_cast<int64_t>(warps) * size;  // runs of a step
 
   // Runs are counted from the last one, q = 0; run q begins at token (runs - 1 - q) kWarpRun.
-  int64_t next = rank * warps + warp;  // to be copied next
+  int64_t next = (runs - 1 - static_cast<int64_t>(rank * warps + warp)) * G::kWarpRun;
+  const int64_t by = stride * G::kWarpRun;  // tokens of a step
+  const T* xn = static_cast<const T*>(p.x) + b * p.st.xb + ch0 + next * p.st.xt;
+  const T* in = static_cast<const T*>(p.ig) + b * p.st.ib + ch0 + next * p.st.it;
+  const T* rn = static_cast<const T*>(p.rg) + b * p.st.rb + ch0 + next * p.st.rt;
+  const T* gn = static_cast<const T*>(p.dy) + b * p.st.gb + ch0 + next * p.st.gt;
   auto fetch = [&](int stage) {
-    if (next < runs) {
-      const int64_t t = (runs - 1 - next) * G::kWarpRun;
-      const int len = T_ - t < G::kWarpRun ? static_cast<int>(T_ - t) : G::kWarpRun;
+    if (next >= 0) {
+      const int len = T_ - next < G::kWarpRun ? static_cast<int>(T_ - next) : G::kWarpRun;
       T* to = ring + stage * (4 * kTile);
-      copy_tile<G, kBytes>(to, static_cast<const T*>(p.x) + b * p.st.xb + t * p.st.xt + ch0,
-                           p.st.xt, len, D - ch0, lane);
-      copy_tile<G, kBytes>(to + kTile, static_cast<const T*>(p.ig) + b * p.st.ib + t * p.st.it + ch0,
-                           p.st.it, len, D - ch0, lane);
-      copy_tile<G, kBytes>(to + 2 * kTile,
-                           static_cast<const T*>(p.rg) + b * p.st.rb + t * p.st.rt + ch0, p.st.rt,
-                           len, D - ch0, lane);
-      copy_tile<G, kBytes>(to + 3 * kTile,
-                           static_cast<const T*>(p.dy) + b * p.st.gb + t * p.st.gt + ch0, p.st.gt,
-                           len, D - ch0, lane);
-      next += stride;
+      copy_tile<G, kBytes>(to, xn, p.st.xt, len, D - ch0, lane);
+      copy_tile<G, kBytes>(to + kTile, in, p.st.it, len, D - ch0, lane);
+      copy_tile<G, kBytes>(to + 2 * kTile, rn, p.st.rt, len, D - ch0, lane);
+      copy_tile<G, kBytes>(to + 3 * kTile, gn, p.st.gt, len, D - ch0, lane);
+      xn -= by * p.st.xt;
+      in -= by * p.st.it;
+      rn -= by * p.st.rt;
+      gn -= by * p.st.gt;
+      next -= by;
     }
     copies_commit();  // a group a step, empty past the end
   };
@@ -790,7 +870,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
   if (!kPacked) carry = load_state(p.dhT ? p.dhT + b * D + ch : nullptr, have);
   ex.init(warp, warps, size, pair);
 
-  int64_t seq_lo = 0, seq_hi = 0;
+  Seqs seqs{kPacked ? p.N - 1 : 0, 0, 0};
   int par = 0, stage = 0;
   for (int64_t base = 0; base < runs; base += stride, par ^= 1) {
     const int64_t q = base + rank * warps + warp;
@@ -805,20 +885,21 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     if (mine_exists) {
       state = load_state(p.states + (b * runs + w0 / kSegment) * D + ch, have);
       if (kPacked) {
-        starts = start_bits<G>(p.cu, p.N, w0, group, lane, seq_lo, seq_hi);
+        starts = start_bits<G>(p.cu, p.N, w0, group, lane, seqs);
         bounds = __any_sync(~0u, starts != 0) || w0 + G::kWarpRun >= T_;
-        if (bounds && len > 0) {
-          stops = starts >> 1 | (t0 + len == T_ ? 1u << (len - 1) : 0u);
-          stops &= (1u << len) - 1;
+        if (bounds) {
+          if (len > 0)
+            stops = (starts >> 1 | (t0 + len == T_ ? 1u << (len - 1) : 0u)) & ((1u << len) - 1);
           starts &= (1u << len) - 1;
+          get_bounds(starts, p.h0, first_slot, p.cu, p.N, t0, D, ch, have, lane, seqs.n0);
+          get_bounds(stops, p.dhT, last_slot, p.cu, p.N, t0, D, ch, have, lane, seqs.n0);
         }
       }
     }
-    auto begins = [&](int j) { return kPacked && bounds && (starts >> j & 1); };
-    auto ends = [&](int j) { return kPacked && bounds && (stops >> j & 1); };
-    auto of_seq = [&](const float* v, int j) {  // v of token j's sequence
-      return load_state(v ? v + seq_of(p.cu, p.N, t0 + j) * D + ch : nullptr, have);
-    };
+    auto begins = [&](int j) { return kPacked && (starts >> j & 1); };
+    auto ends = [&](int j) { return kPacked && (stops >> j & 1); };
+    auto before_seq = [&](int j) { return first_slot[j * 32 + lane]; };
+    auto after_seq = [&](int j) { return last_slot[j * 32 + lane]; };
 
     float2 a[kRun], hp[kRun], si[kRun], sr[kRun];
     copies_wait<kStages - 1>();
@@ -841,7 +922,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
 
     // Maps of the run: of the states (forwards) and of what is carried (backwards).
     // `plain`: nothing begins, ends or is missing in the warp's run, so nothing is asked.
-    const bool plain = mine_exists && !bounds && kBytes == 16 && ch0 + G::kChans <= D &&
+    const bool plain = !bounds && mine_exists && kBytes == 16 && ch0 + G::kChans <= D &&
                        w0 + G::kWarpRun <= T_;
     Run fwd(both(1.0f), both(0.0f)), bwd(both(1.0f), both(0.0f));
     if (plain) {
@@ -853,21 +934,26 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     } else {
 #pragma unroll
       for (int j = 0; j < kRun; ++j) {
-        if (begins(j)) fwd = Run(both(kForget), of_seq(p.h0, j));
-        fwd = join<kPacked>(fwd, Run(a[j], hp[j]));
+        if (begins(j)) fwd = Run(both(kForget), before_seq(j));
+        fwd = kPacked ? Run(fwd.A.x < 0.0f ? fwd.A : fmul2(fwd.A, a[j]), ffma2(a[j], fwd.H, hp[j]))
+                      : join<false>(fwd, Run(a[j], hp[j]));
       }
 #pragma unroll
       for (int j = kRun - 1; j >= 0; --j) {
-        if (ends(j)) bwd = Run(both(kForget), of_seq(p.dhT, j));
-        bwd = join<kPacked>(bwd, Run(a[j], fmul2(a[j], dy_at(j))));
+        if (ends(j)) bwd = Run(both(kForget), after_seq(j));
+        bwd = Run(kPacked && bwd.A.x < 0.0f ? bwd.A : fmul2(bwd.A, a[j]),
+                  fmul2(a[j], fadd2(dy_at(j), bwd.H)));
       }
     }
-    const Run earlier = scan_groups<G, kPacked, false>(fwd, lane);
-    const Run later = scan_groups<G, kPacked, true>(bwd, lane);
-    float2 cr = ex.template before<kPacked>(bwd, group == 0, carry, par, base == 0,
+    const Run earlier = scan_groups<G, kPacked, false>(fwd, lane, bounds);
+    const Run later = scan_groups<G, kPacked, true>(bwd, lane, bounds);
+    float2 cr = ex.template before<kPacked>(bwd, bounds, group == 0, carry, par, base == 0,
                                             base + stride < runs, warp, warps, size, rank, pair);
-    if (group < G::kGroups - 1) cr = apply<kPacked>(later, cr);
-    float2 h = group > 0 ? apply<kPacked>(earlier, state) : state;
+    if (group < G::kGroups - 1)
+      cr = kPacked && bounds ? apply<true>(later, cr) : apply<false>(later, cr);
+    float2 h = state;
+    if (group > 0)
+      h = kPacked && bounds ? apply<true>(earlier, state) : apply<false>(earlier, state);
     const int64_t row0 = (b * T_ + t0) * D + ch;
     T *dxp = static_cast<T*>(p.dx) + row0, *dip = static_cast<T*>(p.di) + row0,
       *drp = static_cast<T*>(p.dr) + row0;
@@ -875,7 +961,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     auto finish = [&](auto all_near, auto asks) {
 #pragma unroll
       for (int j = 0; j < kRun; ++j) {
-        if (asks.value && begins(j)) h = of_seq(p.h0, j);
+        if (asks.value && begins(j)) h = before_seq(j);
         const float2 u = hp[j];
         hp[j] = h;
         h = ffma2(a[j], h, u);
@@ -887,7 +973,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
       }
 #pragma unroll
       for (int j = kRun - 1; j >= 0; --j) {
-        if (asks.value && ends(j)) cr = of_seq(p.dhT, j);
+        if (asks.value && ends(j)) cr = after_seq(j);
         if (asks.value && j >= len) continue;
         const TokenGrads o = token_grads<all_near.value>(
             fadd2(word(3, j), cr), hp[j], word(0, j), a[j], si[j], sr[j], k, p.consts);
@@ -897,7 +983,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
           store_pair<T, kBytes>(dxp + j * D, o.dx, have);
           store_pair<T, kBytes>(dip + j * D, o.di, have);
           store_pair<T, kBytes>(drp + j * D, o.dr, have);
-          if (begins(j)) store_state(p.dh0 + seq_of(p.cu, p.N, t0 + j) * D + ch, cr, have);
+          if (begins(j)) first_slot[j * 32 + lane] = cr;
         } else {
           store_pair<T, kBytes>(dxp, o.dx, 2);
           store_pair<T, kBytes>(dip, o.di, 2);
@@ -912,8 +998,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
       finish(std::true_type(), std::false_type());
     else if (plain)
       finish(std::false_type(), std::false_type());
+    else if (kPacked && near)
+      finish(std::true_type(), std::true_type());
     else
       finish(std::false_type(), std::true_type());
+    if (kPacked && bounds)
+      put_bounds(starts, p.dh0, first_slot, p.cu, p.N, t0, D, ch, have, lane, seqs.n0);
     if (!kPacked && mine_exists && t0 == 0) store_state(p.dh0 + b * D + ch, cr, have);
     __syncwarp();  // read by every lane before they are overwritten
     fetch(stage);
@@ -1033,7 +1123,8 @@ template <typename T, int kBytes>
 int launch_bwd_bytes(const BwdArgs& a, int64_t batch, cudaStream_t s) {
   constexpr int kStages = sizeof(T) == 2 ? GLR_BSTAGES : GLR_BSTAGES / 2;
   const ScanGrid g = scan_grid<BwdGeo>(batch, a.T, a.D);
-  const size_t smem = static_cast<size_t>(g.warps) * kStages * 4 * BwdGeo::kTile * sizeof(T);
+  size_t smem = static_cast<size_t>(g.warps) * kStages * 4 * BwdGeo::kTile * sizeof(T);
+  if (a.cu) smem += static_cast<size_t>(g.warps) * 2 * BwdGeo::kRun * 32 * sizeof(float2);
   return launch_scan(a.cu ? glr_bwd_scan<T, BwdGeo, kBytes, true, kStages>
                           : glr_bwd_scan<T, BwdGeo, kBytes, false, kStages>,
                      g, batch, smem, a, s);
