@@ -254,7 +254,7 @@ int tileops_gla_decode_fwd(const void* q, const void* k, const void* v, const vo
  * num_seqs + 1 offsets, batch 1, the rules of tileops_gdn_prefill_varlen_fwd
  * (0 = cu[0] <= ... <= cu[num_seqs] = seq_len; device error 2 and meaningless
  * results otherwise, never an access out of range).  batch up to 65535,
- * seq_len >= 1.  No output may alias an input.  No counterpart in the
+ * seq_len 1 .. 2^31 - 2^16.  No output may alias an input.  No counterpart in the
  * reference. */
 int tileops_glr_fwd(const void* x, const void* input_gate, const void* decay_gate,
                     const float* decay_param, const float* initial_state,

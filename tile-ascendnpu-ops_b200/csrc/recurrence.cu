@@ -83,7 +83,7 @@ __device__ __forceinline__ float decay_rate(float lambda, float c) {
 // ---- packed sequences ----
 // The sequence token t belongs to, the last n with cu[n] <= t, in [0, N); from a guess
 // nearby: doubling steps away from it, then halves.
-__device__ __forceinline__ int seq_near(const int32_t* cu, int N, int64_t t, int guess) {
+__device__ __forceinline__ int seq_near(const int32_t* cu, int N, int t, int guess) {
   int lo = guess, hi = guess + 1;
   if (cu[guess] <= t) {
     for (int by = 1; hi < N && cu[hi] <= t; by *= 2) {
@@ -262,12 +262,6 @@ __device__ __forceinline__ Run join(const Run& first, const Run& then) {
   return r;
 }
 
-#ifndef GLR_FILL
-#define GLR_FILL 2
-#endif
-#ifndef GLR_BSTAGES
-#define GLR_BSTAGES 2
-#endif
 constexpr int kMaxWarps = 8;    // warps of a CTA
 constexpr int kMaxCluster = 8;  // CTAs of a cluster
 
@@ -363,8 +357,8 @@ __device__ __forceinline__ void store_state(float* p, float2 v, int have) {
 
 // Where a warp is among the packed sequences, the same in all lanes.
 struct Seqs {
-  int n0;          // the sequence of the run's first token w0
-  int64_t lo, hi;  // its bounds
+  int n0;      // the sequence of the run's first token w0
+  int lo, hi;  // its bounds
 };
 
 // Which tokens of a lane's run start a sequence: bit j for token t0 + j, j = 0 .. kRun (one
@@ -373,7 +367,7 @@ struct Seqs {
 // run strictly inside the sequence found last needs no search; one that is not
 // costs two loads by the whole warp where the next sequence is near.
 template <typename G>
-__device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t w0, int group,
+__device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int w0, int group,
                                                int lane, Seqs& s) {
   static_assert(G::kWarpRun <= 64, "bits of a warp's run");
   if (s.lo < w0 && w0 + G::kWarpRun < s.hi) return 0;
@@ -397,7 +391,7 @@ __device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t
   uint64_t bits = s.lo == w0 ? 1 : 0;
   uint32_t beyond = 0;  // token w0 + 64
   for (int n = s.n0 + 1;; n += 32) {
-    const int64_t far = n + lane < N ? cu[n + lane] - w0 : G::kWarpRun + 1;
+    const int64_t far = n + lane < N ? int64_t{cu[n + lane]} - w0 : G::kWarpRun + 1;
     const int at = static_cast<int>(min(max(far, int64_t{-1}), int64_t{G::kWarpRun + 1}));
     const uint64_t mine = at > 0 && at < 64 ? 1ull << at : 0ull;
     bits |= static_cast<uint64_t>(__reduce_or_sync(~0u, static_cast<uint32_t>(mine >> 32))) << 32 |
@@ -414,7 +408,7 @@ __device__ __forceinline__ uint32_t start_bits(const int32_t* cu, int N, int64_t
 // Rolled on purpose, like put_bounds: unrolled over the tokens the searches made the kernels
 // miss the instruction cache (5 us a bound).
 __device__ __forceinline__ void get_bounds(uint32_t bits, const float* v, float2* slot,
-                                           const int32_t* cu, int N, int64_t t0, int64_t D,
+                                           const int32_t* cu, int N, int t0, int64_t D,
                                            int64_t ch, int have, int lane, int n0) {
 #pragma unroll 1
   for (; bits; bits &= bits - 1) {
@@ -425,7 +419,7 @@ __device__ __forceinline__ void get_bounds(uint32_t bits, const float* v, float2
 }
 // The reverse: slot[token][lane] to v of the token's sequence.
 __device__ __forceinline__ void put_bounds(uint32_t bits, float* v, const float2* slot,
-                                           const int32_t* cu, int N, int64_t t0, int64_t D,
+                                           const int32_t* cu, int N, int t0, int64_t D,
                                            int64_t ch, int have, int lane, int n0) {
 #pragma unroll 1
   for (; bits; bits &= bits - 1) {
@@ -534,7 +528,7 @@ struct Exchange {
 };
 
 // cu_seqlens must be 0 = cu[0] <= ... <= cu[N] = total; reported otherwise.
-__device__ __forceinline__ void check_seqlens(const int32_t* cu, int N, int64_t total, int lane,
+__device__ __forceinline__ void check_seqlens(const int32_t* cu, int N, int total, int lane,
                                               int* err) {
   bool bad = false;
   for (int n = lane; n < N; n += 32) bad |= cu[n + 1] < cu[n];
@@ -549,7 +543,8 @@ struct FwdArgs {
   const int32_t* cu;
   void* y;
   float *hT, *states;
-  int64_t T, D;
+  int T;  // tokens; all counts of tokens fit an int (bad_shape)
+  int64_t D;
   Strides st;
   int N;
   float c;
@@ -595,21 +590,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
   const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
   const int warps = blockDim.x >> 5;
   const uint32_t size = cluster_size(), rank = cluster_rank();
-  const int64_t b = blockIdx.y, T_ = p.T, D = p.D;
+  const int64_t b = blockIdx.y, D = p.D;
+  const int T_ = p.T;
   const int group = lane / G::kPairs, pair = lane % G::kPairs;
   const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * G::kChans, ch = ch0 + 2 * pair;
   const int have = ch + 1 < D ? 2 : (ch < D ? 1 : 0);  // channels of this lane
   T* ring = reinterpret_cast<T*>(dynamic_smem) + warp * (kStages * 3 * kTile);
-  const int64_t nseg = (T_ + kSegment - 1) / kSegment;
-  const int64_t stride = static_cast<int64_t>(G::kWarpRun) * warps * size;  // tokens of a step
+  const int nseg = (T_ + kSegment - 1) / kSegment;
+  const int stride = G::kWarpRun * warps * static_cast<int>(size);  // tokens of a step
 
-  int64_t next = static_cast<int64_t>(rank * warps + warp) * G::kWarpRun;  // to be copied next
+  int next = (static_cast<int>(rank) * warps + warp) * G::kWarpRun;  // to be copied next
   const T* xn = static_cast<const T*>(p.x) + b * p.st.xb + ch0 + next * p.st.xt;
   const T* in = static_cast<const T*>(p.ig) + b * p.st.ib + ch0 + next * p.st.it;
   const T* rn = static_cast<const T*>(p.rg) + b * p.st.rb + ch0 + next * p.st.rt;
   auto fetch = [&](int stage) {
     if (next < T_) {
-      const int len = T_ - next < G::kWarpRun ? static_cast<int>(T_ - next) : G::kWarpRun;
+      const int len = min(T_ - next, G::kWarpRun);
       T* t = ring + stage * (3 * kTile);
       copy_tile<G, kBytes>(t, xn, p.st.xt, len, D - ch0, lane);
       copy_tile<G, kBytes>(t + kTile, in, p.st.it, len, D - ch0, lane);
@@ -644,15 +640,15 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
 
   Seqs seqs{0, 0, 0};
   int par = 0, stage = 0;
+  // (64-bit counters here: with 32-bit ones ptxas spilled 44 bytes, 214 -> 247 us.)
   for (int64_t base = 0; base < T_; base += stride, par ^= 1) {
-    const int64_t w0 = base + static_cast<int64_t>(rank * warps + warp) * G::kWarpRun;
-    const int64_t t0 = w0 + group * kRun;
-    const int64_t left = T_ - t0;
+    const int64_t w0 = base + (static_cast<int>(rank) * warps + warp) * G::kWarpRun;
+    const int64_t t0 = w0 + group * kRun, left = T_ - t0;
     const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
     uint32_t starts = 0, stops = 0;  // bit j: token j begins its sequence / ends it
     bool bounds = false;             // one of the warp's tokens does
     if (kPacked && w0 < T_) {
-      starts = start_bits<G>(p.cu, p.N, w0, group, lane, seqs);
+      starts = start_bits<G>(p.cu, p.N, static_cast<int>(w0), group, lane, seqs);
       bounds = __any_sync(~0u, starts != 0) || w0 + G::kWarpRun >= T_;
       if (bounds) {
         if (len > 0)
@@ -673,9 +669,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     }
     __syncwarp();  // read by every lane before they are overwritten
     // A run with bounds keeps its tile a while longer, for their states.
-    float2* slot = reinterpret_cast<float2*>(ring + stage * (3 * kTile));
+    const int here = stage;
+    float2* slot = reinterpret_cast<float2*>(ring + here * (3 * kTile));
     static_assert(3 * kTile * sizeof(T) >= kRun * 32 * sizeof(float2), "a state for every token");
-    if (!bounds) fetch(stage);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    if (!bounds) fetch(here);
     if (len < kRun)
 #pragma unroll
       for (int j = 0; j < kRun; ++j)
@@ -723,9 +721,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
     if (kPacked && bounds) {
       put_bounds(stops, p.hT, slot, p.cu, p.N, t0, D, ch, have, lane, seqs.n0);
       __syncwarp();
-      fetch(stage);
+      fetch(here);
     }
-    stage = stage + 1 == kStages ? 0 : stage + 1;
     if (!kPacked && len > 0 && t0 + len == T_) store_state(p.hT + b * D + ch, h, have);
   }
   copies_wait<0>();
@@ -738,7 +735,8 @@ struct BwdArgs {
   const int32_t* cu;
   void *dx, *di, *dr;
   float *part, *dh0;
-  int64_t T, D;
+  int T;  // tokens; all counts of tokens fit an int (bad_shape)
+  int64_t D;
   Strides st;
   int N;
   float c;
@@ -814,7 +812,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
   const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
   const int warps = blockDim.x >> 5;
   const uint32_t size = cluster_size(), rank = cluster_rank();
-  const int64_t b = blockIdx.y, T_ = p.T, D = p.D;
+  const int64_t b = blockIdx.y, D = p.D;
+  const int T_ = p.T;
   const int group = lane / G::kPairs, pair = lane % G::kPairs;
   const int64_t ch0 = static_cast<int64_t>(blockIdx.x / size) * G::kChans, ch = ch0 + 2 * pair;
   const int have = ch + 1 < D ? 2 : (ch < D ? 1 : 0);  // channels of this lane
@@ -823,19 +822,19 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
   float2* first_slot = reinterpret_cast<float2*>(dynamic_smem + warps * (kStages * 4 * kTile) * sizeof(T)) +
                        warp * (2 * kRun * 32);
   float2* last_slot = first_slot + kRun * 32;
-  const int64_t runs = (T_ + G::kWarpRun - 1) / G::kWarpRun;
-  const int64_t stride = static_cast<int64_t>(warps) * size;  // runs of a step
+  const int runs = (T_ + G::kWarpRun - 1) / G::kWarpRun;
+  const int stride = warps * static_cast<int>(size);  // runs of a step
 
   // Runs are counted from the last one, q = 0; run q begins at token (runs - 1 - q) kWarpRun.
-  int64_t next = (runs - 1 - static_cast<int64_t>(rank * warps + warp)) * G::kWarpRun;
-  const int64_t by = stride * G::kWarpRun;  // tokens of a step
+  int next = (runs - 1 - (static_cast<int>(rank) * warps + warp)) * G::kWarpRun;
+  const int by = stride * G::kWarpRun;  // tokens of a step
   const T* xn = static_cast<const T*>(p.x) + b * p.st.xb + ch0 + next * p.st.xt;
   const T* in = static_cast<const T*>(p.ig) + b * p.st.ib + ch0 + next * p.st.it;
   const T* rn = static_cast<const T*>(p.rg) + b * p.st.rb + ch0 + next * p.st.rt;
   const T* gn = static_cast<const T*>(p.dy) + b * p.st.gb + ch0 + next * p.st.gt;
   auto fetch = [&](int stage) {
     if (next >= 0) {
-      const int len = T_ - next < G::kWarpRun ? static_cast<int>(T_ - next) : G::kWarpRun;
+      const int len = min(T_ - next, G::kWarpRun);
       T* to = ring + stage * (4 * kTile);
       copy_tile<G, kBytes>(to, xn, p.st.xt, len, D - ch0, lane);
       copy_tile<G, kBytes>(to + kTile, in, p.st.it, len, D - ch0, lane);
@@ -872,13 +871,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
 
   Seqs seqs{kPacked ? p.N - 1 : 0, 0, 0};
   int par = 0, stage = 0;
-  for (int64_t base = 0; base < runs; base += stride, par ^= 1) {
-    const int64_t q = base + rank * warps + warp;
+  for (int base = 0; base < runs; base += stride, par ^= 1) {
+    const int q = base + static_cast<int>(rank) * warps + warp;
     const bool mine_exists = q < runs;
-    const int64_t w0 = mine_exists ? (runs - 1 - q) * G::kWarpRun : 0;
-    const int64_t t0 = w0 + group * kRun;
-    const int64_t left = mine_exists ? T_ - t0 : 0;
-    const int len = left >= kRun ? kRun : (left > 0 ? static_cast<int>(left) : 0);
+    const int w0 = mine_exists ? (runs - 1 - q) * G::kWarpRun : 0;
+    const int t0 = w0 + group * kRun;
+    const int len = mine_exists ? max(0, min(T_ - t0, kRun)) : 0;
     float2 state = both(0.0f);
     uint32_t starts = 0, stops = 0;  // bit j: token j begins its sequence / ends it
     bool bounds = false;             // one of the warp's tokens does
@@ -1046,7 +1044,7 @@ ScanGrid scan_grid(int64_t batch, int64_t seq_len, int64_t dim) {
   const int64_t runs = (seq_len + G::kWarpRun - 1) / G::kWarpRun;
   g.warps = static_cast<int>(std::min<int64_t>(runs, kMaxWarps));
   g.cluster = 1;
-  while (g.cluster < kMaxCluster && g.blocks * batch * g.cluster < GLR_FILL * sm_count() / 2 &&
+  while (g.cluster < kMaxCluster && g.blocks * batch * g.cluster < sm_count() &&
          g.cluster * g.warps < runs)
     g.cluster *= 2;
   return g;
@@ -1121,7 +1119,7 @@ using BwdGeo = Geo<16, 8>;
 
 template <typename T, int kBytes>
 int launch_bwd_bytes(const BwdArgs& a, int64_t batch, cudaStream_t s) {
-  constexpr int kStages = sizeof(T) == 2 ? GLR_BSTAGES : GLR_BSTAGES / 2;
+  constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
   const ScanGrid g = scan_grid<BwdGeo>(batch, a.T, a.D);
   size_t smem = static_cast<size_t>(g.warps) * kStages * 4 * BwdGeo::kTile * sizeof(T);
   if (a.cu) smem += static_cast<size_t>(g.warps) * 2 * BwdGeo::kRun * 32 * sizeof(float2);
@@ -1169,9 +1167,10 @@ __global__ void __launch_bounds__(128)
   hn[b * D + d] = h;
 }
 
-// Sizes every kernel here indexes with: batch in a grid's y, 64-bit element offsets.
+// Sizes every kernel here indexes with: batch in a grid's y, token counts in an int (with
+// room for a step past the end), 64-bit element offsets.
 bool bad_shape(int64_t batch, int64_t seq_len, int64_t dim) {
-  return batch < 0 || seq_len < 0 || dim < 0 || batch > 65535 || seq_len > 0x7fffffffLL ||
+  return batch < 0 || seq_len < 0 || dim < 0 || batch > 65535 || seq_len > 0x7fff0000LL ||
          dim > 0x7fffffffLL;
 }
 
@@ -1198,7 +1197,7 @@ extern "C" int tileops_glr_fwd(const void* x, const void* input_gate, const void
   cudaStream_t s = as_stream(stream);
   const Strides st{x_stride_b, x_stride_t, i_stride_b, i_stride_t, r_stride_b, r_stride_t, 0, 0};
   const FwdArgs args{x, input_gate, decay_gate, decay_param, initial_state, cu_seqlens, y,
-                     final_state, states, seq_len, dim, st, static_cast<int>(num_seqs),
+                     final_state, states, static_cast<int>(seq_len), dim, st, static_cast<int>(num_seqs),
                      static_cast<float>(decay_scale), cu_seqlens ? device_error_ptr() : nullptr, Consts()};
   switch (dtype) {
     case TILEOPS_DT_F32: return launch_fwd<float>(args, batch, s);
@@ -1238,7 +1237,7 @@ extern "C" int tileops_glr_bwd(const void* dy, const void* x, const void* input_
   float* part = static_cast<float*>(workspace);
   const BwdArgs args{dy, x, input_gate, decay_gate, decay_param, states, initial_state,
                      d_final_state, cu_seqlens, dx, d_input_gate, d_decay_gate, part,
-                     d_initial_state, seq_len, dim, st, static_cast<int>(num_seqs), c,
+                     d_initial_state, static_cast<int>(seq_len), dim, st, static_cast<int>(num_seqs), c,
                      cu_seqlens ? device_error_ptr() : nullptr, Consts()};
   int status;
   switch (dtype) {

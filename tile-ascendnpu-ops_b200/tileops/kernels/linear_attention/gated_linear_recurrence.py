@@ -33,9 +33,10 @@ class _GatedLinearRecurrenceKernel(Kernel):
                  dtype: torch.dtype = torch.bfloat16, config: Optional[dict] = None):
         super().__init__()
         check_dtype(self, dtype, self.SUPPORTED_DTYPES)
-        if min(batch, seq_len) < 0 or dim < 1 or batch > 65535 or max(seq_len, dim) > 2**31 - 1:
-            raise ValueError(f"{type(self).__name__} supports batch 0..65535, seq_len >= 0 and "
-                             f"dim >= 1 below 2^31, got ({batch}, {seq_len}, {dim})")
+        if (min(batch, seq_len) < 0 or dim < 1 or batch > 65535 or seq_len > 2**31 - 2**16
+                or dim > 2**31 - 1):
+            raise ValueError(f"{type(self).__name__} supports batch 0..65535, seq_len "
+                             f"0..2^31 - 2^16 and dim 1..2^31 - 1, got ({batch}, {seq_len}, {dim})")
         if not 0.0 < decay_scale < float("inf"):
             raise ValueError(f"decay_scale must be positive and finite, got {decay_scale}")
         self.batch, self.seq_len, self.dim = batch, seq_len, dim
