@@ -17,6 +17,16 @@
 //   dw2 = sum dy s^, db2 = sum dy, dgate_g = w1 P_g + b1 Q_g,
 //   dw1 = sum_g gate_g P_g, db1 = sum_g gate_g Q_g
 // ([mean ..] terms: LayerNorm only).
+//
+// Both passes read each row once and write it once: persistent CTAs walk
+// consecutive rows, a thread owns the same columns in every row (parameters and
+// column sums stay in registers) and copies its own packets of the rows ahead into
+// a private slot of a shared-memory ring.  A row costs two barriers, one
+// for each norm: a LayerNorm's mean and variance are taken warp by warp, centred
+// there, and joined (Chan, Golub & LeVeque, "Updating formulae and a
+// pairwise algorithm for computing sample variances", 1979).
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace tileops {
@@ -28,7 +38,572 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sum over the CTA; every thread gets the total.  `red` holds 32 floats.
+template <typename W>
+__device__ __forceinline__ float param(const W* p, int64_t i, float otherwise) {
+  return p ? Cvt<W>::to_f(p[i]) : otherwise;
+}
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A thread's packets of a row: packet j is the row's packet threadIdx.x + j kThreads, kV
+// elements.  kAligned: rows of whole packets on 16-byte boundaries; otherwise
+// packets are read and written element by element and the last one may be short.
+template <typename T, int kThreads, int kPackets, bool kAligned>
+struct Cols {
+  static constexpr int kV = 16 / sizeof(T);
+  static __device__ __forceinline__ int first(int j) { return (threadIdx.x + j * kThreads) * kV; }
+  // How many elements packet j has.
+  static __device__ __forceinline__ int count(int j, int N) {
+    const int left = N - first(j);
+    return kAligned ? (left > 0 ? kV : 0) : max(0, min(kV, left));
+  }
+  static __device__ __forceinline__ void fetch(uint4* slot, const T* row, int j, int N) {
+    if constexpr (kAligned) {
+      if (first(j) < N) copy16(slot, row + first(j));
+    } else {
+      T e[kV];
+      const int n = count(j, N);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) e[i] = i < n ? row[first(j) + i] : Cvt<T>::from_f(0.0f);
+      memcpy(slot, e, 16);
+    }
+  }
+  static __device__ __forceinline__ void read(const uint4* slot, float* v) {
+    T e[kV];
+    const uint4 u = *slot;
+    memcpy(e, &u, 16);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) v[i] = Cvt<T>::to_f(e[i]);
+  }
+  static __device__ __forceinline__ void write(T* row, int j, int N, const float* v) {
+    T e[kV];
+#pragma unroll
+    for (int i = 0; i < kV; ++i) e[i] = Cvt<T>::from_f(v[i]);
+    if constexpr (kAligned) {
+      uint4 u;
+      memcpy(&u, e, 16);
+      if (first(j) < N) st_stream(row + first(j), u);
+    } else {
+      const int n = count(j, N);
+#pragma unroll
+      for (int i = 0; i < kV; ++i)
+        if (i < n) row[first(j) + i] = e[i];
+    }
+  }
+};
+
+// Rows of CTA c of C: consecutive, so that a CTA meets few gate groups.
+__device__ __forceinline__ int first_row(int64_t M, int c, int C) {
+  return static_cast<int>(M * c / C);
+}
+
+// ---- statistics of a row over a CTA, one barrier ----
+// Each warp publishes kSums numbers; after the barrier lane l holds warp l's and
+// the sums over warps are butterflies.  Callers alternate two buffers: one is
+// written again only after a barrier that every reader of it has passed.
+template <int kSums, int kWarps>
+struct WarpSums {
+  float v[kSums][kWarps];
+};
+
+template <int kWarps>
+__device__ __forceinline__ float over_warps(float v) {
+#pragma unroll
+  for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Number of row elements that lie in warp w.
+template <typename C, int kThreads, int kPackets>
+__device__ __forceinline__ float in_warp(int w, int N) {
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < kPackets; ++j) {
+    const int from = (w * 32 + j * kThreads) * C::kV;
+    n += max(0, min(32 * C::kV, N - from));
+  }
+  return static_cast<float>(n);
+}
+
+// What a warp knows of a row: its sum (LayerNorm) and its sum of squares about its
+// own mean (RMS: about zero).
+struct Moments {
+  float sum, sq;
+};
+template <int kV, int kPackets>
+__device__ __forceinline__ Moments warp_moments(const float (&v)[kPackets][kV],
+                                                const int (&n)[kPackets], bool layer,
+                                                float inv_in_warp, float& mean) {
+  Moments m{0.0f, 0.0f};
+  mean = 0.0f;
+  if (layer) {
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+      for (int i = 0; i < kV; ++i) m.sum += v[j][i];  // zeros past the end
+    m.sum = warp_sum(m.sum);
+    mean = m.sum * inv_in_warp;
+  }
+#pragma unroll
+  for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+      const float d = i < n[j] ? v[j][i] - mean : 0.0f;
+      m.sq = fmaf(d, d, m.sq);
+    }
+  m.sq = warp_sum(m.sq);
+  return m;
+}
+
+// ---- forward ----
+struct FwdArgs {
+  const void *x, *res, *w1, *w2, *gate, *b1, *b2;
+  void *y, *res_out;
+  int64_t M;
+  int N;
+  int64_t rows_per_group;
+  bool layer;
+  float eps, alpha;
+};
+
+template <typename T, typename W, int kThreads, int kPackets, int kStages, bool kAligned>
+__global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
+  using C = Cols<T, kThreads, kPackets, kAligned>;
+  constexpr int kV = C::kV, kWarps = kThreads / 32;
+  extern __shared__ uint4 ring[];  // [stage][x, residual][packet][thread]
+  __shared__ WarpSums<2, kWarps> sums[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, N = p.N;
+  const bool layer = p.layer;
+  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.res);
+  const W *w1 = static_cast<const W*>(p.w1), *w2 = static_cast<const W*>(p.w2),
+          *gate = static_cast<const W*>(p.gate), *b1 = static_cast<const W*>(p.b1),
+          *b2 = static_cast<const W*>(p.b2);
+  const int64_t row0 = first_row(p.M, blockIdx.x, gridDim.x),
+                end = first_row(p.M, blockIdx.x + 1, gridDim.x);
+  auto slot = [&](int stage, int tensor, int j) {
+    return ring + ((stage * 2 + tensor) * kPackets + j) * kThreads + threadIdx.x;
+  };
+  auto fetch = [&](int stage, int64_t row) {
+    if (row < end)
+#pragma unroll
+      for (int j = 0; j < kPackets; ++j) {
+        C::fetch(slot(stage, 0, j), x + row * N, j, N);
+        C::fetch(slot(stage, 1, j), res + row * N, j, N);
+      }
+    copies_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) fetch(s, row0 + s);
+
+  int n[kPackets];
+  float wg[kPackets][kV], bg[kPackets][kV], wn[kPackets][kV], bn[kPackets][kV];
+#pragma unroll
+  for (int j = 0; j < kPackets; ++j) {
+    n[j] = C::count(j, N);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+      const int c = C::first(j) + i;
+      const bool in = i < n[j];
+      wn[j][i] = in ? Cvt<W>::to_f(w2[c]) : 0.0f;
+      bn[j][i] = in ? param(b2, c, 0.0f) : 0.0f;
+    }
+  }
+  const float inv_n = 1.0f / static_cast<float>(N);
+  const float mine = in_warp<C, kThreads, kPackets>(warp, N);
+  const float inv_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
+  const int from = lane < kWarps ? lane : 0;  // the warp whose sums this lane joins
+  const float theirs = in_warp<C, kThreads, kPackets>(from, N);
+  const float inv_theirs = theirs > 0.0f ? 1.0f / theirs : 0.0f;
+
+  // mean and 1 / deviation of the row held in v.
+  auto stats = [&](const float(&v)[kPackets][kV], WarpSums<2, kWarps>& buf) {
+    float warp_mean;
+    const Moments m = warp_moments<kV, kPackets>(v, n, layer, inv_mine, warp_mean);
+    if (lane == 0) {
+      buf.v[0][warp] = m.sum;
+      buf.v[1][warp] = m.sq;
+    }
+    __syncthreads();
+    const float sum = buf.v[0][from];
+    float sq = buf.v[1][from], mean = 0.0f;
+    if (layer) {
+      mean = over_warps<kWarps>(sum) * inv_n;
+      const float d = sum * inv_theirs - mean;
+      sq = fmaf(theirs * d, d, sq);
+    }
+    sq = over_warps<kWarps>(sq);
+    // lanes beyond the warps hold copies of warp 0's sums: take lane 0's result
+    mean = __shfl_sync(0xffffffffu, mean, 0);
+    sq = __shfl_sync(0xffffffffu, sq, 0);
+    return make_float2(mean, 1.0f / sqrtf(sq * inv_n + p.eps));
+  };
+
+  int stage = 0;
+  int64_t next_group = row0;  // the row that starts another gate
+  for (int64_t row = row0; row < end; ++row) {
+    if (row >= next_group) {
+      const int64_t g = row / p.rows_per_group;
+      next_group = (g + 1) * p.rows_per_group;
+#pragma unroll
+      for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          const int c = C::first(j) + i;
+          const bool in = i < n[j];
+          const float ga = in ? param(gate, g * N + c, 1.0f) : 0.0f;
+          wg[j][i] = in ? ga * Cvt<W>::to_f(w1[c]) : 0.0f;
+          bg[j][i] = in ? ga * param(b1, c, 0.0f) : 0.0f;
+        }
+    }
+    fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
+    copies_wait<kStages - 1>();
+    float v[kPackets][kV];
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j) {
+      if (n[j] > 0)
+        C::read(slot(stage, 0, j), v[j]);
+      else
+#pragma unroll
+        for (int i = 0; i < kV; ++i) v[j][i] = 0.0f;
+    }
+    const float2 sx = stats(v, sums[0]);
+    T* out = static_cast<T*>(p.res_out) + row * N;
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j) {
+      if (n[j] > 0) {
+        float r[kV];
+        C::read(slot(stage, 1, j), r);
+#pragma unroll
+        for (int i = 0; i < kV; ++i)
+          v[j][i] = fmaf(p.alpha, r[i], fmaf((v[j][i] - sx.x) * sx.y, wg[j][i], bg[j][i]));
+        C::write(out, j, N, v[j]);
+#pragma unroll
+        for (int i = 0; i < kV; ++i)
+          v[j][i] = i < n[j] ? Cvt<T>::to_f(Cvt<T>::from_f(v[j][i])) : 0.0f;
+      }
+    }
+    const float2 ss = stats(v, sums[1]);
+    T* yr = static_cast<T*>(p.y) + row * N;
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j) {
+      if (n[j] > 0) {
+#pragma unroll
+        for (int i = 0; i < kV; ++i)
+          v[j][i] = fmaf((v[j][i] - ss.x) * ss.y, wn[j][i], bn[j][i]);
+        C::write(yr, j, N, v[j]);
+      }
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  copies_wait<0>();
+}
+
+// ---- backward ----
+struct BwdArgs {
+  const void *dy, *ds, *x, *s, *w1, *w2, *gate;
+  void *dx, *dres;
+  float* part;
+  int64_t M;
+  int N;
+  int64_t rows_per_group;
+  bool layer;
+  float eps, alpha;
+};
+
+// Column sums of one stretch of rows (one CTA, one group): kBias ? P, Q, R, S : P, R, rows of N.
+// Stretch (c, g) of CTA c and group g lies at index c + g, which grows from one
+// stretch to the next, so no two share an index.
+__device__ __forceinline__ float* stretch(float* part, int64_t c, int64_t g, int sums, int N) {
+  return part + (c + g) * sums * N;
+}
+
+template <typename T, typename W, int kThreads, int kPackets, int kStages, bool kAligned,
+          bool kBias>
+__global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
+  using C = Cols<T, kThreads, kPackets, kAligned>;
+  constexpr int kV = C::kV, kWarps = kThreads / 32, kSums = kBias ? 4 : 2;
+  extern __shared__ uint4 ring[];  // [stage][x, s, dy, ds][packet][thread]
+  __shared__ WarpSums<6, kWarps> first_sums[2];
+  __shared__ WarpSums<2, kWarps> second_sums[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, N = p.N;
+  const bool layer = p.layer;
+  const T *x = static_cast<const T*>(p.x), *s = static_cast<const T*>(p.s),
+          *dy = static_cast<const T*>(p.dy), *ds = static_cast<const T*>(p.ds);
+  const W *w1 = static_cast<const W*>(p.w1), *w2 = static_cast<const W*>(p.w2),
+          *gate = static_cast<const W*>(p.gate);
+  const int64_t row0 = first_row(p.M, blockIdx.x, gridDim.x),
+                end = first_row(p.M, blockIdx.x + 1, gridDim.x);
+  auto slot = [&](int stage, int tensor, int j) {
+    return ring + ((stage * 4 + tensor) * kPackets + j) * kThreads + threadIdx.x;
+  };
+  auto fetch = [&](int stage, int64_t row) {
+    if (row < end)
+#pragma unroll
+      for (int j = 0; j < kPackets; ++j) {
+        C::fetch(slot(stage, 0, j), x + row * N, j, N);
+        C::fetch(slot(stage, 1, j), s + row * N, j, N);
+        C::fetch(slot(stage, 2, j), dy + row * N, j, N);
+        if (ds) C::fetch(slot(stage, 3, j), ds + row * N, j, N);
+      }
+    copies_commit();
+  };
+#pragma unroll
+  for (int st = 0; st < kStages - 1; ++st) fetch(st, row0 + st);
+
+  int n[kPackets];
+  float wg[kPackets][kV], wn[kPackets][kV];
+  float P[kPackets][kV], R[kPackets][kV], Q[kBias ? kPackets : 1][kV], S[kBias ? kPackets : 1][kV];
+#pragma unroll
+  for (int j = 0; j < kPackets; ++j) {
+    n[j] = C::count(j, N);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+      wn[j][i] = i < n[j] ? Cvt<W>::to_f(w2[C::first(j) + i]) : 0.0f;
+      P[j][i] = R[j][i] = 0.0f;
+      if (kBias) Q[j][i] = S[j][i] = 0.0f;
+    }
+  }
+  const float inv_n = 1.0f / static_cast<float>(N);
+  const float mine = in_warp<C, kThreads, kPackets>(warp, N);
+  const float inv_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
+  const int from = lane < kWarps ? lane : 0;
+  const float theirs = in_warp<C, kThreads, kPackets>(from, N);
+  const float inv_theirs = theirs > 0.0f ? 1.0f / theirs : 0.0f;
+  auto from_lane0 = [](float v) { return __shfl_sync(0xffffffffu, v, 0); };
+  auto give = [&](int64_t g) {  // the column sums of the rows so far, which are of group g
+    float* to = stretch(p.part, blockIdx.x, g, kSums, N);
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+      for (int i = 0; i < kV; ++i)
+        if (i < n[j]) {
+          const int c = C::first(j) + i;
+          to[c] = P[j][i];
+          to[N + c] = R[j][i];
+          if (kBias) {
+            to[2 * N + c] = Q[j][i];
+            to[3 * N + c] = S[j][i];
+          }
+          P[j][i] = R[j][i] = 0.0f;
+          if (kBias) Q[j][i] = S[j][i] = 0.0f;
+        }
+  };
+
+  int stage = 0, par = 0;
+  int64_t group = row0 / p.rows_per_group, next_group = row0;
+  for (int64_t row = row0; row < end; ++row, par ^= 1) {
+    if (row >= next_group) {
+      if (row > row0) give(group);
+      group = row / p.rows_per_group;
+      next_group = (group + 1) * p.rows_per_group;
+#pragma unroll
+      for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          const int c = C::first(j) + i;
+          wg[j][i] = i < n[j] ? param(gate, group * N + c, 1.0f) * Cvt<W>::to_f(w1[c]) : 0.0f;
+        }
+    }
+    fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
+    copies_wait<kStages - 1>();
+    float xv[kPackets][kV], sv[kPackets][kV], fv[kPackets][kV];
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j) {
+      if (n[j] > 0) {
+        C::read(slot(stage, 0, j), xv[j]);
+        C::read(slot(stage, 1, j), sv[j]);
+        C::read(slot(stage, 2, j), fv[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) xv[j][i] = sv[j][i] = fv[j][i] = 0.0f;
+      }
+    }
+    // Statistics of x and s, and of f = dy w2 with the centred s: one exchange.
+    float mean_xw, mean_sw, F = 0.0f, Fs = 0.0f;
+    const Moments mx = warp_moments<kV, kPackets>(xv, n, layer, inv_mine, mean_xw);
+    const Moments ms = warp_moments<kV, kPackets>(sv, n, layer, inv_mine, mean_sw);
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const float f = fv[j][i] * wn[j][i];
+        F += f;
+        Fs = fmaf(f, sv[j][i] - mean_sw, Fs);
+      }
+    if (layer) F = warp_sum(F);
+    Fs = warp_sum(Fs);
+    WarpSums<6, kWarps>& buf = first_sums[par];
+    if (lane == 0) {
+      buf.v[0][warp] = mx.sum;
+      buf.v[1][warp] = mx.sq;
+      buf.v[2][warp] = ms.sum;
+      buf.v[3][warp] = ms.sq;
+      buf.v[4][warp] = F;
+      buf.v[5][warp] = Fs;
+    }
+    __syncthreads();
+    float mean_x = 0.0f, mean_s = 0.0f, mean_f = 0.0f;
+    float sqx = buf.v[1][from], sqs = buf.v[3][from], fs = buf.v[5][from];
+    if (layer) {
+      const float sum_x = buf.v[0][from], sum_s = buf.v[2][from], f = buf.v[4][from];
+      mean_x = over_warps<kWarps>(sum_x) * inv_n;
+      mean_s = over_warps<kWarps>(sum_s) * inv_n;
+      mean_f = from_lane0(over_warps<kWarps>(f)) * inv_n;
+      const float ex = sum_x * inv_theirs - mean_x, es = sum_s * inv_theirs - mean_s;
+      sqx = fmaf(theirs * ex, ex, sqx);
+      sqs = fmaf(theirs * es, es, sqs);
+      fs = fmaf(f, es, fs);
+      mean_x = from_lane0(mean_x);
+      mean_s = from_lane0(mean_s);
+    }
+    const float rx = 1.0f / sqrtf(from_lane0(over_warps<kWarps>(sqx)) * inv_n + p.eps);
+    const float rs = 1.0f / sqrtf(from_lane0(over_warps<kWarps>(sqs)) * inv_n + p.eps);
+    const float mean_fs = from_lane0(over_warps<kWarps>(fs)) * inv_n * rs;
+
+    // ds' and the sums for dx; xv becomes x^, sv becomes ds'.
+    T* dres = static_cast<T*>(p.dres) + row * N;
+    float E = 0.0f, Ex = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j) {
+      if (n[j] > 0) {
+        float t[kV], o[kV];
+        if (ds) {
+          C::read(slot(stage, 3, j), t);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kV; ++i) t[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          const bool in = kAligned || i < n[j];
+          const float hat = (sv[j][i] - mean_s) * rs, xh = (xv[j][i] - mean_x) * rx;
+          const float f = fv[j][i] * wn[j][i];
+          t[i] = in ? fmaf(rs, f - mean_f - hat * mean_fs, t[i]) : 0.0f;
+          R[j][i] = fmaf(fv[j][i], hat, R[j][i]);
+          P[j][i] = fmaf(t[i], xh, P[j][i]);
+          if (kBias) {
+            Q[j][i] += t[i];
+            S[j][i] += fv[j][i];
+          }
+          const float e = t[i] * wg[j][i];
+          E += e;
+          Ex = fmaf(e, xh, Ex);
+          o[i] = p.alpha * t[i];
+          xv[j][i] = xh;
+          sv[j][i] = e;
+        }
+        C::write(dres, j, N, o);
+      }
+    }
+    if (layer) E = warp_sum(E);
+    Ex = warp_sum(Ex);
+    WarpSums<2, kWarps>& buf2 = second_sums[par];
+    if (lane == 0) {
+      buf2.v[0][warp] = E;
+      buf2.v[1][warp] = Ex;
+    }
+    __syncthreads();
+    const float mean_e =
+        layer ? from_lane0(over_warps<kWarps>(buf2.v[0][from])) * inv_n : 0.0f;
+    const float mean_ex = from_lane0(over_warps<kWarps>(buf2.v[1][from])) * inv_n;
+    T* dx = static_cast<T*>(p.dx) + row * N;
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j) {
+      if (n[j] > 0) {
+        float o[kV];
+#pragma unroll
+        for (int i = 0; i < kV; ++i) o[i] = rx * (sv[j][i] - mean_e - xv[j][i] * mean_ex);
+        C::write(dx, j, N, o);
+      }
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  if (row0 < end) give(group);
+  copies_wait<0>();
+}
+
+// Gradients of the parameters from the column sums of the stretches, added in a fixed
+// order: 32 columns a CTA, kSlices threads a column.  With few groups the slices
+// share the stretches of each group; with many, each takes whole groups.
+constexpr int kSlices = 16;
+
+template <typename W>
+__global__ void __launch_bounds__(32 * kSlices)
+    sn_params(const float* part, const W* w1, const W* gate, const W* b1, W* dw1, W* dw2, W* dgate,
+              W* db1, W* db2, int64_t M, int N, int64_t G, int C, int sums) {
+  __shared__ float red[4][kSlices][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  const bool in = c < N;
+  const float w1c = in ? Cvt<W>::to_f(w1[c]) : 0.0f, b1c = in ? param(b1, c, 0.0f) : 0.0f;
+  const int64_t rpg = M / G;
+  const bool by_group = G >= kSlices;
+  // The CTA that has row r: the last one whose rows start at or before it.
+  auto cta_of = [&](int64_t r) {
+    int k = static_cast<int>(r * C / M);
+    while (k + 1 < C && first_row(M, k + 1, C) <= r) ++k;
+    while (first_row(M, k, C) > r) --k;
+    return k;
+  };
+  auto across = [&](float (&v)[4]) {  // sums over the slices, in every thread
+#pragma unroll
+    for (int q = 0; q < 4; ++q) red[q][slice][lane] = v[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v[q] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kSlices; ++i) v[q] += red[q][i][lane];
+    }
+    __syncthreads();
+  };
+  float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // dw1, dw2, db1, db2
+  for (int64_t g = by_group ? slice : 0; g < G; g += by_group ? kSlices : 1) {
+    const int c0 = cta_of(g * rpg), c1 = cta_of((g + 1) * rpg - 1);
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // P, R, Q, S
+    if (in)
+#pragma unroll 4
+      for (int k = c0 + (by_group ? 0 : slice); k <= c1; k += by_group ? 1 : kSlices) {
+        const float* p = part + (k + g) * sums * N + c;
+        v[0] += p[0];
+        v[1] += p[N];
+        if (sums == 4) {
+          v[2] += p[2 * static_cast<int64_t>(N)];
+          v[3] += p[3 * static_cast<int64_t>(N)];
+        }
+      }
+    if (!by_group) across(v);
+    const float ga = in ? param(gate, g * N + c, 1.0f) : 0.0f;
+    if (in && dgate && (by_group || slice == 0))
+      dgate[g * N + c] = Cvt<W>::from_f(w1c * v[0] + b1c * v[2]);
+    total[0] = fmaf(ga, v[0], total[0]);
+    total[1] += v[1];
+    total[2] = fmaf(ga, v[2], total[2]);
+    total[3] += v[3];
+  }
+  if (by_group) across(total);
+  if (in && slice == 0) {
+    dw1[c] = Cvt<W>::from_f(total[0]);
+    dw2[c] = Cvt<W>::from_f(total[1]);
+    if (db1) db1[c] = Cvt<W>::from_f(total[2]);
+    if (db2) db2[c] = Cvt<W>::from_f(total[3]);
+  }
+}
+
+// ---- rows too wide for a thread's registers ----
+// Passes over the row that read it again from L2.
 __device__ __forceinline__ float block_sum(float v, float* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nwarps = (blockDim.x + 31) >> 5;
@@ -37,11 +612,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   if (lane == 0) red[warp] = v;
   __syncthreads();
   return warp_sum(lane < nwarps ? red[lane] : 0.0f);
-}
-
-template <typename W>
-__device__ __forceinline__ float param(const W* p, int64_t i, float otherwise) {
-  return p ? Cvt<W>::to_f(p[i]) : otherwise;
 }
 
 // mean and rstd of a row read through `at`.
@@ -61,102 +631,92 @@ __device__ __forceinline__ float2 row_stats(F at, int64_t N, bool layer, float e
 }
 
 template <typename T, typename W>
-__global__ void __launch_bounds__(256)
-    sn_fwd_simple(const T* x, const T* res, const W* w1, const W* w2, const W* gate, const W* b1,
-                  const W* b2, T* y, T* res_out, int64_t N, int64_t rows_per_group, bool layer,
-                  float eps, float alpha) {
+__global__ void __launch_bounds__(1024) sn_fwd_wide(const FwdArgs p) {
   __shared__ float red[32];
-  const int64_t row = blockIdx.x, g = row / rows_per_group;
-  const T* xr = x + row * N;
-  T* sr = res_out + row * N;
+  const int64_t row = blockIdx.x, N = p.N, g = row / p.rows_per_group;
+  const T *xr = static_cast<const T*>(p.x) + row * N, *rr = static_cast<const T*>(p.res) + row * N;
+  const W *w1 = static_cast<const W*>(p.w1), *w2 = static_cast<const W*>(p.w2),
+          *gate = static_cast<const W*>(p.gate), *b1 = static_cast<const W*>(p.b1),
+          *b2 = static_cast<const W*>(p.b2);
+  T *sr = static_cast<T*>(p.res_out) + row * N, *yr = static_cast<T*>(p.y) + row * N;
   const float2 sx =
-      row_stats([&](int64_t c) { return Cvt<T>::to_f(xr[c]); }, N, layer, eps, red);
+      row_stats([&](int64_t c) { return Cvt<T>::to_f(xr[c]); }, N, p.layer, p.eps, red);
   for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-    const float p = (Cvt<T>::to_f(xr[c]) - sx.x) * sx.y * Cvt<W>::to_f(w1[c]) + param(b1, c, 0.0f);
-    sr[c] = Cvt<T>::from_f(fmaf(alpha, Cvt<T>::to_f(res[row * N + c]),
-                                param(gate, g * N + c, 1.0f) * p));
+    const float v = (Cvt<T>::to_f(xr[c]) - sx.x) * sx.y * Cvt<W>::to_f(w1[c]) + param(b1, c, 0.0f);
+    sr[c] = Cvt<T>::from_f(fmaf(p.alpha, Cvt<T>::to_f(rr[c]), param(gate, g * N + c, 1.0f) * v));
   }
   const float2 ss =
-      row_stats([&](int64_t c) { return Cvt<T>::to_f(sr[c]); }, N, layer, eps, red);
+      row_stats([&](int64_t c) { return Cvt<T>::to_f(sr[c]); }, N, p.layer, p.eps, red);
   for (int64_t c = threadIdx.x; c < N; c += blockDim.x)
-    y[row * N + c] = Cvt<T>::from_f((Cvt<T>::to_f(sr[c]) - ss.x) * ss.y * Cvt<W>::to_f(w2[c]) +
-                                    param(b2, c, 0.0f));
+    yr[c] = Cvt<T>::from_f((Cvt<T>::to_f(sr[c]) - ss.x) * ss.y * Cvt<W>::to_f(w2[c]) +
+                           param(b2, c, 0.0f));
 }
 
-struct RowStats {
-  float mean_x, rstd_x, mean_s, rstd_s, mean_f, mean_fs;
-};
-
-template <typename T, typename W>
-__global__ void __launch_bounds__(256)
-    sn_bwd_rows_simple(const T* dy, const T* ds, const T* x, const T* s, const W* w1, const W* w2,
-                       const W* gate, T* dx, T* dres, RowStats* stats, int64_t N,
-                       int64_t rows_per_group, bool layer, float eps, float alpha) {
+// One CTA a stretch of rows: each row's statistics, its outputs, then its share of the
+// column sums, which stay in the workspace (a thread adds to its own columns).
+template <typename T, typename W, bool kBias>
+__global__ void __launch_bounds__(1024) sn_bwd_wide(const BwdArgs p) {
+  constexpr int kSums = kBias ? 4 : 2;
   __shared__ float red[32];
-  const int64_t row = blockIdx.x, g = row / rows_per_group, o = row * N;
+  const int64_t N = p.N;
+  const T *x = static_cast<const T*>(p.x), *s = static_cast<const T*>(p.s),
+          *dy = static_cast<const T*>(p.dy), *ds = static_cast<const T*>(p.ds);
+  const W *w1 = static_cast<const W*>(p.w1), *w2 = static_cast<const W*>(p.w2),
+          *gate = static_cast<const W*>(p.gate);
   const float inv_n = 1.0f / static_cast<float>(N);
-  const float2 sx = row_stats([&](int64_t c) { return Cvt<T>::to_f(x[o + c]); }, N, layer, eps, red);
-  const float2 ss = row_stats([&](int64_t c) { return Cvt<T>::to_f(s[o + c]); }, N, layer, eps, red);
-  float f0 = 0.0f, f1 = 0.0f;
-  for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-    const float f = Cvt<T>::to_f(dy[o + c]) * Cvt<W>::to_f(w2[c]);
-    f0 += f;
-    f1 += f * (Cvt<T>::to_f(s[o + c]) - ss.x) * ss.y;
-  }
-  const float mf = layer ? block_sum(f0, red) * inv_n : 0.0f, mfs = block_sum(f1, red) * inv_n;
-  auto total = [&](int64_t c) {
-    const float hat = (Cvt<T>::to_f(s[o + c]) - ss.x) * ss.y;
-    const float f = Cvt<T>::to_f(dy[o + c]) * Cvt<W>::to_f(w2[c]);
-    return (ds ? Cvt<T>::to_f(ds[o + c]) : 0.0f) + ss.y * (f - mf - hat * mfs);
-  };
-  float e0 = 0.0f, e1 = 0.0f;
-  for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-    const float e = total(c) * param(gate, g * N + c, 1.0f) * Cvt<W>::to_f(w1[c]);
-    e0 += e;
-    e1 += e * (Cvt<T>::to_f(x[o + c]) - sx.x) * sx.y;
-  }
-  const float me = layer ? block_sum(e0, red) * inv_n : 0.0f, mex = block_sum(e1, red) * inv_n;
-  for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-    const float t = total(c), e = t * param(gate, g * N + c, 1.0f) * Cvt<W>::to_f(w1[c]);
-    dres[o + c] = Cvt<T>::from_f(alpha * t);
-    dx[o + c] = Cvt<T>::from_f(sx.y * (e - me - (Cvt<T>::to_f(x[o + c]) - sx.x) * sx.y * mex));
-  }
-  if (threadIdx.x == 0) stats[row] = RowStats{sx.x, sx.y, ss.x, ss.y, mf, mfs};
-}
-
-template <typename T, typename W>
-__global__ void __launch_bounds__(128)
-    sn_bwd_cols_simple(const T* dy, const T* ds, const T* x, const T* s, const W* w1, const W* w2,
-                       const W* gate, const W* b1, const RowStats* stats, W* dw1, W* dw2, W* dgate,
-                       W* db1, W* db2, int64_t M, int64_t N, int64_t G) {
-  const int64_t c = blockIdx.x * 128ll + threadIdx.x;
-  if (c >= N) return;
-  const float w1c = Cvt<W>::to_f(w1[c]), w2c = Cvt<W>::to_f(w2[c]), b1c = param(b1, c, 0.0f);
-  float aw1 = 0.0f, ab1 = 0.0f, R = 0.0f, S = 0.0f;
-  for (int64_t g = 0; g < G; ++g) {
-    float P = 0.0f, Q = 0.0f;
-    for (int64_t row = g * (M / G); row < (g + 1) * (M / G); ++row) {
-      const RowStats st = stats[row];
-      const float dyv = Cvt<T>::to_f(dy[row * N + c]);
-      const float hat = (Cvt<T>::to_f(s[row * N + c]) - st.mean_s) * st.rstd_s;
-      const float t = (ds ? Cvt<T>::to_f(ds[row * N + c]) : 0.0f) +
-                      st.rstd_s * (dyv * w2c - st.mean_f - hat * st.mean_fs);
-      P = fmaf(t, (Cvt<T>::to_f(x[row * N + c]) - st.mean_x) * st.rstd_x, P);
-      Q += t;
-      R = fmaf(dyv, hat, R);
-      S += dyv;
+  const int64_t row0 = first_row(p.M, blockIdx.x, gridDim.x),
+                end = first_row(p.M, blockIdx.x + 1, gridDim.x);
+  int64_t group = -1;
+  for (int64_t row = row0; row < end; ++row) {
+    const int64_t g = row / p.rows_per_group, o = row * N;
+    float* to = stretch(p.part, blockIdx.x, g, kSums, p.N);
+    if (g != group)
+      for (int64_t c = threadIdx.x; c < N; c += blockDim.x)
+        for (int q = 0; q < kSums; ++q) to[q * N + c] = 0.0f;
+    group = g;
+    const float2 sx =
+        row_stats([&](int64_t c) { return Cvt<T>::to_f(x[o + c]); }, N, p.layer, p.eps, red);
+    const float2 ss =
+        row_stats([&](int64_t c) { return Cvt<T>::to_f(s[o + c]); }, N, p.layer, p.eps, red);
+    float f0 = 0.0f, f1 = 0.0f;
+    for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
+      const float f = Cvt<T>::to_f(dy[o + c]) * Cvt<W>::to_f(w2[c]);
+      f0 += f;
+      f1 = fmaf(f, (Cvt<T>::to_f(s[o + c]) - ss.x) * ss.y, f1);
     }
-    const float gc = param(gate, g * N + c, 1.0f);
-    if (dgate) dgate[g * N + c] = Cvt<W>::from_f(w1c * P + b1c * Q);
-    aw1 = fmaf(gc, P, aw1);
-    ab1 = fmaf(gc, Q, ab1);
+    const float mf = p.layer ? block_sum(f0, red) * inv_n : 0.0f;
+    const float mfs = block_sum(f1, red) * inv_n;
+    float e0 = 0.0f, e1 = 0.0f;
+    for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
+      const float hat = (Cvt<T>::to_f(s[o + c]) - ss.x) * ss.y, dyv = Cvt<T>::to_f(dy[o + c]);
+      const float xh = (Cvt<T>::to_f(x[o + c]) - sx.x) * sx.y;
+      const float t = (ds ? Cvt<T>::to_f(ds[o + c]) : 0.0f) +
+                      ss.y * (dyv * Cvt<W>::to_f(w2[c]) - mf - hat * mfs);
+      to[c] = fmaf(t, xh, to[c]);
+      to[N + c] = fmaf(dyv, hat, to[N + c]);
+      if (kBias) {
+        to[2 * N + c] += t;
+        to[3 * N + c] += dyv;
+      }
+      const float e = t * param(gate, g * N + c, 1.0f) * Cvt<W>::to_f(w1[c]);
+      e0 += e;
+      e1 = fmaf(e, xh, e1);
+    }
+    const float me = p.layer ? block_sum(e0, red) * inv_n : 0.0f;
+    const float mex = block_sum(e1, red) * inv_n;
+    for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
+      const float hat = (Cvt<T>::to_f(s[o + c]) - ss.x) * ss.y;
+      const float t = (ds ? Cvt<T>::to_f(ds[o + c]) : 0.0f) +
+                      ss.y * (Cvt<T>::to_f(dy[o + c]) * Cvt<W>::to_f(w2[c]) - mf - hat * mfs);
+      const float e = t * param(gate, g * N + c, 1.0f) * Cvt<W>::to_f(w1[c]);
+      static_cast<T*>(p.dres)[o + c] = Cvt<T>::from_f(p.alpha * t);
+      static_cast<T*>(p.dx)[o + c] = Cvt<T>::from_f(
+          sx.y * (e - me - (Cvt<T>::to_f(x[o + c]) - sx.x) * sx.y * mex));
+    }
   }
-  dw1[c] = Cvt<W>::from_f(aw1);
-  dw2[c] = Cvt<W>::from_f(R);
-  if (db1) db1[c] = Cvt<W>::from_f(ab1);
-  if (db2) db2[c] = Cvt<W>::from_f(S);
 }
 
+// ---- launches ----
 // Calls f with values of the row type and the parameter type.
 template <typename F>
 int with_types(int dtype, int affine_dtype, F f) {
@@ -172,7 +732,54 @@ int with_types(int dtype, int affine_dtype, F f) {
 }
 
 bool bad_shape(int64_t M, int64_t N, int64_t G) {
-  return M < 0 || N <= 0 || G < 1 || M > 0x7fffffffLL || N > 0x7fffffffLL || M % G != 0;
+  return M < 0 || N <= 0 || G < 1 || M > 0x7fffffffLL || N > 0x3fffffffLL || M % G != 0;
+}
+
+template <typename A>
+int launch_rows(void (*kernel)(const A), int threads, size_t smem, int64_t ctas, const A& args,
+                cudaStream_t s) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem)) != cudaSuccess)
+    return TILEOPS_ELAUNCH;
+  kernel<<<static_cast<unsigned>(ctas), threads, smem, s>>>(args);
+  return launch_status();
+}
+
+// CTAs of the backward pass: one an SM.  Its registers allow no second one, and each
+// adds a stretch of column sums to write and read.
+int64_t bwd_ctas(int64_t M) { return std::min<int64_t>(M, sm_count()); }
+constexpr int kMaxCtas = 512;  // workspace: more SMs than any device of this architecture has
+
+template <typename T, typename W, bool kAligned>
+int launch_fwd(const FwdArgs& a, cudaStream_t s) {
+  const int64_t packets = (a.N + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+  // per: CTAs an SM that fit; more rows ahead where a row is short.
+  auto go = [&](auto kernel, int threads, int per_thread, int stages, int per) {
+    return launch_rows(kernel, threads, static_cast<size_t>(stages) * 2 * per_thread * threads * 16,
+                       std::min<int64_t>(a.M, static_cast<int64_t>(sm_count()) * per), a, s);
+  };
+  if (packets <= 64) return go(sn_fwd<T, W, 64, 1, 8, kAligned>, 64, 1, 8, 12);
+  if (packets <= 128) return go(sn_fwd<T, W, 128, 1, 6, kAligned>, 128, 1, 6, 6);
+  if (packets <= 256) return go(sn_fwd<T, W, 256, 1, 4, kAligned>, 256, 1, 4, 3);
+  if (packets <= 512) return go(sn_fwd<T, W, 256, 2, 4, kAligned>, 256, 2, 4, 2);
+  if (packets <= 1024) return go(sn_fwd<T, W, 512, 2, 3, kAligned>, 512, 2, 3, 1);
+  sn_fwd_wide<T, W><<<static_cast<unsigned>(a.M), 1024, 0, s>>>(a);
+  return launch_status();
+}
+
+template <typename T, typename W, bool kAligned, bool kBias>
+int launch_bwd(const BwdArgs& a, int64_t ctas, cudaStream_t s) {
+  const int64_t packets = (a.N + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+  auto go = [&](auto kernel, int threads, int per_thread, int stages) {
+    return launch_rows(kernel, threads, static_cast<size_t>(stages) * 4 * per_thread * threads * 16,
+                       ctas, a, s);
+  };
+  if (packets <= 128) return go(sn_bwd<T, W, 128, 1, 6, kAligned, kBias>, 128, 1, 6);
+  if (packets <= 256) return go(sn_bwd<T, W, 256, 1, 5, kAligned, kBias>, 256, 1, 5);
+  if (packets <= 512) return go(sn_bwd<T, W, 512, 1, 4, kAligned, kBias>, 512, 1, 4);
+  if (packets <= 1024) return go(sn_bwd<T, W, 512, 2, 3, kAligned, kBias>, 512, 2, 3);
+  sn_bwd_wide<T, W, kBias><<<static_cast<unsigned>(ctas), 1024, 0, s>>>(a);
+  return launch_status();
 }
 
 }  // namespace
@@ -192,25 +799,24 @@ extern "C" int tileops_sandwich_norm_fwd(const void* x, const void* residual,
   if (M == 0) return TILEOPS_OK;
   if (!x || !residual || !post_weight || !pre_weight || !y || !residual_out)
     return TILEOPS_EINVAL;
+  const FwdArgs args{x, residual, post_weight, pre_weight, gate, post_bias, pre_bias, y,
+                     residual_out, M, static_cast<int>(N), M / gate_rows,
+                     norm == TILEOPS_NORM_LAYER, static_cast<float>(eps),
+                     static_cast<float>(residual_scale)};
   return with_types(dtype, affine_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
-    sn_fwd_simple<T, W><<<static_cast<unsigned>(M), 256, 0, as_stream(stream)>>>(
-        static_cast<const T*>(x), static_cast<const T*>(residual),
-        static_cast<const W*>(post_weight), static_cast<const W*>(pre_weight),
-        static_cast<const W*>(gate), static_cast<const W*>(post_bias),
-        static_cast<const W*>(pre_bias), static_cast<T*>(y), static_cast<T*>(residual_out), N,
-        M / gate_rows, norm == TILEOPS_NORM_LAYER, static_cast<float>(eps),
-        static_cast<float>(residual_scale));
-    return launch_status();
+    const bool aligned = N * sizeof(T) % 16 == 0 && aligned16(x) && aligned16(residual) &&
+                         aligned16(y) && aligned16(residual_out);
+    return aligned ? launch_fwd<T, W, true>(args, as_stream(stream))
+                   : launch_fwd<T, W, false>(args, as_stream(stream));
   });
 }
 
 extern "C" int64_t tileops_sandwich_norm_bwd_workspace_bytes(int64_t M, int64_t N,
                                                              int64_t gate_rows, int has_bias) {
-  (void)has_bias;
   if (bad_shape(M, N, gate_rows)) return -1;
-  return M * static_cast<int64_t>(sizeof(RowStats));
+  return (std::min<int64_t>(M, kMaxCtas) + gate_rows) * (has_bias ? 4 : 2) * N * 4;
 }
 
 extern "C" int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_out, const void* x,
@@ -230,21 +836,34 @@ extern "C" int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_
       (d_post_bias && !post_bias))
     return TILEOPS_EINVAL;
   cudaStream_t st = as_stream(stream);
+  // The gate's gradient takes Q when there is a post_bias, whether or not that has one.
+  const bool bias = post_bias || d_pre_bias;
+  float* part = static_cast<float*>(workspace);
+  const BwdArgs args{dy, d_residual_out, x, residual_out, post_weight, pre_weight, gate, dx,
+                     d_residual, part, M, static_cast<int>(N), M / gate_rows,
+                     norm == TILEOPS_NORM_LAYER, static_cast<float>(eps),
+                     static_cast<float>(residual_scale)};
+  const int64_t ctas = std::min<int64_t>(bwd_ctas(M), kMaxCtas);
   return with_types(dtype, affine_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
-    RowStats* stats = static_cast<RowStats*>(workspace);
-    auto in = [](const void* p) { return static_cast<const T*>(p); };
+    const bool aligned = N * sizeof(T) % 16 == 0 && aligned16(dy) && aligned16(d_residual_out) &&
+                         aligned16(x) && aligned16(residual_out) && aligned16(dx) &&
+                         aligned16(d_residual);
+    int status;
+    if (aligned)
+      status = bias ? launch_bwd<T, W, true, true>(args, ctas, st)
+                    : launch_bwd<T, W, true, false>(args, ctas, st);
+    else
+      status = bias ? launch_bwd<T, W, false, true>(args, ctas, st)
+                    : launch_bwd<T, W, false, false>(args, ctas, st);
+    if (status != TILEOPS_OK) return status;
     auto par = [](const void* p) { return static_cast<const W*>(p); };
     auto out = [](void* p) { return static_cast<W*>(p); };
-    sn_bwd_rows_simple<T, W><<<static_cast<unsigned>(M), 256, 0, st>>>(
-        in(dy), in(d_residual_out), in(x), in(residual_out), par(post_weight), par(pre_weight),
-        par(gate), static_cast<T*>(dx), static_cast<T*>(d_residual), stats, N, M / gate_rows,
-        norm == TILEOPS_NORM_LAYER, static_cast<float>(eps), static_cast<float>(residual_scale));
-    sn_bwd_cols_simple<T, W><<<static_cast<unsigned>((N + 127) / 128), 128, 0, st>>>(
-        in(dy), in(d_residual_out), in(x), in(residual_out), par(post_weight), par(pre_weight),
-        par(gate), par(post_bias), stats, out(d_post_weight), out(d_pre_weight), out(d_gate),
-        out(d_post_bias), out(d_pre_bias), M, N, gate_rows);
+    sn_params<W><<<static_cast<unsigned>((N + 31) / 32), 32 * kSlices, 0, st>>>(
+        part, par(post_weight), par(gate), par(post_bias), out(d_post_weight), out(d_pre_weight),
+        out(d_gate), out(d_post_bias), out(d_pre_bias), M, static_cast<int>(N), gate_rows,
+        static_cast<int>(ctas), bias ? 4 : 2);
     return launch_status();
   });
 }
