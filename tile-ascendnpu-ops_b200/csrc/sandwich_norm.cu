@@ -26,6 +26,7 @@
 // there, and joined (Chan, Golub & LeVeque, "Updating formulae and a
 // pairwise algorithm for computing sample variances", 1979).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -63,8 +64,9 @@ __device__ __forceinline__ void copies_wait() {
 template <typename T, int kThreads, int kPackets, bool kAligned>
 struct Cols {
   static constexpr int kV = 16 / sizeof(T);
+  static constexpr bool kWhole = kAligned;
   static __device__ __forceinline__ int first(int j) { return (threadIdx.x + j * kThreads) * kV; }
-  // How many elements packet j has.
+  // How many elements packet j has (all or none of an aligned row).
   static __device__ __forceinline__ int count(int j, int N) {
     const int left = N - first(j);
     return kAligned ? (left > 0 ? kV : 0) : max(0, min(kV, left));
@@ -80,22 +82,58 @@ struct Cols {
       memcpy(slot, e, 16);
     }
   }
-  static __device__ __forceinline__ void read(const uint4* slot, float* v) {
-    T e[kV];
+  // Two neighbouring columns at a time: the arithmetic is packed (fma.rn.f32x2 and its kin).
+  static constexpr int kP = kV / 2;
+  static __device__ __forceinline__ void read(const uint4* slot, float2 (&v)[kP]) {
     const uint4 u = *slot;
-    memcpy(e, &u, 16);
-#pragma unroll
-    for (int i = 0; i < kV; ++i) v[i] = Cvt<T>::to_f(e[i]);
-  }
-  static __device__ __forceinline__ void write(T* row, int j, int N, const float* v) {
-    T e[kV];
-#pragma unroll
-    for (int i = 0; i < kV; ++i) e[i] = Cvt<T>::from_f(v[i]);
-    if constexpr (kAligned) {
-      uint4 u;
-      memcpy(&u, e, 16);
-      if (first(j) < N) st_stream(row + first(j), u);
+    if constexpr (sizeof(T) == 4) {
+      v[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+      v[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
     } else {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = unpack(w[i]);
+    }
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    if constexpr (std::is_same_v<T, __half>) {
+      __half2 h;
+      memcpy(&h, &w, 4);
+      return __half22float2(h);
+    } else {
+      return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+  }
+  static __device__ __forceinline__ uint32_t pack(float2 v) {
+    uint32_t w;
+    if constexpr (std::is_same_v<T, __half>) {
+      const __half2 h = __float22half2_rn(v);
+      memcpy(&w, &h, 4);
+    } else {
+      const __nv_bfloat162 h = __float22bfloat162_rn(v);
+      memcpy(&w, &h, 4);
+    }
+    return w;
+  }
+  // v rounded to T, as it will be read again.
+  static __device__ __forceinline__ void round(float2 (&v)[kP]) {
+    if constexpr (sizeof(T) == 2)
+#pragma unroll
+      for (int i = 0; i < kP; ++i) v[i] = unpack(pack(v[i]));
+  }
+  static __device__ __forceinline__ void write(T* row, int j, int N, const float2 (&v)[kP]) {
+    uint4 u;
+    if constexpr (sizeof(T) == 4) {
+      u = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x),
+                     __float_as_uint(v[1].y));
+    } else {
+      u = make_uint4(pack(v[0]), pack(v[1]), pack(v[2]), pack(v[3]));
+    }
+    if constexpr (kAligned) {
+      st_stream(row + first(j), u);
+    } else {
+      T e[kV];
+      memcpy(e, &u, 16);
       const int n = count(j, N);
 #pragma unroll
       for (int i = 0; i < kV; ++i)
@@ -104,20 +142,24 @@ struct Cols {
   }
 };
 
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float total(float2 v) { return v.x + v.y; }
+
 // Rows of CTA c of C: consecutive, so that a CTA meets few gate groups.
 __device__ __forceinline__ int first_row(int64_t M, int c, int C) {
   return static_cast<int>(M * c / C);
 }
 
 // ---- statistics of a row over a CTA, one barrier ----
-// Each warp publishes kSums numbers; after the barrier lane l holds warp l's and
-// the sums over warps are butterflies.  Callers alternate two buffers: one is
+// Each warp publishes kSums numbers; after the barrier lane l takes those of warp
+// l % kWarps and the sums over warps are butterflies.  Callers alternate two buffers: one is
 // written again only after a barrier that every reader of it has passed.
 template <int kSums, int kWarps>
 struct WarpSums {
   float v[kSums][kWarps];
 };
 
+// Sum over the warps of what lane l holds of warp l % kWarps; in every lane.
 template <int kWarps>
 __device__ __forceinline__ float over_warps(float v) {
 #pragma unroll
@@ -142,29 +184,52 @@ __device__ __forceinline__ float in_warp(int w, int N) {
 struct Moments {
   float sum, sq;
 };
-template <int kV, int kPackets>
-__device__ __forceinline__ Moments warp_moments(const float (&v)[kPackets][kV],
+template <typename C, int kPackets>
+__device__ __forceinline__ Moments warp_moments(const float2 (&v)[kPackets][C::kP],
                                                 const int (&n)[kPackets], bool layer,
                                                 float inv_in_warp, float& mean) {
   Moments m{0.0f, 0.0f};
   mean = 0.0f;
+  float2 sq = both(0.0f);
   if (layer) {
+    float2 sum = both(0.0f);
 #pragma unroll
     for (int j = 0; j < kPackets; ++j)
 #pragma unroll
-      for (int i = 0; i < kV; ++i) m.sum += v[j][i];  // zeros past the end
-    m.sum = warp_sum(m.sum);
+      for (int i = 0; i < C::kP; ++i) sum = fadd2(sum, v[j][i]);  // zeros past the end
+    m.sum = warp_sum(total(sum));
     mean = m.sum * inv_in_warp;
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j)
+      if (n[j] > 0)
+#pragma unroll
+        for (int i = 0; i < C::kP; ++i) {
+          float2 d = fadd2(v[j][i], both(-mean));
+          if (!C::kWhole && 2 * i >= n[j]) d.x = 0.0f;
+          if (!C::kWhole && 2 * i + 1 >= n[j]) d.y = 0.0f;
+          sq = ffma2(d, d, sq);
+        }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+      for (int i = 0; i < C::kP; ++i) sq = ffma2(v[j][i], v[j][i], sq);
   }
+  m.sq = warp_sum(total(sq));
+  return m;
+}
+
+// Parameters of a thread's columns (zero where there are none).
+template <typename C, typename W, int kPackets, typename F>
+__device__ __forceinline__ void load_params(float2 (&v)[kPackets][C::kP], const int (&n)[kPackets],
+                                            F at) {
 #pragma unroll
   for (int j = 0; j < kPackets; ++j)
 #pragma unroll
-    for (int i = 0; i < kV; ++i) {
-      const float d = i < n[j] ? v[j][i] - mean : 0.0f;
-      m.sq = fmaf(d, d, m.sq);
+    for (int i = 0; i < C::kP; ++i) {
+      const int c = C::first(j) + 2 * i;
+      v[j][i] = make_float2(2 * i < n[j] ? at(c) : 0.0f, 2 * i + 1 < n[j] ? at(c + 1) : 0.0f);
     }
-  m.sq = warp_sum(m.sq);
-  return m;
 }
 
 // ---- forward ----
@@ -181,7 +246,7 @@ struct FwdArgs {
 template <typename T, typename W, int kThreads, int kPackets, int kStages, bool kAligned>
 __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
   using C = Cols<T, kThreads, kPackets, kAligned>;
-  constexpr int kV = C::kV, kWarps = kThreads / 32;
+  constexpr int kP = C::kP, kWarps = kThreads / 32;
   extern __shared__ uint4 ring[];  // [stage][x, residual][packet][thread]
   __shared__ WarpSums<2, kWarps> sums[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, N = p.N;
@@ -208,46 +273,36 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
   for (int s = 0; s < kStages - 1; ++s) fetch(s, row0 + s);
 
   int n[kPackets];
-  float wg[kPackets][kV], bg[kPackets][kV], wn[kPackets][kV], bn[kPackets][kV];
 #pragma unroll
-  for (int j = 0; j < kPackets; ++j) {
-    n[j] = C::count(j, N);
-#pragma unroll
-    for (int i = 0; i < kV; ++i) {
-      const int c = C::first(j) + i;
-      const bool in = i < n[j];
-      wn[j][i] = in ? Cvt<W>::to_f(w2[c]) : 0.0f;
-      bn[j][i] = in ? param(b2, c, 0.0f) : 0.0f;
-    }
-  }
+  for (int j = 0; j < kPackets; ++j) n[j] = C::count(j, N);
+  float2 wg[kPackets][kP], bg[kPackets][kP], wn[kPackets][kP], bn[kPackets][kP];
+  load_params<C, W, kPackets>(wn, n, [&](int c) { return Cvt<W>::to_f(w2[c]); });
+  load_params<C, W, kPackets>(bn, n, [&](int c) { return param(b2, c, 0.0f); });
   const float inv_n = 1.0f / static_cast<float>(N);
   const float mine = in_warp<C, kThreads, kPackets>(warp, N);
   const float inv_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
-  const int from = lane < kWarps ? lane : 0;  // the warp whose sums this lane joins
+  const int from = lane % kWarps;  // the warp whose sums this lane joins
   const float theirs = in_warp<C, kThreads, kPackets>(from, N);
   const float inv_theirs = theirs > 0.0f ? 1.0f / theirs : 0.0f;
 
   // mean and 1 / deviation of the row held in v.
-  auto stats = [&](const float(&v)[kPackets][kV], WarpSums<2, kWarps>& buf) {
+  auto stats = [&](const float2(&v)[kPackets][kP], WarpSums<2, kWarps>& buf) {
     float warp_mean;
-    const Moments m = warp_moments<kV, kPackets>(v, n, layer, inv_mine, warp_mean);
+    const Moments m = warp_moments<C, kPackets>(v, n, layer, inv_mine, warp_mean);
     if (lane == 0) {
       buf.v[0][warp] = m.sum;
       buf.v[1][warp] = m.sq;
     }
     __syncthreads();
-    const float sum = buf.v[0][from];
     float sq = buf.v[1][from], mean = 0.0f;
     if (layer) {
+      const float sum = buf.v[0][from];
       mean = over_warps<kWarps>(sum) * inv_n;
       const float d = sum * inv_theirs - mean;
       sq = fmaf(theirs * d, d, sq);
     }
-    sq = over_warps<kWarps>(sq);
-    // lanes beyond the warps hold copies of warp 0's sums: take lane 0's result
-    mean = __shfl_sync(0xffffffffu, mean, 0);
-    sq = __shfl_sync(0xffffffffu, sq, 0);
-    return make_float2(mean, 1.0f / sqrtf(sq * inv_n + p.eps));
+    const float rstd = rsqrtf(fmaf(over_warps<kWarps>(sq), inv_n, p.eps));
+    return make_float2(mean, rstd);
   };
 
   int stage = 0;
@@ -256,42 +311,38 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
     if (row >= next_group) {
       const int64_t g = row / p.rows_per_group;
       next_group = (g + 1) * p.rows_per_group;
-#pragma unroll
-      for (int j = 0; j < kPackets; ++j)
-#pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          const int c = C::first(j) + i;
-          const bool in = i < n[j];
-          const float ga = in ? param(gate, g * N + c, 1.0f) : 0.0f;
-          wg[j][i] = in ? ga * Cvt<W>::to_f(w1[c]) : 0.0f;
-          bg[j][i] = in ? ga * param(b1, c, 0.0f) : 0.0f;
-        }
+      auto gate_at = [&](int c) { return param(gate, g * N + c, 1.0f); };
+      load_params<C, W, kPackets>(wg, n, [&](int c) { return gate_at(c) * Cvt<W>::to_f(w1[c]); });
+      load_params<C, W, kPackets>(bg, n, [&](int c) { return gate_at(c) * param(b1, c, 0.0f); });
     }
     fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
     copies_wait<kStages - 1>();
-    float v[kPackets][kV];
+    float2 v[kPackets][kP];
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0)
         C::read(slot(stage, 0, j), v[j]);
       else
 #pragma unroll
-        for (int i = 0; i < kV; ++i) v[j][i] = 0.0f;
+        for (int i = 0; i < kP; ++i) v[j][i] = both(0.0f);
     }
     const float2 sx = stats(v, sums[0]);
     T* out = static_cast<T*>(p.res_out) + row * N;
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
-        float r[kV];
+        float2 r[kP];
         C::read(slot(stage, 1, j), r);
 #pragma unroll
-        for (int i = 0; i < kV; ++i)
-          v[j][i] = fmaf(p.alpha, r[i], fmaf((v[j][i] - sx.x) * sx.y, wg[j][i], bg[j][i]));
+        for (int i = 0; i < kP; ++i) {
+          // (v - mean) first: v rstd - mean rstd would cancel where the mean is large
+          const float2 hat = fmul2(fadd2(v[j][i], both(-sx.x)), both(sx.y));
+          v[j][i] = ffma2(both(p.alpha), r[i], ffma2(hat, wg[j][i], bg[j][i]));
+          if (!kAligned && 2 * i >= n[j]) v[j][i].x = 0.0f;
+          if (!kAligned && 2 * i + 1 >= n[j]) v[j][i].y = 0.0f;
+        }
         C::write(out, j, N, v[j]);
-#pragma unroll
-        for (int i = 0; i < kV; ++i)
-          v[j][i] = i < n[j] ? Cvt<T>::to_f(Cvt<T>::from_f(v[j][i])) : 0.0f;
+        C::round(v[j]);
       }
     }
     const float2 ss = stats(v, sums[1]);
@@ -300,8 +351,8 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
 #pragma unroll
-        for (int i = 0; i < kV; ++i)
-          v[j][i] = fmaf((v[j][i] - ss.x) * ss.y, wn[j][i], bn[j][i]);
+        for (int i = 0; i < kP; ++i)
+          v[j][i] = ffma2(fmul2(fadd2(v[j][i], both(-ss.x)), both(ss.y)), wn[j][i], bn[j][i]);
         C::write(yr, j, N, v[j]);
       }
     }
@@ -333,7 +384,7 @@ template <typename T, typename W, int kThreads, int kPackets, int kStages, bool 
           bool kBias>
 __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
   using C = Cols<T, kThreads, kPackets, kAligned>;
-  constexpr int kV = C::kV, kWarps = kThreads / 32, kSums = kBias ? 4 : 2;
+  constexpr int kP = C::kP, kWarps = kThreads / 32, kSums = kBias ? 4 : 2;
   extern __shared__ uint4 ring[];  // [stage][x, s, dy, ds][packet][thread]
   __shared__ WarpSums<6, kWarps> first_sums[2];
   __shared__ WarpSums<2, kWarps> second_sums[2];
@@ -363,42 +414,46 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
   for (int st = 0; st < kStages - 1; ++st) fetch(st, row0 + st);
 
   int n[kPackets];
-  float wg[kPackets][kV], wn[kPackets][kV];
-  float P[kPackets][kV], R[kPackets][kV], Q[kBias ? kPackets : 1][kV], S[kBias ? kPackets : 1][kV];
 #pragma unroll
-  for (int j = 0; j < kPackets; ++j) {
-    n[j] = C::count(j, N);
-#pragma unroll
-    for (int i = 0; i < kV; ++i) {
-      wn[j][i] = i < n[j] ? Cvt<W>::to_f(w2[C::first(j) + i]) : 0.0f;
-      P[j][i] = R[j][i] = 0.0f;
-      if (kBias) Q[j][i] = S[j][i] = 0.0f;
-    }
-  }
-  const float inv_n = 1.0f / static_cast<float>(N);
-  const float mine = in_warp<C, kThreads, kPackets>(warp, N);
-  const float inv_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
-  const int from = lane < kWarps ? lane : 0;
-  const float theirs = in_warp<C, kThreads, kPackets>(from, N);
-  const float inv_theirs = theirs > 0.0f ? 1.0f / theirs : 0.0f;
-  auto from_lane0 = [](float v) { return __shfl_sync(0xffffffffu, v, 0); };
-  auto give = [&](int64_t g) {  // the column sums of the rows so far, which are of group g
-    float* to = stretch(p.part, blockIdx.x, g, kSums, N);
+  for (int j = 0; j < kPackets; ++j) n[j] = C::count(j, N);
+  float2 wg[kPackets][kP], wn[kPackets][kP];
+  float2 P[kPackets][kP], R[kPackets][kP], Q[kBias ? kPackets : 1][kP], S[kBias ? kPackets : 1][kP];
+  load_params<C, W, kPackets>(wn, n, [&](int c) { return Cvt<W>::to_f(w2[c]); });
+  auto clear = [&] {
 #pragma unroll
     for (int j = 0; j < kPackets; ++j)
 #pragma unroll
-      for (int i = 0; i < kV; ++i)
-        if (i < n[j]) {
-          const int c = C::first(j) + i;
-          to[c] = P[j][i];
-          to[N + c] = R[j][i];
-          if (kBias) {
-            to[2 * N + c] = Q[j][i];
-            to[3 * N + c] = S[j][i];
-          }
-          P[j][i] = R[j][i] = 0.0f;
-          if (kBias) Q[j][i] = S[j][i] = 0.0f;
+      for (int i = 0; i < kP; ++i) {
+        P[j][i] = R[j][i] = both(0.0f);
+        if (kBias) Q[j][i] = S[j][i] = both(0.0f);
+      }
+  };
+  clear();
+  const float inv_n = 1.0f / static_cast<float>(N);
+  const float mine = in_warp<C, kThreads, kPackets>(warp, N);
+  const float inv_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
+  const int from = lane % kWarps;
+  const float theirs = in_warp<C, kThreads, kPackets>(from, N);
+  const float inv_theirs = theirs > 0.0f ? 1.0f / theirs : 0.0f;
+  auto give = [&](int64_t g) {  // the column sums of the rows so far, which are of group g
+    float* to = stretch(p.part, blockIdx.x, g, kSums, N);
+    auto put = [&](int which, const float2& v, int c, int left) {
+      if (left > 0) to[which * static_cast<int64_t>(N) + c] = v.x;
+      if (left > 1) to[which * static_cast<int64_t>(N) + c + 1] = v.y;
+    };
+#pragma unroll
+    for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        const int c = C::first(j) + 2 * i, left = n[j] - 2 * i;
+        put(0, P[j][i], c, left);
+        put(1, R[j][i], c, left);
+        if (kBias) {
+          put(2, Q[j][i], c, left);
+          put(3, S[j][i], c, left);
         }
+      }
+    clear();
   };
 
   int stage = 0, par = 0;
@@ -408,42 +463,40 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
       if (row > row0) give(group);
       group = row / p.rows_per_group;
       next_group = (group + 1) * p.rows_per_group;
-#pragma unroll
-      for (int j = 0; j < kPackets; ++j)
-#pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          const int c = C::first(j) + i;
-          wg[j][i] = i < n[j] ? param(gate, group * N + c, 1.0f) * Cvt<W>::to_f(w1[c]) : 0.0f;
-        }
+      load_params<C, W, kPackets>(
+          wg, n, [&](int c) { return param(gate, group * N + c, 1.0f) * Cvt<W>::to_f(w1[c]); });
     }
     fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
     copies_wait<kStages - 1>();
-    float xv[kPackets][kV], sv[kPackets][kV], fv[kPackets][kV];
+    float2 xv[kPackets][kP], sv[kPackets][kP];
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
         C::read(slot(stage, 0, j), xv[j]);
         C::read(slot(stage, 1, j), sv[j]);
-        C::read(slot(stage, 2, j), fv[j]);
       } else {
 #pragma unroll
-        for (int i = 0; i < kV; ++i) xv[j][i] = sv[j][i] = fv[j][i] = 0.0f;
+        for (int i = 0; i < kP; ++i) xv[j][i] = sv[j][i] = both(0.0f);
       }
     }
     // Statistics of x and s, and of f = dy w2 with the centred s: one exchange.
-    float mean_xw, mean_sw, F = 0.0f, Fs = 0.0f;
-    const Moments mx = warp_moments<kV, kPackets>(xv, n, layer, inv_mine, mean_xw);
-    const Moments ms = warp_moments<kV, kPackets>(sv, n, layer, inv_mine, mean_sw);
+    float mean_xw, mean_sw;
+    float2 F2 = both(0.0f), Fs2 = both(0.0f);
+    const Moments mx = warp_moments<C, kPackets>(xv, n, layer, inv_mine, mean_xw);
+    const Moments ms = warp_moments<C, kPackets>(sv, n, layer, inv_mine, mean_sw);
 #pragma unroll
     for (int j = 0; j < kPackets; ++j)
+      if (n[j] > 0) {
+        float2 g[kP];
+        C::read(slot(stage, 2, j), g);
 #pragma unroll
-      for (int i = 0; i < kV; ++i) {
-        const float f = fv[j][i] * wn[j][i];
-        F += f;
-        Fs = fmaf(f, sv[j][i] - mean_sw, Fs);
+        for (int i = 0; i < kP; ++i) {
+          const float2 f = fmul2(g[i], wn[j][i]);
+          F2 = fadd2(F2, f);
+          Fs2 = ffma2(f, fadd2(sv[j][i], both(-mean_sw)), Fs2);
+        }
       }
-    if (layer) F = warp_sum(F);
-    Fs = warp_sum(Fs);
+    const float F = layer ? warp_sum(total(F2)) : 0.0f, Fs = warp_sum(total(Fs2));
     WarpSums<6, kWarps>& buf = first_sums[par];
     if (lane == 0) {
       buf.v[0][warp] = mx.sum;
@@ -460,71 +513,71 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
       const float sum_x = buf.v[0][from], sum_s = buf.v[2][from], f = buf.v[4][from];
       mean_x = over_warps<kWarps>(sum_x) * inv_n;
       mean_s = over_warps<kWarps>(sum_s) * inv_n;
-      mean_f = from_lane0(over_warps<kWarps>(f)) * inv_n;
+      mean_f = over_warps<kWarps>(f) * inv_n;
       const float ex = sum_x * inv_theirs - mean_x, es = sum_s * inv_theirs - mean_s;
       sqx = fmaf(theirs * ex, ex, sqx);
       sqs = fmaf(theirs * es, es, sqs);
       fs = fmaf(f, es, fs);
-      mean_x = from_lane0(mean_x);
-      mean_s = from_lane0(mean_s);
     }
-    const float rx = 1.0f / sqrtf(from_lane0(over_warps<kWarps>(sqx)) * inv_n + p.eps);
-    const float rs = 1.0f / sqrtf(from_lane0(over_warps<kWarps>(sqs)) * inv_n + p.eps);
-    const float mean_fs = from_lane0(over_warps<kWarps>(fs)) * inv_n * rs;
+    const float rx = rsqrtf(fmaf(over_warps<kWarps>(sqx), inv_n, p.eps));
+    const float rs = rsqrtf(fmaf(over_warps<kWarps>(sqs), inv_n, p.eps));
+    const float mean_fs = over_warps<kWarps>(fs) * inv_n * rs;
 
-    // ds' and the sums for dx; xv becomes x^, sv becomes ds'.
+    // ds' and the sums for dx; xv becomes x^, sv becomes e.
     T* dres = static_cast<T*>(p.dres) + row * N;
-    float E = 0.0f, Ex = 0.0f;
+    float2 E2 = both(0.0f), Ex2 = both(0.0f);
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
-        float t[kV], o[kV];
+        float2 t[kP], g[kP];
+        C::read(slot(stage, 2, j), g);
         if (ds) {
           C::read(slot(stage, 3, j), t);
         } else {
 #pragma unroll
-          for (int i = 0; i < kV; ++i) t[i] = 0.0f;
+          for (int i = 0; i < kP; ++i) t[i] = both(0.0f);
         }
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          const bool in = kAligned || i < n[j];
-          const float hat = (sv[j][i] - mean_s) * rs, xh = (xv[j][i] - mean_x) * rx;
-          const float f = fv[j][i] * wn[j][i];
-          t[i] = in ? fmaf(rs, f - mean_f - hat * mean_fs, t[i]) : 0.0f;
-          R[j][i] = fmaf(fv[j][i], hat, R[j][i]);
-          P[j][i] = fmaf(t[i], xh, P[j][i]);
+        for (int i = 0; i < kP; ++i) {
+          const float2 hat = fmul2(fadd2(sv[j][i], both(-mean_s)), both(rs));
+          const float2 xh = fmul2(fadd2(xv[j][i], both(-mean_x)), both(rx));
+          const float2 f = ffma2(g[i], wn[j][i], ffma2(hat, both(-mean_fs), both(-mean_f)));
+          t[i] = ffma2(both(rs), f, t[i]);
+          if (!kAligned && 2 * i >= n[j]) t[i].x = 0.0f;
+          if (!kAligned && 2 * i + 1 >= n[j]) t[i].y = 0.0f;
+          R[j][i] = ffma2(g[i], hat, R[j][i]);
+          P[j][i] = ffma2(t[i], xh, P[j][i]);
           if (kBias) {
-            Q[j][i] += t[i];
-            S[j][i] += fv[j][i];
+            Q[j][i] = fadd2(Q[j][i], t[i]);
+            S[j][i] = fadd2(S[j][i], g[i]);
           }
-          const float e = t[i] * wg[j][i];
-          E += e;
-          Ex = fmaf(e, xh, Ex);
-          o[i] = p.alpha * t[i];
+          const float2 e = fmul2(t[i], wg[j][i]);
+          E2 = fadd2(E2, e);
+          Ex2 = ffma2(e, xh, Ex2);
+          t[i] = fmul2(both(p.alpha), t[i]);
           xv[j][i] = xh;
           sv[j][i] = e;
         }
-        C::write(dres, j, N, o);
+        C::write(dres, j, N, t);
       }
     }
-    if (layer) E = warp_sum(E);
-    Ex = warp_sum(Ex);
+    const float E = layer ? warp_sum(total(E2)) : 0.0f, Ex = warp_sum(total(Ex2));
     WarpSums<2, kWarps>& buf2 = second_sums[par];
     if (lane == 0) {
       buf2.v[0][warp] = E;
       buf2.v[1][warp] = Ex;
     }
     __syncthreads();
-    const float mean_e =
-        layer ? from_lane0(over_warps<kWarps>(buf2.v[0][from])) * inv_n : 0.0f;
-    const float mean_ex = from_lane0(over_warps<kWarps>(buf2.v[1][from])) * inv_n;
+    const float mean_e = layer ? over_warps<kWarps>(buf2.v[0][from]) * inv_n : 0.0f;
+    const float mean_ex = over_warps<kWarps>(buf2.v[1][from]) * inv_n;
     T* dx = static_cast<T*>(p.dx) + row * N;
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
-        float o[kV];
+        float2 o[kP];
 #pragma unroll
-        for (int i = 0; i < kV; ++i) o[i] = rx * (sv[j][i] - mean_e - xv[j][i] * mean_ex);
+        for (int i = 0; i < kP; ++i)
+          o[i] = fmul2(both(rx), ffma2(xv[j][i], both(-mean_ex), fadd2(sv[j][i], both(-mean_e))));
         C::write(dx, j, N, o);
       }
     }
