@@ -21,10 +21,11 @@
 // Both passes read each row once and write it once: persistent CTAs walk
 // consecutive rows, a thread owns the same columns in every row (parameters and
 // column sums stay in registers) and copies its own packets of the rows ahead into
-// a private slot of a shared-memory ring.  A row costs two barriers, one
-// for each norm: a LayerNorm's mean and variance are taken warp by warp, centred
-// there, and joined (Chan, Golub & LeVeque, "Updating formulae and a
-// pairwise algorithm for computing sample variances", 1979).
+// a private slot of a shared-memory ring.  A row costs one barrier, although it
+// has two reductions one after another: the second of a row is exchanged together with the
+// first of the next one.  A LayerNorm's mean and variance are taken warp by
+// warp, centred there, and joined (Chan, Golub & LeVeque, "Updating formulae
+// and a pairwise algorithm for computing sample variances", 1979).
 #include <algorithm>
 #include <type_traits>
 
@@ -37,6 +38,15 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// Several sums over a warp at once: their shuffles are independent of each other.
+template <int K>
+__device__ __forceinline__ void warp_sums(float (&v)[K]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
 }
 
 template <typename W>
@@ -159,12 +169,13 @@ struct WarpSums {
   float v[kSums][kWarps];
 };
 
-// Sum over the warps of what lane l holds of warp l % kWarps; in every lane.
-template <int kWarps>
-__device__ __forceinline__ float over_warps(float v) {
+// Sums over the warps of what lane l holds of warp l % kWarps; in every lane.
+template <int kWarps, int K>
+__device__ __forceinline__ void over_warps(float (&v)[K]) {
 #pragma unroll
-  for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  for (int o = kWarps / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
 }
 
 // Number of row elements that lie in warp w.
@@ -179,44 +190,35 @@ __device__ __forceinline__ float in_warp(int w, int N) {
   return static_cast<float>(n);
 }
 
-// What a warp knows of a row: its sum (LayerNorm) and its sum of squares about its
-// own mean (RMS: about zero).
-struct Moments {
-  float sum, sq;
-};
+// A thread's sum of a row, and its sum of squares about `mean`.
 template <typename C, int kPackets>
-__device__ __forceinline__ Moments warp_moments(const float2 (&v)[kPackets][C::kP],
-                                                const int (&n)[kPackets], bool layer,
-                                                float inv_in_warp, float& mean) {
-  Moments m{0.0f, 0.0f};
-  mean = 0.0f;
+__device__ __forceinline__ float sum_of(const float2 (&v)[kPackets][C::kP]) {
+  float2 sum = both(0.0f);
+#pragma unroll
+  for (int j = 0; j < kPackets; ++j)
+#pragma unroll
+    for (int i = 0; i < C::kP; ++i) sum = fadd2(sum, v[j][i]);  // zeros past the end
+  return total(sum);
+}
+template <typename C, int kPackets>
+__device__ __forceinline__ float squares_of(const float2 (&v)[kPackets][C::kP],
+                                            const int (&n)[kPackets], bool layer, float mean) {
   float2 sq = both(0.0f);
-  if (layer) {
-    float2 sum = both(0.0f);
 #pragma unroll
-    for (int j = 0; j < kPackets; ++j)
-#pragma unroll
-      for (int i = 0; i < C::kP; ++i) sum = fadd2(sum, v[j][i]);  // zeros past the end
-    m.sum = warp_sum(total(sum));
-    mean = m.sum * inv_in_warp;
-#pragma unroll
-    for (int j = 0; j < kPackets; ++j)
-      if (n[j] > 0)
-#pragma unroll
-        for (int i = 0; i < C::kP; ++i) {
-          float2 d = fadd2(v[j][i], both(-mean));
-          if (!C::kWhole && 2 * i >= n[j]) d.x = 0.0f;
-          if (!C::kWhole && 2 * i + 1 >= n[j]) d.y = 0.0f;
-          sq = ffma2(d, d, sq);
-        }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kPackets; ++j)
+  for (int j = 0; j < kPackets; ++j)
+    if (!layer) {
 #pragma unroll
       for (int i = 0; i < C::kP; ++i) sq = ffma2(v[j][i], v[j][i], sq);
-  }
-  m.sq = warp_sum(total(sq));
-  return m;
+    } else if (n[j] > 0) {
+#pragma unroll
+      for (int i = 0; i < C::kP; ++i) {
+        float2 d = fadd2(v[j][i], both(-mean));
+        if (!C::kWhole && 2 * i >= n[j]) d.x = 0.0f;
+        if (!C::kWhole && 2 * i + 1 >= n[j]) d.y = 0.0f;
+        sq = ffma2(d, d, sq);
+      }
+    }
+  return total(sq);
 }
 
 // Parameters of a thread's columns (zero where there are none).
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
   using C = Cols<T, kThreads, kPackets, kAligned>;
   constexpr int kP = C::kP, kWarps = kThreads / 32;
   extern __shared__ uint4 ring[];  // [stage][x, residual][packet][thread]
-  __shared__ WarpSums<2, kWarps> sums[2];
+  __shared__ WarpSums<4, kWarps> sums[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, N = p.N;
   const bool layer = p.layer;
   const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.res);
@@ -285,39 +287,8 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
   const float theirs = in_warp<C, kThreads, kPackets>(from, N);
   const float inv_theirs = theirs > 0.0f ? 1.0f / theirs : 0.0f;
 
-  // mean and 1 / deviation of the row held in v.
-  auto stats = [&](const float2(&v)[kPackets][kP], WarpSums<2, kWarps>& buf) {
-    float warp_mean;
-    const Moments m = warp_moments<C, kPackets>(v, n, layer, inv_mine, warp_mean);
-    if (lane == 0) {
-      buf.v[0][warp] = m.sum;
-      buf.v[1][warp] = m.sq;
-    }
-    __syncthreads();
-    float sq = buf.v[1][from], mean = 0.0f;
-    if (layer) {
-      const float sum = buf.v[0][from];
-      mean = over_warps<kWarps>(sum) * inv_n;
-      const float d = sum * inv_theirs - mean;
-      sq = fmaf(theirs * d, d, sq);
-    }
-    const float rstd = rsqrtf(fmaf(over_warps<kWarps>(sq), inv_n, p.eps));
-    return make_float2(mean, rstd);
-  };
-
-  int stage = 0;
-  int64_t next_group = row0;  // the row that starts another gate
-  for (int64_t row = row0; row < end; ++row) {
-    if (row >= next_group) {
-      const int64_t g = row / p.rows_per_group;
-      next_group = (g + 1) * p.rows_per_group;
-      auto gate_at = [&](int c) { return param(gate, g * N + c, 1.0f); };
-      load_params<C, W, kPackets>(wg, n, [&](int c) { return gate_at(c) * Cvt<W>::to_f(w1[c]); });
-      load_params<C, W, kPackets>(bg, n, [&](int c) { return gate_at(c) * param(b1, c, 0.0f); });
-    }
-    fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
-    copies_wait<kStages - 1>();
-    float2 v[kPackets][kP];
+  // x of the row in `stage`, zeros where the thread has no packet.
+  auto read_x = [&](int stage, float2 (&v)[kPackets][kP]) {
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0)
@@ -326,7 +297,61 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
 #pragma unroll
         for (int i = 0; i < kP; ++i) v[j][i] = both(0.0f);
     }
-    const float2 sx = stats(v, sums[0]);
+  };
+  // One exchange: the moments of x of the next row and of s of this one -> their means and
+  // 1 / deviations (mean_x, rstd_x, mean_s, rstd_s).
+  int par = 0;
+  auto exchange = [&](const float2(&xv)[kPackets][kP], const float2(&sv)[kPackets][kP]) {
+    WarpSums<4, kWarps>& buf = sums[par];
+    par ^= 1;
+    float m[2] = {0.0f, 0.0f};
+    if (layer) {
+      m[0] = sum_of<C, kPackets>(xv);
+      m[1] = sum_of<C, kPackets>(sv);
+      warp_sums(m);
+    }
+    float q[2] = {squares_of<C, kPackets>(xv, n, layer, m[0] * inv_mine),
+                  squares_of<C, kPackets>(sv, n, layer, m[1] * inv_mine)};
+    warp_sums(q);
+    if (lane == 0) {
+      buf.v[0][warp] = m[0];
+      buf.v[1][warp] = m[1];
+      buf.v[2][warp] = q[0];
+      buf.v[3][warp] = q[1];
+    }
+    __syncthreads();
+    float mean[2] = {0.0f, 0.0f}, sq[2] = {buf.v[2][from], buf.v[3][from]};
+    if (layer) {
+      const float sum[2] = {buf.v[0][from], buf.v[1][from]};
+      mean[0] = sum[0];
+      mean[1] = sum[1];
+      over_warps<kWarps>(mean);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        mean[k] *= inv_n;
+        const float d = sum[k] * inv_theirs - mean[k];
+        sq[k] = fmaf(theirs * d, d, sq[k]);
+      }
+    }
+    over_warps<kWarps>(sq);
+    return make_float4(mean[0], rsqrtf(fmaf(sq[0], inv_n, p.eps)), mean[1],
+                       rsqrtf(fmaf(sq[1], inv_n, p.eps)));
+  };
+
+  int stage = 0;
+  int64_t next_group = row0;  // the row that starts another gate
+  float2 v[kPackets][kP], xv[kPackets][kP];  // s of the row, x of the next one
+  copies_wait<kStages - 2>();
+  read_x(0, xv);
+  float4 stat = exchange(xv, xv);
+  for (int64_t row = row0; row < end; ++row) {
+    if (row >= next_group) {
+      const int64_t g = row / p.rows_per_group;
+      next_group = (g + 1) * p.rows_per_group;
+      auto gate_at = [&](int c) { return param(gate, g * N + c, 1.0f); };
+      load_params<C, W, kPackets>(wg, n, [&](int c) { return gate_at(c) * Cvt<W>::to_f(w1[c]); });
+      load_params<C, W, kPackets>(bg, n, [&](int c) { return gate_at(c) * param(b1, c, 0.0f); });
+    }
     T* out = static_cast<T*>(p.res_out) + row * N;
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
@@ -335,28 +360,34 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
         C::read(slot(stage, 1, j), r);
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
-          // (v - mean) first: v rstd - mean rstd would cancel where the mean is large
-          const float2 hat = fmul2(fadd2(v[j][i], both(-sx.x)), both(sx.y));
+          // (x - mean) first: x rstd - mean rstd would cancel where the mean is large
+          const float2 hat = fmul2(fadd2(xv[j][i], both(-stat.x)), both(stat.y));
           v[j][i] = ffma2(both(p.alpha), r[i], ffma2(hat, wg[j][i], bg[j][i]));
           if (!kAligned && 2 * i >= n[j]) v[j][i].x = 0.0f;
           if (!kAligned && 2 * i + 1 >= n[j]) v[j][i].y = 0.0f;
         }
         C::write(out, j, N, v[j]);
         C::round(v[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kP; ++i) v[j][i] = both(0.0f);
       }
     }
-    const float2 ss = stats(v, sums[1]);
+    fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
+    copies_wait<kStages - 2>();
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    read_x(stage, xv);  // past the last row: what an earlier one left there, unused
+    stat = exchange(xv, v);
     T* yr = static_cast<T*>(p.y) + row * N;
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
 #pragma unroll
         for (int i = 0; i < kP; ++i)
-          v[j][i] = ffma2(fmul2(fadd2(v[j][i], both(-ss.x)), both(ss.y)), wn[j][i], bn[j][i]);
+          v[j][i] = ffma2(fmul2(fadd2(v[j][i], both(-stat.z)), both(stat.w)), wn[j][i], bn[j][i]);
         C::write(yr, j, N, v[j]);
       }
     }
-    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   copies_wait<0>();
 }
@@ -386,8 +417,7 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
   using C = Cols<T, kThreads, kPackets, kAligned>;
   constexpr int kP = C::kP, kWarps = kThreads / 32, kSums = kBias ? 4 : 2;
   extern __shared__ uint4 ring[];  // [stage][x, s, dy, ds][packet][thread]
-  __shared__ WarpSums<6, kWarps> first_sums[2];
-  __shared__ WarpSums<2, kWarps> second_sums[2];
+  __shared__ WarpSums<8, kWarps> sums[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, N = p.N;
   const bool layer = p.layer;
   const T *x = static_cast<const T*>(p.x), *s = static_cast<const T*>(p.s),
@@ -456,34 +486,37 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
     clear();
   };
 
-  int stage = 0, par = 0;
-  int64_t group = row0 / p.rows_per_group, next_group = row0;
-  for (int64_t row = row0; row < end; ++row, par ^= 1) {
-    if (row >= next_group) {
-      if (row > row0) give(group);
-      group = row / p.rows_per_group;
-      next_group = (group + 1) * p.rows_per_group;
-      load_params<C, W, kPackets>(
-          wg, n, [&](int c) { return param(gate, group * N + c, 1.0f) * Cvt<W>::to_f(w1[c]); });
-    }
-    fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
-    copies_wait<kStages - 1>();
-    float2 xv[kPackets][kP], sv[kPackets][kP];
+  auto read = [&](int stage, int tensor, float2 (&v)[kPackets][kP]) {
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
-      if (n[j] > 0) {
-        C::read(slot(stage, 0, j), xv[j]);
-        C::read(slot(stage, 1, j), sv[j]);
-      } else {
+      if (n[j] > 0)
+        C::read(slot(stage, tensor, j), v[j]);
+      else
 #pragma unroll
-        for (int i = 0; i < kP; ++i) xv[j][i] = sv[j][i] = both(0.0f);
-      }
+        for (int i = 0; i < kP; ++i) v[j][i] = both(0.0f);
     }
-    // Statistics of x and s, and of f = dy w2 with the centred s: one exchange.
-    float mean_xw, mean_sw;
+  };
+  // One exchange: of the row in `stage` the statistics of x and s, and of f = dy w2 with the
+  // centred s; of the row before it E = sum e and Ex = sum e x^ (the thread's
+  // sums), which come back over the CTA.
+  struct Stats {
+    float mean_x, rx, mean_s, rs, mean_f, mean_fs;
+  };
+  int par = 0;
+  auto exchange = [&](int stage, float& E, float& Ex) {
+    WarpSums<8, kWarps>& buf = sums[par];
+    par ^= 1;
+    float2 xv[kPackets][kP], sv[kPackets][kP];
+    read(stage, 0, xv);
+    read(stage, 1, sv);
+    float m[2] = {0.0f, 0.0f};
+    if (layer) {
+      m[0] = sum_of<C, kPackets>(xv);
+      m[1] = sum_of<C, kPackets>(sv);
+      warp_sums(m);
+    }
+    const float mean_sw = m[1] * inv_mine;
     float2 F2 = both(0.0f), Fs2 = both(0.0f);
-    const Moments mx = warp_moments<C, kPackets>(xv, n, layer, inv_mine, mean_xw);
-    const Moments ms = warp_moments<C, kPackets>(sv, n, layer, inv_mine, mean_sw);
 #pragma unroll
     for (int j = 0; j < kPackets; ++j)
       if (n[j] > 0) {
@@ -496,40 +529,74 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
           Fs2 = ffma2(f, fadd2(sv[j][i], both(-mean_sw)), Fs2);
         }
       }
-    const float F = layer ? warp_sum(total(F2)) : 0.0f, Fs = warp_sum(total(Fs2));
-    WarpSums<6, kWarps>& buf = first_sums[par];
+    float q[4] = {squares_of<C, kPackets>(xv, n, layer, m[0] * inv_mine),
+                  squares_of<C, kPackets>(sv, n, layer, mean_sw), total(Fs2), Ex};
+    float l[2] = {total(F2), E};
+    warp_sums(q);
+    if (layer) warp_sums(l);
     if (lane == 0) {
-      buf.v[0][warp] = mx.sum;
-      buf.v[1][warp] = mx.sq;
-      buf.v[2][warp] = ms.sum;
-      buf.v[3][warp] = ms.sq;
-      buf.v[4][warp] = F;
-      buf.v[5][warp] = Fs;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) buf.v[k][warp] = q[k];
+      buf.v[4][warp] = m[0];
+      buf.v[5][warp] = m[1];
+      buf.v[6][warp] = l[0];
+      buf.v[7][warp] = l[1];
     }
     __syncthreads();
-    float mean_x = 0.0f, mean_s = 0.0f, mean_f = 0.0f;
-    float sqx = buf.v[1][from], sqs = buf.v[3][from], fs = buf.v[5][from];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[k] = buf.v[k][from];
+    float mean[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of x, s, f; and E
     if (layer) {
-      const float sum_x = buf.v[0][from], sum_s = buf.v[2][from], f = buf.v[4][from];
-      mean_x = over_warps<kWarps>(sum_x) * inv_n;
-      mean_s = over_warps<kWarps>(sum_s) * inv_n;
-      mean_f = over_warps<kWarps>(f) * inv_n;
-      const float ex = sum_x * inv_theirs - mean_x, es = sum_s * inv_theirs - mean_s;
-      sqx = fmaf(theirs * ex, ex, sqx);
-      sqs = fmaf(theirs * es, es, sqs);
-      fs = fmaf(f, es, fs);
+      const float sum_x = buf.v[4][from], sum_s = buf.v[5][from], f = buf.v[6][from];
+      mean[0] = sum_x;
+      mean[1] = sum_s;
+      mean[2] = f;
+      mean[3] = buf.v[7][from];
+      over_warps<kWarps>(mean);
+      mean[0] *= inv_n;
+      mean[1] *= inv_n;
+      mean[2] *= inv_n;
+      const float ex = sum_x * inv_theirs - mean[0], es = sum_s * inv_theirs - mean[1];
+      q[0] = fmaf(theirs * ex, ex, q[0]);
+      q[1] = fmaf(theirs * es, es, q[1]);
+      q[2] = fmaf(f, es, q[2]);
     }
-    const float rx = rsqrtf(fmaf(over_warps<kWarps>(sqx), inv_n, p.eps));
-    const float rs = rsqrtf(fmaf(over_warps<kWarps>(sqs), inv_n, p.eps));
-    const float mean_fs = over_warps<kWarps>(fs) * inv_n * rs;
+    over_warps<kWarps>(q);
+    E = mean[3];
+    Ex = q[3];
+    Stats st;
+    st.mean_x = mean[0];
+    st.mean_s = mean[1];
+    st.mean_f = mean[2];
+    st.rx = rsqrtf(fmaf(q[0], inv_n, p.eps));
+    st.rs = rsqrtf(fmaf(q[1], inv_n, p.eps));
+    st.mean_fs = q[2] * inv_n * st.rs;
+    return st;
+  };
 
+  int stage = 0;
+  int64_t group = row0 / p.rows_per_group, next_group = row0;
+  float E = 0.0f, Ex = 0.0f;
+  copies_wait<kStages - 2>();
+  Stats st = exchange(0, E, Ex);
+  for (int64_t row = row0; row < end; ++row) {
+    if (row >= next_group) {
+      if (row > row0) give(group);
+      group = row / p.rows_per_group;
+      next_group = (group + 1) * p.rows_per_group;
+      load_params<C, W, kPackets>(
+          wg, n, [&](int c) { return param(gate, group * N + c, 1.0f) * Cvt<W>::to_f(w1[c]); });
+    }
     // ds' and the sums for dx; xv becomes x^, sv becomes e.
+    float2 xv[kPackets][kP], sv[kPackets][kP];
     T* dres = static_cast<T*>(p.dres) + row * N;
     float2 E2 = both(0.0f), Ex2 = both(0.0f);
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
         float2 t[kP], g[kP];
+        C::read(slot(stage, 0, j), xv[j]);
+        C::read(slot(stage, 1, j), sv[j]);
         C::read(slot(stage, 2, j), g);
         if (ds) {
           C::read(slot(stage, 3, j), t);
@@ -539,10 +606,10 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
         }
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
-          const float2 hat = fmul2(fadd2(sv[j][i], both(-mean_s)), both(rs));
-          const float2 xh = fmul2(fadd2(xv[j][i], both(-mean_x)), both(rx));
-          const float2 f = ffma2(g[i], wn[j][i], ffma2(hat, both(-mean_fs), both(-mean_f)));
-          t[i] = ffma2(both(rs), f, t[i]);
+          const float2 hat = fmul2(fadd2(sv[j][i], both(-st.mean_s)), both(st.rs));
+          const float2 xh = fmul2(fadd2(xv[j][i], both(-st.mean_x)), both(st.rx));
+          const float2 f = ffma2(g[i], wn[j][i], ffma2(hat, both(-st.mean_fs), both(-st.mean_f)));
+          t[i] = ffma2(both(st.rs), f, t[i]);
           if (!kAligned && 2 * i >= n[j]) t[i].x = 0.0f;
           if (!kAligned && 2 * i + 1 >= n[j]) t[i].y = 0.0f;
           R[j][i] = ffma2(g[i], hat, R[j][i]);
@@ -561,15 +628,14 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
         C::write(dres, j, N, t);
       }
     }
-    const float E = layer ? warp_sum(total(E2)) : 0.0f, Ex = warp_sum(total(Ex2));
-    WarpSums<2, kWarps>& buf2 = second_sums[par];
-    if (lane == 0) {
-      buf2.v[0][warp] = E;
-      buf2.v[1][warp] = Ex;
-    }
-    __syncthreads();
-    const float mean_e = layer ? over_warps<kWarps>(buf2.v[0][from]) * inv_n : 0.0f;
-    const float mean_ex = over_warps<kWarps>(buf2.v[1][from]) * inv_n;
+    E = total(E2);
+    Ex = total(Ex2);
+    const float rx = st.rx;
+    fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
+    copies_wait<kStages - 2>();
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    st = exchange(stage, E, Ex);  // past the last row: of what an earlier one left there, unused
+    const float mean_e = E * inv_n, mean_ex = Ex * inv_n;
     T* dx = static_cast<T*>(p.dx) + row * N;
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
@@ -581,7 +647,6 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
         C::write(dx, j, N, o);
       }
     }
-    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   if (row0 < end) give(group);
   copies_wait<0>();
@@ -798,10 +863,10 @@ int launch_rows(void (*kernel)(const A), int threads, size_t smem, int64_t ctas,
   return launch_status();
 }
 
-// CTAs of the backward pass: one an SM.  Its registers allow no second one, and each
-// adds a stretch of column sums to write and read.
-int64_t bwd_ctas(int64_t M) { return std::min<int64_t>(M, sm_count()); }
-constexpr int kMaxCtas = 512;  // workspace: more SMs than any device of this architecture has
+// CTAs of the backward pass: one an SM, two or four where rows are short and so CTAs are
+// small (each adds a stretch of column sums to write and read).
+int64_t ctas_per_sm(int64_t N) { return N <= 1024 ? 4 : (N <= 2048 ? 2 : 1); }
+constexpr int kMaxSms = 256;  // workspace: more than any device of this architecture has
 
 template <typename T, typename W, bool kAligned>
 int launch_fwd(const FwdArgs& a, cudaStream_t s) {
@@ -869,7 +934,7 @@ extern "C" int tileops_sandwich_norm_fwd(const void* x, const void* residual,
 extern "C" int64_t tileops_sandwich_norm_bwd_workspace_bytes(int64_t M, int64_t N,
                                                              int64_t gate_rows, int has_bias) {
   if (bad_shape(M, N, gate_rows)) return -1;
-  return (std::min<int64_t>(M, kMaxCtas) + gate_rows) * (has_bias ? 4 : 2) * N * 4;
+  return (std::min<int64_t>(M, kMaxSms * ctas_per_sm(N)) + gate_rows) * (has_bias ? 4 : 2) * N * 4;
 }
 
 extern "C" int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_out, const void* x,
@@ -896,7 +961,7 @@ extern "C" int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_
                      d_residual, part, M, static_cast<int>(N), M / gate_rows,
                      norm == TILEOPS_NORM_LAYER, static_cast<float>(eps),
                      static_cast<float>(residual_scale)};
-  const int64_t ctas = std::min<int64_t>(bwd_ctas(M), kMaxCtas);
+  const int64_t ctas = std::min<int64_t>(M, std::min(sm_count(), kMaxSms) * ctas_per_sm(N));
   return with_types(dtype, affine_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);

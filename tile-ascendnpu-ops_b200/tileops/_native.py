@@ -180,6 +180,11 @@ def ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
+def data_ptr(t: Optional[torch.Tensor]) -> int:
+    """``ptr`` as a plain number, which ctypes turns into a pointer by itself."""
+    return 0 if t is None else t.data_ptr()
+
+
 def launch(name: str, device: torch.device, *args) -> None:
     """Call ``name(*args, stream)`` on ``device``'s current torch stream.
 

@@ -82,8 +82,8 @@ class GatedLinearRecurrenceFwdKernel(_GatedLinearRecurrenceKernel):
         decay_param = decay_param.contiguous()
         _native.launch(
             "tileops_glr_fwd", dev, x.data_ptr(), input_gate.data_ptr(), decay_gate.data_ptr(),
-            decay_param.data_ptr(), _native.ptr(initial_state), _native.ptr(cu), nseq,
-            y.data_ptr(), final.data_ptr(), _native.ptr(states), B, T, D,
+            decay_param.data_ptr(), _native.data_ptr(initial_state), _native.data_ptr(cu), nseq,
+            y.data_ptr(), final.data_ptr(), _native.data_ptr(states), B, T, D,
             x.stride(0), x.stride(1), input_gate.stride(0), input_gate.stride(1),
             decay_gate.stride(0), decay_gate.stride(1), self.decay_scale, self._code)
         return y, final, states
@@ -114,8 +114,8 @@ class GatedLinearRecurrenceBwdKernel(_GatedLinearRecurrenceKernel):
         decay_param, states = decay_param.contiguous(), states.contiguous()
         _native.launch(
             "tileops_glr_bwd", dev, dy.data_ptr(), x.data_ptr(), input_gate.data_ptr(),
-            decay_gate.data_ptr(), decay_param.data_ptr(), states.data_ptr(), _native.ptr(initial_state),
-            _native.ptr(d_final_state), _native.ptr(cu), nseq, dx.data_ptr(), di.data_ptr(),
+            decay_gate.data_ptr(), decay_param.data_ptr(), states.data_ptr(), _native.data_ptr(initial_state),
+            _native.data_ptr(d_final_state), _native.data_ptr(cu), nseq, dx.data_ptr(), di.data_ptr(),
             dr.data_ptr(), d_param.data_ptr(), d_initial.data_ptr(), ws.data_ptr(), B, T, D,
             dy.stride(0), dy.stride(1), x.stride(0), x.stride(1), input_gate.stride(0),
             input_gate.stride(1), decay_gate.stride(0), decay_gate.stride(1), self.decay_scale,
@@ -142,7 +142,7 @@ class GatedLinearRecurrenceDecodeKernel(_GatedLinearRecurrenceKernel):
         decay_param = decay_param.contiguous()
         if not inplace:
             state = state.contiguous()
-        y = torch.empty((B, D), dtype=self.dtype, device=dev)
+        y = torch.empty_like(x)  # dense: rows of contiguous channels
         new_state = state if inplace else torch.empty_like(state)
         _native.launch(
             "tileops_glr_decode_fwd", dev, x.data_ptr(), input_gate.data_ptr(),

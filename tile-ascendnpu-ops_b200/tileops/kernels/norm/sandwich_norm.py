@@ -50,15 +50,15 @@ class FusedSandwichNormFwdKernel(_SandwichNormKernel):
 
     def forward(self, x, residual, post_weight, pre_weight, gate=None, post_bias=None,
                 pre_bias=None):
-        """``(y, residual_out)`` of contiguous (M, N) rows; gate (rows, N) or None."""
+        """``(y, residual_out)``, shaped like ``x``: contiguous, M rows of N."""
         y, residual_out = torch.empty_like(x), torch.empty_like(x)
+        ptr = _native.data_ptr
         _native.launch(
             "tileops_sandwich_norm_fwd", x.device, x.data_ptr(), residual.data_ptr(),
-            post_weight.data_ptr(), pre_weight.data_ptr(), _native.ptr(gate),
-            _native.ptr(post_bias), _native.ptr(pre_bias), y.data_ptr(),
-            residual_out.data_ptr(), self.M, self.N, 1 if gate is None else gate.shape[0],
-            self._norm_code, self.eps, self.residual_scale, self._code,
-            _native.dtype_code(post_weight.dtype))
+            post_weight.data_ptr(), pre_weight.data_ptr(), ptr(gate), ptr(post_bias),
+            ptr(pre_bias), y.data_ptr(), residual_out.data_ptr(), self.M, self.N,
+            1 if gate is None else gate.numel() // self.N, self._norm_code, self.eps,
+            self.residual_scale, self._code, _native.dtype_code(post_weight.dtype))
         return y, residual_out
 
 
@@ -74,14 +74,14 @@ class FusedSandwichNormBwdKernel(_SandwichNormKernel):
                  for p in (post_weight, pre_weight, gate, post_bias, pre_bias)]
         if self.M == 0:
             return dx, d_residual, *(None if g is None else g.zero_() for g in grads)
-        groups = 1 if gate is None else gate.shape[0]
+        groups = 1 if gate is None else gate.numel() // self.N
+        ptr = _native.data_ptr
         size = _native.lib().tileops_sandwich_norm_bwd_workspace_bytes(
             self.M, self.N, groups, post_bias is not None or pre_bias is not None)
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         _native.launch(
-            "tileops_sandwich_norm_bwd", x.device, dy.data_ptr(), _native.ptr(d_residual_out),
+            "tileops_sandwich_norm_bwd", x.device, dy.data_ptr(), ptr(d_residual_out),
             x.data_ptr(), residual_out.data_ptr(), post_weight.data_ptr(), pre_weight.data_ptr(),
-            _native.ptr(gate), _native.ptr(post_bias), dx.data_ptr(), d_residual.data_ptr(),
-            *map(_native.ptr, grads), ws.data_ptr(), self.M, self.N, groups, self._norm_code,
+            ptr(gate), ptr(post_bias), dx.data_ptr(), d_residual.data_ptr(), *map(ptr, grads), ws.data_ptr(), self.M, self.N, groups, self._norm_code,
             self.eps, self.residual_scale, self._code, _native.dtype_code(post_weight.dtype))
         return dx, d_residual, *grads

@@ -56,17 +56,19 @@ __all__ = ["GatedLinearRecurrenceBwdOp", "GatedLinearRecurrenceDecodeOp",
 _SEGMENT = 32
 
 
-def _check(device: torch.device, name: str, t: torch.Tensor, shape: tuple,
+def _check(is_device_tensor, device: torch.device, name: str, t: torch.Tensor, shape: tuple,
            dtype: torch.dtype) -> None:
-    if not get_device_backend().is_device_tensor(t):
-        raise ValueError(f"{name} must be a {get_device_backend().name} tensor, "
+    if (is_device_tensor(t) and t.dtype is dtype and t.shape == shape and t.device == device):
+        return
+    backend = get_device_backend()
+    if not backend.is_device_tensor(t):
+        raise ValueError(f"{name} must be a {backend.name} tensor, "
                          f"got {getattr(t, 'device', type(t).__name__)}")
     if t.device != device:
         raise ValueError(f"Expected {name} on {device}, got {t.device}")
     if t.shape != shape:
         raise ValueError(f"Expected {name}.shape {shape}, got {tuple(t.shape)}")
-    if t.dtype != dtype:
-        raise ValueError(f"Expected {name}.dtype {dtype}, got {t.dtype}")
+    raise ValueError(f"Expected {name}.dtype {dtype}, got {t.dtype}")
 
 
 def _num_seqs(batch: int, device: torch.device, cu_seqlens: Optional[torch.Tensor]) -> int:
@@ -118,14 +120,14 @@ class GatedLinearRecurrenceFwdOp(Op):
                 decay_param: torch.Tensor, initial_state: Optional[torch.Tensor] = None,
                 cu_seqlens: Optional[torch.Tensor] = None):
         rows = (self.batch, self.seq_len, self.dim)
-        dev = getattr(x, "device", None)
-        _check(dev, "x", x, rows, self.dtype)
-        _check(dev, "input_gate", input_gate, rows, self.dtype)
-        _check(dev, "decay_gate", decay_gate, rows, self.dtype)
-        _check(dev, "decay_param", decay_param, (self.dim,), torch.float32)
+        dev, on_device = getattr(x, "device", None), get_device_backend().is_device_tensor
+        _check(on_device, dev, "x", x, rows, self.dtype)
+        _check(on_device, dev, "input_gate", input_gate, rows, self.dtype)
+        _check(on_device, dev, "decay_gate", decay_gate, rows, self.dtype)
+        _check(on_device, dev, "decay_param", decay_param, (self.dim,), torch.float32)
         nseq = _num_seqs(self.batch, dev, cu_seqlens)
         if initial_state is not None:
-            _check(dev, "initial_state", initial_state, (nseq, self.dim), torch.float32)
+            _check(on_device, dev, "initial_state", initial_state, (nseq, self.dim), torch.float32)
         out = self.kernel(x, input_gate, decay_gate, decay_param, initial_state, cu_seqlens,
                           self.save_states)
         return out if self.save_states else out[:2]
@@ -164,18 +166,18 @@ class GatedLinearRecurrenceBwdOp(Op):
                 d_final_state: Optional[torch.Tensor] = None,
                 cu_seqlens: Optional[torch.Tensor] = None):
         rows = (self.batch, self.seq_len, self.dim)
-        dev = getattr(x, "device", None)
-        _check(dev, "x", x, rows, self.dtype)
-        _check(dev, "dy", dy, rows, self.dtype)
-        _check(dev, "input_gate", input_gate, rows, self.dtype)
-        _check(dev, "decay_gate", decay_gate, rows, self.dtype)
-        _check(dev, "decay_param", decay_param, (self.dim,), torch.float32)
-        _check(dev, "states", states, (self.batch, -(-self.seq_len // _SEGMENT), self.dim),
+        dev, on_device = getattr(x, "device", None), get_device_backend().is_device_tensor
+        _check(on_device, dev, "x", x, rows, self.dtype)
+        _check(on_device, dev, "dy", dy, rows, self.dtype)
+        _check(on_device, dev, "input_gate", input_gate, rows, self.dtype)
+        _check(on_device, dev, "decay_gate", decay_gate, rows, self.dtype)
+        _check(on_device, dev, "decay_param", decay_param, (self.dim,), torch.float32)
+        _check(on_device, dev, "states", states, (self.batch, -(-self.seq_len // _SEGMENT), self.dim),
                torch.float32)
         nseq = _num_seqs(self.batch, dev, cu_seqlens)
         for name, t in (("initial_state", initial_state), ("d_final_state", d_final_state)):
             if t is not None:
-                _check(dev, name, t, (nseq, self.dim), torch.float32)
+                _check(on_device, dev, name, t, (nseq, self.dim), torch.float32)
         return self.kernel(dy, x, input_gate, decay_gate, decay_param, states, initial_state,
                            d_final_state, cu_seqlens)
 
@@ -216,12 +218,12 @@ class GatedLinearRecurrenceDecodeOp(Op):
                 decay_param: torch.Tensor,
                 state: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         rows = (self.batch, self.dim)
-        dev = getattr(x, "device", None)
-        _check(dev, "x", x, rows, self.dtype)
-        _check(dev, "input_gate", input_gate, rows, self.dtype)
-        _check(dev, "decay_gate", decay_gate, rows, self.dtype)
-        _check(dev, "decay_param", decay_param, (self.dim,), torch.float32)
-        _check(dev, "state", state, rows, torch.float32)
+        dev, on_device = getattr(x, "device", None), get_device_backend().is_device_tensor
+        _check(on_device, dev, "x", x, rows, self.dtype)
+        _check(on_device, dev, "input_gate", input_gate, rows, self.dtype)
+        _check(on_device, dev, "decay_gate", decay_gate, rows, self.dtype)
+        _check(on_device, dev, "decay_param", decay_param, (self.dim,), torch.float32)
+        _check(on_device, dev, "state", state, rows, torch.float32)
         if self.inplace and not state.is_contiguous():
             raise ValueError("state must be contiguous when it is updated in place")
         return self.kernel(x, input_gate, decay_gate, decay_param, state, self.inplace)

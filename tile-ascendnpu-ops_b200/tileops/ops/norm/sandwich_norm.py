@@ -71,54 +71,68 @@ class _SandwichNormOp(Op):
         self._kernel_cache: Dict[tuple, Kernel] = {}
         self._last: Optional[tuple[int, int, int, int]] = None
 
-    def _check(self, rows: tuple, params: tuple, gate: Optional[torch.Tensor]) -> int:
-        """Validate ((name, tensor), ...) rows and parameters; returns M."""
+    def _check(self, rows: tuple, params: tuple, gate: Optional[torch.Tensor]) -> None:
+        """Validate (name, tensor, name, tensor, ...) rows, x first, and parameters.
+
+        A decode step is bound by the host: tensors are compared against x and the first
+        parameter in one pass each, and told apart only when something is wrong."""
         is_device_tensor = get_device_backend().is_device_tensor
-        for name, t in rows + params + (("gate", gate),):
+        for t in rows[1::2] + params[1::2] + (gate,):
             if t is not None and not is_device_tensor(t):
-                raise ValueError(f"{name} must be a {get_device_backend().name} tensor")
-        x = dict(rows)["x"]
+                self._refuse_device(rows + params + ("gate", gate))
+        x = rows[1]
         committed_m, committed_n, committed_dtype = self._committed
-        dtype = committed_dtype or x.dtype
-        if x.dim() < 1 or x.shape[-1] < 1:
-            raise ValueError(f"Expected x of shape (..., N) with N >= 1, got {tuple(x.shape)}")
-        N = x.shape[-1]
+        dtype, shape, device = committed_dtype or x.dtype, x.shape, x.device
+        N = shape[-1] if shape else 0
+        if N < 1:
+            raise ValueError(f"Expected x of shape (..., N) with N >= 1, got {tuple(shape)}")
         M = x.numel() // N
-        affine = params[0][1].dtype
-        if affine not in (dtype, torch.float32):
-            raise ValueError(f"Expected {params[0][0]}.dtype {dtype} or {torch.float32}, "
+        affine = params[1].dtype
+        if affine is not dtype and affine is not torch.float32:
+            raise ValueError(f"Expected {params[0]}.dtype {dtype} or {torch.float32}, "
                              f"got {affine}")
-        for name, t in rows:
-            if t is None:
-                continue
-            if t.dtype != dtype:
-                raise ValueError(f"Expected {name}.dtype {dtype}, got {t.dtype}")
-            if t.shape != x.shape:
-                raise ValueError(f"Expected {name} shape {tuple(x.shape)}, got {tuple(t.shape)}")
-            if t.device != x.device:
-                raise ValueError(f"Expected {name} on {x.device}, got {t.device}")
-        for name, t in params + (("gate", gate),):
-            if t is None:
-                continue
-            if t.dtype != affine:
-                raise ValueError(f"Expected {name}.dtype {affine}, got {t.dtype}")
-            if t.device != x.device:
-                raise ValueError(f"Expected {name} on {x.device}, got {t.device}")
-            if name != "gate" and t.shape != (N,):
-                raise ValueError(f"Expected {name} shape {(N,)}, got {tuple(t.shape)}")
-        if gate is not None and (gate.dim() not in (1, 2) or gate.shape[-1] != N
-                                 or gate.dim() == 2 and (gate.shape[0] < 1 or M % gate.shape[0])):
-            raise ValueError(f"Expected gate shape {(N,)} or (G, {N}) with G dividing the {M} "
-                             f"rows, got {tuple(gate.shape)}")
+        for i in range(1, len(rows), 2):
+            t = rows[i]
+            if t is not None and not (t.dtype is dtype and t.shape == shape
+                                      and t.device == device):
+                self._refuse(rows[i - 1], t, dtype, shape, device)
+        vectors, vector = 0, (N,)
+        for i in range(1, len(params), 2):
+            t = params[i]
+            if t is not None:
+                vectors += 1
+                if not (t.dtype is affine and t.shape == vector and t.device == device):
+                    self._refuse(params[i - 1], t, affine, vector, device)
+        if gate is not None:
+            if gate.dtype is not affine or gate.device != device:
+                self._refuse("gate", gate, affine, gate.shape, device)
+            gate_shape = gate.shape
+            if (len(gate_shape) not in (1, 2) or gate_shape[-1] != N
+                    or len(gate_shape) == 2 and (gate_shape[0] < 1 or M % gate_shape[0])):
+                raise ValueError(f"Expected gate shape {(N,)} or (G, {N}) with G dividing the "
+                                 f"{M} rows, got {tuple(gate_shape)}")
+            vectors += gate.numel() // N
         if committed_n is not None and committed_n != N:
             raise ValueError(f"Expected hidden dim {committed_n}, got {N}")
         if committed_m is not None and committed_m != M:
             raise ValueError(f"Expected M={committed_m} (product of leading dims), got {M}")
         self.M, self.N, self.dtype = M, N, dtype
-        vectors = sum(t is not None for _, t in params)
-        self._last = (M, N, dtype.itemsize,
-                      (vectors + (0 if gate is None else gate.numel() // N)) * affine.itemsize)
-        return M
+        self._last = (M, N, dtype.itemsize, vectors * affine.itemsize)
+
+    @staticmethod
+    def _refuse_device(named: tuple) -> None:
+        backend = get_device_backend()
+        for name, t in zip(named[::2], named[1::2]):
+            if t is not None and not backend.is_device_tensor(t):
+                raise ValueError(f"{name} must be a {backend.name} tensor")
+
+    @staticmethod
+    def _refuse(name: str, t: torch.Tensor, dtype: torch.dtype, shape, device) -> None:
+        if t.dtype is not dtype:
+            raise ValueError(f"Expected {name}.dtype {dtype}, got {t.dtype}")
+        if t.shape != shape:
+            raise ValueError(f"Expected {name} shape {tuple(shape)}, got {tuple(t.shape)}")
+        raise ValueError(f"Expected {name} on {device}, got {t.device}")
 
     def _get_kernel(self, device_index) -> Kernel:
         key = (self.M, self.N, self.dtype, device_index)
@@ -135,11 +149,7 @@ class _SandwichNormOp(Op):
         return flops * M * N, rows * M * N * eb + passes * vectors * N
 
 
-def _flat(t: Optional[torch.Tensor], M: int, N: int) -> Optional[torch.Tensor]:
-    return None if t is None else t.contiguous().view(M, N)
-
-
-def _param(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else t.contiguous()
 
 
@@ -167,15 +177,12 @@ class FusedSandwichNormFwdOp(_SandwichNormOp):
                 post_bias: Optional[torch.Tensor] = None,
                 pre_bias: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Return ``(y, residual_out)``, both shaped like ``x``."""
-        M = self._check((("x", x), ("residual", residual)),
-                        (("post_weight", post_weight), ("pre_weight", pre_weight),
-                         ("post_bias", post_bias), ("pre_bias", pre_bias)), gate)
-        N = self.N
-        y, residual_out = self._get_kernel(x.device.index)(
-            _flat(x, M, N), _flat(residual, M, N), _param(post_weight), _param(pre_weight),
-            None if gate is None else gate.contiguous().view(-1, N), _param(post_bias),
-            _param(pre_bias))
-        return y.view(x.shape), residual_out.view(x.shape)
+        self._check(("x", x, "residual", residual),
+                    ("post_weight", post_weight, "pre_weight", pre_weight,
+                     "post_bias", post_bias, "pre_bias", pre_bias), gate)
+        return self._get_kernel(x.device.index)(
+            x.contiguous(), residual.contiguous(), post_weight.contiguous(),
+            pre_weight.contiguous(), _dense(gate), _dense(post_bias), _dense(pre_bias))
 
     def eval_roofline(self) -> tuple[int, int]:
         """``(14 * M * N, 4 * M * N * elem_bytes + the parameters once)`` of the last forward."""
@@ -197,19 +204,14 @@ class FusedSandwichNormBwdOp(_SandwichNormOp):
                 pre_bias: Optional[torch.Tensor] = None):
         """Return ``(dx, d_residual, d_post_weight, d_pre_weight, d_gate, d_post_bias,
         d_pre_bias)``, None in the place of a gradient of what was None."""
-        M = self._check((("x", x), ("dy", dy), ("d_residual_out", d_residual_out),
-                         ("residual_out", residual_out)),
-                        (("post_weight", post_weight), ("pre_weight", pre_weight),
-                         ("post_bias", post_bias), ("pre_bias", pre_bias)), gate)
-        N = self.N
-        dx, d_residual, *grads = self._get_kernel(x.device.index)(
-            _flat(dy, M, N), _flat(d_residual_out, M, N), _flat(x, M, N),
-            _flat(residual_out, M, N), _param(post_weight), _param(pre_weight),
-            None if gate is None else gate.contiguous().view(-1, N), _param(post_bias),
-            _param(pre_bias))
-        if gate is not None:
-            grads[2] = grads[2].view(gate.shape)
-        return dx.view(x.shape), d_residual.view(x.shape), *grads
+        self._check(("x", x, "dy", dy, "d_residual_out", d_residual_out,
+                     "residual_out", residual_out),
+                    ("post_weight", post_weight, "pre_weight", pre_weight,
+                     "post_bias", post_bias, "pre_bias", pre_bias), gate)
+        return self._get_kernel(x.device.index)(
+            dy.contiguous(), _dense(d_residual_out), x.contiguous(), residual_out.contiguous(),
+            post_weight.contiguous(), pre_weight.contiguous(), _dense(gate), _dense(post_bias),
+            _dense(pre_bias))
 
     def eval_roofline(self) -> tuple[int, int]:
         """``(30 * M * N, 6 * M * N * elem_bytes + the parameters and their gradients)``."""
