@@ -1154,17 +1154,53 @@ __global__ void __launch_bounds__(128)
   dlam[d] = -s * c / (1.0f + expf(-lam[d]));
 }
 
-template <typename T>
+// ---- one token ----
+// Four channels a thread where every row starts on the boundary of four (kVec = 4), one
+// otherwise.  A thread reads all it needs before it writes, so hn may be h0.
+template <typename T, int kVec>
 __global__ void __launch_bounds__(128)
     glr_decode(const T* x, const T* ig, const T* rg, const float* lam, const float* h0, T* y,
                float* hn, int64_t D, Strides st, float c) {
-  const int64_t d = blockIdx.x * 128ll + threadIdx.x, b = blockIdx.y;
+  const int64_t d = (blockIdx.x * 128ll + threadIdx.x) * kVec, b = blockIdx.y;
   if (d >= D) return;
-  const Gates g = gates_of(Cvt<T>::to_f(ig[b * st.ib + d]), Cvt<T>::to_f(rg[b * st.rb + d]),
-                           decay_rate(lam[d], c));
-  const float h = fmaf(g.a, h0[b * D + d], sqrtf(g.m2) * g.si * Cvt<T>::to_f(x[b * st.xb + d]));
-  y[b * D + d] = Cvt<T>::from_f(h);
-  hn[b * D + d] = h;
+  T xv[kVec], iv[kVec], rv[kVec], yv[kVec];
+  float lv[kVec], hv[kVec];
+  auto load = [](auto* to, const auto* from) {
+    if constexpr (kVec == 1) {
+      *to = *from;
+    } else {
+      struct alignas(kVec * sizeof(*to)) Words {
+        uint32_t w[kVec * sizeof(*to) / 4];
+      };
+      const Words words = *reinterpret_cast<const Words*>(from);
+      memcpy(to, &words, sizeof(words));
+    }
+  };
+  auto store = [](auto* to, const auto* from) {
+    if constexpr (kVec == 1) {
+      *to = *from;
+    } else {
+      struct alignas(kVec * sizeof(*to)) Words {
+        uint32_t w[kVec * sizeof(*to) / 4];
+      };
+      Words words;
+      memcpy(&words, from, sizeof(words));
+      *reinterpret_cast<Words*>(to) = words;
+    }
+  };
+  load(lv, lam + d);
+  load(hv, h0 + b * D + d);
+  load(iv, ig + b * st.ib + d);
+  load(rv, rg + b * st.rb + d);
+  load(xv, x + b * st.xb + d);
+#pragma unroll
+  for (int v = 0; v < kVec; ++v) {
+    const Gates g = gates_of(Cvt<T>::to_f(iv[v]), Cvt<T>::to_f(rv[v]), decay_rate(lv[v], c));
+    hv[v] = fmaf(g.a, hv[v], sqrt_approx_f(g.m2) * g.si * Cvt<T>::to_f(xv[v]));
+    yv[v] = Cvt<T>::from_f(hv[v]);
+  }
+  store(y + b * D + d, yv);
+  store(hn + b * D + d, hv);
 }
 
 // Sizes every kernel here indexes with: batch in a grid's y, token counts in an int (with
@@ -1265,13 +1301,22 @@ extern "C" int tileops_glr_decode_fwd(const void* x, const void* input_gate,
     return TILEOPS_EINVAL;
   cudaStream_t s = as_stream(stream);
   const Strides st{x_stride, 0, i_stride, 0, r_stride, 0, 0, 0};
-  const dim3 grid(static_cast<unsigned>((dim + 127) / 128), static_cast<unsigned>(batch));
   const float c = static_cast<float>(decay_scale);
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    glr_decode<T><<<grid, 128, 0, s>>>(static_cast<const T*>(x), static_cast<const T*>(input_gate),
-                                       static_cast<const T*>(decay_gate), decay_param, state,
-                                       static_cast<T*>(y), new_state, dim, st, c);
+    auto fits = [](const void* p, int64_t stride, size_t itemsize) {
+      return reinterpret_cast<uintptr_t>(p) % (4 * itemsize) == 0 && stride % 4 == 0;
+    };
+    const bool vec = fits(x, x_stride, sizeof(T)) && fits(input_gate, i_stride, sizeof(T)) &&
+                     fits(decay_gate, r_stride, sizeof(T)) && fits(y, dim, sizeof(T)) &&
+                     fits(state, dim, 4) && fits(new_state, dim, 4) && fits(decay_param, 4, 4);
+    const int64_t per_cta = vec ? 512 : 128;
+    const dim3 grid(static_cast<unsigned>((dim + per_cta - 1) / per_cta),
+                    static_cast<unsigned>(batch));
+    auto kernel = vec ? glr_decode<T, 4> : glr_decode<T, 1>;
+    kernel<<<grid, 128, 0, s>>>(static_cast<const T*>(x), static_cast<const T*>(input_gate),
+                                static_cast<const T*>(decay_gate), decay_param, state,
+                                static_cast<T*>(y), new_state, dim, st, c);
     return launch_status();
   };
   switch (dtype) {

@@ -221,17 +221,41 @@ __device__ __forceinline__ float squares_of(const float2 (&v)[kPackets][C::kP],
   return total(sq);
 }
 
-// Parameters of a thread's columns (zero where there are none).
-template <typename C, typename W, int kPackets, typename F>
+// Parameters of a thread's columns: `otherwise` where there is no vector p, zero where there
+// is no column.  vec: p starts on a 16-byte boundary (and rows are aligned).
+template <typename C, typename W, int kPackets>
 __device__ __forceinline__ void load_params(float2 (&v)[kPackets][C::kP], const int (&n)[kPackets],
-                                            F at) {
+                                            const W* p, float otherwise, bool vec) {
+#pragma unroll
+  for (int j = 0; j < kPackets; ++j) {
+    const int c = C::first(j);
+    if (C::kWhole && vec && p) {
+      constexpr int kWords = C::kV * sizeof(W) / 16;  // 16-byte words of a packet's parameters
+      alignas(16) W e[C::kV];
+      if (n[j] > 0) {
+#pragma unroll
+        for (int q = 0; q < kWords; ++q)
+          reinterpret_cast<uint4*>(e)[q] = __ldg(reinterpret_cast<const uint4*>(p + c) + q);
+      }
+#pragma unroll
+      for (int i = 0; i < C::kP; ++i)
+        v[j][i] = n[j] > 0 ? make_float2(Cvt<W>::to_f(e[2 * i]), Cvt<W>::to_f(e[2 * i + 1]))
+                           : both(0.0f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C::kP; ++i)
+        v[j][i] = make_float2(2 * i < n[j] ? param(p, c + 2 * i, otherwise) : 0.0f,
+                              2 * i + 1 < n[j] ? param(p, c + 2 * i + 1, otherwise) : 0.0f);
+    }
+  }
+}
+template <typename C, int kPackets>
+__device__ __forceinline__ void multiply(float2 (&v)[kPackets][C::kP],
+                                         const float2 (&by)[kPackets][C::kP]) {
 #pragma unroll
   for (int j = 0; j < kPackets; ++j)
 #pragma unroll
-    for (int i = 0; i < C::kP; ++i) {
-      const int c = C::first(j) + 2 * i;
-      v[j][i] = make_float2(2 * i < n[j] ? at(c) : 0.0f, 2 * i + 1 < n[j] ? at(c + 1) : 0.0f);
-    }
+    for (int i = 0; i < C::kP; ++i) v[j][i] = fmul2(v[j][i], by[j][i]);
 }
 
 // ---- forward ----
@@ -243,6 +267,7 @@ struct FwdArgs {
   int64_t rows_per_group;
   bool layer;
   float eps, alpha;
+  bool vec;  // every parameter vector starts on a 16-byte boundary
 };
 
 template <typename T, typename W, int kThreads, int kPackets, int kStages, bool kAligned>
@@ -278,8 +303,8 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
 #pragma unroll
   for (int j = 0; j < kPackets; ++j) n[j] = C::count(j, N);
   float2 wg[kPackets][kP], bg[kPackets][kP], wn[kPackets][kP], bn[kPackets][kP];
-  load_params<C, W, kPackets>(wn, n, [&](int c) { return Cvt<W>::to_f(w2[c]); });
-  load_params<C, W, kPackets>(bn, n, [&](int c) { return param(b2, c, 0.0f); });
+  load_params<C>(wn, n, w2, 0.0f, p.vec);
+  load_params<C>(bn, n, b2, 0.0f, p.vec);
   const float inv_n = 1.0f / static_cast<float>(N);
   const float mine = in_warp<C, kThreads, kPackets>(warp, N);
   const float inv_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
@@ -348,9 +373,12 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
     if (row >= next_group) {
       const int64_t g = row / p.rows_per_group;
       next_group = (g + 1) * p.rows_per_group;
-      auto gate_at = [&](int c) { return param(gate, g * N + c, 1.0f); };
-      load_params<C, W, kPackets>(wg, n, [&](int c) { return gate_at(c) * Cvt<W>::to_f(w1[c]); });
-      load_params<C, W, kPackets>(bg, n, [&](int c) { return gate_at(c) * param(b1, c, 0.0f); });
+      float2 ga[kPackets][kP];
+      load_params<C>(ga, n, gate ? gate + g * N : nullptr, 1.0f, p.vec);
+      load_params<C>(wg, n, w1, 0.0f, p.vec);
+      load_params<C>(bg, n, b1, 0.0f, p.vec);
+      multiply<C>(wg, ga);
+      multiply<C>(bg, ga);
     }
     T* out = static_cast<T*>(p.res_out) + row * N;
 #pragma unroll
@@ -402,6 +430,7 @@ struct BwdArgs {
   int64_t rows_per_group;
   bool layer;
   float eps, alpha;
+  bool vec;  // every parameter vector starts on a 16-byte boundary
 };
 
 // Column sums of one stretch of rows (one CTA, one group): kBias ? P, Q, R, S : P, R, rows of N.
@@ -411,9 +440,9 @@ __device__ __forceinline__ float* stretch(float* part, int64_t c, int64_t g, int
   return part + (c + g) * sums * N;
 }
 
-template <typename T, typename W, int kThreads, int kPackets, int kStages, bool kAligned,
+template <typename T, typename W, int kThreads, int kPackets, int kStages, int kCtas, bool kAligned,
           bool kBias>
-__global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
+__global__ void __launch_bounds__(kThreads, kCtas) sn_bwd(const BwdArgs p) {
   using C = Cols<T, kThreads, kPackets, kAligned>;
   constexpr int kP = C::kP, kWarps = kThreads / 32, kSums = kBias ? 4 : 2;
   extern __shared__ uint4 ring[];  // [stage][x, s, dy, ds][packet][thread]
@@ -448,7 +477,7 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
   for (int j = 0; j < kPackets; ++j) n[j] = C::count(j, N);
   float2 wg[kPackets][kP], wn[kPackets][kP];
   float2 P[kPackets][kP], R[kPackets][kP], Q[kBias ? kPackets : 1][kP], S[kBias ? kPackets : 1][kP];
-  load_params<C, W, kPackets>(wn, n, [&](int c) { return Cvt<W>::to_f(w2[c]); });
+  load_params<C>(wn, n, w2, 0.0f, p.vec);
   auto clear = [&] {
 #pragma unroll
     for (int j = 0; j < kPackets; ++j)
@@ -467,35 +496,32 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
   const float inv_theirs = theirs > 0.0f ? 1.0f / theirs : 0.0f;
   auto give = [&](int64_t g) {  // the column sums of the rows so far, which are of group g
     float* to = stretch(p.part, blockIdx.x, g, kSums, N);
-    auto put = [&](int which, const float2& v, int c, int left) {
-      if (left > 0) to[which * static_cast<int64_t>(N) + c] = v.x;
-      if (left > 1) to[which * static_cast<int64_t>(N) + c + 1] = v.y;
+    auto put = [&](int which, const float2& v, const float2& w, int c, int left) {
+      float* at = to + which * static_cast<int64_t>(N) + c;
+      if constexpr (kAligned) {
+        if (left > 0) *reinterpret_cast<float4*>(at) = make_float4(v.x, v.y, w.x, w.y);
+      } else {
+        if (left > 0) at[0] = v.x;
+        if (left > 1) at[1] = v.y;
+        if (left > 2) at[2] = w.x;
+        if (left > 3) at[3] = w.y;
+      }
     };
 #pragma unroll
     for (int j = 0; j < kPackets; ++j)
 #pragma unroll
-      for (int i = 0; i < kP; ++i) {
+      for (int i = 0; i < kP; i += 2) {
         const int c = C::first(j) + 2 * i, left = n[j] - 2 * i;
-        put(0, P[j][i], c, left);
-        put(1, R[j][i], c, left);
-        if (kBias) {
-          put(2, Q[j][i], c, left);
-          put(3, S[j][i], c, left);
+        put(0, P[j][i], P[j][i + 1], c, left);
+        put(1, R[j][i], R[j][i + 1], c, left);
+        if constexpr (kBias) {
+          put(2, Q[j][i], Q[j][i + 1], c, left);
+          put(3, S[j][i], S[j][i + 1], c, left);
         }
       }
     clear();
   };
 
-  auto read = [&](int stage, int tensor, float2 (&v)[kPackets][kP]) {
-#pragma unroll
-    for (int j = 0; j < kPackets; ++j) {
-      if (n[j] > 0)
-        C::read(slot(stage, tensor, j), v[j]);
-      else
-#pragma unroll
-        for (int i = 0; i < kP; ++i) v[j][i] = both(0.0f);
-    }
-  };
   // One exchange: of the row in `stage` the statistics of x and s, and of f = dy w2 with the
   // centred s; of the row before it E = sum e and Ex = sum e x^ (the thread's
   // sums), which come back over the CTA.
@@ -506,31 +532,42 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
   auto exchange = [&](int stage, float& E, float& Ex) {
     WarpSums<8, kWarps>& buf = sums[par];
     par ^= 1;
-    float2 xv[kPackets][kP], sv[kPackets][kP];
-    read(stage, 0, xv);
-    read(stage, 1, sv);
+    // The row's packets are read from the ring in each pass: held in registers they would
+    // cost a second resident CTA.
     float m[2] = {0.0f, 0.0f};
     if (layer) {
-      m[0] = sum_of<C, kPackets>(xv);
-      m[1] = sum_of<C, kPackets>(sv);
+#pragma unroll
+      for (int j = 0; j < kPackets; ++j)
+        if (n[j] > 0) {
+          float2 xv[1][kP], sv[1][kP];
+          C::read(slot(stage, 0, j), xv[0]);
+          C::read(slot(stage, 1, j), sv[0]);
+          m[0] += sum_of<C, 1>(xv);
+          m[1] += sum_of<C, 1>(sv);
+        }
       warp_sums(m);
     }
-    const float mean_sw = m[1] * inv_mine;
+    const float mean_xw = m[0] * inv_mine, mean_sw = m[1] * inv_mine;
     float2 F2 = both(0.0f), Fs2 = both(0.0f);
+    float q[4] = {0.0f, 0.0f, 0.0f, Ex};
 #pragma unroll
     for (int j = 0; j < kPackets; ++j)
       if (n[j] > 0) {
-        float2 g[kP];
+        float2 xv[1][kP], sv[1][kP], g[kP];
+        const int one[1] = {n[j]};
+        C::read(slot(stage, 0, j), xv[0]);
+        C::read(slot(stage, 1, j), sv[0]);
         C::read(slot(stage, 2, j), g);
+        q[0] += squares_of<C, 1>(xv, one, layer, mean_xw);
+        q[1] += squares_of<C, 1>(sv, one, layer, mean_sw);
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
           const float2 f = fmul2(g[i], wn[j][i]);
           F2 = fadd2(F2, f);
-          Fs2 = ffma2(f, fadd2(sv[j][i], both(-mean_sw)), Fs2);
+          Fs2 = ffma2(f, fadd2(sv[0][i], both(-mean_sw)), Fs2);
         }
       }
-    float q[4] = {squares_of<C, kPackets>(xv, n, layer, m[0] * inv_mine),
-                  squares_of<C, kPackets>(sv, n, layer, mean_sw), total(Fs2), Ex};
+    q[2] = total(Fs2);
     float l[2] = {total(F2), E};
     warp_sums(q);
     if (layer) warp_sums(l);
@@ -584,19 +621,21 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
       if (row > row0) give(group);
       group = row / p.rows_per_group;
       next_group = (group + 1) * p.rows_per_group;
-      load_params<C, W, kPackets>(
-          wg, n, [&](int c) { return param(gate, group * N + c, 1.0f) * Cvt<W>::to_f(w1[c]); });
+      float2 ga[kPackets][kP];
+      load_params<C>(ga, n, gate ? gate + group * N : nullptr, 1.0f, p.vec);
+      load_params<C>(wg, n, w1, 0.0f, p.vec);
+      multiply<C>(wg, ga);
     }
-    // ds' and the sums for dx; xv becomes x^, sv becomes e.
-    float2 xv[kPackets][kP], sv[kPackets][kP];
+    // ds' and the sums for dx; e is kept for it.
+    float2 ev[kPackets][kP];
     T* dres = static_cast<T*>(p.dres) + row * N;
     float2 E2 = both(0.0f), Ex2 = both(0.0f);
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
-        float2 t[kP], g[kP];
-        C::read(slot(stage, 0, j), xv[j]);
-        C::read(slot(stage, 1, j), sv[j]);
+        float2 t[kP], g[kP], xv[kP], sv[kP];
+        C::read(slot(stage, 0, j), xv);
+        C::read(slot(stage, 1, j), sv);
         C::read(slot(stage, 2, j), g);
         if (ds) {
           C::read(slot(stage, 3, j), t);
@@ -606,8 +645,8 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
         }
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
-          const float2 hat = fmul2(fadd2(sv[j][i], both(-st.mean_s)), both(st.rs));
-          const float2 xh = fmul2(fadd2(xv[j][i], both(-st.mean_x)), both(st.rx));
+          const float2 hat = fmul2(fadd2(sv[i], both(-st.mean_s)), both(st.rs));
+          const float2 xh = fmul2(fadd2(xv[i], both(-st.mean_x)), both(st.rx));
           const float2 f = ffma2(g[i], wn[j][i], ffma2(hat, both(-st.mean_fs), both(-st.mean_f)));
           t[i] = ffma2(both(st.rs), f, t[i]);
           if (!kAligned && 2 * i >= n[j]) t[i].x = 0.0f;
@@ -622,28 +661,31 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
           E2 = fadd2(E2, e);
           Ex2 = ffma2(e, xh, Ex2);
           t[i] = fmul2(both(p.alpha), t[i]);
-          xv[j][i] = xh;
-          sv[j][i] = e;
+          ev[j][i] = e;
         }
         C::write(dres, j, N, t);
       }
     }
     E = total(E2);
     Ex = total(Ex2);
-    const float rx = st.rx;
+    const float rx = st.rx, mean_x = st.mean_x;
+    const int here = stage;
     fetch(stage == 0 ? kStages - 1 : stage - 1, row + kStages - 1);
     copies_wait<kStages - 2>();
     stage = stage + 1 == kStages ? 0 : stage + 1;
     st = exchange(stage, E, Ex);  // past the last row: of what an earlier one left there, unused
-    const float mean_e = E * inv_n, mean_ex = Ex * inv_n;
+    // dx = rx (e - mean e - x^ mean(e x^)), x^ = (x - mean) rx
+    const float mean_e = E * inv_n, slope = -Ex * inv_n * rx;
     T* dx = static_cast<T*>(p.dx) + row * N;
 #pragma unroll
     for (int j = 0; j < kPackets; ++j) {
       if (n[j] > 0) {
         float2 o[kP];
+        C::read(slot(here, 0, j), o);
 #pragma unroll
         for (int i = 0; i < kP; ++i)
-          o[i] = fmul2(both(rx), ffma2(xv[j][i], both(-mean_ex), fadd2(sv[j][i], both(-mean_e))));
+          o[i] = fmul2(both(rx), ffma2(fadd2(o[i], both(-mean_x)), both(slope),
+                                       fadd2(ev[j][i], both(-mean_e))));
         C::write(dx, j, N, o);
       }
     }
@@ -655,13 +697,13 @@ __global__ void __launch_bounds__(kThreads) sn_bwd(const BwdArgs p) {
 // Gradients of the parameters from the column sums of the stretches, added in a fixed
 // order: 32 columns a CTA, kSlices threads a column.  With few groups the slices
 // share the stretches of each group; with many, each takes whole groups.
-constexpr int kSlices = 16;
+constexpr int kSlices = 32;
 
 template <typename W>
 __global__ void __launch_bounds__(32 * kSlices)
     sn_params(const float* part, const W* w1, const W* gate, const W* b1, W* dw1, W* dw2, W* dgate,
               W* db1, W* db2, int64_t M, int N, int64_t G, int C, int sums) {
-  __shared__ float red[4][kSlices][33];
+  __shared__ float red[4][kSlices][32], out[4][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   const bool in = c < N;
@@ -677,19 +719,23 @@ __global__ void __launch_bounds__(32 * kSlices)
   };
   auto across = [&](float (&v)[4]) {  // sums over the slices, in every thread
 #pragma unroll
-    for (int q = 0; q < 4; ++q) red[q][slice][lane] = v[q];
+    for (int q = 0; q < 4; ++q)
+      if (q < sums) red[q][slice][lane] = v[q];
     __syncthreads();
+    if (slice < sums) {  // slice q adds up sum q
+      float sum = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      v[q] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kSlices; ++i) v[q] += red[q][i][lane];
+      for (int i = 0; i < kSlices; ++i) sum += red[slice][i][lane];
+      out[slice][lane] = sum;
     }
     __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < sums) v[q] = out[q][lane];
   };
   float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // dw1, dw2, db1, db2
   for (int64_t g = by_group ? slice : 0; g < G; g += by_group ? kSlices : 1) {
-    const int c0 = cta_of(g * rpg), c1 = cta_of((g + 1) * rpg - 1);
+    const int c0 = g == 0 ? 0 : cta_of(g * rpg), c1 = g == G - 1 ? C - 1 : cta_of((g + 1) * rpg - 1);
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // P, R, Q, S
     if (in)
 #pragma unroll 4
@@ -863,9 +909,13 @@ int launch_rows(void (*kernel)(const A), int threads, size_t smem, int64_t ctas,
   return launch_status();
 }
 
-// CTAs of the backward pass: one an SM, two or four where rows are short and so CTAs are
-// small (each adds a stretch of column sums to write and read).
-int64_t ctas_per_sm(int64_t N) { return N <= 1024 ? 4 : (N <= 2048 ? 2 : 1); }
+// CTAs an SM of the backward pass: as many as their registers allow (each adds a stretch of
+// column sums to write and read).  With biases there are twice the sums, and a row of
+// 4096 takes more than the 128 registers a thread of two CTAs has (16384 x 4096
+// bf16: two CTAs 152 us without and 284 us with biases, one 165 and 225 us).
+int64_t ctas_per_sm(int64_t N, bool bias) {
+  return N <= 1024 ? 4 : (N <= 2048 ? 2 : (N <= 4096 && !bias ? 2 : 1));
+}
 constexpr int kMaxSms = 256;  // workspace: more than any device of this architecture has
 
 template <typename T, typename W, bool kAligned>
@@ -892,10 +942,12 @@ int launch_bwd(const BwdArgs& a, int64_t ctas, cudaStream_t s) {
     return launch_rows(kernel, threads, static_cast<size_t>(stages) * 4 * per_thread * threads * 16,
                        ctas, a, s);
   };
-  if (packets <= 128) return go(sn_bwd<T, W, 128, 1, 6, kAligned, kBias>, 128, 1, 6);
-  if (packets <= 256) return go(sn_bwd<T, W, 256, 1, 5, kAligned, kBias>, 256, 1, 5);
-  if (packets <= 512) return go(sn_bwd<T, W, 512, 1, 4, kAligned, kBias>, 512, 1, 4);
-  if (packets <= 1024) return go(sn_bwd<T, W, 512, 2, 3, kAligned, kBias>, 512, 2, 3);
+  if (packets <= 128) return go(sn_bwd<T, W, 128, 1, 6, 4, kAligned, kBias>, 128, 1, 6);
+  if (packets <= 256) return go(sn_bwd<T, W, 256, 1, 5, 2, kAligned, kBias>, 256, 1, 5);
+  if (packets <= 512)
+    return kBias ? go(sn_bwd<T, W, 256, 2, 4, 1, kAligned, kBias>, 256, 2, 4)
+                 : go(sn_bwd<T, W, 256, 2, 3, 2, kAligned, kBias>, 256, 2, 3);
+  if (packets <= 1024) return go(sn_bwd<T, W, 512, 2, 3, 1, kAligned, kBias>, 512, 2, 3);
   sn_bwd_wide<T, W, kBias><<<static_cast<unsigned>(ctas), 1024, 0, s>>>(a);
   return launch_status();
 }
@@ -920,7 +972,9 @@ extern "C" int tileops_sandwich_norm_fwd(const void* x, const void* residual,
   const FwdArgs args{x, residual, post_weight, pre_weight, gate, post_bias, pre_bias, y,
                      residual_out, M, static_cast<int>(N), M / gate_rows,
                      norm == TILEOPS_NORM_LAYER, static_cast<float>(eps),
-                     static_cast<float>(residual_scale)};
+                     static_cast<float>(residual_scale),
+                     aligned16(post_weight) && aligned16(pre_weight) && aligned16(gate) &&
+                         aligned16(post_bias) && aligned16(pre_bias)};
   return with_types(dtype, affine_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
@@ -934,7 +988,7 @@ extern "C" int tileops_sandwich_norm_fwd(const void* x, const void* residual,
 extern "C" int64_t tileops_sandwich_norm_bwd_workspace_bytes(int64_t M, int64_t N,
                                                              int64_t gate_rows, int has_bias) {
   if (bad_shape(M, N, gate_rows)) return -1;
-  return (std::min<int64_t>(M, kMaxSms * ctas_per_sm(N)) + gate_rows) * (has_bias ? 4 : 2) * N * 4;
+  return (std::min<int64_t>(M, kMaxSms * ctas_per_sm(N, has_bias)) + gate_rows) * (has_bias ? 4 : 2) * N * 4;
 }
 
 extern "C" int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_out, const void* x,
@@ -960,8 +1014,9 @@ extern "C" int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_
   const BwdArgs args{dy, d_residual_out, x, residual_out, post_weight, pre_weight, gate, dx,
                      d_residual, part, M, static_cast<int>(N), M / gate_rows,
                      norm == TILEOPS_NORM_LAYER, static_cast<float>(eps),
-                     static_cast<float>(residual_scale)};
-  const int64_t ctas = std::min<int64_t>(M, std::min(sm_count(), kMaxSms) * ctas_per_sm(N));
+                     static_cast<float>(residual_scale),
+                     aligned16(post_weight) && aligned16(pre_weight) && aligned16(gate)};
+  const int64_t ctas = std::min<int64_t>(M, std::min(sm_count(), kMaxSms) * ctas_per_sm(N, bias));
   return with_types(dtype, affine_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);

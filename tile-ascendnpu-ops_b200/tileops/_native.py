@@ -194,9 +194,12 @@ def launch(name: str, device: torch.device, *args) -> None:
     """
     if device.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a cuda device, got {device}")
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    if idx != torch.cuda.current_device():
+    current = torch.cuda.current_device()
+    idx = device.index if device.index is not None else current
+    # The stream's handle by itself costs 0.1 us, a torch.cuda.Stream object around it 2.5 us.
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    if idx != current:
         with torch.cuda.device(idx):
-            call(name, *args, stream_handle(device))
+            call(name, *args, stream)
     else:
-        call(name, *args, stream_handle(device))
+        call(name, *args, stream)
