@@ -155,7 +155,8 @@ int tileops_sandwich_norm_fwd(const void* x, const void* residual, const void* p
                               double residual_scale, int dtype, int affine_dtype, void* stream);
 
 /* Bytes of scratch tileops_sandwich_norm_bwd needs, or -1 for an unsupported
- * shape.  has_bias: post_bias or pre_bias has a gradient. */
+ * shape: two fp32 rows (four with has_bias: there is a post_bias or a gradient
+ * of pre_bias) for each of up to 1024 stretches of rows and for each gate row. */
 int64_t tileops_sandwich_norm_bwd_workspace_bytes(int64_t M, int64_t N, int64_t gate_rows,
                                                   int has_bias);
 
@@ -253,7 +254,9 @@ int tileops_gla_decode_fwd(const void* q, const void* k, const void* v, const vo
  * cu_seqlens (NULL = one sequence per batch row): an int32 DEVICE array of
  * num_seqs + 1 offsets, batch 1, the rules of tileops_gdn_prefill_varlen_fwd
  * (0 = cu[0] <= ... <= cu[num_seqs] = seq_len; device error 2 and meaningless
- * results otherwise, never an access out of range).  batch up to 65535,
+ * results otherwise, never an access out of range; num_seqs below 2^30).  The
+ * first packed call on a device looks up the device error word: make it outside
+ * any stream capture.  batch up to 65535,
  * seq_len 1 .. 2^31 - 2^16.  No output may alias an input.  No counterpart in the
  * reference. */
 int tileops_glr_fwd(const void* x, const void* input_gate, const void* decay_gate,

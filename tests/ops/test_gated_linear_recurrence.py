@@ -85,6 +85,29 @@ def test_long_and_wide(B, T, D):
     _check_all(*_inputs(B, T, D, torch.bfloat16))
 
 
+@pytest.mark.parametrize("B, T, D", [
+    (3, 1100, 1024),   # CTAs of 32 channels that have an SM each, several steps
+    (1, 2100, 1600),   # of 16 channels
+    (1, 1500, 1000),   # clusters of two
+    (1, 5000, 272),    # clusters of eight
+    (40, 700, 200),    # more CTAs than SMs
+])
+@pytest.mark.parametrize("packed", [False, True])
+def test_every_split_of_the_tokens(B, T, D, packed):
+    """Long enough for each choice of warps and clusters to take several steps."""
+    if packed:
+        B = 1
+        cuts = torch.randint(0, T + 1, (20,)).sort().values.tolist()
+        lengths = [b - a for a, b in zip([0, *cuts], [*cuts, T])]
+        _check_all(*_inputs(1, T, D, torch.bfloat16, nseq=21), cu=_cu(lengths))
+    else:
+        _check_all(*_inputs(B, T, D, torch.bfloat16))
+
+
+def test_many_partial_sums():
+    _check_all(*_inputs(300, 5, 40, torch.float32))
+
+
 def test_without_states():
     gates, _, dy, _ = _inputs(2, 100, 66, torch.float32)
     y, final = GatedLinearRecurrenceFwdOp(2, 100, 66, dtype=torch.float32)(*gates)

@@ -313,7 +313,7 @@ extern "C" int tileops_glr_fwd(const void* x, const void* input_gate, const void
                                int64_t i_stride_b, int64_t i_stride_t, int64_t r_stride_b,
                                int64_t r_stride_t, double decay_scale, int dtype, void* stream) {
   if (bad_shape(batch, seq_len, dim)) return TILEOPS_EBADSHAPE;
-  if (cu_seqlens && (batch != 1 || num_seqs < 1 || num_seqs > 0x7ffffffeLL))
+  if (cu_seqlens && (batch != 1 || num_seqs < 1 || num_seqs > 0x3fffffffLL))
     return TILEOPS_EBADSHAPE;
   if (!is_float_dtype(dtype)) return TILEOPS_EBADDTYPE;
   if (batch == 0 || dim == 0) return TILEOPS_OK;

@@ -342,14 +342,24 @@ int launch_bwd(const BwdArgs& a, int64_t batch, cudaStream_t s, int64_t* parts) 
   return launch_bwd_geo<T, Eight, 4>(a, batch, s, parts);
 }
 
-// dlambda = c sigmoid(lambda) sum of the partial sums, added in a fixed order.
-__global__ void __launch_bounds__(128)
+// dlambda = -c sigmoid(lambda) sum of the partial sums, added in a fixed order: 32 channels
+// a CTA, eight threads a channel.
+__global__ void __launch_bounds__(256)
     glr_dparam(const float* part, const float* lam, float* dlam, int64_t parts, int64_t D, float c) {
-  const int64_t d = blockIdx.x * 128ll + threadIdx.x;
-  if (d >= D) return;
+  __shared__ float red[8][32];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int64_t d = blockIdx.x * 32ll + lane;
   float s = 0.0f;
-  for (int64_t p = 0; p < parts; ++p) s += part[p * D + d];
-  dlam[d] = -s * c / (1.0f + expf(-lam[d]));
+  if (d < D)
+#pragma unroll 4
+    for (int64_t p = slice; p < parts; p += 8) s += part[p * D + d];
+  red[slice][lane] = s;
+  __syncthreads();
+  if (slice == 0 && d < D) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i][lane];
+    dlam[d] = -s * c / (1.0f + expf(-lam[d]));
+  }
 }
 
 }  // namespace
@@ -373,7 +383,7 @@ extern "C" int tileops_glr_bwd(const void* dy, const void* x, const void* input_
                                int64_t i_stride_b, int64_t i_stride_t, int64_t r_stride_b,
                                int64_t r_stride_t, double decay_scale, int dtype, void* stream) {
   if (bad_shape(batch, seq_len, dim)) return TILEOPS_EBADSHAPE;
-  if (cu_seqlens && (batch != 1 || num_seqs < 1 || num_seqs > 0x7ffffffeLL))
+  if (cu_seqlens && (batch != 1 || num_seqs < 1 || num_seqs > 0x3fffffffLL))
     return TILEOPS_EBADSHAPE;
   if (!is_float_dtype(dtype)) return TILEOPS_EBADDTYPE;
   if (batch == 0 || dim == 0) return TILEOPS_OK;
@@ -398,8 +408,8 @@ extern "C" int tileops_glr_bwd(const void* dy, const void* x, const void* input_
     default: status = launch_bwd<__nv_bfloat16>(args, batch, s, &parts);
   }
   if (status != TILEOPS_OK) return status;
-  glr_dparam<<<static_cast<unsigned>((dim + 127) / 128), 128, 0, s>>>(part, decay_param,
-                                                                      d_decay_param, parts, dim, c);
+  glr_dparam<<<static_cast<unsigned>((dim + 31) / 32), 256, 0, s>>>(part, decay_param,
+                                                                    d_decay_param, parts, dim, c);
   return launch_status();
 }
 
