@@ -76,6 +76,9 @@ __device__ __forceinline__ TokenGrads token_grads(float2 g, float2 hp, float2 x,
 // H = a_t (dy_t + H).  The states h are walked anew from the forward's saved ones, one a
 // warp's run.  A lane takes 8 tokens: decay, state and both sigmoids of each stay in
 // registers, so no element's gates are computed twice but for m.
+// An element takes 82 issue slots (6 on the special-function unit), and that bounds it: 8 x
+// 4096 x 4096 bf16 takes 450 us, 4.2 TB/s of its 14.25 bytes an element, 0.64 of
+// the copy rate, with 58 to 64% of the issue slots used.
 template <typename T, typename G, int kBytes, bool kPacked, int kStages>
 __global__ void __launch_bounds__(G::kWarps * 32, G::kCtas)
     glr_bwd_scan(const __grid_constant__ BwdArgs p) {
