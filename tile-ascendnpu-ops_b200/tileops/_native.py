@@ -161,11 +161,17 @@ def status_string(status: int) -> str:
     return lib().tileops_status_string(status).decode()
 
 
+_functions: dict[str, object] = {}  # entry points called so far
+
+
 def call(name: str, *args) -> None:
     """Invoke entry point ``name``; raise on a non-zero status."""
-    fn = getattr(lib(), name, None)
+    fn = _functions.get(name)
     if fn is None:
-        raise NativeLibraryError(f"{LIB_PATH.name} does not export {name}")
+        fn = getattr(lib(), name, None)
+        if fn is None:
+            raise NativeLibraryError(f"{LIB_PATH.name} does not export {name}")
+        _functions[name] = fn
     status = fn(*args)
     if status == OK:
         return

@@ -26,6 +26,13 @@ def _channels_last(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _rows_like(t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
+    """A dense output (``empty_like`` costs the host half of what ``empty`` does)."""
+    if t.dtype is dtype and t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(shape, dtype=dtype, device=t.device)
+
+
 class _GatedLinearRecurrenceKernel(Kernel):
     SUPPORTED_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -43,6 +50,7 @@ class _GatedLinearRecurrenceKernel(Kernel):
         self.decay_scale = float(decay_scale)
         self.dtype = dtype
         self._code = _native.dtype_code(dtype)
+        self._ws_bytes: Optional[int] = None
         self.init_config(config)
 
     def _sequences(self, cu_seqlens, device):
@@ -70,14 +78,15 @@ class GatedLinearRecurrenceFwdKernel(_GatedLinearRecurrenceKernel):
         cu, nseq = self._sequences(cu_seqlens, dev)
         if initial_state is not None:
             initial_state = initial_state.contiguous()
-        y = torch.empty((B, T, D), dtype=self.dtype, device=dev)
+        y = _rows_like(x, self.dtype, (B, T, D))
         states = (torch.empty((B, -(-T // SEGMENT), D), dtype=torch.float32, device=dev)
                   if save_states else None)
         if B == 0 or T == 0 or nseq == 0:  # no token anywhere: every sequence ends where it began
             final = (torch.zeros((nseq, D), dtype=torch.float32, device=dev)
                      if initial_state is None else initial_state.clone())
             return y, final, states
-        final = torch.empty((nseq, D), dtype=torch.float32, device=dev)
+        final = (torch.empty((nseq, D), dtype=torch.float32, device=dev)
+                 if initial_state is None else torch.empty_like(initial_state))
         x, input_gate, decay_gate = map(_channels_last, (x, input_gate, decay_gate))
         decay_param = decay_param.contiguous()
         _native.launch(
@@ -101,15 +110,16 @@ class GatedLinearRecurrenceBwdKernel(_GatedLinearRecurrenceKernel):
             initial_state = initial_state.contiguous()
         if d_final_state is not None:
             d_final_state = d_final_state.contiguous()
-        dx, di, dr = (torch.empty((B, T, D), dtype=self.dtype, device=dev) for _ in range(3))
+        dx, di, dr = (_rows_like(t, self.dtype, (B, T, D)) for t in (x, input_gate, decay_gate))
         if B == 0 or T == 0 or nseq == 0:
             d_initial = (torch.zeros((nseq, D), dtype=torch.float32, device=dev)
                          if d_final_state is None else d_final_state.clone())
             return dx, di, dr, torch.zeros(D, dtype=torch.float32, device=dev), d_initial
         d_param = torch.empty(D, dtype=torch.float32, device=dev)
         d_initial = torch.empty((nseq, D), dtype=torch.float32, device=dev)
-        ws = torch.empty(_native.lib().tileops_glr_bwd_workspace_bytes(B, T, D),
-                         dtype=torch.uint8, device=dev)
+        if self._ws_bytes is None:
+            self._ws_bytes = _native.lib().tileops_glr_bwd_workspace_bytes(B, T, D)
+        ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=dev)
         dy, x, input_gate, decay_gate = map(_channels_last, (dy, x, input_gate, decay_gate))
         decay_param, states = decay_param.contiguous(), states.contiguous()
         _native.launch(
@@ -138,8 +148,8 @@ class GatedLinearRecurrenceDecodeKernel(_GatedLinearRecurrenceKernel):
     def forward(self, x, input_gate, decay_gate, decay_param, state, inplace: bool = False):
         """Return ``(y, new_state)``; ``inplace`` writes the new state over ``state``."""
         B, D, dev = self.batch, self.dim, x.device
-        x, input_gate, decay_gate = map(_channels_last, (x, input_gate, decay_gate))
-        decay_param = decay_param.contiguous()
+        x, input_gate = _channels_last(x), _channels_last(input_gate)
+        decay_gate, decay_param = _channels_last(decay_gate), decay_param.contiguous()
         if not inplace:
             state = state.contiguous()
         y = torch.empty_like(x)  # dense: rows of contiguous channels

@@ -33,6 +33,7 @@ class _SandwichNormKernel(Kernel):
         self.eps, self.residual_scale = float(eps), float(residual_scale)
         self.dtype = dtype
         self._code, self._norm_code = _native.dtype_code(dtype), NORMS[norm]
+        self._ws_bytes: dict = {}
         self.init_config(config)
 
 
@@ -76,8 +77,11 @@ class FusedSandwichNormBwdKernel(_SandwichNormKernel):
             return dx, d_residual, *(None if g is None else g.zero_() for g in grads)
         groups = 1 if gate is None else gate.numel() // self.N
         ptr = _native.data_ptr
-        size = _native.lib().tileops_sandwich_norm_bwd_workspace_bytes(
-            self.M, self.N, groups, post_bias is not None or pre_bias is not None)
+        key = (groups, post_bias is not None or pre_bias is not None)
+        size = self._ws_bytes.get(key)
+        if size is None:
+            size = self._ws_bytes[key] = _native.lib().tileops_sandwich_norm_bwd_workspace_bytes(
+                self.M, self.N, *key)
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         _native.launch(
             "tileops_sandwich_norm_bwd", x.device, dy.data_ptr(), ptr(d_residual_out),
