@@ -57,7 +57,7 @@ def _check_bwd(dy, ds, x, s, params, **kw):
 @pytest.mark.parametrize("dtype, affine", TYPES)
 @pytest.mark.parametrize("M, N", [
     (1, 1), (3, 2), (2, 7), (5, 64), (3, 100), (7, 1000), (4, 1024), (2, 1155), (3, 4096),
-    (2, 4097), (2, 8192), (1, 16384), (2, 20000),
+    (2, 4097), (2, 8192), (1, 16384), (2, 20000), (3, 4098), (2, 1001), (2, 20001),
 ])
 def test_sizes(M, N, dtype, affine, norm):
     x, residual, dy, ds, params = _inputs(M, N, dtype, affine)
@@ -95,6 +95,14 @@ def test_many_rows(M, N, dtype, affine, norm, bias):
     x, residual, dy, ds, params = _inputs(M, N, dtype, affine, bias=bias)
     _check_fwd(x, residual, params, norm=norm, residual_scale=1.5)
     _check_bwd(dy, ds, x, residual, params, norm=norm, residual_scale=1.5)
+
+
+@pytest.mark.parametrize("M, N, G", [(700, 10000, 7), (320, 20002, 1), (600, 8200, 600)])
+def test_many_wide_rows(M, N, G):
+    """Rows beyond a thread's registers, several a CTA, with the sums of several groups."""
+    x, residual, dy, ds, params = _inputs(M, N, torch.bfloat16, torch.float32, G)
+    _check_fwd(x, residual, params, norm="layer")
+    _check_bwd(dy, ds, x, residual, params, norm="layer")
 
 
 @pytest.mark.parametrize("M, G", [(6, 6), (6, 2), (12, 4), (400, 400), (900, 2), (1000, 8), (999, 9)])
@@ -207,6 +215,39 @@ def test_deterministic_streams_and_graphs():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_one_op_in_two_threads():
+    """An op object called by two threads, on two streams, with different sizes."""
+    from threading import Barrier, Thread
+
+    op, bwd = FusedSandwichNormFwdOp(norm="layer"), FusedSandwichNormBwdOp(norm="layer")
+    cases = [_inputs(300, 1024, torch.bfloat16, torch.float32, 3),
+             _inputs(7, 264, torch.bfloat16, torch.float32, 7)]
+
+    def both(case):
+        x, residual, dy, ds, params = case
+        y, s = op(x, residual, *params)
+        return y, s, *bwd(dy, ds, x, s, *params)
+
+    want = [both(c) for c in cases]
+    torch.cuda.synchronize()
+    got, start = [None, None], Barrier(2)
+
+    def work(n):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait()
+            for _ in range(50):
+                got[n] = both(cases[n])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_offsets_beyond_32_bits():

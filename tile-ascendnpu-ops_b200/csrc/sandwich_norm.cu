@@ -199,26 +199,39 @@ __global__ void __launch_bounds__(kThreads) sn_fwd(const FwdArgs p) {
   copies_wait<0>();
 }
 
-template <typename T, typename W>
+template <typename T, typename W, int kV>
 __global__ void __launch_bounds__(1024) sn_fwd_wide(const FwdArgs p) {
   __shared__ float red[32];
   const int64_t row = blockIdx.x, N = p.N, g = row / p.rows_per_group;
+  const int64_t first = static_cast<int64_t>(threadIdx.x) * kV, step = blockDim.x * kV;
   const T *xr = static_cast<const T*>(p.x) + row * N, *rr = static_cast<const T*>(p.res) + row * N;
   const W *w1 = static_cast<const W*>(p.w1), *w2 = static_cast<const W*>(p.w2),
           *gate = static_cast<const W*>(p.gate), *b1 = static_cast<const W*>(p.b1),
           *b2 = static_cast<const W*>(p.b2);
   T *sr = static_cast<T*>(p.res_out) + row * N, *yr = static_cast<T*>(p.y) + row * N;
-  const float2 sx =
-      row_stats([&](int64_t c) { return Cvt<T>::to_f(xr[c]); }, N, p.layer, p.eps, red);
-  for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-    const float v = (Cvt<T>::to_f(xr[c]) - sx.x) * sx.y * Cvt<W>::to_f(w1[c]) + param(b1, c, 0.0f);
-    sr[c] = Cvt<T>::from_f(fmaf(p.alpha, Cvt<T>::to_f(rr[c]), param(gate, g * N + c, 1.0f) * v));
+  const float2 sx = row_stats<kV>(xr, N, p.layer, p.eps, red);
+  float v[kV], r[kV], w[kV], o[kV], ga[kV];
+  for (int64_t c = first; c < N; c += step) {
+    load_cols<kV>(xr + c, v);
+    load_cols<kV>(rr + c, r);
+    load_vector<kV>(w1, c, 1.0f, p.vec, w);
+    load_vector<kV>(b1, c, 0.0f, p.vec, o);
+    load_vector<kV>(gate ? gate + g * N : nullptr, c, 1.0f, p.vec, ga);
+#pragma unroll
+    for (int i = 0; i < kV; ++i)
+      v[i] = fmaf(p.alpha, r[i], ga[i] * fmaf((v[i] - sx.x) * sx.y, w[i], o[i]));
+    store_cols<kV>(sr + c, v);
   }
-  const float2 ss =
-      row_stats([&](int64_t c) { return Cvt<T>::to_f(sr[c]); }, N, p.layer, p.eps, red);
-  for (int64_t c = threadIdx.x; c < N; c += blockDim.x)
-    yr[c] = Cvt<T>::from_f((Cvt<T>::to_f(sr[c]) - ss.x) * ss.y * Cvt<W>::to_f(w2[c]) +
-                           param(b2, c, 0.0f));
+  // (a thread reads back only what it wrote)
+  const float2 ss = row_stats<kV>(sr, N, p.layer, p.eps, red);
+  for (int64_t c = first; c < N; c += step) {
+    load_cols<kV>(sr + c, v);
+    load_vector<kV>(w2, c, 1.0f, p.vec, w);
+    load_vector<kV>(b2, c, 0.0f, p.vec, o);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) v[i] = fmaf((v[i] - ss.x) * ss.y, w[i], o[i]);
+    store_cols<kV>(yr + c, v);
+  }
 }
 
 template <typename T, typename W, int kBytes, bool kLayer>
@@ -234,7 +247,7 @@ int launch_fwd(const FwdArgs& a, cudaStream_t s) {
   if (packets <= 256) return go(sn_fwd<T, W, 256, 1, 4, kBytes, kLayer>, 256, 1, 4, 3);
   if (packets <= 512) return go(sn_fwd<T, W, 256, 2, 4, kBytes, kLayer>, 256, 2, 4, 2);
   if (packets <= 1024) return go(sn_fwd<T, W, 512, 2, 3, kBytes, kLayer>, 512, 2, 3, 1);
-  sn_fwd_wide<T, W><<<static_cast<unsigned>(a.M), 1024, 0, s>>>(a);
+  sn_fwd_wide<T, W, kBytes == 16 ? 16 / sizeof(T) : 1><<<static_cast<unsigned>(a.M), 1024, 0, s>>>(a);
   return launch_status();
 }
 

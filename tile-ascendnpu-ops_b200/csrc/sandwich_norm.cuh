@@ -265,7 +265,8 @@ __device__ __forceinline__ void multiply(float2 (&v)[kPackets][C::kP],
 }
 
 // ---- rows too wide for a thread's registers ----
-// Passes over the row that read it again from L2.
+// Passes over the row, which is read again from L1 or L2; kV columns at a time, a 16-byte
+// packet where rows allow it.
 __device__ __forceinline__ float block_sum(float v, float* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nwarps = (blockDim.x + 31) >> 5;
@@ -276,18 +277,68 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return warp_sum(lane < nwarps ? red[lane] : 0.0f);
 }
 
-// mean and rstd of a row read through `at`.
-template <typename F>
-__device__ __forceinline__ float2 row_stats(F at, int64_t N, bool layer, float eps, float* red) {
-  float mean = 0.0f, sq = 0.0f;
+template <int kV, typename T>
+__device__ __forceinline__ void load_cols(const T* p, float (&v)[kV], bool vec = true) {
+  constexpr int kSize = kV * static_cast<int>(sizeof(T));
+  T e[kV];
+  if (kSize % 16 == 0 && vec) {
+#pragma unroll
+    for (int q = 0; q < kSize / 16; ++q) {
+      const uint4 u = reinterpret_cast<const uint4*>(p)[q];
+      memcpy(reinterpret_cast<char*>(e) + 16 * q, &u, 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) e[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kV; ++i) v[i] = Cvt<T>::to_f(e[i]);
+}
+// kV parameters from p on, `otherwise` where there is no vector.
+template <int kV, typename W>
+__device__ __forceinline__ void load_vector(const W* p, int64_t at, float otherwise, bool vec,
+                                            float (&v)[kV]) {
+  if (p) {
+    load_cols<kV>(p + at, v, vec);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) v[i] = otherwise;
+  }
+}
+template <int kV, typename T>
+__device__ __forceinline__ void store_cols(T* p, const float (&v)[kV]) {
+  T e[kV];
+#pragma unroll
+  for (int i = 0; i < kV; ++i) e[i] = Cvt<T>::from_f(v[i]);
+  if constexpr (kV * sizeof(T) == 16) {
+    uint4 u;
+    memcpy(&u, e, 16);
+    *reinterpret_cast<uint4*>(p) = u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) p[i] = e[i];
+  }
+}
+
+// mean and rstd of a row.
+template <int kV, typename T>
+__device__ __forceinline__ float2 row_stats(const T* row, int64_t N, bool layer, float eps,
+                                            float* red) {
+  float mean = 0.0f, sq = 0.0f, v[kV];
+  const int64_t first = static_cast<int64_t>(threadIdx.x) * kV, step = blockDim.x * kV;
   if (layer) {
     float sum = 0.0f;
-    for (int64_t c = threadIdx.x; c < N; c += blockDim.x) sum += at(c);
+    for (int64_t c = first; c < N; c += step) {
+      load_cols<kV>(row + c, v);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) sum += v[i];
+    }
     mean = block_sum(sum, red) / static_cast<float>(N);
   }
-  for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-    const float d = at(c) - mean;
-    sq = fmaf(d, d, sq);
+  for (int64_t c = first; c < N; c += step) {
+    load_cols<kV>(row + c, v);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) sq = fmaf(v[i] - mean, v[i] - mean, sq);
   }
   return make_float2(mean, 1.0f / sqrtf(block_sum(sq, red) / static_cast<float>(N) + eps));
 }

@@ -355,64 +355,112 @@ __global__ void __launch_bounds__(32 * kSlices)
 
 // One CTA a stretch of rows: each row's statistics, its outputs, then its share of the
 // column sums, which stay in the workspace (a thread adds to its own columns).
-template <typename T, typename W, bool kBias>
-__global__ void __launch_bounds__(1024) sn_bwd_wide(const BwdArgs p) {
+template <typename T, typename W, bool kBias, int kV>
+__global__ void __launch_bounds__(512) sn_bwd_wide(const BwdArgs p) {
   constexpr int kSums = kBias ? 4 : 2;
   __shared__ float red[32];
   const int64_t N = p.N;
-  const T *x = static_cast<const T*>(p.x), *s = static_cast<const T*>(p.s),
-          *dy = static_cast<const T*>(p.dy), *ds = static_cast<const T*>(p.ds);
-  const W *w1 = static_cast<const W*>(p.w1), *w2 = static_cast<const W*>(p.w2),
-          *gate = static_cast<const W*>(p.gate);
+  const int64_t first = static_cast<int64_t>(threadIdx.x) * kV, step = blockDim.x * kV;
+  const W *w1 = static_cast<const W*>(p.w1), *w2 = static_cast<const W*>(p.w2);
   const float inv_n = 1.0f / static_cast<float>(N);
   const int64_t row0 = first_row(p.M, blockIdx.x, gridDim.x),
                 end = first_row(p.M, blockIdx.x + 1, gridDim.x);
   int64_t group = -1;
   for (int64_t row = row0; row < end; ++row) {
-    const int64_t g = row / p.rows_per_group, o = row * N;
+    const int64_t g = row / p.rows_per_group;
+    const T *x = static_cast<const T*>(p.x) + row * N, *s = static_cast<const T*>(p.s) + row * N,
+            *dy = static_cast<const T*>(p.dy) + row * N,
+            *ds = p.ds ? static_cast<const T*>(p.ds) + row * N : nullptr;
+    const W* gate = p.gate ? static_cast<const W*>(p.gate) + g * N : nullptr;
     float* to = stretch(p.part, blockIdx.x, g, kSums, p.N);
-    if (g != group)
-      for (int64_t c = threadIdx.x; c < N; c += blockDim.x)
-        for (int q = 0; q < kSums; ++q) to[q * N + c] = 0.0f;
+    const bool fresh = g != group;
     group = g;
-    const float2 sx =
-        row_stats([&](int64_t c) { return Cvt<T>::to_f(x[o + c]); }, N, p.layer, p.eps, red);
-    const float2 ss =
-        row_stats([&](int64_t c) { return Cvt<T>::to_f(s[o + c]); }, N, p.layer, p.eps, red);
+    const float2 sx = row_stats<kV>(x, N, p.layer, p.eps, red);
+    const float2 ss = row_stats<kV>(s, N, p.layer, p.eps, red);
     float f0 = 0.0f, f1 = 0.0f;
-    for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-      const float f = Cvt<T>::to_f(dy[o + c]) * Cvt<W>::to_f(w2[c]);
-      f0 += f;
-      f1 = fmaf(f, (Cvt<T>::to_f(s[o + c]) - ss.x) * ss.y, f1);
+    float sv[kV], gv[kV], w[kV], xv[kV], ga[kV], t[kV];
+    for (int64_t c = first; c < N; c += step) {
+      load_cols<kV>(s + c, sv);
+      load_cols<kV>(dy + c, gv);
+      load_vector<kV>(w2, c, 1.0f, p.vec, w);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const float f = gv[i] * w[i];
+        f0 += f;
+        f1 = fmaf(f, (sv[i] - ss.x) * ss.y, f1);
+      }
     }
     const float mf = p.layer ? block_sum(f0, red) * inv_n : 0.0f;
     const float mfs = block_sum(f1, red) * inv_n;
-    float e0 = 0.0f, e1 = 0.0f;
-    for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-      const float hat = (Cvt<T>::to_f(s[o + c]) - ss.x) * ss.y, dyv = Cvt<T>::to_f(dy[o + c]);
-      const float xh = (Cvt<T>::to_f(x[o + c]) - sx.x) * sx.y;
-      const float t = (ds ? Cvt<T>::to_f(ds[o + c]) : 0.0f) +
-                      ss.y * (dyv * Cvt<W>::to_f(w2[c]) - mf - hat * mfs);
-      to[c] = fmaf(t, xh, to[c]);
-      to[N + c] = fmaf(dyv, hat, to[N + c]);
-      if (kBias) {
-        to[2 * N + c] += t;
-        to[3 * N + c] += dyv;
+    // ds' of a packet (t), with s^ in sv and x^ in xv.
+    auto packet = [&](int64_t c) {
+      load_cols<kV>(s + c, sv);
+      load_cols<kV>(dy + c, gv);
+      load_cols<kV>(x + c, xv);
+      load_vector<kV>(w2, c, 1.0f, p.vec, w);
+      if (ds) {
+        load_cols<kV>(ds + c, t);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) t[i] = 0.0f;
       }
-      const float e = t * param(gate, g * N + c, 1.0f) * Cvt<W>::to_f(w1[c]);
-      e0 += e;
-      e1 = fmaf(e, xh, e1);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        sv[i] = (sv[i] - ss.x) * ss.y;
+        xv[i] = (xv[i] - sx.x) * sx.y;
+        t[i] = fmaf(ss.y, gv[i] * w[i] - mf - sv[i] * mfs, t[i]);
+      }
+      load_vector<kV>(w1, c, 1.0f, p.vec, w);
+      load_vector<kV>(gate, c, 1.0f, p.vec, ga);
+    };
+    float e0 = 0.0f, e1 = 0.0f;
+    for (int64_t c = first; c < N; c += step) {
+      packet(c);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const float e = t[i] * ga[i] * w[i];
+        e0 += e;
+        e1 = fmaf(e, xv[i], e1);
+      }
+      // This thread's columns of the sums, which it alone adds to.
+      auto add = [&](int which, auto term) {
+        float a[kV];
+        float* at = to + which * N + c;
+        if (fresh) {
+#pragma unroll
+          for (int i = 0; i < kV; ++i) a[i] = 0.0f;
+        } else {
+          load_cols<kV>(at, a);
+        }
+#pragma unroll
+        for (int i = 0; i < kV; ++i) a[i] += term(i);
+        if constexpr (kV % 4 == 0) {
+#pragma unroll
+          for (int i = 0; i < kV; i += 4)
+            *reinterpret_cast<float4*>(at + i) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+        } else {
+          at[0] = a[0];
+        }
+      };
+      add(0, [&](int i) { return t[i] * xv[i]; });
+      add(1, [&](int i) { return gv[i] * sv[i]; });
+      if (kBias) {
+        add(2, [&](int i) { return t[i]; });
+        add(3, [&](int i) { return gv[i]; });
+      }
     }
     const float me = p.layer ? block_sum(e0, red) * inv_n : 0.0f;
     const float mex = block_sum(e1, red) * inv_n;
-    for (int64_t c = threadIdx.x; c < N; c += blockDim.x) {
-      const float hat = (Cvt<T>::to_f(s[o + c]) - ss.x) * ss.y;
-      const float t = (ds ? Cvt<T>::to_f(ds[o + c]) : 0.0f) +
-                      ss.y * (Cvt<T>::to_f(dy[o + c]) * Cvt<W>::to_f(w2[c]) - mf - hat * mfs);
-      const float e = t * param(gate, g * N + c, 1.0f) * Cvt<W>::to_f(w1[c]);
-      static_cast<T*>(p.dres)[o + c] = Cvt<T>::from_f(p.alpha * t);
-      static_cast<T*>(p.dx)[o + c] = Cvt<T>::from_f(
-          sx.y * (e - me - (Cvt<T>::to_f(x[o + c]) - sx.x) * sx.y * mex));
+    for (int64_t c = first; c < N; c += step) {
+      packet(c);
+      float dr[kV], dx[kV];
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        dr[i] = p.alpha * t[i];
+        dx[i] = sx.y * (t[i] * ga[i] * w[i] - me - xv[i] * mex);
+      }
+      store_cols<kV>(static_cast<T*>(p.dres) + row * N + c, dr);
+      store_cols<kV>(static_cast<T*>(p.dx) + row * N + c, dx);
     }
   }
 }
@@ -423,6 +471,7 @@ __global__ void __launch_bounds__(1024) sn_bwd_wide(const BwdArgs p) {
 // bf16, before the norms were kernels of their own: two CTAs 152 us without and 284 us
 // with biases, one 165 and 225 us).
 int64_t ctas_per_sm(int64_t N, bool bias) {
+  if (N > 8192) return 2;  // the passes over L2, or one CTA at a time of the others
   return N <= 1024 ? 4 : (N <= 2048 ? 2 : (N <= 4096 && !bias ? 2 : 1));
 }
 constexpr int kMaxSms = 256;  // workspace: more than any device of this architecture has
@@ -443,7 +492,8 @@ int launch_bwd(const BwdArgs& a, int64_t ctas, cudaStream_t s) {
       return go(sn_bwd<T, W, 256, 2, 3, 2, kBytes, kBias, kLayer>, 256, 2, 3);
   }
   if (packets <= 1024) return go(sn_bwd<T, W, 512, 2, 3, 1, kBytes, kBias, kLayer>, 512, 2, 3);
-  sn_bwd_wide<T, W, kBias><<<static_cast<unsigned>(ctas), 1024, 0, s>>>(a);
+  sn_bwd_wide<T, W, kBias, kBytes == 16 ? 16 / sizeof(T) : 1>
+      <<<static_cast<unsigned>(ctas), 512, 0, s>>>(a);
   return launch_status();
 }
 

@@ -8,7 +8,8 @@ recurrent block behind a causal depthwise conv1d.  Per channel, with
     h_t = a_t * h_{t-1} + sqrt(1 - a_t^2) * sigmoid(input_gate_t) * x_t
     y_t = h_t                                   (h in fp32, y rounded once)
 
-A decay gate of -inf has a = 1 exactly and takes no input: a padded token.
+A decay gate of -inf has a = 1 exactly and takes no input: a padded token (whose
+x and input_gate are still read and must be finite).
 
     GatedLinearRecurrenceFwdOp(batch, seq_len, dim, decay_scale=8.0, dtype=torch.bfloat16,
                                save_states=False, kernel_map=None)

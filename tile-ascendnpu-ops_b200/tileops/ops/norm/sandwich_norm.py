@@ -27,7 +27,8 @@ are G equal consecutive groups (a batch of G samples) with a gate each; None
 means 1.  A bias of None means 0.  The backward op takes the forward's x and
 residual_out and the same parameters; ``d_residual_out`` may be None, and
 gradients of what was None are None.  Gradients have their tensors' types,
-summed in fp32 in a fixed order.
+summed in fp32 in a fixed order; the backward pass takes a workspace of two or
+four fp32 rows for each gate row besides those of its CTAs.
 """
 
 from __future__ import annotations
@@ -71,8 +72,9 @@ class _SandwichNormOp(Op):
         self._kernel_cache: Dict[tuple, Kernel] = {}
         self._last: Optional[tuple[int, int, int, int]] = None
 
-    def _check(self, rows: tuple, params: tuple, gate: Optional[torch.Tensor]) -> None:
-        """Validate (name, tensor, name, tensor, ...) rows, x first, and parameters.
+    def _check(self, rows: tuple, params: tuple, gate: Optional[torch.Tensor]) -> Kernel:
+        """Validate (name, tensor, name, tensor, ...) rows, x first, and parameters; returns the
+        kernel of these sizes (the op's own attributes may be another thread's by then).
 
         A decode step is bound by the host: tensors are compared against x and the first
         parameter in one pass each, and told apart only when something is wrong."""
@@ -118,6 +120,12 @@ class _SandwichNormOp(Op):
             raise ValueError(f"Expected M={committed_m} (product of leading dims), got {M}")
         self.M, self.N, self.dtype = M, N, dtype
         self._last = (M, N, dtype.itemsize, vectors * affine.itemsize)
+        key = (M, N, dtype, device.index)
+        kernel = self._kernel_cache.get(key)
+        if kernel is None:
+            kernel = self._kernel_cache[key] = self.kernel_map[self._op_name](
+                M, N, self.norm, self.eps, self.residual_scale, dtype)
+        return kernel
 
     @staticmethod
     def _refuse_device(named: tuple) -> None:
@@ -133,13 +141,6 @@ class _SandwichNormOp(Op):
         if t.shape != shape:
             raise ValueError(f"Expected {name} shape {tuple(shape)}, got {tuple(t.shape)}")
         raise ValueError(f"Expected {name} on {device}, got {t.device}")
-
-    def _get_kernel(self, device_index) -> Kernel:
-        key = (self.M, self.N, self.dtype, device_index)
-        if key not in self._kernel_cache:
-            self._kernel_cache[key] = self.kernel_map[self._op_name](
-                self.M, self.N, self.norm, self.eps, self.residual_scale, self.dtype)
-        return self._kernel_cache[key]
 
     def _work(self, flops: int, rows: int, passes: int) -> tuple[int, int]:
         if self._last is None:
@@ -177,10 +178,10 @@ class FusedSandwichNormFwdOp(_SandwichNormOp):
                 post_bias: Optional[torch.Tensor] = None,
                 pre_bias: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Return ``(y, residual_out)``, both shaped like ``x``."""
-        self._check(("x", x, "residual", residual),
-                    ("post_weight", post_weight, "pre_weight", pre_weight,
-                     "post_bias", post_bias, "pre_bias", pre_bias), gate)
-        return self._get_kernel(x.device.index)(
+        kernel = self._check(("x", x, "residual", residual),
+                             ("post_weight", post_weight, "pre_weight", pre_weight,
+                              "post_bias", post_bias, "pre_bias", pre_bias), gate)
+        return kernel(
             x.contiguous(), residual.contiguous(), post_weight.contiguous(),
             pre_weight.contiguous(), _dense(gate), _dense(post_bias), _dense(pre_bias))
 
@@ -204,11 +205,11 @@ class FusedSandwichNormBwdOp(_SandwichNormOp):
                 pre_bias: Optional[torch.Tensor] = None):
         """Return ``(dx, d_residual, d_post_weight, d_pre_weight, d_gate, d_post_bias,
         d_pre_bias)``, None in the place of a gradient of what was None."""
-        self._check(("x", x, "dy", dy, "d_residual_out", d_residual_out,
-                     "residual_out", residual_out),
-                    ("post_weight", post_weight, "pre_weight", pre_weight,
-                     "post_bias", post_bias, "pre_bias", pre_bias), gate)
-        return self._get_kernel(x.device.index)(
+        kernel = self._check(("x", x, "dy", dy, "d_residual_out", d_residual_out,
+                              "residual_out", residual_out),
+                             ("post_weight", post_weight, "pre_weight", pre_weight,
+                              "post_bias", post_bias, "pre_bias", pre_bias), gate)
+        return kernel(
             dy.contiguous(), _dense(d_residual_out), x.contiguous(), residual_out.contiguous(),
             post_weight.contiguous(), pre_weight.contiguous(), _dense(gate), _dense(post_bias),
             _dense(pre_bias))
