@@ -92,16 +92,23 @@ def test_long_and_wide(B, T, D):
     (1, 5000, 272),    # clusters of eight
     (40, 700, 200),    # more CTAs than SMs
 ])
-@pytest.mark.parametrize("packed", [False, True])
-def test_every_split_of_the_tokens(B, T, D, packed):
+@pytest.mark.parametrize("packed, dtype", [(False, torch.bfloat16), (True, torch.bfloat16),
+                                           (True, torch.float32)])
+def test_every_split_of_the_tokens(B, T, D, packed, dtype):
     """Long enough for each choice of warps and clusters to take several steps."""
     if packed:
         B = 1
         cuts = torch.randint(0, T + 1, (20,)).sort().values.tolist()
         lengths = [b - a for a, b in zip([0, *cuts], [*cuts, T])]
-        _check_all(*_inputs(1, T, D, torch.bfloat16, nseq=21), cu=_cu(lengths))
+        _check_all(*_inputs(1, T, D, dtype, nseq=21), cu=_cu(lengths))
     else:
-        _check_all(*_inputs(B, T, D, torch.bfloat16))
+        _check_all(*_inputs(B, T, D, dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_whole_sm_a_cta(dtype):
+    """One sequence whose channels fill more than half the SMs, over several steps."""
+    _check_all(*_inputs(1, 1000, 2600, dtype))
 
 
 def test_many_partial_sums():
