@@ -258,10 +258,10 @@ constexpr int kMaxCluster = 8;  // CTAs of a cluster
 // algorithm's).  Forward, an element takes 31 issue slots, of which 5 on the
 // special-function unit (16 lanes a clock and SM: 37 us of the 41 us that 8 x
 // 1024 x 4096 bf16 takes at the copy rate); 16 warps of 128 registers an SM
-// keep that unit at 58 to 68% (profiles: 71 us; with full waves 5.0 TB/s, 0.77
-// of the copy rate).  Kept apart by measurement: 24 warps with runs of 8
-// tokens 20% slower (twice the joins); 64 channels a CTA 12% slower at few
-// CTAs; a barrier a step in place of the chain of warps 3% slower.
+// keep that unit at 58 to 68% busy (71 us; 8 x 4096 x 4096 214 us, 0.77 of the
+// copy rate).  Measured and not taken: 24 warps with runs of 8 tokens, 20%
+// slower (twice the joins); a barrier a step in place of the chain of warps,
+// 3% slower; 64 channels a CTA, 10% slower (half as many CTAs to fill the SMs).
 
 // How a warp lies over channels and tokens: `Chans` channels side by side, two a lane,
 // and groups of lanes one after another in time, `Run` tokens a lane; up to `Warps` warps a
