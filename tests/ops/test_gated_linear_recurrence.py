@@ -454,3 +454,35 @@ def test_decode_follows_a_prefill():
         y, _ = step(x[:, t], i[:, t], r[:, t], lam, state)
         ref.assert_within(y, y_ref[:, t], y_tol[:, t], f"token {t}")
     ref.assert_within(state, h_ref, h_tol, "state")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["overlapping", "step 2", "expanded", "strided"])
+@pytest.mark.parametrize("B, D", [(8, 32), (3, 65), (40, 48)])
+def test_decode_layouts(B, D, layout, dtype):
+    """Rows of x and the gates at any distance, none and one element among them."""
+    def rows():
+        signal = torch.randn(2 * (B + D), device="cuda").to(dtype)
+        wide = torch.randn(2 * B, 3 * D, device="cuda").to(dtype)
+        return {"overlapping": signal.unfold(0, D, 1)[:B], "step 2": signal.unfold(0, D, 2)[:B],
+                "expanded": signal[:D].expand(B, D), "strided": wide[::2, 1:1 + D]}[layout]
+
+    x, i, r = rows(), rows(), rows()
+    assert x.shape == (B, D)
+    lam, h0 = torch.randn(D, device="cuda") - 2, torch.randn(B, D, device="cuda")
+    y_ref, h_ref, y_tol, h_tol = ref.glr_fwd(x[:, None], i[:, None], r[:, None], lam, h0)
+    y, h = GatedLinearRecurrenceDecodeOp(B, D, dtype=dtype)(x, i, r, lam, h0)
+    ref.assert_within(y, y_ref[:, 0], y_tol[:, 0], "y")
+    ref.assert_within(h, h_ref, h_tol, "state")
+    y2, h2 = GatedLinearRecurrenceDecodeOp(B, D, dtype=dtype, inplace=True)(x, i, r, lam, h0)
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_overlapping_rows_in_whole_sequences(dtype):
+    """Tokens that overlap, of x, the gates and dy."""
+    B, T, D = 2, 70, 40
+    x, i, r, dy = (torch.randn(B, T + D, device="cuda").to(dtype).unfold(1, D, 1)[:, :T]
+                   for _ in range(4))
+    (_, _, _, lam), h0, _, dT = _inputs(B, T, D, dtype)
+    _check_all((x, i, r, lam), h0, dy, dT)

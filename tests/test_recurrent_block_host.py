@@ -311,3 +311,28 @@ def test_sandwich_entry_points_check_their_arguments():
 def test_supported_types_of_the_kernels():
     for dtype in GatedLinearRecurrenceFwdKernel.SUPPORTED_DTYPES:
         assert GatedLinearRecurrenceFwdKernel(1, 1, 1, 1.0, dtype).dtype_str
+
+
+# ------------------------------------------------------------ layouts, with the launch stubbed
+def _overlapping(B, D, dtype=torch.float32):
+    """Rows that overlap: a window slid along one signal, strides (1, 1)."""
+    return torch.randn(B + 2 * D, dtype=dtype).unfold(0, D, 1)[:B]
+
+
+@pytest.mark.parametrize("layout", ["overlapping", "expanded", "strided", "dense"])
+def test_decode_output_rows_are_dense(accept_cpu, monkeypatch, layout):
+    """The entry point writes y as dense rows, whatever strides x has."""
+    B, D = 8, 32
+    x = {"overlapping": lambda: _overlapping(B, D), "expanded": lambda: torch.randn(D).expand(B, D),
+         "strided": lambda: torch.randn(2 * B, 2 * D)[::2, 3:3 + D],
+         "dense": lambda: torch.randn(B, D)}[layout]()
+    written = torch.arange(B * D, dtype=torch.float32)
+
+    def launch(name, device, *args):
+        assert name == "tileops_glr_decode_fwd" and args[0] == x.data_ptr() and args[9] == x.stride(0)
+        ctypes.memmove(args[5], written.data_ptr(), 4 * B * D)
+
+    monkeypatch.setattr(_native, "launch", launch)
+    y, _ = GatedLinearRecurrenceDecodeOp(B, D, dtype=torch.float32)(
+        x, torch.randn(B, D), torch.randn(B, D), torch.randn(D), torch.randn(B, D))
+    assert torch.equal(y, written.view(B, D))

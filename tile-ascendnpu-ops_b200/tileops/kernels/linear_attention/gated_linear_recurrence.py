@@ -27,7 +27,8 @@ def _channels_last(t: torch.Tensor) -> torch.Tensor:
 
 
 def _rows_like(t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
-    """A dense output (``empty_like`` costs the host half of what ``empty`` does)."""
+    """A dense output (``empty_like`` costs the host half of what ``empty`` does, but takes over
+    the order of ``t``'s strides: rows that overlap, strides (1, 1), give a transposed one)."""
     if t.dtype is dtype and t.is_contiguous():
         return torch.empty_like(t)
     return torch.empty(shape, dtype=dtype, device=t.device)
@@ -152,7 +153,7 @@ class GatedLinearRecurrenceDecodeKernel(_GatedLinearRecurrenceKernel):
         decay_gate, decay_param = _channels_last(decay_gate), decay_param.contiguous()
         if not inplace:
             state = state.contiguous()
-        y = torch.empty_like(x)  # dense: rows of contiguous channels
+        y = _rows_like(x, self.dtype, (B, D))
         new_state = state if inplace else torch.empty_like(state)
         _native.launch(
             "tileops_glr_decode_fwd", dev, x.data_ptr(), input_gate.data_ptr(),
