@@ -336,3 +336,34 @@ def test_decode_output_rows_are_dense(accept_cpu, monkeypatch, layout):
     y, _ = GatedLinearRecurrenceDecodeOp(B, D, dtype=torch.float32)(
         x, torch.randn(B, D), torch.randn(B, D), torch.randn(D), torch.randn(B, D))
     assert torch.equal(y, written.view(B, D))
+
+
+# ------------------------------------------------------------ required arguments left out
+@pytest.mark.parametrize("at, name", [(0, "x"), (1, "residual"), (2, "post_weight"),
+                                      (3, "pre_weight")])
+def test_sandwich_names_a_required_argument_that_is_none(accept_cpu, at, name):
+    x, w = torch.randn(4, 8), torch.randn(8)
+    args = [x, x, w, w]
+    args[at] = None
+    with pytest.raises(ValueError, match=f"{name} must be a cuda tensor"):
+        FusedSandwichNormFwdOp()(*args)
+
+
+@pytest.mark.parametrize("at, name", [(0, "dy"), (2, "x"), (3, "residual_out"),
+                                      (4, "post_weight"), (5, "pre_weight")])
+def test_sandwich_backward_names_a_required_argument_that_is_none(accept_cpu, at, name):
+    x, w = torch.randn(4, 8), torch.randn(8)
+    for ds in (None, x):
+        args = [x, ds, x, x, w, w]
+        args[at] = None
+        with pytest.raises(ValueError, match=f"{name} must be a cuda tensor"):
+            FusedSandwichNormBwdOp()(*args)
+
+
+@pytest.mark.parametrize("at", [2, 4, 5, 6])
+def test_sandwich_refuses_what_is_no_tensor(accept_cpu, at):
+    x, w = torch.randn(4, 8), torch.randn(8)
+    args = [x, x, w, w, w, w, w]
+    args[at] = w.tolist()
+    with pytest.raises(ValueError, match="must be a cuda tensor"):
+        FusedSandwichNormFwdOp()(*args)

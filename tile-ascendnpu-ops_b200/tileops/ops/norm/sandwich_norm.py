@@ -73,15 +73,19 @@ class _SandwichNormOp(Op):
         self._last: Optional[tuple[int, int, int, int]] = None
 
     def _check(self, rows: tuple, params: tuple, gate: Optional[torch.Tensor]) -> Kernel:
-        """Validate (name, tensor, name, tensor, ...) rows, x first, and parameters; returns the
-        kernel of these sizes (the op's own attributes may be another thread's by then).
+        """Validate (name, tensor, name, tensor, ...) rows, x first, and parameters, the two
+        weights first (only the biases and the gate may be None); returns the kernel of these
+        sizes (the op's own attributes may be another thread's by then).
 
         A decode step is bound by the host: tensors are compared against x and the first
         parameter in one pass each, and told apart only when something is wrong."""
         is_device_tensor = get_device_backend().is_device_tensor
-        for t in rows[1::2] + params[1::2] + (gate,):
+        for t in rows[1::2] + params[1:4:2]:
+            if not is_device_tensor(t):
+                self._refuse_device(rows + params[:4])
+        for t in (params[5], params[7], gate):
             if t is not None and not is_device_tensor(t):
-                self._refuse_device(rows + params + ("gate", gate))
+                self._refuse_device((*params[4:], "gate", gate), optional=True)
         x = rows[1]
         committed_m, committed_n, committed_dtype = self._committed
         dtype, shape, device = committed_dtype or x.dtype, x.shape, x.device
@@ -95,8 +99,7 @@ class _SandwichNormOp(Op):
                              f"got {affine}")
         for i in range(1, len(rows), 2):
             t = rows[i]
-            if t is not None and not (t.dtype is dtype and t.shape == shape
-                                      and t.device == device):
+            if not (t.dtype is dtype and t.shape == shape and t.device == device):
                 self._refuse(rows[i - 1], t, dtype, shape, device)
         vectors, vector = 0, (N,)
         for i in range(1, len(params), 2):
@@ -128,10 +131,10 @@ class _SandwichNormOp(Op):
         return kernel
 
     @staticmethod
-    def _refuse_device(named: tuple) -> None:
+    def _refuse_device(named: tuple, optional: bool = False) -> None:
         backend = get_device_backend()
         for name, t in zip(named[::2], named[1::2]):
-            if t is not None and not backend.is_device_tensor(t):
+            if not (optional and t is None or backend.is_device_tensor(t)):
                 raise ValueError(f"{name} must be a {backend.name} tensor")
 
     @staticmethod
@@ -205,8 +208,10 @@ class FusedSandwichNormBwdOp(_SandwichNormOp):
                 pre_bias: Optional[torch.Tensor] = None):
         """Return ``(dx, d_residual, d_post_weight, d_pre_weight, d_gate, d_post_bias,
         d_pre_bias)``, None in the place of a gradient of what was None."""
-        kernel = self._check(("x", x, "dy", dy, "d_residual_out", d_residual_out,
-                              "residual_out", residual_out),
+        rows = ("x", x, "dy", dy, "residual_out", residual_out)
+        if d_residual_out is not None:
+            rows += ("d_residual_out", d_residual_out)
+        kernel = self._check(rows,
                              ("post_weight", post_weight, "pre_weight", pre_weight,
                               "post_bias", post_bias, "pre_bias", pre_bias), gate)
         return kernel(
