@@ -486,3 +486,18 @@ def test_overlapping_rows_in_whole_sequences(dtype):
                    for _ in range(4))
     (_, _, _, lam), h0, _, dT = _inputs(B, T, D, dtype)
     _check_all((x, i, r, lam), h0, dy, dT)
+
+
+@pytest.mark.parametrize("offsets", [[0, 2**32 + 50, 100], [0, 50, 2**32 + 100], [-2**32, 50, 100]])
+def test_offsets_that_int32_cannot_hold_set_the_error_flag(offsets):
+    (x, i, r, lam), _, dy, _ = _inputs(1, 100, 66, torch.bfloat16)
+    cu = torch.tensor(offsets, device="cuda")
+    flag = lambda: nat.lib().tileops_device_error_flag(nat.stream_handle(x.device), 1)  # noqa: E731
+    flag()
+    _, _, states = GatedLinearRecurrenceFwdOp(1, 100, 66, save_states=True)(x, i, r, lam, None, cu)
+    assert flag() == 2
+    GatedLinearRecurrenceBwdOp(1, 100, 66)(dy, x, i, r, lam, states, None, None, cu)
+    assert flag() == 2
+    cu = torch.tensor([0, 50, 100], device="cuda")
+    GatedLinearRecurrenceFwdOp(1, 100, 66)(x, i, r, lam, None, cu)
+    assert flag() == 0

@@ -367,3 +367,20 @@ def test_sandwich_refuses_what_is_no_tensor(accept_cpu, at):
     args[at] = w.tolist()
     with pytest.raises(ValueError, match="must be a cuda tensor"):
         FusedSandwichNormFwdOp()(*args)
+
+
+# ------------------------------------------------------------ offsets beyond int32
+@pytest.mark.parametrize("offsets", [[0, 2**32 + 50, 100], [0, 50, 2**32 + 100], [-2**32, 50, 100],
+                                     [0, -2**32 + 50, 100], [0, -2**40, 2**33]])
+def test_offsets_keep_their_sign_and_order_in_32_bits(offsets):
+    """64-bit offsets that int32 cannot hold saturate: what breaks the rule still breaks it."""
+    kernel = GatedLinearRecurrenceFwdKernel(1, 100, 8, 8.0, torch.float32)
+    wide = torch.tensor(offsets)
+    cu, nseq = kernel._sequences(wide, torch.device("cpu"))
+    assert cu.dtype == torch.int32 and nseq == 2
+    whole = lambda c: c[0] == 0 and c[-1] == 100 and (c.diff() >= 0).all()  # noqa: E731
+    assert not whole(wide) and not whole(cu)
+    good = torch.tensor([0, 50, 100])
+    for t in (good, good.int(), good.int().repeat_interleave(2)[::2]):
+        cu, _ = kernel._sequences(t, torch.device("cpu"))
+        assert cu.tolist() == [0, 50, 100] and cu.is_contiguous() and cu.dtype == torch.int32

@@ -58,6 +58,8 @@ class _GatedLinearRecurrenceKernel(Kernel):
         """Device int32 offsets (or None) and the number of sequences."""
         if cu_seqlens is None:
             return None, self.batch
+        if cu_seqlens.dtype is torch.int64:  # saturated: a cast alone would wrap 2^32 + n to n
+            cu_seqlens = cu_seqlens.clamp(-1, 2**31 - 1)
         return (cu_seqlens.to(device=device, dtype=torch.int32).contiguous(),
                 cu_seqlens.numel() - 1)
 
