@@ -384,3 +384,15 @@ def test_offsets_keep_their_sign_and_order_in_32_bits(offsets):
     for t in (good, good.int(), good.int().repeat_interleave(2)[::2]):
         cu, _ = kernel._sequences(t, torch.device("cpu"))
         assert cu.tolist() == [0, 50, 100] and cu.is_contiguous() and cu.dtype == torch.int32
+
+
+@pytest.mark.parametrize("c", [1e39, 1e-39, 5e-324])
+def test_recurrence_rejects_a_decay_scale_that_float32_cannot_hold(c):
+    """1e39 would be inf in the kernels, and inf * sigmoid(-inf) NaN; 1e-39 a subnormal."""
+    for cls in (GatedLinearRecurrenceFwdOp, GatedLinearRecurrenceBwdOp):
+        with pytest.raises(ValueError, match="decay_scale"):
+            cls(1, 4, 8, c)
+    with pytest.raises(ValueError, match="decay_scale"):
+        GatedLinearRecurrenceDecodeOp(1, 8, c)
+    GatedLinearRecurrenceDecodeOp(1, 8, 1e38)
+    GatedLinearRecurrenceDecodeOp(1, 8, 1.2e-38)

@@ -45,8 +45,9 @@ class _GatedLinearRecurrenceKernel(Kernel):
                 or dim > 2**31 - 1):
             raise ValueError(f"{type(self).__name__} supports batch 0..65535, seq_len "
                              f"0..2^31 - 2^16 and dim 1..2^31 - 1, got ({batch}, {seq_len}, {dim})")
-        if not 0.0 < decay_scale < float("inf"):
-            raise ValueError(f"decay_scale must be positive and finite, got {decay_scale}")
+        fp32 = torch.finfo(torch.float32)  # what the kernels compute with
+        if not fp32.tiny <= decay_scale <= fp32.max:
+            raise ValueError(f"decay_scale must be positive and a normal float32, got {decay_scale}")
         self.batch, self.seq_len, self.dim = batch, seq_len, dim
         self.decay_scale = float(decay_scale)
         self.dtype = dtype

@@ -97,7 +97,7 @@ class GatedLinearRecurrenceFwdOp(Op):
 
     Args:
         batch, seq_len, dim: Batch size, tokens, channels.
-        decay_scale: Decay rate per unit of ``softplus(decay_param)``, positive.
+        decay_scale: Decay rate per unit of ``softplus(decay_param)``, a positive normal float32.
         dtype: float32, float16 or bfloat16.
         save_states: Also return the states the backward op takes.
         kernel_map: Optional override of ``"glr_fwd"``.
