@@ -10,7 +10,10 @@ import torch
 from oracle import recurrent as ref
 from tileops import _native
 from tileops.benchmark.msprof import _extract_op_init_args
-from tileops.kernels.linear_attention import GatedLinearRecurrenceFwdKernel
+from tileops.kernels.linear_attention import (
+    GatedLinearRecurrenceBwdKernel,
+    GatedLinearRecurrenceFwdKernel,
+)
 from tileops.kernels.norm import FusedSandwichNormFwdKernel
 from tileops.manifest import load_workloads
 from tileops.ops.linear_attention import (
@@ -396,3 +399,16 @@ def test_recurrence_rejects_a_decay_scale_that_float32_cannot_hold(c):
         GatedLinearRecurrenceDecodeOp(1, 8, c)
     GatedLinearRecurrenceDecodeOp(1, 8, 1e38)
     GatedLinearRecurrenceDecodeOp(1, 8, 1.2e-38)
+
+
+# ------------------------------------------------------------ no token: states pass through
+def test_states_that_pass_through_carry_no_graph():
+    """These ops build no autograd graph, without a token either."""
+    x, lam = torch.randn(2, 0, 8), torch.randn(8)
+    h0 = torch.randn(2, 8, requires_grad=True)
+    _, final, states = GatedLinearRecurrenceFwdKernel(2, 0, 8, 8.0, torch.float32)(
+        x, x, x, lam, h0, None, True)
+    assert not final.requires_grad and torch.equal(final, h0) and final.data_ptr() != h0.data_ptr()
+    *_, d0 = GatedLinearRecurrenceBwdKernel(2, 0, 8, 8.0, torch.float32)(
+        x, x, x, x, lam, states, None, h0)
+    assert not d0.requires_grad and torch.equal(d0, h0) and d0.data_ptr() != h0.data_ptr()

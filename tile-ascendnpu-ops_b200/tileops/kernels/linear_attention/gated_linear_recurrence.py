@@ -87,7 +87,7 @@ class GatedLinearRecurrenceFwdKernel(_GatedLinearRecurrenceKernel):
                   if save_states else None)
         if B == 0 or T == 0 or nseq == 0:  # no token anywhere: every sequence ends where it began
             final = (torch.zeros((nseq, D), dtype=torch.float32, device=dev)
-                     if initial_state is None else initial_state.clone())
+                     if initial_state is None else initial_state.detach().clone())
             return y, final, states
         final = (torch.empty((nseq, D), dtype=torch.float32, device=dev)
                  if initial_state is None else torch.empty_like(initial_state))
@@ -117,7 +117,7 @@ class GatedLinearRecurrenceBwdKernel(_GatedLinearRecurrenceKernel):
         dx, di, dr = (_rows_like(t, self.dtype, (B, T, D)) for t in (x, input_gate, decay_gate))
         if B == 0 or T == 0 or nseq == 0:
             d_initial = (torch.zeros((nseq, D), dtype=torch.float32, device=dev)
-                         if d_final_state is None else d_final_state.clone())
+                         if d_final_state is None else d_final_state.detach().clone())
             return dx, di, dr, torch.zeros(D, dtype=torch.float32, device=dev), d_initial
         d_param = torch.empty(D, dtype=torch.float32, device=dev)
         d_initial = torch.empty((nseq, D), dtype=torch.float32, device=dev)
