@@ -412,3 +412,17 @@ def test_states_that_pass_through_carry_no_graph():
     *_, d0 = GatedLinearRecurrenceBwdKernel(2, 0, 8, 8.0, torch.float32)(
         x, x, x, x, lam, states, None, h0)
     assert not d0.requires_grad and torch.equal(d0, h0) and d0.data_ptr() != h0.data_ptr()
+
+
+# ------------------------------------------------------------ roofline of packed calls
+def test_rooflines_count_a_state_for_each_packed_sequence(accept_cpu, monkeypatch):
+    monkeypatch.setattr(_native, "launch", lambda *args: None)
+    args, cu = _rec(B=1, T=100), torch.tensor([0, 10, 10, 70, 100])
+    op = GatedLinearRecurrenceFwdOp(1, 100, 8, dtype=torch.float32, save_states=True)
+    states = op(*args, None, cu)[2]
+    assert op.eval_roofline() == (20 * 800, 4 * 800 * 4 + 8 * 4 * 8 + 4 * 8)
+    op(*args)
+    assert op.eval_roofline() == (20 * 800, 4 * 800 * 4 + 8 * 8 + 4 * 8)
+    bwd = GatedLinearRecurrenceBwdOp(1, 100, 8, dtype=torch.float32)
+    bwd(torch.randn(1, 100, 8), *args, states, None, None, cu)
+    assert bwd.eval_roofline() == (40 * 800, 7 * 800 * 4 + 4 * 4 * 8 + 8 * 4 * 8 + 8 * 8)

@@ -107,6 +107,7 @@ class GatedLinearRecurrenceFwdOp(Op):
                  dtype: torch.dtype = torch.bfloat16, save_states: bool = False,
                  kernel_map: Optional[Dict[str, Kernel]] = None) -> None:
         self.batch, self.seq_len, self.dim = batch, seq_len, dim
+        self._nseq = batch  # sequences of the last call
         self.decay_scale = decay_scale
         self.dtype = dtype
         self.save_states = save_states
@@ -126,7 +127,7 @@ class GatedLinearRecurrenceFwdOp(Op):
         _check(on_device, dev, "input_gate", input_gate, rows, self.dtype)
         _check(on_device, dev, "decay_gate", decay_gate, rows, self.dtype)
         _check(on_device, dev, "decay_param", decay_param, (self.dim,), torch.float32)
-        nseq = _num_seqs(self.batch, dev, cu_seqlens)
+        nseq = self._nseq = _num_seqs(self.batch, dev, cu_seqlens)
         if initial_state is not None:
             _check(on_device, dev, "initial_state", initial_state, (nseq, self.dim), torch.float32)
         out = self.kernel(x, input_gate, decay_gate, decay_param, initial_state, cu_seqlens,
@@ -134,9 +135,11 @@ class GatedLinearRecurrenceFwdOp(Op):
         return out if self.save_states else out[:2]
 
     def eval_roofline(self) -> tuple[int, int]:
-        """``(20 * B * T * D, 4 * B * T * D * elem_bytes + 2 * B * D * 4 + D * 4)``."""
+        """``(20 * B * T * D, 4 * B * T * D * elem_bytes + 2 * S * D * 4 + D * 4)``, S the sequences
+        of the last call (B without packed ones).  What a forward pass cannot do without: the
+        states for the backward op, 4 / 32 bytes an element, are not in it."""
         elems = self.batch * self.seq_len * self.dim
-        nbytes = 4 * elems * self.dtype.itemsize + 8 * self.batch * self.dim + 4 * self.dim
+        nbytes = 4 * elems * self.dtype.itemsize + 8 * self._nseq * self.dim + 4 * self.dim
         return 20 * elems, nbytes
 
 
@@ -152,6 +155,7 @@ class GatedLinearRecurrenceBwdOp(Op):
                  dtype: torch.dtype = torch.bfloat16,
                  kernel_map: Optional[Dict[str, Kernel]] = None) -> None:
         self.batch, self.seq_len, self.dim = batch, seq_len, dim
+        self._nseq = batch  # sequences of the last call
         self.decay_scale = decay_scale
         self.dtype = dtype
         self.dispatch_kernel(kernel_map)
@@ -175,7 +179,7 @@ class GatedLinearRecurrenceBwdOp(Op):
         _check(on_device, dev, "decay_param", decay_param, (self.dim,), torch.float32)
         _check(on_device, dev, "states", states, (self.batch, -(-self.seq_len // _SEGMENT), self.dim),
                torch.float32)
-        nseq = _num_seqs(self.batch, dev, cu_seqlens)
+        nseq = self._nseq = _num_seqs(self.batch, dev, cu_seqlens)
         for name, t in (("initial_state", initial_state), ("d_final_state", d_final_state)):
             if t is not None:
                 _check(on_device, dev, name, t, (nseq, self.dim), torch.float32)
@@ -183,10 +187,11 @@ class GatedLinearRecurrenceBwdOp(Op):
                            d_final_state, cu_seqlens)
 
     def eval_roofline(self) -> tuple[int, int]:
-        """``(40 * B * T * D, 7 * B * T * D * elem_bytes + the fp32 states and gradients)``."""
+        """``(40 * B * T * D, 7 * B * T * D * elem_bytes + the fp32 states and gradients)``, of as
+        many sequences as the last call had."""
         elems = self.batch * self.seq_len * self.dim
         saved = self.batch * -(-self.seq_len // _SEGMENT) * self.dim
-        nbytes = (7 * elems * self.dtype.itemsize + 4 * saved + 8 * self.batch * self.dim
+        nbytes = (7 * elems * self.dtype.itemsize + 4 * saved + 8 * self._nseq * self.dim
                   + 8 * self.dim)
         return 40 * elems, nbytes
 
