@@ -501,3 +501,49 @@ def test_offsets_that_int32_cannot_hold_set_the_error_flag(offsets):
     cu = torch.tensor([0, 50, 100], device="cuda")
     GatedLinearRecurrenceFwdOp(1, 100, 66)(x, i, r, lam, None, cu)
     assert flag() == 0
+
+
+# ------------------------------------------------------------ padded tokens
+def _padded(T, D, dtype, B=2):
+    """Inputs whose decay gate is shut over some tokens, and those tokens."""
+    (x, i, r, lam), h0, dy, dT = _inputs(B, T, D, dtype)
+    shut = torch.zeros(T, dtype=torch.bool, device="cuda")
+    for a, b in ((0, 5), (16, 32), (40, 70), (T - 9, T)):
+        shut[a:b] = True
+    r[:, shut] = -float("inf")
+    return x, i, r, lam, h0, dy, dT, shut
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T, D", [(90, 66), (700, 64), (2100, 272)])
+def test_padded_tokens_have_no_say(T, D, dtype):
+    """Whatever finite x and input gate a padded token holds, its type's ends too, every output is
+    the same to the bit, and its own gradients are zeros."""
+    x, i, r, lam, h0, dy, dT, shut = _padded(T, D, dtype)
+    B, most = x.shape[0], torch.finfo(dtype).max
+    lam[::2] = -torch.rand(lam[::2].shape, device="cuda")  # every second channel decays fast
+    fwd = GatedLinearRecurrenceFwdOp(B, T, D, dtype=dtype, save_states=True)
+    bwd = GatedLinearRecurrenceBwdOp(B, T, D, dtype=dtype)
+    first = None
+    for xs, gs in ((0.0, 0.0), (most, most), (-most, 1.0), (most, -most), (1.0, -most)):
+        x[:, shut], i[:, shut] = xs, gs
+        out = fwd(x, i, r, lam, h0)
+        out += bwd(dy, x, i, r, lam, out[2], h0, dT)
+        for name, t in zip(NAMES[:3], out[3:6]):
+            assert (t[:, shut] == 0).all(), (name, xs, gs)
+        assert all(t.isfinite().all() for t in out), (xs, gs)
+        first = first or out
+        assert all(torch.equal(a, b) for a, b in zip(first, out)), (xs, gs)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_padded_tokens_repeat_the_state(dtype):
+    """A run of 16 tokens is walked from one state: a padded token in it has its neighbour's y to
+    the bit."""
+    x, i, r, lam, h0, _, _, shut = _padded(90, 66, dtype)
+    y, final = GatedLinearRecurrenceFwdOp(2, 90, 66, dtype=dtype)(x, i, r, lam, h0)
+    for t in range(1, 90):
+        if shut[t] and t % 16:
+            assert torch.equal(y[:, t], y[:, t - 1]), t
+    if dtype == torch.float32:
+        assert torch.equal(final, y[:, -1])

@@ -60,12 +60,14 @@ __device__ __forceinline__ TokenGrads token_grads(float2 g, float2 hp, float2 x,
   decay2<kAllNear>(fmul2(sr, k), a2, m2, c);
   const float2 rm = rsqrt2(m2);
   TokenGrads o;
-  const float2 sx = fmul2(si, x);                       // sigma_i x
-  o.dx = fmul2(g, fmul2(fmul2(m2, rm), si));
+  const float2 q = fmul2(rm, si);  // sigma_i / m
+  o.dx = fmul2(g, fmul2(m2, q));
   o.di = fmul2(fmul2(o.dx, x), fsub2(c.one, si));
   o.back = fmul2(a, g);
-  const float2 dla = fmul2(o.back, fsub2(hp, fmul2(fmul2(a, sx), rm)));
-  o.dk = fmul2(sr, dla);
+  // sigma_r before x: at a shut gate (sigma_r = 0, m = 0, q up to 2^63) x then meets a zero, where
+  // x q could overflow first and leave inf * 0 = NaN for a padded token's x above 4e19.
+  const float2 second = fmul2(fmul2(a, fmul2(sr, q)), x);
+  o.dk = fmul2(o.back, fsub2(fmul2(sr, hp), second));
   o.dr = fmul2(fmul2(o.dk, k), fsub2(sr, c.one));
   return o;
 }
