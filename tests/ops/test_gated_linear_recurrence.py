@@ -547,3 +547,59 @@ def test_padded_tokens_repeat_the_state(dtype):
             assert torch.equal(y[:, t], y[:, t - 1]), t
     if dtype == torch.float32:
         assert torch.equal(final, y[:, -1])
+
+
+# ------------------------------------------------------------ infinities stay what they are
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lam", [2.0, 30.0])  # decays of e^-8 and of e^-120 a token
+@pytest.mark.parametrize("B, T, D", [(2, 150, 66), (1, 700, 272), (3, 600, 1024), (40, 300, 200)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_infinities_outlive_any_decay(B, T, D, lam, packed, dtype):
+    """a > 0 however strong: an infinite state stays infinite to its sequence's end, and an
+    infinite gradient to its beginning, wherever the tokens are split; as token by token."""
+    if packed:
+        B, cu = 1, _cu([T // 3, 0, T - T // 3])
+    else:
+        cu = None
+    (x, i, r, _), h0, dy, dT = _inputs(B, T, D, dtype, nseq=3 if packed else None)
+    i, r, x = i.clamp(-3, 3), r.clamp(-3, 3), torch.where(x < 0, x - 0.1, x + 0.1)
+    lam = torch.full((D,), lam, device="cuda")
+    fwd = GatedLinearRecurrenceFwdOp(B, T, D, dtype=dtype, save_states=True)
+    bwd = GatedLinearRecurrenceBwdOp(B, T, D, dtype=dtype)
+    clean = fwd(x, i, r, lam, h0, cu)
+    clean += bwd(dy, x, i, r, lam, clean[2], h0, dT, cu)
+    inf = float("inf")
+    h1, x1, dy1, dT1 = h0.clone(), x.clone(), dy.clone(), dT.clone()
+    h1[0, 3], h1[-1, 8] = inf, -inf
+    x1[0, T // 2, 5] = -inf
+    dT1[-1, 17], dT1[0, 22], dy1[0, T // 2 + 3, 30] = -inf, inf, inf
+    y, final, states = fwd(x1, i, r, lam, h1, cu)
+    y_ref, f_ref, _, _ = ref.glr_fwd(x1, i, r, lam, h1, cu)
+    dx, di, _, _, d0 = bwd(dy1, x1, i, r, lam, states, h1, dT1, cu)
+    want, _ = ref.glr_bwd(dy1, x1, i, r, lam, h1, dT1, cu)
+    assert y_ref.isinf().any() and want[0].isinf().any() and want[4].isinf().any()
+    same = torch.ones(D, dtype=torch.bool, device="cuda")
+    same[[3, 5, 8, 17, 22, 30]] = False
+    for name, got, exact, before in (("y", y, y_ref, clean[0]), ("final", final, f_ref, clean[1]),
+                                     ("dx", dx, want[0], clean[3]), ("d0", d0, want[4], clean[7]),
+                                     ("di", di, want[1], clean[4])):
+        assert torch.equal(got[..., same], before[..., same]), name
+        if name == "di":  # x = -inf times 0 at one token, by the formula too
+            got, exact = got[..., [17, 22, 30]], exact[..., [17, 22, 30]]
+        got = got.cpu().double()
+        assert not got.isnan().any(), name
+        assert torch.equal(got.isinf() * got.sign(), exact.isinf() * exact.sign()), name
+
+
+def test_infinities_token_by_token():
+    D, inf = 66, float("inf")
+    for lam in (2.0, 30.0):
+        (x, i, r, _), h0, _, _ = _inputs(2, 30, D, torch.float32)
+        h0[0, 3], h0[1, 4] = inf, -inf
+        lam = torch.full((D,), lam, device="cuda")
+        y_ref, _, _, _ = ref.glr_fwd(x, i, r, lam, h0)
+        step = GatedLinearRecurrenceDecodeOp(2, D, dtype=torch.float32, inplace=True)
+        for t in range(30):
+            y, _ = step(x[:, t], i[:, t], r[:, t], lam, h0)
+            assert not y.isnan().any()
+            assert torch.equal(y.cpu().isinf(), y_ref[:, t].isinf())

@@ -215,13 +215,14 @@ __global__ void __launch_bounds__(G::kWarps * 32, G::kCtas)
 #pragma unroll
       for (int j = 0; j < kRun; ++j) {
         if (begins(j)) fwd = Run(both(kForget), before_seq(j));
-        fwd = kPacked ? Run(fwd.A.x < 0.0f ? fwd.A : fmul2(fwd.A, a[j]), ffma2(a[j], fwd.H, hp[j]))
+        fwd = kPacked ? Run(fwd.A.x < 0.0f ? fwd.A : ffma2(fwd.A, a[j], both(kLeastDecay)),
+                            ffma2(a[j], fwd.H, hp[j]))
                       : join<false>(fwd, Run(a[j], hp[j]));
       }
 #pragma unroll
       for (int j = kRun - 1; j >= 0; --j) {
         if (ends(j)) bwd = Run(both(kForget), after_seq(j));
-        bwd = Run(kPacked && bwd.A.x < 0.0f ? bwd.A : fmul2(bwd.A, a[j]),
+        bwd = Run(kPacked && bwd.A.x < 0.0f ? bwd.A : ffma2(bwd.A, a[j], both(kLeastDecay)),
                   fmul2(a[j], fadd2(dy_at(j), bwd.H)));
       }
     }
