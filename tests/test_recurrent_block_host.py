@@ -426,3 +426,18 @@ def test_rooflines_count_a_state_for_each_packed_sequence(accept_cpu, monkeypatc
     bwd = GatedLinearRecurrenceBwdOp(1, 100, 8, dtype=torch.float32)
     bwd(torch.randn(1, 100, 8), *args, states, None, None, cu)
     assert bwd.eval_roofline() == (40 * 800, 7 * 800 * 4 + 4 * 4 * 8 + 8 * 4 * 8 + 8 * 8)
+
+
+# ------------------------------------------------------------ workspaces of the C entry points
+def test_entry_points_refuse_a_misaligned_workspace():
+    """16-byte words go to the workspace: one off that boundary is refused before any launch."""
+    lib = _native.lib()
+    some = ctypes.c_void_p(1 << 20)
+    for off in (1, 2, 4, 8):
+        ws = ctypes.c_void_p((1 << 20) + off)
+        assert lib.tileops_glr_bwd(*[some] * 6, NULL, NULL, NULL, 0, *[some] * 5, ws, 1, 4, 8,
+                                   *[8] * 8, 8.0, 2, NULL) == _native.EALIGN
+        for bias in (NULL, some):
+            assert lib.tileops_sandwich_norm_bwd(
+                some, NULL, some, some, some, some, NULL, bias, some, some, some, some, NULL, bias,
+                NULL, ws, 4, 8, 1, 0, 1e-6, 1.0, 2, 2, NULL) == _native.EALIGN

@@ -397,6 +397,7 @@ extern "C" int tileops_glr_bwd(const void* dy, const void* x, const void* input_
   if (!dy || !x || !input_gate || !decay_gate || !decay_param || !states || !dx ||
       !d_input_gate || !d_decay_gate || !d_decay_param || !d_initial_state || !workspace)
     return TILEOPS_EINVAL;
+  if (!aligned16(workspace)) return TILEOPS_EALIGN;
   cudaStream_t s = as_stream(stream);
   const Strides st{x_stride_b, x_stride_t, i_stride_b, i_stride_t,
                    r_stride_b, r_stride_t, g_stride_b, g_stride_t};

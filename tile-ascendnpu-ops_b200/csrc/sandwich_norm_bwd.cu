@@ -524,6 +524,7 @@ extern "C" int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_
       !d_post_weight || !d_pre_weight || !workspace || (d_gate && !gate) ||
       (d_post_bias && !post_bias))
     return TILEOPS_EINVAL;
+  if (!aligned16(workspace)) return TILEOPS_EALIGN;
   cudaStream_t st = as_stream(stream);
   // The gate's gradient takes Q when there is a post_bias, whether or not that has one.
   const bool bias = post_bias || d_pre_bias;
