@@ -56,7 +56,8 @@ const char* tileops_status_string(int status);
 /* Device-side error word, read back by the host after the stream is
  * synchronised: 0 = none; 1 = a bounded mbarrier wait timed out (attention,
  * gated delta net); 2 = a malformed cu_seqlens was passed to
- * tileops_gdn_prefill_varlen_fwd, tileops_glr_fwd or tileops_glr_bwd.  The first code set is kept until cleared. */
+ * tileops_gdn_prefill_varlen_fwd, tileops_glr_fwd or tileops_glr_bwd.  The
+ * first code set is kept until cleared. */
 int tileops_device_error_flag(void* stream, int clear);
 
 /* Self-test of the give-up path the tensor-core kernels take when a wait
@@ -166,7 +167,8 @@ int64_t tileops_sandwich_norm_bwd_workspace_bytes(int64_t M, int64_t N, int64_t 
  * (gate_rows, N) of `affine_dtype`, summed in fp32 in a fixed order.  d_gate
  * needs gate and d_post_bias needs post_bias; those two and d_pre_bias may be
  * NULL (not written).  `workspace` holds
- * tileops_sandwich_norm_bwd_workspace_bytes() bytes, 16-byte aligned.  M >= 1. */
+ * tileops_sandwich_norm_bwd_workspace_bytes() bytes, 16-byte aligned
+ * (TILEOPS_EALIGN otherwise).  M >= 1. */
 int tileops_sandwich_norm_bwd(const void* dy, const void* d_residual_out, const void* x,
                               const void* residual_out, const void* post_weight,
                               const void* pre_weight, const void* gate, const void* post_bias,
@@ -245,8 +247,9 @@ int tileops_gla_decode_fwd(const void* q, const void* k, const void* v, const vo
 /* Per channel, with k = decay_scale * softplus(decay_param):
  *   a_t = exp(-k sigmoid(decay_gate_t));
  *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t;  y_t = h_t,
- * h in fp32.  x, input_gate, decay_gate (batch, seq_len, dim) of `dtype`
- * (f32/f16/bf16), channels contiguous, with their own batch and token strides
+ * h in fp32, a_t at least 2^-149 (infinite states stay infinite).
+ * x, input_gate, decay_gate (batch, seq_len, dim) of `dtype` (f32/f16/bf16),
+ * channels contiguous, with their own batch and token strides
  * in elements (>= 0); y (batch, seq_len, dim) dense; decay_param (dim,),
  * initial_state (NULL = zeros) and final_state (sequences, dim) fp32.
  * states (NULL = not written): (batch, ceil(seq_len / TILEOPS_GLR_SEGMENT), dim)
@@ -275,7 +278,8 @@ int64_t tileops_glr_bwd_workspace_bytes(int64_t batch, int64_t seq_len, int64_t 
  * inputs, its states and its initial_state: dx, d_input_gate, d_decay_gate
  * dense, of `dtype`; d_decay_param (dim,) and d_initial_state (sequences, dim)
  * fp32, summed in a fixed order.  `workspace` holds
- * tileops_glr_bwd_workspace_bytes() bytes, 16-byte aligned. */
+ * tileops_glr_bwd_workspace_bytes() bytes, 16-byte aligned (TILEOPS_EALIGN
+ * otherwise). */
 int tileops_glr_bwd(const void* dy, const void* x, const void* input_gate,
                     const void* decay_gate, const float* decay_param, const float* states,
                     const float* initial_state, const float* d_final_state,

@@ -12,7 +12,8 @@
 //   dloga = a G h_{t-1} - G sigma_i x a^2 / m
 //   dr    = -k sigma_r (1 - sigma_r) dloga  dlambda = -c sigmoid(lambda) sum sigma_r dloga
 // Where m = 0 (a gate closed to the last bit) the second term of dloga is 0,
-// its limit: it enters dr and dlambda as k sigma_r / m -> sqrt(k sigma_r / 2).
+// its limit: it enters dr and dlambda as k sigma_r / m -> sqrt(k sigma_r / 2).  1 / m stops
+// at 2^63.
 //
 // Packed sequences (cu_seqlens): the first token of a sequence takes its
 // predecessor from initial_state by selection, not by a zero factor, so
@@ -64,8 +65,9 @@ __device__ __forceinline__ void fwd_run(const T* mine, float2 k, const Consts& c
 //   4. so each lane has the state before its run;
 //   5. the run again, token by token from that state, and the stores.
 // Step 5 repeats the sequential recurrence itself, so y differs from it by the
-// rounding of the state a run starts with only.  x and the gates are read once
-// and y is written once.
+// rounding of the state a run starts with only (infinities stay infinite as there: decays
+// and their products never reach zero).  x and the gates are read once and y is
+// written once.
 template <typename T, typename G, int kBytes, bool kPacked, int kStages>
 __global__ void __launch_bounds__(G::kWarps * 32, G::kCtas)
     glr_fwd_scan(const __grid_constant__ FwdArgs p) {
@@ -237,8 +239,9 @@ int launch_fwd(const FwdArgs& a, int64_t batch, cudaStream_t s) {
     // itself, of 16 channels (more copies and shuffles an element) where those of 32
     // would leave half the SMs idle.  Fewer still: two of 8 warps an SM in
     // clusters, as one waits for its cluster while the other computes.
-    // 1 x 16384 x D bf16: D = 4096 120 us, with 8 warps and 16 channels 147; 2048 76 us,
-    // with 8 warps 83; 1024 57 us in clusters, with 15 warps 73; 256 29 and 48.
+    // 1 x 16384 x D bf16: D = 4096 120 us, with 8 warps and 16 channels 147; 2048 72 us,
+    // with 8 warps 83; 1024 55 us in clusters, with 15 warps 73; 256 28 and 48.  Above the
+    // first bound: 5120 236 us, with 15 warps 235; 1 x 1024 x 5120 21 us and 27.
     const int64_t ctas = (a.D + 31) / 32 * batch, sms = sm_count();
     if (ctas > sms) return launch_fwd_geo<T, Wide, 16, kStages>(a, batch, s);
     if (2 * ctas > sms) return launch_fwd_geo<T, Geo<32, 16, 15>, 16, kStages>(a, batch, s);

@@ -262,10 +262,10 @@ constexpr int kMaxCluster = 8;  // CTAs of a cluster
 // no predecessor, so runs are worked out side by side, their maps joined, and
 // each walked again from its true state: two fma an element more than the
 // chain, and every tensor is still read once (DRAM traffic measured within 1% of the
-// algorithm's).  Forward, an element takes 31 issue slots, of which 5 on the
+// algorithm's).  Forward, an element takes 32 to 33 issue slots, of which 5 on the
 // special-function unit (16 lanes a clock and SM: 37 us of the 41 us that 8 x
 // 1024 x 4096 bf16 takes at the copy rate); 16 warps of 128 registers an SM
-// keep that unit at 58 to 68% busy (71 us; 8 x 4096 x 4096 214 us, 0.77 of the
+// keep that unit at 58 to 68% busy (72 us; 8 x 4096 x 4096 215 us, 0.77 of the
 // copy rate).  Measured and not taken: 24 warps with runs of 8 tokens, 20%
 // slower (twice the joins); a barrier a step in place of the chain of warps,
 // 3% slower; 64 channels a CTA, 10% slower (half as many CTAs to fill the SMs).

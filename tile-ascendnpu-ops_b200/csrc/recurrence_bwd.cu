@@ -78,9 +78,9 @@ __device__ __forceinline__ TokenGrads token_grads(float2 g, float2 hp, float2 x,
 // H = a_t (dy_t + H).  The states h are walked anew from the forward's saved ones, one a
 // warp's run.  A lane takes 8 tokens: decay, state and both sigmoids of each stay in
 // registers, so no element's gates are computed twice but for m.
-// An element takes 82 issue slots (6 on the special-function unit), and that bounds it: 8 x
-// 4096 x 4096 bf16 takes 450 us, 4.2 TB/s of its 14.25 bytes an element, 0.64 of
-// the copy rate, with 58 to 64% of the issue slots used.
+// An element takes 79 to 82 issue slots (6 on the special-function unit): 8 x 4096 x 4096 bf16
+// takes 453 us, 4.2 TB/s of its 14.125 bytes an element, 0.64 of the copy rate, with 58 to
+// 63% of the issue slots used, neither of the two full.
 template <typename T, typename G, int kBytes, bool kPacked, int kStages>
 __global__ void __launch_bounds__(G::kWarps * 32, G::kCtas)
     glr_bwd_scan(const __grid_constant__ BwdArgs p) {
@@ -336,7 +336,9 @@ int launch_bwd(const BwdArgs& a, int64_t batch, cudaStream_t s, int64_t* parts) 
                               copy_bytes(a.dr, a.D, a.D, eb)});
   if (bytes == 16) {
     // One CTA of 15 warps an SM where the channels make at most one each, and at least one
-    // for every second (the forward's rule; 1 x 16384 x 2048 bf16 135 us, with 8 warps 180).
+    // for every second (the forward's rule; 1 x 16384 x 2048 bf16 134 us, with 8 warps 180).
+    // With more channels it would gain nothing: 1 x 16384 x 2560 256 us both ways, x 4096 251
+    // and 257, 1 x 1024 x 4096 32 and 34.
     const int64_t ctas = (a.D + 15) / 16 * batch, sms = sm_count();
     if (ctas <= sms && 2 * ctas > sms)
       return launch_bwd_geo<T, Geo<16, 8, 15>, 16>(a, batch, s, parts);

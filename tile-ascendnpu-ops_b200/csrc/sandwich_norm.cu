@@ -20,16 +20,19 @@
 //
 // Both passes read each row once and write it once: persistent CTAs walk
 // consecutive rows, a thread owns the same columns in every row (parameters and
-// column sums stay in registers) and copies its own packets of the rows ahead into
-// a private slot of a shared-memory ring.  A row costs one barrier, although it
-// has two reductions one after another: the second of a row is exchanged together with the
+// column sums stay with it, in registers but for the spills named below) and copies its own
+// packets of the rows ahead into a private slot of a shared-memory ring.  A row costs one
+// barrier, although it has two reductions one after another: the second of a row is exchanged together with the
 // first of the next one.  A LayerNorm's mean and variance are taken warp by
 // warp, centred there, and joined (Chan, Golub & LeVeque, "Updating formulae
 // and a pairwise algorithm for computing sample variances", 1979).
 //
-// Measured (bf16, fp32 parameters): forward 8192 x 4096 52 us RMS, 54 us LayerNorm with
-// biases and 8 gates (0.80 and 0.77 of the copy rate); backward 16384 x 4096 with its
-// parameter sums 142 us (0.87), LayerNorm with biases 195 us (0.64).  Steps on the
+// Measured (bf16, fp32 parameters): forward 8192 x 4096 52 us RMS, 53 us LayerNorm with
+// biases and 8 gates (0.80 and 0.78 of the copy rate); backward 16384 x 4096 with its
+// parameter sums 143 us (0.87), LayerNorm with biases 195 us (0.64).  All fp32: 8192 x
+// 4096 92 us (0.90) and 147 us (0.84).  Rows of 4097 to 8192 in 16 bits take 512 threads
+// of 128 registers; backward with biases these spill 96 to 364 bytes a thread, up to 428 where
+// copies are of 4 bytes (4096 x 8192 LayerNorm with biases 162 us, 0.38).  Steps on the
 // way: two barriers a row instead of one 60 and 193 us; scalar in place of packed
 // arithmetic 72 and 234 us; the kind of norm tested at run time 55 and 149 us.
 #include "sandwich_norm.cuh"

@@ -465,11 +465,14 @@ __global__ void __launch_bounds__(512) sn_bwd_wide(const BwdArgs p) {
   }
 }
 
-// CTAs an SM of the backward pass: as many as their registers allow (each adds a stretch of
-// column sums to write and read).  With biases there are twice the sums, and a row of
-// 4096 takes more than the 128 registers a thread of two CTAs has (16384 x 4096
+// CTAs an SM of the backward pass: for 16-bit rows, as many as their registers allow (each adds
+// a stretch of column sums to write and read).  With biases there are twice the sums, and
+// a row of 4096 takes more than the 128 registers a thread of two CTAs has (16384 x 4096
 // bf16, before the norms were kernels of their own: two CTAs 152 us without and 284 us
-// with biases, one 165 and 225 us).
+// with biases, one 165 and 225 us).  The rule was measured in 16 bits only.  An fp32 row has
+// twice the packets and a larger ring: of 513 to 1024 columns, 1025 to 2048 with biases and
+// 2049 to 4096 without, half of these CTAs are resident and the others follow them (1025 x
+// 1155 LayerNorm with biases 37 us, 0.12 of the copy rate; 8192 x 4096 RMS 147 us, 0.84).
 int64_t ctas_per_sm(int64_t N, bool bias) {
   if (N > 8192) return 2;  // the passes over L2, or one CTA at a time of the others
   return N <= 1024 ? 4 : (N <= 2048 ? 2 : (N <= 4096 && !bias ? 2 : 1));

@@ -86,6 +86,7 @@ class FusedSandwichNormBwdKernel(_SandwichNormKernel):
         _native.launch(
             "tileops_sandwich_norm_bwd", x.device, dy.data_ptr(), ptr(d_residual_out),
             x.data_ptr(), residual_out.data_ptr(), post_weight.data_ptr(), pre_weight.data_ptr(),
-            ptr(gate), ptr(post_bias), dx.data_ptr(), d_residual.data_ptr(), *map(ptr, grads), ws.data_ptr(), self.M, self.N, groups, self._norm_code,
-            self.eps, self.residual_scale, self._code, _native.dtype_code(post_weight.dtype))
+            ptr(gate), ptr(post_bias), dx.data_ptr(), d_residual.data_ptr(), *map(ptr, grads),
+            ws.data_ptr(), self.M, self.N, groups, self._norm_code, self.eps,
+            self.residual_scale, self._code, _native.dtype_code(post_weight.dtype))
         return dx, d_residual, *grads

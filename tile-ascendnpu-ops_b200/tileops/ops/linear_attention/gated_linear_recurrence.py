@@ -9,7 +9,8 @@ recurrent block behind a causal depthwise conv1d.  Per channel, with
     y_t = h_t                                   (h in fp32, y rounded once)
 
 A decay gate of -inf has a = 1 exactly and takes no input: a padded token (whose
-x and input_gate are still read and must be finite).
+x and input_gate are still read and must be finite, but have no say).  a stays
+above zero however strong the decay: an infinite state stays infinite.
 
     GatedLinearRecurrenceFwdOp(batch, seq_len, dim, decay_scale=8.0, dtype=torch.bfloat16,
                                save_states=False, kernel_map=None)
@@ -32,7 +33,9 @@ decay_param (dim,), the states (batch, dim) and ``states`` (batch,
 ceil(seq_len / 32), dim) are float32.  Packed sequences follow the GDN op:
 batch 1, ``cu_seqlens`` an integer device tensor of N + 1 offsets 0, ...,
 seq_len, one initial and final state per sequence; offsets that break this
-rule set the device error flag to 2.  Like every op here, these build no
+rule set the device error flag to 2 (with seq_len 0 nothing is launched and they
+are not read).  A device's first packed call looks that flag up: make it outside
+a graph's capture.  Like every op here, these build no
 autograd graph: a training loop calls the two ops itself.
 """
 
