@@ -56,8 +56,10 @@ const char* tileops_status_string(int status);
 /* Device-side error word, read back by the host after the stream is
  * synchronised: 0 = none; 1 = a bounded mbarrier wait timed out (attention,
  * gated delta net); 2 = a malformed cu_seqlens was passed to
- * tileops_gdn_prefill_varlen_fwd, tileops_glr_fwd or tileops_glr_bwd.  The
- * first code set is kept until cleared. */
+ * tileops_gdn_prefill_varlen_fwd, tileops_glr_fwd, tileops_glr_bwd or
+ * tileops_paged_kv_append; 3 = a token in use has no valid page
+ * (tileops_paged_kv_append, tileops_paged_decode_fwd).  The first code set is
+ * kept until cleared. */
 int tileops_device_error_flag(void* stream, int clear);
 
 /* Self-test of the give-up path the tensor-core kernels take when a wait
@@ -399,6 +401,74 @@ int tileops_gdn_prefill_fwd_noalloc(const void* q, const void* k, const void* v,
                                     float* final_state, int64_t batch, int64_t seq_len,
                                     int64_t heads, int64_t dim_k, int64_t dim_v,
                                     int64_t chunk_size, double scale, int dtype, void* stream);
+
+/* ---- rotary positions, paged cache, single-token attention -------------- */
+/* No counterpart in the reference. */
+
+/* q (batch, seq_len, heads, dim) and k (batch, seq_len, heads_kv, dim) of
+ * `dtype` (f32 / f16 / bf16) with their first rotary_dim channels (even, <= 256)
+ * rotated by their positions:  x'_a = c x_a - s x_b, x'_b = s x_a + c x_b,
+ * c, s = amplitude * cos, sin of position * angle, (a, b) = (i, i + rotary_dim / 2)
+ * or, `interleaved`, (2i, 2i + 1).  `backward`: the transposed map.  turns (a
+ * HOST array of rotary_dim / 2, read before the call returns): the pairs'
+ * angles a token in whole 2^-64 turns, modulo one turn.  positions: int32 or
+ * int64 (position_dtype) at position_stride * b + t, or NULL for t.  strides12
+ * (HOST): elements from a batch entry, token and head to the next of q, k,
+ * q_out, k_out; channels are contiguous.  q_out may be q and k_out k with the
+ * same strides (in place); they may not overlap otherwise.  heads or heads_kv
+ * may be 0 (their pointers are then not used). */
+int tileops_rotary(const void* q, const void* k, const void* positions, void* q_out, void* k_out,
+                   const uint64_t* turns, int64_t batch, int64_t seq_len, int64_t heads,
+                   int64_t heads_kv, int64_t dim, int64_t rotary_dim, const int64_t* strides12,
+                   int64_t position_stride, int position_dtype, int interleaved, int backward,
+                   double amplitude, int dtype, void* stream);
+
+/* The new tokens of num_seqs sequences into a paged cache: k rotated (as in
+ * tileops_rotary) and v to slot p % page_size of page page_table[b][p / page_size],
+ * p the token's position; q (heads may be 0) rotated into q_out.  Sequence b's
+ * new tokens are its last: rows [cu_seqlens[b], cu_seqlens[b + 1]) of the
+ * `tokens` rows, or with cu_seqlens NULL tokens / num_seqs rows each, row i of
+ * n at position seq_lens[b] - n + i (seq_lens: lengths after the call).  A row
+ * of a negative position is padding, as are rows behind cu_seqlens[num_seqs]:
+ * zeros in q_out, nothing in the caches.  A cu_seqlens that is not 0 = first
+ * <= ... <= last <= tokens sets the device error flag to 2; a position without
+ * a page in [0, num_pages) sets it to 3 and is not written.  page_table
+ * (num_seqs, table_width) with rows table_stride apart, entries behind a
+ * sequence's end are not read.  strides18 (HOST): elements from a batch entry,
+ * token and head to the next of q, k, v, q_out (packed: the first is not used),
+ * and from a page, slot and head to the next of k_cache and v_cache.  Two rows
+ * with the same slot race. */
+int tileops_paged_kv_append(const void* q, const void* k, const void* v, void* q_out,
+                            void* k_cache, void* v_cache, const int32_t* page_table,
+                            const int32_t* seq_lens, const int32_t* cu_seqlens,
+                            const uint64_t* turns, int64_t num_seqs, int64_t tokens, int64_t heads,
+                            int64_t heads_kv, int64_t dim, int64_t rotary_dim, int64_t num_pages,
+                            int64_t page_size, int64_t table_width, int64_t table_stride,
+                            const int64_t* strides18, int interleaved, double amplitude, int dtype,
+                            void* stream);
+
+/* Bytes of scratch tileops_paged_decode_fwd needs, whatever the batch and the
+ * lengths, or -1 for an unsupported shape. */
+int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t heads_kv, int64_t dim);
+
+/* Attention of one token of every sequence over the cached tokens
+ * max(0, seq_lens[b] - window) .. seq_lens[b] - 1 (window 0: all):  o (batch,
+ * heads, dim) of `dtype` (f16 / bf16) dense, lse (batch, heads) fp32 in the log2
+ * domain.  Query head h reads key head h / (heads / heads_kv).  A sequence of
+ * no token (seq_lens[b] <= 0) has o = 0 and lse = -inf.  dim a multiple of 8 up
+ * to 256, page_size * table_width < 2^31 - 64.  strides8 (HOST, multiples of 8):
+ * elements from a sequence and head to the next of q, from a page, slot and
+ * head to the next of k_cache and of v_cache.  q, caches, workspace 16-byte
+ * aligned; `workspace` holds tileops_paged_decode_workspace_bytes() bytes.  A
+ * seq_lens[b] above page_size * table_width (taken as that) or a page outside
+ * [0, num_pages) (taken as zeros) sets the device error flag to 3; table
+ * entries of no token in use are not read. */
+int tileops_paged_decode_fwd(const void* q, const void* k_cache, const void* v_cache,
+                             const int32_t* page_table, const int32_t* seq_lens, void* o,
+                             float* lse, void* workspace, int64_t batch, int64_t heads,
+                             int64_t heads_kv, int64_t dim, int64_t num_pages, int64_t page_size,
+                             int64_t table_width, int64_t table_stride, const int64_t* strides8,
+                             int64_t window, double scale, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

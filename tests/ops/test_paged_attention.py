@@ -1,0 +1,443 @@
+"""GPU parity of the paged-cache ops against the 64-bit oracle; values are held to its error bound
+plus half a step of their type."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import serving_attention as ref
+from oracle.recurrent import assert_within
+from tileops import _native as nat
+from tileops.ops.attention import PagedAttentionDecodeOp, PagedKVAppendOp, rotary_frequencies
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+HALF = [torch.float16, torch.bfloat16]
+
+
+def _flag(clear=1):
+    return nat.lib().tileops_device_error_flag(nat.stream_handle(torch.device("cuda", 0)), clear)
+
+
+@pytest.fixture(autouse=True)
+def no_flag():
+    _flag()
+    yield
+    assert _flag() == 0
+
+
+def _cache(pages, P, Hkv, D, dtype, layout="token", fill=None):
+    shape = (pages, P, Hkv, D) if layout == "token" else (pages, Hkv, P, D)
+    c = torch.randn(shape, device="cuda").to(dtype) if fill is None else torch.full(
+        shape, fill, device="cuda", dtype=dtype)
+    return c if layout == "token" else c.transpose(1, 2)
+
+
+def _table(lens, P, extra=0, spare=3):
+    """Pages of every sequence in a mixed order, -1 behind its end, and how many pages there are."""
+    need = [max(0, -(-n // P)) for n in lens]
+    width = max([1, *need]) + extra
+    order = torch.randperm(sum(need) + spare).tolist()
+    table = torch.full((len(lens), width), -1, dtype=torch.int32)
+    for b, n in enumerate(need):
+        for c in range(n):
+            table[b, c] = order.pop()
+    return table.cuda(), sum(need) + spare
+
+
+def _lens(lens):
+    return torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------ attention
+def _whole(*shape, dtype):
+    """Whole numbers from -2 to 2: products and sums of them are exact."""
+    return torch.randint(-2, 3, shape, device="cuda").to(dtype)
+
+
+def _attend(lens, H, Hkv, D, P, dtype, layout="token", window=None, scale=None, exact=True, extra=0):
+    """Behind each sequence's end (and before its window) the cache holds NaN; the first and last
+    tokens that count hold large values, so that one too few shows in o."""
+    table, pages = _table(lens, P, extra)
+    kc, vc = _cache(pages, P, Hkv, D, dtype, layout, fill=math.nan), _cache(
+        pages, P, Hkv, D, dtype, layout, fill=math.nan)
+    for b, n in enumerate(lens):
+        first = max(0, n - window) if window else 0
+        at = torch.arange(first, max(n, 0), device="cuda")
+        where = (table[b].long()[at // P], at % P)
+        kc[where] = _whole(len(at), Hkv, D, dtype=dtype) if exact else torch.randn(
+            len(at), Hkv, D, device="cuda").to(dtype)
+        v = torch.randn(len(at), Hkv, D, device="cuda")
+        if n > 0:
+            v[0] += 50
+            v[-1] -= 70
+        vc[where] = v.to(dtype)
+    q = _whole(len(lens), H, D, dtype=dtype) if exact else (
+        2 * torch.randn(len(lens), H, D, device="cuda")).to(dtype)
+    scale = 0.25 / D**0.5 if scale is None and exact else scale
+    op = PagedAttentionDecodeOp(H, Hkv, D, P, scale, window, dtype)
+    lens = _lens(lens)
+    o, lse = op(q, kc, vc, table, lens)
+    want = ref.attend(q, kc, vc, table, lens, scale, window, exact_scores=exact)
+    assert_within(o, want[0], want[2], "o")
+    live = lens > 0
+    assert_within(lse[live], want[1][live.cpu()], want[3][live.cpu()], "lse")
+    assert (lse[~live] == -math.inf).all() and (o[~live] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("H, Hkv, D", [
+    (1, 1, 64), (32, 8, 128), (4, 4, 128), (12, 2, 80), (6, 1, 96), (8, 1, 40), (16, 1, 128),
+    (24, 1, 64), (17, 1, 128), (33, 1, 72), (64, 2, 128), (80, 1, 256), (16, 8, 192), (3, 3, 8),
+    (20, 1, 104), (40, 1, 96),
+])
+def test_heads_and_widths(H, Hkv, D, dtype):
+    _attend([70, 1, 0, 200], H, Hkv, D, 16, dtype)
+
+
+@pytest.mark.parametrize("layout", ["token", "head"])
+@pytest.mark.parametrize("P", [1, 2, 7, 16, 64, 100, 256])
+@pytest.mark.parametrize("lens", [
+    [1], [15], [16], [17], [63], [64], [65], [0, 0, 129, 0], [127, 128, 3], [1000, 5, 64, 0, 333],
+])
+def test_lengths_and_pages(lens, P, layout):
+    _attend(lens, 4, 2, 64, P, torch.bfloat16, layout)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("lens", [
+    [5000], [20000], [1, 9000, 17, 0, 4000], [300] * 100, [64] * 400, [1] * 700, list(range(200)),
+    [0] * 300 + [777] + [0] * 300,
+])
+def test_splits(lens, dtype):
+    """One item over many CTAs, CTAs of many items, items that begin and end inside a CTA."""
+    _attend(lens, 2, 1, 64, 16, dtype)
+
+
+@pytest.mark.parametrize("H, Hkv, D", [(8, 8, 128), (40, 2, 128), (32, 1, 256), (16, 4, 192)])
+def test_splits_of_many_heads(H, Hkv, D):
+    _attend([3000, 1, 700, 0, 64], H, Hkv, D, 32, torch.float16)
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 65, 200, 10000])
+def test_window(window):
+    _attend([0, 1, 64, 65, 500, 1500], 4, 2, 64, 16, torch.bfloat16, window=window)
+    _attend([0, 1, 64, 65, 500, 1500], 4, 2, 64, 7, torch.float16, "head", window=window)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("scale", [None, 1.0, 0.0, -0.3])
+def test_ordinary_numbers(scale, dtype):
+    _attend([300, 7, 1200], 8, 2, 128, 16, dtype, scale=scale, exact=False)
+
+
+def test_one_key_takes_all():
+    """A score far above the others', first, last or between, and far below."""
+    D, P, n = 64, 16, 1000
+    table, pages = _table([n], P)
+    kc, vc = _cache(pages, P, 1, D, torch.float16), _cache(pages, P, 1, D, torch.float16)
+    kc.mul_(0.01)
+    q = torch.ones(1, 3, D, device="cuda", dtype=torch.float16)
+    op = PagedAttentionDecodeOp(3, 1, D, P, dtype=torch.float16)
+    for at in (0, 1, 63, 64, 500, n - 1):
+        for size in (40.0, -40.0):
+            page, slot = int(table[0, at // P]), at % P
+            keep = kc[page, slot].clone()
+            kc[page, slot] = size
+            o, lse = op(q, kc, vc, table, _lens([n]))
+            want = ref.attend(q, kc, vc, table, _lens([n]))
+            assert_within(o, want[0], want[2], f"o, key {at}")
+            assert_within(lse, want[1], want[3], f"lse, key {at}")
+            if size > 0:
+                assert torch.equal(o[0], vc[page, slot].expand(3, D))
+            kc[page, slot] = keep
+
+
+def test_infinities_and_nan():
+    """-inf scores have no weight; +inf and NaN make their head's row NaN and no other's."""
+    D, P, n = 64, 16, 300
+    table, pages = _table([n, n], P)
+    kc, vc = _cache(pages, P, 2, D, torch.bfloat16), _cache(pages, P, 2, D, torch.bfloat16)
+    q = torch.rand(2, 4, D, device="cuda").to(torch.bfloat16) + 0.5
+    op = PagedAttentionDecodeOp(4, 2, D, P)
+    clean, lse0 = op(q, kc, vc, table, _lens([n, n]))
+    for at, value in ((10, math.inf), (299, math.nan), (0, math.inf)):
+        bad = kc.clone()
+        bad[int(table[1, at // P]), at % P, 1] = value
+        o, lse = op(q, bad, vc, table, _lens([n, n]))
+        assert torch.equal(o[0], clean[0]) and torch.equal(o[1, :2], clean[1, :2])
+        assert torch.equal(lse[0], lse0[0]) and torch.equal(lse[1, :2], lse0[1, :2])
+        assert o[1, 2:].isnan().all() and lse[1, 2:].isnan().all()
+    less = kc.clone()  # every key but the first 5 at -inf: what is left is a sequence of 5
+    for at in range(5, n):
+        less[int(table[1, at // P]), at % P] = -math.inf
+    o, lse = op(q, less, vc, table, _lens([n, n]))
+    want = ref.attend(q, kc, vc, table, _lens([n, 5]))
+    assert_within(o, want[0], want[2])
+    assert_within(lse, want[1], want[3])
+    for at in range(5):
+        less[int(table[1, at // P]), at % P] = -math.inf
+    o, lse = op(q, less, vc, table, _lens([n, n]))  # no key with a weight
+    assert (o[1] == 0).all() and (lse[1] == -math.inf).all() and torch.equal(o[0], clean[0])
+
+
+def test_fp16_keeps_small_weights():
+    """One weight of 1 and thousands of 2^-20, which fp16 alone would hold in 4 bits."""
+    D, P, n = 64, 16, 8000
+    table, pages = _table([n], P)
+    kc = _cache(pages, P, 1, D, torch.float16, fill=0.0)
+    vc = _cache(pages, P, 1, D, torch.float16, fill=1.0)
+    at = 77
+    kc[int(table[0, at // P]), at % P, 0, 0] = 20.3
+    vc[int(table[0, at // P]), at % P] = 0.0
+    q = torch.zeros(1, 1, D, device="cuda", dtype=torch.float16)
+    q[0, 0, 0] = 1.0
+    op = PagedAttentionDecodeOp(1, 1, D, P, math.log(2.0), dtype=torch.float16)
+    o, _ = op(q, kc, vc, table, _lens([n]))
+    want = 1.0 / (1.0 + 2.0 ** float(kc[int(table[0, 4]), 13, 0, 0]) / (n - 1))
+    # The weights all round alike, half a step, and so does the output; the rest is below 2^-14.
+    assert abs(float(o[0, 0, 0]) - want) < want * (2**-10 + 2**-14)
+
+
+def test_shared_prefix_pages_and_a_cache_without_pages():
+    D, P = 64, 16
+    kc, vc = _cache(9, P, 2, D, torch.bfloat16), _cache(9, P, 2, D, torch.bfloat16)
+    table = torch.tensor([[0, 1, 2, 3], [0, 1, 4, 5], [0, 1, 2, 6]], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 4, D, device="cuda").to(torch.bfloat16)
+    o, lse = PagedAttentionDecodeOp(4, 2, D, P)(q, kc, vc, table, _lens([60, 64, 49]))
+    want = ref.attend(q, kc, vc, table, _lens([60, 64, 49]))
+    assert_within(o, want[0], want[2])
+    assert_within(lse, want[1], want[3])
+    k, v = (torch.randn(3, 200, 2, D, device="cuda").to(torch.bfloat16) for _ in range(2))
+    table = torch.arange(3, dtype=torch.int32, device="cuda")[:, None]
+    o, lse = PagedAttentionDecodeOp(4, 2, D, 200)(q, k, v, table, _lens([200, 3, 77]))
+    want = ref.attend(q, k, v, table, _lens([200, 3, 77]))
+    assert_within(o, want[0], want[2])
+
+
+def test_layouts():
+    """q as a column slice, keys and values side by side in one buffer, a table with wide rows."""
+    D, P, lens = 64, 16, [100, 33, 0]
+    table, pages = _table(lens, P)
+    wide = torch.full((3, 20), -1, dtype=torch.int32, device="cuda")
+    wide[:, 5:5 + table.shape[1]] = table
+    both = torch.randn(pages, P, 2, 2, D, device="cuda").to(torch.bfloat16)
+    kc, vc = both[:, :, 0], both[:, :, 1]
+    qkv = torch.randn(3, 4 * D + 24, device="cuda").to(torch.bfloat16)
+    op = PagedAttentionDecodeOp(4, 2, D, P)
+    for q in (qkv[:, 24:], qkv[:, 3:3 + 4 * D], torch.randn(D, 4, 3, device="cuda").bfloat16().permute(2, 1, 0).flip(2)):
+        q = q.unflatten(1, (4, D)) if q.dim() == 2 else q
+        for t in (table, wide[:, 5:], table.t().contiguous().t()):
+            o, lse = op(q, kc, vc, t, _lens(lens))
+            want = ref.attend(q, kc, vc, t, _lens(lens))
+            assert_within(o, want[0], want[2])
+            assert_within(lse[:2], want[1][:2], want[3][:2])
+    spread = torch.tensor([100, 9, 33, 9, 0, 9], dtype=torch.int32, device="cuda")[::2]
+    assert torch.equal(op(q, kc, vc, table, spread)[0], o)
+
+
+def test_nothing_to_do():
+    kc = _cache(1, 16, 2, 64, torch.bfloat16)
+    op = PagedAttentionDecodeOp(4, 2, 64, 16)
+    o, lse = op(torch.empty(0, 4, 64, device="cuda", dtype=torch.bfloat16), kc, kc,
+                torch.empty(0, 3, dtype=torch.int32, device="cuda"), _lens([]))
+    assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
+    q = torch.randn(2, 4, 64, device="cuda").to(torch.bfloat16)
+    o, lse = op(q, kc, kc, torch.empty(2, 0, dtype=torch.int32, device="cuda"), _lens([0, -5]))
+    assert (o == 0).all() and (lse == -math.inf).all()
+
+
+def test_repeats_to_the_bit_and_runs_on_two_streams():
+    lens = [4000, 17, 900, 0, 2500]
+    table, pages = _table(lens, 16)
+    kc, vc = _cache(pages, 16, 2, 128, torch.bfloat16), _cache(pages, 16, 2, 128, torch.bfloat16)
+    q = torch.randn(5, 8, 128, device="cuda").to(torch.bfloat16)
+    op = PagedAttentionDecodeOp(8, 2, 128, 16)
+    want = op(q, kc, vc, table, _lens(lens))
+    lens = _lens(lens)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s in side:
+            with torch.cuda.stream(s):
+                got.append(op(q, kc, vc, table, lens))
+    torch.cuda.synchronize()
+    for o, lse in got:
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+
+
+def test_two_graphs_of_one_pool():
+    """Two captured steps that may share their workspace's memory, replayed in turn with lengths
+    that change between replays."""
+    lens = _lens([300, 0, 2000])
+    table, pages = _table([2100, 2100, 2100], 16)
+    kc, vc = _cache(pages, 16, 1, 64, torch.bfloat16), _cache(pages, 16, 1, 64, torch.bfloat16)
+    q = torch.randn(3, 2, 64, device="cuda").to(torch.bfloat16)
+    op = PagedAttentionDecodeOp(2, 1, 64, 16)
+    op(q, kc, vc, table, lens)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    pool = torch.cuda.graph_pool_handle()
+    for g in graphs:
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(op(q, kc, vc, table, lens))
+    for now in ([300, 0, 2000], [1, 2100, 64], [0, 0, 0], [2100, 2100, 2100]):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        for g in graphs:
+            g.replay()
+        want = ref.attend(q, kc, vc, table, lens)
+        for o, lse in outs:
+            assert_within(o, want[0], want[2], str(now))
+            live = lens > 0
+            assert_within(lse[live], want[1][live.cpu()], want[3][live.cpu()])
+
+
+def test_offsets_past_32_bits():
+    """Pages more than 2^32 elements apart."""
+    far = torch.empty(2**32 + 2**16, dtype=torch.bfloat16, device="cuda")
+    kc = far.as_strided((2, 16, 2, 64), (2**32, 128, 64, 1))
+    vc = far.as_strided((2, 16, 2, 64), (2**32, 128, 64, 1), 4096)
+    kc.normal_()
+    vc.normal_()
+    table = torch.tensor([[1, 0]], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 4, 64, device="cuda").to(torch.bfloat16)
+    o, lse = PagedAttentionDecodeOp(4, 2, 64, 16)(q, kc, vc, table, _lens([30]))
+    want = ref.attend(q, kc, vc, table, _lens([30]))
+    assert_within(o, want[0], want[2])
+    k, v = (torch.randn(1, 30, 2, 64, device="cuda").to(torch.bfloat16) for _ in range(2))
+    PagedKVAppendOp(2, 64, 16)(k, v, kc, vc, table, _lens([30]))
+    assert torch.equal(kc[1], k[0, :16]) and torch.equal(kc[0, :14], k[0, 16:])
+    assert torch.equal(vc[1], v[0, :16]) and torch.equal(vc[0, :14], v[0, 16:])
+
+
+def test_a_token_without_a_page_sets_the_flag():
+    kc, vc = _cache(4, 16, 1, 64, torch.bfloat16), _cache(4, 16, 1, 64, torch.bfloat16)
+    q = torch.randn(1, 1, 64, device="cuda").to(torch.bfloat16)
+    op = PagedAttentionDecodeOp(1, 1, 64, 16)
+    for table, n in (([0, 4], 20), ([0, -1], 20), ([1, 2], 33), ([1, 2], 2**31 - 1)):
+        table = torch.tensor([table], dtype=torch.int32, device="cuda")
+        op(q, kc, vc, table, _lens([n]))
+        assert _flag() == 3
+    op(q, kc, vc, torch.tensor([[0, 99]], dtype=torch.int32, device="cuda"), _lens([16]))
+    assert _flag() == 0  # the entry is of no token in use
+
+
+# ------------------------------------------------------------ append
+def _append(lens, new, H, Hkv, D, P, dtype, layout="token", packed=False, R=None, interleaved=False,
+            frequencies=None, amplitude=1.0, tail=0, queries=True, extra=0):
+    R = D if R is None else R
+    f = rotary_frequencies(R) if frequencies is None else frequencies
+    table, pages = _table(lens, P, extra)
+    kc, vc = _cache(pages, P, Hkv, D, dtype, layout), _cache(pages, P, Hkv, D, dtype, layout)
+    cu = None
+    if packed:
+        cu = torch.tensor([0, *new]).cumsum(0).to(torch.int32).cuda()
+        rows = (sum(new) + tail,)
+    else:
+        rows = (len(lens),) if new == 1 else (len(lens), new)
+    q, k, v = (torch.randn(*rows, h, D, device="cuda").to(dtype) for h in (H, Hkv, Hkv))
+    q = q if queries else None
+    want = ref.append(k, v, kc, vc, table, _lens(lens), f, q, cu, amplitude, interleaved)
+    op = PagedKVAppendOp(Hkv, D, P, H, R, interleaved, frequencies, amplitude, dtype)
+    got = op(k, v, kc, vc, table, _lens(lens), q, cu)
+    if queries:
+        assert_within(got, want[0], want[1], "q")
+    else:
+        assert got is None
+    assert_within(kc, want[2], want[3], "k_cache")
+    assert torch.equal(vc.cpu().double(), want[4])
+    live = (want[3] > 0).any(-1)  # slots that nothing was written to are as they were
+    assert_within(kc[~live], want[2][~live], torch.zeros_like(want[2][~live]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["token", "head"])
+@pytest.mark.parametrize("P", [1, 7, 16, 64])
+@pytest.mark.parametrize("lens, new", [
+    ([1], 1), ([100], 1), ([5, 0, 64, 17], 1), ([40], 40), ([40, 16, 0], 7), ([3, 2, 50], 5),
+])
+def test_append(lens, new, P, layout, dtype):
+    _append(lens, new, 4, 2, 64, P, dtype, layout)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens, new", [
+    ([9], [9]), ([20, 64, 5], [4, 64, 1]), ([0, 30, 30, 7], [0, 0, 30, 2]), ([5, 3], [9, 9]),
+    ([100] * 40, [1, 2, 3, 0] * 10),
+])
+@pytest.mark.parametrize("tail", [0, 5])
+def test_append_packed(lens, new, tail, dtype):
+    _append(lens, new, 4, 1, 64, 16, dtype, packed=True, tail=tail)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H, Hkv, D, R, interleaved", [
+    (1, 1, 8, 0, False), (32, 8, 128, 128, False), (3, 1, 80, 40, True), (2, 2, 33, 10, False),
+    (2, 2, 33, 10, True), (5, 1, 256, 256, True), (2, 1, 50, 50, False), (64, 4, 96, 96, False),
+])
+def test_append_heads_and_rotations(H, Hkv, D, R, interleaved, dtype):
+    _append([50, 3, 77], 3, H, Hkv, D, 16, dtype, R=R, interleaved=interleaved)
+    _append([50, 3, 77], [3, 3, 20], H, Hkv, D, 16, dtype, packed=True, R=R,
+            interleaved=interleaved, queries=False)
+
+
+def test_append_scaled():
+    f = rotary_frequencies(64, factor=8.0, original_length=4096)
+    _append([5000, 12], 12, 2, 1, 64, 32, torch.float32, frequencies=f, amplitude=1.2)
+
+
+def test_append_many_tokens():
+    _append([700, 2000], [700, 1500], 3, 1, 64, 16, torch.bfloat16, packed=True, tail=100)
+
+
+def test_append_layouts():
+    """Slices of one projection's output, keys and values in one buffer."""
+    D, P, lens = 64, 16, [40, 7]
+    table, pages = _table(lens, P)
+    both = torch.randn(pages, P, 2, 2, D, device="cuda")
+    keep = both.clone()
+    qkv = torch.randn(2, 5, 8 * D, device="cuda")
+    q, k, v = (t.unflatten(-1, (-1, D)) for t in qkv.split([4 * D, 2 * D, 2 * D], dim=-1))
+    want = ref.append(k, v, keep[:, :, 0], keep[:, :, 1], table, _lens(lens), rotary_frequencies(D), q)
+    got = PagedKVAppendOp(2, D, P, 4, D, dtype=torch.float32)(
+        k, v, both[:, :, 0], both[:, :, 1], table, _lens(lens), q)
+    assert_within(got, want[0], want[1])
+    assert_within(both[:, :, 0], want[2], want[3])
+    assert torch.equal(both[:, :, 1].cpu().double(), want[4])
+
+
+def test_append_nothing():
+    kc, vc = _cache(2, 16, 1, 64, torch.bfloat16), _cache(2, 16, 1, 64, torch.bfloat16)
+    keep = kc.clone(), vc.clone()
+    op = PagedKVAppendOp(1, 64, 16, 2, 64)
+    none = torch.empty(0, 1, 64, device="cuda", dtype=torch.bfloat16)
+    q = torch.empty(0, 2, 64, device="cuda", dtype=torch.bfloat16)
+    table = torch.zeros(0, 1, dtype=torch.int32, device="cuda")
+    assert op(none, none, kc, vc, table, _lens([]), q).shape == (0, 2, 64)
+    row = torch.randn(3, 1, 64, device="cuda").to(torch.bfloat16)
+    q = torch.randn(3, 2, 64, device="cuda").to(torch.bfloat16)
+    got = op(row, row, kc, vc, table, _lens([]), q, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert (got == 0).all()  # rows behind the last sequence
+    assert torch.equal(kc, keep[0]) and torch.equal(vc, keep[1])
+
+
+def test_append_refused_on_the_device_sets_the_flag():
+    """Nothing but the good tokens is written."""
+    kc, vc = _cache(4, 16, 1, 64, torch.float32), _cache(4, 16, 1, 64, torch.float32)
+    op = PagedKVAppendOp(1, 64, 16, dtype=torch.float32)
+    k, v = torch.randn(1, 20, 1, 64, device="cuda"), torch.randn(1, 20, 1, 64, device="cuda")
+    for table, n in (([0, 4], 20), ([0, -1], 20), ([0], 20)):
+        keep = kc.clone()
+        op(k, v, kc, vc, torch.tensor([table], dtype=torch.int32, device="cuda"), _lens([n]))
+        assert _flag() == 3
+        assert torch.equal(kc[0], k[0, :16]) and torch.equal(kc[1:], keep[1:])
+    op(k, v, kc, vc, torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), _lens([2**31 - 1]))
+    assert _flag() == 3
+    k, v = k[0], v[0]
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda")
+    for cu in ([0, 15, 10], [3, 5, 20], [0, 5, 21], [0, 2**31 - 1, -(2**31)]):
+        op(k, v, kc, vc, table, _lens([20, 20]), None, torch.tensor(cu, dtype=torch.int32, device="cuda"))
+        assert _flag() in (2, 3)

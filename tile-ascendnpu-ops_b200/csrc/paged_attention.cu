@@ -1,0 +1,628 @@
+// Attention of one new token of every sequence over a paged cache of keys and values.
+//
+//   o   = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q.k_j)      (per sequence b, query head h)
+//   lse = log2(sum_j w_j)
+//
+// over the tokens max(0, len_b - window) <= j < len_b; token j lies in slot j % P of page
+// page_table[b][j / P].  q (B, H, D); the caches (pages, P, Hkv, D) with any strides that are
+// multiples of 16 bytes; query head h reads key head h / (H / Hkv).  A sequence without a token
+// has o = 0 and lse = -inf.
+//
+// Every key and value is read once, 4 D e bytes for 4 D (H / Hkv) flops a token and key head: 1 to
+// 16 flops a byte, so HBM bounds it.  8 flops a byte at the memory's rate are 52 TFLOP/s, which
+// the fp32 pipes do not reach beside the conversions; the two products go to the tensor cores as
+// m16n8k16 (the query heads of a key head are the 16 rows; a 128-row tcgen05 tile would be
+// 7/8 padding and would take the scores through TMEM and back, for rates not needed here).
+//
+// The split.  The tokens of each (sequence, key head) are cut into units of 64, and all units of
+// the call in a row are shared out evenly: CTA c of n takes units [U c / n, U (c + 1) / n), whatever
+// the sequences' lengths are (they stay on the device).  An item (sequence and key head) whose
+// units lie in one CTA is finished there; of one that lies in several, each writes its sums,
+// and a second small kernel joins them in the order of the CTAs, so results repeat to the bit.
+// A CTA has at most two items it shares with others: its first and its last.
+//
+// In a CTA each of 4 warps takes 16 tokens of a unit on its own: it copies their keys and values
+// with 16-byte cp.async through its own ring of stages (no CTA barrier), multiplies, and keeps a
+// running maximum, sum and output of the softmax in registers (fp32).  The 4 warps join at an
+// item's end, through the stage just used; the copies of the next items' units are in flight
+// meanwhile.  Tokens outside the sequence are copied as zeros (size 0), never read: infinities
+// and NaN behind a sequence's end have no say.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "device_error.cuh"
+
+namespace tileops {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kWarpTokens = 16;
+constexpr int kUnit = kWarps * kWarpTokens;
+constexpr int kMaxCtas = 2 * 148;  // two on each of a B200's SMs
+constexpr float kNegInf = -__builtin_huge_valf();
+
+struct CacheStrides {
+  int64_t page, slot, head;
+};
+
+struct DecodeArgs {
+  const void *q, *k, *v;
+  const int32_t *table, *lens;
+  void* o;
+  float* lse;
+  float* partial;  // [CTA][2][row][D + 2]: sums, maximum, sum of weights
+  int2* shared;    // [CTA]: the item that it begins and others go on with (or -1), how many of them
+  int64_t q_b, q_h;
+  CacheStrides ks, vs;
+  int64_t table_stride, num_pages;
+  int batch, heads, heads_kv, group, dim, page_size, width, window, blocks;  // blocks of rows a key head
+  FastDivU32 div_page{1};
+  float scale;  // log2(e) times the scale
+  int* err;
+};
+
+// ---- the products ----
+__device__ __forceinline__ uint32_t smem_at(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void ldsm(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  const int bytes = there ? 16 : 0;  // 0: the 16 bytes are zeroed and src is not read
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+
+// Weights go to the second product in the inputs' type, half a step (2^-8 in bf16, 2^-11 in fp16) off
+// each; their sum takes them unrounded.  In fp16 they are held times 2^15 (the largest is 2^15), so that
+// weights down to 2^-29 of the largest keep all their bits.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ constexpr float kShift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
+
+// A sequence's tokens, and units of them.
+struct Span {
+  int begin, end, units;
+};
+__device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
+  const int64_t room = static_cast<int64_t>(a.width) * a.page_size;
+  int64_t len = a.lens[b];
+  if (len > room) {
+    report_device_error(a.err, kErrBadPage);
+    len = room;
+  }
+  Span s;
+  s.end = static_cast<int>(max(len, static_cast<int64_t>(0)));
+  s.begin = a.window > 0 ? max(s.end - a.window, 0) : 0;
+  s.units = (s.end - s.begin + kUnit - 1) / kUnit;
+  return s;
+}
+
+// Where in the row of all units a warp is: item (b, head), head counting blocks of rows of key
+// heads, and the unit of it.
+struct Cursor {
+  int b, head, unit;
+  Span span;
+  __device__ __forceinline__ void next(const DecodeArgs& a) {
+    if (++unit < span.units) return;
+    unit = 0;
+    if (++head < a.heads_kv * a.blocks) return;
+    head = 0;
+    do {
+      if (++b >= a.batch) return;
+      span = span_of(a, b);
+    } while (span.units == 0);
+  }
+};
+
+template <int DP, int MT>
+struct Layout {
+  static constexpr int kChunks = DP / 8;                       // 16-byte chunks of a row
+  static constexpr int kRow = (DP + 63) / 64 * 64;             // elements of a row in shared memory
+  static constexpr int kStages = DP <= 64 ? 6 : DP <= 128 ? 3 : DP <= 192 ? 4 : 3;
+  static constexpr int kCtasSm = DP <= 128 ? 2 : 1;
+  static constexpr int kTile = kWarpTokens * kRow;             // elements of a warp's keys (or values)
+  static constexpr int kRows = 16 * MT;
+  static constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * 2 * kTile * 2;
+  static constexpr size_t kQ = static_cast<size_t>(kRows) * kRow * 2;
+  static constexpr size_t kStats = static_cast<size_t>(kWarps) * kRows * 2 * 4;
+  static constexpr size_t kBytes = kRing + kQ + kStats;
+  // Chunk c of row r lies at chunk c ^ (r % 8): the 8 rows of a matrix in 8 different banks.
+  static __device__ __forceinline__ uint32_t at(int r, int c) {
+    return (r * (kRow / 8) + (c ^ (r & 7))) * 16;
+  }
+};
+
+template <typename T, int DP, int MT>
+__global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
+    paged_decode(const __grid_constant__ DecodeArgs a) {
+  using L = Layout<DP, MT>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int64_t sums[kWarps];
+  __shared__ Cursor first;
+  T* const q_smem = reinterpret_cast<T*>(smem + L::kRing);
+  float2* const stats = reinterpret_cast<float2*>(smem + L::kRing + L::kQ);  // [warp][row]
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int heads = a.heads_kv * a.blocks;
+
+  // ---- units of the call, and this CTA's ----
+  const int per = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = min(static_cast<int>(threadIdx.x) * per, a.batch), b1 = min(b0 + per, a.batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += span_of(a, b).units;
+  int64_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int64_t v = __shfl_up_sync(~0u, upto, d);
+    if (lane >= d) upto += v;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  int64_t total = 0, before = upto - mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  total *= heads;
+  const int64_t ctas = min(total, static_cast<int64_t>(gridDim.x));
+  const int64_t c = blockIdx.x;
+
+  // Sequences without a token.
+  for (int b = static_cast<int>(c); b < a.batch; b += gridDim.x) {
+    if (span_of(a, b).units) continue;
+    for (int64_t n = threadIdx.x; n < static_cast<int64_t>(a.heads) * a.dim; n += kThreads)
+      static_cast<T*>(a.o)[b * static_cast<int64_t>(a.heads) * a.dim + n] = Cvt<T>::from_f(0.0f);
+    for (int h = threadIdx.x; h < a.heads; h += kThreads)
+      a.lse[static_cast<int64_t>(b) * a.heads + h] = kNegInf;
+  }
+  if (c >= ctas) {
+    if (threadIdx.x == 0) a.shared[c] = make_int2(-1, 0);
+    return;
+  }
+  const int64_t u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
+  if (before * heads <= u0 && u0 < (before + mine) * heads) {
+    int64_t at = before * heads;
+    for (int b = b0; b < b1; ++b) {
+      const Span s = span_of(a, b);
+      const int64_t n = static_cast<int64_t>(s.units) * heads;
+      if (u0 < at + n) {
+        first.b = b;
+        first.head = static_cast<int>((u0 - at) / s.units);
+        first.unit = static_cast<int>((u0 - at) % s.units);
+        first.span = s;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  Cursor put = first, get = first;  // of the copies and of the products
+  int64_t to_put = u1 - u0, to_get = u1 - u0;
+
+  // ---- copies ----
+  const uint32_t ring = smem_at(smem) + warp * (L::kStages * 2 * L::kTile * 2);
+  auto page_of = [&]() {  // this lane's token of the unit at `put`: its page
+    const int t = put.span.begin + put.unit * kUnit + warp * kWarpTokens + lane;
+    int page = -1;
+    if (to_put > 0 && lane < kWarpTokens && t < put.span.end) {
+      page = a.table[put.b * a.table_stride + a.div_page.div(t)];
+      if (page < 0 || page >= a.num_pages) {
+        report_device_error(a.err, kErrBadPage);
+        page = -1;
+      }
+    }
+    return page;
+  };
+  int page = page_of();
+  auto issue = [&](int stage) {
+    if (to_put > 0) {
+      const int t = put.span.begin + put.unit * kUnit + warp * kWarpTokens + lane;
+      const int slot = t - static_cast<int>(a.div_page.div(max(t, 0))) * a.page_size;
+      const int head = put.head / a.blocks;
+      const T* k = static_cast<const T*>(a.k) + head * a.ks.head;
+      const T* v = static_cast<const T*>(a.v) + head * a.vs.head;
+      int64_t k_at = 0, v_at = 0;
+      if (page >= 0) {
+        k_at = page * a.ks.page + slot * a.ks.slot;
+        v_at = page * a.vs.page + slot * a.vs.slot;
+      }
+      const uint32_t to = ring + stage * (2 * L::kTile * 2);
+#pragma unroll
+      for (int i = 0; i < kWarpTokens * L::kChunks / 32; ++i) {
+        const int row = (i * 32 + lane) / L::kChunks, chunk = (i * 32 + lane) % L::kChunks;
+        const bool there = __shfl_sync(~0u, page, row) >= 0 && chunk * 8 < a.dim;
+        const int64_t ka = __shfl_sync(~0u, k_at, row), va = __shfl_sync(~0u, v_at, row);
+        const int64_t col = there ? chunk * 8 : 0;
+        copy16(to + L::at(row, chunk), k + ka + col, there);
+        copy16(to + L::kTile * 2 + L::at(row, chunk), v + va + col, there);
+      }
+      put.next(a);
+      --to_put;
+      page = page_of();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int s = 0; s < L::kStages; ++s) issue(s);
+
+  // ---- products ----
+  // top: the exponent that a row's weights are relative to, its largest score (in fp16 less 15).
+  float out[MT][DP / 8][4], top[MT][2], sum[MT][2];
+  auto reset = [&]() {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[m][n][e] = 0.0f;
+      top[m][0] = top[m][1] = kNegInf;
+      sum[m][0] = sum[m][1] = 0.0f;
+    }
+  };
+  auto load_q = [&]() {  // the rows of the item at `get`, zeros behind them
+    const int h0 = (get.head / a.blocks) * a.group + (get.head % a.blocks) * L::kRows;
+    const int rows = min(L::kRows, a.group - (get.head % a.blocks) * L::kRows);
+    for (int n = threadIdx.x; n < L::kRows * L::kChunks; n += kThreads) {
+      const int r = n / L::kChunks, ch = n % L::kChunks;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (r < rows && ch * 8 < a.dim)
+        w = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + get.b * a.q_b +
+                                            (h0 + r) * a.q_h + ch * 8);
+      *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(q_smem) + L::at(r, ch)) = w;
+    }
+  };
+  load_q();
+  reset();
+  __syncthreads();
+  bool began = get.unit == 0;  // the item at `get` began in this CTA
+  int stage = 0;
+  const uint32_t q_at = smem_at(q_smem);
+#pragma unroll 1
+  while (true) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
+    __syncwarp();
+    const uint32_t keys = ring + stage * (2 * L::kTile * 2), values = keys + L::kTile * 2;
+    const int t0 = get.span.begin + get.unit * kUnit + warp * kWarpTokens;
+    if (t0 < get.span.end) {
+      float s[MT][2][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[m][n][e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        uint32_t kb[4];
+        ldsm(keys + L::at((lane & 7) + ((lane >> 4) << 3), k * 2 + ((lane >> 3) & 1)), kb);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          uint32_t qa[4];
+          ldsm(q_at + L::at(m * 16 + (lane & 15), k * 2 + (lane >> 4)), qa);
+          mma<T>(s[m][0], qa, kb[0], kb[1]);
+          mma<T>(s[m][1], qa, kb[2], kb[3]);
+        }
+      }
+      uint32_t w[MT][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = t0 + n * 8 + (lane & 3) * 2 + (e & 1);
+            s[m][n][e] = t < get.span.end ? s[m][n][e] * a.scale : kNegInf;
+          }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {  // rows lane / 4 and lane / 4 + 8
+          float (&x)[4] = s[m][0], (&y)[4] = s[m][1];
+          float high = fmaxf(fmaxf(x[2 * r], x[2 * r + 1]), fmaxf(y[2 * r], y[2 * r + 1]));
+          high = fmaxf(high, __shfl_xor_sync(~0u, high, 1));
+          high = fmaxf(high, __shfl_xor_sync(~0u, high, 2));
+          const float top_new = fmaxf(high - kShift<T>, top[m][r]);
+          // A row of nothing but -inf so far: exp2(-inf - 0) = 0, not exp2(-inf + inf).
+          const float base = top_new == kNegInf ? 0.0f : top_new;
+          const float fade = ex2_approx_f(top[m][r] - base);
+          top[m][r] = top_new;
+          x[2 * r] = ex2_approx_f(x[2 * r] - base);
+          x[2 * r + 1] = ex2_approx_f(x[2 * r + 1] - base);
+          y[2 * r] = ex2_approx_f(y[2 * r] - base);
+          y[2 * r + 1] = ex2_approx_f(y[2 * r + 1] - base);
+          sum[m][r] = sum[m][r] * fade + ((x[2 * r] + x[2 * r + 1]) + (y[2 * r] + y[2 * r + 1]));
+          w[m][r] = pack2<T>(x[2 * r], x[2 * r + 1]);
+          w[m][2 + r] = pack2<T>(y[2 * r], y[2 * r + 1]);
+          if (__any_sync(~0u, fade != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n) {
+              out[m][n][2 * r] *= fade;
+              out[m][n][2 * r + 1] *= fade;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < DP / 16; ++n) {
+        uint32_t vb[4];
+        ldsm_t(values + L::at(lane & 15, n * 2 + (lane >> 4)), vb);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma<T>(out[m][2 * n], w[m], vb[0], vb[1]);
+          mma<T>(out[m][2 * n + 1], w[m], vb[2], vb[3]);
+        }
+      }
+    }
+    --to_get;
+    const bool ended = get.unit + 1 == get.span.units;
+    if (ended || to_get == 0) {
+      // ---- the warps' sums of the item, joined through the stage just used ----
+      const int block = get.head % a.blocks;
+      const int h0 = (get.head / a.blocks) * a.group + block * L::kRows;
+      const int rows = min(L::kRows, a.group - block * L::kRows);
+      const bool whole = began && ended;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float v = sum[m][r];
+          v += __shfl_xor_sync(~0u, v, 1);
+          v += __shfl_xor_sync(~0u, v, 2);
+          if ((lane & 3) == 0)
+            stats[warp * L::kRows + m * 16 + r * 8 + lane / 4] = make_float2(top[m][r], v);
+        }
+      unsigned char* const own = smem + (warp * L::kStages + stage) * (2 * L::kTile * 2);
+      constexpr int kPad = L::kRow;  // floats of a row there: 16 rows fill the stage
+#pragma unroll 1
+      for (int m = 0; m < MT; ++m) {
+        __syncwarp();
+        // 8-column group n of row r at group (n + r) % groups: the 8 rows in different banks.
+#pragma unroll
+        for (int mm = 0; mm < MT; ++mm) {
+          if (mm != m) continue;
+#pragma unroll
+          for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int row = r * 8 + lane / 4;
+              const int col = (n + lane / 4) % (DP / 8) * 8 + (lane & 3) * 2;
+              *reinterpret_cast<float2*>(own + (row * kPad + col) * 4) =
+                  make_float2(out[mm][n][2 * r], out[mm][n][2 * r + 1]);
+            }
+        }
+        __syncthreads();
+        for (int n = threadIdx.x; n < 16 * DP; n += kThreads) {
+          const int r = n / DP, d = n % DP, row = m * 16 + r;
+          if (row >= rows || d >= a.dim) continue;
+          const int col = (d / 8 + (r & 7)) % (DP / 8) * 8 + d % 8;
+          float high = kNegInf;
+#pragma unroll
+          for (int x = 0; x < kWarps; ++x) high = fmaxf(high, stats[x * L::kRows + row].x);
+          const float base = high == kNegInf ? 0.0f : high;
+          float all = 0.0f, v = 0.0f;
+#pragma unroll
+          for (int x = 0; x < kWarps; ++x) {
+            const float2 st = stats[x * L::kRows + row];
+            const float f = ex2_approx_f(st.x - base);
+            all += f * st.y;
+            v += f * *reinterpret_cast<const float*>(
+                         smem + (x * L::kStages + stage) * (2 * L::kTile * 2) + (r * kPad + col) * 4);
+          }
+          if (whole) {
+            const int64_t at = static_cast<int64_t>(get.b) * a.heads + h0 + row;
+            static_cast<T*>(a.o)[at * a.dim + d] = Cvt<T>::from_f(all == 0.0f ? 0.0f : v / all);
+            if (d == 0) a.lse[at] = base + log2f(all);
+          } else {
+            float* to = a.partial + ((c * 2 + (began ? 1 : 0)) * L::kRows + row) * (a.dim + 2);
+            to[d] = v;
+            if (d == 0) {
+              to[a.dim] = high;
+              to[a.dim + 1] = all;
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if (to_get == 0) {
+        if (threadIdx.x == 0) {
+          int2 told = make_int2(-1, 0);
+          if (began && !ended) {
+            // The item's last unit, and the last CTA whose units begin at or before it.
+            const int64_t last = u1 - 1 + (get.span.units - 1 - get.unit);
+            told = make_int2(get.b * heads + get.head, static_cast<int>(((last + 1) * ctas - 1) / total - c));
+          }
+          a.shared[c] = told;
+        }
+        break;
+      }
+      get.next(a);
+      began = true;
+      load_q();
+      reset();
+      __syncthreads();
+    } else {
+      get.next(a);
+      __syncwarp();
+    }
+    issue(stage);
+    stage = stage + 1 == L::kStages ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// One CTA an item that several CTAs share, found by the CTA that begins it: their sums, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_join(const __grid_constant__ DecodeArgs a, int rows_max) {
+  const int64_t c = blockIdx.x;
+  const int2 told = a.shared[c];
+  if (told.x < 0) return;
+  const int heads = a.heads_kv * a.blocks, b = told.x / heads, head = told.x % heads;
+  const int block = head % a.blocks;
+  const int h0 = (head / a.blocks) * a.group + block * rows_max;
+  const int rows = min(rows_max, a.group - block * rows_max);
+  const int64_t step = static_cast<int64_t>(rows_max) * (a.dim + 2);
+  for (int n = threadIdx.x; n < rows * a.dim; n += blockDim.x) {
+    const int row = n / a.dim, d = n % a.dim;
+    const float* p = a.partial + (c * 2 + 1) * step + row * (a.dim + 2);
+    const float* rest = a.partial + (c + 1) * 2 * step + row * (a.dim + 2);
+    float high = p[a.dim];
+    for (int x = 0; x < told.y; ++x) high = fmaxf(high, rest[2 * x * step + a.dim]);
+    const float base = high == kNegInf ? 0.0f : high;
+    float f = ex2_approx_f(p[a.dim] - base);
+    float all = f * p[a.dim + 1], v = f * p[d];
+    for (int x = 0; x < told.y; ++x) {
+      const float* r = rest + 2 * x * step;
+      f = ex2_approx_f(r[a.dim] - base);
+      all += f * r[a.dim + 1];
+      v += f * r[d];
+    }
+    const int64_t at = static_cast<int64_t>(b) * a.heads + h0 + row;
+    static_cast<T*>(a.o)[at * a.dim + d] = Cvt<T>::from_f(all == 0.0f ? 0.0f : v / all);
+    if (d == 0) a.lse[at] = base + log2f(all);
+  }
+}
+
+int padded_dim(int64_t dim) {
+  return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
+}
+int rows_of(int64_t group, int dp) { return group > 16 && dp <= 128 ? 32 : 16; }
+bool bad_sizes(int64_t batch, int64_t heads, int64_t heads_kv, int64_t dim) {
+  return batch < 0 || batch > 0x7fffff || heads < 1 || heads > 4096 || heads_kv < 1 ||
+         heads % heads_kv != 0 || dim < 8 || dim > 256 || dim % 8 != 0;
+}
+
+template <typename T, int DP, int MT>
+int launch_tile(const DecodeArgs& a, int64_t grid, cudaStream_t s) {
+  using L = Layout<DP, MT>;
+  if (cudaFuncSetAttribute(paged_decode<T, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(L::kBytes)) != cudaSuccess)
+    return TILEOPS_ELAUNCH;
+  grid = std::min<int64_t>({grid, static_cast<int64_t>(sm_count()) * L::kCtasSm, kMaxCtas});
+  paged_decode<T, DP, MT><<<static_cast<unsigned>(grid), kThreads, L::kBytes, s>>>(a);
+  paged_join<T><<<static_cast<unsigned>(grid), 256, 0, s>>>(a, L::kRows);
+  return launch_status();
+}
+
+template <typename T>
+int launch_type(const DecodeArgs& a, int64_t grid, cudaStream_t s) {
+  const int dp = padded_dim(a.dim);
+  const bool wide = rows_of(a.group, dp) == 32;
+  switch (dp) {
+    case 64: return wide ? launch_tile<T, 64, 2>(a, grid, s) : launch_tile<T, 64, 1>(a, grid, s);
+    case 96: return wide ? launch_tile<T, 96, 2>(a, grid, s) : launch_tile<T, 96, 1>(a, grid, s);
+    case 128: return wide ? launch_tile<T, 128, 2>(a, grid, s) : launch_tile<T, 128, 1>(a, grid, s);
+    case 192: return launch_tile<T, 192, 1>(a, grid, s);
+    default: return launch_tile<T, 256, 1>(a, grid, s);
+  }
+}
+
+constexpr int64_t kSharedBytes = kMaxCtas * sizeof(int2);
+
+}  // namespace
+}  // namespace tileops
+
+using namespace tileops;
+
+extern "C" int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t heads_kv,
+                                                        int64_t dim) {
+  if (bad_sizes(1, heads, heads_kv, dim)) return -1;
+  const int rows = rows_of(heads / heads_kv, padded_dim(dim));
+  return kSharedBytes + static_cast<int64_t>(kMaxCtas) * 2 * rows * (dim + 2) * 4;
+}
+
+extern "C" int tileops_paged_decode_fwd(
+    const void* q, const void* k_cache, const void* v_cache, const int32_t* page_table,
+    const int32_t* seq_lens, void* o, float* lse, void* workspace, int64_t batch, int64_t heads,
+    int64_t heads_kv, int64_t dim, int64_t num_pages, int64_t page_size, int64_t table_width,
+    int64_t table_stride, const int64_t* strides8, int64_t window, double scale, int dtype,
+    void* stream) {
+  if (bad_sizes(batch, heads, heads_kv, dim) || num_pages < 0 || num_pages > 0x7fffffffLL ||
+      page_size < 1 || page_size > 0x7fffffffLL || table_width < 0 || table_width > 0x7fffffffLL ||
+      page_size * table_width > 0x7fffffffLL - kUnit || window < 0 || window > 0x7fffffffLL)
+    return TILEOPS_EBADSHAPE;
+  if (dtype != TILEOPS_DT_F16 && dtype != TILEOPS_DT_BF16) return TILEOPS_EBADDTYPE;
+  if (batch == 0) return TILEOPS_OK;
+  if (!q || !k_cache || !v_cache || !seq_lens || !o || !lse || !workspace || !strides8 ||
+      (table_width && !page_table))
+    return TILEOPS_EINVAL;
+  for (int n = 0; n < 8; ++n)
+    if (strides8[n] % 8 != 0) return TILEOPS_EALIGN;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
+    return TILEOPS_EALIGN;
+  DecodeArgs a{};
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.table = page_table;
+  a.lens = seq_lens;
+  a.o = o;
+  a.lse = lse;
+  a.shared = static_cast<int2*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kSharedBytes);
+  a.q_b = strides8[0];
+  a.q_h = strides8[1];
+  a.ks = {strides8[2], strides8[3], strides8[4]};
+  a.vs = {strides8[5], strides8[6], strides8[7]};
+  a.table_stride = table_stride;
+  a.num_pages = num_pages;
+  a.batch = static_cast<int>(batch);
+  a.heads = static_cast<int>(heads);
+  a.heads_kv = static_cast<int>(heads_kv);
+  a.group = static_cast<int>(heads / heads_kv);
+  a.dim = static_cast<int>(dim);
+  a.page_size = static_cast<int>(page_size);
+  a.width = static_cast<int>(table_width);
+  a.window = static_cast<int>(window);
+  const int rows = rows_of(a.group, padded_dim(dim));
+  a.blocks = (a.group + rows - 1) / rows;
+  a.div_page = FastDivU32(static_cast<uint32_t>(page_size));
+  a.scale = static_cast<float>(scale * 1.4426950408889634);
+  a.err = device_error_ptr();
+  // No more CTAs than there can be units.
+  const int64_t room = std::min<int64_t>(page_size * table_width,
+                                         window ? window : page_size * table_width);
+  const int64_t units = std::max<int64_t>(1, (room + kUnit - 1) / kUnit);
+  const int64_t grid = std::min<int64_t>(units * batch * heads_kv * a.blocks, 1 << 20);
+  cudaStream_t s = as_stream(stream);
+  return dtype == TILEOPS_DT_F16 ? launch_type<__half>(a, grid, s)
+                                 : launch_type<__nv_bfloat16>(a, grid, s);
+}

@@ -90,6 +90,10 @@ _SIGNATURES: dict[str, list] = {
     "tileops_glr_bwd": [_p] * 9 + [_i64] + [_p] * 6 + [_i64] * 11 + [_d, _i, _p],
     "tileops_glr_decode_fwd": [_p] * 7 + [_i64] * 5 + [_d, _i, _p],
     "tileops_ssd_chunk_scan_fwd": [_p] * 7 + [_i64] * 7 + [_i, _p],
+    "tileops_rotary": [_p] * 6 + [_i64] * 6 + [_p, _i64] + [_i] * 3 + [_d, _i, _p],
+    "tileops_paged_kv_append": [_p] * 10 + [_i64] * 10 + [_p, _i, _d, _i, _p],
+    "tileops_paged_decode_workspace_bytes": [_i64] * 3,
+    "tileops_paged_decode_fwd": [_p] * 8 + [_i64] * 8 + [_p, _i64, _d, _i, _p],
     "tileops_device_error_flag": [_p, _i],
     "tileops_selftest_wait_timeout": [_p, _i64, _i64, _p, _p],
     "tileops_abi_version": [],
@@ -132,6 +136,7 @@ def lib() -> ctypes.CDLL:
                     "tileops_gdn_varlen_workspace_bytes": ctypes.c_int64,
                     "tileops_glr_bwd_workspace_bytes": ctypes.c_int64,
                     "tileops_sandwich_norm_bwd_workspace_bytes": ctypes.c_int64,
+                    "tileops_paged_decode_workspace_bytes": ctypes.c_int64,
                 }.get(name, ctypes.c_int)
             _lib = handle
     return _lib
