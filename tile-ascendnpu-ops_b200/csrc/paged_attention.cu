@@ -52,8 +52,9 @@ struct DecodeArgs {
   const int32_t *table, *lens;
   void* o;
   float* lse;
-  float* partial;  // [CTA][2][row][D + 2]: sums, maximum, sum of weights
-  int2* shared;    // [CTA]: the item that it begins and others go on with (or -1), how many of them
+  int2* shared;     // [CTA]: the item that it begins and others go on with (or -1), how many of them
+  float2* stats;    // [CTA][2][row]: exponent the sums are relative to, sum of weights
+  float* partial;   // [CTA][2][row][D]: weighted sums
   int64_t q_b, q_h;
   CacheStrides ks, vs;
   int64_t table_stride, num_pages;
@@ -155,6 +156,17 @@ struct Cursor {
   }
 };
 
+// Four channels of a finished row.
+template <typename T>
+__device__ __forceinline__ void store_row(T* to, float4 v, float all) {
+  const float r = all == 0.0f ? 0.0f : 1.0f / all;
+  uint2 w;
+  if (all == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  w.x = pack2<T>(v.x * r, v.y * r);
+  w.y = pack2<T>(v.z * r, v.w * r);
+  *reinterpret_cast<uint2*>(to) = w;
+}
+
 template <int DP, int MT>
 struct Layout {
   static constexpr int kChunks = DP / 8;                       // 16-byte chunks of a row
@@ -184,6 +196,7 @@ __global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
   float2* const stats = reinterpret_cast<float2*>(smem + L::kRing + L::kQ);  // [warp][row]
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int heads = a.heads_kv * a.blocks;
+  asm volatile("griddepcontrol.launch_dependents;");
 
   // ---- units of the call, and this CTA's ----
   const int per = (a.batch + kThreads - 1) / kThreads;
@@ -300,19 +313,31 @@ __global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
       sum[m][0] = sum[m][1] = 0.0f;
     }
   };
-  auto load_q = [&]() {  // the rows of the item at `get`, zeros behind them
-    const int h0 = (get.head / a.blocks) * a.group + (get.head % a.blocks) * L::kRows;
-    const int rows = min(L::kRows, a.group - (get.head % a.blocks) * L::kRows);
-    for (int n = threadIdx.x; n < L::kRows * L::kChunks; n += kThreads) {
-      const int r = n / L::kChunks, ch = n % L::kChunks;
-      uint4 w = make_uint4(0, 0, 0, 0);
+  // The rows of an item, zeros behind them: fetched while the item before is joined.
+  constexpr int kQChunks = (L::kRows * L::kChunks + kThreads - 1) / kThreads;
+  uint4 q_next[kQChunks];
+  auto fetch_q = [&](const Cursor& at) {
+    const int h0 = (at.head / a.blocks) * a.group + (at.head % a.blocks) * L::kRows;
+    const int rows = min(L::kRows, a.group - (at.head % a.blocks) * L::kRows);
+#pragma unroll
+    for (int i = 0; i < kQChunks; ++i) {
+      const int n = i * kThreads + threadIdx.x, r = n / L::kChunks, ch = n % L::kChunks;
+      q_next[i] = make_uint4(0, 0, 0, 0);
       if (r < rows && ch * 8 < a.dim)
-        w = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + get.b * a.q_b +
-                                            (h0 + r) * a.q_h + ch * 8);
-      *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(q_smem) + L::at(r, ch)) = w;
+        q_next[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at.b * a.q_b +
+                                                    (h0 + r) * a.q_h + ch * 8);
     }
   };
-  load_q();
+  auto store_q = [&]() {
+#pragma unroll
+    for (int i = 0; i < kQChunks; ++i) {
+      const int n = i * kThreads + threadIdx.x, r = n / L::kChunks, ch = n % L::kChunks;
+      if (r < L::kRows)
+        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(q_smem) + L::at(r, ch)) = q_next[i];
+    }
+  };
+  fetch_q(get);
+  store_q();
   reset();
   __syncthreads();
   bool began = get.unit == 0;  // the item at `get` began in this CTA
@@ -396,10 +421,15 @@ __global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
     const bool ended = get.unit + 1 == get.span.units;
     if (ended || to_get == 0) {
       // ---- the warps' sums of the item, joined through the stage just used ----
-      const int block = get.head % a.blocks;
-      const int h0 = (get.head / a.blocks) * a.group + block * L::kRows;
-      const int rows = min(L::kRows, a.group - block * L::kRows);
+      const Cursor item = get;
       const bool whole = began && ended;
+      if (to_get > 0) {
+        get.next(a);
+        fetch_q(get);
+      }
+      const int block = item.head % a.blocks;
+      const int h0 = (item.head / a.blocks) * a.group + block * L::kRows;
+      const int rows = min(L::kRows, a.group - block * L::kRows);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -412,52 +442,56 @@ __global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
         }
       unsigned char* const own = smem + (warp * L::kStages + stage) * (2 * L::kTile * 2);
       constexpr int kPad = L::kRow;  // floats of a row there: 16 rows fill the stage
-#pragma unroll 1
+#pragma unroll
       for (int m = 0; m < MT; ++m) {
         __syncwarp();
         // 8-column group n of row r at group (n + r) % groups: the 8 rows in different banks.
 #pragma unroll
-        for (int mm = 0; mm < MT; ++mm) {
-          if (mm != m) continue;
+        for (int r = 0; r < 2; ++r) {
+          if (m * 16 + r * 8 >= rows) continue;
 #pragma unroll
-          for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int row = r * 8 + lane / 4;
-              const int col = (n + lane / 4) % (DP / 8) * 8 + (lane & 3) * 2;
-              *reinterpret_cast<float2*>(own + (row * kPad + col) * 4) =
-                  make_float2(out[mm][n][2 * r], out[mm][n][2 * r + 1]);
-            }
+          for (int n = 0; n < DP / 8; ++n) {
+            const int row = r * 8 + lane / 4;
+            const int col = (n + lane / 4) % (DP / 8) * 8 + (lane & 3) * 2;
+            *reinterpret_cast<float2*>(own + (row * kPad + col) * 4) =
+                make_float2(out[m][n][2 * r], out[m][n][2 * r + 1]);
+          }
         }
         __syncthreads();
-        for (int n = threadIdx.x; n < 16 * DP; n += kThreads) {
-          const int r = n / DP, d = n % DP, row = m * 16 + r;
-          if (row >= rows || d >= a.dim) continue;
+        if (m == 0) store_q();
+        for (int n = threadIdx.x; n < min(16, rows - m * 16) * (DP / 4); n += kThreads) {
+          const int r = n / (DP / 4), d = n % (DP / 4) * 4, row = m * 16 + r;
+          if (d >= a.dim) continue;
           const int col = (d / 8 + (r & 7)) % (DP / 8) * 8 + d % 8;
+          float2 st[kWarps];
           float high = kNegInf;
 #pragma unroll
-          for (int x = 0; x < kWarps; ++x) high = fmaxf(high, stats[x * L::kRows + row].x);
+          for (int x = 0; x < kWarps; ++x) {
+            st[x] = stats[x * L::kRows + row];
+            high = fmaxf(high, st[x].x);
+          }
           const float base = high == kNegInf ? 0.0f : high;
-          float all = 0.0f, v = 0.0f;
+          float all = 0.0f;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
           for (int x = 0; x < kWarps; ++x) {
-            const float2 st = stats[x * L::kRows + row];
-            const float f = ex2_approx_f(st.x - base);
-            all += f * st.y;
-            v += f * *reinterpret_cast<const float*>(
-                         smem + (x * L::kStages + stage) * (2 * L::kTile * 2) + (r * kPad + col) * 4);
+            const float f = ex2_approx_f(st[x].x - base);
+            const float4 p = *reinterpret_cast<const float4*>(
+                smem + (x * L::kStages + stage) * (2 * L::kTile * 2) + (r * kPad + col) * 4);
+            all += f * st[x].y;
+            v.x += f * p.x;
+            v.y += f * p.y;
+            v.z += f * p.z;
+            v.w += f * p.w;
           }
           if (whole) {
-            const int64_t at = static_cast<int64_t>(get.b) * a.heads + h0 + row;
-            static_cast<T*>(a.o)[at * a.dim + d] = Cvt<T>::from_f(all == 0.0f ? 0.0f : v / all);
+            const int64_t at = static_cast<int64_t>(item.b) * a.heads + h0 + row;
+            store_row(static_cast<T*>(a.o) + at * a.dim + d, v, all);
             if (d == 0) a.lse[at] = base + log2f(all);
           } else {
-            float* to = a.partial + ((c * 2 + (began ? 1 : 0)) * L::kRows + row) * (a.dim + 2);
-            to[d] = v;
-            if (d == 0) {
-              to[a.dim] = high;
-              to[a.dim + 1] = all;
-            }
+            const int64_t at = (c * 2 + (began ? 1 : 0)) * L::kRows + row;
+            *reinterpret_cast<float4*>(a.partial + at * a.dim + d) = v;
+            if (d == 0) a.stats[at] = make_float2(high, all);
           }
         }
         __syncthreads();
@@ -467,18 +501,16 @@ __global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
           int2 told = make_int2(-1, 0);
           if (began && !ended) {
             // The item's last unit, and the last CTA whose units begin at or before it.
-            const int64_t last = u1 - 1 + (get.span.units - 1 - get.unit);
-            told = make_int2(get.b * heads + get.head, static_cast<int>(((last + 1) * ctas - 1) / total - c));
+            const int64_t last = u1 - 1 + (item.span.units - 1 - item.unit);
+            told = make_int2(item.b * heads + item.head,
+                             static_cast<int>(((last + 1) * ctas - 1) / total - c));
           }
           a.shared[c] = told;
         }
         break;
       }
-      get.next(a);
       began = true;
-      load_q();
       reset();
-      __syncthreads();
     } else {
       get.next(a);
       __syncwarp();
@@ -490,34 +522,95 @@ __global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
 }
 
 // One CTA an item that several CTAs share, found by the CTA that begins it: their sums, in order.
+// A team of warps takes a row: each lane holds the factors of up to kParts / 32 CTAs' sums and four or
+// eight channels; the warps of a team share out the CTAs, and their sums meet in shared memory.
+constexpr int kJoinWarps = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) paged_join(const __grid_constant__ DecodeArgs a, int rows_max) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join(const __grid_constant__ DecodeArgs a,
+                                                              int rows_max) {
+  constexpr int kParts = (kMaxCtas + 31) / 32;
+  __shared__ float4 met[kJoinWarps][64];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t c = blockIdx.x;
   const int2 told = a.shared[c];
   if (told.x < 0) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int heads = a.heads_kv * a.blocks, b = told.x / heads, head = told.x % heads;
   const int block = head % a.blocks;
   const int h0 = (head / a.blocks) * a.group + block * rows_max;
   const int rows = min(rows_max, a.group - block * rows_max);
-  const int64_t step = static_cast<int64_t>(rows_max) * (a.dim + 2);
-  for (int n = threadIdx.x; n < rows * a.dim; n += blockDim.x) {
-    const int row = n / a.dim, d = n % a.dim;
-    const float* p = a.partial + (c * 2 + 1) * step + row * (a.dim + 2);
-    const float* rest = a.partial + (c + 1) * 2 * step + row * (a.dim + 2);
-    float high = p[a.dim];
-    for (int x = 0; x < told.y; ++x) high = fmaxf(high, rest[2 * x * step + a.dim]);
-    const float base = high == kNegInf ? 0.0f : high;
-    float f = ex2_approx_f(p[a.dim] - base);
-    float all = f * p[a.dim + 1], v = f * p[d];
-    for (int x = 0; x < told.y; ++x) {
-      const float* r = rest + 2 * x * step;
-      f = ex2_approx_f(r[a.dim] - base);
-      all += f * r[a.dim + 1];
-      v += f * r[d];
+  int team = 1;  // warps of a row
+  while (team * 2 * rows <= kJoinWarps) team *= 2;
+  const int parts = told.y + 1;
+  // Sums of part x: slot 1 of this CTA, then slot 0 of those behind it.
+  auto slot = [&](int x, int row) { return ((c + x) * 2 + (x == 0)) * rows_max + row; };
+#pragma unroll 1
+  for (int row0 = 0; row0 < rows; row0 += kJoinWarps / team) {
+    const int row = row0 + warp / team, first = warp % team;
+    float f[kParts], all = 0.0f, base = 0.0f;
+    float4 v[2];
+    v[0] = v[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (row < rows) {
+      float2 st[kParts];
+      float high = kNegInf;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        const int x = j * 32 + lane;
+        st[j] = x < parts ? a.stats[slot(x, row)] : make_float2(kNegInf, 0.0f);
+        high = fmaxf(high, st[j].x);
+      }
+#pragma unroll
+      for (int d = 16; d; d /= 2) high = fmaxf(high, __shfl_xor_sync(~0u, high, d));
+      base = high == kNegInf ? 0.0f : high;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        f[j] = ex2_approx_f(st[j].x - base);
+        all += f[j] * st[j].y;
+      }
+#pragma unroll
+      for (int d = 16; d; d /= 2) all += __shfl_xor_sync(~0u, all, d);
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        if (j * 32 >= parts) break;
+#pragma unroll 4
+        for (int x = first; x < 32; x += team) {
+          const float fx = __shfl_sync(~0u, f[j], x);
+          if (j * 32 + x >= parts) break;
+          const float* p = a.partial + slot(j * 32 + x, row) * a.dim;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int d = (i * 32 + lane) * 4;
+            if (d >= a.dim) continue;
+            const float4 w = *reinterpret_cast<const float4*>(p + d);
+            v[i].x += fx * w.x;
+            v[i].y += fx * w.y;
+            v[i].z += fx * w.z;
+            v[i].w += fx * w.w;
+          }
+        }
+      }
     }
-    const int64_t at = static_cast<int64_t>(b) * a.heads + h0 + row;
-    static_cast<T*>(a.o)[at * a.dim + d] = Cvt<T>::from_f(all == 0.0f ? 0.0f : v / all);
-    if (d == 0) a.lse[at] = base + log2f(all);
+    met[warp][lane] = v[0];
+    met[warp][32 + lane] = v[1];
+    __syncthreads();
+    if (row < rows && first == 0) {
+      const int64_t at = static_cast<int64_t>(b) * a.heads + h0 + row;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int d = (i * 32 + lane) * 4;
+        if (d >= a.dim) continue;
+        for (int w = 1; w < team; ++w) {
+          const float4 o = met[warp + w][i * 32 + lane];
+          v[i].x += o.x;
+          v[i].y += o.y;
+          v[i].z += o.z;
+          v[i].w += o.w;
+        }
+        store_row(static_cast<T*>(a.o) + at * a.dim + d, v[i], all);
+      }
+      if (lane == 0) a.lse[at] = base + log2f(all);
+    }
+    __syncthreads();
   }
 }
 
@@ -538,7 +631,19 @@ int launch_tile(const DecodeArgs& a, int64_t grid, cudaStream_t s) {
     return TILEOPS_ELAUNCH;
   grid = std::min<int64_t>({grid, static_cast<int64_t>(sm_count()) * L::kCtasSm, kMaxCtas});
   paged_decode<T, DP, MT><<<static_cast<unsigned>(grid), kThreads, L::kBytes, s>>>(a);
-  paged_join<T><<<static_cast<unsigned>(grid), 256, 0, s>>>(a, L::kRows);
+  if (int status = launch_status()) return status;
+  // The join's CTAs may be placed while the first kernel's last ones run; they wait for its end.
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(grid));
+  config.blockDim = dim3(kJoinWarps * 32);
+  config.stream = s;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, paged_join<T>, a, static_cast<int>(L::kRows)) != cudaSuccess)
+    return TILEOPS_ELAUNCH;
   return launch_status();
 }
 
@@ -566,7 +671,7 @@ extern "C" int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t h
                                                         int64_t dim) {
   if (bad_sizes(1, heads, heads_kv, dim)) return -1;
   const int rows = rows_of(heads / heads_kv, padded_dim(dim));
-  return kSharedBytes + static_cast<int64_t>(kMaxCtas) * 2 * rows * (dim + 2) * 4;
+  return kSharedBytes + static_cast<int64_t>(kMaxCtas) * 2 * rows * (dim + 2) * 4;  // stats, sums
 }
 
 extern "C" int tileops_paged_decode_fwd(
@@ -597,7 +702,6 @@ extern "C" int tileops_paged_decode_fwd(
   a.o = o;
   a.lse = lse;
   a.shared = static_cast<int2*>(workspace);
-  a.partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kSharedBytes);
   a.q_b = strides8[0];
   a.q_h = strides8[1];
   a.ks = {strides8[2], strides8[3], strides8[4]};
@@ -614,6 +718,8 @@ extern "C" int tileops_paged_decode_fwd(
   a.window = static_cast<int>(window);
   const int rows = rows_of(a.group, padded_dim(dim));
   a.blocks = (a.group + rows - 1) / rows;
+  a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + kSharedBytes);
+  a.partial = reinterpret_cast<float*>(a.stats + static_cast<int64_t>(kMaxCtas) * 2 * rows);
   a.div_page = FastDivU32(static_cast<uint32_t>(page_size));
   a.scale = static_cast<float>(scale * 1.4426950408889634);
   a.err = device_error_ptr();
