@@ -15,11 +15,13 @@
 // 7/8 padding and would take the scores through TMEM and back, for rates not needed here).
 //
 // The split.  The tokens of each (sequence, key head) are cut into units of 64, and all units of
-// the call in a row are shared out evenly: CTA c of n takes units [U c / n, U (c + 1) / n), whatever
-// the sequences' lengths are (they stay on the device).  An item (sequence and key head) whose
-// units lie in one CTA is finished there; of one that lies in several, each writes its sums,
-// and a second small kernel joins them in the order of the CTAs, so results repeat to the bit.
-// A CTA has at most two items it shares with others: its first and its last.
+// the call in a row are shared out evenly, a run of them to each CTA, whatever the sequences'
+// lengths are (they stay on the device).  An item (sequence and key head) whose
+// units lie in one CTA is finished there; of one that lies in several, each writes its sums
+// and counts itself, and the last one to do so joins them all, in the order of the CTAs, so that
+// results repeat to the bit.  A CTA has at most two items it shares with others: its first and its
+// last.  (A second kernel for the joins cost 5 to 7 us a call.)  The counters are cleared by a
+// small kernel in front, beside which this one starts (programmatic launch).
 //
 // In a CTA each of 4 warps takes 16 tokens of a unit on its own: it copies their keys and values
 // with 16-byte cp.async through its own ring of stages (no CTA barrier), multiplies, and keeps a
@@ -36,10 +38,7 @@
 namespace tileops {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kWarpTokens = 16;
-constexpr int kUnit = kWarps * kWarpTokens;
 constexpr int kMaxCtas = 2 * 148;  // two on each of a B200's SMs
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -52,13 +51,14 @@ struct DecodeArgs {
   const int32_t *table, *lens;
   void* o;
   float* lse;
-  int2* shared;     // [CTA]: the item that it begins and others go on with (or -1), how many of them
+  int* counters;    // [CTA]: how many CTAs have written their sums of the item that it begins
   float2* stats;    // [CTA][2][row]: exponent the sums are relative to, sum of weights
   float* partial;   // [CTA][2][row][D]: weighted sums
   int64_t q_b, q_h;
   CacheStrides ks, vs;
   int64_t table_stride, num_pages;
-  int batch, heads, heads_kv, group, dim, page_size, width, window, blocks;  // blocks of rows a key head
+  int batch, heads, heads_kv, group, dim, page_size, window, blocks;  // blocks of rows a key head
+  int room;  // tokens that a row of the table has pages for
   FastDivU32 div_page{1};
   float scale;  // log2(e) times the scale
   int* err;
@@ -125,34 +125,47 @@ __device__ constexpr float kShift = std::is_same<T, __half>::value ? 15.0f : 0.0
 struct Span {
   int begin, end, units;
 };
+template <int UNIT>
 __device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
-  const int64_t room = static_cast<int64_t>(a.width) * a.page_size;
-  int64_t len = a.lens[b];
-  if (len > room) {
-    report_device_error(a.err, kErrBadPage);
-    len = room;
-  }
   Span s;
-  s.end = static_cast<int>(max(len, static_cast<int64_t>(0)));
+  s.end = min(max(a.lens[b], 0), a.room);
   s.begin = a.window > 0 ? max(s.end - a.window, 0) : 0;
-  s.units = (s.end - s.begin + kUnit - 1) / kUnit;
+  s.units = (s.end - s.begin + UNIT - 1) / UNIT;
   return s;
 }
 
-// Where in the row of all units a warp is: item (b, head), head counting blocks of rows of key
-// heads, and the unit of it.
-struct Cursor {
-  int b, head, unit;
+// The row of all units, cut into equal runs: the first `longer` CTAs take size + 1 places, the rest
+// size.  An item takes a place for each of its units and one more, behind them, for the time that
+// joining its warps takes (about that of a unit, measured).  There are fewer than 2^31 places.
+struct Runs {
+  uint32_t size, longer;
+  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * size + min(c, longer); }
+  __device__ __forceinline__ uint32_t cta_of(uint32_t place) const {
+    const uint32_t head = longer * (size + 1);
+    return place < head ? place / (size + 1) : longer + (place - head) / size;
+  }
+};
+
+// A unit: item (b, head), head counting blocks of rows of key heads, and which unit of it.
+struct Unit {
+  int b, head, unit;  // b < 0: none
   Span span;
+};
+struct Cursor {
+  Unit u;
+  uint32_t place;
+  template <int UNIT>
   __device__ __forceinline__ void next(const DecodeArgs& a) {
-    if (++unit < span.units) return;
-    unit = 0;
-    if (++head < a.heads_kv * a.blocks) return;
-    head = 0;
+    ++place;
+    if (++u.unit < u.span.units) return;
+    ++place;
+    u.unit = 0;
+    if (++u.head < a.heads_kv * a.blocks) return;
+    u.head = 0;
     do {
-      if (++b >= a.batch) return;
-      span = span_of(a, b);
-    } while (span.units == 0);
+      if (++u.b >= a.batch) return;
+      u.span = span_of<UNIT>(a, u.b);
+    } while (u.span.units == 0);
   }
 };
 
@@ -167,156 +180,136 @@ __device__ __forceinline__ void store_row(T* to, float4 v, float all) {
   *reinterpret_cast<uint2*>(to) = w;
 }
 
-template <int DP, int MT>
+// What a warp knows of a unit ahead.
+struct Looked {
+  Unit u;
+  uint32_t place;
+  bool last;               // the CTA's last one
+  int page[kWarpTokens];   // of the warp's tokens in it, where they are inside the sequence
+};
+
+template <int DP, int MT, int WARPS>
 struct Layout {
   static constexpr int kChunks = DP / 8;                       // 16-byte chunks of a row
   static constexpr int kRow = (DP + 63) / 64 * 64;             // elements of a row in shared memory
   static constexpr int kStages = DP <= 64 ? 6 : DP <= 128 ? 3 : DP <= 192 ? 4 : 3;
-  static constexpr int kCtasSm = DP <= 128 ? 2 : 1;
+  static constexpr int kCtasSm = DP <= 128 && WARPS == 4 ? 2 : 1;
+  static constexpr int kUnit = WARPS * kWarpTokens;
+  static constexpr int kThreads = WARPS * 32;
   static constexpr int kTile = kWarpTokens * kRow;             // elements of a warp's keys (or values)
   static constexpr int kRows = 16 * MT;
-  static constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * 2 * kTile * 2;
+  static constexpr size_t kRing = static_cast<size_t>(WARPS) * kStages * 2 * kTile * 2;
   static constexpr size_t kQ = static_cast<size_t>(kRows) * kRow * 2;
-  static constexpr size_t kStats = static_cast<size_t>(kWarps) * kRows * 2 * 4;
-  static constexpr size_t kBytes = kRing + kQ + kStats;
+  static constexpr size_t kStats = static_cast<size_t>(WARPS) * kRows * 2 * 4;
+  static constexpr int kAhead = 2 * kStages;                   // units whose pages are on their way
+  static constexpr size_t kUnits = static_cast<size_t>(WARPS) * kAhead * sizeof(Looked);
+  static constexpr size_t kBytes = kRing + kQ + kStats + kUnits;
   // Chunk c of row r lies at chunk c ^ (r % 8): the 8 rows of a matrix in 8 different banks.
   static __device__ __forceinline__ uint32_t at(int r, int c) {
     return (r * (kRow / 8) + (c ^ (r & 7))) * 16;
   }
 };
 
-template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
+// Waits for the end of the kernel that clears the counters: before the first count, and before the
+// end, so that it has ended when what follows in the stream starts.
+__device__ __forceinline__ void behind_clearing() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename T, int DP, int MT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     paged_decode(const __grid_constant__ DecodeArgs a) {
-  using L = Layout<DP, MT>;
+  using L = Layout<DP, MT, WARPS>;
+  constexpr int kThreads = L::kThreads, kUnit = L::kUnit;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int64_t sums[kWarps];
-  __shared__ Cursor first;
+  __shared__ bool complete;
   T* const q_smem = reinterpret_cast<T*>(smem + L::kRing);
   float2* const stats = reinterpret_cast<float2*>(smem + L::kRing + L::kQ);  // [warp][row]
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  Looked* const ahead = reinterpret_cast<Looked*>(smem + L::kRing + L::kQ + L::kStats) + warp * L::kAhead;
   const int heads = a.heads_kv * a.blocks;
-  asm volatile("griddepcontrol.launch_dependents;");
 
-  // ---- units of the call, and this CTA's ----
-  const int per = (a.batch + kThreads - 1) / kThreads;
-  const int b0 = min(static_cast<int>(threadIdx.x) * per, a.batch), b1 = min(b0 + per, a.batch);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += span_of(a, b).units;
-  int64_t upto = mine;
+  // ---- places of the call ----
+  // By each warp on its own: every lane takes as many sequences, and then the lane whose sequences
+  // hold the run's begin has them shared out likewise.
+  auto places = [&](int b) {
+    const int units = span_of<kUnit>(a, b).units;
+    return units ? static_cast<uint32_t>(units + 1) * heads : 0u;
+  };
+  int from = 0, count = a.batch;  // the sequences in question
+  uint32_t mine, upto, total;
+  auto scan = [&]() {
+    const int per = (count + 31) / 32;
+    mine = 0;
+#pragma unroll 4
+    for (int i = 0; i < per; ++i) {
+      const int n = lane * per + i;
+      if (n < count) mine += places(from + n);
+    }
+    upto = mine;
 #pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const int64_t v = __shfl_up_sync(~0u, upto, d);
-    if (lane >= d) upto += v;
-  }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  int64_t total = 0, before = upto - mine;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += sums[w];
-    total += sums[w];
-  }
-  total *= heads;
-  const int64_t ctas = min(total, static_cast<int64_t>(gridDim.x));
-  const int64_t c = blockIdx.x;
+    for (int d = 1; d < 32; d *= 2) {
+      const uint32_t v = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += v;
+    }
+    return per;
+  };
+  int per = scan();
+  total = __shfl_sync(~0u, upto, 31);
+  const uint32_t c = blockIdx.x, ctas = min(total, gridDim.x);
 
-  // Sequences without a token.
-  for (int b = static_cast<int>(c); b < a.batch; b += gridDim.x) {
-    if (span_of(a, b).units) continue;
-    for (int64_t n = threadIdx.x; n < static_cast<int64_t>(a.heads) * a.dim; n += kThreads)
-      static_cast<T*>(a.o)[b * static_cast<int64_t>(a.heads) * a.dim + n] = Cvt<T>::from_f(0.0f);
-    for (int h = threadIdx.x; h < a.heads; h += kThreads)
-      a.lse[static_cast<int64_t>(b) * a.heads + h] = kNegInf;
-  }
+  auto without_tokens = [&]() {  // sequences of none; lengths that the table has no room for
+    for (int b = c; b < a.batch; b += gridDim.x) {
+      if (threadIdx.x == 0 && a.lens[b] > a.room) report_device_error(a.err, kErrBadPage);
+      if (span_of<kUnit>(a, b).units) continue;
+      for (int64_t n = threadIdx.x; n < static_cast<int64_t>(a.heads) * a.dim; n += kThreads)
+        static_cast<T*>(a.o)[static_cast<int64_t>(b) * a.heads * a.dim + n] = Cvt<T>::from_f(0.0f);
+      for (int h = threadIdx.x; h < a.heads; h += kThreads)
+        a.lse[static_cast<int64_t>(b) * a.heads + h] = kNegInf;
+    }
+  };
   if (c >= ctas) {
-    if (threadIdx.x == 0) a.shared[c] = make_int2(-1, 0);
+    without_tokens();
+    behind_clearing();
     return;
   }
-  const int64_t u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
-  if (before * heads <= u0 && u0 < (before + mine) * heads) {
-    int64_t at = before * heads;
-    for (int b = b0; b < b1; ++b) {
-      const Span s = span_of(a, b);
-      const int64_t n = static_cast<int64_t>(s.units) * heads;
-      if (u0 < at + n) {
-        first.b = b;
-        first.head = static_cast<int>((u0 - at) / s.units);
-        first.unit = static_cast<int>((u0 - at) % s.units);
-        first.span = s;
-        break;
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
-  Cursor put = first, get = first;  // of the copies and of the products
-  int64_t to_put = u1 - u0, to_get = u1 - u0;
+  Runs runs;
+  runs.size = total / ctas;
+  runs.longer = total - runs.size * ctas;
+  const uint32_t u0 = runs.begin(c), u1 = runs.begin(c + 1);
 
-  // ---- copies ----
-  const uint32_t ring = smem_at(smem) + warp * (L::kStages * 2 * L::kTile * 2);
-  auto page_of = [&]() {  // this lane's token of the unit at `put`: its page
-    const int t = put.span.begin + put.unit * kUnit + warp * kWarpTokens + lane;
-    int page = -1;
-    if (to_put > 0 && lane < kWarpTokens && t < put.span.end) {
-      page = a.table[put.b * a.table_stride + a.div_page.div(t)];
-      if (page < 0 || page >= a.num_pages) {
-        report_device_error(a.err, kErrBadPage);
-        page = -1;
-      }
-    }
-    return page;
-  };
-  int page = page_of();
-  auto issue = [&](int stage) {
-    if (to_put > 0) {
-      const int t = put.span.begin + put.unit * kUnit + warp * kWarpTokens + lane;
-      const int slot = t - static_cast<int>(a.div_page.div(max(t, 0))) * a.page_size;
-      const int head = put.head / a.blocks;
-      const T* k = static_cast<const T*>(a.k) + head * a.ks.head;
-      const T* v = static_cast<const T*>(a.v) + head * a.vs.head;
-      int64_t k_at = 0, v_at = 0;
-      if (page >= 0) {
-        k_at = page * a.ks.page + slot * a.ks.slot;
-        v_at = page * a.vs.page + slot * a.vs.slot;
-      }
-      const uint32_t to = ring + stage * (2 * L::kTile * 2);
-#pragma unroll
-      for (int i = 0; i < kWarpTokens * L::kChunks / 32; ++i) {
-        const int row = (i * 32 + lane) / L::kChunks, chunk = (i * 32 + lane) % L::kChunks;
-        const bool there = __shfl_sync(~0u, page, row) >= 0 && chunk * 8 < a.dim;
-        const int64_t ka = __shfl_sync(~0u, k_at, row), va = __shfl_sync(~0u, v_at, row);
-        const int64_t col = there ? chunk * 8 : 0;
-        copy16(to + L::at(row, chunk), k + ka + col, there);
-        copy16(to + L::kTile * 2 + L::at(row, chunk), v + va + col, there);
-      }
-      put.next(a);
-      --to_put;
-      page = page_of();
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
+  // ---- the run's first unit ----
+  uint32_t before = 0;  // places of the sequences before `from`
 #pragma unroll 1
-  for (int s = 0; s < L::kStages; ++s) issue(s);
+  while (true) {
+    const int at = __ffs(__ballot_sync(~0u, before + upto > u0)) - 1;
+    before += __shfl_sync(~0u, upto - mine, at);
+    from += at * per;
+    if (per == 1) break;
+    count = min(per, count - at * per);
+    per = scan();
+  }
+  Cursor look;
+  look.u.b = from;
+  look.u.span = span_of<kUnit>(a, from);
+  look.u.head = (u0 - before) / (look.u.span.units + 1);
+  look.u.unit = (u0 - before) - look.u.head * (look.u.span.units + 1);
+  look.place = u0;
+  if (look.u.unit == look.u.span.units) {  // behind an item: on to the next
+    --look.u.unit;
+    --look.place;
+    look.template next<kUnit>(a);
+  }
+  if (look.place >= u1) {  // a place behind an item and no more
+    without_tokens();
+    behind_clearing();
+    return;
+  }
 
-  // ---- products ----
-  // top: the exponent that a row's weights are relative to, its largest score (in fp16 less 15).
-  float out[MT][DP / 8][4], top[MT][2], sum[MT][2];
-  auto reset = [&]() {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[m][n][e] = 0.0f;
-      top[m][0] = top[m][1] = kNegInf;
-      sum[m][0] = sum[m][1] = 0.0f;
-    }
-  };
   // The rows of an item, zeros behind them: fetched while the item before is joined.
   constexpr int kQChunks = (L::kRows * L::kChunks + kThreads - 1) / kThreads;
   uint4 q_next[kQChunks];
-  auto fetch_q = [&](const Cursor& at) {
+  auto fetch_q = [&](const Unit& at) {
     const int h0 = (at.head / a.blocks) * a.group + (at.head % a.blocks) * L::kRows;
     const int rows = min(L::kRows, a.group - (at.head % a.blocks) * L::kRows);
 #pragma unroll
@@ -336,17 +329,102 @@ __global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
         *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(q_smem) + L::at(r, ch)) = q_next[i];
     }
   };
-  fetch_q(get);
+  fetch_q(look.u);
+
+  // ---- copies: the pages of a unit kAhead units ahead, its keys and values kStages ahead ----
+  const uint32_t ring = smem_at(smem) + warp * (L::kStages * 2 * L::kTile * 2);
+  auto look_up = [&](int slot) {
+    Looked& w = ahead[slot];
+    Unit u = look.u;
+    const uint32_t place = look.place;
+    if (look.place >= u1) {
+      u.b = -1;
+    } else {
+      const int t = u.span.begin + u.unit * kUnit + warp * kWarpTokens + lane;
+      if (lane < kWarpTokens && t < u.span.end)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(&w.page[lane])),
+                     "l"(a.table + u.b * a.table_stride + a.div_page.div(t))
+                     : "memory");
+      look.template next<kUnit>(a);
+    }
+    if (lane == 0) {
+      w.u = u;
+      w.place = place;
+      w.last = look.place >= u1;
+    }
+  };
+  auto issue = [&](int stage, int slot) {
+    const Looked& w = ahead[slot];
+    const Unit u = w.u;
+    if (u.b < 0) return;
+    const int t = u.span.begin + u.unit * kUnit + warp * kWarpTokens + lane;
+    const int head = u.head / a.blocks;
+    const T* k = static_cast<const T*>(a.k) + head * a.ks.head;
+    const T* v = static_cast<const T*>(a.v) + head * a.vs.head;
+    int64_t k_at = 0, v_at = 0;
+    bool inside = lane < kWarpTokens && t < u.span.end;
+    if (inside) {
+      const int page = w.page[lane];
+      if (page >= 0 && page < a.num_pages) {
+        const int place = t - static_cast<int>(a.div_page.div(t)) * a.page_size;
+        k_at = page * a.ks.page + place * a.ks.slot;
+        v_at = page * a.vs.page + place * a.vs.slot;
+      } else {
+        report_device_error(a.err, kErrBadPage);
+        inside = false;
+      }
+    }
+    const uint32_t rows = __ballot_sync(~0u, inside);
+    const uint32_t to = ring + stage * (2 * L::kTile * 2);
+#pragma unroll
+    for (int i = 0; i < kWarpTokens * L::kChunks / 32; ++i) {
+      const int row = (i * 32 + lane) / L::kChunks, chunk = (i * 32 + lane) % L::kChunks;
+      const bool there = ((rows >> row) & 1) && chunk * 8 < a.dim;
+      const int64_t ka = __shfl_sync(~0u, k_at, row), va = __shfl_sync(~0u, v_at, row);
+      const int64_t col = there ? chunk * 8 : 0;
+      copy16(to + L::at(row, chunk), k + ka + col, there);
+      copy16(to + L::kTile * 2 + L::at(row, chunk), v + va + col, there);
+    }
+  };
+#pragma unroll 1
+  for (int n = 0; n < L::kStages; ++n) look_up(n);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+#pragma unroll 1
+  for (int n = 0; n < L::kStages; ++n) {
+    issue(n, n);
+    look_up(L::kStages + n);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  // ---- products ----
+  // top: the exponent that a row's weights are relative to, its largest score (in fp16 less 15).
+  float out[MT][DP / 8][4], top[MT][2], sum[MT][2];
+  auto reset = [&]() {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[m][n][e] = 0.0f;
+      top[m][0] = top[m][1] = kNegInf;
+      sum[m][0] = sum[m][1] = 0.0f;
+    }
+  };
   store_q();
   reset();
   __syncthreads();
-  bool began = get.unit == 0;  // the item at `get` began in this CTA
-  int stage = 0;
+  without_tokens();
+  behind_clearing();
+  bool began = ahead[0].u.unit == 0;  // the item in hand began in this CTA
+  int stage = 0, slot = 0;
   const uint32_t q_at = smem_at(q_smem);
 #pragma unroll 1
   while (true) {
     asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
     __syncwarp();
+    const Unit get = ahead[slot].u;
+    const bool last = ahead[slot].last;
     const uint32_t keys = ring + stage * (2 * L::kTile * 2), values = keys + L::kTile * 2;
     const int t0 = get.span.begin + get.unit * kUnit + warp * kWarpTokens;
     if (t0 < get.span.end) {
@@ -417,201 +495,147 @@ __global__ void __launch_bounds__(kThreads, Layout<DP, MT>::kCtasSm)
         }
       }
     }
-    --to_get;
     const bool ended = get.unit + 1 == get.span.units;
-    if (ended || to_get == 0) {
+    if (ended || last) {
       // ---- the warps' sums of the item, joined through the stage just used ----
-      const Cursor item = get;
-      const bool whole = began && ended;
-      if (to_get > 0) {
-        get.next(a);
-        fetch_q(get);
-      }
-      const int block = item.head % a.blocks;
-      const int h0 = (item.head / a.blocks) * a.group + block * L::kRows;
+      bool whole = began && ended;
+      if (!last) fetch_q(ahead[slot + 1 == L::kAhead ? 0 : slot + 1].u);
+      const int block = get.head % a.blocks;
+      const int h0 = (get.head / a.blocks) * a.group + block * L::kRows;
       const int rows = min(L::kRows, a.group - block * L::kRows);
+#pragma unroll 1
+      while (true) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float v = sum[m][r];
-          v += __shfl_xor_sync(~0u, v, 1);
-          v += __shfl_xor_sync(~0u, v, 2);
-          if ((lane & 3) == 0)
-            stats[warp * L::kRows + m * 16 + r * 8 + lane / 4] = make_float2(top[m][r], v);
-        }
-      unsigned char* const own = smem + (warp * L::kStages + stage) * (2 * L::kTile * 2);
-      constexpr int kPad = L::kRow;  // floats of a row there: 16 rows fill the stage
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        __syncwarp();
-        // 8-column group n of row r at group (n + r) % groups: the 8 rows in different banks.
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (m * 16 + r * 8 >= rows) continue;
-#pragma unroll
-          for (int n = 0; n < DP / 8; ++n) {
-            const int row = r * 8 + lane / 4;
-            const int col = (n + lane / 4) % (DP / 8) * 8 + (lane & 3) * 2;
-            *reinterpret_cast<float2*>(own + (row * kPad + col) * 4) =
-                make_float2(out[m][n][2 * r], out[m][n][2 * r + 1]);
+          for (int r = 0; r < 2; ++r) {
+            float v = sum[m][r];
+            v += __shfl_xor_sync(~0u, v, 1);
+            v += __shfl_xor_sync(~0u, v, 2);
+            if ((lane & 3) == 0)
+              stats[warp * L::kRows + m * 16 + r * 8 + lane / 4] = make_float2(top[m][r], v);
           }
+        unsigned char* const own = smem + (warp * L::kStages + stage) * (2 * L::kTile * 2);
+        constexpr int kPad = L::kRow;  // floats of a row there: 16 rows fill the stage
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          __syncwarp();
+          // 8-column group n of row r at group (n + r) % groups: the 8 rows in different banks.
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (m * 16 + r * 8 >= rows) continue;
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n) {
+              const int row = r * 8 + lane / 4;
+              const int col = (n + lane / 4) % (DP / 8) * 8 + (lane & 3) * 2;
+              *reinterpret_cast<float2*>(own + (row * kPad + col) * 4) =
+                  make_float2(out[m][n][2 * r], out[m][n][2 * r + 1]);
+            }
+          }
+          __syncthreads();
+          if (m == 0) store_q();
+          for (int n = threadIdx.x; n < min(16, rows - m * 16) * (DP / 4); n += kThreads) {
+            const int r = n / (DP / 4), d = n % (DP / 4) * 4, row = m * 16 + r;
+            if (d >= a.dim) continue;
+            const int col = (d / 8 + (r & 7)) % (DP / 8) * 8 + d % 8;
+            float2 st[WARPS];
+            float high = kNegInf;
+#pragma unroll
+            for (int x = 0; x < WARPS; ++x) {
+              st[x] = stats[x * L::kRows + row];
+              high = fmaxf(high, st[x].x);
+            }
+            const float base = high == kNegInf ? 0.0f : high;
+            float all = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int x = 0; x < WARPS; ++x) {
+              const float f = ex2_approx_f(st[x].x - base);
+              const float4 p = *reinterpret_cast<const float4*>(
+                  smem + (x * L::kStages + stage) * (2 * L::kTile * 2) + (r * kPad + col) * 4);
+              all += f * st[x].y;
+              v.x += f * p.x;
+              v.y += f * p.y;
+              v.z += f * p.z;
+              v.w += f * p.w;
+            }
+            if (whole) {
+              const int64_t at = static_cast<int64_t>(get.b) * a.heads + h0 + row;
+              store_row(static_cast<T*>(a.o) + at * a.dim + d, v, all);
+              if (d == 0) a.lse[at] = base + log2f(all);
+            } else {
+              const int64_t at = (c * 2 + (began ? 1 : 0)) * L::kRows + row;
+              *reinterpret_cast<float4*>(a.partial + at * a.dim + d) = v;
+              if (d == 0) a.stats[at] = make_float2(high, all);
+            }
+          }
+          __syncthreads();
+        }
+        if (whole) break;
+        const uint32_t place = ahead[slot].place;
+        const uint32_t owner = began ? c : runs.cta_of(place - get.unit);
+        const uint32_t end = ended ? c : runs.cta_of(place + (get.span.units - 1 - get.unit));
+        if (threadIdx.x == 0) {  // releases the CTA's sums, written before the barrier
+          int count;
+          asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
+                       : "=r"(count)
+                       : "l"(a.counters + owner)
+                       : "memory");
+          complete = count == static_cast<int>(end - owner);
         }
         __syncthreads();
-        if (m == 0) store_q();
-        for (int n = threadIdx.x; n < min(16, rows - m * 16) * (DP / 4); n += kThreads) {
-          const int r = n / (DP / 4), d = n % (DP / 4) * 4, row = m * 16 + r;
-          if (d >= a.dim) continue;
-          const int col = (d / 8 + (r & 7)) % (DP / 8) * 8 + d % 8;
-          float2 st[kWarps];
-          float high = kNegInf;
+        if (!complete) break;
+        // The last of the item's CTAs: their sums, shared out to the warps.
+        whole = true;
+        reset();
+#pragma unroll 1
+        for (uint32_t x = owner + warp; x <= end; x += WARPS) {
+          const int64_t at = (x * 2 + (x == owner)) * L::kRows;
 #pragma unroll
-          for (int x = 0; x < kWarps; ++x) {
-            st[x] = stats[x * L::kRows + row];
-            high = fmaxf(high, st[x].x);
-          }
-          const float base = high == kNegInf ? 0.0f : high;
-          float all = 0.0f;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int x = 0; x < kWarps; ++x) {
-            const float f = ex2_approx_f(st[x].x - base);
-            const float4 p = *reinterpret_cast<const float4*>(
-                smem + (x * L::kStages + stage) * (2 * L::kTile * 2) + (r * kPad + col) * 4);
-            all += f * st[x].y;
-            v.x += f * p.x;
-            v.y += f * p.y;
-            v.z += f * p.z;
-            v.w += f * p.w;
-          }
-          if (whole) {
-            const int64_t at = static_cast<int64_t>(item.b) * a.heads + h0 + row;
-            store_row(static_cast<T*>(a.o) + at * a.dim + d, v, all);
-            if (d == 0) a.lse[at] = base + log2f(all);
-          } else {
-            const int64_t at = (c * 2 + (began ? 1 : 0)) * L::kRows + row;
-            *reinterpret_cast<float4*>(a.partial + at * a.dim + d) = v;
-            if (d == 0) a.stats[at] = make_float2(high, all);
-          }
+            for (int r = 0; r < 2; ++r) {
+              const int row = m * 16 + r * 8 + lane / 4;
+              if (row >= rows) continue;
+              const float2 st = __ldcg(a.stats + at + row);
+              const float* p = a.partial + (at + row) * a.dim + (lane & 3) * 2;
+              float2 v[DP / 8];
+#pragma unroll
+              for (int n = 0; n < DP / 8; ++n)
+                v[n] = n * 8 < a.dim ? __ldcg(reinterpret_cast<const float2*>(p + n * 8))
+                                     : make_float2(0.0f, 0.0f);
+              const float top_new = fmaxf(top[m][r], st.x);
+              const float base = top_new == kNegInf ? 0.0f : top_new;
+              const float fade = ex2_approx_f(top[m][r] - base), f = ex2_approx_f(st.x - base);
+              top[m][r] = top_new;
+              sum[m][r] = sum[m][r] * fade + ((lane & 3) == 0 ? f * st.y : 0.0f);
+#pragma unroll
+              for (int n = 0; n < DP / 8; ++n) {
+                out[m][n][2 * r] = out[m][n][2 * r] * fade + f * v[n].x;
+                out[m][n][2 * r + 1] = out[m][n][2 * r + 1] * fade + f * v[n].y;
+              }
+            }
         }
-        __syncthreads();
       }
-      if (to_get == 0) {
-        if (threadIdx.x == 0) {
-          int2 told = make_int2(-1, 0);
-          if (began && !ended) {
-            // The item's last unit, and the last CTA whose units begin at or before it.
-            const int64_t last = u1 - 1 + (item.span.units - 1 - item.unit);
-            told = make_int2(item.b * heads + item.head,
-                             static_cast<int>(((last + 1) * ctas - 1) / total - c));
-          }
-          a.shared[c] = told;
-        }
-        break;
-      }
+      if (last) break;
       began = true;
       reset();
     } else {
-      get.next(a);
       __syncwarp();
     }
-    issue(stage);
+    const int put = slot + L::kStages < L::kAhead ? slot + L::kStages : slot - L::kStages;
+    issue(stage, put);
+    look_up(slot);
+    asm volatile("cp.async.commit_group;" ::: "memory");
     stage = stage + 1 == L::kStages ? 0 : stage + 1;
+    slot = slot + 1 == L::kAhead ? 0 : slot + 1;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// One CTA an item that several CTAs share, found by the CTA that begins it: their sums, in order.
-// A team of warps takes a row: each lane holds the factors of up to kParts / 32 CTAs' sums and four or
-// eight channels; the warps of a team share out the CTAs, and their sums meet in shared memory.
-constexpr int kJoinWarps = 16;
-template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join(const __grid_constant__ DecodeArgs a,
-                                                              int rows_max) {
-  constexpr int kParts = (kMaxCtas + 31) / 32;
-  __shared__ float4 met[kJoinWarps][64];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t c = blockIdx.x;
-  const int2 told = a.shared[c];
-  if (told.x < 0) return;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int heads = a.heads_kv * a.blocks, b = told.x / heads, head = told.x % heads;
-  const int block = head % a.blocks;
-  const int h0 = (head / a.blocks) * a.group + block * rows_max;
-  const int rows = min(rows_max, a.group - block * rows_max);
-  int team = 1;  // warps of a row
-  while (team * 2 * rows <= kJoinWarps) team *= 2;
-  const int parts = told.y + 1;
-  // Sums of part x: slot 1 of this CTA, then slot 0 of those behind it.
-  auto slot = [&](int x, int row) { return ((c + x) * 2 + (x == 0)) * rows_max + row; };
-#pragma unroll 1
-  for (int row0 = 0; row0 < rows; row0 += kJoinWarps / team) {
-    const int row = row0 + warp / team, first = warp % team;
-    float f[kParts], all = 0.0f, base = 0.0f;
-    float4 v[2];
-    v[0] = v[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (row < rows) {
-      float2 st[kParts];
-      float high = kNegInf;
-#pragma unroll
-      for (int j = 0; j < kParts; ++j) {
-        const int x = j * 32 + lane;
-        st[j] = x < parts ? a.stats[slot(x, row)] : make_float2(kNegInf, 0.0f);
-        high = fmaxf(high, st[j].x);
-      }
-#pragma unroll
-      for (int d = 16; d; d /= 2) high = fmaxf(high, __shfl_xor_sync(~0u, high, d));
-      base = high == kNegInf ? 0.0f : high;
-#pragma unroll
-      for (int j = 0; j < kParts; ++j) {
-        f[j] = ex2_approx_f(st[j].x - base);
-        all += f[j] * st[j].y;
-      }
-#pragma unroll
-      for (int d = 16; d; d /= 2) all += __shfl_xor_sync(~0u, all, d);
-#pragma unroll
-      for (int j = 0; j < kParts; ++j) {
-        if (j * 32 >= parts) break;
-#pragma unroll 4
-        for (int x = first; x < 32; x += team) {
-          const float fx = __shfl_sync(~0u, f[j], x);
-          if (j * 32 + x >= parts) break;
-          const float* p = a.partial + slot(j * 32 + x, row) * a.dim;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int d = (i * 32 + lane) * 4;
-            if (d >= a.dim) continue;
-            const float4 w = *reinterpret_cast<const float4*>(p + d);
-            v[i].x += fx * w.x;
-            v[i].y += fx * w.y;
-            v[i].z += fx * w.z;
-            v[i].w += fx * w.w;
-          }
-        }
-      }
-    }
-    met[warp][lane] = v[0];
-    met[warp][32 + lane] = v[1];
-    __syncthreads();
-    if (row < rows && first == 0) {
-      const int64_t at = static_cast<int64_t>(b) * a.heads + h0 + row;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int d = (i * 32 + lane) * 4;
-        if (d >= a.dim) continue;
-        for (int w = 1; w < team; ++w) {
-          const float4 o = met[warp + w][i * 32 + lane];
-          v[i].x += o.x;
-          v[i].y += o.y;
-          v[i].z += o.z;
-          v[i].w += o.w;
-        }
-        store_row(static_cast<T*>(a.o) + at * a.dim + d, v[i], all);
-      }
-      if (lane == 0) a.lse[at] = base + log2f(all);
-    }
-    __syncthreads();
-  }
+__global__ void __launch_bounds__(kMaxCtas) clear_counters(int* counters) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  counters[threadIdx.x] = 0;
 }
 
 int padded_dim(int64_t dim) {
@@ -623,44 +647,63 @@ bool bad_sizes(int64_t batch, int64_t heads, int64_t heads_kv, int64_t dim) {
          heads % heads_kv != 0 || dim < 8 || dim > 256 || dim % 8 != 0;
 }
 
-template <typename T, int DP, int MT>
-int launch_tile(const DecodeArgs& a, int64_t grid, cudaStream_t s) {
-  using L = Layout<DP, MT>;
-  if (cudaFuncSetAttribute(paged_decode<T, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+template <typename T, int DP, int MT, int WARPS>
+int launch_tile(const DecodeArgs& a, cudaStream_t s) {
+  using L = Layout<DP, MT, WARPS>;
+  if (cudaFuncSetAttribute(paged_decode<T, DP, MT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(L::kBytes)) != cudaSuccess)
     return TILEOPS_ELAUNCH;
-  grid = std::min<int64_t>({grid, static_cast<int64_t>(sm_count()) * L::kCtasSm, kMaxCtas});
-  paged_decode<T, DP, MT><<<static_cast<unsigned>(grid), kThreads, L::kBytes, s>>>(a);
+  // No more CTAs than there can be units.
+  const int64_t seen = a.window ? std::min(a.room, a.window) : a.room;
+  const int64_t units = std::max<int64_t>(1, (seen + L::kUnit - 1) / L::kUnit);
+  const int64_t places = (units + 1) * a.batch * (a.heads_kv * a.blocks);
+  if (places > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
+  const int64_t grid =
+      std::min<int64_t>({places, static_cast<int64_t>(sm_count()) * L::kCtasSm, kMaxCtas});
+  clear_counters<<<1, kMaxCtas, 0, s>>>(a.counters);
   if (int status = launch_status()) return status;
-  // The join's CTAs may be placed while the first kernel's last ones run; they wait for its end.
+  // Starts once the first kernel has started, and so behind all that came before that one; the
+  // CTAs wait for its end before they count.
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(grid));
-  config.blockDim = dim3(kJoinWarps * 32);
+  config.blockDim = dim3(L::kThreads);
+  config.dynamicSmemBytes = L::kBytes;
   config.stream = s;
   config.attrs = &early;
   config.numAttrs = 1;
-  if (cudaLaunchKernelEx(&config, paged_join<T>, a, static_cast<int>(L::kRows)) != cudaSuccess)
+  if (cudaLaunchKernelEx(&config, paged_decode<T, DP, MT, WARPS>, a) != cudaSuccess)
     return TILEOPS_ELAUNCH;
   return launch_status();
 }
 
+template <typename T, int DP, int MT>
+int launch_warps(const DecodeArgs& a, cudaStream_t s) {
+  // Few items are shared by many CTAs each: one CTA of 8 warps an SM halves the sums that are joined.
+  // Many items: two CTAs of 4, so that one copies and multiplies while the other joins its warps.
+  if constexpr (DP <= 128) {
+    if (static_cast<int64_t>(a.batch) * a.heads_kv * a.blocks <= sm_count())
+      return launch_tile<T, DP, MT, 8>(a, s);
+  }
+  return launch_tile<T, DP, MT, 4>(a, s);
+}
+
 template <typename T>
-int launch_type(const DecodeArgs& a, int64_t grid, cudaStream_t s) {
+int launch_type(const DecodeArgs& a, cudaStream_t s) {
   const int dp = padded_dim(a.dim);
   const bool wide = rows_of(a.group, dp) == 32;
   switch (dp) {
-    case 64: return wide ? launch_tile<T, 64, 2>(a, grid, s) : launch_tile<T, 64, 1>(a, grid, s);
-    case 96: return wide ? launch_tile<T, 96, 2>(a, grid, s) : launch_tile<T, 96, 1>(a, grid, s);
-    case 128: return wide ? launch_tile<T, 128, 2>(a, grid, s) : launch_tile<T, 128, 1>(a, grid, s);
-    case 192: return launch_tile<T, 192, 1>(a, grid, s);
-    default: return launch_tile<T, 256, 1>(a, grid, s);
+    case 64: return wide ? launch_warps<T, 64, 2>(a, s) : launch_warps<T, 64, 1>(a, s);
+    case 96: return wide ? launch_warps<T, 96, 2>(a, s) : launch_warps<T, 96, 1>(a, s);
+    case 128: return wide ? launch_warps<T, 128, 2>(a, s) : launch_warps<T, 128, 1>(a, s);
+    case 192: return launch_warps<T, 192, 1>(a, s);
+    default: return launch_warps<T, 256, 1>(a, s);
   }
 }
 
-constexpr int64_t kSharedBytes = kMaxCtas * sizeof(int2);
+constexpr int64_t kCounterBytes = (kMaxCtas * sizeof(int) + 15) / 16 * 16;
 
 }  // namespace
 }  // namespace tileops
@@ -671,7 +714,7 @@ extern "C" int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t h
                                                         int64_t dim) {
   if (bad_sizes(1, heads, heads_kv, dim)) return -1;
   const int rows = rows_of(heads / heads_kv, padded_dim(dim));
-  return kSharedBytes + static_cast<int64_t>(kMaxCtas) * 2 * rows * (dim + 2) * 4;  // stats, sums
+  return kCounterBytes + static_cast<int64_t>(kMaxCtas) * 2 * rows * (dim + 2) * 4;  // stats, sums
 }
 
 extern "C" int tileops_paged_decode_fwd(
@@ -682,7 +725,7 @@ extern "C" int tileops_paged_decode_fwd(
     void* stream) {
   if (bad_sizes(batch, heads, heads_kv, dim) || num_pages < 0 || num_pages > 0x7fffffffLL ||
       page_size < 1 || page_size > 0x7fffffffLL || table_width < 0 || table_width > 0x7fffffffLL ||
-      page_size * table_width > 0x7fffffffLL - kUnit || window < 0 || window > 0x7fffffffLL)
+      page_size * table_width > 0x7fffffffLL - 128 || window < 0 || window > 0x7fffffffLL)
     return TILEOPS_EBADSHAPE;
   if (dtype != TILEOPS_DT_F16 && dtype != TILEOPS_DT_BF16) return TILEOPS_EBADDTYPE;
   if (batch == 0) return TILEOPS_OK;
@@ -701,7 +744,7 @@ extern "C" int tileops_paged_decode_fwd(
   a.lens = seq_lens;
   a.o = o;
   a.lse = lse;
-  a.shared = static_cast<int2*>(workspace);
+  a.counters = static_cast<int*>(workspace);
   a.q_b = strides8[0];
   a.q_h = strides8[1];
   a.ks = {strides8[2], strides8[3], strides8[4]};
@@ -714,21 +757,15 @@ extern "C" int tileops_paged_decode_fwd(
   a.group = static_cast<int>(heads / heads_kv);
   a.dim = static_cast<int>(dim);
   a.page_size = static_cast<int>(page_size);
-  a.width = static_cast<int>(table_width);
+  a.room = static_cast<int>(page_size * table_width);
   a.window = static_cast<int>(window);
   const int rows = rows_of(a.group, padded_dim(dim));
   a.blocks = (a.group + rows - 1) / rows;
-  a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + kSharedBytes);
+  a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + kCounterBytes);
   a.partial = reinterpret_cast<float*>(a.stats + static_cast<int64_t>(kMaxCtas) * 2 * rows);
   a.div_page = FastDivU32(static_cast<uint32_t>(page_size));
   a.scale = static_cast<float>(scale * 1.4426950408889634);
   a.err = device_error_ptr();
-  // No more CTAs than there can be units.
-  const int64_t room = std::min<int64_t>(page_size * table_width,
-                                         window ? window : page_size * table_width);
-  const int64_t units = std::max<int64_t>(1, (room + kUnit - 1) / kUnit);
-  const int64_t grid = std::min<int64_t>(units * batch * heads_kv * a.blocks, 1 << 20);
   cudaStream_t s = as_stream(stream);
-  return dtype == TILEOPS_DT_F16 ? launch_type<__half>(a, grid, s)
-                                 : launch_type<__nv_bfloat16>(a, grid, s);
+  return dtype == TILEOPS_DT_F16 ? launch_type<__half>(a, s) : launch_type<__nv_bfloat16>(a, s);
 }

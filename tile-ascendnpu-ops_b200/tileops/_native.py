@@ -205,7 +205,7 @@ def launch(name: str, device: torch.device, *args) -> None:
     """
     if device.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a cuda device, got {device}")
-    current = torch.cuda.current_device()
+    current = torch._C._cuda_getDevice()  # a cuda tensor exists: CUDA is initialised
     idx = device.index if device.index is not None else current
     # The stream's handle by itself costs 0.1 us, a torch.cuda.Stream object around it 2.5 us.
     stream = torch._C._cuda_getCurrentRawStream(idx)

@@ -15,26 +15,11 @@ from typing import Optional, Sequence
 import torch
 
 from tileops import _native
-from tileops.kernels.attention.rotary_embedding import (
-    channels_last,
-    check_rotation,
-    dense_like,
-    overlaps,
-    turns_array,
-)
+from tileops.kernels.attention._layouts import Layouts, channels_last, layout_of, overlaps, row_of
+from tileops.kernels.attention.rotary_embedding import check_rotation, turns_array
 from tileops.kernels.kernel_base import Kernel, check_dtype
 
 __all__ = ["PagedAttentionDecodeKernel", "PagedKVAppendKernel"]
-
-_KEPT = 64  # layouts an op keeps the stride arrays of
-
-
-def _keep(kept: dict, key, made):
-    if len(kept) >= _KEPT:
-        kept.clear()
-    kept[key] = made
-    return made
-
 
 class PagedKVAppendKernel(Kernel):
     """New tokens into a paged cache, keys (and queries) rotated on the way.
@@ -66,50 +51,65 @@ class PagedKVAppendKernel(Kernel):
         self.dtype = dtype
         self._code = _native.dtype_code(dtype)
         self._turns = turns_array(frequencies)
-        self._strides: dict = {}
+        self._plans = Layouts()
         self.init_config(config)
 
-    def _layout(self, k_cache, v_cache):
-        """The caches' strides; refuses caches whose slots share memory."""
+    def _plan(self, k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens):
+        """Device, which arguments have to be copied, the stride array, the table's stride, the rows and
+        the queries' shape; refuses caches that cannot be written."""
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-            if c.stride(-1) != 1 and c.shape[-1] > 1:
+            if not channels_last(c):
                 raise ValueError(f"{name} must have contiguous channels, got strides {c.stride()}")
             if overlaps(c.shape, c.stride()):
                 raise ValueError(f"{name} has slots that share memory: shape {tuple(c.shape)}, "
                                  f"strides {c.stride()}")
-        return k_cache.stride()[:3] + v_cache.stride()[:3]
-
-    def forward(self, k, v, k_cache, v_cache, page_table, seq_lens, q=None, cu_seqlens=None):
-        """Write the caches; return the rotated queries (None without ``q``)."""
-        k, v = channels_last(k), channels_last(v)
-        q = None if q is None else channels_last(q)
-        if page_table.stride(-1) != 1:
-            page_table = page_table.contiguous()
-        if seq_lens.stride(0) != 1:
-            seq_lens = seq_lens.contiguous()
-        if cu_seqlens is not None and cu_seqlens.stride(0) != 1:
-            cu_seqlens = cu_seqlens.contiguous()
-        q_out = None if q is None else dense_like(q)
-        key = (k.stride(), v.stride(), k_cache.stride(), v_cache.stride(), k_cache.shape[0],
-               None if q is None else q.stride(), cu_seqlens is None)
-        strides = self._strides.get(key)
-        if strides is None:
-            values = []
-            for t in (q, k, v, q_out):
-                s = (0, 0, 0) if t is None else t.stride()[:-1]
-                if len(s) == 2:  # rows of packed sequences, or one token each
-                    s = (s[0], 0, s[1]) if cu_seqlens is None else (0, s[0], s[1])
-                values += s
-            values += self._layout(k_cache, v_cache)
-            strides = _keep(self._strides, key, (ctypes.c_int64 * 18)(*values))
+        copy, values = [], []
+        for t, dense in ((q, False), (k, False), (v, False), (q, True)):
+            if t is None:
+                copy.append(False)
+                values += (0, 0, 0)
+                continue
+            copy.append(not channels_last(t))
+            dense |= copy[-1]
+            *rows, heads, dim = t.shape
+            if len(rows) == 2:
+                values += (rows[1] * heads * dim, heads * dim, dim) if dense else t.stride()[:3]
+                continue
+            token, head = (heads * dim, dim) if dense else t.stride()[:2]
+            values += (token, 0, head) if cu_seqlens is None else (0, token, head)
+        values += k_cache.stride()[:3] + v_cache.stride()[:3]
+        copy = (*copy[:3], page_table.stride(-1) != 1, seq_lens.stride(0) != 1,
+                cu_seqlens is not None and cu_seqlens.stride(0) != 1)
+        table_stride = page_table.shape[1] if copy[3] else page_table.stride(0)
         tokens = k.shape[0] if k.dim() == 3 else k.shape[0] * k.shape[1]
+        return (k.device, copy if any(copy) else None, (ctypes.c_int64 * 18)(*values), table_stride,
+                seq_lens.shape[0], tokens, k_cache.shape[0], page_table.shape[1],
+                None if q is None else row_of(q))
+
+    def forward(self, k, v, k_cache, v_cache, page_table, seq_lens, q=None, cu_seqlens=None,
+                layout=None):
+        """Write the caches; return the rotated queries (None without ``q``).  ``layout``: that of
+        (k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens), if it is at hand."""
+        if layout is None:
+            layout = layout_of(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
+        plan = self._plans.get(layout)
+        if plan is None:
+            plan = self._plans.keep(layout, self._plan(k, v, k_cache, v_cache, page_table, seq_lens,
+                                                       q, cu_seqlens))
+        device, copy, strides, table_stride, seqs, tokens, pages, columns, q_like = plan
+        if copy is not None:
+            q, k, v, page_table, seq_lens, cu_seqlens = (
+                t.contiguous() if c else t
+                for t, c in zip((q, k, v, page_table, seq_lens, cu_seqlens), copy))
+        q_out = None if q is None else torch.empty_like(q_like)
         _native.launch(
-            "tileops_paged_kv_append", k.device, _native.data_ptr(q), k.data_ptr(), v.data_ptr(),
-            _native.data_ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
-            seq_lens.data_ptr(), _native.data_ptr(cu_seqlens), self._turns, seq_lens.shape[0],
-            tokens, 0 if q is None else self.heads, self.heads_kv, self.dim, self.rotary_dim,
-            k_cache.shape[0], self.page_size, page_table.shape[1], page_table.stride(0), strides,
-            self.interleaved, self.amplitude, self._code)
+            "tileops_paged_kv_append", device, 0 if q is None else q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), 0 if q is None else q_out.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
+            0 if cu_seqlens is None else cu_seqlens.data_ptr(), self._turns, seqs, tokens,
+            0 if q is None else self.heads, self.heads_kv, self.dim, self.rotary_dim, pages,
+            self.page_size, columns, table_stride, strides, self.interleaved, self.amplitude,
+            self._code)
         return q_out
 
 
@@ -144,43 +144,49 @@ class PagedAttentionDecodeKernel(Kernel):
         self.scale, self.window = float(scale), int(window)
         self.dtype = dtype
         self._code = _native.dtype_code(dtype)
-        self._ws_bytes: Optional[int] = None
-        self._strides: dict = {}
+        self._plans = Layouts()
         self.init_config(config)
 
-    def _layout(self, q, k_cache, v_cache):
-        """Strides of q and the caches, multiples of 16 bytes (copies are never made of a cache)."""
+    def _plan(self, q, k_cache, v_cache, page_table, seq_lens):
+        """Device, which arguments have to be copied (never a cache), the stride array, the table's
+        stride and sizes, and the shapes of the outputs and the workspace."""
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-            if c.stride(-1) != 1 or any(s % 8 for s, n in zip(c.stride()[:3], c.shape) if n > 1):
+            if not channels_last(c) or any(s % 8 for s, n in zip(c.stride()[:3], c.shape) if n > 1):
                 raise ValueError(f"{name} must have contiguous channels and strides that are "
                                  f"multiples of 8, got {c.stride()}")
-        strides = [*q.stride()[:2]]
+        batch, heads, dim = q.shape
+        copy = (not channels_last(q) or q.stride(0) % 8 != 0 or q.stride(1) % 8 != 0,
+                page_table.stride(-1) != 1, seq_lens.stride(0) != 1)
+        strides = [heads * dim, dim] if copy[0] else [*q.stride()[:2]]
         for c in (k_cache, v_cache):  # what a single page, slot or head is apart has no say
             strides += [s if n > 1 else 0 for s, n in zip(c.stride()[:3], c.shape)]
-        return (ctypes.c_int64 * 8)(*strides)
+        table_stride = page_table.shape[1] if copy[1] else page_table.stride(0)
+        room = _native.lib().tileops_paged_decode_workspace_bytes(heads, self.heads_kv, dim)
+        like = torch.empty(1, dtype=torch.float32, device=q.device)
+        return (q.device, copy if any(copy) else None, (ctypes.c_int64 * 8)(*strides), table_stride,
+                batch, k_cache.shape[0], page_table.shape[1], row_of(q),
+                like.expand(batch, heads), like.expand(-(-room // 4)))
 
-    def forward(self, q, k_cache, v_cache, page_table, seq_lens):
-        """Return ``(o, lse)``."""
-        dev = q.device
-        if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-            q = q.clone(memory_format=torch.contiguous_format)
-        if page_table.stride(-1) != 1:
-            page_table = page_table.contiguous()
-        if seq_lens.stride(0) != 1:
-            seq_lens = seq_lens.contiguous()
-        key = (q.stride(), k_cache.stride(), v_cache.stride(), k_cache.shape[0])
-        strides = self._strides.get(key)
-        if strides is None:
-            strides = _keep(self._strides, key, self._layout(q, k_cache, v_cache))
-        if self._ws_bytes is None:
-            self._ws_bytes = _native.lib().tileops_paged_decode_workspace_bytes(
-                self.heads, self.heads_kv, self.dim)
-        o = dense_like(q)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
-        ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=dev)
+    def forward(self, q, k_cache, v_cache, page_table, seq_lens, layout=None):
+        """Return ``(o, lse)``.  ``layout``: that of the arguments, if it is at hand."""
+        if layout is None:
+            layout = layout_of(q, k_cache, v_cache, page_table, seq_lens)
+        plan = self._plans.get(layout)
+        if plan is None:
+            plan = self._plans.keep(layout, self._plan(q, k_cache, v_cache, page_table, seq_lens))
+        device, copy, strides, table_stride, batch, pages, columns, o_like, lse_like, ws_like = plan
+        if copy is not None:
+            q, page_table, seq_lens = (t.contiguous() if c else t
+                                       for t, c in zip((q, page_table, seq_lens), copy))
+        at = q.data_ptr()
+        if at % 16:  # strides of whole 16 bytes, but not its start
+            q = q.clone()
+            at = q.data_ptr()
+            strides = (ctypes.c_int64 * 8)(*q.stride()[:2], *strides[2:])
+        o, lse, ws = torch.empty_like(o_like), torch.empty_like(lse_like), torch.empty_like(ws_like)
         _native.launch(
-            "tileops_paged_decode_fwd", dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            page_table.data_ptr(), seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws.data_ptr(),
-            q.shape[0], self.heads, self.heads_kv, self.dim, k_cache.shape[0], self.page_size,
-            page_table.shape[1], page_table.stride(0), strides, self.window, self.scale, self._code)
+            "tileops_paged_decode_fwd", device, at, k_cache.data_ptr(), v_cache.data_ptr(),
+            page_table.data_ptr(), seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(),
+            ws.data_ptr(), batch, self.heads, self.heads_kv, self.dim, pages, self.page_size,
+            columns, table_stride, strides, self.window, self.scale, self._code)
         return o, lse

@@ -8,25 +8,26 @@ channels are contiguous are read in place whatever their other strides are
 from __future__ import annotations
 
 import ctypes
-import math
-from fractions import Fraction
 from typing import Optional, Sequence
 
 import torch
 
 from tileops import _native
+from tileops.kernels.attention._layouts import Layouts, channels_last, layout_of, row_of
 from tileops.kernels.kernel_base import Kernel, check_dtype
 
 __all__ = ["RotaryEmbeddingBwdKernel", "RotaryEmbeddingFwdKernel"]
 
 MAX_ROTARY_DIM = 256
-_TURNS_PER_RADIAN = Fraction("0.15915494309189533576888376337251436203445964574046")  # 1 / 2 pi
-_KEPT = 64  # layouts an op keeps the stride arrays of
+_TURNS_PER_RADIAN = 0x28be60db9391054a7f09d5f47d4d377036d8a5664f10e4107f9458  # 2^216 / 2 pi
 
 
 def turns_array(frequencies: Sequence[float]) -> ctypes.Array:
     """Angles a token, in radians, as whole numbers of 2^-64 turns modulo one turn."""
-    turns = [round(Fraction(f) * _TURNS_PER_RADIAN * 2**64) % 2**64 for f in frequencies]
+    turns = []
+    for f in frequencies:
+        n, d = float(f).as_integer_ratio()  # d a power of two
+        turns.append(((n * _TURNS_PER_RADIAN // d >> 151) + 1 >> 1) % 2**64)  # rounded
     return (ctypes.c_uint64 * max(1, len(turns)))(*turns)
 
 
@@ -38,33 +39,10 @@ def check_rotation(name: str, dim: int, rotary_dim: int, frequencies: Sequence[f
     if len(frequencies) != rotary_dim // 2:
         raise ValueError(f"frequencies must have rotary_dim / 2 = {rotary_dim // 2} values, got "
                          f"{len(frequencies)}")
-    if not all(math.isfinite(f) for f in frequencies):
-        raise ValueError("frequencies must be finite")
+    if not all(abs(f) < 2.0**64 for f in frequencies):
+        raise ValueError("frequencies must be finite and below 2^64")
     if not abs(amplitude) <= torch.finfo(torch.float32).max:
         raise ValueError(f"amplitude must be a finite float32, got {amplitude}")
-
-
-def overlaps(shape: Sequence[int], strides: Sequence[int]) -> bool:
-    """Whether two indices of a tensor can share an element (never wrongly no)."""
-    reach = 0
-    for stride, size in sorted((st, n) for st, n in zip(strides, shape) if n > 1):
-        if stride <= reach:
-            return True
-        reach += stride * (size - 1)
-    return False
-
-
-def dense_like(t: torch.Tensor) -> torch.Tensor:
-    """A dense output of ``t``'s shape and type (``empty_like`` costs the host half of what
-    ``empty`` does, but takes over the order of ``t``'s strides)."""
-    if t.is_contiguous():
-        return torch.empty_like(t)
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
-def channels_last(t: torch.Tensor) -> torch.Tensor:
-    """``t``, copied only when its channels are not contiguous."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 class _RotaryEmbeddingKernel(Kernel):
@@ -89,40 +67,52 @@ class _RotaryEmbeddingKernel(Kernel):
         self.dtype = dtype
         self._code = _native.dtype_code(dtype)
         self._turns = turns_array(frequencies)
-        self._strides: dict = {}
+        self._plans = Layouts()
         self.init_config(config)
 
-    def _stride_array(self, q, k, q_out, k_out):
-        key = tuple(None if t is None else t.stride() for t in (q, k, q_out, k_out))
-        found = self._strides.get(key)
-        if found is None:
-            if len(self._strides) >= _KEPT:
-                self._strides.clear()
-            found = (ctypes.c_int64 * 12)(*(v for s in key for v in (s[:3] if s else (0, 0, 0))))
-            self._strides[key] = found
-        return found
-
-    def forward(self, q, k, positions=None, inplace: bool = False):
-        """Return ``(q_out, k_out)``; ``inplace`` writes over ``q`` and ``k``."""
-        if inplace:
-            q_out, k_out = q, k
-        else:
-            q = None if q is None else channels_last(q)
-            k = None if k is None else channels_last(k)
-            q_out = None if q is None else dense_like(q)
-            k_out = None if k is None else dense_like(k)
-        stride, code = 0, 7
+    def _plan(self, q, k, positions, inplace: bool):
+        """Device, whether q, k and positions have to be copied, the stride array, the positions'
+        stride and type, and the outputs' shapes."""
+        copy = tuple(t is not None and not channels_last(t) and not inplace for t in (q, k))
+        like = tuple(None if t is None or inplace else row_of(t) for t in (q, k))
+        values = []
+        for t, dense in (*zip((q, k), copy), (q, not inplace), (k, not inplace)):
+            if t is None:
+                values += (0, 0, 0)
+            elif dense:
+                values += (t.shape[1] * t.shape[2] * t.shape[3], t.shape[2] * t.shape[3], t.shape[3])
+            else:
+                values += t.stride()[:3]
+        stride, code, copy_at = 0, 7, False
         if positions is not None:
-            if positions.stride(-1) != 1:
-                positions = positions.contiguous()
-            stride = positions.stride(0) if positions.dim() == 2 else 0
+            copy_at = positions.stride(-1) != 1
+            if positions.dim() == 2:
+                stride = positions.shape[1] if copy_at else positions.stride(0)
             code = 7 if positions.dtype is torch.int32 else 8
+        return ((k if q is None else q).device, any(copy) or copy_at, (*copy, copy_at),
+                (ctypes.c_int64 * 12)(*values), stride, code, like)
+
+    def forward(self, q, k, positions=None, inplace: bool = False, layout=None):
+        """Return ``(q_out, k_out)``; ``inplace`` writes over ``q`` and ``k``.  ``layout``: that of
+        (q, k, positions), if it is at hand."""
+        if layout is None:
+            layout = layout_of(q, k, positions)
+        key = None if layout is None else (layout, inplace)
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plans.keep(key, self._plan(q, k, positions, inplace))
+        device, copies, copy, strides, stride, code, (q_like, k_like) = plan
+        if copies:
+            q, k, positions = (t.contiguous() if c else t for t, c in zip((q, k, positions), copy))
+        q_out = q if q_like is None else torch.empty_like(q_like)
+        k_out = k if k_like is None else torch.empty_like(k_like)
         _native.launch(
-            "tileops_rotary", (k if q is None else q).device, _native.data_ptr(q),
-            _native.data_ptr(k), _native.data_ptr(positions), _native.data_ptr(q_out),
-            _native.data_ptr(k_out), self._turns, self.batch, self.seq_len, self.heads,
-            self.heads_kv, self.dim, self.rotary_dim, self._stride_array(q, k, q_out, k_out),
-            stride, code, self.interleaved, self.BACKWARD, self.amplitude, self._code)
+            "tileops_rotary", device, 0 if q is None else q.data_ptr(),
+            0 if k is None else k.data_ptr(), 0 if positions is None else positions.data_ptr(),
+            0 if q is None else q_out.data_ptr(), 0 if k is None else k_out.data_ptr(),
+            self._turns, self.batch, self.seq_len, self.heads, self.heads_kv, self.dim,
+            self.rotary_dim, strides, stride, code, self.interleaved, self.BACKWARD,
+            self.amplitude, self._code)
         return q_out, k_out
 
 

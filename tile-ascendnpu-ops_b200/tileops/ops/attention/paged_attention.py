@@ -42,6 +42,7 @@ import torch
 
 from tileops.device import get_device_backend
 from tileops.kernels.attention import PagedAttentionDecodeKernel, PagedKVAppendKernel
+from tileops.kernels.attention._layouts import Layouts, layout_of
 from tileops.kernels.kernel_base import Kernel
 from tileops.ops.attention._arguments import check_tensor
 from tileops.ops.attention.rotary_embedding import rotary_frequencies
@@ -90,7 +91,8 @@ class PagedKVAppendOp(Op):
                             else tuple(float(f) for f in frequencies))
         self.amplitude = amplitude
         self.dtype = dtype
-        self._tokens = 0, False  # of the last call: tokens, whether there were queries
+        self._last = (0, 0, 0), False  # of the last call: k's shape, whether there were queries
+        self._checked = Layouts()  # those that were found right
         self.dispatch_kernel(kernel_map)
         self.kernel = self.kernel_map["paged_kv_append"](
             heads_kv, dim, page_size, heads, rotary_dim, interleaved, self.frequencies, amplitude,
@@ -104,6 +106,14 @@ class PagedKVAppendOp(Op):
                 v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
                 q: Optional[torch.Tensor] = None,
                 cu_seqlens: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        layout = layout_of(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
+        if layout not in self._checked:
+            self._check(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
+            self._checked.keep(layout, True)
+        self._last = layout[0][0], q is not None
+        return self.kernel(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens, layout)
+
+    def _check(self, k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens) -> None:
         dev = getattr(k, "device", None)
         if get_device_backend().is_device_tensor(k) and k.dim() not in (3, 4):
             raise ValueError("k must be (batch, heads_kv, dim), (batch, tokens, heads_kv, dim) or packed "
@@ -118,22 +128,21 @@ class PagedKVAppendOp(Op):
             if len(rows) != 1:
                 raise ValueError("k must be packed, (tokens, heads_kv, dim), when using `cu_seqlens`, "
                                  f"got shape {tuple(k.shape)}")
-            batch = cu_seqlens.numel() - 1
-            check_tensor(dev, "cu_seqlens", cu_seqlens, (batch + 1,), torch.int32)
-            if batch < 0:
+            offsets = cu_seqlens.numel() if get_device_backend().is_device_tensor(cu_seqlens) else 0
+            check_tensor(dev, "cu_seqlens", cu_seqlens, (offsets,), torch.int32)
+            if offsets < 1:
                 raise ValueError("cu_seqlens must have at least one offset")
+            batch = offsets - 1
         _check_cache(dev, k_cache, v_cache, page_table, seq_lens, batch,
                      (self.page_size, self.heads_kv, self.dim), self.dtype)
-        count = rows[0] if len(rows) == 1 else rows[0] * rows[1]
-        if count >= 2**31:
-            raise ValueError(f"at most 2^31 - 1 tokens are supported, got {count}")
-        self._tokens = count, q is not None
-        return self.kernel(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
+        if k.numel() // (self.heads_kv * self.dim) >= 2**31:
+            raise ValueError(f"at most 2^31 - 1 tokens are supported, got shape {tuple(k.shape)}")
 
     def eval_roofline(self) -> tuple[int, int]:
         """``(3 * T * (H + Hkv) * rotary_dim, 2 * T * (H + 2 * Hkv) * dim * elem_bytes)`` of the T
         tokens of the last call, H 0 where it had no queries."""
-        tokens, queries = self._tokens
+        shape, queries = self._last
+        tokens = shape[0] if len(shape) == 3 else shape[0] * shape[1]
         heads = self.heads if queries else 0
         return (3 * tokens * (heads + self.heads_kv) * self.rotary_dim,
                 2 * tokens * (heads + 2 * self.heads_kv) * self.dim * self.dtype.itemsize)
@@ -162,7 +171,8 @@ class PagedAttentionDecodeOp(Op):
             raise ValueError(f"window must be at least 1 token, got {window}")
         self.window = window
         self.dtype = dtype
-        self._last = 0, 0  # of the last call: sequences, cached tokens there is room for
+        self._last = 0, 0  # of the last call: sequences, columns of the page table
+        self._checked = Layouts()  # those that were found right
         self.dispatch_kernel(kernel_map)
         self.kernel = self.kernel_map["paged_attention_decode"](
             heads, heads_kv, dim, page_size, self.scale, window or 0, dtype)
@@ -174,23 +184,29 @@ class PagedAttentionDecodeOp(Op):
     def forward(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 page_table: torch.Tensor,
                 seq_lens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        layout = layout_of(q, k_cache, v_cache, page_table, seq_lens)
+        if layout not in self._checked:
+            self._check(q, k_cache, v_cache, page_table, seq_lens)
+            self._checked.keep(layout, True)
+        self._last = layout[3][0]
+        return self.kernel(q, k_cache, v_cache, page_table, seq_lens, layout)
+
+    def _check(self, q, k_cache, v_cache, page_table, seq_lens) -> None:
         dev = getattr(q, "device", None)
         batch = q.shape[0] if hasattr(q, "shape") and len(q.shape) else 0
         check_tensor(dev, "q", q, (batch, self.heads, self.dim), self.dtype)
         _check_cache(dev, k_cache, v_cache, page_table, seq_lens, batch,
                      (self.page_size, self.heads_kv, self.dim), self.dtype)
-        room = page_table.shape[1] * self.page_size
-        if room >= 2**31 - 64:
-            raise ValueError("page_table has room for at most 2^31 - 65 tokens a sequence, got "
+        if page_table.shape[1] * self.page_size >= 2**31 - 128:
+            raise ValueError("page_table has room for at most 2^31 - 129 tokens a sequence, got "
                              f"{page_table.shape[1]} pages of {self.page_size}")
-        self._last = batch, min(room, self.window or room)
-        return self.kernel(q, k_cache, v_cache, page_table, seq_lens)
 
     def eval_roofline(self) -> tuple[int, int]:
         """``(4 * B * S * H * D, (2 * B * S * Hkv * D + 2 * B * H * D) * elem_bytes + 4 * B * H)``, S
         the tokens the last call's page table had room for, its window at most (the lengths
         themselves are on the device)."""
-        batch, seen = self._last
+        batch, columns = self._last
+        seen = min(columns * self.page_size, self.window or columns * self.page_size)
         q = batch * self.heads * self.dim
         return (4 * q * seen, (2 * batch * seen * self.heads_kv * self.dim + 2 * q)
                 * self.dtype.itemsize + 4 * batch * self.heads)

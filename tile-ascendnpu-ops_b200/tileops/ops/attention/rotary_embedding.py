@@ -34,7 +34,7 @@ import torch
 
 from tileops.device import get_device_backend
 from tileops.kernels.attention import RotaryEmbeddingBwdKernel, RotaryEmbeddingFwdKernel
-from tileops.kernels.attention.rotary_embedding import overlaps
+from tileops.kernels.attention._layouts import Layouts, channels_last, layout_of, overlaps
 from tileops.kernels.kernel_base import Kernel
 from tileops.ops.attention._arguments import check_tensor
 from tileops.ops.op_base import Op
@@ -94,18 +94,28 @@ class _RotaryEmbeddingOp(Op):
         self.kernel = self.kernel_map[name](batch, seq_len, heads, heads_kv, dim, self.rotary_dim,
                                             interleaved, self.frequencies, amplitude, dtype)
         self._shapes = (batch, seq_len, heads, dim), (batch, seq_len, heads_kv, dim)
+        self._checked = Layouts()  # those that were found right
 
     def forward(self, q: Optional[torch.Tensor], k: Optional[torch.Tensor],
                 positions: Optional[torch.Tensor] = None):
+        layout = layout_of(q, k, positions)
+        if layout not in self._checked:
+            self._check(q, k, positions)
+            self._checked.keep(layout, True)
+        if q is None and k is None:
+            return None, None
+        if self.inplace and q is not None and k is not None and q.data_ptr() == k.data_ptr() != 0:
+            raise ValueError(f"{self._names[0]} and {self._names[1]} share memory: they cannot both "
+                             "be rotated in place")
+        return self.kernel(q, k, positions, self.inplace, layout)
+
+    def _check(self, q, k, positions) -> None:
         dev = getattr(k if q is None else q, "device", None)
         for name, t, shape in zip(self._names, (q, k), self._shapes):
             if t is not None or shape[2]:
                 check_tensor(dev, name, t, shape, self.dtype)
                 if self.inplace:
                     self._check_inplace(name, t)
-        if self.inplace and q is not None and k is not None and q.data_ptr() == k.data_ptr() != 0:
-            raise ValueError(f"{self._names[0]} and {self._names[1]} share memory: they cannot both "
-                             "be rotated in place")
         if positions is not None:
             backend = get_device_backend()
             if not backend.is_device_tensor(positions):
@@ -118,13 +128,10 @@ class _RotaryEmbeddingOp(Op):
                                  f"{self.seq_len}), got {tuple(positions.shape)}")
             if positions.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-        if q is None and k is None:
-            return None, None
-        return self.kernel(q, k, positions, self.inplace)
 
     @staticmethod
     def _check_inplace(name: str, t: torch.Tensor) -> None:
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
+        if not channels_last(t):
             raise ValueError(f"{name} must have contiguous channels when it is rotated in place")
         if overlaps(t.shape, t.stride()):
             raise ValueError(f"{name} has elements that share memory: it cannot be rotated in place")
