@@ -10,10 +10,13 @@
 // Angles.  p f_i in fp32 is off by p f_i 2^-24 radians, 0.06 at a million tokens.  Here f_i is a
 // whole number of 2^-64 turns (made on the host in 64 bits): p times it, modulo 2^64, is the
 // phase exactly but for p 2^-65 turns, whatever the sign of p.  Its upper 32 bits as a signed
-// fraction go to sincospif: an argument off by 2^-25 half turns at most.
-// The angles of a token are made once by its CTA and serve all of its heads.
+// fraction, less whole quarter turns, go to sincospif: an argument off by 2^-27 half turns at most.
 //
-// HBM-bound: every channel is read and written once, about 3 flops each.
+// HBM-bound: every channel is read and written once, about 3 flops each.  An item is two vectors of
+// a head, 16 bytes each where layouts allow, that hold whole pairs.  A thread keeps one item of a
+// token (or of each of several at once, where a token has few items) and walks a tile of tokens with
+// it, so that addresses cost two multiplications; the tile's angles are made once, by all threads
+// and while the first loads are on their way, and serve all of its heads from shared memory.
 #include <algorithm>
 
 #include "common.cuh"
@@ -22,9 +25,9 @@
 namespace tileops {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of a CTA, at most
 constexpr int kMaxPairs = 128;  // rotated channels of a head <= 256
-constexpr int kMaxTokens = 16;  // of a CTA
+constexpr int kMaxTokens = 16;  // of a tile
 
 // Elements from a batch entry, token and head to the next.
 struct RowStrides {
@@ -38,12 +41,12 @@ struct RotaryArgs {
   const void* positions;  // of the tokens, or NULL: 0, 1, ... in each batch entry
   int64_t pos_stride;     // from a batch entry to the next
   int pos64;
-  int seq_len;            // tokens of a batch entry
-  int64_t tokens;         // in all
-  int heads, heads_kv, dim, rotary, tokens_cta;
+  uint32_t tokens;        // in all
+  int heads, heads_kv, dim, rotary, tile;  // tile: tokens of a CTA
   float amplitude, sign;
-  uint32_t per_row;       // items of a head: pairs of vectors
-  FastDivU32 div_token{1}, div_row{1};
+  uint32_t per_row, items;  // items of a head, of a token
+  uint32_t lanes;           // tokens that a CTA's threads take at once
+  FastDivU32 div_seq{1}, div_row{1}, div_items{1};  // by the tokens of a batch entry, per_row, items
   // paged
   const int32_t *page_table, *seq_lens, *cu_seqlens;
   int64_t table_stride, num_pages;
@@ -114,16 +117,16 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int num_seqs, int6
   return lo;
 }
 
-__device__ Token appended_token(const RotaryArgs& a, int64_t token) {
+__device__ Token appended_token(const RotaryArgs& a, uint32_t token) {
   Token k{0, 0, -1, 0};
   int b;
   if (a.cu_seqlens) {
     b = sequence_of(a.cu_seqlens, a.num_seqs, token);
     if (b == a.num_seqs) return k;  // behind the last sequence
-    k.position = a.seq_lens[b] - (a.cu_seqlens[b + 1] - token);
+    k.position = a.seq_lens[b] - (a.cu_seqlens[b + 1] - static_cast<int64_t>(token));
   } else {
-    b = static_cast<int>(token / a.seq_len);
-    k.position = static_cast<int64_t>(a.seq_lens[b]) - a.seq_len + token % a.seq_len;
+    b = a.div_seq.div(token);
+    k.position = static_cast<int64_t>(a.seq_lens[b]) - a.div_seq.d + (token - b * a.div_seq.d);
   }
   if (k.position < 0) return k;  // padding
   k.kept = 1;
@@ -141,150 +144,176 @@ __device__ Token appended_token(const RotaryArgs& a, int64_t token) {
   return k;
 }
 
-// One CTA: tokens_cta tokens, all heads.  An item is two vectors of VEC channels of a head that
-// hold VEC pairs (or up to 2 VEC channels behind the rotated ones); a thread keeps kBatch items'
-// loads in flight, the first of them while the angles are made.
+// cos and sin, times the amplitude, of a phase in 2^-32 turns.
+__device__ __forceinline__ float2 turn(uint32_t phase, float amplitude) {
+  const uint32_t quarters = (phase + 0x20000000u) >> 30;
+  const float half_turns = static_cast<int32_t>(phase - (quarters << 30)) * 0x1p-31f;
+  float s, c;
+  sincospif(half_turns, &s, &c);
+  s *= amplitude;
+  c *= amplitude;
+  const float cq = quarters & 1 ? -s : c, sq = quarters & 1 ? c : s;
+  return quarters & 2 ? make_float2(-cq, -sq) : make_float2(cq, sq);
+}
+
 template <typename T, int VEC, bool INTER, bool PAGED>
-__global__ void __launch_bounds__(kThreads) rotary_rows(const __grid_constant__ RotaryArgs a) {
-  constexpr int kBatch = 4;
-  __shared__ Token told[kMaxTokens];
-  extern __shared__ float2 angles[];  // [token][pair]
-  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * a.tokens_cta;
-  const int ntok = static_cast<int>(min(static_cast<int64_t>(a.tokens_cta), a.tokens - token0));
+__global__ void __launch_bounds__(kThreads, 3) rotary_rows(const __grid_constant__ RotaryArgs a) {
+  constexpr int kBatch = 2;  // tokens of a step; the next step's loads are in flight meanwhile
+  __shared__ Token told[PAGED ? kMaxTokens : 1];
+  extern __shared__ __align__(16) float angles[];  // [token][cos, sin][pair]
+  const uint32_t token0 = blockIdx.x * static_cast<uint32_t>(a.tile);
+  const int ntok = min(static_cast<uint32_t>(a.tile), a.tokens - token0);
   const int pairs = a.rotary / 2;
-  const uint32_t rows = a.heads + (PAGED ? 2 : 1) * a.heads_kv;
-  const uint32_t items = ntok * rows * a.per_row;
-  const uint32_t turned = pairs / VEC;  // items of a head that rotate
 
-  struct Item {
-    Vec<T, VEC> x, y;
-    int token, row, ca, cb;  // row: of q, then k, then v; ca < 0: no item; cb < 0: no second vector
-    int pair;                // < 0: passes unchanged
+  // ---- this thread's item ----
+  const int lane = a.lanes == 1 ? 0 : a.div_items.div(threadIdx.x);
+  const uint32_t item = blockIdx.y * blockDim.x + threadIdx.x - lane * a.items;
+  const bool mine = item < a.items && lane < a.lanes;
+  int row = a.div_row.div(item);  // of q, then k, then v
+  const uint32_t j = item - row * a.per_row;
+  const bool in_turn = j < static_cast<uint32_t>(pairs / VEC);
+  const int pair = j * VEC;  // the first of its pairs
+  int ca, cb;                // its channels; cb < 0: no second vector
+  if (in_turn) {
+    ca = INTER ? 2 * pair : pair;
+    cb = ca + (INTER ? VEC : pairs);
+  } else {
+    ca = a.rotary + (j - pairs / VEC) * 2 * VEC;
+    cb = ca + VEC < a.dim ? ca + VEC : -1;
+  }
+  const T* src;
+  T* dst;
+  RowStrides from, to;
+  int kind = 0;  // 0 q, 1 k, 2 v
+  if (row < a.heads) {
+    src = static_cast<const T*>(a.q);
+    dst = static_cast<T*>(a.q_out);
+    from = a.qs;
+    to = a.qo;
+  } else if (!PAGED || row < a.heads + a.heads_kv) {
+    row -= a.heads;
+    src = static_cast<const T*>(a.k);
+    dst = static_cast<T*>(a.k_out);
+    from = a.ks;
+    to = a.ko;
+    kind = 1;
+  } else {
+    row -= a.heads + a.heads_kv;
+    src = static_cast<const T*>(a.v);
+    dst = static_cast<T*>(a.v_out);
+    from = a.vs;
+    to = a.vo;
+    kind = 2;
+  }
+  src += row * from.h + ca;
+  dst += row * to.h + ca;
+  const int second = cb < 0 ? 0 : cb - ca;
+  const bool turns = in_turn && kind != 2;
+
+  struct Step {
+    Vec<T, VEC> x[kBatch], y[kBatch];
   };
-  Item it[kBatch];
-
-  auto fetch = [&](uint32_t base) {
+  Step even, odd;
+  const int step = kBatch * a.lanes;
+  auto fetch = [&](Step& in, int t) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      Item& m = it[u];
-      const uint32_t at = base + u * kThreads;
-      m.ca = -1;
-      if (at >= items) continue;
-      m.token = a.div_token.div(at);
-      const uint32_t rest = at - m.token * (rows * a.per_row);
-      m.row = a.div_row.div(rest);
-      const uint32_t j = rest - m.row * a.per_row;
-      if (j < turned) {
-        m.pair = j * VEC;
-        m.ca = INTER ? 2 * j * VEC : j * VEC;
-        m.cb = m.ca + (INTER ? VEC : pairs);
-      } else {
-        m.pair = -1;
-        m.ca = a.rotary + (j - turned) * 2 * VEC;
-        m.cb = m.ca + VEC < a.dim ? m.ca + VEC : -1;
-      }
-      const int64_t token = token0 + m.token;
-      int64_t b = 0, t = token;
-      if (!PAGED || !a.cu_seqlens) {
-        b = token / a.seq_len;
-        t = token - b * a.seq_len;
-      }
-      int h = m.row;
-      const void* src = a.q;
-      const RowStrides* s = &a.qs;
-      if (h >= a.heads) {
-        h -= a.heads;
-        src = a.k;
-        s = &a.ks;
-        if (PAGED && h >= a.heads_kv) {
-          h -= a.heads_kv;
-          src = a.v;
-          s = &a.vs;
-          m.pair = -1;
-        }
-      }
-      const T* p = static_cast<const T*>(src) + b * s->b + t * s->t + h * s->h;
-      load<T, VEC>(m.x, p + m.ca);
-      if (m.cb >= 0) load<T, VEC>(m.y, p + m.cb);
+      const int at = t + u * a.lanes;
+      if (!mine || at >= ntok) continue;
+      const uint32_t token = token0 + at, b = a.div_seq.div(token);
+      const T* p = src + b * from.b + (token - b * a.div_seq.d) * from.t;
+      load<T, VEC>(in.x[u], p);
+      if (cb >= 0) load<T, VEC>(in.y[u], p + second);
     }
   };
+  fetch(even, lane);
 
-  fetch(threadIdx.x);
-
+  // ---- the tile's angles ----
   if (PAGED) {
     if (threadIdx.x < ntok) told[threadIdx.x] = appended_token(a, token0 + threadIdx.x);
-    if (a.cu_seqlens && blockIdx.x == 0) {
-      bool bad = threadIdx.x == 0 && (a.cu_seqlens[0] != 0 || a.cu_seqlens[a.num_seqs] > a.tokens);
-      for (int n = threadIdx.x; n < a.num_seqs; n += kThreads)
+    if (a.cu_seqlens && blockIdx.x == 0 && blockIdx.y == 0) {
+      bool bad = threadIdx.x == 0 && (a.cu_seqlens[0] != 0 || a.cu_seqlens[a.num_seqs] > static_cast<int64_t>(a.tokens));
+      for (int n = threadIdx.x; n < a.num_seqs; n += blockDim.x)
         bad |= a.cu_seqlens[n] > a.cu_seqlens[n + 1];
       if (bad) report_device_error(a.err, kErrBadSeqlens);
     }
     __syncthreads();
   }
-  for (int n = threadIdx.x; n < ntok * pairs; n += kThreads) {
-    const int token = n / pairs, i = n - token * pairs;
+  for (int n = threadIdx.x; n < ntok * pairs; n += blockDim.x) {
+    const int at = n / pairs, i = n - at * pairs;
     int64_t position;
     if (PAGED) {
-      position = told[token].position;
+      position = told[at].position;
     } else {
-      const int64_t b = (token0 + token) / a.seq_len, t = token0 + token - b * a.seq_len;
-      const int64_t at = b * a.pos_stride + t;
+      const uint32_t b = a.div_seq.div(token0 + at), t = token0 + at - b * a.div_seq.d;
+      const int64_t place = b * a.pos_stride + t;
       position = !a.positions ? t
-                 : a.pos64    ? static_cast<const int64_t*>(a.positions)[at]
-                              : static_cast<const int32_t*>(a.positions)[at];
+                 : a.pos64    ? static_cast<const int64_t*>(a.positions)[place]
+                              : static_cast<const int32_t*>(a.positions)[place];
     }
-    const uint64_t phase = static_cast<uint64_t>(position) * a.turns[i];
-    const float half_turns = static_cast<int32_t>(phase >> 32) * 0x1p-31f;
-    float s, c;
-    sincospif(half_turns, &s, &c);
-    angles[n] = make_float2(a.amplitude * c, a.sign * a.amplitude * s);
+    const float2 w = turn(static_cast<uint32_t>((static_cast<uint64_t>(position) * a.turns[i]) >> 32),
+                          a.amplitude);
+    angles[at * a.rotary + i] = w.x;
+    angles[at * a.rotary + pairs + i] = a.sign * w.y;
   }
   __syncthreads();
 
-  for (uint32_t base = threadIdx.x; base < items; base += kBatch * kThreads) {
-    if (base != threadIdx.x) fetch(base);
+  auto finish = [&](Step& in, int t) {
+    Vec<T, VEC>(&x)[kBatch] = in.x, (&y)[kBatch] = in.y;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      Item& m = it[u];
-      if (m.ca < 0) continue;
-      if (m.pair >= 0) {
-        const float2* w = angles + m.token * pairs + m.pair;
+      const int at = t + u * a.lanes;
+      if (!mine || at >= ntok) continue;
+      if (turns) {
+        const float* c = angles + at * a.rotary + pair;
+        const float* s = c + pairs;
+        if constexpr (VEC % 2 == 0) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          T& first = INTER ? (2 * e < VEC ? m.x.e[2 * e % VEC] : m.y.e[2 * e - VEC]) : m.x.e[e];
-          T& second = INTER ? (2 * e + 1 < VEC ? m.x.e[(2 * e + 1) % VEC] : m.y.e[2 * e + 1 - VEC])
-                            : m.y.e[e];
-          const float c = w[e].x, s = w[e].y;
-          const float xa = Cvt<T>::to_f(first), xb = Cvt<T>::to_f(second);
-          first = Cvt<T>::from_f(c * xa - s * xb);
-          second = Cvt<T>::from_f(s * xa + c * xb);
+          for (int e = 0; e < VEC; e += 2) {
+            const float2 c2 = *reinterpret_cast<const float2*>(c + e);
+            const float2 s2 = *reinterpret_cast<const float2*>(s + e);
+            T* const first = INTER ? (2 * e < VEC ? x[u].e + 2 * e : y[u].e + (2 * e - VEC)) : x[u].e + e;
+            T* const other = !INTER ? y[u].e + e : 2 * e + 2 < VEC ? x[u].e + 2 * e + 2 : y[u].e + (2 * e + 2 - VEC);
+            // INTER: pairs (0, 1) of `first` and `other` each; else pairs across the two vectors.
+            const float2 a2 = INTER ? make_float2(Cvt<T>::to_f(first[0]), Cvt<T>::to_f(other[0]))
+                                    : make_float2(Cvt<T>::to_f(first[0]), Cvt<T>::to_f(first[1]));
+            const float2 b2 = INTER ? make_float2(Cvt<T>::to_f(first[1]), Cvt<T>::to_f(other[1]))
+                                    : make_float2(Cvt<T>::to_f(other[0]), Cvt<T>::to_f(other[1]));
+            const float2 sb = fmul2(s2, b2);
+            const float2 ra = ffma2(c2, a2, make_float2(-sb.x, -sb.y));
+            const float2 rb = ffma2(s2, a2, fmul2(c2, b2));
+            first[0] = Cvt<T>::from_f(ra.x);
+            (INTER ? other[0] : first[1]) = Cvt<T>::from_f(ra.y);
+            (INTER ? first[1] : other[0]) = Cvt<T>::from_f(rb.x);
+            other[1] = Cvt<T>::from_f(rb.y);
+          }
+        } else {
+          const float xa = Cvt<T>::to_f(x[u].e[0]), xb = Cvt<T>::to_f(y[u].e[0]);
+          x[u].e[0] = Cvt<T>::from_f(fmaf(c[0], xa, -(s[0] * xb)));
+          y[u].e[0] = Cvt<T>::from_f(fmaf(s[0], xa, c[0] * xb));
         }
       }
-      const int64_t token = token0 + m.token;
-      int64_t b = 0, t = token;
-      if (!PAGED || !a.cu_seqlens) {
-        b = token / a.seq_len;
-        t = token - b * a.seq_len;
-      }
-      T* p;
-      if (m.row < a.heads) {
-        p = static_cast<T*>(a.q_out) + b * a.qo.b + t * a.qo.t + m.row * a.qo.h;
-        if (PAGED && !(told[m.token].kept & 1)) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) m.x.e[e] = m.y.e[e] = Cvt<T>::from_f(0.0f);
-        }
-      } else if (!PAGED) {
-        p = static_cast<T*>(a.k_out) + b * a.ko.b + t * a.ko.t + (m.row - a.heads) * a.ko.h;
+      T* p = dst;
+      if (PAGED && kind != 0) {
+        if (!(told[at].kept & 2)) continue;
+        p += kind == 1 ? told[at].k_at : told[at].v_at;
       } else {
-        if (!(told[m.token].kept & 2)) continue;
-        const int h = m.row - a.heads;
-        p = h < a.heads_kv ? static_cast<T*>(a.k_out) + told[m.token].k_at + h * a.ko.h
-                           : static_cast<T*>(a.v_out) + told[m.token].v_at +
-                                 (h - a.heads_kv) * a.vo.h;
+        const uint32_t token = token0 + at, b = a.div_seq.div(token);
+        p += b * to.b + (token - b * a.div_seq.d) * to.t;
+        if (PAGED && !(told[at].kept & 1)) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) x[u].e[e] = y[u].e[e] = Cvt<T>::from_f(0.0f);
+        }
       }
-      *reinterpret_cast<decltype(m.x.w)*>(p + m.ca) = m.x.w;
-      if (m.cb >= 0) *reinterpret_cast<decltype(m.y.w)*>(p + m.cb) = m.y.w;
+      *reinterpret_cast<decltype(x[u].w)*>(p) = x[u].w;
+      if (cb >= 0) *reinterpret_cast<decltype(y[u].w)*>(p + second) = y[u].w;
     }
+  };
+  for (int t = lane; t < ntok; t += 2 * step) {
+    fetch(odd, t + step);
+    finish(even, t);
+    fetch(even, t + 2 * step);
+    finish(odd, t + step);
   }
 }
 
@@ -297,19 +326,22 @@ bool fits(const void* p, const RowStrides& s, int vec, size_t size) {
 template <typename T, int VEC, bool PAGED>
 int launch_vec(RotaryArgs& a, bool interleaved, cudaStream_t s) {
   a.per_row = a.rotary / (2 * VEC) + (a.dim - a.rotary + 2 * VEC - 1) / (2 * VEC);
-  const uint32_t rows = a.heads + (PAGED ? 2 : 1) * a.heads_kv;
-  const uint32_t per_token = rows * a.per_row;
-  a.div_token = FastDivU32(per_token);
+  a.items = (a.heads + (PAGED ? 2 : 1) * a.heads_kv) * a.per_row;
+  a.lanes = std::max<uint32_t>(1, kThreads / a.items);
   a.div_row = FastDivU32(a.per_row);
-  // Enough tokens a CTA for one batch of loads a thread, as long as every SM has some.
-  const int64_t full = std::max<int64_t>(1, 4 * kThreads / per_token);
-  const int64_t spread = std::max<int64_t>(1, a.tokens / (2 * sm_count()));
-  a.tokens_cta = static_cast<int>(std::min<int64_t>({full, spread, kMaxTokens}));
-  const int64_t grid = (a.tokens + a.tokens_cta - 1) / a.tokens_cta;
-  if (grid > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
-  const size_t smem = static_cast<size_t>(a.tokens_cta) * (a.rotary / 2) * sizeof(float2);
+  a.div_items = FastDivU32(a.items);
+  // The items of a token in as many CTAs as they need, in equal parts of whole warps.
+  const uint32_t groups = (a.items + kThreads - 1) / kThreads;
+  const uint32_t threads = groups == 1 ? kThreads : ((a.items + groups - 1) / groups + 31) / 32 * 32;
+  if (groups > 65535) return TILEOPS_EBADSHAPE;
+  // Tiles as long as the angles' room allows, while there are four CTAs an SM.
+  const int64_t spread = static_cast<int64_t>(a.tokens) * groups / (4 * sm_count());
+  a.tile = static_cast<int>(std::min<int64_t>(
+      kMaxTokens, std::max<int64_t>(spread, std::min<uint32_t>(a.lanes, kMaxTokens))));
+  const dim3 grid((a.tokens + a.tile - 1) / a.tile, groups);
+  const size_t smem = static_cast<size_t>(a.tile) * a.rotary * sizeof(float);
   auto kernel = interleaved ? rotary_rows<T, VEC, true, PAGED> : rotary_rows<T, VEC, false, PAGED>;
-  kernel<<<static_cast<unsigned>(grid), kThreads, smem, s>>>(a);
+  kernel<<<grid, threads, smem, s>>>(a);
   return launch_status();
 }
 
@@ -361,6 +393,7 @@ extern "C" int tileops_rotary(const void* q, const void* k, const void* position
                               int position_dtype, int interleaved, int backward, double amplitude,
                               int dtype, void* stream) {
   if (batch < 0 || seq_len < 0 || batch > 0x7fffffffLL || seq_len > 0x7fffffffLL ||
+      batch * seq_len > 0x7fffffffLL ||
       bad_heads(heads, heads_kv, dim, rotary_dim))
     return TILEOPS_EBADSHAPE;
   if (!is_float_dtype(dtype)) return TILEOPS_EBADDTYPE;
@@ -382,8 +415,8 @@ extern "C" int tileops_rotary(const void* q, const void* k, const void* position
   a.positions = positions;
   a.pos_stride = position_stride;
   a.pos64 = position_dtype == TILEOPS_DT_I64;
-  a.seq_len = static_cast<int>(seq_len);
-  a.tokens = batch * seq_len;
+  a.div_seq = FastDivU32(static_cast<uint32_t>(seq_len));
+  a.tokens = static_cast<uint32_t>(batch * seq_len);
   a.heads = static_cast<int>(heads);
   a.heads_kv = static_cast<int>(heads_kv);
   a.dim = static_cast<int>(dim);
@@ -425,8 +458,9 @@ extern "C" int tileops_paged_kv_append(
   a.qo = strides(strides18 + 9);
   a.ko = strides(strides18 + 12);
   a.vo = strides(strides18 + 15);
-  a.seq_len = static_cast<int>(cu_seqlens ? tokens : tokens / num_seqs);
-  a.tokens = tokens;
+  // Packed: one batch entry of all tokens.
+  a.div_seq = FastDivU32(static_cast<uint32_t>(cu_seqlens ? tokens : tokens / num_seqs));
+  a.tokens = static_cast<uint32_t>(tokens);
   a.heads = static_cast<int>(heads);
   a.heads_kv = static_cast<int>(heads_kv);
   a.dim = static_cast<int>(dim);
