@@ -27,7 +27,8 @@ namespace {
 
 constexpr int kThreads = 256;  // of a CTA, at most
 constexpr int kMaxPairs = 128;  // rotated channels of a head <= 256
-constexpr int kMaxTokens = 16;  // of a tile
+constexpr int kTile = 4;        // tokens of a CTA, for each that its threads take at once
+constexpr int kMaxTokens = 64;  // of a CTA
 
 // Elements from a batch entry, token and head to the next.
 struct RowStrides {
@@ -46,6 +47,7 @@ struct RotaryArgs {
   float amplitude, sign;
   uint32_t per_row, items;  // items of a head, of a token
   uint32_t lanes;           // tokens that a CTA's threads take at once
+  uint32_t groups;          // CTAs that share the items of a tile: neighbours, so that they run together
   FastDivU32 div_seq{1}, div_row{1}, div_items{1};  // by the tokens of a batch entry, per_row, items
   // paged
   const int32_t *page_table, *seq_lens, *cu_seqlens;
@@ -107,14 +109,15 @@ struct Token {
   int kept;            // bit 0: its queries are rotated (else zeroed), bit 1: it is appended
 };
 
-// Sequence of packed token t: the first whose end lies behind t, num_seqs where there is none.
+// Sequence of packed token t: the first whose end lies behind t, num_seqs where there is none.  (By
+// a warp, 32 ends at a time, the search waits less often, but the call is slower: its registers.)
 __device__ __forceinline__ int sequence_of(const int32_t* cu, int num_seqs, int64_t t) {
-  int lo = 0, hi = num_seqs;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid + 1] > t) hi = mid; else lo = mid + 1;
+  int from = 0, to = num_seqs;
+  while (from < to) {
+    const int middle = (from + to) >> 1;
+    if (cu[middle + 1] > t) to = middle; else from = middle + 1;
   }
-  return lo;
+  return from;
 }
 
 __device__ Token appended_token(const RotaryArgs& a, uint32_t token) {
@@ -157,17 +160,20 @@ __device__ __forceinline__ float2 turn(uint32_t phase, float amplitude) {
 }
 
 template <typename T, int VEC, bool INTER, bool PAGED>
-__global__ void __launch_bounds__(kThreads, 3) rotary_rows(const __grid_constant__ RotaryArgs a) {
-  constexpr int kBatch = 2;  // tokens of a step; the next step's loads are in flight meanwhile
+__global__ void __launch_bounds__(kThreads, 5) rotary_rows(const __grid_constant__ RotaryArgs a) {
   __shared__ Token told[PAGED ? kMaxTokens : 1];
-  extern __shared__ __align__(16) float angles[];  // [token][cos, sin][pair]
-  const uint32_t token0 = blockIdx.x * static_cast<uint32_t>(a.tile);
+  // [token], then as the items read them (16 bytes and no bank twice in 8 threads): two pairs' cos and
+  // sin together, those of the items' first pairs, of their next, ...
+  extern __shared__ __align__(16) float angles[];
+  constexpr int kTwo = VEC % 2 == 0 ? 2 : 1;  // pairs together
+  const uint32_t column = blockIdx.x / a.groups, group = blockIdx.x - column * a.groups;
+  const uint32_t token0 = column * static_cast<uint32_t>(a.tile);
   const int ntok = min(static_cast<uint32_t>(a.tile), a.tokens - token0);
   const int pairs = a.rotary / 2;
 
   // ---- this thread's item ----
   const int lane = a.lanes == 1 ? 0 : a.div_items.div(threadIdx.x);
-  const uint32_t item = blockIdx.y * blockDim.x + threadIdx.x - lane * a.items;
+  const uint32_t item = group * blockDim.x + threadIdx.x - lane * a.items;
   const bool mine = item < a.items && lane < a.lanes;
   int row = a.div_row.div(item);  // of q, then k, then v
   const uint32_t j = item - row * a.per_row;
@@ -210,28 +216,23 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_rows(const __grid_constant
   const int second = cb < 0 ? 0 : cb - ca;
   const bool turns = in_turn && kind != 2;
 
-  struct Step {
-    Vec<T, VEC> x[kBatch], y[kBatch];
+  Vec<T, VEC> x, y;
+  auto place = [&](int at, const RowStrides& s) {
+    const uint32_t token = token0 + at, b = a.div_seq.div(token);
+    return b * s.b + (token - b * a.div_seq.d) * s.t;
   };
-  Step even, odd;
-  const int step = kBatch * a.lanes;
-  auto fetch = [&](Step& in, int t) {
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int at = t + u * a.lanes;
-      if (!mine || at >= ntok) continue;
-      const uint32_t token = token0 + at, b = a.div_seq.div(token);
-      const T* p = src + b * from.b + (token - b * a.div_seq.d) * from.t;
-      load<T, VEC>(in.x[u], p);
-      if (cb >= 0) load<T, VEC>(in.y[u], p + second);
-    }
+  auto fetch = [&](int at) {
+    if (!mine || at >= ntok) return;
+    const T* p = src + place(at, from);
+    load<T, VEC>(x, p);
+    if (cb >= 0) load<T, VEC>(y, p + second);
   };
-  fetch(even, lane);
+  fetch(lane);
 
   // ---- the tile's angles ----
   if (PAGED) {
     if (threadIdx.x < ntok) told[threadIdx.x] = appended_token(a, token0 + threadIdx.x);
-    if (a.cu_seqlens && blockIdx.x == 0 && blockIdx.y == 0) {
+    if (a.cu_seqlens && blockIdx.x == 0) {
       bool bad = threadIdx.x == 0 && (a.cu_seqlens[0] != 0 || a.cu_seqlens[a.num_seqs] > static_cast<int64_t>(a.tokens));
       for (int n = threadIdx.x; n < a.num_seqs; n += blockDim.x)
         bad |= a.cu_seqlens[n] > a.cu_seqlens[n + 1];
@@ -253,67 +254,57 @@ __global__ void __launch_bounds__(kThreads, 3) rotary_rows(const __grid_constant
     }
     const float2 w = turn(static_cast<uint32_t>((static_cast<uint64_t>(position) * a.turns[i]) >> 32),
                           a.amplitude);
-    angles[at * a.rotary + i] = w.x;
-    angles[at * a.rotary + pairs + i] = a.sign * w.y;
+    const int of = i / VEC, r = i - of * VEC;
+    float* const to = angles + at * a.rotary + ((r / kTwo) * (pairs / VEC) + of) * 2 * kTwo + r % kTwo;
+    to[0] = w.x;
+    to[kTwo] = a.sign * w.y;
   }
   __syncthreads();
 
-  auto finish = [&](Step& in, int t) {
-    Vec<T, VEC>(&x)[kBatch] = in.x, (&y)[kBatch] = in.y;
+  for (int at = lane; at < ntok; at += a.lanes) {
+    if (!mine) break;
+    if (at != lane) fetch(at);
+    if (turns) {
+      const float* w = angles + at * a.rotary + j * 2 * kTwo;
+      if constexpr (VEC % 2 == 0) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int at = t + u * a.lanes;
-      if (!mine || at >= ntok) continue;
-      if (turns) {
-        const float* c = angles + at * a.rotary + pair;
-        const float* s = c + pairs;
-        if constexpr (VEC % 2 == 0) {
-#pragma unroll
-          for (int e = 0; e < VEC; e += 2) {
-            const float2 c2 = *reinterpret_cast<const float2*>(c + e);
-            const float2 s2 = *reinterpret_cast<const float2*>(s + e);
-            T* const first = INTER ? (2 * e < VEC ? x[u].e + 2 * e : y[u].e + (2 * e - VEC)) : x[u].e + e;
-            T* const other = !INTER ? y[u].e + e : 2 * e + 2 < VEC ? x[u].e + 2 * e + 2 : y[u].e + (2 * e + 2 - VEC);
-            // INTER: pairs (0, 1) of `first` and `other` each; else pairs across the two vectors.
-            const float2 a2 = INTER ? make_float2(Cvt<T>::to_f(first[0]), Cvt<T>::to_f(other[0]))
-                                    : make_float2(Cvt<T>::to_f(first[0]), Cvt<T>::to_f(first[1]));
-            const float2 b2 = INTER ? make_float2(Cvt<T>::to_f(first[1]), Cvt<T>::to_f(other[1]))
-                                    : make_float2(Cvt<T>::to_f(other[0]), Cvt<T>::to_f(other[1]));
-            const float2 sb = fmul2(s2, b2);
-            const float2 ra = ffma2(c2, a2, make_float2(-sb.x, -sb.y));
-            const float2 rb = ffma2(s2, a2, fmul2(c2, b2));
-            first[0] = Cvt<T>::from_f(ra.x);
-            (INTER ? other[0] : first[1]) = Cvt<T>::from_f(ra.y);
-            (INTER ? first[1] : other[0]) = Cvt<T>::from_f(rb.x);
-            other[1] = Cvt<T>::from_f(rb.y);
-          }
-        } else {
-          const float xa = Cvt<T>::to_f(x[u].e[0]), xb = Cvt<T>::to_f(y[u].e[0]);
-          x[u].e[0] = Cvt<T>::from_f(fmaf(c[0], xa, -(s[0] * xb)));
-          y[u].e[0] = Cvt<T>::from_f(fmaf(s[0], xa, c[0] * xb));
+        for (int e = 0; e < VEC; e += 2) {
+          const float4 cs = *reinterpret_cast<const float4*>(w + e * (pairs / VEC) * 2);
+          const float2 c2 = make_float2(cs.x, cs.y), s2 = make_float2(cs.z, cs.w);
+          T* const first = INTER ? (2 * e < VEC ? x.e + 2 * e : y.e + (2 * e - VEC)) : x.e + e;
+          T* const other = !INTER ? y.e + e : 2 * e + 2 < VEC ? x.e + 2 * e + 2 : y.e + (2 * e + 2 - VEC);
+          // INTER: pairs (0, 1) of `first` and `other` each; else pairs across the two vectors.
+          const float2 a2 = INTER ? make_float2(Cvt<T>::to_f(first[0]), Cvt<T>::to_f(other[0]))
+                                  : make_float2(Cvt<T>::to_f(first[0]), Cvt<T>::to_f(first[1]));
+          const float2 b2 = INTER ? make_float2(Cvt<T>::to_f(first[1]), Cvt<T>::to_f(other[1]))
+                                  : make_float2(Cvt<T>::to_f(other[0]), Cvt<T>::to_f(other[1]));
+          const float2 sb = fmul2(s2, b2);
+          const float2 ra = ffma2(c2, a2, make_float2(-sb.x, -sb.y));
+          const float2 rb = ffma2(s2, a2, fmul2(c2, b2));
+          first[0] = Cvt<T>::from_f(ra.x);
+          (INTER ? other[0] : first[1]) = Cvt<T>::from_f(ra.y);
+          (INTER ? first[1] : other[0]) = Cvt<T>::from_f(rb.x);
+          other[1] = Cvt<T>::from_f(rb.y);
         }
-      }
-      T* p = dst;
-      if (PAGED && kind != 0) {
-        if (!(told[at].kept & 2)) continue;
-        p += kind == 1 ? told[at].k_at : told[at].v_at;
       } else {
-        const uint32_t token = token0 + at, b = a.div_seq.div(token);
-        p += b * to.b + (token - b * a.div_seq.d) * to.t;
-        if (PAGED && !(told[at].kept & 1)) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) x[u].e[e] = y[u].e[e] = Cvt<T>::from_f(0.0f);
-        }
+        const float xa = Cvt<T>::to_f(x.e[0]), xb = Cvt<T>::to_f(y.e[0]);
+        x.e[0] = Cvt<T>::from_f(fmaf(w[0], xa, -(w[1] * xb)));
+        y.e[0] = Cvt<T>::from_f(fmaf(w[1], xa, w[0] * xb));
       }
-      *reinterpret_cast<decltype(x[u].w)*>(p) = x[u].w;
-      if (cb >= 0) *reinterpret_cast<decltype(y[u].w)*>(p + second) = y[u].w;
     }
-  };
-  for (int t = lane; t < ntok; t += 2 * step) {
-    fetch(odd, t + step);
-    finish(even, t);
-    fetch(even, t + 2 * step);
-    finish(odd, t + step);
+    T* p = dst;
+    if (PAGED && kind != 0) {
+      if (!(told[at].kept & 2)) continue;
+      p += kind == 1 ? told[at].k_at : told[at].v_at;
+    } else {
+      p += place(at, to);
+      if (PAGED && !(told[at].kept & 1)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x.e[e] = y.e[e] = Cvt<T>::from_f(0.0f);
+      }
+    }
+    *reinterpret_cast<decltype(x.w)*>(p) = x.w;
+    if (cb >= 0) *reinterpret_cast<decltype(y.w)*>(p + second) = y.w;
   }
 }
 
@@ -327,21 +318,26 @@ template <typename T, int VEC, bool PAGED>
 int launch_vec(RotaryArgs& a, bool interleaved, cudaStream_t s) {
   a.per_row = a.rotary / (2 * VEC) + (a.dim - a.rotary + 2 * VEC - 1) / (2 * VEC);
   a.items = (a.heads + (PAGED ? 2 : 1) * a.heads_kv) * a.per_row;
-  a.lanes = std::max<uint32_t>(1, kThreads / a.items);
+  // The items of a token in as many CTAs as they need, in equal parts of whole warps; or several
+  // tokens side by side, as far as their tile's angles fit 16 KB.
+  const uint32_t groups = (a.items + kThreads - 1) / kThreads;
+  const uint32_t fit = std::min(kMaxTokens / kTile, 1024 / std::max(a.rotary, 1));
+  a.lanes = std::max<uint32_t>(1, std::min<uint32_t>(kThreads / a.items, fit));
+  // At least a thread for each token of the tile.
+  const uint32_t threads = (std::max((a.items + groups - 1) / groups, uint32_t{kTile}) * a.lanes + 31) / 32 * 32;
   a.div_row = FastDivU32(a.per_row);
   a.div_items = FastDivU32(a.items);
-  // The items of a token in as many CTAs as they need, in equal parts of whole warps.
-  const uint32_t groups = (a.items + kThreads - 1) / kThreads;
-  const uint32_t threads = groups == 1 ? kThreads : ((a.items + groups - 1) / groups + 31) / 32 * 32;
-  if (groups > 65535) return TILEOPS_EBADSHAPE;
-  // Tiles as long as the angles' room allows, while there are four CTAs an SM.
-  const int64_t spread = static_cast<int64_t>(a.tokens) * groups / (4 * sm_count());
-  a.tile = static_cast<int>(std::min<int64_t>(
-      kMaxTokens, std::max<int64_t>(spread, std::min<uint32_t>(a.lanes, kMaxTokens))));
-  const dim3 grid((a.tokens + a.tile - 1) / a.tile, groups);
+  // kTile tokens for each that is taken at once, while that makes four CTAs an SM.  (Tiles of 8 and 16
+  // were slower, 8 x 4096 x 64 heads x 128 bf16 174 and 188 us for 165: CTAs that run together then
+  // lie further apart in memory.)
+  const int64_t spread = static_cast<int64_t>(a.tokens) * groups / (4 * sm_count() * a.lanes);
+  a.tile = static_cast<int>(a.lanes * std::min<int64_t>(kTile, std::max<int64_t>(spread, 1)));
+  a.groups = groups;
+  const int64_t grid = static_cast<int64_t>((a.tokens + a.tile - 1) / a.tile) * groups;
+  if (grid > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
   const size_t smem = static_cast<size_t>(a.tile) * a.rotary * sizeof(float);
   auto kernel = interleaved ? rotary_rows<T, VEC, true, PAGED> : rotary_rows<T, VEC, false, PAGED>;
-  kernel<<<grid, threads, smem, s>>>(a);
+  kernel<<<static_cast<unsigned>(grid), threads, smem, s>>>(a);
   return launch_status();
 }
 
