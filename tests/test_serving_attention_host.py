@@ -1,0 +1,465 @@
+"""Host side of the rotary and paged-cache ops: the 64-bit oracle against differences and against
+itself by another route, refusals before any launch, roofline formulas, the C entry points'
+argument checks.  CPU only."""
+
+import ctypes
+import math
+from fractions import Fraction
+
+import pytest
+import torch
+
+from oracle import serving_attention as ref
+from tileops import _native
+from tileops.benchmark.msprof import _extract_op_init_args
+from tileops.kernels.attention import (
+    PagedAttentionDecodeKernel,
+    PagedKVAppendKernel,
+    RotaryEmbeddingBwdKernel,
+    RotaryEmbeddingFwdKernel,
+)
+from tileops.kernels.attention._layouts import Layouts, layout_of, overlaps
+from tileops.kernels.attention.rotary_embedding import turns_array
+from tileops.manifest import load_workloads
+from tileops.ops.attention import (
+    PagedAttentionDecodeOp,
+    PagedKVAppendOp,
+    RotaryEmbeddingBwdOp,
+    RotaryEmbeddingFwdOp,
+    rotary_frequencies,
+)
+
+NULL = ctypes.c_void_p(0)
+SOME = ctypes.c_void_p(1 << 20)  # never read: every call here fails its checks before a launch
+
+
+# ------------------------------------------------------------ the oracle
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_gradient_against_differences(interleaved):
+    f = rotary_frequencies(6)
+    x, d = (torch.randn(3, 2, 8, dtype=torch.float64) for _ in range(2))
+    at = torch.tensor([0, 5, -3])
+    grad, _ = ref.rotate(d, at, f, 1.5, interleaved, backward=True)
+
+    def loss():
+        return (ref.rotate(x, at, f, 1.5, interleaved)[0] * d).sum().item()
+
+    for n in range(x.numel()):
+        flat, keep = x.view(-1), x.view(-1)[n].item()
+        flat[n] = keep + 0.5
+        up = loss()
+        flat[n] = keep - 0.5
+        # A linear map: the difference is exact but for rounding, 2^-53 of sums below 100.
+        assert abs((up - loss()) - grad.view(-1)[n].item()) < 1e-12
+        flat[n] = keep
+
+
+def test_rotation_keeps_lengths_and_relative_positions():
+    f = rotary_frequencies(32)
+    q, k = (torch.randn(1, 32, dtype=torch.float64) for _ in range(2))
+
+    def score(p, r):
+        a, _ = ref.rotate(q[None], torch.tensor([p]), f)
+        b, _ = ref.rotate(k[None], torch.tensor([r]), f)
+        return (a * b).sum().item()
+
+    assert abs(score(7, 3) - score(1000007, 1000003)) < 1e-9
+    a, _ = ref.rotate(q[None], torch.tensor([12345]), f)
+    assert abs(a.norm() - q.norm()) < 1e-12
+
+
+def test_angles_of_far_positions_lose_nothing():
+    """Against 64-bit products where those are exact enough, and by whole turns where not."""
+    f = rotary_frequencies(16)
+    near = torch.arange(-500, 500)
+    want = near[:, None].double() * torch.tensor(f, dtype=torch.float64)
+    off = (torch.sin(ref.angles(near, f)) - torch.sin(want)).abs().max()
+    assert off < 1e-12
+    turn = [math.tau]  # math.tau is 2 pi less 2.45e-16: a million turns are 2.45e-10 off
+    assert (torch.sin(ref.angles(torch.tensor([10**6]), turn)) + 2.4492935982947064e-10).abs() < 1e-15
+
+
+def test_attention_oracle_against_torch():
+    B, H, Hkv, D, P = 2, 4, 2, 16, 4
+    k, v = (torch.randn(2, 12, Hkv, D, dtype=torch.float64) for _ in range(2))
+    q = torch.randn(B, H, D, dtype=torch.float64)
+    table = torch.tensor([[2, 0, 5], [1, 3, 4]])
+    kc, vc = (torch.full((6, P, Hkv, D), math.nan, dtype=torch.float64) for _ in range(2))
+    lens = torch.tensor([11, 5])
+    for b in range(B):
+        for t in range(int(lens[b])):
+            kc[table[b, t // P], t % P], vc[table[b, t // P], t % P] = k[b, t], v[b, t]
+    o, lse, _, _ = ref.attend(q, kc, vc, table, lens, window=6)
+    for b in range(B):
+        n, first = int(lens[b]), max(0, int(lens[b]) - 6)
+        for h in range(H):
+            s = k[b, first:n, h // 2] @ q[b, h] / D**0.5
+            torch.testing.assert_close(o[b, h], torch.softmax(s, 0) @ v[b, first:n, h // 2])
+            torch.testing.assert_close(lse[b, h], torch.logsumexp(s, 0) / math.log(2))
+
+
+def test_append_oracle_positions_and_padding():
+    kc, vc = torch.zeros(3, 4, 1, 2), torch.zeros(3, 4, 1, 2)
+    k = torch.arange(1.0, 7.0).repeat_interleave(2).view(6, 1, 2)
+    table = torch.tensor([[2, -1], [0, 1]])
+    cu = torch.tensor([0, 3, 5])
+    _, _, got, bound, values = ref.append(k, -k, kc, vc, table, torch.tensor([2, 6]), cu_seqlens=cu)
+    want = torch.zeros(3, 4)
+    want[2, 0], want[2, 1] = 2, 3  # row 0 has position -1: padding; row 5 lies behind the last
+    want[1, 0], want[1, 1] = 4, 5
+    assert torch.equal(got[..., 0, 0], want.double()) and torch.equal(values, -got)
+    assert not bound.any()
+
+
+# ------------------------------------------------------------ frequencies
+def test_frequencies():
+    f = rotary_frequencies(8)
+    assert f == pytest.approx((1.0, 0.1, 0.01, 0.001), rel=1e-15)
+    assert rotary_frequencies(8, factor=4.0) == pytest.approx([x / 4 for x in f], rel=1e-15)
+    g = rotary_frequencies(8, factor=4.0, original_length=1000, slow_turns=1.0, fast_turns=32.0)
+    turns = [1000 * x / math.tau for x in f]  # 159, 15.9, 1.59, 0.159
+    kept = [1.0, (turns[1] - 1) / 31, (turns[2] - 1) / 31, 0.0]
+    assert g == pytest.approx([x * (r + (1 - r) / 4) for x, r in zip(f, kept)], rel=1e-15)
+    assert rotary_frequencies(0) == ()
+    for bad in (dict(rotary_dim=7), dict(rotary_dim=-2), dict(rotary_dim=8, base=0.0),
+                dict(rotary_dim=8, base=math.inf), dict(rotary_dim=8, factor=0.0),
+                dict(rotary_dim=8, factor=math.nan), dict(rotary_dim=8, original_length=0),
+                dict(rotary_dim=8, original_length=9, slow_turns=2.0, fast_turns=2.0)):
+        with pytest.raises(ValueError):
+            rotary_frequencies(**bad)
+
+
+def test_turns_are_rounded_once():
+    f = rotary_frequencies(64, 500000.0) + (0.0, -1.0, 1e-30, 100.0, 1e15)
+    exact = [round(Fraction(x) * ref._TURNS_PER_RADIAN * 2**64) % 2**64 for x in f]
+    assert list(turns_array(f)) == exact
+
+
+# ------------------------------------------------------------ layouts
+def test_overlaps():
+    t = torch.empty(4, 6, 8)
+    for fine in (t, t.transpose(0, 2), t[:, ::2, 1:], t[:1].expand(1, 6, 8), t.permute(2, 0, 1)):
+        assert not overlaps(fine.shape, fine.stride())
+    for bad in (t[:1].expand(3, 6, 8), t.as_strided((4, 4), (1, 1)), t.as_strided((3, 5), (4, 1))):
+        assert overlaps(bad.shape, bad.stride())
+
+
+def test_layouts_are_values():
+    """Another tensor of the same layout has the same one; whatever differs shows."""
+    a, b = torch.empty(2, 3, 4), torch.empty(2, 3, 4)
+    assert layout_of(a, None) == layout_of(b, None)
+    for other in (a.half(), a.transpose(0, 1), a.expand(2, 3, 4)[:1], torch.empty(2, 4, 3)):
+        assert layout_of(a) != layout_of(other)
+    assert layout_of("no tensor") is None and layout_of(a, 3) is None
+    kept = Layouts()
+    for n in range(1000):
+        kept.keep((n,), n)
+    assert len(kept) <= 256 and kept.get((999,)) == 999
+    kept.keep(None, 5)
+    assert kept.get(None) is None
+
+
+# ------------------------------------------------------------ refusals
+class _AcceptCpu:
+    name = "cuda"
+
+    def is_device_tensor(self, t):
+        return isinstance(t, torch.Tensor)
+
+    def is_available(self):
+        return False
+
+
+@pytest.fixture
+def accept_cpu(monkeypatch):
+    """Admit CPU tensors so the later checks run here; every case raises before a launch."""
+    import tileops.ops.attention._arguments as arguments
+    import tileops.ops.attention.paged_attention as paged
+    import tileops.ops.attention.rotary_embedding as rotary
+
+    fake = _AcceptCpu()
+    for mod in (arguments, paged, rotary):
+        monkeypatch.setattr(mod, "get_device_backend", lambda: fake)
+
+
+def _rotary_args(B=2, S=5, H=4, Hkv=2, D=8, dtype=torch.float32):
+    return torch.randn(B, S, H, D).to(dtype), torch.randn(B, S, Hkv, D).to(dtype)
+
+
+@pytest.mark.parametrize("cls, names", [(RotaryEmbeddingFwdOp, "q"), (RotaryEmbeddingBwdOp, "dq")])
+def test_rotary_refusals(cls, names, accept_cpu):
+    op = cls(2, 5, 4, 2, 8, dtype=torch.float32)
+    q, k = _rotary_args()
+    with pytest.raises(ValueError, match="must be on a cuda device"):  # all checks passed
+        op(q, k)
+    with pytest.raises(ValueError, match=rf"Expected {names}.shape \(2, 5, 4, 8\)"):
+        op(q[:, :4], k)
+    with pytest.raises(ValueError, match=rf"Expected {names}.dtype"):
+        op(q.half(), k)
+    with pytest.raises(ValueError, match="shape"):
+        op(q, q)
+    with pytest.raises(ValueError, match="must be a cuda tensor"):
+        op(q, None)
+    with pytest.raises(ValueError, match="must be a cuda tensor"):
+        op(q.tolist(), k)
+    for at, match in ((torch.zeros(4, dtype=torch.int32), "positions.shape"),
+                      (torch.zeros(5, 2, dtype=torch.int32), "positions.shape"),
+                      (torch.zeros(5), "int32 or int64"), ([0] * 5, "must be a cuda tensor")):
+        with pytest.raises(ValueError, match=match):
+            op(q, k, at)
+
+
+def test_rotary_in_place_refusals(accept_cpu):
+    op = RotaryEmbeddingFwdOp(2, 5, 4, 4, 8, dtype=torch.float32, inplace=True)
+    q, k = _rotary_args(Hkv=4)
+    with pytest.raises(ValueError, match="share memory"):
+        op(q[:1].expand(2, 5, 4, 8), k)
+    with pytest.raises(ValueError, match="contiguous channels"):
+        op(torch.randn(2, 5, 8, 4).transpose(2, 3), k)
+    with pytest.raises(ValueError, match="q and k share memory"):
+        op(q, q)
+    with pytest.raises(ValueError, match="must be on a cuda device"):
+        op(q, k)
+
+
+@pytest.mark.parametrize("cls", [RotaryEmbeddingFwdOp, RotaryEmbeddingBwdOp])
+def test_rotary_rejects_sizes_and_types_at_construction(cls):
+    with pytest.raises(ValueError, match="only supports dtypes"):
+        cls(1, 4, 2, 2, 8, dtype=torch.float64)
+    with pytest.raises(ValueError, match="rotary_dim"):
+        cls(1, 4, 2, 2, 8, rotary_dim=7)
+    with pytest.raises(ValueError, match="rotary_dim"):
+        cls(1, 4, 2, 2, 8, rotary_dim=10)
+    with pytest.raises(ValueError, match="rotary_dim"):
+        cls(1, 4, 2, 2, 512)
+    with pytest.raises(ValueError, match="frequencies must have"):
+        cls(1, 4, 2, 2, 8, frequencies=[1.0] * 3)
+    for f in (math.nan, math.inf, 1e20):
+        with pytest.raises(ValueError, match="frequencies must be finite"):
+            cls(1, 4, 2, 2, 8, frequencies=[1.0, 1.0, 1.0, f])
+    for amplitude in (math.nan, math.inf, 1e39):
+        with pytest.raises(ValueError, match="amplitude"):
+            cls(1, 4, 2, 2, 8, amplitude=amplitude)
+    for size in ((-1, 4, 2, 2, 8), (1, -1, 2, 2, 8), (1, 4, -1, 2, 8), (1, 4, 2, 5000, 8),
+                 (1, 4, 2, 2, 0), (1, 4, 2, 2, 5000), (2**31, 1, 1, 1, 8), (2**16, 2**15, 1, 1, 8)):
+        with pytest.raises(ValueError, match="supports"):
+            cls(*size, rotary_dim=0)
+
+
+def test_rejects_cpu_tensors():
+    q, k = _rotary_args()
+    with pytest.raises(ValueError, match="q must be a cuda tensor"):
+        RotaryEmbeddingFwdOp(2, 5, 4, 2, 8, dtype=torch.float32)(q, k)
+    with pytest.raises(ValueError, match="dq must be a cuda tensor"):
+        RotaryEmbeddingBwdOp(2, 5, 4, 2, 8, dtype=torch.float32)(q, k)
+    c = torch.zeros(3, 4, 2, 8)
+    table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="k must be a cuda tensor"):
+        PagedKVAppendOp(2, 8, 4, dtype=torch.float32)(k[:, 0], k[:, 0], c, c, table, lens)
+    with pytest.raises(ValueError, match="q must be a cuda tensor"):
+        PagedAttentionDecodeOp(4, 2, 8, 4, dtype=torch.float16)(q[:, 0].half(), c, c, table, lens)
+
+
+def _paged(dtype, B=2, H=4, Hkv=2, D=8, P=4, pages=3):
+    c = torch.zeros(2, pages, P, Hkv, D, dtype=dtype)
+    return dict(k=torch.zeros(B, Hkv, D, dtype=dtype), v=torch.zeros(B, Hkv, D, dtype=dtype),
+                q=torch.zeros(B, H, D, dtype=dtype), k_cache=c[0], v_cache=c[1],
+                page_table=torch.zeros(B, 3, dtype=torch.int32),
+                seq_lens=torch.ones(B, dtype=torch.int32))
+
+
+COMMON = [
+    (dict(k_cache=torch.zeros(3, 4, 2, 8)[..., :4]), "k_cache.shape"),
+    (dict(k_cache=torch.zeros(3, 4, 16)), "k_cache must have 4 dimensions"),
+    (dict(v_cache=torch.zeros(2, 4, 2, 8)), "v_cache.shape"),
+    (dict(v_cache=torch.zeros(3, 4, 2, 8, dtype=torch.float64)), "v_cache.dtype"),
+    (dict(k_cache=torch.zeros(0, 4, 2, 8), v_cache=torch.zeros(0, 4, 2, 8)), "between 1 and"),
+    (dict(page_table=torch.zeros(3, 3, dtype=torch.int32)), "page_table.shape"),
+    (dict(page_table=torch.zeros(2, 3, dtype=torch.int64)), "page_table.dtype"),
+    (dict(page_table=torch.zeros(6, dtype=torch.int32)), "page_table must have 2 dimensions"),
+    (dict(page_table=None), "page_table must be a cuda tensor"),
+    (dict(seq_lens=torch.ones(3, dtype=torch.int32)), "seq_lens.shape"),
+    (dict(seq_lens=torch.ones(2, dtype=torch.int64)), "seq_lens.dtype"),
+    (dict(seq_lens=[1, 1]), "seq_lens must be a cuda tensor"),
+]
+
+
+def _cast(change, dtype):
+    return {k: v.to(dtype) if isinstance(v, torch.Tensor) and v.dtype is torch.float32 else v
+            for k, v in change.items()}
+
+
+@pytest.mark.parametrize("change, match", COMMON + [
+    (dict(k=torch.zeros(2, 3, 8)), "k.shape"), (dict(v=torch.zeros(3, 2, 8)), "v.shape"),
+    (dict(v=torch.zeros(2, 2, 8, dtype=torch.float64)), "v.dtype"), (dict(k=torch.zeros(2, 16)), "k must be"),
+    (dict(q=torch.zeros(2, 3, 8)), "q.shape"), (dict(q=torch.zeros(3, 4, 8)), "q.shape"),
+    (dict(cu_seqlens=torch.tensor([0, 2])), "cu_seqlens.dtype"),
+    (dict(cu_seqlens=torch.tensor([[0, 1, 2]], dtype=torch.int32)), "cu_seqlens.shape"),
+    (dict(cu_seqlens=torch.zeros(0, dtype=torch.int32)), "at least one offset"),
+    (dict(cu_seqlens=torch.tensor([0, 2], dtype=torch.int32)), "page_table.shape"),
+    (dict(cu_seqlens=[0, 1, 2]), "cu_seqlens must be a cuda tensor"),
+    (dict(k=torch.zeros(2, 1, 2, 8), v=torch.zeros(2, 1, 2, 8), q=None,
+          cu_seqlens=torch.tensor([0, 1, 2], dtype=torch.int32)), "must be packed"),
+    (dict(k_cache=torch.zeros(1, 4, 2, 8).expand(3, 4, 2, 8)), "share memory"),
+    (dict(v_cache=torch.zeros(3, 4, 8, 2).transpose(2, 3)), "contiguous channels"),
+])
+def test_append_refusals(change, match, accept_cpu):
+    op = PagedKVAppendOp(2, 8, 4, 4, 8, dtype=torch.float32)
+    args = _paged(torch.float32)
+    with pytest.raises(ValueError, match="must be on a cuda device"):
+        op(**args)
+    with pytest.raises(ValueError, match=match):
+        op(**{**args, **change})
+
+
+@pytest.mark.parametrize("change, match", COMMON + [
+    (dict(q=torch.zeros(2, 3, 8)), "q.shape"), (dict(q=torch.zeros(2, 4, 1, 8)), "q.shape"),
+    (dict(q=torch.zeros(2, 4, 8, dtype=torch.float64)), "q.dtype"), (dict(q=None), "q must be a cuda tensor"),
+    (dict(page_table=torch.zeros(2, 1, dtype=torch.int32).expand(2, 2**29)), "at most 2\\^31 - 129"),
+    (dict(k_cache=torch.zeros(3, 4, 2, 12, dtype=torch.float16)[..., :8]), "multiples of 8"),
+    (dict(v_cache=torch.zeros(3, 4, 8, 2).transpose(2, 3)), "contiguous channels"),
+])
+def test_decode_refusals(change, match, accept_cpu):
+    op = PagedAttentionDecodeOp(4, 2, 8, 4, dtype=torch.float16)
+    args = _paged(torch.float16)
+    del args["k"], args["v"]
+    with pytest.raises(ValueError, match="must be on a cuda device"):
+        op(**args)
+    with pytest.raises(ValueError, match=match):
+        op(**{**args, **_cast(change, torch.float16)})
+
+
+def test_paged_ops_reject_sizes_and_types_at_construction():
+    for bad in (dict(heads_kv=0), dict(dim=0), dict(page_size=0), dict(heads=-1), dict(dim=5000),
+                dict(rotary_dim=10), dict(rotary_dim=3), dict(frequencies=[1.0]),
+                dict(dtype=torch.int32), dict(amplitude=math.nan)):
+        with pytest.raises(ValueError):
+            PagedKVAppendOp(**{**dict(heads_kv=2, dim=8, page_size=4), **bad})
+    for bad in (dict(heads=3), dict(heads_kv=0), dict(dim=12), dict(dim=264), dict(dim=0),
+                dict(page_size=0), dict(page_size=2**31), dict(scale=math.inf), dict(scale=math.nan),
+                dict(window=0), dict(window=-1), dict(window=2**31), dict(dtype=torch.float32),
+                dict(heads=8192, heads_kv=1)):
+        with pytest.raises(ValueError):
+            PagedAttentionDecodeOp(**{**dict(heads=4, heads_kv=2, dim=8, page_size=4), **bad})
+
+
+def test_kernel_maps():
+    for op, key, cls in (
+            (RotaryEmbeddingFwdOp(1, 1, 1, 1, 8), "rotary_fwd", RotaryEmbeddingFwdKernel),
+            (RotaryEmbeddingBwdOp(1, 1, 1, 1, 8), "rotary_bwd", RotaryEmbeddingBwdKernel),
+            (PagedKVAppendOp(1, 8, 4), "paged_kv_append", PagedKVAppendKernel),
+            (PagedAttentionDecodeOp(1, 1, 8, 4), "paged_attention_decode", PagedAttentionDecodeKernel)):
+        assert op.default_kernel_map == {key: cls} and type(op.kernel) is cls
+
+
+# ------------------------------------------------------------ C entry points
+def _ints(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def test_rotary_entry_point_checks():
+    fn = _native.lib().tileops_rotary
+    turns = (ctypes.c_uint64 * 128)()
+    s = _ints(*[0] * 12)
+
+    def call(q=SOME, k=SOME, at=NULL, out=SOME, t=turns, B=1, S=4, H=2, Hkv=1, D=8, R=8, st=s, at_type=7,
+             dtype=2):
+        return fn(q, k, at, out, out, t, B, S, H, Hkv, D, R, st, 0, at_type, 0, 0, 1.0, dtype, NULL)
+
+    for bad in (dict(B=-1), dict(S=-1), dict(H=-1), dict(H=5000), dict(D=0), dict(D=5000), dict(R=7),
+                dict(R=10), dict(R=-2), dict(D=512, R=258), dict(B=2**16, S=2**15)):
+        assert call(**bad) == _native.EBADSHAPE, bad
+    assert call(dtype=7) == _native.EBADDTYPE and call(at=SOME, at_type=0) == _native.EBADDTYPE
+    for bad in (dict(q=NULL), dict(k=NULL), dict(out=NULL), dict(st=None), dict(t=None)):
+        assert call(**bad) == _native.EINVAL, bad
+    assert call(q=NULL, k=NULL, B=0) == _native.OK and call(q=NULL, k=NULL, H=0, Hkv=0) == _native.OK
+
+
+def test_append_entry_point_checks():
+    fn = _native.lib().tileops_paged_kv_append
+    turns = (ctypes.c_uint64 * 128)()
+    s = _ints(*[0] * 18)
+
+    def call(q=SOME, k=SOME, v=SOME, c=SOME, table=SOME, lens=SOME, cu=NULL, t=turns, N=2, T=4, H=2,
+             Hkv=1, D=8, R=8, pages=3, P=4, width=2, st=s, dtype=2):
+        return fn(q, k, v, q, c, c, table, lens, cu, t, N, T, H, Hkv, D, R, pages, P, width, width, st,
+                  0, 1.0, dtype, NULL)
+
+    for bad in (dict(N=-1), dict(T=-1), dict(T=5), dict(N=0), dict(H=-1), dict(Hkv=0), dict(D=0),
+                dict(R=9), dict(pages=-1), dict(pages=2**31), dict(P=0), dict(P=2**31), dict(width=-1)):
+        assert call(**bad) == _native.EBADSHAPE, bad
+    assert call(dtype=3) == _native.EBADDTYPE
+    for bad in (dict(q=NULL), dict(k=NULL), dict(v=NULL), dict(c=NULL), dict(table=NULL), dict(lens=NULL),
+                dict(t=None), dict(st=None)):
+        assert call(**bad) == _native.EINVAL, bad
+    assert call(q=NULL, k=NULL, N=0, T=0) == _native.OK
+
+
+def test_decode_entry_point_checks():
+    lib = _native.lib()
+    fn = lib.tileops_paged_decode_fwd
+
+    def call(q=SOME, c=SOME, table=SOME, lens=SOME, out=SOME, ws=SOME, B=2, H=4, Hkv=2, D=8, pages=3, P=4,
+             width=2, st=_ints(*[8] * 8), window=0, dtype=2):
+        return fn(q, c, c, table, lens, out, out, ws, B, H, Hkv, D, pages, P, width, width, st, window,
+                  1.0, dtype, NULL)
+
+    for bad in (dict(B=-1), dict(H=3), dict(H=0), dict(Hkv=0), dict(D=12), dict(D=264), dict(D=0),
+                dict(pages=-1), dict(P=0), dict(P=2**30, width=2), dict(width=-1), dict(window=-1)):
+        assert call(**bad) == _native.EBADSHAPE, bad
+    # 2^31 and more units of 64 tokens
+    assert call(B=2**20, H=32, Hkv=32, P=64, width=2**10) == _native.EBADSHAPE
+    assert call(dtype=0) == _native.EBADDTYPE and call(dtype=7) == _native.EBADDTYPE
+    for bad in (dict(q=NULL), dict(c=NULL), dict(table=NULL), dict(lens=NULL), dict(out=NULL),
+                dict(ws=NULL), dict(st=None)):
+        assert call(**bad) == _native.EINVAL, bad
+    off = ctypes.c_void_p((1 << 20) + 8)
+    for bad in (dict(q=off), dict(c=off), dict(ws=off), dict(st=_ints(*[8] * 7, 4))):
+        assert call(**bad) == _native.EALIGN, bad
+    assert call(q=NULL, c=NULL, B=0) == _native.OK
+    assert lib.tileops_paged_decode_workspace_bytes(4, 3, 8) == -1
+    assert lib.tileops_paged_decode_workspace_bytes(4, 2, 12) == -1
+    # counters, then (exponent, sum) and sums of 2 x 16 rows for each of 296 CTAs
+    assert lib.tileops_paged_decode_workspace_bytes(4, 2, 64) == 296 * 4 + 296 * 2 * 16 * (2 + 64) * 4
+    assert lib.tileops_paged_decode_workspace_bytes(32, 1, 64) == 296 * 4 + 296 * 2 * 32 * (2 + 64) * 4
+
+
+# ------------------------------------------------------------ formulas, manifest
+def test_rooflines():
+    assert RotaryEmbeddingFwdOp(2, 10, 4, 2, 64, 32).eval_roofline() == (
+        3 * 20 * 6 * 32, 2 * 20 * 6 * 64 * 2)
+    assert RotaryEmbeddingBwdOp(2, 10, 4, 2, 64, dtype=torch.float32).eval_roofline() == (
+        3 * 20 * 6 * 64, 2 * 20 * 6 * 64 * 4)
+    op = PagedKVAppendOp(2, 64, 16, 4, 64)
+    assert op.eval_roofline() == (0, 0)
+    op._last = (7, 2, 64), True
+    assert op.eval_roofline() == (3 * 7 * 6 * 64, 2 * 7 * 8 * 64 * 2)
+    op._last = (3, 7, 2, 64), False
+    assert op.eval_roofline() == (3 * 21 * 2 * 64, 2 * 21 * 4 * 64 * 2)
+    op = PagedAttentionDecodeOp(8, 2, 64, 16)
+    op._last = (3, 5)
+    assert op.eval_roofline() == (4 * 3 * 8 * 64 * 80, (2 * 3 * 80 * 2 * 64 + 2 * 3 * 8 * 64) * 2 + 4 * 24)
+    op = PagedAttentionDecodeOp(8, 2, 64, 16, window=10)
+    op._last = (3, 5)
+    assert op.eval_roofline()[0] == 4 * 3 * 8 * 64 * 10
+
+
+def test_manifest_has_the_serving_ops():
+    for row in load_workloads("RotaryEmbeddingFwdOp") + load_workloads("RotaryEmbeddingBwdOp"):
+        RotaryEmbeddingFwdOp(row["batch"], row["seq_len"], row["heads"], row["heads_kv"], row["dim"],
+                             row.get("rotary_dim"))
+    for row in load_workloads("PagedKVAppendOp"):
+        PagedKVAppendOp(row["heads_kv"], row["dim"], row["page_size"], row["heads"], row["rotary_dim"])
+    for row in load_workloads("PagedAttentionDecodeOp"):
+        PagedAttentionDecodeOp(row["heads"], row["heads_kv"], row["dim"], row["page_size"],
+                               window=row.get("window"))
+
+
+def test_ops_are_rebuilt_from_their_attributes():
+    f = rotary_frequencies(32, factor=2.0)
+    for op in (RotaryEmbeddingFwdOp(2, 10, 4, 2, 64, 32, True, f, 1.5, torch.float16, True),
+               PagedKVAppendOp(2, 64, 16, 4, 32, True, f, 1.5, torch.float16),
+               PagedAttentionDecodeOp(8, 2, 64, 16, 0.3, 100, torch.float16)):
+        again = type(op)(**_extract_op_init_args(op))
+        assert _extract_op_init_args(again) == _extract_op_init_args(op)
+        assert len(_extract_op_init_args(op)) >= 7

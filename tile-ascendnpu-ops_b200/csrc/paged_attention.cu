@@ -30,6 +30,7 @@
 // meanwhile.  Tokens outside the sequence are copied as zeros (size 0), never read: infinities
 // and NaN behind a sequence's end have no say.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -647,19 +648,34 @@ bool bad_sizes(int64_t batch, int64_t heads, int64_t heads_kv, int64_t dim) {
          heads % heads_kv != 0 || dim < 8 || dim > 256 || dim % 8 != 0;
 }
 
+// Places of a call at most: of sequences as long as the table has room for.
+int64_t places_of(const DecodeArgs& a, int unit) {
+  const int64_t seen = a.window ? std::min(a.room, a.window) : a.room;
+  return (std::max<int64_t>(1, (seen + unit - 1) / unit) + 1) * a.batch * (a.heads_kv * a.blocks);
+}
+
+// Lets the kernel have its shared memory, once on each device (0.5 us a call otherwise).
+template <typename T, int DP, int MT, int WARPS>
+bool opt_in() {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(paged_decode<T, DP, MT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(Layout<DP, MT, WARPS>::kBytes)) != cudaSuccess)
+    return false;
+  done.fetch_or(bit, std::memory_order_release);
+  return true;
+}
+
 template <typename T, int DP, int MT, int WARPS>
 int launch_tile(const DecodeArgs& a, cudaStream_t s) {
   using L = Layout<DP, MT, WARPS>;
-  if (cudaFuncSetAttribute(paged_decode<T, DP, MT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(L::kBytes)) != cudaSuccess)
-    return TILEOPS_ELAUNCH;
-  // No more CTAs than there can be units.
-  const int64_t seen = a.window ? std::min(a.room, a.window) : a.room;
-  const int64_t units = std::max<int64_t>(1, (seen + L::kUnit - 1) / L::kUnit);
-  const int64_t places = (units + 1) * a.batch * (a.heads_kv * a.blocks);
-  if (places > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
-  const int64_t grid =
-      std::min<int64_t>({places, static_cast<int64_t>(sm_count()) * L::kCtasSm, kMaxCtas});
+  // No more CTAs than there can be places.
+  const int64_t grid = std::min<int64_t>(
+      {places_of(a, L::kUnit), static_cast<int64_t>(sm_count()) * L::kCtasSm, kMaxCtas});
+  if (!opt_in<T, DP, MT, WARPS>()) return TILEOPS_ELAUNCH;
   clear_counters<<<1, kMaxCtas, 0, s>>>(a.counters);
   if (int status = launch_status()) return status;
   // Starts once the first kernel has started, and so behind all that came before that one; the
@@ -765,6 +781,7 @@ extern "C" int tileops_paged_decode_fwd(
   a.partial = reinterpret_cast<float*>(a.stats + static_cast<int64_t>(kMaxCtas) * 2 * rows);
   a.div_page = FastDivU32(static_cast<uint32_t>(page_size));
   a.scale = static_cast<float>(scale * 1.4426950408889634);
+  if (places_of(a, 4 * kWarpTokens) > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
   a.err = device_error_ptr();
   cudaStream_t s = as_stream(stream);
   return dtype == TILEOPS_DT_F16 ? launch_type<__half>(a, s) : launch_type<__nv_bfloat16>(a, s);

@@ -55,11 +55,10 @@ class _RotaryEmbeddingKernel(Kernel):
                  config: Optional[dict] = None):
         super().__init__()
         check_dtype(self, dtype, self.SUPPORTED_DTYPES)
-        if (min(batch, seq_len, heads, heads_kv) < 0 or max(batch, seq_len) > 2**31 - 1
+        if (min(batch, seq_len, heads, heads_kv) < 0 or max(batch, seq_len, batch * seq_len) >= 2**31
                 or max(heads, heads_kv) > 4096 or not 1 <= dim <= 4096):
-            raise ValueError(f"{type(self).__name__} supports batch and seq_len below 2^31, up to "
-                             f"4096 heads and dim 1..4096, got ({batch}, {seq_len}, {heads}, "
-                             f"{heads_kv}, {dim})")
+            raise ValueError(f"{type(self).__name__} supports fewer than 2^31 tokens, up to 4096 heads "
+                             f"and dim 1..4096, got ({batch}, {seq_len}, {heads}, {heads_kv}, {dim})")
         check_rotation(type(self).__name__, dim, rotary_dim, frequencies, amplitude)
         self.batch, self.seq_len, self.heads, self.heads_kv = batch, seq_len, heads, heads_kv
         self.dim, self.rotary_dim, self.interleaved = dim, rotary_dim, bool(interleaved)

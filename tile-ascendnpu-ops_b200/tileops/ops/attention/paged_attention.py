@@ -166,7 +166,7 @@ class PagedAttentionDecodeOp(Op):
                  dtype: torch.dtype = torch.bfloat16,
                  kernel_map: Optional[Dict[str, Kernel]] = None) -> None:
         self.heads, self.heads_kv, self.dim, self.page_size = heads, heads_kv, dim, page_size
-        self.scale = dim**-0.5 if scale is None else scale
+        self.scale = max(dim, 1)**-0.5 if scale is None else scale  # dim is checked by the kernel
         if window is not None and window < 1:
             raise ValueError(f"window must be at least 1 token, got {window}")
         self.window = window
