@@ -419,9 +419,9 @@ def test_decode_entry_point_checks():
     assert call(q=NULL, c=NULL, B=0) == _native.OK
     assert lib.tileops_paged_decode_workspace_bytes(4, 3, 8) == -1
     assert lib.tileops_paged_decode_workspace_bytes(4, 2, 12) == -1
-    # counters, then (exponent, sum) and sums of 2 x 16 rows for each of 296 CTAs
-    assert lib.tileops_paged_decode_workspace_bytes(4, 2, 64) == 296 * 4 + 296 * 2 * 16 * (2 + 64) * 4
-    assert lib.tileops_paged_decode_workspace_bytes(32, 1, 64) == 296 * 4 + 296 * 2 * 32 * (2 + 64) * 4
+    # counters, then (exponent, sum) and sums of 2 x 2 rows for each of 592 CTAs
+    assert lib.tileops_paged_decode_workspace_bytes(4, 2, 64) == 592 * 4 + 592 * 2 * 2 * (2 + 64) * 4
+    assert lib.tileops_paged_decode_workspace_bytes(32, 1, 72) == 592 * 4 + 592 * 2 * 32 * (2 + 80) * 4
 
 
 # ------------------------------------------------------------ formulas, manifest

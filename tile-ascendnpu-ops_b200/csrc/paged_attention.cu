@@ -39,8 +39,7 @@
 namespace tileops {
 namespace {
 
-constexpr int kWarpTokens = 16;
-constexpr int kMaxCtas = 2 * 148;  // two on each of a B200's SMs
+constexpr int kMaxCtas = 4 * 148;  // four on each of a B200's SMs
 constexpr float kNegInf = -__builtin_huge_valf();
 
 struct CacheStrides {
@@ -54,11 +53,14 @@ struct DecodeArgs {
   float* lse;
   int* counters;    // [CTA]: how many CTAs have written their sums of the item that it begins
   float2* stats;    // [CTA][2][row]: exponent the sums are relative to, sum of weights
-  float* partial;   // [CTA][2][row][D]: weighted sums
+  // [CTA][2][row][D, of 16 channels each]: weighted sums, of 16 channels the four of a lane's fragment
+  // together (2 t, 2 t + 1, 8 + 2 t, 9 + 2 t), so that they are read by 16 bytes.
+  float* partial;
   int64_t q_b, q_h;
   CacheStrides ks, vs;
   int64_t table_stride, num_pages;
   int batch, heads, heads_kv, group, dim, page_size, window, blocks;  // blocks of rows a key head
+  int part_rows, part_dim;  // rows of an item, at most; D rounded up to 16
   int room;  // tokens that a row of the table has pages for
   FastDivU32 div_page{1};
   float scale;  // log2(e) times the scale
@@ -186,18 +188,21 @@ struct Looked {
   Unit u;
   uint32_t place;
   bool last;               // the CTA's last one
-  int page[kWarpTokens];   // of the warp's tokens in it, where they are inside the sequence
+  int page[32];            // of the warp's tokens in it, where they are inside the sequence
 };
 
 template <int DP, int MT, int WARPS>
 struct Layout {
   static constexpr int kChunks = DP / 8;                       // 16-byte chunks of a row
   static constexpr int kRow = (DP + 63) / 64 * 64;             // elements of a row in shared memory
-  static constexpr int kStages = DP <= 64 ? 6 : DP <= 128 ? 3 : DP <= 192 ? 4 : 3;
-  static constexpr int kCtasSm = DP <= 128 && WARPS == 4 ? 2 : 1;
-  static constexpr int kUnit = WARPS * kWarpTokens;
+  // Tokens of a warp in a unit: 8 KB of keys and values and more, for what a unit costs besides.
+  static constexpr int kTokens = DP <= 64 ? 32 : 16;
+  static constexpr int kStages = DP <= 128 ? 3 : DP <= 192 ? (WARPS == 4 ? 4 : 2) : (WARPS == 4 ? 3 : 2);
+  static constexpr int kCtasSm =
+      WARPS == 8 ? 1 : WARPS == 4 ? (DP <= 128 ? 2 : 1) : DP <= 192 ? 4 : 3;
+  static constexpr int kUnit = WARPS * kTokens;
   static constexpr int kThreads = WARPS * 32;
-  static constexpr int kTile = kWarpTokens * kRow;             // elements of a warp's keys (or values)
+  static constexpr int kTile = kTokens * kRow;                 // elements of a warp's keys (or values)
   static constexpr int kRows = 16 * MT;
   static constexpr size_t kRing = static_cast<size_t>(WARPS) * kStages * 2 * kTile * 2;
   static constexpr size_t kQ = static_cast<size_t>(kRows) * kRow * 2;
@@ -307,7 +312,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     return;
   }
 
-  // The rows of an item, zeros behind them: fetched while the item before is joined.
+  // The rows of an item, zeros behind them: fetched while the last unit of the item before is multiplied.
   constexpr int kQChunks = (L::kRows * L::kChunks + kThreads - 1) / kThreads;
   uint4 q_next[kQChunks];
   auto fetch_q = [&](const Unit& at) {
@@ -341,8 +346,8 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     if (look.place >= u1) {
       u.b = -1;
     } else {
-      const int t = u.span.begin + u.unit * kUnit + warp * kWarpTokens + lane;
-      if (lane < kWarpTokens && t < u.span.end)
+      const int t = u.span.begin + u.unit * kUnit + warp * L::kTokens + lane;
+      if (lane < L::kTokens && t < u.span.end)
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(&w.page[lane])),
                      "l"(a.table + u.b * a.table_stride + a.div_page.div(t))
                      : "memory");
@@ -358,12 +363,12 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     const Looked& w = ahead[slot];
     const Unit u = w.u;
     if (u.b < 0) return;
-    const int t = u.span.begin + u.unit * kUnit + warp * kWarpTokens + lane;
+    const int t = u.span.begin + u.unit * kUnit + warp * L::kTokens + lane;
     const int head = u.head / a.blocks;
     const T* k = static_cast<const T*>(a.k) + head * a.ks.head;
     const T* v = static_cast<const T*>(a.v) + head * a.vs.head;
     int64_t k_at = 0, v_at = 0;
-    bool inside = lane < kWarpTokens && t < u.span.end;
+    bool inside = lane < L::kTokens && t < u.span.end;
     if (inside) {
       const int page = w.page[lane];
       if (page >= 0 && page < a.num_pages) {
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     const uint32_t rows = __ballot_sync(~0u, inside);
     const uint32_t to = ring + stage * (2 * L::kTile * 2);
 #pragma unroll
-    for (int i = 0; i < kWarpTokens * L::kChunks / 32; ++i) {
+    for (int i = 0; i < L::kTokens * L::kChunks / 32; ++i) {
       const int row = (i * 32 + lane) / L::kChunks, chunk = (i * 32 + lane) % L::kChunks;
       const bool there = ((rows >> row) & 1) && chunk * 8 < a.dim;
       const int64_t ka = __shfl_sync(~0u, k_at, row), va = __shfl_sync(~0u, v_at, row);
@@ -426,33 +431,40 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     __syncwarp();
     const Unit get = ahead[slot].u;
     const bool last = ahead[slot].last;
+    const bool ended = get.unit + 1 == get.span.units;
+    if (ended && !last) fetch_q(ahead[slot + 1 == L::kAhead ? 0 : slot + 1].u);
     const uint32_t keys = ring + stage * (2 * L::kTile * 2), values = keys + L::kTile * 2;
-    const int t0 = get.span.begin + get.unit * kUnit + warp * kWarpTokens;
+    const int t0 = get.span.begin + get.unit * kUnit + warp * L::kTokens;
     if (t0 < get.span.end) {
-      float s[MT][2][4];
+      constexpr int kBlocks = L::kTokens / 16;
+      float s[MT][2 * kBlocks][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2 * kBlocks; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[m][n][e] = 0.0f;
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
-        uint32_t kb[4];
-        ldsm(keys + L::at((lane & 7) + ((lane >> 4) << 3), k * 2 + ((lane >> 3) & 1)), kb);
+        uint32_t qa[MT][4];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          uint32_t qa[4];
-          ldsm(q_at + L::at(m * 16 + (lane & 15), k * 2 + (lane >> 4)), qa);
-          mma<T>(s[m][0], qa, kb[0], kb[1]);
-          mma<T>(s[m][1], qa, kb[2], kb[3]);
+        for (int m = 0; m < MT; ++m) ldsm(q_at + L::at(m * 16 + (lane & 15), k * 2 + (lane >> 4)), qa[m]);
+#pragma unroll
+        for (int t = 0; t < kBlocks; ++t) {
+          uint32_t kb[4];
+          ldsm(keys + L::at(t * 16 + (lane & 7) + ((lane >> 4) << 3), k * 2 + ((lane >> 3) & 1)), kb);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma<T>(s[m][2 * t], qa[m], kb[0], kb[1]);
+            mma<T>(s[m][2 * t + 1], qa[m], kb[2], kb[3]);
+          }
         }
       }
-      uint32_t w[MT][4];
+      uint32_t w[MT][kBlocks][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2 * kBlocks; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = t0 + n * 8 + (lane & 3) * 2 + (e & 1);
@@ -460,8 +472,10 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
           }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {  // rows lane / 4 and lane / 4 + 8
-          float (&x)[4] = s[m][0], (&y)[4] = s[m][1];
-          float high = fmaxf(fmaxf(x[2 * r], x[2 * r + 1]), fmaxf(y[2 * r], y[2 * r + 1]));
+          float high = kNegInf;
+#pragma unroll
+          for (int n = 0; n < 2 * kBlocks; ++n)
+            high = fmaxf(high, fmaxf(s[m][n][2 * r], s[m][n][2 * r + 1]));
           high = fmaxf(high, __shfl_xor_sync(~0u, high, 1));
           high = fmaxf(high, __shfl_xor_sync(~0u, high, 2));
           const float top_new = fmaxf(high - kShift<T>, top[m][r]);
@@ -469,13 +483,15 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
           const float base = top_new == kNegInf ? 0.0f : top_new;
           const float fade = ex2_approx_f(top[m][r] - base);
           top[m][r] = top_new;
-          x[2 * r] = ex2_approx_f(x[2 * r] - base);
-          x[2 * r + 1] = ex2_approx_f(x[2 * r + 1] - base);
-          y[2 * r] = ex2_approx_f(y[2 * r] - base);
-          y[2 * r + 1] = ex2_approx_f(y[2 * r + 1] - base);
-          sum[m][r] = sum[m][r] * fade + ((x[2 * r] + x[2 * r + 1]) + (y[2 * r] + y[2 * r + 1]));
-          w[m][r] = pack2<T>(x[2 * r], x[2 * r + 1]);
-          w[m][2 + r] = pack2<T>(y[2 * r], y[2 * r + 1]);
+          float add = 0.0f;
+#pragma unroll
+          for (int n = 0; n < 2 * kBlocks; ++n) {
+            const float w0 = ex2_approx_f(s[m][n][2 * r] - base);
+            const float w1 = ex2_approx_f(s[m][n][2 * r + 1] - base);
+            add += w0 + w1;
+            w[m][n / 2][n % 2 * 2 + r] = pack2<T>(w0, w1);
+          }
+          sum[m][r] = sum[m][r] * fade + add;
           if (__any_sync(~0u, fade != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n) {
@@ -487,20 +503,21 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
       }
 #pragma unroll
       for (int n = 0; n < DP / 16; ++n) {
-        uint32_t vb[4];
-        ldsm_t(values + L::at(lane & 15, n * 2 + (lane >> 4)), vb);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          mma<T>(out[m][2 * n], w[m], vb[0], vb[1]);
-          mma<T>(out[m][2 * n + 1], w[m], vb[2], vb[3]);
+        for (int t = 0; t < kBlocks; ++t) {
+          uint32_t vb[4];
+          ldsm_t(values + L::at(t * 16 + (lane & 15), n * 2 + (lane >> 4)), vb);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma<T>(out[m][2 * n], w[m][t], vb[0], vb[1]);
+            mma<T>(out[m][2 * n + 1], w[m][t], vb[2], vb[3]);
+          }
         }
       }
     }
-    const bool ended = get.unit + 1 == get.span.units;
     if (ended || last) {
       // ---- the warps' sums of the item, joined through the stage just used ----
       bool whole = began && ended;
-      if (!last) fetch_q(ahead[slot + 1 == L::kAhead ? 0 : slot + 1].u);
       const int block = get.head % a.blocks;
       const int h0 = (get.head / a.blocks) * a.group + block * L::kRows;
       const int rows = min(L::kRows, a.group - block * L::kRows);
@@ -536,9 +553,12 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
           __syncthreads();
           if (m == 0) store_q();
           for (int n = threadIdx.x; n < min(16, rows - m * 16) * (DP / 4); n += kThreads) {
-            const int r = n / (DP / 4), d = n % (DP / 4) * 4, row = m * 16 + r;
-            if (d >= a.dim) continue;
-            const int col = (d / 8 + (r & 7)) % (DP / 8) * 8 + d % 8;
+            const int r = n / (DP / 4), quad = n % (DP / 4), row = m * 16 + r;
+            // Four channels in a row for o; of a lane's fragment for other CTAs.
+            const int d0 = whole ? quad * 4 : quad / 4 * 16 + quad % 4 * 2, d1 = whole ? d0 + 2 : d0 + 8;
+            if (d0 >= a.dim) continue;
+            auto at_col = [&](int d) { return (d / 8 + (r & 7)) % (DP / 8) * 8 + d % 8; };
+            const int c0 = at_col(d0), c1 = at_col(d1);
             float2 st[WARPS];
             float high = kNegInf;
 #pragma unroll
@@ -552,22 +572,24 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
 #pragma unroll
             for (int x = 0; x < WARPS; ++x) {
               const float f = ex2_approx_f(st[x].x - base);
-              const float4 p = *reinterpret_cast<const float4*>(
-                  smem + (x * L::kStages + stage) * (2 * L::kTile * 2) + (r * kPad + col) * 4);
+              const float* p = reinterpret_cast<const float*>(
+                  smem + (x * L::kStages + stage) * (2 * L::kTile * 2)) + r * kPad;
+              const float2 p0 = *reinterpret_cast<const float2*>(p + c0);
+              const float2 p1 = *reinterpret_cast<const float2*>(p + c1);
               all += f * st[x].y;
-              v.x += f * p.x;
-              v.y += f * p.y;
-              v.z += f * p.z;
-              v.w += f * p.w;
+              v.x += f * p0.x;
+              v.y += f * p0.y;
+              v.z += f * p1.x;
+              v.w += f * p1.y;
             }
             if (whole) {
               const int64_t at = static_cast<int64_t>(get.b) * a.heads + h0 + row;
-              store_row(static_cast<T*>(a.o) + at * a.dim + d, v, all);
-              if (d == 0) a.lse[at] = base + log2f(all);
+              store_row(static_cast<T*>(a.o) + at * a.dim + d0, v, all);
+              if (quad == 0) a.lse[at] = base + log2f(all);
             } else {
-              const int64_t at = (c * 2 + (began ? 1 : 0)) * L::kRows + row;
-              *reinterpret_cast<float4*>(a.partial + at * a.dim + d) = v;
-              if (d == 0) a.stats[at] = make_float2(high, all);
+              const int64_t at = (c * 2 + (began ? 1 : 0)) * a.part_rows + row;
+              *reinterpret_cast<float4*>(a.partial + at * a.part_dim + quad * 4) = v;
+              if (quad == 0) a.stats[at] = make_float2(high, all);
             }
           }
           __syncthreads();
@@ -591,7 +613,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
         reset();
 #pragma unroll 1
         for (uint32_t x = owner + warp; x <= end; x += WARPS) {
-          const int64_t at = (x * 2 + (x == owner)) * L::kRows;
+          const int64_t at = (x * 2 + (x == owner)) * a.part_rows;
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -599,21 +621,24 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
               const int row = m * 16 + r * 8 + lane / 4;
               if (row >= rows) continue;
               const float2 st = __ldcg(a.stats + at + row);
-              const float* p = a.partial + (at + row) * a.dim + (lane & 3) * 2;
-              float2 v[DP / 8];
+              const float* p = a.partial + (at + row) * a.part_dim + (lane & 3) * 4;
+              float4 v[DP / 16];
 #pragma unroll
-              for (int n = 0; n < DP / 8; ++n)
-                v[n] = n * 8 < a.dim ? __ldcg(reinterpret_cast<const float2*>(p + n * 8))
-                                     : make_float2(0.0f, 0.0f);
+              for (int n = 0; n < DP / 16; ++n)
+                v[n] = n * 16 < a.dim ? __ldcg(reinterpret_cast<const float4*>(p + n * 16))
+                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
               const float top_new = fmaxf(top[m][r], st.x);
               const float base = top_new == kNegInf ? 0.0f : top_new;
               const float fade = ex2_approx_f(top[m][r] - base), f = ex2_approx_f(st.x - base);
               top[m][r] = top_new;
               sum[m][r] = sum[m][r] * fade + ((lane & 3) == 0 ? f * st.y : 0.0f);
 #pragma unroll
-              for (int n = 0; n < DP / 8; ++n) {
-                out[m][n][2 * r] = out[m][n][2 * r] * fade + f * v[n].x;
-                out[m][n][2 * r + 1] = out[m][n][2 * r + 1] * fade + f * v[n].y;
+              for (int n = 0; n < DP / 16; ++n) {
+                float(&x)[4] = out[m][2 * n], (&y)[4] = out[m][2 * n + 1];
+                x[2 * r] = x[2 * r] * fade + f * v[n].x;
+                x[2 * r + 1] = x[2 * r + 1] * fade + f * v[n].y;
+                y[2 * r] = y[2 * r] * fade + f * v[n].z;
+                y[2 * r + 1] = y[2 * r + 1] * fade + f * v[n].w;
               }
             }
         }
@@ -634,11 +659,12 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(kMaxCtas) clear_counters(int* counters) {
+__global__ void __launch_bounds__(512) clear_counters(int* counters, int count) {
   asm volatile("griddepcontrol.launch_dependents;");
-  counters[threadIdx.x] = 0;
+  for (int n = threadIdx.x; n < count; n += 512) counters[n] = 0;
 }
 
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 int padded_dim(int64_t dim) {
   return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
 }
@@ -676,7 +702,7 @@ int launch_tile(const DecodeArgs& a, cudaStream_t s) {
   const int64_t grid = std::min<int64_t>(
       {places_of(a, L::kUnit), static_cast<int64_t>(sm_count()) * L::kCtasSm, kMaxCtas});
   if (!opt_in<T, DP, MT, WARPS>()) return TILEOPS_ELAUNCH;
-  clear_counters<<<1, kMaxCtas, 0, s>>>(a.counters);
+  clear_counters<<<1, 512, 0, s>>>(a.counters, static_cast<int>(grid));
   if (int status = launch_status()) return status;
   // Starts once the first kernel has started, and so behind all that came before that one; the
   // CTAs wait for its end before they count.
@@ -697,13 +723,22 @@ int launch_tile(const DecodeArgs& a, cudaStream_t s) {
 
 template <typename T, int DP, int MT>
 int launch_warps(const DecodeArgs& a, cudaStream_t s) {
-  // Few items are shared by many CTAs each: one CTA of 8 warps an SM halves the sums that are joined.
-  // Many items: two CTAs of 4, so that one copies and multiplies while the other joins its warps.
-  if constexpr (DP <= 128) {
-    if (static_cast<int64_t>(a.batch) * a.heads_kv * a.blocks <= sm_count())
-      return launch_tile<T, DP, MT, 8>(a, s);
+  // Few items are shared by many CTAs each: one CTA of 8 warps an SM, so that there are fewer sums to join
+  // (131072 tokens of 8 heads of 128 bf16 93 us, 97 with two CTAs of 4; 256 items 32.6 and 29.1).  Many
+  // items: smaller CTAs, more of them at different points of an item (512 sequences of up to 256 tokens,
+  // 4096 items, four CTAs of 2 warps 43.5 us, two of 4 54.7; 512 items of up to 8192 tokens 85.6 and 84.0).
+  // Heads of 192 have no room for two CTAs of 4, nor heads of 256 for 8 warps.
+  const int64_t items = static_cast<int64_t>(a.batch) * a.heads_kv * a.blocks;
+  if constexpr (DP <= 192) {
+    if (items <= sm_count()) return launch_tile<T, DP, MT, 8>(a, s);
   }
-  return launch_tile<T, DP, MT, 4>(a, s);
+  if constexpr (DP <= 128) {
+    if (items <= 4 * sm_count()) return launch_tile<T, DP, MT, 4>(a, s);
+  }
+  if constexpr (DP > 192) {
+    if (items <= sm_count()) return launch_tile<T, DP, MT, 4>(a, s);
+  }
+  return launch_tile<T, DP, MT, 2>(a, s);
 }
 
 template <typename T>
@@ -729,8 +764,9 @@ using namespace tileops;
 extern "C" int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t heads_kv,
                                                         int64_t dim) {
   if (bad_sizes(1, heads, heads_kv, dim)) return -1;
-  const int rows = rows_of(heads / heads_kv, padded_dim(dim));
-  return kCounterBytes + static_cast<int64_t>(kMaxCtas) * 2 * rows * (dim + 2) * 4;  // stats, sums
+  const int64_t group = heads / heads_kv;
+  const int64_t rows = std::min<int64_t>(group, rows_of(group, padded_dim(dim)));
+  return kCounterBytes + static_cast<int64_t>(kMaxCtas) * 2 * rows * (round16(dim) + 2) * 4;
 }
 
 extern "C" int tileops_paged_decode_fwd(
@@ -777,11 +813,13 @@ extern "C" int tileops_paged_decode_fwd(
   a.window = static_cast<int>(window);
   const int rows = rows_of(a.group, padded_dim(dim));
   a.blocks = (a.group + rows - 1) / rows;
+  a.part_rows = std::min(a.group, rows);
+  a.part_dim = static_cast<int>(round16(dim));
   a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + kCounterBytes);
-  a.partial = reinterpret_cast<float*>(a.stats + static_cast<int64_t>(kMaxCtas) * 2 * rows);
+  a.partial = reinterpret_cast<float*>(a.stats + static_cast<int64_t>(kMaxCtas) * 2 * a.part_rows);
   a.div_page = FastDivU32(static_cast<uint32_t>(page_size));
   a.scale = static_cast<float>(scale * 1.4426950408889634);
-  if (places_of(a, 4 * kWarpTokens) > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
+  if (places_of(a, 32) > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
   a.err = device_error_ptr();
   cudaStream_t s = as_stream(stream);
   return dtype == TILEOPS_DT_F16 ? launch_type<__half>(a, s) : launch_type<__nv_bfloat16>(a, s);
