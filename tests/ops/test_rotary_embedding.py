@@ -26,14 +26,19 @@ def _check(q, k, positions=None, rotary_dim=None, interleaved=False, frequencies
     at = torch.arange(S) if positions is None else positions
     if at.dim() == 1:
         at = at.expand(B, S)
+    k = k if k.shape[2] else None
     for cls, back in ((RotaryEmbeddingFwdOp, False), (RotaryEmbeddingBwdOp, True)):
-        op = cls(B, S, H, k.shape[2], D, rotary_dim, interleaved, frequencies, amplitude, q.dtype,
+        op = cls(B, S, H, 0 if k is None else k.shape[2], D, rotary_dim, interleaved, frequencies, amplitude, q.dtype,
                  inplace)
-        ins = [t.clone(memory_format=torch.preserve_format) if inplace else t for t in (q, k)]
+        ins = [t.clone(memory_format=torch.preserve_format) if inplace and t is not None else t
+               for t in (q, k)]
         got = op(*ins, positions)
         if inplace:
             assert got[0] is ins[0] and got[1] is ins[1]
         for name, g, t in zip("qk", got, (q, k)):
+            if t is None:
+                assert g is None
+                continue
             assert g.dtype == t.dtype and (inplace or g.is_contiguous())
             assert_within(g, *ref.rotate(t, at, f, amplitude, interleaved, back), name)
             assert torch.equal(g[..., r:], t[..., r:])
@@ -44,15 +49,34 @@ def _check(q, k, positions=None, rotary_dim=None, interleaved=False, frequencies
 @pytest.mark.parametrize("B, S, H, Hkv, D, R", [
     (1, 1, 1, 1, 2, 2), (1, 1, 32, 8, 128, 128), (2, 7, 4, 2, 64, 64), (1, 33, 3, 1, 80, 80),
     (2, 5, 2, 2, 72, 36), (1, 130, 5, 1, 96, 24), (3, 17, 2, 1, 33, 6), (1, 9, 1, 3, 35, 34),
+    (1, 9, 3, 1, 128, 30), (2, 6, 2, 1, 40, 34), (1, 20, 5, 2, 60, 38), (1, 3, 30, 2, 256, 108),
+    (1, 5, 40, 8, 128, 98), (2, 1, 1, 1, 8, 2), (1, 70, 1, 0, 16, 6),
     (2, 3, 40, 1, 256, 256), (1, 11, 2, 1, 576, 64), (5, 4, 1, 1, 40, 20), (1, 6, 2, 2, 64, 0),
 ])
 def test_sizes(B, S, H, Hkv, D, R, interleaved, dtype):
     _check(*_pair(B, S, H, Hkv, D, dtype), rotary_dim=R, interleaved=interleaved)
 
 
-@pytest.mark.parametrize("S, H, D", [(4096, 4, 128), (1500, 33, 64), (700, 128, 128)])
-def test_more_tokens_than_ctas(S, H, D):
-    _check(*_pair(1, S, H, 1, D, torch.bfloat16))
+@pytest.mark.parametrize("S, H, D, R", [(4096, 4, 128, 128), (1500, 33, 64, 64), (700, 128, 128, 128),
+                                        (2500, 7, 64, 22), (900, 70, 40, 34), (3000, 1, 16, 2)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_more_tokens_than_ctas(S, H, D, R, interleaved):
+    _check(*_pair(1, S, H, 1, D, torch.bfloat16), rotary_dim=R, interleaved=interleaved)
+
+
+def test_the_same_bits_whatever_the_words():
+    """Dense rows, slices that allow words of 8, 4 and 2 bytes only, and a head with channels to
+    spare (partners through shared memory) are rotated by the same operations."""
+    B, S, H, D = 2, 50, 5, 64
+    for R, interleaved in ((64, False), (64, True), (32, False), (12, False), (22, False), (22, True)):
+        q = torch.randn(B, S, H, D, device="cuda").to(torch.bfloat16)
+        op = RotaryEmbeddingFwdOp(B, S, H, 0, D, R, interleaved)
+        want, _ = op(q, None)
+        for at in (0, 4, 2, 1):
+            wide = torch.empty(B, S, H, D + 8, device="cuda", dtype=torch.bfloat16)
+            t = wide[..., at:at + D]
+            t.copy_(q)
+            assert torch.equal(op(t, None)[0], want), (R, interleaved, at)
 
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])

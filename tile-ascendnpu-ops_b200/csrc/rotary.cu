@@ -43,6 +43,7 @@ struct RotaryArgs {
   int64_t pos_stride;     // from a batch entry to the next
   int pos64;
   uint32_t tokens;        // in all
+  int interleaved;
   int heads, heads_kv, dim, rotary, tile;  // tile: tokens of a CTA
   float amplitude, sign;
   uint32_t per_row, items;  // items of a head, of a token
@@ -159,6 +160,93 @@ __device__ __forceinline__ float2 turn(uint32_t phase, float amplitude) {
   return quarters & 2 ? make_float2(-cq, -sq) : make_float2(cq, sq);
 }
 
+// A thread's row: of q, then k, then v.
+template <typename T, bool PAGED>
+struct Rows {
+  const T* src;
+  T* dst;
+  RowStrides from, to;
+  int kind;  // 0 q, 1 k, 2 v
+  __device__ __forceinline__ Rows(const RotaryArgs& a, int row) {
+    if (row < a.heads) {
+      src = static_cast<const T*>(a.q);
+      dst = static_cast<T*>(a.q_out);
+      from = a.qs;
+      to = a.qo;
+      kind = 0;
+    } else if (!PAGED || row < a.heads + a.heads_kv) {
+      row -= a.heads;
+      src = static_cast<const T*>(a.k);
+      dst = static_cast<T*>(a.k_out);
+      from = a.ks;
+      to = a.ko;
+      kind = 1;
+    } else {
+      row -= a.heads + a.heads_kv;
+      src = static_cast<const T*>(a.v);
+      dst = static_cast<T*>(a.v_out);
+      from = a.vs;
+      to = a.vo;
+      kind = 2;
+    }
+    src += row * from.h;
+    dst += row * to.h;
+  }
+  static __device__ __forceinline__ int64_t place(const RotaryArgs& a, uint32_t token,
+                                                  const RowStrides& s) {
+    const uint32_t b = a.div_seq.div(token);
+    return b * s.b + (token - b * a.div_seq.d) * s.t;
+  }
+  // Where a token's row goes, or NULL; zeroed: a row of padding.
+  __device__ __forceinline__ T* target(const RotaryArgs& a, uint32_t token, const Token& told,
+                                       bool& zeroed) const {
+    zeroed = false;
+    if (PAGED && kind != 0) {
+      if (!(told.kept & 2)) return nullptr;
+      return dst + (kind == 1 ? told.k_at : told.v_at);
+    }
+    if (PAGED) zeroed = !(told.kept & 1);
+    return dst + place(a, token, to);
+  }
+};
+
+// cu_seqlens as a whole, by one CTA.
+__device__ __forceinline__ void check_offsets(const RotaryArgs& a) {
+  bool bad = threadIdx.x == 0 && (a.cu_seqlens[0] != 0 ||
+                                  a.cu_seqlens[a.num_seqs] > static_cast<int64_t>(a.tokens));
+  for (int n = threadIdx.x; n < a.num_seqs; n += blockDim.x)
+    bad |= a.cu_seqlens[n] > a.cu_seqlens[n + 1];
+  if (bad) report_device_error(a.err, kErrBadSeqlens);
+}
+
+// cos and (signed) sin of every pair of a tile's tokens, by the whole CTA, to put(token, pair, cos, sin).
+template <bool PAGED, typename Put>
+__device__ __forceinline__ void make_angles(const RotaryArgs& a, uint32_t token0, int ntok,
+                                            Token* told, Put put) {
+  if (PAGED) {
+    if (threadIdx.x < ntok) told[threadIdx.x] = appended_token(a, token0 + threadIdx.x);
+    if (a.cu_seqlens && blockIdx.x == 0) check_offsets(a);
+    __syncthreads();
+  }
+  const int pairs = a.rotary / 2;
+  for (int n = threadIdx.x; n < ntok * pairs; n += blockDim.x) {
+    const int at = n / pairs, i = n - at * pairs;
+    int64_t position;
+    if (PAGED) {
+      position = told[at].position;
+    } else {
+      const uint32_t b = a.div_seq.div(token0 + at), t = token0 + at - b * a.div_seq.d;
+      const int64_t place = b * a.pos_stride + t;
+      position = !a.positions ? t
+                 : a.pos64    ? static_cast<const int64_t*>(a.positions)[place]
+                              : static_cast<const int32_t*>(a.positions)[place];
+    }
+    const float2 w = turn(static_cast<uint32_t>((static_cast<uint64_t>(position) * a.turns[i]) >> 32),
+                          a.amplitude);
+    put(at, i, w.x, a.sign * w.y);
+  }
+}
+
 template <typename T, int VEC, bool INTER, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 5) rotary_rows(const __grid_constant__ RotaryArgs a) {
   __shared__ Token told[PAGED ? kMaxTokens : 1];
@@ -175,8 +263,7 @@ __global__ void __launch_bounds__(kThreads, 5) rotary_rows(const __grid_constant
   const int lane = a.lanes == 1 ? 0 : a.div_items.div(threadIdx.x);
   const uint32_t item = group * blockDim.x + threadIdx.x - lane * a.items;
   const bool mine = item < a.items && lane < a.lanes;
-  int row = a.div_row.div(item);  // of q, then k, then v
-  const uint32_t j = item - row * a.per_row;
+  const uint32_t row = a.div_row.div(item), j = item - row * a.per_row;
   const bool in_turn = j < static_cast<uint32_t>(pairs / VEC);
   const int pair = j * VEC;  // the first of its pairs
   int ca, cb;                // its channels; cb < 0: no second vector
@@ -187,78 +274,25 @@ __global__ void __launch_bounds__(kThreads, 5) rotary_rows(const __grid_constant
     ca = a.rotary + (j - pairs / VEC) * 2 * VEC;
     cb = ca + VEC < a.dim ? ca + VEC : -1;
   }
-  const T* src;
-  T* dst;
-  RowStrides from, to;
-  int kind = 0;  // 0 q, 1 k, 2 v
-  if (row < a.heads) {
-    src = static_cast<const T*>(a.q);
-    dst = static_cast<T*>(a.q_out);
-    from = a.qs;
-    to = a.qo;
-  } else if (!PAGED || row < a.heads + a.heads_kv) {
-    row -= a.heads;
-    src = static_cast<const T*>(a.k);
-    dst = static_cast<T*>(a.k_out);
-    from = a.ks;
-    to = a.ko;
-    kind = 1;
-  } else {
-    row -= a.heads + a.heads_kv;
-    src = static_cast<const T*>(a.v);
-    dst = static_cast<T*>(a.v_out);
-    from = a.vs;
-    to = a.vo;
-    kind = 2;
-  }
-  src += row * from.h + ca;
-  dst += row * to.h + ca;
-  const int second = cb < 0 ? 0 : cb - ca;
-  const bool turns = in_turn && kind != 2;
+  const Rows<T, PAGED> rows(a, row);
+  const bool turns = in_turn && rows.kind != 2;
 
   Vec<T, VEC> x, y;
-  auto place = [&](int at, const RowStrides& s) {
-    const uint32_t token = token0 + at, b = a.div_seq.div(token);
-    return b * s.b + (token - b * a.div_seq.d) * s.t;
-  };
   auto fetch = [&](int at) {
     if (!mine || at >= ntok) return;
-    const T* p = src + place(at, from);
-    load<T, VEC>(x, p);
-    if (cb >= 0) load<T, VEC>(y, p + second);
+    const T* p = rows.src + rows.place(a, token0 + at, rows.from);
+    load<T, VEC>(x, p + ca);
+    if (cb >= 0) load<T, VEC>(y, p + cb);
   };
   fetch(lane);
 
   // ---- the tile's angles ----
-  if (PAGED) {
-    if (threadIdx.x < ntok) told[threadIdx.x] = appended_token(a, token0 + threadIdx.x);
-    if (a.cu_seqlens && blockIdx.x == 0) {
-      bool bad = threadIdx.x == 0 && (a.cu_seqlens[0] != 0 || a.cu_seqlens[a.num_seqs] > static_cast<int64_t>(a.tokens));
-      for (int n = threadIdx.x; n < a.num_seqs; n += blockDim.x)
-        bad |= a.cu_seqlens[n] > a.cu_seqlens[n + 1];
-      if (bad) report_device_error(a.err, kErrBadSeqlens);
-    }
-    __syncthreads();
-  }
-  for (int n = threadIdx.x; n < ntok * pairs; n += blockDim.x) {
-    const int at = n / pairs, i = n - at * pairs;
-    int64_t position;
-    if (PAGED) {
-      position = told[at].position;
-    } else {
-      const uint32_t b = a.div_seq.div(token0 + at), t = token0 + at - b * a.div_seq.d;
-      const int64_t place = b * a.pos_stride + t;
-      position = !a.positions ? t
-                 : a.pos64    ? static_cast<const int64_t*>(a.positions)[place]
-                              : static_cast<const int32_t*>(a.positions)[place];
-    }
-    const float2 w = turn(static_cast<uint32_t>((static_cast<uint64_t>(position) * a.turns[i]) >> 32),
-                          a.amplitude);
+  make_angles<PAGED>(a, token0, ntok, told, [&](int at, int i, float c, float sn) {
     const int of = i / VEC, r = i - of * VEC;
     float* const to = angles + at * a.rotary + ((r / kTwo) * (pairs / VEC) + of) * 2 * kTwo + r % kTwo;
-    to[0] = w.x;
-    to[kTwo] = a.sign * w.y;
-  }
+    to[0] = c;
+    to[kTwo] = sn;
+  });
   __syncthreads();
 
   for (int at = lane; at < ntok; at += a.lanes) {
@@ -280,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 5) rotary_rows(const __grid_constant
                                   : make_float2(Cvt<T>::to_f(other[0]), Cvt<T>::to_f(other[1]));
           const float2 sb = fmul2(s2, b2);
           const float2 ra = ffma2(c2, a2, make_float2(-sb.x, -sb.y));
-          const float2 rb = ffma2(s2, a2, fmul2(c2, b2));
+          const float2 rb = ffma2(c2, b2, fmul2(s2, a2));
           first[0] = Cvt<T>::from_f(ra.x);
           (INTER ? other[0] : first[1]) = Cvt<T>::from_f(ra.y);
           (INTER ? first[1] : other[0]) = Cvt<T>::from_f(rb.x);
@@ -289,22 +323,90 @@ __global__ void __launch_bounds__(kThreads, 5) rotary_rows(const __grid_constant
       } else {
         const float xa = Cvt<T>::to_f(x.e[0]), xb = Cvt<T>::to_f(y.e[0]);
         x.e[0] = Cvt<T>::from_f(fmaf(w[0], xa, -(w[1] * xb)));
-        y.e[0] = Cvt<T>::from_f(fmaf(w[1], xa, w[0] * xb));
+        y.e[0] = Cvt<T>::from_f(fmaf(w[0], xb, w[1] * xa));
       }
     }
-    T* p = dst;
-    if (PAGED && kind != 0) {
-      if (!(told[at].kept & 2)) continue;
-      p += kind == 1 ? told[at].k_at : told[at].v_at;
-    } else {
-      p += place(at, to);
-      if (PAGED && !(told[at].kept & 1)) {
+    bool zeroed;
+    T* const p = rows.target(a, token0 + at, told[PAGED ? at : 0], zeroed);
+    if (!p) continue;
+    if (zeroed) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x.e[e] = y.e[e] = Cvt<T>::from_f(0.0f);
+      for (int e = 0; e < VEC; ++e) x.e[e] = y.e[e] = Cvt<T>::from_f(0.0f);
+    }
+    *reinterpret_cast<decltype(x.w)*>(p + ca) = x.w;
+    if (cb >= 0) *reinterpret_cast<decltype(y.w)*>(p + cb) = y.w;
+  }
+}
+
+// Where the two channels of a pair do not lie whole vectors apart (half of the rotated channels is odd,
+// say), a vector of channels is loaded as it lies and its partners come through shared memory (interleaved:
+// they are in the vector): a thread keeps one vector of one row over the tile's tokens, angles are laid out
+// by channel with the sine's sign in place.  Words a quarter as wide in the form above take longer (6123
+// tokens x 48 rows x 128 bf16, 30 channels rotated, 109 us and 52), words half as wide do not (19488 x 20 x
+// 96, 8 rotated, 48 and 68).
+template <typename T, int VEC, bool INTER, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 4) rotary_staged(const __grid_constant__ RotaryArgs a) {
+  __shared__ Token told[PAGED ? kMaxTokens : 1];
+  __shared__ __align__(16) Vec<T, VEC> stage[INTER ? 1 : 2][INTER ? 1 : kThreads];
+  extern __shared__ __align__(16) float angles[];  // [token][cos, sin][channel]
+  const uint32_t column = blockIdx.x / a.groups, group = blockIdx.x - column * a.groups;
+  const uint32_t token0 = column * static_cast<uint32_t>(a.tile);
+  const int ntok = min(static_cast<uint32_t>(a.tile), a.tokens - token0);
+  const int wide = (a.rotary + VEC - 1) / VEC * VEC;  // channels of an angle table
+
+  // ---- this thread's vector: of row `row` of the group's, of token `lane` of those at once ----
+  const int lane = a.lanes == 1 ? 0 : a.div_items.div(threadIdx.x);
+  const uint32_t item = threadIdx.x - lane * a.items;  // items: of a group here
+  const uint32_t row = a.div_row.div(item), j = item - row * a.per_row;
+  const uint32_t row_all = group * (a.items / a.per_row) + row;
+  const bool mine = item < a.items && lane < a.lanes &&
+                    row_all < static_cast<uint32_t>(a.heads + (PAGED ? 2 : 1) * a.heads_kv);
+  const int channel = j * VEC;
+  const Rows<T, PAGED> rows(a, mine ? row_all : 0);
+  const bool turns = mine && rows.kind != 2 && channel < a.rotary;
+
+  Vec<T, VEC> x;
+  auto fetch = [&](int at) {
+    if (mine && at < ntok)
+      load<T, VEC>(x, rows.src + rows.place(a, token0 + at, rows.from) + channel);
+  };
+  fetch(lane);
+  make_angles<PAGED>(a, token0, ntok, told, [&](int at, int i, float c, float sn) {
+    const int first = INTER ? 2 * i : i, other = INTER ? first + 1 : i + a.rotary / 2;
+    float* const to = angles + at * 2 * wide;
+    to[first] = to[other] = c;
+    to[wide + first] = -sn;
+    to[wide + other] = sn;
+  });
+  int buf = 0;
+  for (int begin = 0; begin < ntok; begin += a.lanes, buf ^= 1) {
+    const int at = begin + lane;
+    Vec<T, VEC> v = x;
+    if (!INTER) stage[buf][threadIdx.x] = v;
+    fetch(at + a.lanes);
+    if (!INTER || begin == 0) __syncthreads();  // also of the angles, the first time
+    if (!mine || at >= ntok) continue;
+    if (turns) {
+      const float* const w = angles + at * 2 * wide + channel;
+      const T* const head = reinterpret_cast<const T*>(stage[INTER ? 0 : buf]) + (threadIdx.x - j) * VEC;
+      const int half = a.rotary / 2;
+      const Vec<T, VEC> own = v;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int d = channel + e;
+        if (d >= a.rotary) continue;
+        const float p = Cvt<T>::to_f(INTER ? own.e[e ^ 1] : head[d < half ? d + half : d - half]);
+        v.e[e] = Cvt<T>::from_f(fmaf(w[e], Cvt<T>::to_f(v.e[e]), w[wide + e] * p));
       }
     }
-    *reinterpret_cast<decltype(x.w)*>(p) = x.w;
-    if (cb >= 0) *reinterpret_cast<decltype(y.w)*>(p + second) = y.w;
+    bool zeroed;
+    T* const p = rows.target(a, token0 + at, told[PAGED ? at : 0], zeroed);
+    if (!p) continue;
+    if (zeroed) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v.e[e] = Cvt<T>::from_f(0.0f);
+    }
+    *reinterpret_cast<decltype(v.w)*>(p + channel) = v.w;
   }
 }
 
@@ -314,38 +416,63 @@ bool fits(const void* p, const RowStrides& s, int vec, size_t size) {
          s.h % vec == 0;
 }
 
-template <typename T, int VEC, bool PAGED>
-int launch_vec(RotaryArgs& a, bool interleaved, cudaStream_t s) {
-  a.per_row = a.rotary / (2 * VEC) + (a.dim - a.rotary + 2 * VEC - 1) / (2 * VEC);
-  a.items = (a.heads + (PAGED ? 2 : 1) * a.heads_kv) * a.per_row;
-  // The items of a token in as many CTAs as they need, in equal parts of whole warps; or several
-  // tokens side by side, as far as their tile's angles fit 16 KB.
-  const uint32_t groups = (a.items + kThreads - 1) / kThreads;
-  const uint32_t fit = std::min(kMaxTokens / kTile, 1024 / std::max(a.rotary, 1));
-  a.lanes = std::max<uint32_t>(1, std::min<uint32_t>(kThreads / a.items, fit));
-  // At least a thread for each token of the tile.
-  const uint32_t threads = (std::max((a.items + groups - 1) / groups, uint32_t{kTile}) * a.lanes + 31) / 32 * 32;
-  a.div_row = FastDivU32(a.per_row);
-  a.div_items = FastDivU32(a.items);
+// Tile, CTAs and launch of either kernel; `items` of a token in `groups` CTAs side by side, `room` floats of
+// angles a token.
+template <typename K>
+int launch_tiles(RotaryArgs& a, K kernel, uint32_t items, uint32_t groups, uint32_t threads, int room,
+                 cudaStream_t s) {
   // kTile tokens for each that is taken at once, while that makes four CTAs an SM.  (Tiles of 8 and 16
   // were slower, 8 x 4096 x 64 heads x 128 bf16 174 and 188 us for 165: CTAs that run together then
   // lie further apart in memory.)
   const int64_t spread = static_cast<int64_t>(a.tokens) * groups / (4 * sm_count() * a.lanes);
   a.tile = static_cast<int>(a.lanes * std::min<int64_t>(kTile, std::max<int64_t>(spread, 1)));
+  a.items = items;
   a.groups = groups;
+  a.div_row = FastDivU32(a.per_row);
+  a.div_items = FastDivU32(items);
   const int64_t grid = static_cast<int64_t>((a.tokens + a.tile - 1) / a.tile) * groups;
   if (grid > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
-  const size_t smem = static_cast<size_t>(a.tile) * a.rotary * sizeof(float);
-  auto kernel = interleaved ? rotary_rows<T, VEC, true, PAGED> : rotary_rows<T, VEC, false, PAGED>;
-  kernel<<<static_cast<unsigned>(grid), threads, smem, s>>>(a);
+  // At least a thread for each token of the tile.
+  threads = (std::max(threads, static_cast<uint32_t>(a.tile)) + 31) / 32 * 32;
+  kernel<<<static_cast<unsigned>(grid), threads, static_cast<size_t>(a.tile) * room * sizeof(float), s>>>(a);
   return launch_status();
 }
 
+// Tokens side by side: as their items fit a CTA, and their tile's angles 16 KB.
+uint32_t lanes_of(uint32_t items, int room) {
+  const uint32_t fit = std::min(kMaxTokens / kTile, 1024 / std::max(room, 1));
+  return std::max<uint32_t>(1, std::min<uint32_t>(kThreads / items, fit));
+}
+
+template <typename T, int VEC, bool PAGED>
+int launch_vec(RotaryArgs& a, cudaStream_t s) {
+  a.per_row = a.rotary / (2 * VEC) + (a.dim - a.rotary + 2 * VEC - 1) / (2 * VEC);
+  const uint32_t items = (a.heads + (PAGED ? 2 : 1) * a.heads_kv) * a.per_row;
+  // The items of a token in as many CTAs as they need, in equal parts of whole warps.
+  const uint32_t groups = (items + kThreads - 1) / kThreads;
+  a.lanes = lanes_of(items, a.rotary);
+  const uint32_t threads = ((items + groups - 1) / groups * a.lanes + 31) / 32 * 32;
+  return launch_tiles(a, a.interleaved ? rotary_rows<T, VEC, true, PAGED> : rotary_rows<T, VEC, false, PAGED>,
+                      items, groups, threads, a.rotary, s);
+}
+
+template <typename T, int VEC, bool PAGED>
+int launch_staged(RotaryArgs& a, cudaStream_t s) {
+  a.per_row = a.dim / VEC;  // at most kThreads
+  const uint32_t rows = a.heads + (PAGED ? 2 : 1) * a.heads_kv;
+  // Whole rows in a CTA, in equal parts.
+  const uint32_t most = kThreads / a.per_row, groups = (rows + most - 1) / most;
+  const uint32_t items = (rows + groups - 1) / groups * a.per_row;
+  const int room = 2 * ((a.rotary + VEC - 1) / VEC * VEC);
+  a.lanes = groups == 1 ? lanes_of(items, room) : 1;
+  return launch_tiles(a, a.interleaved ? rotary_staged<T, VEC, true, PAGED> : rotary_staged<T, VEC, false, PAGED>, items, groups, items * a.lanes, room, s);
+}
+
 template <typename T, bool PAGED>
-int launch_type(RotaryArgs& a, bool interleaved, cudaStream_t s) {
-  auto vector = [&](int vec) {
-    const int pairs = a.rotary / 2;
-    bool ok = pairs % vec == 0 && (a.dim - a.rotary) % vec == 0 && a.dim % vec == 0;
+int launch_type(RotaryArgs& a, cudaStream_t s) {
+  const int pairs = a.rotary / 2;
+  auto rows_fit = [&](int vec) {  // rows in words of vec elements
+    bool ok = a.dim % vec == 0;
     if (a.heads) ok = ok && fits(a.q, a.qs, vec, sizeof(T)) && fits(a.q_out, a.qo, vec, sizeof(T));
     if (a.heads_kv)
       ok = ok && fits(a.k, a.ks, vec, sizeof(T)) && fits(a.k_out, a.ko, vec, sizeof(T));
@@ -353,20 +480,28 @@ int launch_type(RotaryArgs& a, bool interleaved, cudaStream_t s) {
     return ok;
   };
   constexpr int kFull = 16 / sizeof(T);
-  if (vector(kFull)) return launch_vec<T, kFull, PAGED>(a, interleaved, s);
-  if (vector(kFull / 2)) return launch_vec<T, kFull / 2, PAGED>(a, interleaved, s);
-  if constexpr (kFull > 4) {
-    if (vector(2)) return launch_vec<T, 2, PAGED>(a, interleaved, s);
+  int wide = kFull;
+  while (wide > 1 && !rows_fit(wide)) wide /= 2;
+  int narrow = wide;  // and pairs whole words apart
+  while (narrow > 1 && (pairs % narrow != 0 || (a.dim - a.rotary) % narrow != 0)) narrow /= 2;
+  if (4 * narrow <= wide && a.dim / wide <= kThreads) {
+    if (wide == kFull) return launch_staged<T, kFull, PAGED>(a, s);
+    return launch_staged<T, 4, PAGED>(a, s);
   }
-  return launch_vec<T, 1, PAGED>(a, interleaved, s);
+  if (narrow == kFull) return launch_vec<T, kFull, PAGED>(a, s);
+  if (narrow == kFull / 2) return launch_vec<T, kFull / 2, PAGED>(a, s);
+  if constexpr (kFull > 4) {
+    if (narrow == 2) return launch_vec<T, 2, PAGED>(a, s);
+  }
+  return launch_vec<T, 1, PAGED>(a, s);
 }
 
 template <bool PAGED>
-int launch(RotaryArgs& a, bool interleaved, int dtype, cudaStream_t s) {
+int launch(RotaryArgs& a, int dtype, cudaStream_t s) {
   switch (dtype) {
-    case TILEOPS_DT_F32: return launch_type<float, PAGED>(a, interleaved, s);
-    case TILEOPS_DT_F16: return launch_type<__half, PAGED>(a, interleaved, s);
-    default: return launch_type<__nv_bfloat16, PAGED>(a, interleaved, s);
+    case TILEOPS_DT_F32: return launch_type<float, PAGED>(a, s);
+    case TILEOPS_DT_F16: return launch_type<__half, PAGED>(a, s);
+    default: return launch_type<__nv_bfloat16, PAGED>(a, s);
   }
 }
 
@@ -420,7 +555,8 @@ extern "C" int tileops_rotary(const void* q, const void* k, const void* position
   a.amplitude = static_cast<float>(amplitude);
   a.sign = backward ? -1.0f : 1.0f;
   std::copy_n(turns, rotary_dim / 2, a.turns);
-  return launch<false>(a, interleaved != 0, dtype, as_stream(stream));
+  a.interleaved = interleaved != 0;
+  return launch<false>(a, dtype, as_stream(stream));
 }
 
 extern "C" int tileops_paged_kv_append(
@@ -473,5 +609,6 @@ extern "C" int tileops_paged_kv_append(
   a.page_size = static_cast<int>(page_size);
   a.err = device_error_ptr();
   std::copy_n(turns, rotary_dim / 2, a.turns);
-  return launch<true>(a, interleaved != 0, dtype, as_stream(stream));
+  a.interleaved = interleaved != 0;
+  return launch<true>(a, dtype, as_stream(stream));
 }
