@@ -436,8 +436,8 @@ int tileops_rotary(const void* q, const void* k, const void* positions, void* q_
  * (num_seqs, table_width) with rows table_stride apart, entries behind a
  * sequence's end are not read.  strides18 (HOST): elements from a batch entry,
  * token and head to the next of q, k, v, q_out (packed: the first is not used),
- * and from a page, slot and head to the next of k_cache and v_cache.  Two rows
- * with the same slot race. */
+ * and from a page, slot and head to the next of k_cache and v_cache, which are
+ * two different buffers.  Two rows with the same slot race. */
 int tileops_paged_kv_append(const void* q, const void* k, const void* v, void* q_out,
                             void* k_cache, void* v_cache, const int32_t* page_table,
                             const int32_t* seq_lens, const int32_t* cu_seqlens,

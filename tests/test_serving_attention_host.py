@@ -301,6 +301,7 @@ def _cast(change, dtype):
     (dict(k=torch.zeros(2, 1, 2, 8), v=torch.zeros(2, 1, 2, 8), q=None,
           cu_seqlens=torch.tensor([0, 1, 2], dtype=torch.int32)), "must be packed"),
     (dict(k_cache=torch.zeros(1, 4, 2, 8).expand(3, 4, 2, 8)), "share memory"),
+    ((lambda c: dict(k_cache=c, v_cache=c))(torch.zeros(3, 4, 2, 8)), "k_cache and v_cache share memory"),
     (dict(v_cache=torch.zeros(3, 4, 8, 2).transpose(2, 3)), "contiguous channels"),
 ])
 def test_append_refusals(change, match, accept_cpu):
@@ -380,17 +381,17 @@ def test_append_entry_point_checks():
     turns = (ctypes.c_uint64 * 128)()
     s = _ints(*[0] * 18)
 
-    def call(q=SOME, k=SOME, v=SOME, c=SOME, table=SOME, lens=SOME, cu=NULL, t=turns, N=2, T=4, H=2,
-             Hkv=1, D=8, R=8, pages=3, P=4, width=2, st=s, dtype=2):
-        return fn(q, k, v, q, c, c, table, lens, cu, t, N, T, H, Hkv, D, R, pages, P, width, width, st,
+    def call(q=SOME, k=SOME, v=SOME, c=SOME, vc=ctypes.c_void_p(1 << 21), table=SOME, lens=SOME, cu=NULL,
+             t=turns, N=2, T=4, H=2, Hkv=1, D=8, R=8, pages=3, P=4, width=2, st=s, dtype=2):
+        return fn(q, k, v, q, c, vc, table, lens, cu, t, N, T, H, Hkv, D, R, pages, P, width, width, st,
                   0, 1.0, dtype, NULL)
 
     for bad in (dict(N=-1), dict(T=-1), dict(T=5), dict(N=0), dict(H=-1), dict(Hkv=0), dict(D=0),
                 dict(R=9), dict(pages=-1), dict(pages=2**31), dict(P=0), dict(P=2**31), dict(width=-1)):
         assert call(**bad) == _native.EBADSHAPE, bad
     assert call(dtype=3) == _native.EBADDTYPE
-    for bad in (dict(q=NULL), dict(k=NULL), dict(v=NULL), dict(c=NULL), dict(table=NULL), dict(lens=NULL),
-                dict(t=None), dict(st=None)):
+    for bad in (dict(q=NULL), dict(k=NULL), dict(v=NULL), dict(c=NULL), dict(vc=NULL), dict(vc=SOME),
+                dict(table=NULL), dict(lens=NULL), dict(t=None), dict(st=None)):
         assert call(**bad) == _native.EINVAL, bad
     assert call(q=NULL, k=NULL, N=0, T=0) == _native.OK
 

@@ -14,21 +14,28 @@
 // m16n8k16 (the query heads of a key head are the 16 rows; a 128-row tcgen05 tile would be
 // 7/8 padding and would take the scores through TMEM and back, for rates not needed here).
 //
-// The split.  The tokens of each (sequence, key head) are cut into units of 64, and all units of
-// the call in a row are shared out evenly, a run of them to each CTA, whatever the sequences'
-// lengths are (they stay on the device).  An item (sequence and key head) whose
-// units lie in one CTA is finished there; of one that lies in several, each writes its sums
+// The split.  The tokens of each (sequence, key head) are cut into units of 16 or 32 for each warp of
+// a CTA, and all units of the call in a row are shared out evenly, a run of them to each CTA,
+// whatever the sequences' lengths are (they stay on the device).  An item (sequence and key head)
+// whose units lie in one CTA is finished there; of one that lies in several, each writes its sums
 // and counts itself, and the last one to do so joins them all, in the order of the CTAs, so that
 // results repeat to the bit.  A CTA has at most two items it shares with others: its first and its
 // last.  (A second kernel for the joins cost 5 to 7 us a call.)  The counters are cleared by a
-// small kernel in front, beside which this one starts (programmatic launch).
+// small kernel in front, beside which this one starts (programmatic launch: 0.6 us; clearing them by
+// a memset 4 us).
 //
-// In a CTA each of 4 warps takes 16 tokens of a unit on its own: it copies their keys and values
+// In a CTA each warp takes its tokens of a unit on its own: it copies their keys and values
 // with 16-byte cp.async through its own ring of stages (no CTA barrier), multiplies, and keeps a
-// running maximum, sum and output of the softmax in registers (fp32).  The 4 warps join at an
-// item's end, through the stage just used; the copies of the next items' units are in flight
-// meanwhile.  Tokens outside the sequence are copied as zeros (size 0), never read: infinities
-// and NaN behind a sequence's end have no say.
+// running maximum, sum and output of the softmax in registers (fp32).  The page numbers are
+// copied two rings ahead.  The warps join at an item's end, through the stage just used; the copies
+// of the next items' units are in flight meanwhile.  Tokens outside the sequence are copied as
+// zeros (size 0), never read: infinities and NaN behind a sequence's end have no say.
+//
+// Measured (bf16 and fp16, in a graph): 131072 tokens x 8 heads x 128 92 us (0.90 of the copy rate), 64
+// sequences of up to 8192 x 8 x 128 85 us (0.90), 8 of up to 4096 x 32 x 128 29 us (0.68), 1000 x 8 x 128
+// 8.4 us.  The body runs at the rate of a kernel that only reads; before it 2.5 us (lengths, pages, first
+// keys: three waits one after another, and code that is not in the SM yet), behind it 1.5 to 5 us
+// of joining (more where one item is shared by many CTAs).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

@@ -17,6 +17,10 @@
 // token (or of each of several at once, where a token has few items) and walks a tile of tokens with
 // it, so that addresses cost two multiplications; the tile's angles are made once, by all threads
 // and while the first loads are on their way, and serve all of its heads from shared memory.
+// Measured (bf16, in a graph): 8 x 4096 x 64 heads x 128 164 us, the time of a plain copy of as many
+// bytes; 8 x 4096 x 40 heads x 128 108 us (0.94); append of 16384 packed tokens x 48 rows x 128 77 us (0.80).
+// What did not help: shares of the tokens for as many CTAs as run at once (200 us for the first of
+// these), the next token's loads in flight during one's arithmetic (171 us: more registers, fewer CTAs).
 #include <algorithm>
 
 #include "common.cuh"
@@ -575,7 +579,7 @@ extern "C" int tileops_paged_kv_append(
   if (!is_float_dtype(dtype)) return TILEOPS_EBADDTYPE;
   if (tokens == 0) return TILEOPS_OK;
   if ((heads && (!q || !q_out)) || !k || !v || !k_cache || !v_cache ||
-      !strides18 || (num_seqs && !seq_lens) || (num_seqs && table_width && !page_table) || (rotary_dim && !turns))
+      k_cache == v_cache || !strides18 || (num_seqs && !seq_lens) || (num_seqs && table_width && !page_table) || (rotary_dim && !turns))
     return TILEOPS_EINVAL;
   RotaryArgs a{};
   a.q = q;

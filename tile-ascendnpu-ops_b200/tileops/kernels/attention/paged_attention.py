@@ -101,11 +101,13 @@ class PagedKVAppendKernel(Kernel):
             q, k, v, page_table, seq_lens, cu_seqlens = (
                 t.contiguous() if c else t
                 for t, c in zip((q, k, v, page_table, seq_lens, cu_seqlens), copy))
+        k_at, v_at = k_cache.data_ptr(), v_cache.data_ptr()
+        if k_at == v_at:
+            raise ValueError("k_cache and v_cache share memory: they cannot both be written")
         q_out = None if q is None else torch.empty_like(q_like)
         _native.launch(
             "tileops_paged_kv_append", device, 0 if q is None else q.data_ptr(), k.data_ptr(),
-            v.data_ptr(), 0 if q is None else q_out.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
+            v.data_ptr(), 0 if q is None else q_out.data_ptr(), k_at, v_at, page_table.data_ptr(), seq_lens.data_ptr(),
             0 if cu_seqlens is None else cu_seqlens.data_ptr(), self._turns, seqs, tokens,
             0 if q is None else self.heads, self.heads_kv, self.dim, self.rotary_dim, pages,
             self.page_size, columns, table_stride, strides, self.interleaved, self.amplitude,
