@@ -31,10 +31,10 @@
 // of the next items' units are in flight meanwhile.  Tokens outside the sequence are copied as
 // zeros (size 0), never read: infinities and NaN behind a sequence's end have no say.
 //
-// Measured (bf16 and fp16, in a graph): 131072 tokens x 8 heads x 128 92 us (0.90 of the copy rate), 64
-// sequences of up to 8192 x 8 x 128 85 us (0.90), 8 of up to 4096 x 32 x 128 29 us (0.68), 1000 x 8 x 128
-// 8.4 us.  The body runs at the rate of a kernel that only reads; before it 2.5 us (lengths, pages, first
-// keys: three waits one after another, and code that is not in the SM yet), behind it 1.5 to 5 us
+// Measured (bf16 and fp16, in a graph): 131072 tokens x 8 heads x 128 89 us (0.92 of the copy rate), 64
+// sequences of up to 8192 x 8 x 128 85 us (0.90), 8 of up to 4096 x 32 x 128 28 us (0.71), 1000 x 8 x 128
+// 8.2 us.  The body runs at 0.94 of the rate of a kernel that only reads; before it 2.5 us (lengths, pages,
+// first keys: three waits one after another, and code that is not in the SM yet), behind it 1.5 to 5 us
 // of joining (more where one item is shared by many CTAs).
 #include <algorithm>
 #include <atomic>
@@ -206,9 +206,12 @@ struct Layout {
   static constexpr int kRow = (DP + 63) / 64 * 64;             // elements of a row in shared memory
   // Tokens of a warp in a unit: 8 KB of keys and values and more, for what a unit costs besides.
   static constexpr int kTokens = DP <= 64 ? 32 : 16;
-  static constexpr int kStages = DP <= 128 ? 3 : DP <= 192 ? (WARPS == 4 ? 4 : 2) : (WARPS == 4 ? 3 : 2);
-  static constexpr int kCtasSm =
-      WARPS == 8 ? 1 : WARPS == 4 ? (DP <= 128 ? 2 : 1) : DP <= 192 ? 4 : 3;
+  // Two stages of 8 KB a warp and 12 warps an SM (8 where 16 rows more take the registers): 256 items of
+  // up to 4096 tokens x 128 27.9 us, 29.3 with three stages and 8 warps; heads of 192 and 256 as they fit.
+  static constexpr int kStages = DP <= 128 ? 2 : DP <= 192 ? (WARPS == 4 ? 4 : 2) : (WARPS == 4 ? 3 : 2);
+  static constexpr int kCtasSm = WARPS == 8   ? 1
+                                 : WARPS == 4 ? (DP > 128 ? 1 : MT == 1 ? 3 : 2)
+                                              : (DP <= 192 ? 4 : 3);
   static constexpr int kUnit = WARPS * kTokens;
   static constexpr int kThreads = WARPS * 32;
   static constexpr int kTile = kTokens * kRow;                 // elements of a warp's keys (or values)
@@ -711,9 +714,14 @@ bool opt_in() {
 template <typename T, int DP, int MT, int WARPS>
 int launch_tile(const DecodeArgs& a, cudaStream_t s) {
   using L = Layout<DP, MT, WARPS>;
+  // Where heads lie side by side and share 128-byte lines, fewer CTAs: those of neighbouring heads then stay
+  // close to each other in the tokens, and a line is fetched once (320 items of 8009 tokens x 80 189 us
+  // for 227; with whole lines a head more CTAs are as good or better, 512 items x 128 85 us for 89).
+  int ctas_sm = L::kCtasSm;
+  if (WARPS == 4 && a.heads_kv > 1 && a.ks.head * 2 % 128 != 0) ctas_sm = std::min(ctas_sm, 2);
   // No more CTAs than there can be places.
   const int64_t grid = std::min<int64_t>(
-      {places_of(a, L::kUnit), static_cast<int64_t>(sm_count()) * L::kCtasSm, kMaxCtas});
+      {places_of(a, L::kUnit), static_cast<int64_t>(sm_count()) * ctas_sm, kMaxCtas});
   if (!opt_in<T, DP, MT, WARPS>()) return TILEOPS_ELAUNCH;
   clear_counters<<<1, 512, 0, s>>>(a.counters, static_cast<int>(grid));
   if (int status = launch_status()) return status;
@@ -737,9 +745,9 @@ int launch_tile(const DecodeArgs& a, cudaStream_t s) {
 template <typename T, int DP, int MT>
 int launch_warps(const DecodeArgs& a, cudaStream_t s) {
   // Few items are shared by many CTAs each: one CTA of 8 warps an SM, so that there are fewer sums to join
-  // (131072 tokens of 8 heads of 128 bf16 93 us, 97 with two CTAs of 4; 256 items 32.6 and 29.1).  Many
+  // (32 items of 32768 tokens x 128 89 us, 94 with CTAs of 4; but 256 items of up to 4096 33 and 28 us).  Many
   // items: smaller CTAs, more of them at different points of an item (512 sequences of up to 256 tokens,
-  // 4096 items, four CTAs of 2 warps 43.5 us, two of 4 54.7; 512 items of up to 8192 tokens 85.6 and 84.0).
+  // 4096 items, CTAs of 2 warps 44 us, of 4 51; 512 items of up to 8192 tokens 87 and 85).
   // Heads of 192 have no room for two CTAs of 4, nor heads of 256 for 8 warps.
   const int64_t items = static_cast<int64_t>(a.batch) * a.heads_kv * a.blocks;
   if constexpr (DP <= 192) {
