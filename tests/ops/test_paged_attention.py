@@ -116,6 +116,29 @@ def test_splits(lens, dtype):
     _attend(lens, 2, 1, 64, 16, dtype)
 
 
+def test_many_sequences():
+    """More than a warp finds its place among in two looks."""
+    _attend([3] * 1500 + [70] + [0] * 40 + [130, 1], 1, 1, 64, 16, torch.float16)
+
+
+@pytest.mark.parametrize("H, Hkv, D, lens", [
+    (2, 1, 64, [500, 0, 33]), (32, 32, 128, [200] * 6), (4, 2, 192, [90] * 100), (2, 2, 256, [90] * 100),
+])
+def test_tables_with_room_to_spare(H, Hkv, D, lens):
+    _attend(lens, H, Hkv, D, 16, torch.bfloat16, extra=700)
+
+
+@pytest.mark.parametrize("H, Hkv, D, count", [
+    (12, 6, 80, 30), (12, 12, 40, 16), (8, 8, 128, 90), (8, 8, 64, 90), (32, 1, 96, 200), (3, 3, 192, 60),
+    (4, 4, 256, 50),
+])
+def test_each_size_of_cta(H, Hkv, D, count):
+    """Numbers of items on both sides of the rules, whole and shared."""
+    lens = [int(n) for n in torch.randint(0, 400, (count,))]
+    _attend(lens, H, Hkv, D, 16, torch.float16)
+    _attend(lens[:5] + [3000], H, Hkv, D, 16, torch.bfloat16, "head")
+
+
 @pytest.mark.parametrize("H, Hkv, D", [(8, 8, 128), (40, 2, 128), (32, 1, 256), (16, 4, 192)])
 def test_splits_of_many_heads(H, Hkv, D):
     _attend([3000, 1, 700, 0, 64], H, Hkv, D, 32, torch.float16)
@@ -293,6 +316,25 @@ def test_two_graphs_of_one_pool():
             assert_within(o, want[0], want[2], str(now))
             live = lens > 0
             assert_within(lse[live], want[1][live.cpu()], want[3][live.cpu()])
+
+
+def test_a_first_call_inside_a_capture():
+    """An op's first call of its kind captured (another has looked the device's error flag up)."""
+    table, pages = _table([70, 200], 16)
+    lens = _lens([70, 200])
+    kc, vc = _cache(pages, 16, 3, 72, torch.bfloat16), _cache(pages, 16, 3, 72, torch.bfloat16)
+    q, k = (torch.randn(2, n, 72, device="cuda").to(torch.bfloat16) for n in (6, 3))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qr = PagedKVAppendOp(3, 72, 16, 6, 20, True)(k, k, kc, vc, table, lens, q)
+        o, lse = PagedAttentionDecodeOp(6, 3, 72, 16, window=100)(qr, kc, vc, table, lens)
+    expect = ref.append(k, k, kc, vc, table, lens, rotary_frequencies(20), q, interleaved=True)
+    graph.replay()
+    assert_within(qr, expect[0], expect[1])
+    assert_within(kc, expect[2], expect[3])
+    want = ref.attend(qr, kc, vc, table, lens, window=100)
+    assert_within(o, want[0], want[2])
+    assert_within(lse, want[1], want[3])
 
 
 def test_offsets_past_32_bits():
