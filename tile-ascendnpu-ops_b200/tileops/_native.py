@@ -169,21 +169,27 @@ def status_string(status: int) -> str:
 _functions: dict[str, object] = {}  # entry points called so far
 
 
-def call(name: str, *args) -> None:
-    """Invoke entry point ``name``; raise on a non-zero status."""
-    fn = _functions.get(name)
+def _entry(name: str):
+    """Entry point ``name``, kept for the next call."""
+    fn = getattr(lib(), name, None)
     if fn is None:
-        fn = getattr(lib(), name, None)
-        if fn is None:
-            raise NativeLibraryError(f"{LIB_PATH.name} does not export {name}")
-        _functions[name] = fn
-    status = fn(*args)
-    if status == OK:
-        return
+        raise NativeLibraryError(f"{LIB_PATH.name} does not export {name}")
+    _functions[name] = fn
+    return fn
+
+
+def _raise(name: str, status: int) -> None:
     msg = f"{name} failed: {status_string(status)} (status {status})"
     if status in (EBADDTYPE, EBADSHAPE, EALIGN, EINVAL):
         raise ValueError(msg)
     raise RuntimeError(msg)
+
+
+def call(name: str, *args) -> None:
+    """Invoke entry point ``name``; raise on a non-zero status."""
+    status = (_functions.get(name) or _entry(name))(*args)
+    if status != OK:
+        _raise(name, status)
 
 
 def ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
@@ -212,5 +218,7 @@ def launch(name: str, device: torch.device, *args) -> None:
     if idx != current:
         with torch.cuda.device(idx):
             call(name, *args, stream)
-    else:
-        call(name, *args, stream)
+        return
+    status = (_functions.get(name) or _entry(name))(*args, stream)  # call(), one layer less
+    if status != OK:
+        _raise(name, status)

@@ -15,7 +15,7 @@ from typing import Optional, Sequence
 import torch
 
 from tileops import _native
-from tileops.kernels.attention._layouts import Layouts, channels_last, layout_of, overlaps, row_of
+from tileops.kernels.attention._layouts import channels_last, overlaps, row_of
 from tileops.kernels.attention.rotary_embedding import check_rotation, turns_array
 from tileops.kernels.kernel_base import Kernel, check_dtype
 
@@ -51,11 +51,10 @@ class PagedKVAppendKernel(Kernel):
         self.dtype = dtype
         self._code = _native.dtype_code(dtype)
         self._turns = turns_array(frequencies)
-        self._plans = Layouts()
         self.init_config(config)
 
-    def _plan(self, k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens):
-        """Device, which arguments have to be copied, the stride array, the table's stride, the rows and
+    def plan(self, k, v, k_cache, v_cache, page_table, seq_lens, q=None, cu_seqlens=None):
+        """What a call of this layout needs, for ``forward``: device, which arguments have to be copied, the stride array, the table's stride, the rows and
         the queries' shape; refuses caches that cannot be written."""
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
             if not channels_last(c):
@@ -87,15 +86,11 @@ class PagedKVAppendKernel(Kernel):
                 None if q is None else row_of(q))
 
     def forward(self, k, v, k_cache, v_cache, page_table, seq_lens, q=None, cu_seqlens=None,
-                layout=None):
-        """Write the caches; return the rotated queries (None without ``q``).  ``layout``: that of
-        (k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens), if it is at hand."""
-        if layout is None:
-            layout = layout_of(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
-        plan = self._plans.get(layout)
+                plan=None):
+        """Write the caches; return the rotated queries (None without ``q``).  ``plan``: what
+        ``plan()`` gave for arguments of the same layout."""
         if plan is None:
-            plan = self._plans.keep(layout, self._plan(k, v, k_cache, v_cache, page_table, seq_lens,
-                                                       q, cu_seqlens))
+            plan = self.plan(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
         device, copy, strides, table_stride, seqs, tokens, pages, columns, q_like = plan
         if copy is not None:
             q, k, v, page_table, seq_lens, cu_seqlens = (
@@ -146,11 +141,10 @@ class PagedAttentionDecodeKernel(Kernel):
         self.scale, self.window = float(scale), int(window)
         self.dtype = dtype
         self._code = _native.dtype_code(dtype)
-        self._plans = Layouts()
         self.init_config(config)
 
-    def _plan(self, q, k_cache, v_cache, page_table, seq_lens):
-        """Device, which arguments have to be copied (never a cache), the stride array, the table's
+    def plan(self, q, k_cache, v_cache, page_table, seq_lens):
+        """What a call of this layout needs, for ``forward``: device, which arguments have to be copied (never a cache), the stride array, the table's
         stride and sizes, and the shapes of the outputs and the workspace."""
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
             if not channels_last(c) or any(s % 8 for s, n in zip(c.stride()[:3], c.shape) if n > 1):
@@ -169,13 +163,10 @@ class PagedAttentionDecodeKernel(Kernel):
                 batch, k_cache.shape[0], page_table.shape[1], row_of(q),
                 like.expand(batch, heads), like.expand(-(-room // 4)))
 
-    def forward(self, q, k_cache, v_cache, page_table, seq_lens, layout=None):
-        """Return ``(o, lse)``.  ``layout``: that of the arguments, if it is at hand."""
-        if layout is None:
-            layout = layout_of(q, k_cache, v_cache, page_table, seq_lens)
-        plan = self._plans.get(layout)
+    def forward(self, q, k_cache, v_cache, page_table, seq_lens, plan=None):
+        """Return ``(o, lse)``.  ``plan``: what ``plan()`` gave for arguments of the same layout."""
         if plan is None:
-            plan = self._plans.keep(layout, self._plan(q, k_cache, v_cache, page_table, seq_lens))
+            plan = self.plan(q, k_cache, v_cache, page_table, seq_lens)
         device, copy, strides, table_stride, batch, pages, columns, o_like, lse_like, ws_like = plan
         if copy is not None:
             q, page_table, seq_lens = (t.contiguous() if c else t

@@ -13,7 +13,7 @@ from typing import Optional, Sequence
 import torch
 
 from tileops import _native
-from tileops.kernels.attention._layouts import Layouts, channels_last, layout_of, row_of
+from tileops.kernels.attention._layouts import channels_last, row_of
 from tileops.kernels.kernel_base import Kernel, check_dtype
 
 __all__ = ["RotaryEmbeddingBwdKernel", "RotaryEmbeddingFwdKernel"]
@@ -66,11 +66,10 @@ class _RotaryEmbeddingKernel(Kernel):
         self.dtype = dtype
         self._code = _native.dtype_code(dtype)
         self._turns = turns_array(frequencies)
-        self._plans = Layouts()
         self.init_config(config)
 
-    def _plan(self, q, k, positions, inplace: bool):
-        """Device, whether q, k and positions have to be copied, the stride array, the positions'
+    def plan(self, q, k, positions=None, inplace: bool = False):
+        """What a call of this layout needs, for ``forward``: device, whether q, k and positions have to be copied, the stride array, the positions'
         stride and type, and the outputs' shapes."""
         copy = tuple(t is not None and not channels_last(t) and not inplace for t in (q, k))
         like = tuple(None if t is None or inplace else row_of(t) for t in (q, k))
@@ -91,15 +90,11 @@ class _RotaryEmbeddingKernel(Kernel):
         return ((k if q is None else q).device, any(copy) or copy_at, (*copy, copy_at),
                 (ctypes.c_int64 * 12)(*values), stride, code, like)
 
-    def forward(self, q, k, positions=None, inplace: bool = False, layout=None):
-        """Return ``(q_out, k_out)``; ``inplace`` writes over ``q`` and ``k``.  ``layout``: that of
-        (q, k, positions), if it is at hand."""
-        if layout is None:
-            layout = layout_of(q, k, positions)
-        key = None if layout is None else (layout, inplace)
-        plan = self._plans.get(key)
+    def forward(self, q, k, positions=None, inplace: bool = False, plan=None):
+        """Return ``(q_out, k_out)``; ``inplace`` writes over ``q`` and ``k``.  ``plan``: what
+        ``plan()`` gave for arguments of the same layout."""
         if plan is None:
-            plan = self._plans.keep(key, self._plan(q, k, positions, inplace))
+            plan = self.plan(q, k, positions, inplace)
         device, copies, copy, strides, stride, code, (q_like, k_like) = plan
         if copies:
             q, k, positions = (t.contiguous() if c else t for t, c in zip((q, k, positions), copy))

@@ -92,7 +92,7 @@ class PagedKVAppendOp(Op):
         self.amplitude = amplitude
         self.dtype = dtype
         self._last = (0, 0, 0), False  # of the last call: k's shape, whether there were queries
-        self._checked = Layouts()  # those that were found right
+        self._plans = Layouts()  # of the arguments that were found right
         self.dispatch_kernel(kernel_map)
         self.kernel = self.kernel_map["paged_kv_append"](
             heads_kv, dim, page_size, heads, rotary_dim, interleaved, self.frequencies, amplitude,
@@ -107,11 +107,13 @@ class PagedKVAppendOp(Op):
                 q: Optional[torch.Tensor] = None,
                 cu_seqlens: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         layout = layout_of(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
-        if layout not in self._checked:
+        plan = self._plans.get(layout)
+        if plan is None:
             self._check(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
-            self._checked.keep(layout, True)
+            plan = self._plans.keep(layout, self.kernel.plan(k, v, k_cache, v_cache, page_table,
+                                                             seq_lens, q, cu_seqlens))
         self._last = layout[0][0], q is not None
-        return self.kernel(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens, layout)
+        return self.kernel.forward(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens, plan)
 
     def _check(self, k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens) -> None:
         dev = getattr(k, "device", None)
@@ -172,7 +174,7 @@ class PagedAttentionDecodeOp(Op):
         self.window = window
         self.dtype = dtype
         self._last = 0, 0  # of the last call: sequences, columns of the page table
-        self._checked = Layouts()  # those that were found right
+        self._plans = Layouts()  # of the arguments that were found right
         self.dispatch_kernel(kernel_map)
         self.kernel = self.kernel_map["paged_attention_decode"](
             heads, heads_kv, dim, page_size, self.scale, window or 0, dtype)
@@ -185,11 +187,12 @@ class PagedAttentionDecodeOp(Op):
                 page_table: torch.Tensor,
                 seq_lens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         layout = layout_of(q, k_cache, v_cache, page_table, seq_lens)
-        if layout not in self._checked:
+        plan = self._plans.get(layout)
+        if plan is None:
             self._check(q, k_cache, v_cache, page_table, seq_lens)
-            self._checked.keep(layout, True)
+            plan = self._plans.keep(layout, self.kernel.plan(q, k_cache, v_cache, page_table, seq_lens))
         self._last = layout[3][0]
-        return self.kernel(q, k_cache, v_cache, page_table, seq_lens, layout)
+        return self.kernel.forward(q, k_cache, v_cache, page_table, seq_lens, plan)
 
     def _check(self, q, k_cache, v_cache, page_table, seq_lens) -> None:
         dev = getattr(q, "device", None)

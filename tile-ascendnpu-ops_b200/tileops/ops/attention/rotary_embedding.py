@@ -94,20 +94,21 @@ class _RotaryEmbeddingOp(Op):
         self.kernel = self.kernel_map[name](batch, seq_len, heads, heads_kv, dim, self.rotary_dim,
                                             interleaved, self.frequencies, amplitude, dtype)
         self._shapes = (batch, seq_len, heads, dim), (batch, seq_len, heads_kv, dim)
-        self._checked = Layouts()  # those that were found right
+        self._plans = Layouts()  # of the arguments that were found right
 
     def forward(self, q: Optional[torch.Tensor], k: Optional[torch.Tensor],
                 positions: Optional[torch.Tensor] = None):
         layout = layout_of(q, k, positions)
-        if layout not in self._checked:
+        plan = self._plans.get(layout)
+        if plan is None:
             self._check(q, k, positions)
-            self._checked.keep(layout, True)
-        if q is None and k is None:
-            return None, None
+            if q is None and k is None:
+                return None, None
+            plan = self._plans.keep(layout, self.kernel.plan(q, k, positions, self.inplace))
         if self.inplace and q is not None and k is not None and q.data_ptr() == k.data_ptr() != 0:
             raise ValueError(f"{self._names[0]} and {self._names[1]} share memory: they cannot both "
                              "be rotated in place")
-        return self.kernel(q, k, positions, self.inplace, layout)
+        return self.kernel.forward(q, k, positions, self.inplace, plan)
 
     def _check(self, q, k, positions) -> None:
         dev = getattr(k if q is None else q, "device", None)
