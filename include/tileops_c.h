@@ -447,6 +447,8 @@ int tileops_paged_kv_append(const void* q, const void* k, const void* v, void* q
                             const int64_t* strides18, int interleaved, double amplitude, int dtype,
                             void* stream);
 
+#define TILEOPS_PAGED_DECODE_COUNTERS 592
+
 /* Bytes of scratch tileops_paged_decode_fwd needs, whatever the batch and the
  * lengths, or -1 for an unsupported shape. */
 int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t heads_kv, int64_t dim);
@@ -461,7 +463,11 @@ int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t heads_kv, in
  * (HOST, multiples of 8): elements from a sequence and head to the next of q,
  * from a page, slot and head to the next of k_cache and of v_cache.  q, caches,
  * workspace 16-byte aligned; `workspace` holds
- * tileops_paged_decode_workspace_bytes() bytes.  A seq_lens[b] above page_size *
+ * tileops_paged_decode_workspace_bytes() bytes, for one call at a time.  Its first
+ * TILEOPS_PAGED_DECODE_COUNTERS int32 are counters: `counters_zero` says that
+ * they are zero (the call leaves them so: of a workspace that is kept for one
+ * stream they need clearing once); else the call clears them first, with a kernel
+ * more.  A seq_lens[b] above page_size *
  * table_width (taken as that) or a page outside [0, num_pages) (taken as zeros)
  * sets the device error flag to 3; table entries of no token in use are not
  * read. */
@@ -470,7 +476,8 @@ int tileops_paged_decode_fwd(const void* q, const void* k_cache, const void* v_c
                              float* lse, void* workspace, int64_t batch, int64_t heads,
                              int64_t heads_kv, int64_t dim, int64_t num_pages, int64_t page_size,
                              int64_t table_width, int64_t table_stride, const int64_t* strides8,
-                             int64_t window, double scale, int dtype, void* stream);
+                             int64_t window, int counters_zero, double scale, int dtype,
+                             void* stream);
 
 #ifdef __cplusplus
 }

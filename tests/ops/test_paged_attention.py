@@ -293,6 +293,70 @@ def test_repeats_to_the_bit_and_runs_on_two_streams():
         assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
 
 
+def test_a_kept_workspace_serves_calls_of_all_kinds():
+    """Calls of several sizes on one stream, each of which shares items among CTAs, from two host
+    threads and on two streams at once; the counters are zero behind them."""
+    import threading
+
+    from tileops.kernels.attention import paged_attention as kernels
+
+    made = []
+    for lens, H, Hkv, D in (([3000], 2, 1, 64), ([900, 5000, 0, 77], 16, 2, 128), ([2000] * 3, 4, 4, 192),
+                            ([4000, 4000], 40, 1, 96)):
+        table, pages = _table(lens, 16)
+        kc, vc = _cache(pages, 16, Hkv, D, torch.bfloat16), _cache(pages, 16, Hkv, D, torch.bfloat16)
+        q = torch.randn(len(lens), H, D, device="cuda").to(torch.bfloat16)
+        args = (q, kc, vc, table, _lens(lens))
+        made.append((PagedAttentionDecodeOp(H, Hkv, D, 16), args, ref.attend(*args)))
+    want = [op(*args) for op, args, _ in made]
+    for (o, lse), (_, _, exact) in zip(want, made):
+        assert_within(o, exact[0], exact[2])
+    wrong = []
+
+    def work(stream):
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                for (op, args, _), (o, lse) in zip(made, want):
+                    got = op(*args)
+                    if not (torch.equal(got[0], o) and torch.equal(got[1].nan_to_num(neginf=0.0),
+                                                                   lse.nan_to_num(neginf=0.0))):
+                        wrong.append(args[0].shape)
+
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    threads = [threading.Thread(target=work, args=(s,)) for s in (streams[0], streams[0], streams[1])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
+    for ws in kernels._workspaces.values():
+        assert not ws[:4 * 592].any()
+
+
+def test_a_graph_and_calls_beside_it():
+    """A captured step has a workspace of its own: replayed on one stream while calls run on another."""
+    lens = _lens([4000, 100])
+    table, pages = _table([4000, 100], 16)
+    kc, vc = _cache(pages, 16, 1, 64, torch.bfloat16), _cache(pages, 16, 1, 64, torch.bfloat16)
+    q = torch.randn(2, 2, 64, device="cuda").to(torch.bfloat16)
+    op = PagedAttentionDecodeOp(2, 1, 64, 16)
+    want = op(q, kc, vc, table, lens)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = op(q, kc, vc, table, lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(50):
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = op(q, kc, vc, table, lens)
+    torch.cuda.synchronize()
+    for o, lse in (got, beside):
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+
+
 def test_two_graphs_of_one_pool():
     """Two captured steps that may share their workspace's memory, replayed in turn with lengths
     that change between replays."""

@@ -403,7 +403,7 @@ def test_decode_entry_point_checks():
     def call(q=SOME, c=SOME, table=SOME, lens=SOME, out=SOME, ws=SOME, B=2, H=4, Hkv=2, D=8, pages=3, P=4,
              width=2, st=_ints(*[8] * 8), window=0, dtype=2):
         return fn(q, c, c, table, lens, out, out, ws, B, H, Hkv, D, pages, P, width, width, st, window,
-                  1.0, dtype, NULL)
+                  0, 1.0, dtype, NULL)
 
     for bad in (dict(B=-1), dict(H=3), dict(H=0), dict(Hkv=0), dict(D=12), dict(D=264), dict(D=0),
                 dict(pages=-1), dict(P=0), dict(P=2**30, width=2), dict(width=-1), dict(window=-1)):

@@ -20,9 +20,10 @@
 // whose units lie in one CTA is finished there; of one that lies in several, each writes its sums
 // and counts itself, and the last one to do so joins them all, in the order of the CTAs, so that
 // results repeat to the bit.  A CTA has at most two items it shares with others: its first and its
-// last.  (A second kernel for the joins cost 5 to 7 us a call.)  The counters are cleared by a
-// small kernel in front, beside which this one starts (programmatic launch: 0.6 us; clearing them by
-// a memset 4 us).
+// last.  (A second kernel for the joins cost 5 to 7 us a call.)  The counters are zero at the start
+// and whoever joins leaves its item's so; in a workspace of unknown contents they are cleared by a
+// small kernel in front, beside which this one starts (programmatic launch: 0.6 us on the device, 2 us
+// of the host; a memset 4 us).
 //
 // In a CTA each warp takes its tokens of a unit on its own: it copies their keys and values
 // with 16-byte cp.async through its own ring of stages (no CTA barrier), multiplies, and keeps a
@@ -47,7 +48,7 @@
 namespace tileops {
 namespace {
 
-constexpr int kMaxCtas = 4 * 148;  // four on each of a B200's SMs
+constexpr int kMaxCtas = TILEOPS_PAGED_DECODE_COUNTERS;  // four on each of a B200's 148 SMs
 constexpr float kNegInf = -__builtin_huge_valf();
 
 struct CacheStrides {
@@ -228,7 +229,7 @@ struct Layout {
   }
 };
 
-// Waits for the end of the kernel that clears the counters: before the first count, and before the
+// Waits for the end of the kernel that clears the counters (where there is one): before the first count, and before the
 // end, so that it has ended when what follows in the stream starts.
 __device__ __forceinline__ void behind_clearing() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -621,6 +622,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
                        : "l"(a.counters + owner)
                        : "memory");
           complete = count == static_cast<int>(end - owner);
+          if (complete) a.counters[owner] = 0;  // for the next call
         }
         __syncthreads();
         if (!complete) break;
@@ -675,9 +677,9 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(512) clear_counters(int* counters, int count) {
+__global__ void __launch_bounds__(512) clear_counters(int* counters) {
   asm volatile("griddepcontrol.launch_dependents;");
-  for (int n = threadIdx.x; n < count; n += 512) counters[n] = 0;
+  for (int n = threadIdx.x; n < kMaxCtas; n += 512) counters[n] = 0;
 }
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -712,7 +714,7 @@ bool opt_in() {
 }
 
 template <typename T, int DP, int MT, int WARPS>
-int launch_tile(const DecodeArgs& a, cudaStream_t s) {
+int launch_tile(const DecodeArgs& a, bool clear, cudaStream_t s) {
   using L = Layout<DP, MT, WARPS>;
   // Where heads lie side by side and share 128-byte lines, fewer CTAs: those of neighbouring heads then stay
   // close to each other in the tokens, and a line is fetched once (320 items of 8009 tokens x 80 189 us
@@ -723,7 +725,11 @@ int launch_tile(const DecodeArgs& a, cudaStream_t s) {
   const int64_t grid = std::min<int64_t>(
       {places_of(a, L::kUnit), static_cast<int64_t>(sm_count()) * ctas_sm, kMaxCtas});
   if (!opt_in<T, DP, MT, WARPS>()) return TILEOPS_ELAUNCH;
-  clear_counters<<<1, 512, 0, s>>>(a.counters, static_cast<int>(grid));
+  if (clear) {
+    paged_decode<T, DP, MT, WARPS><<<static_cast<unsigned>(grid), L::kThreads, L::kBytes, s>>>(a);
+    return launch_status();
+  }
+  clear_counters<<<1, 512, 0, s>>>(a.counters);
   if (int status = launch_status()) return status;
   // Starts once the first kernel has started, and so behind all that came before that one; the
   // CTAs wait for its end before they count.
@@ -743,7 +749,7 @@ int launch_tile(const DecodeArgs& a, cudaStream_t s) {
 }
 
 template <typename T, int DP, int MT>
-int launch_warps(const DecodeArgs& a, cudaStream_t s) {
+int launch_warps(const DecodeArgs& a, bool clear, cudaStream_t s) {
   // Few items are shared by many CTAs each: one CTA of 8 warps an SM, so that there are fewer sums to join
   // (32 items of 32768 tokens x 128 89 us, 94 with CTAs of 4; but 256 items of up to 4096 33 and 28 us).  Many
   // items: smaller CTAs, more of them at different points of an item (512 sequences of up to 256 tokens,
@@ -751,27 +757,27 @@ int launch_warps(const DecodeArgs& a, cudaStream_t s) {
   // Heads of 192 have no room for two CTAs of 4, nor heads of 256 for 8 warps.
   const int64_t items = static_cast<int64_t>(a.batch) * a.heads_kv * a.blocks;
   if constexpr (DP <= 192) {
-    if (items <= sm_count()) return launch_tile<T, DP, MT, 8>(a, s);
+    if (items <= sm_count()) return launch_tile<T, DP, MT, 8>(a, clear, s);
   }
   if constexpr (DP <= 128) {
-    if (items <= 4 * sm_count()) return launch_tile<T, DP, MT, 4>(a, s);
+    if (items <= 4 * sm_count()) return launch_tile<T, DP, MT, 4>(a, clear, s);
   }
   if constexpr (DP > 192) {
-    if (items <= sm_count()) return launch_tile<T, DP, MT, 4>(a, s);
+    if (items <= sm_count()) return launch_tile<T, DP, MT, 4>(a, clear, s);
   }
-  return launch_tile<T, DP, MT, 2>(a, s);
+  return launch_tile<T, DP, MT, 2>(a, clear, s);
 }
 
 template <typename T>
-int launch_type(const DecodeArgs& a, cudaStream_t s) {
+int launch_type(const DecodeArgs& a, bool clear, cudaStream_t s) {
   const int dp = padded_dim(a.dim);
   const bool wide = rows_of(a.group, dp) == 32;
   switch (dp) {
-    case 64: return wide ? launch_warps<T, 64, 2>(a, s) : launch_warps<T, 64, 1>(a, s);
-    case 96: return wide ? launch_warps<T, 96, 2>(a, s) : launch_warps<T, 96, 1>(a, s);
-    case 128: return wide ? launch_warps<T, 128, 2>(a, s) : launch_warps<T, 128, 1>(a, s);
-    case 192: return launch_warps<T, 192, 1>(a, s);
-    default: return launch_warps<T, 256, 1>(a, s);
+    case 64: return wide ? launch_warps<T, 64, 2>(a, clear, s) : launch_warps<T, 64, 1>(a, clear, s);
+    case 96: return wide ? launch_warps<T, 96, 2>(a, clear, s) : launch_warps<T, 96, 1>(a, clear, s);
+    case 128: return wide ? launch_warps<T, 128, 2>(a, clear, s) : launch_warps<T, 128, 1>(a, clear, s);
+    case 192: return launch_warps<T, 192, 1>(a, clear, s);
+    default: return launch_warps<T, 256, 1>(a, clear, s);
   }
 }
 
@@ -794,8 +800,8 @@ extern "C" int tileops_paged_decode_fwd(
     const void* q, const void* k_cache, const void* v_cache, const int32_t* page_table,
     const int32_t* seq_lens, void* o, float* lse, void* workspace, int64_t batch, int64_t heads,
     int64_t heads_kv, int64_t dim, int64_t num_pages, int64_t page_size, int64_t table_width,
-    int64_t table_stride, const int64_t* strides8, int64_t window, double scale, int dtype,
-    void* stream) {
+    int64_t table_stride, const int64_t* strides8, int64_t window, int counters_zero, double scale,
+    int dtype, void* stream) {
   if (bad_sizes(batch, heads, heads_kv, dim) || num_pages < 0 || num_pages > 0x7fffffffLL ||
       page_size < 1 || page_size > 0x7fffffffLL || table_width < 0 || table_width > 0x7fffffffLL ||
       page_size * table_width > 0x7fffffffLL - 128 || window < 0 || window > 0x7fffffffLL)
@@ -846,5 +852,6 @@ extern "C" int tileops_paged_decode_fwd(
   if (places_of(a, 32) > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
   a.err = device_error_ptr();
   cudaStream_t s = as_stream(stream);
-  return dtype == TILEOPS_DT_F16 ? launch_type<__half>(a, s) : launch_type<__nv_bfloat16>(a, s);
+  return dtype == TILEOPS_DT_F16 ? launch_type<__half>(a, counters_zero != 0, s)
+                                 : launch_type<__nv_bfloat16>(a, counters_zero != 0, s);
 }

@@ -93,7 +93,7 @@ _SIGNATURES: dict[str, list] = {
     "tileops_rotary": [_p] * 6 + [_i64] * 6 + [_p, _i64] + [_i] * 3 + [_d, _i, _p],
     "tileops_paged_kv_append": [_p] * 10 + [_i64] * 10 + [_p, _i, _d, _i, _p],
     "tileops_paged_decode_workspace_bytes": [_i64] * 3,
-    "tileops_paged_decode_fwd": [_p] * 8 + [_i64] * 8 + [_p, _i64, _d, _i, _p],
+    "tileops_paged_decode_fwd": [_p] * 8 + [_i64] * 8 + [_p, _i64, _i, _d, _i, _p],
     "tileops_device_error_flag": [_p, _i],
     "tileops_selftest_wait_timeout": [_p, _i64, _i64, _p, _p],
     "tileops_abi_version": [],

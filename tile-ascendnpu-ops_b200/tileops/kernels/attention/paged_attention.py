@@ -110,6 +110,26 @@ class PagedKVAppendKernel(Kernel):
         return q_out
 
 
+_workspaces: dict = {}  # (device, stream): the largest one that a call of it has needed
+
+
+def _workspace(device: torch.device, room: int):
+    """Scratch of ``room`` bytes on the current stream, and whether its counters are zero.
+
+    Calls of one stream run one after another and each leaves the counters at zero, so they share
+    a workspace that is kept (2.3 us a call less than one of its own that has to be cleared; torch's
+    streams live as long as the process).  A graph under capture, which may be replayed on any
+    stream, gets one of its own, cleared in the graph.
+    """
+    if device.type != "cuda" or torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(room, dtype=torch.uint8, device=device), False
+    key = device.index, torch._C._cuda_getCurrentRawStream(device.index)
+    found = _workspaces.get(key)
+    if found is None or found.numel() < room:
+        found = _workspaces[key] = torch.zeros(room, dtype=torch.uint8, device=device)
+    return found, True
+
+
 class PagedAttentionDecodeKernel(Kernel):
     """Attention of one new token of every sequence over a paged cache.
 
@@ -145,7 +165,7 @@ class PagedAttentionDecodeKernel(Kernel):
 
     def plan(self, q, k_cache, v_cache, page_table, seq_lens):
         """What a call of this layout needs, for ``forward``: device, which arguments have to be copied (never a cache), the stride array, the table's
-        stride and sizes, and the shapes of the outputs and the workspace."""
+        stride and sizes, the shapes of the outputs and the bytes of the workspace."""
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
             if not channels_last(c) or any(s % 8 for s, n in zip(c.stride()[:3], c.shape) if n > 1):
                 raise ValueError(f"{name} must have contiguous channels and strides that are "
@@ -161,13 +181,16 @@ class PagedAttentionDecodeKernel(Kernel):
         like = torch.empty(1, dtype=torch.float32, device=q.device)
         return (q.device, copy if any(copy) else None, (ctypes.c_int64 * 8)(*strides), table_stride,
                 batch, k_cache.shape[0], page_table.shape[1], row_of(q),
-                like.expand(batch, heads), like.expand(-(-room // 4)))
+                like.expand(batch, heads), room)
 
     def forward(self, q, k_cache, v_cache, page_table, seq_lens, plan=None):
         """Return ``(o, lse)``.  ``plan``: what ``plan()`` gave for arguments of the same layout."""
         if plan is None:
             plan = self.plan(q, k_cache, v_cache, page_table, seq_lens)
-        device, copy, strides, table_stride, batch, pages, columns, o_like, lse_like, ws_like = plan
+        device, copy, strides, table_stride, batch, pages, columns, o_like, lse_like, room = plan
+        if device.type == "cuda" and torch._C._cuda_getDevice() != device.index:
+            with torch.cuda.device(device):
+                return self.forward(q, k_cache, v_cache, page_table, seq_lens, plan)
         if copy is not None:
             q, page_table, seq_lens = (t.contiguous() if c else t
                                        for t, c in zip((q, page_table, seq_lens), copy))
@@ -176,10 +199,11 @@ class PagedAttentionDecodeKernel(Kernel):
             q = q.clone()
             at = q.data_ptr()
             strides = (ctypes.c_int64 * 8)(*q.stride()[:2], *strides[2:])
-        o, lse, ws = torch.empty_like(o_like), torch.empty_like(lse_like), torch.empty_like(ws_like)
+        o, lse = torch.empty_like(o_like), torch.empty_like(lse_like)
+        ws, counters_zero = _workspace(device, room)
         _native.launch(
             "tileops_paged_decode_fwd", device, at, k_cache.data_ptr(), v_cache.data_ptr(),
             page_table.data_ptr(), seq_lens.data_ptr(), o.data_ptr(), lse.data_ptr(),
             ws.data_ptr(), batch, self.heads, self.heads_kv, self.dim, pages, self.page_size,
-            columns, table_stride, strides, self.window, self.scale, self._code)
+            columns, table_stride, strides, self.window, counters_zero, self.scale, self._code)
         return o, lse
