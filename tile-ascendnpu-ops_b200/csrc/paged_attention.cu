@@ -229,8 +229,8 @@ struct Layout {
   }
 };
 
-// Waits for the end of the kernel that clears the counters (where there is one): before the first count, and before the
-// end, so that it has ended when what follows in the stream starts.
+// Waits for the end of the kernel that clears the counters (where there is one): before the first
+// count, and before the end, so that it has ended when what follows in the stream starts.
 __device__ __forceinline__ void behind_clearing() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

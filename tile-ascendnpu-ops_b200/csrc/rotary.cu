@@ -310,7 +310,9 @@ __global__ void __launch_bounds__(kThreads, 5) rotary_rows(const __grid_constant
           const float4 cs = *reinterpret_cast<const float4*>(w + e * (pairs / VEC) * 2);
           const float2 c2 = make_float2(cs.x, cs.y), s2 = make_float2(cs.z, cs.w);
           T* const first = INTER ? (2 * e < VEC ? x.e + 2 * e : y.e + (2 * e - VEC)) : x.e + e;
-          T* const other = !INTER ? y.e + e : 2 * e + 2 < VEC ? x.e + 2 * e + 2 : y.e + (2 * e + 2 - VEC);
+          T* const other = !INTER             ? y.e + e
+                           : 2 * e + 2 < VEC ? x.e + 2 * e + 2
+                                             : y.e + (2 * e + 2 - VEC);
           // INTER: pairs (0, 1) of `first` and `other` each; else pairs across the two vectors.
           const float2 a2 = INTER ? make_float2(Cvt<T>::to_f(first[0]), Cvt<T>::to_f(other[0]))
                                   : make_float2(Cvt<T>::to_f(first[0]), Cvt<T>::to_f(first[1]));
@@ -438,7 +440,8 @@ int launch_tiles(RotaryArgs& a, K kernel, uint32_t items, uint32_t groups, uint3
   if (grid > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
   // At least a thread for each token of the tile.
   threads = (std::max(threads, static_cast<uint32_t>(a.tile)) + 31) / 32 * 32;
-  kernel<<<static_cast<unsigned>(grid), threads, static_cast<size_t>(a.tile) * room * sizeof(float), s>>>(a);
+  const size_t smem = static_cast<size_t>(a.tile) * room * sizeof(float);
+  kernel<<<static_cast<unsigned>(grid), threads, smem, s>>>(a);
   return launch_status();
 }
 
@@ -456,8 +459,9 @@ int launch_vec(RotaryArgs& a, cudaStream_t s) {
   const uint32_t groups = (items + kThreads - 1) / kThreads;
   a.lanes = lanes_of(items, a.rotary);
   const uint32_t threads = ((items + groups - 1) / groups * a.lanes + 31) / 32 * 32;
-  return launch_tiles(a, a.interleaved ? rotary_rows<T, VEC, true, PAGED> : rotary_rows<T, VEC, false, PAGED>,
-                      items, groups, threads, a.rotary, s);
+  return launch_tiles(
+      a, a.interleaved ? rotary_rows<T, VEC, true, PAGED> : rotary_rows<T, VEC, false, PAGED>, items,
+      groups, threads, a.rotary, s);
 }
 
 template <typename T, int VEC, bool PAGED>
@@ -469,7 +473,9 @@ int launch_staged(RotaryArgs& a, cudaStream_t s) {
   const uint32_t items = (rows + groups - 1) / groups * a.per_row;
   const int room = 2 * ((a.rotary + VEC - 1) / VEC * VEC);
   a.lanes = groups == 1 ? lanes_of(items, room) : 1;
-  return launch_tiles(a, a.interleaved ? rotary_staged<T, VEC, true, PAGED> : rotary_staged<T, VEC, false, PAGED>, items, groups, items * a.lanes, room, s);
+  return launch_tiles(
+      a, a.interleaved ? rotary_staged<T, VEC, true, PAGED> : rotary_staged<T, VEC, false, PAGED>, items,
+      groups, items * a.lanes, room, s);
 }
 
 template <typename T, bool PAGED>
@@ -578,8 +584,9 @@ extern "C" int tileops_paged_kv_append(
     return TILEOPS_EBADSHAPE;
   if (!is_float_dtype(dtype)) return TILEOPS_EBADDTYPE;
   if (tokens == 0) return TILEOPS_OK;
-  if ((heads && (!q || !q_out)) || !k || !v || !k_cache || !v_cache ||
-      k_cache == v_cache || !strides18 || (num_seqs && !seq_lens) || (num_seqs && table_width && !page_table) || (rotary_dim && !turns))
+  if ((heads && (!q || !q_out)) || !k || !v || !k_cache || !v_cache || k_cache == v_cache ||
+      !strides18 || (num_seqs && !seq_lens) || (num_seqs && table_width && !page_table) ||
+      (rotary_dim && !turns))
     return TILEOPS_EINVAL;
   RotaryArgs a{};
   a.q = q;

@@ -54,8 +54,9 @@ class PagedKVAppendKernel(Kernel):
         self.init_config(config)
 
     def plan(self, k, v, k_cache, v_cache, page_table, seq_lens, q=None, cu_seqlens=None):
-        """What a call of this layout needs, for ``forward``: device, which arguments have to be copied, the stride array, the table's stride, the rows and
-        the queries' shape; refuses caches that cannot be written."""
+        """What a call of this layout needs, for ``forward``: device, which arguments have to be
+        copied, the stride array, the table's stride, the rows and the queries' shape; refuses caches
+        that cannot be written."""
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
             if not channels_last(c):
                 raise ValueError(f"{name} must have contiguous channels, got strides {c.stride()}")
@@ -102,9 +103,9 @@ class PagedKVAppendKernel(Kernel):
         q_out = None if q is None else torch.empty_like(q_like)
         _native.launch(
             "tileops_paged_kv_append", device, 0 if q is None else q.data_ptr(), k.data_ptr(),
-            v.data_ptr(), 0 if q is None else q_out.data_ptr(), k_at, v_at, page_table.data_ptr(), seq_lens.data_ptr(),
-            0 if cu_seqlens is None else cu_seqlens.data_ptr(), self._turns, seqs, tokens,
-            0 if q is None else self.heads, self.heads_kv, self.dim, self.rotary_dim, pages,
+            v.data_ptr(), 0 if q is None else q_out.data_ptr(), k_at, v_at, page_table.data_ptr(),
+            seq_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(), self._turns, seqs,
+            tokens, 0 if q is None else self.heads, self.heads_kv, self.dim, self.rotary_dim, pages,
             self.page_size, columns, table_stride, strides, self.interleaved, self.amplitude,
             self._code)
         return q_out
@@ -164,8 +165,9 @@ class PagedAttentionDecodeKernel(Kernel):
         self.init_config(config)
 
     def plan(self, q, k_cache, v_cache, page_table, seq_lens):
-        """What a call of this layout needs, for ``forward``: device, which arguments have to be copied (never a cache), the stride array, the table's
-        stride and sizes, the shapes of the outputs and the bytes of the workspace."""
+        """What a call of this layout needs, for ``forward``: device, which arguments have to be
+        copied (never a cache), the stride array, the table's stride and sizes, the shapes of the
+        outputs and the bytes of the workspace."""
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
             if not channels_last(c) or any(s % 8 for s, n in zip(c.stride()[:3], c.shape) if n > 1):
                 raise ValueError(f"{name} must have contiguous channels and strides that are "

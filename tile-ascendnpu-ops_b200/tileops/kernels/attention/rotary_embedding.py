@@ -69,8 +69,8 @@ class _RotaryEmbeddingKernel(Kernel):
         self.init_config(config)
 
     def plan(self, q, k, positions=None, inplace: bool = False):
-        """What a call of this layout needs, for ``forward``: device, whether q, k and positions have to be copied, the stride array, the positions'
-        stride and type, and the outputs' shapes."""
+        """What a call of this layout needs, for ``forward``: device, whether q, k and positions have
+        to be copied, the stride array, the positions' stride and type, and the outputs' shapes."""
         copy = tuple(t is not None and not channels_last(t) and not inplace for t in (q, k))
         like = tuple(None if t is None or inplace else row_of(t) for t in (q, k))
         values = []
