@@ -20,6 +20,7 @@ from tileops.kernels.attention import (
 )
 from tileops.kernels.attention._layouts import Layouts, layout_of, overlaps
 from tileops.kernels.attention.rotary_embedding import turns_array
+from tileops.kernels.kernel_base import Kernel
 from tileops.manifest import load_workloads
 from tileops.ops.attention import (
     PagedAttentionDecodeOp,
@@ -351,6 +352,33 @@ def test_kernel_maps():
             (PagedKVAppendOp(1, 8, 4), "paged_kv_append", PagedKVAppendKernel),
             (PagedAttentionDecodeOp(1, 1, 8, 4), "paged_attention_decode", PagedAttentionDecodeKernel)):
         assert op.default_kernel_map == {key: cls} and type(op.kernel) is cls
+
+
+def test_kernel_overrides_need_a_forward_only(accept_cpu):
+    """What a kernel_map puts in a kernel's place gets the op's arguments, after its checks."""
+    seen = []
+
+    class Other(Kernel):
+        def __init__(self, *args):
+            super().__init__()
+
+        def forward(self, *args):
+            seen.append(args)
+            return "done"
+
+    q, k = _rotary_args()
+    op = RotaryEmbeddingFwdOp(2, 5, 4, 2, 8, dtype=torch.float32, kernel_map={"rotary_fwd": Other})
+    for _ in range(2):
+        assert op(q, k) == "done" and seen.pop() == (q, k, None, False)
+    with pytest.raises(ValueError, match="q.shape"):
+        op(q[:1], k)
+    args = _paged(torch.float16)
+    op = PagedKVAppendOp(2, 8, 4, 4, dtype=torch.float16, kernel_map={"paged_kv_append": Other})
+    assert op(**args) == "done" and seen.pop()[6] is args["q"]
+    del args["k"], args["v"]
+    op = PagedAttentionDecodeOp(4, 2, 8, 4, dtype=torch.float16,
+                                kernel_map={"paged_attention_decode": Other})
+    assert op(**args) == "done" and len(seen.pop()) == 5
 
 
 # ------------------------------------------------------------ C entry points

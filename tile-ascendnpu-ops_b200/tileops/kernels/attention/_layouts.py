@@ -11,7 +11,7 @@ from typing import Sequence
 
 import torch
 
-__all__ = ["Layouts", "channels_last", "layout_of", "overlaps", "row_of"]
+__all__ = ["Layouts", "NO_PLAN", "channels_last", "layout_of", "overlaps", "plan_of", "row_of"]
 
 
 def layout_of(*tensors):
@@ -33,6 +33,16 @@ class Layouts(dict):
                 self.clear()
             self[layout] = found
         return found
+
+
+NO_PLAN = ()
+
+
+def plan_of(kernel, *args):
+    """What a kernel works out once for a layout; NO_PLAN of one (an op's override) that only has a
+    ``forward``."""
+    plan = getattr(kernel, "plan", None)
+    return NO_PLAN if plan is None else plan(*args)
 
 
 def overlaps(shape: Sequence[int], strides: Sequence[int]) -> bool:

@@ -43,7 +43,7 @@ import torch
 
 from tileops.device import get_device_backend
 from tileops.kernels.attention import PagedAttentionDecodeKernel, PagedKVAppendKernel
-from tileops.kernels.attention._layouts import Layouts, layout_of
+from tileops.kernels.attention._layouts import NO_PLAN, Layouts, layout_of, plan_of
 from tileops.kernels.kernel_base import Kernel
 from tileops.ops.attention._arguments import check_tensor
 from tileops.ops.attention.rotary_embedding import rotary_frequencies
@@ -111,9 +111,11 @@ class PagedKVAppendOp(Op):
         plan = self._plans.get(layout)
         if plan is None:
             self._check(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
-            plan = self._plans.keep(layout, self.kernel.plan(k, v, k_cache, v_cache, page_table,
-                                                             seq_lens, q, cu_seqlens))
+            plan = self._plans.keep(layout, plan_of(self.kernel, k, v, k_cache, v_cache, page_table,
+                                                    seq_lens, q, cu_seqlens))
         self._last = layout[0][0], q is not None
+        if plan is NO_PLAN:
+            return self.kernel(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
         return self.kernel.forward(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens, plan)
 
     def _check(self, k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens) -> None:
@@ -191,8 +193,11 @@ class PagedAttentionDecodeOp(Op):
         plan = self._plans.get(layout)
         if plan is None:
             self._check(q, k_cache, v_cache, page_table, seq_lens)
-            plan = self._plans.keep(layout, self.kernel.plan(q, k_cache, v_cache, page_table, seq_lens))
+            plan = self._plans.keep(layout, plan_of(self.kernel, q, k_cache, v_cache, page_table,
+                                                    seq_lens))
         self._last = layout[3][0]
+        if plan is NO_PLAN:
+            return self.kernel(q, k_cache, v_cache, page_table, seq_lens)
         return self.kernel.forward(q, k_cache, v_cache, page_table, seq_lens, plan)
 
     def _check(self, q, k_cache, v_cache, page_table, seq_lens) -> None:

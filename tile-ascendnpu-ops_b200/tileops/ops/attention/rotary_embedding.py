@@ -34,7 +34,14 @@ import torch
 
 from tileops.device import get_device_backend
 from tileops.kernels.attention import RotaryEmbeddingBwdKernel, RotaryEmbeddingFwdKernel
-from tileops.kernels.attention._layouts import Layouts, channels_last, layout_of, overlaps
+from tileops.kernels.attention._layouts import (
+    NO_PLAN,
+    Layouts,
+    channels_last,
+    layout_of,
+    overlaps,
+    plan_of,
+)
 from tileops.kernels.kernel_base import Kernel
 from tileops.ops.attention._arguments import check_tensor
 from tileops.ops.op_base import Op
@@ -104,10 +111,12 @@ class _RotaryEmbeddingOp(Op):
             self._check(q, k, positions)
             if q is None and k is None:
                 return None, None
-            plan = self._plans.keep(layout, self.kernel.plan(q, k, positions, self.inplace))
+            plan = self._plans.keep(layout, plan_of(self.kernel, q, k, positions, self.inplace))
         if self.inplace and q is not None and k is not None and q.data_ptr() == k.data_ptr() != 0:
             raise ValueError(f"{self._names[0]} and {self._names[1]} share memory: they cannot both "
                              "be rotated in place")
+        if plan is NO_PLAN:
+            return self.kernel(q, k, positions, self.inplace)
         return self.kernel.forward(q, k, positions, self.inplace, plan)
 
     def _check(self, q, k, positions) -> None:
