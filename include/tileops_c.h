@@ -458,7 +458,7 @@ int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t heads_kv, in
  * heads, dim) of `dtype` (f16 / bf16) dense, lse (batch, heads) fp32 in the log2
  * domain.  Query head h reads key head h / (heads / heads_kv).  A sequence of
  * no token (seq_lens[b] <= 0) has o = 0 and lse = -inf.  dim a multiple of 8 up
- * to 256, page_size * table_width < 2^31 - 128, and fewer than 2^31 units of 64
+ * to 256, page_size * table_width < 2^31 - 128, and fewer than 2^31 units of 32
  * tokens a key head in all, were every sequence as long as its table.  strides8
  * (HOST, multiples of 8): elements from a sequence and head to the next of q,
  * from a page, slot and head to the next of k_cache and of v_cache.  q, caches,
@@ -467,10 +467,9 @@ int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t heads_kv, in
  * TILEOPS_PAGED_DECODE_COUNTERS int32 are counters: `counters_zero` says that
  * they are zero (the call leaves them so: of a workspace that is kept for one
  * stream they need clearing once); else the call clears them first, with a kernel
- * more.  A seq_lens[b] above page_size *
- * table_width (taken as that) or a page outside [0, num_pages) (taken as zeros)
- * sets the device error flag to 3; table entries of no token in use are not
- * read. */
+ * more.  A seq_lens[b] above page_size * table_width (taken as that) or a page
+ * outside [0, num_pages) (taken as zeros) sets the device error flag to 3; table
+ * entries of no token in use are not read. */
 int tileops_paged_decode_fwd(const void* q, const void* k_cache, const void* v_cache,
                              const int32_t* page_table, const int32_t* seq_lens, void* o,
                              float* lse, void* workspace, int64_t batch, int64_t heads,

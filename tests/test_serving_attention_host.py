@@ -436,7 +436,7 @@ def test_decode_entry_point_checks():
     for bad in (dict(B=-1), dict(H=3), dict(H=0), dict(Hkv=0), dict(D=12), dict(D=264), dict(D=0),
                 dict(pages=-1), dict(P=0), dict(P=2**30, width=2), dict(width=-1), dict(window=-1)):
         assert call(**bad) == _native.EBADSHAPE, bad
-    # 2^31 and more units of 64 tokens
+    # 2^31 and more units of 32 tokens
     assert call(B=2**20, H=32, Hkv=32, P=64, width=2**10) == _native.EBADSHAPE
     assert call(dtype=0) == _native.EBADDTYPE and call(dtype=7) == _native.EBADDTYPE
     for bad in (dict(q=NULL), dict(c=NULL), dict(table=NULL), dict(lens=NULL), dict(out=NULL),
