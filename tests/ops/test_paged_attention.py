@@ -547,3 +547,39 @@ def test_append_refused_on_the_device_sets_the_flag():
     for cu in ([0, 15, 10], [3, 5, 20], [0, 5, 21], [0, 2**31 - 1, -(2**31)]):
         op(k, v, kc, vc, table, _lens([20, 20]), None, torch.tensor(cu, dtype=torch.int32, device="cuda"))
         assert _flag() in (2, 3)
+
+
+# ------------------------------------------------------------ scores of any size
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("scale", [1e3, 1e4, 1e6, -1e6, 1e8, 2.0**100])
+@pytest.mark.parametrize("n", [30, 1000, 30000])
+def test_scores_of_any_size(n, scale, dtype):
+    """A weight is relative to the largest score's, whose own is 1 whatever the scale: a key far above
+    the others takes all, wherever it lies among warps and CTAs, and two such keys half each."""
+    D, P = 64, 16
+    table, pages = _table([n], P)
+    kc, vc = _cache(pages, P, 1, D, dtype), _cache(pages, P, 1, D, dtype)
+    kc.mul_(0.01)
+    q = torch.ones(1, 3, D, device="cuda", dtype=dtype)
+    op = PagedAttentionDecodeOp(3, 1, D, P, scale, dtype=dtype)
+
+    def slot(at):
+        return int(table[0, at // P]), at % P
+
+    for size in (40.0, 38.75, 12.125):  # sums of 64 of them are exact in both types
+        size = math.copysign(size, scale)
+        for first, second in ((0, n - 1), (n // 2, 3), (n - 1, n // 3)):
+            kept = kc.clone()
+            top = abs(64 * size * scale) / math.log(2.0)
+            kc[slot(first)] = size
+            o, lse = op(q, kc, vc, table, _lens([n]))
+            assert torch.equal(o[0], vc[slot(first)].expand(3, D)), (size, first)
+            # log2(e) scale, its product with the score and the sum round once each
+            assert ((lse.double() - top).abs() <= 4 * ref.U * top).all(), (size, first, lse)
+            kc[slot(second)] = size
+            o, lse = op(q, kc, vc, table, _lens([n]))
+            a, b = (vc[slot(at)].double().expand(3, D).cpu() for at in (first, second))
+            # the sum may cut (2 u of its terms), its product with 1 / 2 rounds
+            assert_within(o[0], (a + b) / 2, 4 * ref.U * (a.abs() + b.abs()))
+            assert ((lse.double() - (top + 1)).abs() <= 4 * ref.U * (top + 1)).all(), (size, second, lse)
+            kc.copy_(kept)

@@ -61,7 +61,7 @@ struct DecodeArgs {
   void* o;
   float* lse;
   int* counters;    // [CTA]: how many CTAs have written their sums of the item that it begins
-  float2* stats;    // [CTA][2][row]: exponent the sums are relative to, sum of weights
+  float2* stats;    // [CTA][2][row]: score the sums are relative to, sum of weights
   // [CTA][2][row][D, of 16 channels each]: weighted sums, of 16 channels the four of a lane's fragment
   // together (2 t, 2 t + 1, 8 + 2 t, 9 + 2 t), so that they are read by 16 bytes.
   float* partial;
@@ -118,6 +118,10 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
                : "memory");
 }
 
+// A weight is exp2((s - top) scale), top the largest score so far: the difference is taken before it is
+// scaled, so the largest weight is 1 to the bit however large scores are.  (Rounded exponents instead,
+// s scale - round(top scale) by one fma, leave the largest weight at 2^r, r up to half a step of top scale:
+// from 2^25 on fp16 weights overflow, or all vanish.)  A pair of scores takes two instructions either way.
 // Weights go to the second product in the inputs' type, half a step (2^-8 in bf16, 2^-11 in fp16) off
 // each; their sum takes them unrounded.  In fp16 they are held times 2^15 (the largest is 2^15), so that
 // weights down to 2^-29 of the largest keep all their bits.
@@ -133,6 +137,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 template <typename T>
 __device__ constexpr float kShift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
+template <typename T>
+__device__ constexpr float kUnshift = std::is_same<T, __half>::value ? 0x1p-15f : 1.0f;
 
 // A sequence's tokens, and units of them.
 struct Span {
@@ -421,7 +427,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
   }
 
   // ---- products ----
-  // top: the exponent that a row's weights are relative to, its largest score (in fp16 less 15).
+  // top: the score that a row's weights are relative to, its largest.
   float out[MT][DP / 8][4], top[MT][2], sum[MT][2];
   auto reset = [&]() {
 #pragma unroll
@@ -495,16 +501,19 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
             high = fmaxf(high, fmaxf(s[m][n][2 * r], s[m][n][2 * r + 1]));
           high = fmaxf(high, __shfl_xor_sync(~0u, high, 1));
           high = fmaxf(high, __shfl_xor_sync(~0u, high, 2));
-          const float top_new = fmaxf(fmaf(high, a.scale, -kShift<T>), top[m][r]);
+          const float top_new = fmaxf(high, top[m][r]);
           // A row of nothing but -inf so far: exp2(-inf - 0) = 0, not exp2(-inf + inf).
           const float base = top_new == kNegInf ? 0.0f : top_new;
-          const float fade = ex2_approx_f(top[m][r] - base);
+          const float fade = ex2_approx_f((top[m][r] - base) * a.scale);
           top[m][r] = top_new;
           float add = 0.0f;
 #pragma unroll
           for (int n = 0; n < 2 * kBlocks; ++n) {
-            const float w0 = ex2_approx_f(fmaf(s[m][n][2 * r], a.scale, -base));
-            const float w1 = ex2_approx_f(fmaf(s[m][n][2 * r + 1], a.scale, -base));
+            const float2 less = fadd2(make_float2(s[m][n][2 * r], s[m][n][2 * r + 1]),
+                                      make_float2(-base, -base));
+            const float2 t = ffma2(less, make_float2(a.scale, a.scale),
+                                   make_float2(kShift<T>, kShift<T>));
+            const float w0 = ex2_approx_f(t.x), w1 = ex2_approx_f(t.y);
             add += w0 + w1;
             w[m][n / 2][n % 2 * 2 + r] = pack2<T>(w0, w1);
           }
@@ -588,7 +597,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int x = 0; x < WARPS; ++x) {
-              const float f = ex2_approx_f(st[x].x - base);
+              const float f = ex2_approx_f((st[x].x - base) * a.scale);
               const float* p = reinterpret_cast<const float*>(
                   smem + (x * L::kStages + stage) * (2 * L::kTile * 2)) + r * kPad;
               const float2 p0 = *reinterpret_cast<const float2*>(p + c0);
@@ -602,7 +611,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
             if (whole) {
               const int64_t at = static_cast<int64_t>(get.b) * a.heads + h0 + row;
               store_row(static_cast<T*>(a.o) + at * a.dim + d0, v, all);
-              if (quad == 0) a.lse[at] = base + log2f(all);
+              if (quad == 0) a.lse[at] = fmaf(base, a.scale, log2f(all * kUnshift<T>));
             } else {
               const int64_t at = (c * 2 + (began ? 1 : 0)) * a.part_rows + row;
               *reinterpret_cast<float4*>(a.partial + at * a.part_dim + quad * 4) = v;
@@ -647,7 +656,8 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
               const float top_new = fmaxf(top[m][r], st.x);
               const float base = top_new == kNegInf ? 0.0f : top_new;
-              const float fade = ex2_approx_f(top[m][r] - base), f = ex2_approx_f(st.x - base);
+              const float fade = ex2_approx_f((top[m][r] - base) * a.scale);
+              const float f = ex2_approx_f((st.x - base) * a.scale);
               top[m][r] = top_new;
               sum[m][r] = sum[m][r] * fade + ((lane & 3) == 0 ? f * st.y : 0.0f);
 #pragma unroll
