@@ -583,3 +583,35 @@ def test_scores_of_any_size(n, scale, dtype):
             assert_within(o[0], (a + b) / 2, 4 * ref.U * (a.abs() + b.abs()))
             assert ((lse.double() - (top + 1)).abs() <= 4 * ref.U * (top + 1)).all(), (size, second, lse)
             kc.copy_(kept)
+
+
+# ------------------------------------------------------------ the longest sequences
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("window", [None, 300, 2**30])
+@pytest.mark.parametrize("P, columns", [(2**31 - 129, 1), (21474835, 100), (17043519, 126)])
+def test_the_longest_sequences(P, columns, window, dtype):
+    """As many tokens as a table may have room for, in pages whose slots all lie in one place: units
+    of 256 tokens end beyond 2^31.  The values of the first pages are 1, of the last tenth 3; all
+    keys are alike."""
+    D, room = 8, P * columns
+    assert 2**31 - 255 <= room <= 2**31 - 129
+    kc = torch.ones(2, 1, 1, D, device="cuda", dtype=dtype).expand(2, P, 1, D)
+    vc = (kc[:, :1] * torch.tensor([1.0, 3.0], device="cuda", dtype=dtype)[:, None, None, None]).expand(2, P, 1, D)
+    first = columns - columns // 10  # page of the first 3
+    table = (torch.arange(columns, device="cuda")[None] >= first).to(torch.int32)
+    q = torch.ones(1, 1, D, device="cuda", dtype=dtype)
+    op = PagedAttentionDecodeOp(1, 1, D, P, 0.25, window, dtype)
+    for n in (room, room - 1, room - 254) if window == 300 else (room,):
+        o, lse = op(q, kc, vc, table, _lens([n]))
+        seen = min(n, window or n)
+        threes = min(seen, max(0, n - first * P))
+        want = torch.full((1, 1, D), 1.0 + 2.0 * threes / seen, dtype=torch.float64)
+        # A warp's sums are whole numbers below 2^24; those of 8 warps and up to 148 CTAs round.
+        assert_within(o, want, 64 * ref.U * want, f"o, {n} tokens")
+        want = math.log2(seen) + 2.0 / math.log(2.0)
+        assert abs(float(lse) - want) <= 8 * ref.U * want + 64 * ref.U, (n, float(lse), want)
+    if window:
+        got = op(q, kc, vc, table, _lens([2**31 - 1]))  # longer than the table: taken as its room
+        assert _flag() == 3
+        for a, b in zip(got, op(q, kc, vc, table, _lens([room]))):
+            assert torch.equal(a, b)

@@ -140,15 +140,18 @@ __device__ constexpr float kShift = std::is_same<T, __half>::value ? 15.0f : 0.0
 template <typename T>
 __device__ constexpr float kUnshift = std::is_same<T, __half>::value ? 0x1p-15f : 1.0f;
 
-// A sequence's tokens, and units of them.
+// A sequence's tokens, and units of them.  Tokens are below 2^31, those of the last unit's behind the end
+// may not be: sums of them are unsigned.
 struct Span {
-  int begin, end, units;
+  uint32_t begin, end;
+  int units;
 };
 template <int UNIT>
 __device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
   Span s;
-  s.end = min(max(a.lens[b], 0), a.room);
-  s.begin = a.window > 0 ? max(s.end - a.window, 0) : 0;
+  const int end = min(max(a.lens[b], 0), a.room);
+  s.end = end;
+  s.begin = a.window > 0 ? max(end - a.window, 0) : 0;
   s.units = (s.end - s.begin + UNIT - 1) / UNIT;
   return s;
 }
@@ -253,6 +256,10 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   Looked* const ahead = reinterpret_cast<Looked*>(smem + L::kRing + L::kQ + L::kStats) + warp * L::kAhead;
   const int heads = a.heads_kv * a.blocks;
+  // The first of this warp's tokens in a unit.
+  auto first_token = [&](const Unit& u) {
+    return u.span.begin + static_cast<uint32_t>(u.unit) * kUnit + warp * L::kTokens;
+  };
 
   // ---- places of the call ----
   // By each warp on its own: every lane takes as many sequences, and then the lane whose sequences
@@ -367,7 +374,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     if (look.place >= u1) {
       u.b = -1;
     } else {
-      const int t = u.span.begin + u.unit * kUnit + warp * L::kTokens + lane;
+      const uint32_t t = first_token(u) + lane;
       if (lane < L::kTokens && t < u.span.end)
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(&w.page[lane])),
                      "l"(a.table + u.b * a.table_stride + a.div_page.div(t))
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     const Looked& w = ahead[slot];
     const Unit u = w.u;
     if (u.b < 0) return;
-    const int t = u.span.begin + u.unit * kUnit + warp * L::kTokens + lane;
+    const uint32_t t = first_token(u) + lane;
     const int head = u.head / a.blocks;
     const T* k = static_cast<const T*>(a.k) + head * a.ks.head;
     const T* v = static_cast<const T*>(a.v) + head * a.vs.head;
@@ -393,7 +400,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     if (inside) {
       const int page = w.page[lane];
       if (page >= 0 && page < a.num_pages) {
-        const int place = t - static_cast<int>(a.div_page.div(t)) * a.page_size;
+        const int place = static_cast<int>(t - a.div_page.div(t) * a.page_size);
         k_at = page * a.ks.page + place * a.ks.slot;
         v_at = page * a.vs.page + place * a.vs.slot;
       } else {
@@ -457,7 +464,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
     const bool ended = get.unit + 1 == get.span.units;
     if (ended && !last) fetch_q(ahead[slot + 1 == L::kAhead ? 0 : slot + 1].u);
     const uint32_t keys = ring + stage * (2 * L::kTile * 2), values = keys + L::kTile * 2;
-    const int t0 = get.span.begin + get.unit * kUnit + warp * L::kTokens;
+    const uint32_t t0 = first_token(get);
     if (t0 < get.span.end) {
       constexpr int kBlocks = L::kTokens / 16;
       float s[MT][2 * kBlocks][4];
