@@ -615,3 +615,42 @@ def test_the_longest_sequences(P, columns, window, dtype):
         assert _flag() == 3
         for a, b in zip(got, op(q, kc, vc, table, _lens([room]))):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------ streams
+def test_streams_that_are_not_torchs():
+    """An external stream's calls keep nothing; the per-thread default stream, one handle and a stream
+    in each thread, serves threads at once; torch's own streams are told apart by their numbers."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from tileops.kernels.attention import paged_attention as kernels
+
+    own = torch.cuda.Stream()
+    assert own.stream_id % 2 == 1 and torch.cuda.default_stream().stream_id == 0
+    external = torch.cuda.ExternalStream(own.cuda_stream)
+    assert external.stream_id == own.cuda_stream and external.stream_id % 2 == 0
+    made = []
+    for lens, H, Hkv, D in (([3000, 20], 2, 1, 64), ([900, 5000, 0, 77], 16, 2, 128), ([9000], 40, 1, 96)):
+        table, pages = _table(lens, 16)
+        kc, vc = _cache(pages, 16, Hkv, D, torch.bfloat16), _cache(pages, 16, Hkv, D, torch.bfloat16)
+        q = torch.randn(len(lens), H, D, device="cuda").to(torch.bfloat16)
+        args = (q, kc, vc, table, _lens(lens))
+        op = PagedAttentionDecodeOp(H, Hkv, D, 16)
+        made.append((op, args, op(*args)))
+    torch.cuda.synchronize()
+    kept = dict(kernels._workspaces)
+
+    def work(handle):
+        with torch.cuda.stream(torch.cuda.ExternalStream(handle)):
+            return [(n, op(*args)) for _ in range(40) for n, (op, args, _) in enumerate(made)]
+
+    per_thread = 2
+    with ThreadPoolExecutor(3) as pool:
+        runs = [pool.submit(work, h) for h in (per_thread, per_thread, per_thread, own.cuda_stream)]
+        got = [r.result() for r in runs]
+        torch.cuda.synchronize()
+    for calls in got:
+        assert len(calls) == 40 * len(made)
+        for n, (o, lse) in calls:
+            assert torch.equal(o, made[n][2][0]) and torch.equal(lse, made[n][2][1])
+    assert kernels._workspaces.keys() == kept.keys()

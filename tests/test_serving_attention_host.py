@@ -492,3 +492,43 @@ def test_ops_are_rebuilt_from_their_attributes():
         again = type(op)(**_extract_op_init_args(op))
         assert _extract_op_init_args(again) == _extract_op_init_args(op)
         assert len(_extract_op_init_args(op)) >= 7
+
+
+# ------------------------------------------------------------ kept workspaces
+def test_a_workspace_is_shared_only_by_calls_one_after_another(monkeypatch):
+    """torch's own streams keep one each; others (their number is their handle) may be destroyed and
+    their handle given again, and one handle, 2, is another stream in each host thread."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from tileops.kernels.attention import paged_attention as kernels
+
+    now = dict(number=0, handle=0, capturing=False)
+    monkeypatch.setattr(kernels, "_workspaces", {})
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: now["capturing"], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: now["handle"], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentStream", lambda i: (now["number"], i, 1), raising=False)
+    for name in ("empty", "zeros"):
+        real = getattr(torch, name)
+        monkeypatch.setattr(torch, name, lambda n, dtype, device, real=real: real(n, dtype=dtype))
+
+    def ask(room=64, device=0, **stream):
+        now.update(dict(number=0, handle=0, capturing=False), **stream)
+        return kernels._workspace(torch.device("cuda", device), room)
+
+    default, pool = ask(), ask(number=3, handle=0x7000)
+    assert default[1] and pool[1] and default[0] is not pool[0]
+    assert ask()[0] is default[0] and ask(number=3, handle=0x7000)[0] is pool[0]
+    assert ask(device=1)[0] is not default[0]
+    larger = ask(room=128)
+    assert larger[0].numel() == 128 and larger[1] and ask()[0] is larger[0]
+    assert not ask(capturing=True)[1] and ask(capturing=True)[0] is not larger[0]
+    kept = len(kernels._workspaces)
+    other = [ask(number=0x8000, handle=0x8000) for _ in range(2)]
+    assert other[0][0] is not other[1][0] and not other[0][1] and not other[1][1]
+    assert len(kernels._workspaces) == kept
+    here = ask(number=2, handle=2)
+    with ThreadPoolExecutor(1) as pool:
+        there = pool.submit(ask, number=2, handle=2).result()
+    assert here[0] is not there[0] and here[0] is not other[0][0]
+    if here[1]:
+        assert ask(number=2, handle=2)[0] is here[0]

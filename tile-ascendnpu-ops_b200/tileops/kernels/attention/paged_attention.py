@@ -10,6 +10,7 @@ transposed view.
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Optional, Sequence
 
 import torch
@@ -111,23 +112,34 @@ class PagedKVAppendKernel(Kernel):
         return q_out
 
 
-_workspaces: dict = {}  # (device, stream): the largest one that a call of it has needed
+_workspaces: dict = {}  # (device, stream's number): the largest one that a call of it has needed
+_of_thread = threading.local()  # the same for the thread's per-thread default stream
+_PER_THREAD_DEFAULT = 2  # handle (and number) of that stream
 
 
 def _workspace(device: torch.device, room: int):
     """Scratch of ``room`` bytes on the current stream, and whether its counters are zero.
 
     Calls of one stream run one after another and each leaves the counters at zero, so they share
-    a workspace that is kept (2.3 us a call less than one of its own that has to be cleared; torch's
-    streams live as long as the process).  A graph under capture, which may be replayed on any
-    stream, gets one of its own, cleared in the graph.
+    a workspace that is kept (2.3 us a call less than one of its own that has to be cleared).  That
+    holds for torch's own streams, which live as long as the process: the default one, number 0, and
+    those of its pool, of odd numbers.  Another stream's number is its handle, an even one, which the next
+    stream may get while this one's last call still runs: a call there gets a workspace of its own, cleared.
+    The per-thread default stream is a stream in each thread, and so is what is kept for it.  A graph
+    under capture, which may be replayed on any stream, gets one of its own, cleared in the graph.
     """
     if device.type != "cuda" or torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(room, dtype=torch.uint8, device=device), False
-    key = device.index, torch._C._cuda_getCurrentRawStream(device.index)
-    found = _workspaces.get(key)
+    stream = torch._C._cuda_getCurrentStream(device.index)[0]
+    kept = _workspaces
+    if stream % 2 == 0 and stream != 0:
+        if stream != _PER_THREAD_DEFAULT:
+            return torch.empty(room, dtype=torch.uint8, device=device), False
+        kept = _of_thread.__dict__
+    key = device.index, stream
+    found = kept.get(key)
     if found is None or found.numel() < room:
-        found = _workspaces[key] = torch.zeros(room, dtype=torch.uint8, device=device)
+        found = kept[key] = torch.zeros(room, dtype=torch.uint8, device=device)
     return found, True
 
 

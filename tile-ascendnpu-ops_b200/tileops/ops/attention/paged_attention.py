@@ -32,7 +32,8 @@ multiples of 8.
 Offsets that break their rule set the device error flag to 2; a token in use without a page in
 [0, num_pages) sets it to 3 (its slot is not written, its key and value count as zeros).  A
 device's first call looks that flag up: make it outside a graph's capture.  The decode op keeps a
-workspace of some MB for each stream that it is called on; captured calls have their own.
+workspace of some MB for each of torch's streams that it is called on; captured calls and those on
+other streams have their own.
 """
 
 from __future__ import annotations
