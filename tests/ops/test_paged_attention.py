@@ -654,3 +654,19 @@ def test_streams_that_are_not_torchs():
         for n, (o, lse) in calls:
             assert torch.equal(o, made[n][2][0]) and torch.equal(lse, made[n][2][1])
     assert kernels._workspaces.keys() == kept.keys()
+
+
+# ------------------------------------------------------------ small scales
+@pytest.mark.parametrize("scale", [0.0, 1e-33, -1e-33, 3e-32, 1e-31, 1e-44])
+def test_small_scales_of_large_scores(scale):
+    """Scores of 2^100 and more (their sums are exact) under a scale that brings them near zero, or
+    to nothing: all tokens count alike then."""
+    D, P, lens = 64, 16, [40, 700]
+    table, pages = _table(lens, P)
+    kc = _whole(pages, P, 2, D, dtype=torch.bfloat16) * 2.0**50
+    vc = _cache(pages, P, 2, D, torch.bfloat16)
+    q = _whole(2, 4, D, dtype=torch.bfloat16) * 2.0**50
+    o, lse = PagedAttentionDecodeOp(4, 2, D, P, scale)(q, kc, vc, table, _lens(lens))
+    want = ref.attend(q, kc, vc, table, _lens(lens), scale, exact_scores=True)
+    assert_within(o, want[0], want[2], "o")
+    assert_within(lse, want[1], want[3], "lse")

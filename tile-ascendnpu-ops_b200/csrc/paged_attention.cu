@@ -863,8 +863,8 @@ extern "C" int tileops_paged_decode_fwd(
   a.partial = reinterpret_cast<float*>(a.stats + static_cast<int64_t>(kMaxCtas) * 2 * a.part_rows);
   a.div_page = FastDivU32(static_cast<uint32_t>(page_size));
   // Above zero, so that the largest product has the largest weight and one outside the sequence, -inf,
-  // none: the sign goes to q, and 0 is 2^-100 (weights of 1 all the same).
-  a.scale = static_cast<float>(std::max(std::abs(scale) * 1.4426950408889634, 0x1p-100));
+  // none: the sign goes to q, and 0 is fp32's smallest number (scores below 2^127: weights of 1 - 2^-21 and more).
+  a.scale = static_cast<float>(std::max(std::abs(scale) * 1.4426950408889634, 0x1p-149));
   a.flip = scale < 0.0 ? 0x80008000u : 0u;
   if (places_of(a, 32) > 0x7fffffffLL) return TILEOPS_EBADSHAPE;
   a.err = device_error_ptr();
