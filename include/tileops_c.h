@@ -462,7 +462,7 @@ int64_t tileops_paged_decode_workspace_bytes(int64_t heads, int64_t heads_kv, in
  * tokens a key head in all, were every sequence as long as its table.  strides8
  * (HOST, multiples of 8): elements from a sequence and head to the next of q,
  * from a page, slot and head to the next of k_cache and of v_cache.  q, caches,
- * workspace 16-byte aligned; `workspace` holds
+ * workspace 16-byte aligned, o 8-byte; `workspace` holds
  * tileops_paged_decode_workspace_bytes() bytes, for one call at a time.  Its first
  * TILEOPS_PAGED_DECODE_COUNTERS int32 are counters: `counters_zero` says that
  * they are zero (the call leaves them so: of a workspace that is kept for one

@@ -532,3 +532,12 @@ def test_a_workspace_is_shared_only_by_calls_one_after_another(monkeypatch):
     assert here[0] is not there[0] and here[0] is not other[0][0]
     if here[1]:
         assert ask(number=2, handle=2)[0] is here[0]
+
+
+def test_decode_entry_point_checks_its_output_alignment():
+    """Rows of o are written four channels, 8 bytes, at a time."""
+    fn = _native.lib().tileops_paged_decode_fwd
+    for off, status in ((2, _native.EALIGN), (4, _native.EALIGN)):
+        o = ctypes.c_void_p((1 << 20) + off)
+        assert fn(SOME, SOME, SOME, SOME, SOME, o, SOME, SOME, 2, 4, 2, 8, 3, 4, 2, 2, _ints(*[8] * 8), 0, 0,
+                  1.0, 2, NULL) == status

@@ -830,7 +830,8 @@ extern "C" int tileops_paged_decode_fwd(
     return TILEOPS_EINVAL;
   for (int n = 0; n < 8; ++n)
     if (strides8[n] % 8 != 0) return TILEOPS_EALIGN;
-  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace) ||
+      reinterpret_cast<uintptr_t>(o) % 8 != 0)  // store_row writes 8 bytes
     return TILEOPS_EALIGN;
   DecodeArgs a{};
   a.q = q;
