@@ -541,3 +541,60 @@ def test_decode_entry_point_checks_its_output_alignment():
         o = ctypes.c_void_p((1 << 20) + off)
         assert fn(SOME, SOME, SOME, SOME, SOME, o, SOME, SOME, 2, 4, 2, 8, 3, 4, 2, 2, _ints(*[8] * 8), 0, 0,
                   1.0, 2, NULL) == status
+
+
+def test_kernel_overrides_of_a_shipped_kernel(accept_cpu):
+    """A subclass that has a forward of its own gets the op's arguments and no more; one that calls the
+    shipped forward, or has its own plan as well, keeps what belongs together."""
+    seen = []
+
+    class Rotary(RotaryEmbeddingFwdKernel):
+        def forward(self, q, k, positions=None, inplace=False):
+            seen.append("rotary")
+            return q, k
+
+    class RotaryBack(RotaryEmbeddingBwdKernel):
+        def forward(self, q, k, positions=None, inplace=False):
+            seen.append("back")
+            return super().forward(q, k, positions, inplace)
+
+    class Append(PagedKVAppendKernel):
+        def forward(self, k, v, k_cache, v_cache, page_table, seq_lens, q=None, cu_seqlens=None):
+            seen.append("append")
+
+    class Decode(PagedAttentionDecodeKernel):
+        def forward(self, q, k_cache, v_cache, page_table, seq_lens):
+            seen.append("decode")
+            return q, None
+
+    class Planned(PagedAttentionDecodeKernel):
+        def plan(self, *args):
+            return "planned"
+
+        def forward(self, q, k_cache, v_cache, page_table, seq_lens, plan=None):
+            seen.append(plan)
+
+    class Inherits(PagedAttentionDecodeKernel):
+        pass
+
+    q, k = _rotary_args()
+    sizes = (2, 5, 4, 2, 8)
+    op = RotaryEmbeddingFwdOp(*sizes, dtype=torch.float32, kernel_map={"rotary_fwd": Rotary})
+    for _ in range(2):
+        op(q, k)
+    op = RotaryEmbeddingBwdOp(*sizes, dtype=torch.float32, kernel_map={"rotary_bwd": RotaryBack})
+    with pytest.raises(ValueError, match="must be on a cuda device"):  # the shipped forward's
+        op(q, k)
+    args = _paged(torch.float16)
+    op = PagedKVAppendOp(2, 8, 4, 4, dtype=torch.float16, kernel_map={"paged_kv_append": Append})
+    for _ in range(2):
+        op(**args)
+    del args["k"], args["v"]
+    for cls in (Decode, Planned):
+        op = PagedAttentionDecodeOp(4, 2, 8, 4, dtype=torch.float16, kernel_map={"paged_attention_decode": cls})
+        for _ in range(2):
+            op(**args)
+    op = PagedAttentionDecodeOp(4, 2, 8, 4, dtype=torch.float16, kernel_map={"paged_attention_decode": Inherits})
+    with pytest.raises(ValueError, match="must be on a cuda device"):
+        op(**args)
+    assert seen == ["rotary", "rotary", "back", "append", "append", "decode", "decode", "planned", "planned"]

@@ -39,10 +39,12 @@ NO_PLAN = ()
 
 
 def plan_of(kernel, *args):
-    """What a kernel works out once for a layout; NO_PLAN of one (an op's override) that only has a
-    ``forward``."""
-    plan = getattr(kernel, "plan", None)
-    return NO_PLAN if plan is None else plan(*args)
+    """What a kernel works out once for a layout; NO_PLAN where the class whose ``forward`` it has (an
+    op's override) makes none, since that forward takes the op's arguments only."""
+    for cls in type(kernel).__mro__:
+        if "forward" in vars(cls):
+            return kernel.plan(*args) if "plan" in vars(cls) else NO_PLAN
+    return NO_PLAN
 
 
 def overlaps(shape: Sequence[int], strides: Sequence[int]) -> bool:
