@@ -670,3 +670,36 @@ def test_small_scales_of_large_scores(scale):
     want = ref.attend(q, kc, vc, table, _lens(lens), scale, exact_scores=True)
     assert_within(o, want[0], want[2], "o")
     assert_within(lse, want[1], want[3], "lse")
+
+
+def test_threads_and_streams_finish_all_their_calls():
+    """Two host threads on one of torch's streams and one on another: every call's result is counted
+    and compared; a thread that raises fails the test."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    made = []
+    for lens, H, Hkv, D in (([3000], 2, 1, 64), ([900, 5000, 0, 77], 16, 2, 128), ([2000] * 3, 4, 4, 192),
+                            ([4000, 4000], 40, 1, 96)):
+        table, pages = _table(lens, 16)
+        kc, vc = _cache(pages, 16, Hkv, D, torch.bfloat16), _cache(pages, 16, Hkv, D, torch.bfloat16)
+        q = torch.randn(len(lens), H, D, device="cuda").to(torch.bfloat16)
+        args = (q, kc, vc, table, _lens(lens))
+        op = PagedAttentionDecodeOp(H, Hkv, D, 16)
+        made.append((op, args, op(*args)))
+    torch.cuda.synchronize()
+
+    def work(stream):
+        done = 0
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                for op, args, (o, lse) in made:
+                    got = op(*args)
+                    assert torch.equal(got[0], o) and torch.equal(got[1], lse)
+                    done += 1
+        return done
+
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    with ThreadPoolExecutor(3) as pool:
+        runs = [pool.submit(work, s) for s in (streams[0], streams[0], streams[1])]
+        assert [r.result() for r in runs] == [30 * len(made)] * 3
+    torch.cuda.synchronize()
