@@ -598,3 +598,83 @@ def test_kernel_overrides_of_a_shipped_kernel(accept_cpu):
     with pytest.raises(ValueError, match="must be on a cuda device"):
         op(**args)
     assert seen == ["rotary", "rotary", "back", "append", "append", "decode", "decode", "planned", "planned"]
+
+
+# ------------------------------------------------------------ tensors that share memory in part
+def test_in_place_refuses_rows_that_share_memory_in_part(accept_cpu):
+    """Slices of one projection lie apart; where they share a channel, or a whole head, both would be
+    rotated by two threads."""
+    B, S, D = 2, 5, 8
+    wide = torch.randn(B, S, 8 * D)
+
+    def heads(first, count):
+        return wide[..., first:first + count * D].unflatten(-1, (count, D))
+
+    op = RotaryEmbeddingFwdOp(B, S, 4, 2, D, dtype=torch.float32, inplace=True)
+    for _ in range(2):
+        for q, k in ((0, 4 * D), (2 * D, 0), (0, 6 * D), (16, 4 * D + 16)):
+            with pytest.raises(ValueError, match="must be on a cuda device"):  # all checks passed
+                op(heads(q, 4), heads(k, 2))
+        for q, k in ((0, 0), (0, 2 * D), (0, 4 * D - 1), (4, 0), (D, 4 * D), (2 * D, D + 1)):
+            with pytest.raises(ValueError, match="q and k share memory"):
+                op(heads(q, 4), heads(k, 2))
+    both = torch.randn(B, S, 2, 4, D)  # another stride between tokens than between slices
+    op = RotaryEmbeddingFwdOp(B, S, 4, 4, D, dtype=torch.float32, inplace=True)
+    with pytest.raises(ValueError, match="must be on a cuda device"):
+        op(both[:, :, 0], both[:, :, 1])
+    rows = torch.randn(3, S, 4, D)
+    with pytest.raises(ValueError, match="q and k share memory"):
+        op(rows[:2], rows[1:])  # the second row of one is the first of the other
+
+
+def test_append_refuses_caches_that_share_memory_in_part(accept_cpu):
+    P, Hkv, D = 4, 2, 8
+    op = PagedKVAppendOp(Hkv, D, P, 4, dtype=torch.float32)
+    args = _paged(torch.float32)
+    pool = torch.zeros(4, P, Hkv, D)
+    both = torch.zeros(3, P, 2, Hkv, D)
+    mixed = torch.zeros(3, P, Hkv, 2 * D)
+    halves = torch.zeros(3, 2, Hkv, P, D)
+    for k, v in ((both[:, :, 0], both[:, :, 1]), (both[:, :, 1], both[:, :, 0]),
+                 (mixed[..., :D], mixed[..., D:]),
+                 (halves[:, 0].transpose(1, 2), halves[:, 1].transpose(1, 2))):
+        for _ in range(2):
+            with pytest.raises(ValueError, match="must be on a cuda device"):  # all checks passed
+                op(**{**args, "k_cache": k, "v_cache": v})
+    for k, v in ((pool[:3], pool[1:]), (pool[1:], pool[:3]), (mixed[..., :D], mixed[..., D - 1:-1]),
+                 (both[:, :, 0], both[:, :, 0])):
+        for _ in range(2):
+            with pytest.raises(ValueError, match="k_cache and v_cache share memory"):
+                op(**{**args, "k_cache": k, "v_cache": v})
+
+
+def test_apart_against_every_address():
+    from random import Random
+
+    from tileops.kernels.attention._layouts import Apart
+
+    rng = Random(0)
+    buf = torch.zeros(4000)
+
+    def view():
+        shape = [rng.randint(1, 4) for _ in range(3)] + [rng.randint(1, 5)]
+        strides = [rng.choice([1, 2, 3, 5, 8, 10, 16, 20, 40, 41, 60]) for _ in range(3)] + [1]
+        return torch.as_strided(buf, shape, strides, rng.randint(0, 120))
+
+    counts = [0, 0]
+    for _ in range(3000):
+        a, b = view(), view()
+        if rng.random() < 0.5:
+            b = torch.as_strided(buf, a.shape, a.stride(), b.storage_offset())
+        places = [{t.storage_offset() + sum(i * s for i, s in zip(at, t.stride()))
+                   for at in torch.cartesian_prod(*[torch.arange(n) for n in t.shape]).view(-1, 4).tolist()}
+                  for t in (a, b)]
+        apart = not (places[0] & places[1])
+        counts[apart] += 1
+        assert Apart(a, b)(a.data_ptr(), b.data_ptr()) == apart, (a.shape, a.stride(), b.shape, b.stride())
+    assert min(counts) > 500
+    a = torch.zeros(3, 4)
+    assert not Apart(a, a)(a.data_ptr(), a.data_ptr() + 2)  # across elements
+    assert Apart(a, a)(a.data_ptr(), a.data_ptr() + 48)
+    none = torch.zeros(0, 4)
+    assert Apart(none, a)(a.data_ptr(), a.data_ptr()) and Apart(none, none)(0, 0)

@@ -16,7 +16,7 @@ from typing import Optional, Sequence
 import torch
 
 from tileops import _native
-from tileops.kernels.attention._layouts import channels_last, overlaps, row_of
+from tileops.kernels.attention._layouts import Apart, channels_last, overlaps, row_of
 from tileops.kernels.attention.rotary_embedding import check_rotation, turns_array
 from tileops.kernels.kernel_base import Kernel, check_dtype
 
@@ -56,8 +56,8 @@ class PagedKVAppendKernel(Kernel):
 
     def plan(self, k, v, k_cache, v_cache, page_table, seq_lens, q=None, cu_seqlens=None):
         """What a call of this layout needs, for ``forward``: device, which arguments have to be
-        copied, the stride array, the table's stride, the rows and the queries' shape; refuses caches
-        that cannot be written."""
+        copied, the stride array, the table's stride, the rows, the queries' shape and whether the
+        caches lie apart; refuses caches that cannot be written."""
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
             if not channels_last(c):
                 raise ValueError(f"{name} must have contiguous channels, got strides {c.stride()}")
@@ -85,7 +85,7 @@ class PagedKVAppendKernel(Kernel):
         tokens = k.shape[0] if k.dim() == 3 else k.shape[0] * k.shape[1]
         return (k.device, copy if any(copy) else None, (ctypes.c_int64 * 18)(*values), table_stride,
                 seq_lens.shape[0], tokens, k_cache.shape[0], page_table.shape[1],
-                None if q is None else row_of(q))
+                None if q is None else row_of(q), Apart(k_cache, v_cache))
 
     def forward(self, k, v, k_cache, v_cache, page_table, seq_lens, q=None, cu_seqlens=None,
                 plan=None):
@@ -93,13 +93,13 @@ class PagedKVAppendKernel(Kernel):
         ``plan()`` gave for arguments of the same layout."""
         if plan is None:
             plan = self.plan(k, v, k_cache, v_cache, page_table, seq_lens, q, cu_seqlens)
-        device, copy, strides, table_stride, seqs, tokens, pages, columns, q_like = plan
+        device, copy, strides, table_stride, seqs, tokens, pages, columns, q_like, apart = plan
         if copy is not None:
             q, k, v, page_table, seq_lens, cu_seqlens = (
                 t.contiguous() if c else t
                 for t, c in zip((q, k, v, page_table, seq_lens, cu_seqlens), copy))
         k_at, v_at = k_cache.data_ptr(), v_cache.data_ptr()
-        if k_at == v_at:
+        if not apart(k_at, v_at):
             raise ValueError("k_cache and v_cache share memory: they cannot both be written")
         q_out = None if q is None else torch.empty_like(q_like)
         _native.launch(

@@ -36,6 +36,7 @@ from tileops.device import get_device_backend
 from tileops.kernels.attention import RotaryEmbeddingBwdKernel, RotaryEmbeddingFwdKernel
 from tileops.kernels.attention._layouts import (
     NO_PLAN,
+    Apart,
     Layouts,
     channels_last,
     layout_of,
@@ -102,6 +103,7 @@ class _RotaryEmbeddingOp(Op):
                                             interleaved, self.frequencies, amplitude, dtype)
         self._shapes = (batch, seq_len, heads, dim), (batch, seq_len, heads_kv, dim)
         self._plans = Layouts()  # of the arguments that were found right
+        self._apart = Layouts()  # in place: of q and k
 
     def forward(self, q: Optional[torch.Tensor], k: Optional[torch.Tensor],
                 positions: Optional[torch.Tensor] = None):
@@ -112,9 +114,11 @@ class _RotaryEmbeddingOp(Op):
             if q is None and k is None:
                 return None, None
             plan = self._plans.keep(layout, plan_of(self.kernel, q, k, positions, self.inplace))
-        if self.inplace and q is not None and k is not None and q.data_ptr() == k.data_ptr() != 0:
-            raise ValueError(f"{self._names[0]} and {self._names[1]} share memory: they cannot both "
-                             "be rotated in place")
+        if self.inplace and q is not None and k is not None:
+            apart = self._apart.get(layout) or self._apart.keep(layout, Apart(q, k))
+            if not apart(q.data_ptr(), k.data_ptr()):
+                raise ValueError(f"{self._names[0]} and {self._names[1]} share memory: they cannot "
+                                 "both be rotated in place")
         if plan is NO_PLAN:
             return self.kernel(q, k, positions, self.inplace)
         return self.kernel.forward(q, k, positions, self.inplace, plan)
