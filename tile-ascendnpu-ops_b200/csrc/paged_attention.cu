@@ -730,14 +730,21 @@ bool opt_in() {
   return true;
 }
 
+// Whether the rows of neighbouring heads lie in the same 128-byte lines: less than a line apart, and
+// not in whole lines.
+bool share_lines(const DecodeArgs& a, const CacheStrides& s) {
+  return a.heads_kv > 1 && std::abs(s.head) < a.dim + 64 && s.head % 64 != 0;
+}
+
 template <typename T, int DP, int MT, int WARPS>
 int launch_tile(const DecodeArgs& a, bool clear, cudaStream_t s) {
   using L = Layout<DP, MT, WARPS>;
   // Where heads lie side by side and share 128-byte lines, fewer CTAs: those of neighbouring heads then stay
   // close to each other in the tokens, and a line is fetched once (320 items of 8009 tokens x 80 189 us
-  // for 227; with whole lines a head more CTAs are as good or better, 512 items x 128 85 us for 89).
+  // for 227; with whole lines a head more CTAs are as good or better, 512 items x 128 85 us for 89, and where
+  // heads lie a page apart, 320 items of 8000 tokens x 80 in pages of 7 153 us for 184).
   int ctas_sm = L::kCtasSm;
-  if (WARPS == 4 && a.heads_kv > 1 && a.ks.head * 2 % 128 != 0) ctas_sm = std::min(ctas_sm, 2);
+  if (WARPS == 4 && (share_lines(a, a.ks) || share_lines(a, a.vs))) ctas_sm = std::min(ctas_sm, 2);
   // No more CTAs than there can be places.
   const int64_t grid = std::min<int64_t>(
       {places_of(a, L::kUnit), static_cast<int64_t>(sm_count()) * ctas_sm, kMaxCtas});
