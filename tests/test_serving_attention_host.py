@@ -678,3 +678,25 @@ def test_apart_against_every_address():
     assert Apart(a, a)(a.data_ptr(), a.data_ptr() + 48)
     none = torch.zeros(0, 4)
     assert Apart(none, a)(a.data_ptr(), a.data_ptr()) and Apart(none, none)(0, 0)
+
+
+def test_decode_roofline_counts_the_tokens_of_the_last_call(accept_cpu):
+    """A table is as wide as the longest sequence allowed: what a short batch reads goes by its lengths."""
+
+    class Other(Kernel):
+        def __init__(self, *args):
+            super().__init__()
+
+        def forward(self, *args):
+            return args[0], None
+
+    B, H, Hkv, D, P = 4, 4, 2, 8, 4
+    args = dict(q=torch.zeros(B, H, D, dtype=torch.float16), page_table=torch.zeros(B, 50, dtype=torch.int32))
+    args["k_cache"], args["v_cache"] = torch.zeros(2, 3, P, Hkv, D, dtype=torch.float16)
+    for window, lens, seen in ((None, [5, 0, 12, 3], 20), (None, [-2, 1, 2**31 - 1, 0], 201),
+                               (4, [5, 0, 12, 3], 11)):
+        op = PagedAttentionDecodeOp(H, Hkv, D, P, window=window, dtype=torch.float16,
+                                    kernel_map={"paged_attention_decode": Other})
+        op(**args, seq_lens=torch.tensor(lens, dtype=torch.int32))
+        assert op.eval_roofline() == (4 * seen * H * D,
+                                      (2 * seen * Hkv * D + 2 * B * H * D) * 2 + 4 * B * H)

@@ -178,6 +178,7 @@ class PagedAttentionDecodeOp(Op):
         self.window = window
         self.dtype = dtype
         self._last = 0, 0  # of the last call: sequences, columns of the page table
+        self._seq_lens = None  # and their lengths, on the device
         self._plans = Layouts()  # of the arguments that were found right
         self.dispatch_kernel(kernel_map)
         self.kernel = self.kernel_map["paged_attention_decode"](
@@ -196,7 +197,7 @@ class PagedAttentionDecodeOp(Op):
             self._check(q, k_cache, v_cache, page_table, seq_lens)
             plan = self._plans.keep(layout, plan_of(self.kernel, q, k_cache, v_cache, page_table,
                                                     seq_lens))
-        self._last = layout[3][0]
+        self._last, self._seq_lens = layout[3][0], seq_lens
         if plan is NO_PLAN:
             return self.kernel(q, k_cache, v_cache, page_table, seq_lens)
         return self.kernel.forward(q, k_cache, v_cache, page_table, seq_lens, plan)
@@ -212,11 +213,13 @@ class PagedAttentionDecodeOp(Op):
                              f"{page_table.shape[1]} pages of {self.page_size}")
 
     def eval_roofline(self) -> tuple[int, int]:
-        """``(4 * B * S * H * D, (2 * B * S * Hkv * D + 2 * B * H * D) * elem_bytes + 4 * B * H)``, S
-        the tokens the last call's page table had room for, its window at most (the lengths
-        themselves are on the device)."""
+        """``(4 * T * H * D, (2 * T * Hkv * D + 2 * B * H * D) * elem_bytes + 4 * B * H)``, T the
+        tokens that the B queries of the last call see, by what its ``seq_lens`` holds now (read from
+        the device; without it as many as the table has room for)."""
         batch, columns = self._last
-        seen = min(columns * self.page_size, self.window or columns * self.page_size)
-        q = batch * self.heads * self.dim
-        return (4 * q * seen, (2 * batch * seen * self.heads_kv * self.dim + 2 * q)
+        room = columns * self.page_size
+        lens = [room] * batch if self._seq_lens is None else self._seq_lens.tolist()
+        seen = sum(min(max(n, 0), room, self.window or room) for n in lens)
+        return (4 * seen * self.heads * self.dim,
+                (2 * seen * self.heads_kv * self.dim + 2 * batch * self.heads * self.dim)
                 * self.dtype.itemsize + 4 * batch * self.heads)
