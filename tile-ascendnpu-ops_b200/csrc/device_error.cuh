@@ -9,7 +9,7 @@
 namespace tileops {
 
 constexpr int kErrMbarTimeout = 1;  // an mbarrier wait exceeded its poll limit
-constexpr int kErrBadSeqlens = 2;   // cu_seqlens not 0 = cu[0] <= ... <= cu[N] = total
+constexpr int kErrBadSeqlens = 2;   // cu_seqlens not 0 = cu[0] <= ... <= cu[N] = total (append: <= total)
 constexpr int kErrBadPage = 3;      // a page table without a valid page for a token in use
 
 // Device address of the per-device error word (defined in capi.cu).  Kernels

@@ -8,8 +8,8 @@
 // multiples of 16 bytes; query head h reads key head h / (H / Hkv).  A sequence without a token
 // has o = 0 and lse = -inf.
 //
-// Every key and value is read once, 4 D e bytes for 4 D (H / Hkv) flops a token and key head: 1 to
-// 16 flops a byte, so HBM bounds it.  8 flops a byte at the memory's rate are 52 TFLOP/s, which
+// Every key and value is read once, 2 D e bytes for 4 D (H / Hkv) flops a token and key head: H / Hkv
+// flops a byte, 1 to 16 as a rule, so HBM bounds it.  8 flops a byte at the memory's rate are 52 TFLOP/s, which
 // the fp32 pipes do not reach beside the conversions; the two products go to the tensor cores as
 // m16n8k16 (the query heads of a key head are the 16 rows; a 128-row tcgen05 tile would be
 // 7/8 padding and would take the scores through TMEM and back, for rates not needed here).
@@ -218,7 +218,7 @@ struct Layout {
   static constexpr int kTokens = DP <= 64 ? 32 : 16;
   // Two stages of 8 KB a warp and 12 warps an SM (8 where 16 rows more take the registers): 256 items of
   // up to 4096 tokens x 128 27.9 us, 29.3 with three stages and 8 warps; heads of 192 and 256 as they fit.
-  static constexpr int kStages = DP <= 128 ? 2 : DP <= 192 ? (WARPS == 4 ? 4 : 2) : (WARPS == 4 ? 3 : 2);
+  static constexpr int kStages = DP > 192 && WARPS == 4 ? 3 : 2;
   static constexpr int kCtasSm = WARPS == 8   ? 1
                                  : WARPS == 4 ? (DP > 128 ? 1 : MT == 1 ? 3 : 2)
                                               : (DP <= 192 ? 4 : 3);
@@ -737,7 +737,7 @@ bool share_lines(const DecodeArgs& a, const CacheStrides& s) {
 }
 
 template <typename T, int DP, int MT, int WARPS>
-int launch_tile(const DecodeArgs& a, bool clear, cudaStream_t s) {
+int launch_tile(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   using L = Layout<DP, MT, WARPS>;
   // Where heads lie side by side and share 128-byte lines, fewer CTAs: those of neighbouring heads then stay
   // close to each other in the tokens, and a line is fetched once (320 items of 8009 tokens x 80 189 us
@@ -749,7 +749,7 @@ int launch_tile(const DecodeArgs& a, bool clear, cudaStream_t s) {
   const int64_t grid = std::min<int64_t>(
       {places_of(a, L::kUnit), static_cast<int64_t>(sm_count()) * ctas_sm, kMaxCtas});
   if (!opt_in<T, DP, MT, WARPS>()) return TILEOPS_ELAUNCH;
-  if (clear) {
+  if (counters_zero) {
     paged_decode<T, DP, MT, WARPS><<<static_cast<unsigned>(grid), L::kThreads, L::kBytes, s>>>(a);
     return launch_status();
   }
@@ -773,7 +773,7 @@ int launch_tile(const DecodeArgs& a, bool clear, cudaStream_t s) {
 }
 
 template <typename T, int DP, int MT>
-int launch_warps(const DecodeArgs& a, bool clear, cudaStream_t s) {
+int launch_warps(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   // Few items are shared by many CTAs each: one CTA of 8 warps an SM, so that there are fewer sums to join
   // (32 items of 32768 tokens x 128 89 us, 94 with CTAs of 4; but 256 items of up to 4096 33 and 28 us).  Many
   // items: smaller CTAs, more of them at different points of an item (512 sequences of up to 256 tokens,
@@ -781,27 +781,27 @@ int launch_warps(const DecodeArgs& a, bool clear, cudaStream_t s) {
   // Heads of 192 have no room for two CTAs of 4, nor heads of 256 for 8 warps.
   const int64_t items = static_cast<int64_t>(a.batch) * a.heads_kv * a.blocks;
   if constexpr (DP <= 192) {
-    if (items <= sm_count()) return launch_tile<T, DP, MT, 8>(a, clear, s);
+    if (items <= sm_count()) return launch_tile<T, DP, MT, 8>(a, counters_zero, s);
   }
   if constexpr (DP <= 128) {
-    if (items <= 4 * sm_count()) return launch_tile<T, DP, MT, 4>(a, clear, s);
+    if (items <= 4 * sm_count()) return launch_tile<T, DP, MT, 4>(a, counters_zero, s);
   }
   if constexpr (DP > 192) {
-    if (items <= sm_count()) return launch_tile<T, DP, MT, 4>(a, clear, s);
+    if (items <= sm_count()) return launch_tile<T, DP, MT, 4>(a, counters_zero, s);
   }
-  return launch_tile<T, DP, MT, 2>(a, clear, s);
+  return launch_tile<T, DP, MT, 2>(a, counters_zero, s);
 }
 
 template <typename T>
-int launch_type(const DecodeArgs& a, bool clear, cudaStream_t s) {
+int launch_type(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   const int dp = padded_dim(a.dim);
   const bool wide = rows_of(a.group, dp) == 32;
   switch (dp) {
-    case 64: return wide ? launch_warps<T, 64, 2>(a, clear, s) : launch_warps<T, 64, 1>(a, clear, s);
-    case 96: return wide ? launch_warps<T, 96, 2>(a, clear, s) : launch_warps<T, 96, 1>(a, clear, s);
-    case 128: return wide ? launch_warps<T, 128, 2>(a, clear, s) : launch_warps<T, 128, 1>(a, clear, s);
-    case 192: return launch_warps<T, 192, 1>(a, clear, s);
-    default: return launch_warps<T, 256, 1>(a, clear, s);
+    case 64: return wide ? launch_warps<T, 64, 2>(a, counters_zero, s) : launch_warps<T, 64, 1>(a, counters_zero, s);
+    case 96: return wide ? launch_warps<T, 96, 2>(a, counters_zero, s) : launch_warps<T, 96, 1>(a, counters_zero, s);
+    case 128: return wide ? launch_warps<T, 128, 2>(a, counters_zero, s) : launch_warps<T, 128, 1>(a, counters_zero, s);
+    case 192: return launch_warps<T, 192, 1>(a, counters_zero, s);
+    default: return launch_warps<T, 256, 1>(a, counters_zero, s);
   }
 }
 
