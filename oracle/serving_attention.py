@@ -13,7 +13,8 @@ with u = 2^-24 (half a step of fp32, relative):
   each sum: 2 u a term, (D + 16) 2 u sum |q k| (nothing where q and k are whole numbers so small that
   every sum is exact);
 * a weight exp2(t - base): t and the difference round (4 u of the largest |t|), ex2.approx is off by 4 u;
-* the weights are rounded to the inputs' type for the second product, half a step each, and sums of n
+* up to 8 query heads a key head the weights enter the second product as two numbers of the inputs'
+  type, half a step of half a step off; those of more heads are rounded once, half a step off.  Sums of n
   terms may cut each term.
 """
 
@@ -108,10 +109,12 @@ def append(k, v, k_cache, v_cache, page_table, seq_lens, frequencies=(), q=None,
 # ------------------------------------------------------------ single-token attention
 def attend(q, k_cache, v_cache, page_table, seq_lens, scale=None, window=None,
            exact_scores=False):
-    """``(o, lse, o_bound, lse_bound)``; the bounds count weights rounded to q's type."""
+    """``(o, lse, o_bound, lse_bound)``; the bounds count what weights in q's type are off by."""
     half = torch.finfo(q.dtype).eps / 2
     B, H, D = q.shape
     P, Hkv = k_cache.shape[1], k_cache.shape[2]
+    if H // Hkv <= 8:
+        half *= half
     scale = D**-0.5 if scale is None else scale
     q = _wide(q)
     kc, vc = k_cache.detach().cpu(), v_cache.detach().cpu()

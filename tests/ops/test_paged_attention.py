@@ -703,3 +703,59 @@ def test_threads_and_streams_finish_all_their_calls():
         runs = [pool.submit(work, s) for s in (streams[0], streams[0], streams[1])]
         assert [r.result() for r in runs] == [30 * len(made)] * 3
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------ what weights are held in
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("H, Hkv", [(1, 1), (8, 1), (16, 2), (21, 3), (4, 4)])
+@pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
+def test_weights_of_up_to_8_heads_keep_more_bits_than_the_type(D, H, Hkv, dtype):
+    """Half of the tokens have the value 1, half -1, and scores that differ little: what is left of o
+    after the cancellation are the weights' differences, which their type alone does not hold."""
+    P, n = 16, 64
+    table, pages = _table([n], P)
+    kc = _cache(pages, P, Hkv, D, dtype, fill=0.0)
+    vc = _cache(pages, P, Hkv, D, dtype, fill=1.0)
+    q = torch.zeros(1, H, D, device="cuda", dtype=dtype)
+    q[..., 5] = 1.0
+    odd = torch.randperm(n, device="cuda")[:n // 2]
+    at = table[0].long()[odd // P], odd % P
+    vc[at] = -1.0
+    op = PagedAttentionDecodeOp(H, Hkv, D, P, math.log(2.0), dtype=dtype)  # scores are exponents of 2
+    for less in (2.0**-10, 3 * 2.0**-9, 0.3, 2.7):
+        kc[at + (slice(None), 5)] = -less
+        w = 2.0 ** -float(torch.tensor(less, dtype=dtype))
+        o, _ = op(q, kc, vc, table, _lens([n]))
+        half = torch.finfo(dtype).eps / 2
+        # each weight half a step of half a step off, 8 u of its exponential, sums of n terms 2 u each
+        bound = half**2 + 8 * ref.U + 2 * ref.U * (n + 64)
+        want = torch.full((1, H, D), (1 - w) / (1 + w), dtype=torch.float64)
+        assert_within(o, want, torch.full_like(want, bound), f"{less}")
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("H, Hkv", [(1, 1), (8, 1), (9, 1), (32, 1), (4, 2)])
+@pytest.mark.parametrize("n", [5, 3000])
+def test_infinite_values(n, H, Hkv, dtype):
+    """An infinite value makes its channel infinite, whatever its weight's bits are; two that differ in
+    sign, and NaN, make it NaN; no other channel is touched."""
+    D, P = 64, 16
+    table, pages = _table([n], P)
+    kc, vc = _cache(pages, P, Hkv, D, dtype, fill=0.0), _cache(pages, P, Hkv, D, dtype)
+    kc[..., 0] = (torch.rand(pages, P, Hkv, device="cuda") * -3).to(dtype)
+    kc[int(table[0, 0]), 0, :, 0] = 1.0  # the largest weight is a whole one
+    q = torch.zeros(1, H, D, device="cuda", dtype=dtype)
+    q[..., 0] = 1.0
+    op = PagedAttentionDecodeOp(H, Hkv, D, P, 1.0, dtype=dtype)
+    clean, _ = op(q, kc, vc, table, _lens([n]))
+    for channel, at in ((3, 0), (17, 1), (40, n - 1)):
+        vc[int(table[0, at // P]), at % P, :, channel] = math.inf
+    vc[int(table[0, 0]), 2, :, 8] = -math.inf
+    vc[int(table[0, 0]), 1, :, 9] = math.inf
+    vc[int(table[0, 0]), 3, :, 9] = -math.inf
+    vc[int(table[0, 0]), 4, :, 10] = math.nan
+    o, _ = op(q, kc, vc, table, _lens([n]))
+    assert (o[..., [3, 17, 40]] == math.inf).all() and (o[..., 8] == -math.inf).all()
+    assert o[..., [9, 10]].isnan().all()
+    rest = [c for c in range(D) if c not in (3, 17, 40, 8, 9, 10)]
+    assert torch.equal(o[..., rest], clean[..., rest])

@@ -123,8 +123,12 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
 // s scale - round(top scale) by one fma, leave the largest weight at 2^r, r up to half a step of top scale:
 // from 2^25 on fp16 weights overflow, or all vanish.)  A pair of scores takes two instructions either way.
 // Weights go to the second product in the inputs' type, half a step (2^-8 in bf16, 2^-11 in fp16) off
-// each; their sum takes them unrounded.  In fp16 they are held times 2^15 (the largest is 2^15), so that
-// weights down to 2^-29 of the largest keep all their bits.
+// each; their sum takes them unrounded.  Up to 8 query heads leave rows 8 to 15 of the product's tile free:
+// those take what the weights were rounded off by, also in the inputs' type, and a thread, which has rows
+// r and r + 8, adds the two up at the end.  The weights are then 2^-16 and 2^-22 off, and it costs nothing:
+// no weights of eight rows of padding are made.  More heads would need a second product, 3 to 10% of the
+// time, for what is below the output's own rounding.  In fp16 weights are held times 2^15 (the largest is
+// 2^15), so that those down to 2^-29 of the largest keep all their bits.
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -134,6 +138,20 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+}
+// What a and b were rounded off by in w.
+template <typename T>
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const float2 held = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return pack2<T>(a - held.x, b - held.y);
+  } else {
+    return pack2<T>(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
+  }
+}
+// The rests' part of a sum; none of one that is not finite (a rest of 0 times an infinite value is NaN).
+__device__ __forceinline__ float rest_of(float sum, float rests) {
+  return fabsf(sum) < -kNegInf ? rests : 0.0f;
 }
 template <typename T>
 __device__ constexpr float kShift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
@@ -210,8 +228,11 @@ struct Looked {
   int page[32];            // of the warp's tokens in it, where they are inside the sequence
 };
 
-template <int DP, int MT, int WARPS>
+// ROWS: query heads that share the keys and values of a unit, 8, 16 or 32 at most.
+template <int DP, int ROWS, int WARPS>
 struct Layout {
+  static constexpr int kTiles = ROWS == 32 ? 2 : 1;            // of 16 rows
+  static constexpr int kHalves = ROWS == 8 ? 1 : 2;            // of a tile's rows, that heads have
   static constexpr int kChunks = DP / 8;                       // 16-byte chunks of a row
   static constexpr int kRow = (DP + 63) / 64 * 64;             // elements of a row in shared memory
   // Tokens of a warp in a unit: 8 KB of keys and values and more, for what a unit costs besides.
@@ -220,12 +241,12 @@ struct Layout {
   // up to 4096 tokens x 128 27.9 us, 29.3 with three stages and 8 warps; heads of 192 and 256 as they fit.
   static constexpr int kStages = DP > 192 && WARPS == 4 ? 3 : 2;
   static constexpr int kCtasSm = WARPS == 8   ? 1
-                                 : WARPS == 4 ? (DP > 128 ? 1 : MT == 1 ? 3 : 2)
+                                 : WARPS == 4 ? (DP > 128 ? 1 : kTiles == 1 ? 3 : 2)
                                               : (DP <= 192 ? 4 : 3);
   static constexpr int kUnit = WARPS * kTokens;
   static constexpr int kThreads = WARPS * 32;
   static constexpr int kTile = kTokens * kRow;                 // elements of a warp's keys (or values)
-  static constexpr int kRows = 16 * MT;
+  static constexpr int kRows = 16 * kTiles;
   static constexpr size_t kRing = static_cast<size_t>(WARPS) * kStages * 2 * kTile * 2;
   static constexpr size_t kQ = static_cast<size_t>(kRows) * kRow * 2;
   static constexpr size_t kStats = static_cast<size_t>(WARPS) * kRows * 2 * 4;
@@ -244,11 +265,11 @@ __device__ __forceinline__ void behind_clearing() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-template <typename T, int DP, int MT, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
+template <typename T, int DP, int ROWS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, (Layout<DP, ROWS, WARPS>::kCtasSm))
     paged_decode(const __grid_constant__ DecodeArgs a) {
-  using L = Layout<DP, MT, WARPS>;
-  constexpr int kThreads = L::kThreads, kUnit = L::kUnit;
+  using L = Layout<DP, ROWS, WARPS>;
+  constexpr int kThreads = L::kThreads, kUnit = L::kUnit, MT = L::kTiles, kHalves = L::kHalves;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ bool complete;
   T* const q_smem = reinterpret_cast<T*>(smem + L::kRing);
@@ -435,7 +456,8 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
 
   // ---- products ----
   // top: the score that a row's weights are relative to, its largest.
-  float out[MT][DP / 8][4], top[MT][2], sum[MT][2];
+  // Of eight rows, out[..][2] and [3] are the second numbers' part.
+  float out[MT][DP / 8][4], top[MT][kHalves], sum[MT][kHalves];
   auto reset = [&]() {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -443,8 +465,11 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
       for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[m][n][e] = 0.0f;
-      top[m][0] = top[m][1] = kNegInf;
-      sum[m][0] = sum[m][1] = 0.0f;
+#pragma unroll
+      for (int r = 0; r < kHalves; ++r) {
+        top[m][r] = kNegInf;
+        sum[m][r] = 0.0f;
+      }
     }
   };
   store_q();
@@ -501,7 +526,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
               if (t0 + n * 8 + (lane & 3) * 2 + (e & 1) >= get.span.end) s[m][n][e] = kNegInf;
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {  // rows lane / 4 and lane / 4 + 8
+        for (int r = 0; r < kHalves; ++r) {  // rows lane / 4 and lane / 4 + 8
           float high = kNegInf;
 #pragma unroll
           for (int n = 0; n < 2 * kBlocks; ++n)
@@ -522,7 +547,9 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
                                    make_float2(kShift<T>, kShift<T>));
             const float w0 = ex2_approx_f(t.x), w1 = ex2_approx_f(t.y);
             add += w0 + w1;
-            w[m][n / 2][n % 2 * 2 + r] = pack2<T>(w0, w1);
+            uint32_t(&to)[4] = w[m][n / 2];
+            to[n % 2 * 2 + r] = pack2<T>(w0, w1);
+            if constexpr (kHalves == 1) to[n % 2 * 2 + 1] = rest2<T>(w0, w1, to[n % 2 * 2]);
           }
           sum[m][r] = sum[m][r] * fade + add;
           if (__any_sync(~0u, fade != 1.0f)) {
@@ -530,6 +557,10 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
             for (int n = 0; n < DP / 8; ++n) {
               out[m][n][2 * r] *= fade;
               out[m][n][2 * r + 1] *= fade;
+              if (kHalves == 1) {
+                out[m][n][2] *= fade;
+                out[m][n][3] *= fade;
+              }
             }
           }
         }
@@ -559,7 +590,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
+          for (int r = 0; r < kHalves; ++r) {
             float v = sum[m][r];
             v += __shfl_xor_sync(~0u, v, 1);
             v += __shfl_xor_sync(~0u, v, 2);
@@ -573,14 +604,18 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
           __syncwarp();
           // 8-column group n of row r at group (n + r) % groups: the 8 rows in different banks.
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
+          for (int r = 0; r < kHalves; ++r) {
             if (m * 16 + r * 8 >= rows) continue;
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n) {
               const int row = r * 8 + lane / 4;
               const int col = (n + lane / 4) % (DP / 8) * 8 + (lane & 3) * 2;
-              *reinterpret_cast<float2*>(own + (row * kPad + col) * 4) =
-                  make_float2(out[m][n][2 * r], out[m][n][2 * r + 1]);
+              float2 v = make_float2(out[m][n][2 * r], out[m][n][2 * r + 1]);
+              if (kHalves == 1) {
+                v.x += rest_of(v.x, out[m][n][2]);
+                v.y += rest_of(v.y, out[m][n][3]);
+              }
+              *reinterpret_cast<float2*>(own + (row * kPad + col) * 4) = v;
             }
           }
           __syncthreads();
@@ -651,7 +686,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Layout<DP, MT, WARPS>::kCtasSm))
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < kHalves; ++r) {
               const int row = m * 16 + r * 8 + lane / 4;
               if (row >= rows) continue;
               const float2 st = __ldcg(a.stats + at + row);
@@ -716,15 +751,15 @@ int64_t places_of(const DecodeArgs& a, int unit) {
 }
 
 // Lets the kernel have its shared memory, once on each device (0.5 us a call otherwise).
-template <typename T, int DP, int MT, int WARPS>
+template <typename T, int DP, int ROWS, int WARPS>
 bool opt_in() {
   static std::atomic<uint64_t> done{0};
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return false;
   const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
   if (done.load(std::memory_order_acquire) & bit) return true;
-  if (cudaFuncSetAttribute(paged_decode<T, DP, MT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(Layout<DP, MT, WARPS>::kBytes)) != cudaSuccess)
+  if (cudaFuncSetAttribute(paged_decode<T, DP, ROWS, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(Layout<DP, ROWS, WARPS>::kBytes)) != cudaSuccess)
     return false;
   done.fetch_or(bit, std::memory_order_release);
   return true;
@@ -736,9 +771,9 @@ bool share_lines(const DecodeArgs& a, const CacheStrides& s) {
   return a.heads_kv > 1 && std::abs(s.head) < a.dim + 64 && s.head % 64 != 0;
 }
 
-template <typename T, int DP, int MT, int WARPS>
+template <typename T, int DP, int ROWS, int WARPS>
 int launch_tile(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
-  using L = Layout<DP, MT, WARPS>;
+  using L = Layout<DP, ROWS, WARPS>;
   // Where heads lie side by side and share 128-byte lines, fewer CTAs: those of neighbouring heads then stay
   // close to each other in the tokens, and a line is fetched once (320 items of 8009 tokens x 80 189 us
   // for 227; with whole lines a head more CTAs are as good or better, 512 items x 128 85 us for 89, and where
@@ -748,9 +783,9 @@ int launch_tile(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   // No more CTAs than there can be places.
   const int64_t grid = std::min<int64_t>(
       {places_of(a, L::kUnit), static_cast<int64_t>(sm_count()) * ctas_sm, kMaxCtas});
-  if (!opt_in<T, DP, MT, WARPS>()) return TILEOPS_ELAUNCH;
+  if (!opt_in<T, DP, ROWS, WARPS>()) return TILEOPS_ELAUNCH;
   if (counters_zero) {
-    paged_decode<T, DP, MT, WARPS><<<static_cast<unsigned>(grid), L::kThreads, L::kBytes, s>>>(a);
+    paged_decode<T, DP, ROWS, WARPS><<<static_cast<unsigned>(grid), L::kThreads, L::kBytes, s>>>(a);
     return launch_status();
   }
   clear_counters<<<1, 512, 0, s>>>(a.counters);
@@ -767,12 +802,12 @@ int launch_tile(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   config.stream = s;
   config.attrs = &early;
   config.numAttrs = 1;
-  if (cudaLaunchKernelEx(&config, paged_decode<T, DP, MT, WARPS>, a) != cudaSuccess)
+  if (cudaLaunchKernelEx(&config, paged_decode<T, DP, ROWS, WARPS>, a) != cudaSuccess)
     return TILEOPS_ELAUNCH;
   return launch_status();
 }
 
-template <typename T, int DP, int MT>
+template <typename T, int DP, int ROWS>
 int launch_warps(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   // Few items are shared by many CTAs each: one CTA of 8 warps an SM, so that there are fewer sums to join
   // (32 items of 32768 tokens x 128 89 us, 94 with CTAs of 4; but 256 items of up to 4096 33 and 28 us).  Many
@@ -781,27 +816,34 @@ int launch_warps(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   // Heads of 192 have no room for two CTAs of 4, nor heads of 256 for 8 warps.
   const int64_t items = static_cast<int64_t>(a.batch) * a.heads_kv * a.blocks;
   if constexpr (DP <= 192) {
-    if (items <= sm_count()) return launch_tile<T, DP, MT, 8>(a, counters_zero, s);
+    if (items <= sm_count()) return launch_tile<T, DP, ROWS, 8>(a, counters_zero, s);
   }
   if constexpr (DP <= 128) {
-    if (items <= 4 * sm_count()) return launch_tile<T, DP, MT, 4>(a, counters_zero, s);
+    if (items <= 4 * sm_count()) return launch_tile<T, DP, ROWS, 4>(a, counters_zero, s);
   }
   if constexpr (DP > 192) {
-    if (items <= sm_count()) return launch_tile<T, DP, MT, 4>(a, counters_zero, s);
+    if (items <= sm_count()) return launch_tile<T, DP, ROWS, 4>(a, counters_zero, s);
   }
-  return launch_tile<T, DP, MT, 2>(a, counters_zero, s);
+  return launch_tile<T, DP, ROWS, 2>(a, counters_zero, s);
+}
+
+template <typename T, int DP>
+int launch_rows(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
+  if (a.group <= 8) return launch_warps<T, DP, 8>(a, counters_zero, s);
+  if constexpr (DP <= 128) {
+    if (rows_of(a.group, DP) == 32) return launch_warps<T, DP, 32>(a, counters_zero, s);
+  }
+  return launch_warps<T, DP, 16>(a, counters_zero, s);
 }
 
 template <typename T>
 int launch_type(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
-  const int dp = padded_dim(a.dim);
-  const bool wide = rows_of(a.group, dp) == 32;
-  switch (dp) {
-    case 64: return wide ? launch_warps<T, 64, 2>(a, counters_zero, s) : launch_warps<T, 64, 1>(a, counters_zero, s);
-    case 96: return wide ? launch_warps<T, 96, 2>(a, counters_zero, s) : launch_warps<T, 96, 1>(a, counters_zero, s);
-    case 128: return wide ? launch_warps<T, 128, 2>(a, counters_zero, s) : launch_warps<T, 128, 1>(a, counters_zero, s);
-    case 192: return launch_warps<T, 192, 1>(a, counters_zero, s);
-    default: return launch_warps<T, 256, 1>(a, counters_zero, s);
+  switch (padded_dim(a.dim)) {
+    case 64: return launch_rows<T, 64>(a, counters_zero, s);
+    case 96: return launch_rows<T, 96>(a, counters_zero, s);
+    case 128: return launch_rows<T, 128>(a, counters_zero, s);
+    case 192: return launch_rows<T, 192>(a, counters_zero, s);
+    default: return launch_rows<T, 256>(a, counters_zero, s);
   }
 }
 
