@@ -9,10 +9,10 @@
 // has o = 0 and lse = -inf.
 //
 // Every key and value is read once, 2 D e bytes for 4 D (H / Hkv) flops a token and key head: H / Hkv
-// flops a byte, 1 to 16 as a rule, so HBM bounds it.  8 flops a byte at the memory's rate are 52 TFLOP/s, which
-// the fp32 pipes do not reach beside the conversions; the two products go to the tensor cores as
-// m16n8k16 (the query heads of a key head are the 16 rows; a 128-row tcgen05 tile would be
-// 7/8 padding and would take the scores through TMEM and back, for rates not needed here).
+// flops a byte, 1 to 16 as a rule, so HBM bounds it.  8 flops a byte at the memory's rate are 52
+// TFLOP/s, which the fp32 pipes do not reach beside the conversions; the two products go to the tensor
+// cores as m16n8k16 (the query heads of a key head are the 16 rows, or 8 of them; a 128-row tcgen05 tile
+// would be 7/8 padding and would take the scores through TMEM and back, for rates not needed here).
 //
 // The split.  The tokens of each (sequence, key head) are cut into units of 16 or 32 for each warp of
 // a CTA, and all units of the call in a row are shared out evenly, a run of them to each CTA,
@@ -32,11 +32,15 @@
 // of the next items' units are in flight meanwhile.  Tokens outside the sequence are copied as
 // zeros (size 0), never read: infinities and NaN behind a sequence's end have no say.
 //
-// Measured (bf16 and fp16, in a graph): 131072 tokens x 8 heads x 128 89 us (0.92 of the copy rate), 64
-// sequences of up to 8192 x 8 x 128 85 us (0.90), 8 of up to 4096 x 32 x 128 28 us (0.71), 1000 x 8 x 128
-// 8.2 us.  The body runs at 0.94 of the rate of a kernel that only reads; before it 2.5 us (lengths, pages,
+// Measured (bf16 and fp16, in a graph): 131072 tokens x 8 heads x 128 88 us (0.93 of the copy rate), 64
+// sequences of up to 8192 x 8 x 128 85 us (0.90), 8 of up to 4096 x 32 x 128 29 us (0.69), 1000 x 8 x 128
+// 8.1 us.  The body runs at 0.94 of the rate of a kernel that only reads; before it 2.5 us (lengths, pages,
 // first keys: three waits one after another, and code that is not in the SM yet), behind it 1.5 to 5 us
-// of joining (more where one item is shared by many CTAs).
+// of joining (more where one item is shared by many CTAs).  Narrower heads are bound by a warp's
+// instructions, about 500 cycles for its 16 tokens (32 up to 64 channels) whatever they weigh: 131072
+// tokens x 8 x 96 and x 80 92 us (0.67 and 0.56), x 64 53 us (0.78), x 40 58 us (0.44).  A group of more
+// than 32 heads (16 above 128 channels) is several items, each of which reads all keys and values: 16
+// sequences of 16384 x 1 head x 128 with 32 query heads 48 us, with 64 76 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -237,8 +241,9 @@ struct Layout {
   static constexpr int kRow = (DP + 63) / 64 * 64;             // elements of a row in shared memory
   // Tokens of a warp in a unit: 8 KB of keys and values and more, for what a unit costs besides.
   static constexpr int kTokens = DP <= 64 ? 32 : 16;
-  // Two stages of 8 KB a warp and 12 warps an SM (8 where 16 rows more take the registers): 256 items of
-  // up to 4096 tokens x 128 27.9 us, 29.3 with three stages and 8 warps; heads of 192 and 256 as they fit.
+  // Two stages of 8 KB a warp and 12 warps an SM (8 where 16 rows more take the registers): 512 items of up
+  // to 8192 tokens x 128 87 us, 88.5 with three stages and 8 warps, 320 items x 64 30.2 and 31.0 (256 items of
+  // up to 4096 tokens x 128 28.2 and 28.1); heads of 192 and 256 as they fit.
   static constexpr int kStages = DP > 192 && WARPS == 4 ? 3 : 2;
   static constexpr int kCtasSm = WARPS == 8   ? 1
                                  : WARPS == 4 ? (DP > 128 ? 1 : kTiles == 1 ? 3 : 2)
@@ -775,9 +780,9 @@ template <typename T, int DP, int ROWS, int WARPS>
 int launch_tile(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   using L = Layout<DP, ROWS, WARPS>;
   // Where heads lie side by side and share 128-byte lines, fewer CTAs: those of neighbouring heads then stay
-  // close to each other in the tokens, and a line is fetched once (320 items of 8009 tokens x 80 189 us
-  // for 227; with whole lines a head more CTAs are as good or better, 512 items x 128 85 us for 89, and where
-  // heads lie a page apart, 320 items of 8000 tokens x 80 in pages of 7 153 us for 184).
+  // close to each other in the tokens, and a line is fetched once (320 items of 8009 tokens x 80 199 us
+  // for 223, x 40 112 for 164; more CTAs are better with whole lines a head, 512 items x 128 85 us for 97, and
+  // where heads lie a page apart, 320 items of 8000 tokens x 80 in pages of 7 160 us for 193).
   int ctas_sm = L::kCtasSm;
   if (WARPS == 4 && (share_lines(a, a.ks) || share_lines(a, a.vs))) ctas_sm = std::min(ctas_sm, 2);
   // No more CTAs than there can be places.
@@ -810,9 +815,9 @@ int launch_tile(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
 template <typename T, int DP, int ROWS>
 int launch_warps(const DecodeArgs& a, bool counters_zero, cudaStream_t s) {
   // Few items are shared by many CTAs each: one CTA of 8 warps an SM, so that there are fewer sums to join
-  // (32 items of 32768 tokens x 128 89 us, 94 with CTAs of 4; but 256 items of up to 4096 33 and 28 us).  Many
+  // (32 items of 32768 tokens x 128 89 us, 93 with CTAs of 4; but 256 items of up to 4096 32 and 29 us).  Many
   // items: smaller CTAs, more of them at different points of an item (512 sequences of up to 256 tokens,
-  // 4096 items, CTAs of 2 warps 44 us, of 4 51; 512 items of up to 8192 tokens 87 and 85).
+  // 4096 items, CTAs of 2 warps 42 us, of 4 50; 512 items of up to 8192 tokens 87 and 85).
   // Heads of 192 have no room for two CTAs of 4, nor heads of 256 for 8 warps.
   const int64_t items = static_cast<int64_t>(a.batch) * a.heads_kv * a.blocks;
   if constexpr (DP <= 192) {

@@ -348,8 +348,9 @@ __global__ void __launch_bounds__(kThreads, 5) rotary_rows(const __grid_constant
 // say), a vector of channels is loaded as it lies and its partners come through shared memory (interleaved:
 // they are in the vector): a thread keeps one vector of one row over the tile's tokens, angles are laid out
 // by channel with the sine's sign in place.  Words a quarter as wide in the form above take longer (6123
-// tokens x 48 rows x 128 bf16, 30 channels rotated, 109 us and 52), words half as wide do not (19488 x 20 x
-// 96, 8 rotated, 48 and 68).
+// tokens x 48 rows x 128 bf16, 30 channels rotated, 94 us and 45), words half as wide do not (19488 x 20 x
+// 96, 8 rotated, 35 and 47).  A copy would take 23 us for either: here the threads meet at a barrier for
+// each group of tokens, there the channels that pass move in the pairs' narrow words too.
 template <typename T, int VEC, bool INTER, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 4) rotary_staged(const __grid_constant__ RotaryArgs a) {
   __shared__ Token told[PAGED ? kMaxTokens : 1];

@@ -27,10 +27,13 @@ q, o (batch, heads, dim); query head h reads key head h // (heads // heads_kv). 
 sequence b's token seq_lens[b] - 1 and sees the tokens up to it, the last ``window`` of them if
 given.  lse (batch, heads) float32 is in the log2 domain, as MultiHeadAttentionFwdOp's.  A
 sequence without a token has o = 0 and lse = -inf.  Caches 16-byte aligned, their strides
-multiples of 8.
+multiples of 8.  Softmax statistics and sums are fp32; the weights meet the values as numbers of
+``dtype``, with what those round off beside them where heads // heads_kv is at most 8.
 
 Offsets that break their rule set the device error flag to 2; a token in use without a page in
-[0, num_pages) sets it to 3 (its slot is not written, its key and value count as zeros).  A
+[0, num_pages) sets it to 3 (its slot is not written, its key and value count as zeros), as does a
+length that the table has no room for (attention takes it as the table's room).  Caches that share
+an element are refused; k, v and q may not lie in slots that the call writes.  A
 device's first call looks that flag up: make it outside a graph's capture.  The decode op keeps a
 workspace of some MB for each of torch's streams that it is called on; captured calls and those on
 other streams have their own.

@@ -19,8 +19,9 @@ the position (whole multiples of 2^-64 turns), so no table bounds the length.
 q (batch, seq_len, heads, dim) and k (batch, seq_len, heads_kv, dim) of ``dtype``, the layout of
 MultiHeadAttentionFwdOp; column slices of a wider tensor are read in place.  positions: integers
 (seq_len,) or (batch, seq_len), any sign; None is 0, 1, ....  With heads_kv 0, k is None.
-``inplace`` writes over q and k (contiguous channels, no overlap) and returns them.  Like every op
-here, these build no autograd graph: a training loop calls the two ops itself.
+``inplace`` writes over q and k (contiguous channels, no element twice, in one or in both) and
+returns them.  Like every op here, these build no autograd graph: a training loop calls the two
+ops itself.
 
 ``rotary_frequencies`` makes the angles, also those scaled for long contexts.
 """
